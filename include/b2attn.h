@@ -295,6 +295,103 @@ B2A_API int b2a_prefill_host(const void* q, const void* k, const void* v, void* 
                              int out_fp32, int n_chunks, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
+ * Serving sequences of different lengths together: attention over packed
+ * prompts, a paged KV cache (append, single-token attention) and sampling.
+ *
+ * Packed tensors hold the sequences' tokens one after another: sequence b owns
+ * rows [cu[b], cu[b + 1]) of a tensor, cu int32 [B + 1] on the device, not
+ * decreasing, from 0 or more to at most the tensor's rows. Rows outside every
+ * sequence are neither read nor written. A paged cache is a pool
+ * [n_pages, Hkv, page, D] (bf16; strides {page, head, slot}) and a block
+ * table int32 [B, table_width] (row stride table_ld) on the device: key j of
+ * sequence b is slot j % page of page table[b][j / page]. Entries past a
+ * sequence's last page are not read. Pools may be any stored order with a
+ * contiguous last dimension, [n_pages, page, Hkv, D] included.
+ */
+
+/*
+ * b2a_prefill over packed sequences: q [Nq, Hq, D], k and v [Nk, Hkv, D],
+ * o [Nq, Hq, D], optional gate as q (o = attention * sigmoid(gate)), optional
+ * lse [Hq, Nq] fp32; *_strides = {row, head}. Sequence b's queries are rows
+ * [cu_q[b], cu_q[b + 1]), its keys rows [cu_k[b], cu_k[b + 1]); with causal
+ * its last query sees all its keys: row r sees keys up to
+ * (keys - queries) + r, and a row that sees none gives 0. No replacement in
+ * the reference, whose prompts run one at a time (smollm.py:168-253).
+ * A pair of offsets that is not a stretch of the tensors leaves its sequence
+ * out and reports B2A_ERR_DEVICE_BAD_LEN. Supported D: 64, 128, 256.
+ */
+B2A_API int b2a_prefill_varlen(const void* q, const void* k, const void* v, const void* gate, void* o, float* lse,
+                               const int* cu_q, const int* cu_k, int B, int Nq, int Nk, int Hq, int Hkv, int D,
+                               const long long* q_strides, const long long* k_strides,
+                               const long long* v_strides, const long long* gate_strides,
+                               const long long* o_strides, int gate_bf16, float scale, int causal, int out_fp32,
+                               void* stream);
+
+/* Bytes of device scratch b2a_decode_paged needs for these sizes. */
+B2A_API size_t b2a_decode_paged_workspace_bytes(int B, int Hq, int Hkv, int D);
+
+/*
+ * b2a_decode over a paged cache: q and o [B, Hq, D] (strides {batch, head}),
+ * pools k_pages and v_pages [n_pages, Hkv, page, D], seqlens [B] int32: keys
+ * 0 .. seqlens[b] - 1 are attended, none gives 0. Optional gate as
+ * b2a_decode_gated. Slots past a sequence's end may hold anything. A length
+ * below 0 or above table_width * page is cut to that range, a block table
+ * entry outside the pool reads page 0; both report B2A_ERR_DEVICE_BAD_LEN.
+ * page: a multiple of 16. Supported D: 64, 128, 256; Hq / Hkv <= 16.
+ */
+B2A_API int b2a_decode_paged(const void* q, const void* k_pages, const void* v_pages, const int* block_table,
+                             long long table_ld, int table_width, const int* seqlens, const void* gate, void* o,
+                             int B, int Hq, int Hkv, int n_pages, int page, int D, const long long* q_strides,
+                             const long long* k_strides, const long long* v_strides, const long long* gate_strides,
+                             const long long* o_strides, int gate_bf16, float scale, int out_fp32, void* workspace,
+                             size_t workspace_bytes, void* stream);
+
+/*
+ * b2a_qk_norm_rope_append for packed tokens and a paged cache: q [N, Hq, D],
+ * k and v [N, Hkv, D] views (strides {token, head}), cu_seqlens [B + 1].
+ * Token n of sequence b is at position start + n - cu[b] (start =
+ * start_pos_per_batch[b], device, or start_pos). Writes the rotated q to
+ * q_out [N, Hq, D] and k, v to the sequence's pages (all bf16, q_out
+ * contiguous); k_out / v_out, optional, contiguous [N, Hkv, D] bf16, receive
+ * the same k and v packed (what b2a_prefill_varlen reads). seqlens_out [B],
+ * optional: start + tokens. cos_tab / sin_tab [max_pos, rope_dim] are fp32
+ * (tab_fp32 = 1) or of the source type; computed in fp32, rounded once.
+ * Tokens whose position or page is out of range are skipped and report
+ * B2A_ERR_DEVICE_BAD_LEN. Supported D: 64, 128, 256.
+ */
+B2A_API int b2a_rope_append_paged(const void* q, const void* k, const void* v, const long long* q_strides,
+                                  const long long* k_strides, const long long* v_strides, int src_bf16,
+                                  const void* q_norm, const void* k_norm, float eps, const void* cos_tab,
+                                  const void* sin_tab, int tab_fp32, int max_pos, int rope_dim, void* q_out,
+                                  void* k_out, void* v_out, void* k_pages, void* v_pages,
+                                  const long long* k_page_strides, const long long* v_page_strides,
+                                  const int* block_table, long long table_ld, int table_width, int n_pages,
+                                  int page, const int* cu_seqlens, int B, int N, int Hq, int Hkv, int D,
+                                  int start_pos, const int* start_pos_per_batch, int* seqlens_out, void* stream);
+
+/*
+ * The next token of each row of logits [R, V] (fp32, or bf16 with
+ * logits_bf16 = 1; row stride ld_logits) from given random numbers: noise
+ * [R, V] fp32, independent draws of Exp(1), all above 0 (row stride ld_noise).
+ *
+ * With m the row's maximum, T its temperature: w_i = exp((x_i - m) / T).
+ * Tokens are ranked by logit (descending, lowest index first among equals).
+ * Token j is kept iff fewer than top_k tokens rank ahead of it (top_k <= 0:
+ * no limit), the weight ahead of it is below top_p of the row's total weight
+ * (top_p >= 1: no limit) and w_j >= min_p; the first is always kept. The
+ * result is argmax w_i / noise_i over the kept tokens, lowest index on ties:
+ * token i with probability w_i / (sum of the kept w). T <= 0 gives argmax x.
+ * NaN logits count as -inf; a row without a logit above -inf gives -1.
+ * temperature, top_k, top_p, min_p: per-row device arrays [R], or NULL for
+ * the *_all value in every row. noise may be NULL: every row is then greedy.
+ * Replaces: nothing in the reference, which takes the argmax on the host.
+ */
+B2A_API int b2a_sample(const void* logits, long long ld_logits, int logits_bf16, const float* noise,
+                       long long ld_noise, int R, int V, const float* temperature, float temperature_all,
+                       const int* top_k, int top_k_all, const float* top_p, float top_p_all, const float* min_p,
+                       float min_p_all, long long* out, void* stream);
+
+/*
  * Read (and optionally clear) the device error word the kernels set on the
  * current device. Synchronises `stream`. *status receives B2A_OK,
  * B2A_ERR_DEVICE_TIMEOUT or B2A_ERR_DEVICE_BAD_LEN.

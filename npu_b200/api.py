@@ -2,7 +2,9 @@
 and the fused RoPE + KV-cache append that feeds them.
 
 These are the B200 entry points behind the reference-compatible wrapper in
-npu_b200.fa (NpuAttention.run_batch). Tensors are CUDA bf16 with a contiguous
+npu_b200.fa (NpuAttention.run_batch), and the operators that serve sequences
+of different lengths together: attention over packed prompts, a paged KV cache
+(append, single-token attention) and token sampling. Tensors are CUDA bf16 with a contiguous
 head dimension, except for prefill_host, which takes host bf16 tensors and
 moves them itself; nothing here falls back to a CPU path.
 """
@@ -14,6 +16,11 @@ from typing import Optional
 import torch
 
 from . import _lib
+
+
+# The current stream's handle of a device index.
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else \
+    lambda index: torch.cuda.current_stream(index).cuda_stream
 
 
 def _stream_ptr(device: torch.device) -> int:
@@ -426,6 +433,340 @@ def rope_append(
         )
     _lib.check(rc, "b2a_qk_norm_rope_append")
     return q_out
+
+
+class _SameDevice:
+    __slots__ = ()
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        return False
+
+
+_SAME_DEVICE = _SameDevice()
+
+
+def _on(device: torch.device):
+    """torch.cuda.device(device), without its cost when that device is current."""
+    return _SAME_DEVICE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def _need_int32(name: str, t: torch.Tensor, numel: int, device: torch.device) -> None:
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.device != device or t.numel() != numel \
+            or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 tensor of {numel} on the inputs' device")
+
+
+def _need_pool(name: str, t: torch.Tensor, device: torch.device) -> None:
+    _need_cuda_bf16(name, t, 4)
+    if t.device != device:
+        raise ValueError(f"{name} must be on the inputs' device")
+
+
+def _need_table(t: torch.Tensor, batch: int, device: torch.device) -> None:
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.device != device or t.dim() != 2 \
+            or t.shape[0] != batch or t.stride(1) != 1:
+        raise ValueError(f"block_table must be an int32 tensor [{batch}, pages] on the inputs' device with a "
+                         "contiguous last dim")
+
+
+def prefill_varlen(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    cu_seqlens_q: torch.Tensor,
+    cu_seqlens_k: Optional[torch.Tensor] = None,
+    *,
+    scale: Optional[float] = None,
+    causal: bool = True,
+    out_dtype: torch.dtype = torch.float32,
+    out: Optional[torch.Tensor] = None,
+    return_lse: bool = False,
+    gate: Optional[torch.Tensor] = None,
+):
+    """`prefill` over sequences of different lengths packed along one axis:
+    q [Nq, Hq, D] against k/v [Nk, Hkv, D].
+
+    Sequence b owns query rows cu_seqlens_q[b] .. cu_seqlens_q[b + 1] - 1 and
+    the keys that cu_seqlens_k (default: cu_seqlens_q) gives the same way;
+    both are int32 CUDA tensors [B + 1], and the lengths are never read by the
+    host. With causal, a sequence's last query sees all its keys (row r sees
+    keys up to keys - queries + r); rows that see no key give 0. Rows outside
+    every sequence are not written. Returns o [Nq, Hq, D] in out_dtype (and the
+    natural-log LSE [Hq, Nq] if return_lse); `gate` ([Nq, Hq, D], fp32 or bf16)
+    multiplies the output by sigmoid(gate) as in `prefill`.
+    """
+    _need_cuda_bf16("q", q, 3)
+    _need_cuda_bf16("k", k, 3)
+    _need_cuda_bf16("v", v, 3)
+    Nq, Hq, D = q.shape
+    Nk, Hkv, Dk = k.shape
+    device = q.device
+    if Dk != D or v.shape != k.shape or k.device != device or v.device != device:
+        raise ValueError(f"shape or device mismatch q{tuple(q.shape)} k{tuple(k.shape)} v{tuple(v.shape)}")
+    B = cu_seqlens_q.numel() - 1
+    if B < 1:
+        raise ValueError("cu_seqlens_q must hold at least two offsets")
+    _need_int32("cu_seqlens_q", cu_seqlens_q, B + 1, device)
+    if cu_seqlens_k is None:
+        if Nk != Nq:
+            raise ValueError(f"k has {Nk} rows and q {Nq}: cu_seqlens_k is needed")
+        cu_seqlens_k = cu_seqlens_q
+    else:
+        _need_int32("cu_seqlens_k", cu_seqlens_k, B + 1, device)
+    if out_dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError("out_dtype must be float32 or bfloat16")
+    if out is None:
+        out = torch.empty((Nq, Hq, D), dtype=out_dtype, device=device)
+    elif out.dtype != out_dtype or out.shape != q.shape or out.stride(-1) != 1 or out.device != device:
+        raise ValueError("out must match [Nq, Hq, D], out_dtype and q's device, with a contiguous last dim")
+    lse = torch.empty((Hq, Nq), dtype=torch.float32, device=device) if return_lse else None
+    if gate is not None:
+        _check_gate(gate, (Nq, Hq, D), device)
+    ll2 = _lib.ll2
+    with _on(device):
+        rc = _lib.load().b2a_prefill_varlen(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), gate.data_ptr() if gate is not None else None, out.data_ptr(),
+            lse.data_ptr() if return_lse else None, cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(),
+            B, Nq, Nk, Hq, Hkv, D, ll2(*q.stride()[:2]), ll2(*k.stride()[:2]), ll2(*v.stride()[:2]),
+            ll2(*gate.stride()[:2]) if gate is not None else None, ll2(*out.stride()[:2]),
+            1 if gate is not None and gate.dtype == torch.bfloat16 else 0,
+            1.0 / math.sqrt(D) if scale is None else float(scale), 1 if causal else 0,
+            1 if out_dtype == torch.float32 else 0, _raw_stream(device.index),
+        )
+    _lib.check(rc, "b2a_prefill_varlen")
+    return (out, lse) if return_lse else out
+
+
+def decode_paged_workspace_bytes(B: int, Hq: int, Hkv: int, D: int) -> int:
+    return int(_lib.load().b2a_decode_paged_workspace_bytes(B, Hq, Hkv, D))
+
+
+def decode_paged(
+    q: torch.Tensor,
+    k_pages: torch.Tensor,
+    v_pages: torch.Tensor,
+    block_table: torch.Tensor,
+    seqlens: torch.Tensor,
+    *,
+    scale: Optional[float] = None,
+    out_dtype: torch.dtype = torch.float32,
+    workspace: Optional[torch.Tensor] = None,
+    out: Optional[torch.Tensor] = None,
+    gate: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """`decode` over a paged cache: q [B, Hq, D] against page pools
+    [n_pages, Hkv, page, D] (bf16, page a multiple of 16; any stored order with
+    a contiguous last dim).
+
+    Key j of sequence b is slot j % page of page block_table[b, j // page]
+    (int32 CUDA tensor [B, pages]; entries past the last page of a sequence
+    are not read), and keys 0 .. seqlens[b] - 1 are attended; a sequence without
+    keys gives 0. Slots past a sequence's end may hold anything. The lengths
+    stay on the device; scratch comes from `workspace` (a uint8 CUDA tensor of
+    decode_paged_workspace_bytes) or torch's allocator. `gate` ([B, Hq, D])
+    as in `decode`.
+    """
+    _need_cuda_bf16("q", q, 3)
+    B, Hq, D = q.shape
+    device = q.device
+    _need_pool("k_pages", k_pages, device)
+    _need_pool("v_pages", v_pages, device)
+    n_pages, Hkv, page, Dk = k_pages.shape
+    if Dk != D or v_pages.shape != k_pages.shape:
+        raise ValueError(f"shape mismatch q{tuple(q.shape)} k_pages{tuple(k_pages.shape)} "
+                         f"v_pages{tuple(v_pages.shape)}")
+    _need_table(block_table, B, device)
+    _need_int32("seqlens", seqlens, B, device)
+    if out is None:
+        if out_dtype not in (torch.float32, torch.bfloat16):
+            raise ValueError("out_dtype must be float32 or bfloat16")
+        out = torch.empty((B, Hq, D), dtype=out_dtype, device=device)
+    elif out.dtype != out_dtype or out.shape != q.shape or out.stride(-1) != 1 or out.device != device:
+        raise ValueError("out must match [B, Hq, D], out_dtype and q's device, with a contiguous last dim")
+    if gate is not None:
+        _check_gate(gate, (B, Hq, D), device)
+    lib = _lib.load()
+    need = int(lib.b2a_decode_paged_workspace_bytes(B, Hq, Hkv, D))
+    if workspace is None:
+        workspace = torch.empty(max(need, 16), dtype=torch.uint8, device=device)
+    elif workspace.device != device or workspace.numel() * workspace.element_size() < need:
+        raise ValueError(f"workspace must be a CUDA tensor of at least {need} bytes on q's device")
+    ll2, ll3 = _lib.ll2, _lib.ll3
+    with _on(device):
+        rc = lib.b2a_decode_paged(
+            q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(), block_table.stride(0),
+            block_table.shape[1], seqlens.data_ptr(), gate.data_ptr() if gate is not None else None, out.data_ptr(),
+            B, Hq, Hkv, n_pages, page, D, ll2(*q.stride()[:2]), ll3(*k_pages.stride()[:3]),
+            ll3(*v_pages.stride()[:3]), ll2(*gate.stride()[:2]) if gate is not None else None,
+            ll2(*out.stride()[:2]), 1 if gate is not None and gate.dtype == torch.bfloat16 else 0,
+            1.0 / math.sqrt(D) if scale is None else float(scale), 1 if out_dtype == torch.float32 else 0,
+            workspace.data_ptr(), need, _raw_stream(device.index),
+        )
+    _lib.check(rc, "b2a_decode_paged")
+    return out
+
+
+def rope_append_paged(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    cos: torch.Tensor,
+    sin: torch.Tensor,
+    k_pages: torch.Tensor,
+    v_pages: torch.Tensor,
+    block_table: torch.Tensor,
+    cu_seqlens: torch.Tensor,
+    *,
+    start_pos: int = 0,
+    start_pos_per_batch: Optional[torch.Tensor] = None,
+    seqlens_out: Optional[torch.Tensor] = None,
+    q_out: Optional[torch.Tensor] = None,
+    q_norm: Optional[torch.Tensor] = None,
+    k_norm: Optional[torch.Tensor] = None,
+    norm_eps: float = 1e-6,
+    rope_dim: Optional[int] = None,
+    return_kv: bool = False,
+):
+    """`rope_append` for packed tokens and a paged cache: q [N, Hq, D], k and v
+    [N, Hkv, D] (fp32 or bf16, last dim contiguous; typically views of one fused
+    QKV projection), pools and block_table as `decode_paged`.
+
+    Token n of sequence b (cu_seqlens[b] <= n < cu_seqlens[b + 1]) is at
+    position p_b + n - cu_seqlens[b], p_b = start_pos_per_batch[b] or
+    start_pos; its k and v go to the page and slot of that position, which
+    block_table must already name. seqlens_out (int32 [B], optional) receives
+    p_b + tokens. cos/sin [max_pos, rope_dim] are fp32 or q's dtype; the
+    arithmetic is fp32 and rounds to bf16 once. q_norm, k_norm, norm_eps and
+    rope_dim as in `rope_append`. Returns q rotated, [N, Hq, D] bf16; with
+    return_kv (q, k, v): k rotated and v as packed bf16 [N, Hkv, D] for
+    `prefill_varlen` (v itself when it is bf16 already).
+    """
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dim() != 3 or t.stride(-1) != 1:
+            raise ValueError(f"{name} must be a CUDA [N, H, D] tensor with a contiguous last dim")
+    N, Hq, D = q.shape
+    Hkv = k.shape[1]
+    device, dtype = q.device, q.dtype
+    if k.shape != (N, Hkv, D) or v.shape != k.shape:
+        raise ValueError(f"shape mismatch q{tuple(q.shape)} k{tuple(k.shape)} v{tuple(v.shape)}")
+    if dtype not in (torch.float32, torch.bfloat16) or k.dtype != dtype or v.dtype != dtype:
+        raise ValueError("q, k, v must share one dtype, float32 or bfloat16")
+    if k.device != device or v.device != device or cos.device != device or sin.device != device:
+        raise ValueError("q, k, v, cos and sin must be on one device")
+    rope_dim = D if rope_dim is None else int(rope_dim)
+    if cos.dtype not in (torch.float32, dtype) or sin.dtype != cos.dtype or not cos.is_contiguous() \
+            or not sin.is_contiguous() or cos.dim() != 2 or cos.shape[1] != rope_dim or sin.shape != cos.shape:
+        raise ValueError("cos/sin must be contiguous [max_pos, rope_dim] tensors, float32 or in q's dtype")
+    _need_pool("k_pages", k_pages, device)
+    _need_pool("v_pages", v_pages, device)
+    n_pages, Hc, page, Dc = k_pages.shape
+    if (Hc, Dc) != (Hkv, D) or v_pages.shape != k_pages.shape:
+        raise ValueError(f"cache shape {tuple(k_pages.shape)} does not fit k{tuple(k.shape)}")
+    B = cu_seqlens.numel() - 1
+    if B < 1:
+        raise ValueError("cu_seqlens must hold at least two offsets")
+    _need_int32("cu_seqlens", cu_seqlens, B + 1, device)
+    _need_table(block_table, B, device)
+    if start_pos_per_batch is not None:
+        _need_int32("start_pos_per_batch", start_pos_per_batch, B, device)
+    if seqlens_out is not None:
+        _need_int32("seqlens_out", seqlens_out, B, device)
+    for name, w in (("q_norm", q_norm), ("k_norm", k_norm)):
+        if w is not None and (w.dtype != dtype or w.device != device or w.shape != (D,) or not w.is_contiguous()):
+            raise ValueError(f"{name} must be a contiguous [D] tensor in q's dtype on q's device")
+    if q_out is None:
+        q_out = torch.empty((N, Hq, D), dtype=torch.bfloat16, device=device)
+    elif q_out.dtype != torch.bfloat16 or q_out.shape != q.shape or not q_out.is_contiguous() \
+            or q_out.device != device:
+        raise ValueError("q_out must be a contiguous bf16 [N, Hq, D] tensor on q's device")
+    bf16 = dtype == torch.bfloat16
+    k_out = torch.empty((N, Hkv, D), dtype=torch.bfloat16, device=device) if return_kv else None
+    v_out = torch.empty((N, Hkv, D), dtype=torch.bfloat16, device=device) if return_kv and not bf16 else None
+    ll2, ll3 = _lib.ll2, _lib.ll3
+    with _on(device):
+        rc = _lib.load().b2a_rope_append_paged(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), ll2(*q.stride()[:2]), ll2(*k.stride()[:2]),
+            ll2(*v.stride()[:2]), 1 if bf16 else 0, q_norm.data_ptr() if q_norm is not None else None,
+            k_norm.data_ptr() if k_norm is not None else None, float(norm_eps), cos.data_ptr(), sin.data_ptr(),
+            1 if cos.dtype == torch.float32 else 0, cos.shape[0], rope_dim, q_out.data_ptr(),
+            k_out.data_ptr() if k_out is not None else None, v_out.data_ptr() if v_out is not None else None,
+            k_pages.data_ptr(), v_pages.data_ptr(), ll3(*k_pages.stride()[:3]), ll3(*v_pages.stride()[:3]),
+            block_table.data_ptr(), block_table.stride(0), block_table.shape[1], n_pages, page,
+            cu_seqlens.data_ptr(), B, N, Hq, Hkv, D, int(start_pos),
+            start_pos_per_batch.data_ptr() if start_pos_per_batch is not None else None,
+            seqlens_out.data_ptr() if seqlens_out is not None else None, _raw_stream(device.index),
+        )
+    _lib.check(rc, "b2a_rope_append_paged")
+    if return_kv:
+        return q_out, k_out, (v if bf16 else v_out)
+    return q_out
+
+
+def _per_row(name: str, value, rows: int, dtype: torch.dtype, device: torch.device):
+    """(device pointer or None, value for every row) of a sampling setting."""
+    if isinstance(value, torch.Tensor):
+        if value.dtype != dtype or value.device != device or value.shape != (rows,) or not value.is_contiguous():
+            raise ValueError(f"{name} must be a number or a contiguous {dtype} tensor [{rows}] on the logits' device")
+        return value.data_ptr(), 0
+    return None, value
+
+
+def sample(
+    logits: torch.Tensor,
+    noise: Optional[torch.Tensor] = None,
+    *,
+    temperature=1.0,
+    top_k=0,
+    top_p=1.0,
+    min_p=0.0,
+    out: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """The next token of each row of logits [R, V] (fp32 or bf16), int64 [R].
+
+    noise [R, V] fp32 holds independent Exp(1) draws, all above 0
+    (`torch.empty(R, V).exponential_()`); the same noise gives the same tokens.
+    A row's temperature T, top_k, top_p and min_p are numbers or per-row CUDA
+    tensors (fp32; top_k int32). With w = exp((x - max) / T), tokens ranked by
+    logit (lowest index first among equals): token j is kept iff fewer than
+    top_k tokens rank ahead of it (0: no limit), the weight ahead of it is
+    below top_p of the total (1: no limit) and w_j >= min_p; the first always.
+    Each filter is taken of the whole distribution. The result is
+    argmax w / noise over the kept tokens, so token i comes up with probability
+    w_i / (sum of the kept w). T <= 0 (or no noise) gives the argmax. NaN logits
+    count as -inf; a row without a logit above -inf gives -1.
+    """
+    if not isinstance(logits, torch.Tensor) or not logits.is_cuda or logits.dim() != 2 or logits.stride(1) != 1 \
+            or logits.dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError("logits must be a CUDA float32 or bfloat16 tensor [R, V] with a contiguous last dim")
+    R, V = logits.shape
+    device = logits.device
+    if noise is not None:
+        if not isinstance(noise, torch.Tensor) or noise.dtype != torch.float32 or noise.device != device \
+                or noise.shape != logits.shape or noise.stride(1) != 1:
+            raise ValueError(f"noise must be a float32 tensor [{R}, {V}] on the logits' device with a contiguous "
+                             "last dim")
+    elif isinstance(temperature, torch.Tensor) or temperature > 0:
+        raise ValueError("a temperature above 0 needs noise")
+    t_ptr, t_all = _per_row("temperature", temperature, R, torch.float32, device)
+    k_ptr, k_all = _per_row("top_k", top_k, R, torch.int32, device)
+    p_ptr, p_all = _per_row("top_p", top_p, R, torch.float32, device)
+    m_ptr, m_all = _per_row("min_p", min_p, R, torch.float32, device)
+    if out is None:
+        out = torch.empty(R, dtype=torch.int64, device=device)
+    elif out.dtype != torch.int64 or out.shape != (R,) or not out.is_contiguous() or out.device != device:
+        raise ValueError(f"out must be a contiguous int64 tensor [{R}] on the logits' device")
+    with _on(device):
+        rc = _lib.load().b2a_sample(
+            logits.data_ptr(), logits.stride(0) if R > 1 else V, 1 if logits.dtype == torch.bfloat16 else 0,
+            noise.data_ptr() if noise is not None else None, noise.stride(0) if noise is not None and R > 1 else V,
+            R, V, t_ptr, float(t_all), k_ptr, int(k_all), p_ptr, float(p_all), m_ptr, float(m_all),
+            out.data_ptr(), _raw_stream(device.index),
+        )
+    _lib.check(rc, "b2a_sample")
+    return out
 
 
 def device_error(clear: bool = True, device: Optional[torch.device] = None) -> int:

@@ -8,6 +8,7 @@
 #include <mutex>
 
 #include "b2attn.h"
+#include "capi_internal.cuh"
 #include "decode.cuh"
 #include "prefill.cuh"
 #include "rope_append.cuh"
@@ -372,6 +373,25 @@ namespace b2a {
 int* device_error_word() {
   const int dev = current_device();
   return dev < 0 ? nullptr : device_err_ptr(dev);
+}
+
+int api_prologue(int** err) { return prologue(err); }
+
+int api_tensor_map(CUtensorMap* m, const void* base, int rank, const unsigned long long* dims,
+                   const unsigned long long* byte_strides, const unsigned* box) {
+  auto fn = encode_fn();
+  if (!fn || rank < 1 || rank > 5) return B2A_ERR_TMA;
+  cuuint64_t d[5] = {}, s[5] = {};
+  cuuint32_t b[5] = {}, es[5] = {1u, 1u, 1u, 1u, 1u};
+  for (int i = 0; i < rank; ++i) {
+    d[i] = dims[i] ? dims[i] : 1;
+    b[i] = box[i];
+    if (i + 1 < rank) s[i] = byte_strides[i];
+  }
+  const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (cuuint32_t)rank, const_cast<void*>(base), d, s, b, es,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? B2A_OK : B2A_ERR_TMA;
 }
 }  // namespace b2a
 

@@ -1,0 +1,35 @@
+// What the extern "C" files share: the per-call device checks and the TMA
+// tensor-map encoder (defined in capi.cu), and small argument checks.
+#pragma once
+
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+namespace b2a {
+
+// Current device is sm_100 and its error word is known: B2A_OK and *err, or
+// the status to return.
+int api_prologue(int** err);
+
+// Tiled bf16 tensor map with 128-byte swizzle, out-of-range elements read as
+// zero. dims / box have `rank` entries (innermost first), byte_strides
+// rank - 1 (dimension i + 1). Returns B2A_OK or B2A_ERR_TMA.
+int api_tensor_map(CUtensorMap* m, const void* base, int rank, const unsigned long long* dims,
+                   const unsigned long long* byte_strides, const unsigned* box);
+
+inline bool api_aligned(const void* p, unsigned bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+
+// Strides are not negative and multiples of `mult` elements.
+inline bool api_strides_ok(const long long* s, int n, long long mult) {
+  for (int i = 0; i < n; ++i)
+    if (s[i] < 0 || (s[i] % mult) != 0) return false;
+  return true;
+}
+
+inline size_t api_align256(size_t x) { return (x + 255) & ~(size_t)255; }
+
+constexpr float kApiLog2e = 1.4426950408889634f;
+
+}  // namespace b2a

@@ -1,0 +1,348 @@
+// Attention of one new token per sequence over a paged bf16 KV cache
+// [n_pages, Hkv, page, D], sm_100a.
+//
+//   o_h = sum_j p_j v_j / sum_j p_j,  p_j = 2^(scale log2(e) q_h k_j - m),
+// over keys j < seqlens[b], key j in slot j % page of page table[b][j / page];
+// a sequence without keys gives 0. Query head h uses KV head h / (Hq / Hkv).
+//
+// Bound by HBM: every key and value of a sequence is read once for the whole
+// group of query heads that shares it (8 to 16 flop per byte). One warp
+// streams 64-key K / V tiles through a shared-memory ring with TMA, one copy
+// per run of keys that lies in one page (box_rows, 16 to 64 keys); four warps
+// take 16 keys of a tile each. The query heads of a group are the 16 rows of
+// mma.sync m16n8k16. P goes into the second product as two bf16 terms (its
+// rounding and what the rounding left), so its relative error is 2^-16
+// instead of 2^-8; the extra MMAs hide behind the loads.
+//
+// Slots of a page past the sequence's end may hold anything, NaN included:
+// their scores are replaced by -inf and their V rows by zeros in shared
+// memory before they are used.
+#include "decode_paged.cuh"
+
+namespace b2a {
+
+namespace {
+
+template <int D>
+struct PagedCfg {
+  static constexpr int TK = 64;  // keys per tile
+  static constexpr int TILE_BYTES = TK * D * 2;  // K or V tile
+  static constexpr int STAGE_BYTES = 2 * TILE_BYTES;
+  static constexpr int STAGES = D == 64 ? 6 : 3;
+  static constexpr int CTAS_PER_SM = D == 256 ? 1 : 2;
+  static constexpr int OFF_BAR = STAGES * STAGE_BYTES;
+  static constexpr int SMEM_BYTES = OFF_BAR + 1024 + 1024;  // barriers and m, l; alignment slack
+  static constexpr int THREADS = 160;  // 4 compute warps + 1 producer warp
+  static_assert(4 * 16 * D * 4 <= STAGE_BYTES, "the four warps' outputs are merged in one stage");
+  static_assert((SMEM_BYTES + 1024) * CTAS_PER_SM <= 233472, "shared memory budget");
+};
+
+struct PagedBars {
+  uint64_t full[8];
+  uint64_t empty[8];
+  int abort_flag;
+  float m[4][16];
+  float l[4][16];
+};
+
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
+               : "r"(addr)
+               : "memory");
+}
+
+__device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
+               : "r"(addr)
+               : "memory");
+}
+
+__device__ __forceinline__ void tma_load_5d(void* smem_dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1,
+                                            int c2, int c3, int c4) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(smem_u32(smem_dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4)
+      : "memory");
+}
+
+// The output of (sequence b, query head h), column d: attention value v,
+// gated and rounded as the call asks.
+__device__ __forceinline__ void store_output(const DecodePagedParams& p, int b, int h, int d, float v) {
+  if (p.gate) {
+    const long long gi = b * p.g_sb + h * p.g_sh + d;
+    const float g = p.gate_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p.gate)[gi])
+                                : static_cast<const float*>(p.gate)[gi];
+    v *= __fdividef(1.f, 1.f + __expf(-g));
+  }
+  const long long oi = b * p.o_sb + h * p.o_sh + d;
+  if (p.out_fp32)
+    static_cast<float*>(p.o)[oi] = v;
+  else
+    static_cast<__nv_bfloat16*>(p.o)[oi] = __float2bfloat16_rn(v);
+}
+
+template <int D>
+__global__ void __launch_bounds__(PagedCfg<D>::THREADS, PagedCfg<D>::CTAS_PER_SM)
+    decode_paged_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                        const __grid_constant__ DecodePagedParams p) {
+  using C = PagedCfg<D>;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  const uint32_t pad = (1024u - (smem_u32(smem_raw) & 1023u)) & 1023u;
+  uint8_t* smem = smem_raw + pad;
+  PagedBars* bars = reinterpret_cast<PagedBars*>(smem + C::OFF_BAR);
+  volatile int* abort_flag = &bars->abort_flag;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  const int b = blockIdx.x / p.Hkv, g = blockIdx.x % p.Hkv;
+  const long long cap = (long long)p.table_width * p.page;
+  int len = p.seqlens[b];
+  if (len < 0 || len > cap) {
+    if (threadIdx.x == 0 && g == 0 && p.err) atomicOr(p.err, kErrBadArgs);
+    len = len < 0 ? 0 : (int)cap;
+  }
+  const int n_tiles = (len + C::TK - 1) / C::TK;
+  if (n_tiles == 0) {
+    for (int e = threadIdx.x; e < p.group * D; e += C::THREADS)
+      store_output(p, b, g * p.group + e / D, e % D, 0.f);
+    return;
+  }
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::STAGES; ++s) {
+      mbar_init(&bars->full[s], 1);
+      mbar_init(&bars->empty[s], 4);
+    }
+    bars->abort_flag = 0;
+    fence_mbar_init();
+  }
+  __syncthreads();
+
+  const int br = p.box_rows;
+  if (warp == 4) {
+    // ------------------------------------------------------------ producer
+    // Lane x < 2 * boxes copies one box: K boxes first, then V boxes.
+    const int boxes = C::TK / br;
+    const int box = lane % boxes;
+    const bool is_v = lane >= boxes;
+    const bool mine = lane < 2 * boxes;
+    const int box_bytes = br * D * 2;
+    auto page_of = [&](int i) -> int {  // page of this lane's box in tile i
+      const int key = i * C::TK + box * br;
+      if (!mine || key >= len) return -1;
+      const int id = p.block_table[b * p.table_ld + key / p.page];
+      if (id >= 0 && id < p.n_pages) return id;
+      if (p.err) atomicOr(p.err, kErrBadArgs);
+      return 0;
+    };
+    int next = page_of(0);
+    int issued = 0;
+    for (int i = 0; i < n_tiles; ++i) {
+      const int slot = i % C::STAGES;
+      const int id = next;
+      if (i + 1 < n_tiles) next = page_of(i + 1);
+      if (!__all_sync(0xffffffffu, mbar_wait(&bars->empty[slot], ((uint32_t)(i / C::STAGES) & 1u) ^ 1u, abort_flag,
+                                             p.err)))
+        break;
+      uint8_t* dst = smem + slot * C::STAGE_BYTES + (is_v ? C::TILE_BYTES : 0) + box * box_bytes;
+      const unsigned copies = __ballot_sync(0xffffffffu, id >= 0);
+      if (lane == 0) mbar_arrive_expect_tx(&bars->full[slot], __popc(copies) * box_bytes);
+      __syncwarp();
+      if (id >= 0)
+        tma_load_5d(dst, is_v ? &tm_v : &tm_k, &bars->full[slot], 0, (i * C::TK + box * br) % p.page, 0, g, id);
+      issued = i + 1;
+    }
+    if (*abort_flag && lane == 0)
+      for (int i = max(0, issued - C::STAGES); i < issued; ++i)
+        mbar_wait_quiet(&bars->full[i % C::STAGES], (uint32_t)(i / C::STAGES) & 1u);
+  } else {
+    // ------------------------------------------------------------ compute warps
+    const int gr = lane >> 2, tq = lane & 3;
+    uint32_t qa[D / 16][4];
+    {
+      const bool v0 = gr < p.group, v1 = gr + 8 < p.group;
+      const __nv_bfloat16* q0 = p.q + b * p.q_sb + (long long)(g * p.group + gr) * p.q_sh;
+      const __nv_bfloat16* q1 = q0 + 8 * p.q_sh;
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) {
+        qa[k][0] = v0 ? *reinterpret_cast<const uint32_t*>(q0 + 16 * k + 2 * tq) : 0u;
+        qa[k][1] = v1 ? *reinterpret_cast<const uint32_t*>(q1 + 16 * k + 2 * tq) : 0u;
+        qa[k][2] = v0 ? *reinterpret_cast<const uint32_t*>(q0 + 16 * k + 2 * tq + 8) : 0u;
+        qa[k][3] = v1 ? *reinterpret_cast<const uint32_t*>(q1 + 16 * k + 2 * tq + 8) : 0u;
+      }
+    }
+    float acc[D / 8][4];
+#pragma unroll
+    for (int n = 0; n < D / 8; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
+    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+    const float sl2 = p.scale_log2;
+    const int mi = lane >> 3, mr = lane & 7;  // ldmatrix: matrix index / row in it
+    // This warp's 16 keys of a tile lie in one box: its first row there, and
+    // the distance of the box's 64-column chunks.
+    const uint32_t wbase = (16 * warp / br) * (br * D * 2) + (16 * warp % br) * 128;
+    const uint32_t chunk = br * 128;
+    // 16-byte unit U of row r (0..15): the swizzle XORs the unit with the
+    // row's place in its group of 8.
+    auto at = [&](uint32_t base, int r, int U) -> uint32_t {
+      return base + (U >> 3) * chunk + r * 128 + (((U & 7) ^ (r & 7)) << 4);
+    };
+    bool ok = true;
+    for (int i = 0; i < n_tiles; ++i) {
+      const int slot = i % C::STAGES;
+      if (!__all_sync(0xffffffffu,
+                      mbar_wait(&bars->full[slot], (uint32_t)(i / C::STAGES) & 1u, abort_flag, p.err))) {
+        ok = false;
+        break;
+      }
+      const uint32_t kbase = smem_u32(smem + slot * C::STAGE_BYTES) + wbase;
+      const uint32_t vbase = kbase + C::TILE_BYTES;
+      const int have = len - (i * C::TK + 16 * warp);  // keys of this warp's 16 that exist
+      if (have > 0) {
+        float s[2][4];
+#pragma unroll
+        for (int ng = 0; ng < 2; ++ng) {
+          s[ng][0] = s[ng][1] = s[ng][2] = s[ng][3] = 0.f;
+#pragma unroll
+          for (int kp = 0; kp < D / 32; ++kp) {
+            uint32_t b0, b1, b2, b3;
+            ldsm4(at(kbase, 8 * ng + mr, 4 * kp + mi), b0, b1, b2, b3);
+            mma16816(s[ng], qa[2 * kp], b0, b1);
+            mma16816(s[ng], qa[2 * kp + 1], b2, b3);
+          }
+        }
+        if (have < 16) {
+#pragma unroll
+          for (int ng = 0; ng < 2; ++ng)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              if (8 * ng + 2 * tq + e >= have) s[ng][e] = s[ng][2 + e] = -INFINITY;
+          // V rows without a key: 0 x anything would not do (NaN).
+          for (int u = lane; u < (16 - have) * (D / 8); u += 32)
+            st_shared_v4(at(vbase, have + u / (D / 8), u % (D / 8)), 0u, 0u, 0u, 0u);
+          __syncwarp();
+        }
+        float mx0 = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]));
+        float mx1 = fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3]));
+        mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 1));
+        mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 2));
+        mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 1));
+        mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 2));
+        const float mn0 = fmaxf(m0, mx0 * sl2), mn1 = fmaxf(m1, mx1 * sl2);
+        const float u0 = (mn0 == -INFINITY) ? 0.f : mn0, u1 = (mn1 == -INFINITY) ? 0.f : mn1;
+        const float a0 = ex2(m0 - u0), a1 = ex2(m1 - u1);
+        m0 = mn0;
+        m1 = mn1;
+        float pr[2][4];
+#pragma unroll
+        for (int ng = 0; ng < 2; ++ng) {
+          pr[ng][0] = ex2(fmaf(s[ng][0], sl2, -u0));
+          pr[ng][1] = ex2(fmaf(s[ng][1], sl2, -u0));
+          pr[ng][2] = ex2(fmaf(s[ng][2], sl2, -u1));
+          pr[ng][3] = ex2(fmaf(s[ng][3], sl2, -u1));
+        }
+        l0 = l0 * a0 + pr[0][0] + pr[0][1] + pr[1][0] + pr[1][1];
+        l1 = l1 * a1 + pr[0][2] + pr[0][3] + pr[1][2] + pr[1][3];
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n) {
+          acc[n][0] *= a0;
+          acc[n][1] *= a0;
+          acc[n][2] *= a1;
+          acc[n][3] *= a1;
+        }
+        // P = high + low, each bf16.
+        uint32_t ph[4], pl[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float x = pr[e >> 1][2 * (e & 1)], y = pr[e >> 1][2 * (e & 1) + 1];
+          ph[e] = pack_bf16x2(x, y);
+          pl[e] = pack_bf16x2(x - __uint_as_float(ph[e] << 16), y - __uint_as_float(ph[e] & 0xffff0000u));
+        }
+        const int vr = 8 * (mi & 1) + mr;
+#pragma unroll
+        for (int dn = 0; dn < D / 8; dn += 2) {
+          uint32_t b0, b1, b2, b3;
+          ldsm4_t(at(vbase, vr, dn + (mi >> 1)), b0, b1, b2, b3);
+          mma16816(acc[dn], ph, b0, b1);
+          mma16816(acc[dn + 1], ph, b2, b3);
+          mma16816(acc[dn], pl, b0, b1);
+          mma16816(acc[dn + 1], pl, b2, b3);
+        }
+      }
+      __syncwarp();
+      if (lane == 0 && i + 1 < n_tiles) mbar_arrive(&bars->empty[slot]);
+    }
+    // Merge the four warps' (m, l, O) in the last tile's stage, once all of
+    // them have read it.
+    if (ok) {
+      l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
+      l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
+      l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
+      l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
+    }
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+    float* so = reinterpret_cast<float*>(smem + ((n_tiles - 1) % C::STAGES) * C::STAGE_BYTES);  // [4][16][D]
+#pragma unroll
+    for (int n = 0; n < D / 8; ++n) {
+      float* r0 = so + (warp * 16 + gr) * D + 8 * n + 2 * tq;
+      *reinterpret_cast<float2*>(r0) = make_float2(acc[n][0], acc[n][1]);
+      *reinterpret_cast<float2*>(r0 + 8 * D) = make_float2(acc[n][2], acc[n][3]);
+    }
+    if (tq == 0) {
+      bars->m[warp][gr] = m0;
+      bars->m[warp][gr + 8] = m1;
+      bars->l[warp][gr] = l0;
+      bars->l[warp][gr + 8] = l1;
+    }
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+    for (int e = threadIdx.x; e < p.group * D; e += 128) {
+      const int r = e / D, d = e % D;
+      float M = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) M = fmaxf(M, bars->m[w][r]);
+      const float Mu = (M == -INFINITY) ? 0.f : M;
+      float lsum = 0.f, osum = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float f = ex2(bars->m[w][r] - Mu);
+        lsum += f * bars->l[w][r];
+        osum += f * so[(w * 16 + r) * D + d];
+      }
+      store_output(p, b, g * p.group + r, d, lsum == 0.f ? 0.f : osum / lsum);
+    }
+  }
+}
+
+template <int D>
+int launch_t(const CUtensorMap& tk, const CUtensorMap& tv, const DecodePagedParams& p, cudaStream_t st) {
+  using C = PagedCfg<D>;
+  if (cudaFuncSetAttribute(decode_paged_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES) !=
+      cudaSuccess)
+    return -1;
+  const long long n = (long long)p.B * p.Hkv;
+  if (n > 0x7fffffffLL) return -2;
+  decode_paged_kernel<D><<<(unsigned)n, C::THREADS, C::SMEM_BYTES, st>>>(tk, tv, p);
+  return cudaGetLastError() == cudaSuccess ? 0 : -1;
+}
+
+}  // namespace
+
+int launch_decode_paged(int D, const CUtensorMap& tk, const CUtensorMap& tv, const DecodePagedParams& p,
+                        cudaStream_t st) {
+  switch (D) {
+    case 64: return launch_t<64>(tk, tv, p, st);
+    case 128: return launch_t<128>(tk, tv, p, st);
+    case 256: return launch_t<256>(tk, tv, p, st);
+    default: return -3;
+  }
+}
+
+}  // namespace b2a

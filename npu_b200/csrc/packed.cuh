@@ -1,0 +1,99 @@
+// Work items of attention over packed sequences: which query block of which
+// sequence an item is, found on the device from the offsets alone (no plan,
+// no workspace, no copy of the lengths to the host).
+#pragma once
+
+#include <type_traits>
+
+#include "prefill.cuh"
+
+namespace b2a {
+
+// Blocks are numbered heaviest first, so that the long ones do not start last:
+// a block's level is its number within its sequence plus the blocks' worth of
+// keys ahead of the sequence's first row, and blocks of a level are numbered
+// by sequence. With S(w) = number of blocks of level >= w (a sum over the
+// sequences), block i has the level w with S(w + 1) <= i < S(w), found by
+// bisection, and is the (i - S(w + 1))-th of it, found with ballots.
+// Warp-collective. A call takes about log2(longest / kRows) sums of B / 32
+// steps each, on lengths that stay in L1.
+template <int kRows>
+struct PackedBlocks {
+  const PrefillParams& p;
+  int own_n = 0, own_off = 0;  // this lane's sequence when B <= 32
+  int top = 0;                 // no block has a level above this
+
+  __device__ __forceinline__ void shape(int b, int& n, int& off) const {
+    n = off = 0;
+    if (b >= p.B) return;
+    const int q0 = p.cu_q[b], q1 = p.cu_q[b + 1], k0 = p.cu_k[b], k1 = p.cu_k[b + 1];
+    if (q0 < 0 || q1 < q0 || q1 > p.Tq || k0 < 0 || k1 < k0 || k1 > p.Tk) {
+      if (p.err) atomicOr(p.err, kErrBadArgs);  // not a stretch of the tensors: the sequence is left out
+      return;
+    }
+    const int rows = q1 - q0, keys = k1 - k0;
+    n = (rows + kRows - 1) / kRows;
+    off = max(p.causal ? keys - rows : keys, 0) / kRows;
+  }
+  __device__ __forceinline__ explicit PackedBlocks(const PrefillParams& params) : p(params) {
+    const int lane = threadIdx.x & 31;
+    int most = 0;
+    for (int b0 = 0; b0 < p.B; b0 += 32) {
+      shape(b0 + lane, own_n, own_off);
+      most = max(most, own_n > 0 ? own_n + own_off : 0);
+    }
+    top = __reduce_max_sync(0xffffffffu, most);
+  }
+  __device__ __forceinline__ int count_from(int w) const {
+    const int lane = threadIdx.x & 31;
+    int c = 0;
+    for (int b0 = 0; b0 < p.B; b0 += 32) {
+      int n = own_n, off = own_off;
+      if (p.B > 32) shape(b0 + lane, n, off);
+      c += min(max(n + off - w, 0), n);
+    }
+    return __reduce_add_sync(0xffffffffu, c);
+  }
+  // Block i (every lane gets it). Calls with growing i stay below the last
+  // level found.
+  __device__ __forceinline__ PackedBlock find(int i) {
+    const int lane = threadIdx.x & 31;
+    int lo = 0, hi = top;  // S(hi + 1) <= i always; looking for the largest w with S(w) > i
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (count_from(mid) > i)
+        lo = mid;
+      else
+        hi = mid - 1;
+    }
+    top = lo;
+    int skip = i - count_from(lo + 1);
+    for (int b0 = 0; b0 < p.B; b0 += 32) {
+      int n = own_n, off = own_off;
+      if (p.B > 32) shape(b0 + lane, n, off);
+      const bool has = lo >= off && lo < off + n;
+      const unsigned m = __ballot_sync(0xffffffffu, has);
+      if (skip < __popc(m)) {
+        const bool it = has && __popc(m & ((1u << lane) - 1u)) == skip;
+        const int src = __ffs(__ballot_sync(0xffffffffu, it)) - 1;
+        const int b = b0 + src;
+        PackedBlock k;
+        k.q_base = p.cu_q[b];
+        k.rows = p.cu_q[b + 1] - k.q_base;
+        k.k_base = p.cu_k[b];
+        k.keys = p.cu_k[b + 1] - k.k_base;
+        k.qblk = lo - __shfl_sync(0xffffffffu, off, src);
+        return k;
+      }
+      skip -= __popc(m);
+    }
+    return {0, 0, 0, 0, 0};
+  }
+};
+
+// Stands in for PackedBlocks in kernels that do not pack.
+struct NoBlocks {
+  __device__ __forceinline__ explicit NoBlocks(const PrefillParams&) {}
+};
+
+}  // namespace b2a

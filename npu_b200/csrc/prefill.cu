@@ -3,6 +3,7 @@
 // of this file and is called from capi.cu.
 #include <cstdlib>
 
+#include "packed.cuh"
 #include "prefill.cuh"
 #include "softmax.cuh"
 
@@ -38,13 +39,50 @@ struct PrefillItem {
   int n_t[NQT];  // key blocks query tile t needs; tile 0 never more than
                  // tile 1 and, under the causal mask, at most one fewer
   int n_kv;      // n_t[NQT - 1]: the key blocks that get loaded
+  int Tq, Tk;    // query rows and keys of this item's sequence
+  int q_base, k_base;  // its first row in q and o, its first key in k and v
   __device__ __forceinline__ int head(int t) const { return h + (PAIRS ? t : 0); }
   __device__ __forceinline__ int row0(int t) const { return q0 + (PAIRS ? 0 : 128 * t); }
 };
 
+// The key blocks each tile of an item needs.
+template <int NQT, bool PAIRS>
+__device__ __forceinline__ void prefill_key_blocks(const PrefillParams& p, PrefillItem<NQT, PAIRS>& it) {
+  constexpr int BM = 128, BN = 128;
+#pragma unroll
+  for (int t = 0; t < NQT; ++t) {
+    if (p.causal) {
+      const int last_row = min(it.row0(t) + BM - 1, it.Tq - 1);
+      const long long kv_end = min((long long)it.Tk, (long long)it.sp + last_row + 1);
+      it.n_t[t] = kv_end <= 0 ? 0 : (int)((kv_end + BN - 1) / BN);
+    } else {
+      it.n_t[t] = (it.Tk + BN - 1) / BN;
+    }
+  }
+  it.n_kv = it.n_t[NQT - 1];
+}
+
+// PACKED: item `lin` is head (or head pair) lin % per of block `at`.
+template <int NQT, bool PAIRS>
+__device__ __forceinline__ PrefillItem<NQT, PAIRS> prefill_item_packed(const PrefillParams& p, int lin,
+                                                                       const PackedBlock& at) {
+  PrefillItem<NQT, PAIRS> it;
+  it.h = PAIRS ? 2 * (lin % (p.Hq / 2)) : lin % p.Hq;
+  it.hk = it.h / (p.Hq / p.Hkv);
+  it.b = 0;
+  it.q0 = at.qblk * (128 * (PAIRS ? 1 : NQT));
+  it.Tq = at.rows;
+  it.Tk = at.rows > 0 ? at.keys : 0;
+  it.q_base = at.q_base;
+  it.k_base = at.k_base;
+  it.sp = at.keys - at.rows;
+  prefill_key_blocks(p, it);
+  return it;
+}
+
 template <int NQT, bool PAIRS>
 __device__ __forceinline__ PrefillItem<NQT, PAIRS> prefill_item(const PrefillParams& p, int lin) {
-  constexpr int BM = 128, BN = 128;
+  constexpr int BM = 128;
   PrefillItem<NQT, PAIRS> it;
   int qblk;
   if (PAIRS) {
@@ -69,27 +107,23 @@ __device__ __forceinline__ PrefillItem<NQT, PAIRS> prefill_item(const PrefillPar
     it.q0 = qblk * (BM * NQT);
   }
   it.sp = p.start_pos_arr ? p.start_pos_arr[it.b] : p.start_pos;
-#pragma unroll
-  for (int t = 0; t < NQT; ++t) {
-    if (p.causal) {
-      const int last_row = min(it.row0(t) + BM - 1, p.Tq - 1);
-      const long long kv_end = min((long long)p.Tk, (long long)it.sp + last_row + 1);
-      it.n_t[t] = kv_end <= 0 ? 0 : (int)((kv_end + BN - 1) / BN);
-    } else {
-      it.n_t[t] = (p.Tk + BN - 1) / BN;
-    }
-  }
-  it.n_kv = it.n_t[NQT - 1];
+  it.Tq = p.Tq;
+  it.Tk = p.Tk;
+  it.q_base = it.k_base = 0;
+  prefill_key_blocks(p, it);
   return it;
 }
 
-// PAIRS: head-pair work items (NQT = 2 only), else row blocks.
-template <int D, int NQT, bool PAIRS>
+// PAIRS: head-pair work items (NQT = 2 only), else row blocks. PACKED: the
+// sequences are packed along one row axis (PrefillParams::cu_q, packed.cuh);
+// the scheduler warp then publishes each item's block beside its number.
+template <int D, int NQT, bool PAIRS, bool PACKED>
 __global__ void __launch_bounds__(PrefillCfg<D, NQT>::THREADS, PrefillCfg<D, NQT>::CTAS_PER_SM)
     fa_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                       const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ PrefillParams p) {
   using C = PrefillCfg<D, NQT>;
-  constexpr int kEmuPairs = exp2_emu_pairs<D>();
+  // PACKED keeps every exponential on MUFU (exact to 2^-22).
+  constexpr int kEmuPairs = PACKED ? 0 : exp2_emu_pairs<D>();
   // Warps that take every work item from the scheduler: the producer, the
   // UMMA issuers and the softmax warps.
   constexpr int kConsumerWarps = 1 + NQT + 4 * NQT;
@@ -110,16 +144,33 @@ __global__ void __launch_bounds__(PrefillCfg<D, NQT>::THREADS, PrefillCfg<D, NQT
   // published by the scheduler warp in slot (n - 1) & 1: the blockIdx.x of a
   // CTA it took over, or -1 when there is none (or on abort). Every consumer
   // warp calls this once per item it finishes, in order.
+  PackedBlock at{};  // PACKED: the current item's block
   auto next_item = [&](int n) -> int {
     const int slot = (n - 1) & 1;
     if (!wait_all(&bars->item_full[slot], (uint32_t)((n - 1) >> 1) & 1u)) return -1;
     const int id = *reinterpret_cast<volatile int*>(&bars->item_id[slot]);
+    if constexpr (PACKED) at = bars->item_at[slot];
     __syncwarp();
     if (lane == 0) mbar_arrive(&bars->item_empty[slot]);
     return id;
   };
 
-  const PrefillItem<NQT, PAIRS> first = prefill_item<NQT, PAIRS>(p, blockIdx.x);
+  auto item = [&](int lin) -> PrefillItem<NQT, PAIRS> {
+    if constexpr (PACKED)
+      return prefill_item_packed<NQT, PAIRS>(p, lin, at);
+    else
+      return prefill_item<NQT, PAIRS>(p, lin);
+  };
+  constexpr int kItemRows = 128 * (PAIRS ? 1 : NQT);
+  const int heads_per_block = PAIRS ? p.Hq / 2 : p.Hq;
+  if constexpr (PACKED) {
+    if (warp == 0) {
+      PackedBlocks<kItemRows> blocks(p);
+      at = blocks.find(blockIdx.x / heads_per_block);
+      if (lane == 0) bars->item_at[2] = at;
+    }
+  }
+  const PrefillItem<NQT, PAIRS> first = item(blockIdx.x);  // PACKED: of warp 0 only until the barrier below
   const int first_loads = min(C::STAGES, 2 * first.n_kv);
   if (threadIdx.x == 0) {
     mbar_init(&bars->q_full, 1);
@@ -163,14 +214,14 @@ __global__ void __launch_bounds__(PrefillCfg<D, NQT>::THREADS, PrefillCfg<D, NQT
 #pragma unroll
         for (int c = 0; c < C::KCH; ++c)
           tma_load_4d(sQ + t * C::Q_TILE_BYTES + c * C::CHUNK_BYTES, &tm_q, &bars->q_full, c * 64,
-                      first.row0(t), first.head(t), first.b);
+                      first.q_base + first.row0(t), first.head(t), first.b);
       for (int i = 0; i < first_loads; ++i) {
         uint8_t* dst = sKV + i * C::KV_TILE_BYTES;
         mbar_arrive_expect_tx(&bars->kv_full[i], C::KV_TILE_BYTES);
 #pragma unroll
         for (int c = 0; c < C::KCH; ++c)
           tma_load_4d(dst + c * C::CHUNK_BYTES, (i & 1) ? &tm_v : &tm_k, &bars->kv_full[i], c * 64,
-                      (i >> 1) * C::BN, first.hk, first.b);
+                      first.k_base + (i >> 1) * C::BN, first.hk, first.b);
       }
     }
   }
@@ -182,6 +233,7 @@ __global__ void __launch_bounds__(PrefillCfg<D, NQT>::THREADS, PrefillCfg<D, NQT
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = bars->tmem_base;
+  if constexpr (PACKED) at = bars->item_at[2];
 
   // Each role's code sits entirely inside the branch that set its register
   // budget, so the compiler allocates it against that budget.
@@ -201,7 +253,7 @@ __global__ void __launch_bounds__(PrefillCfg<D, NQT>::THREADS, PrefillCfg<D, NQT
     int q_rounds = 0;  // items with keys (one Q load each)
     bool ok = true;
     for (int n = 1;; ++n) {
-      const PrefillItem<NQT, PAIRS> it = prefill_item<NQT, PAIRS>(p, lin);
+      const PrefillItem<NQT, PAIRS> it = item(lin);
       if (it.n_kv > 0) {
         int i0 = 0;
         if (n == 1) {
@@ -220,7 +272,7 @@ __global__ void __launch_bounds__(PrefillCfg<D, NQT>::THREADS, PrefillCfg<D, NQT
 #pragma unroll
             for (int c = 0; c < C::KCH; ++c)
               tma_load_4d_w(sQ + t * C::Q_TILE_BYTES + c * C::CHUNK_BYTES, &tm_q, &bars->q_full, c * 64,
-                            it.row0(t), it.head(t), it.b);
+                            it.q_base + it.row0(t), it.head(t), it.b);
         }
         ++q_rounds;
         for (int i = i0; i < 2 * it.n_kv; ++i) {
@@ -236,8 +288,8 @@ __global__ void __launch_bounds__(PrefillCfg<D, NQT>::THREADS, PrefillCfg<D, NQT
           mbar_arrive_expect_tx_w(&bars->kv_full[slot], C::KV_TILE_BYTES);
 #pragma unroll
           for (int c = 0; c < C::KCH; ++c)
-            tma_load_4d_w(dst + c * C::CHUNK_BYTES, m, &bars->kv_full[slot], c * 64, (i >> 1) * C::BN, it.hk,
-                          it.b);
+            tma_load_4d_w(dst + c * C::CHUNK_BYTES, m, &bars->kv_full[slot], c * 64, it.k_base + (i >> 1) * C::BN,
+                          it.hk, it.b);
           issued = g + 1;
         }
         if (!ok) break;
@@ -298,7 +350,7 @@ __global__ void __launch_bounds__(PrefillCfg<D, NQT>::THREADS, PrefillCfg<D, NQT
     int stg = 0;       // head-pair items with keys so far (stagger rounds)
     bool ok = true;
     for (int n = 1;; ++n) {
-      const PrefillItem<NQT, PAIRS> it = prefill_item<NQT, PAIRS>(p, lin);
+      const PrefillItem<NQT, PAIRS> it = item(lin);
       const int nt = t == 0 ? it.n_t[0] : it.n_kv;
       if (it.n_kv > 0) {
         auto slot_of = [&](int i) { return (G + i) % C::STAGES; };
@@ -354,6 +406,12 @@ __global__ void __launch_bounds__(PrefillCfg<D, NQT>::THREADS, PrefillCfg<D, NQT
             ok = false;
             break;
           }
+          // The last block may reach into the next sequence's rows of V, and
+          // a P of 0 does not hide a NaN there: clear them. Both issuers do,
+          // each before its own MMAs read the tile (zeros over zeros).
+          if constexpr (PACKED)
+            if ((j + 1) * C::BN > it.Tk)
+              clear_v_rows<D>(smem_u32(sKV) + vslot * C::KV_TILE_BYTES, it.Tk - j * C::BN, C::BN, C::CHUNK_BYTES);
           // Mid-block handoff: the next block's first S half (needed first by
           // the softmax), then the first PV half.
           if (!wait_all(&bars->mid[t], par)) {
@@ -412,6 +470,7 @@ __global__ void __launch_bounds__(PrefillCfg<D, NQT>::THREADS, PrefillCfg<D, NQT
     // n - 1, i.e. has started working on it: one item of look-ahead, so the
     // next Q and K/V can stream in early while the claim stays late enough
     // for the last items to spread over the CTAs that finish first.
+    std::conditional_t<PACKED, PackedBlocks<kItemRows>, NoBlocks> blocks(p);
     for (int n = 1;; ++n) {
       if (n >= 2 && !wait_all(&bars->item_empty[(n - 2) & 1], (uint32_t)((n - 2) >> 1) & 1u)) break;
       const uint32_t cpar = (uint32_t)(n - 1) & 1u;
@@ -428,8 +487,11 @@ __global__ void __launch_bounds__(PrefillCfg<D, NQT>::THREADS, PrefillCfg<D, NQT
       }
       const int id = clc_cancelled_ctaid_x(bars->clc_resp);
       __syncwarp();
+      if constexpr (PACKED)
+        if (id >= 0) at = blocks.find(id / heads_per_block);
       if (lane == 0) {
         bars->item_id[(n - 1) & 1] = id;
+        if constexpr (PACKED) bars->item_at[(n - 1) & 1] = at;
         mbar_arrive(&bars->item_full[(n - 1) & 1]);
       }
       __syncwarp();
@@ -451,12 +513,13 @@ __global__ void __launch_bounds__(PrefillCfg<D, NQT>::THREADS, PrefillCfg<D, NQT
     int o_rounds = 0;  // earlier items in which this tile had key blocks
     bool ok = true;
     for (int n = 1;; ++n) {
-      const PrefillItem<NQT, PAIRS> it = prefill_item<NQT, PAIRS>(p, lin);
+      const PrefillItem<NQT, PAIRS> it = item(lin);
       const int b = it.b, h = it.head(t);
       const int grow = it.row0(t) + row;
-      const bool valid = grow < p.Tq;
+      const bool valid = grow < it.Tq;
+      const int orow = it.q_base + grow;  // row of o, gate and lse
       // Last visible key of this row (fits in int: it is below Tk).
-      const int kv_last = p.causal ? (int)min((long long)it.sp + grow, (long long)p.Tk - 1) : p.Tk - 1;
+      const int kv_last = p.causal ? (int)min((long long)it.sp + grow, (long long)it.Tk - 1) : it.Tk - 1;
       float m_run = -INFINITY;
       float l_run = 0.f;
       const int n_mine = t == 0 ? it.n_t[0] : it.n_kv;
@@ -478,6 +541,11 @@ __global__ void __launch_bounds__(PrefillCfg<D, NQT>::THREADS, PrefillCfg<D, NQT
         tmem_ld32(tR + fcol, s[0]);
         tmem_ld32(tR + fcol + 32, s[1]);
         tmem_wait_ld();
+        // Rows past the sequence's end hold the next sequence's queries: their
+        // scores become 0, as if the rows were zeros, so nothing of a
+        // neighbour (a NaN in it, say) reaches this warp's choices.
+        if constexpr (PACKED)
+          if (!__all_sync(0xffffffffu, valid)) clear_scores(s, valid);
         float hs0, hs1;
         const float a0 = softmax_half_tmem<kEmuPairs>(s, lim, sl2, m_run, tR + fcol, hs0);
         auto rescale_O = [&](float f) {
@@ -506,6 +574,8 @@ __global__ void __launch_bounds__(PrefillCfg<D, NQT>::THREADS, PrefillCfg<D, NQT
         tmem_ld32(tR + scol, s[0]);
         tmem_ld32(tR + scol + 32, s[1]);
         tmem_wait_ld();
+        if constexpr (PACKED)
+          if (!__all_sync(0xffffffffu, valid)) clear_scores(s, valid);
         // One handoff: P for keys 0-63 is in TMEM (the first PV half can go)
         // and the second S half is in registers (its columns can take the
         // first half of S_t(j+1)).
@@ -542,8 +612,8 @@ __global__ void __launch_bounds__(PrefillCfg<D, NQT>::THREADS, PrefillCfg<D, NQT
 #pragma unroll
           for (int i = 0; i < 32; ++i) z[i] = 0u;
 #pragma unroll
-          for (int c = 0; c < D / 32; ++c) store_out_chunk(p, b, h, grow, c, z, 0.f);
-          if (p.lse) p.lse[((long long)b * p.Hq + h) * p.Tq + grow] = -INFINITY;
+          for (int c = 0; c < D / 32; ++c) store_out_chunk(p, b, h, orow, c, z, 0.f);
+          if (p.lse) p.lse[((long long)b * p.Hq + h) * p.Tq + orow] = -INFINITY;
         }
       } else {
         const bool w = ok && mbar_wait(&bars->o_full[t], (uint32_t)o_rounds & 1u, abort_flag, p.err);
@@ -559,12 +629,12 @@ __global__ void __launch_bounds__(PrefillCfg<D, NQT>::THREADS, PrefillCfg<D, NQT
             tmem_ld32(tO + 32 * c + 32, o[1]);
             tmem_wait_ld();
             if (valid) {
-              store_out_chunk(p, b, h, grow, c, o[0], inv_l);
-              store_out_chunk(p, b, h, grow, c + 1, o[1], inv_l);
+              store_out_chunk(p, b, h, orow, c, o[0], inv_l);
+              store_out_chunk(p, b, h, orow, c + 1, o[1], inv_l);
             }
           }
           if (p.lse && valid) {
-            p.lse[((long long)b * p.Hq + h) * p.Tq + grow] =
+            p.lse[((long long)b * p.Hq + h) * p.Tq + orow] =
                 l_run > 0.f ? (m_run + __log2f(l_run)) * 0.69314718055994531f : -INFINITY;
           }
         }
@@ -587,21 +657,21 @@ __global__ void __launch_bounds__(PrefillCfg<D, NQT>::THREADS, PrefillCfg<D, NQT
 }
 
 // ------------------------------------------------------------------ launcher
-template <int D, int NQT, bool PAIRS>
+template <int D, int NQT, bool PAIRS, bool PACKED = false>
 static int launch_prefill_t(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
                             const PrefillParams& p, cudaStream_t st) {
   using C = PrefillCfg<D, NQT>;
-  cudaError_t e = cudaFuncSetAttribute(fa_prefill_kernel<D, NQT, PAIRS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+  cudaError_t e = cudaFuncSetAttribute(fa_prefill_kernel<D, NQT, PAIRS, PACKED>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        C::SMEM_BYTES);
   if (e != cudaSuccess) return -1;
   // The in-kernel register split needs at least MIN_LAUNCH_REGS per thread.
   cudaFuncAttributes fa{};
-  if (cudaFuncGetAttributes(&fa, fa_prefill_kernel<D, NQT, PAIRS>) != cudaSuccess || fa.numRegs < C::MIN_LAUNCH_REGS)
+  if (cudaFuncGetAttributes(&fa, fa_prefill_kernel<D, NQT, PAIRS, PACKED>) != cudaSuccess || fa.numRegs < C::MIN_LAUNCH_REGS)
     return -1;
   // One CTA per work item (query blocks x query heads, or x head pairs).
-  const long long nblk = (long long)p.n_qblk * p.B * (p.head_pairs ? p.Hq / 2 : p.Hq);
+  const long long nblk = (long long)p.n_qblk * (PACKED ? 1 : p.B) * (p.head_pairs ? p.Hq / 2 : p.Hq);
   if (nblk <= 0 || nblk > 0x7fffffffLL) return -2;
-  fa_prefill_kernel<D, NQT, PAIRS><<<(unsigned)nblk, C::THREADS, C::SMEM_BYTES, st>>>(tq, tk, tv, p);
+  fa_prefill_kernel<D, NQT, PAIRS, PACKED><<<(unsigned)nblk, C::THREADS, C::SMEM_BYTES, st>>>(tq, tk, tv, p);
   return cudaGetLastError() == cudaSuccess ? 0 : -1;
 }
 
@@ -639,6 +709,33 @@ PrefillPlan prefill_plan(int D, int Hq, int Hkv, int Tq, int Tk) {
     return PrefillPlan{128, 2, 1, 0};
   if (Tq <= kOneTileMaxRows) return PrefillPlan{128, 1, 0, 0};
   return PrefillPlan{256, 2, 0, 0};
+}
+
+// Packed sequences: by the same rules on the average length (the lengths
+// themselves are on the device). Row pairs only for odd groups: an even group
+// shares its key blocks between heads at any length.
+PrefillPlan prefill_plan_packed(int D, int Hq, int Hkv, long long rows, int B) {
+  if (D == 256) return PrefillPlan{128, 1, 0, 0};
+  const long long mean = rows / B;
+  if ((Hq / Hkv) % 2 == 0) return mean >= kHeadPairMinRows ? PrefillPlan{128, 2, 1, 0} : PrefillPlan{128, 1, 0, 0};
+  return mean <= kOneTileMaxRows ? PrefillPlan{128, 1, 0, 0} : PrefillPlan{256, 2, 0, 0};
+}
+
+int launch_prefill_packed(int D, const PrefillPlan& plan, const CUtensorMap& tq, const CUtensorMap& tk,
+                          const CUtensorMap& tv, const PrefillParams& p, cudaStream_t st) {
+  const bool one = plan.tiles == 1;
+  switch (D) {
+    case 64:
+      return one ? launch_prefill_t<64, 1, false, true>(tq, tk, tv, p, st)
+                 : (plan.head_pairs ? launch_prefill_t<64, 2, true, true>(tq, tk, tv, p, st)
+                                    : launch_prefill_t<64, 2, false, true>(tq, tk, tv, p, st));
+    case 128:
+      return one ? launch_prefill_t<128, 1, false, true>(tq, tk, tv, p, st)
+                 : (plan.head_pairs ? launch_prefill_t<128, 2, true, true>(tq, tk, tv, p, st)
+                                    : launch_prefill_t<128, 2, false, true>(tq, tk, tv, p, st));
+    case 256: return launch_prefill_packed_d256(tq, tk, tv, p, st);
+    default: return -3;
+  }
 }
 
 int launch_prefill(int D, const PrefillPlan& plan, const CUtensorMap& tq, const CUtensorMap& tk,

@@ -74,6 +74,13 @@ struct PrefillParams {
   const void* gate;
   long long g_sb, g_sh, g_st;
   int gate_bf16;
+  // Packed sequences (the kernels' PACKED form, b2a_prefill_varlen): sequence
+  // b owns query rows [cu_q[b], cu_q[b + 1]) and keys [cu_k[b], cu_k[b + 1])
+  // of one packed tensor each (device, [B + 1]); the tensors' batch is one,
+  // Tq is the total number of query rows, n_qblk the number of query blocks
+  // there can be, start_pos is not used.
+  const int* cu_q;
+  const int* cu_k;
   // 1: O's base and strides are 32-byte aligned, so the epilogue's
   // row-per-thread stores may be 32-byte vector stores.
   int o_v8;
@@ -120,6 +127,14 @@ struct PrefillCfg {
   static_assert(MIN_LAUNCH_REGS * THREADS * CTAS_PER_SM <= 65536, "register budget");
 };
 
+// PACKED: one query block of one sequence. Empty (rows == 0) for the grid's
+// spare blocks.
+struct PackedBlock {
+  int q_base, rows;  // the sequence's first row in q, its rows
+  int k_base, keys;  // its first key in k, its keys
+  int qblk;          // query block within the sequence
+};
+
 // Barrier slots inside the OFF_BAR region.
 struct PrefillBars {
   uint64_t q_full;
@@ -145,6 +160,7 @@ struct PrefillBars {
   uint64_t clc_bar;
   alignas(16) uint8_t clc_resp[16];
   int item_id[2];
+  PackedBlock item_at[3];  // PACKED: the two ring slots' blocks, and the CTA's own
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -152,6 +168,15 @@ struct PrefillBars {
 // Head dim 256 variant (one query tile per CTA, prefill_d256.cu).
 int launch_prefill_d256(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
                         const PrefillParams& p, cudaStream_t st);
+
+// Packed sequences (p.cu_q, p.cu_k; any supported D): the plan for `rows`
+// query rows in B sequences, and the launch. Returns as launch_prefill.
+struct PrefillPlan;
+PrefillPlan prefill_plan_packed(int D, int Hq, int Hkv, long long rows, int B);
+int launch_prefill_packed(int D, const PrefillPlan& plan, const CUtensorMap& tq, const CUtensorMap& tk,
+                          const CUtensorMap& tv, const PrefillParams& p, cudaStream_t st);
+int launch_prefill_packed_d256(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
+                               const PrefillParams& p, cudaStream_t st);
 
 // How the D <= 128 kernel cuts this problem into work items: rows per item
 // and per query head (256 or 128: PrefillParams::n_qblk must be computed

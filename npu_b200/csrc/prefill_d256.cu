@@ -14,6 +14,7 @@
 // MMA order: S(0), S(1), then per block j: PV(j), S(j+2). While the softmax
 // warpgroup turns S(j) into P(j), the tensor core runs PV(j-1) and S(j+1).
 // Warps: 0 TMA, 1 TMEM + MMA issue, 2-3 idle, 4-7 softmax + epilogue.
+#include "packed.cuh"
 #include "prefill.cuh"
 #include "softmax.cuh"
 
@@ -51,6 +52,7 @@ struct D256Bars {
   uint64_t pv_done;
   uint64_t o_full;
   uint64_t drain;
+  PackedBlock block;  // PACKED: this CTA's
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -81,6 +83,9 @@ __device__ __forceinline__ bool d256_load_item(int i, int n, int* blk) {
   return true;
 }
 
+// PACKED: the sequences are packed along one row axis (PrefillParams::cu_q,
+// packed.cuh).
+template <bool PACKED>
 __global__ void __launch_bounds__(256, 1)
     fa_prefill_d256_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                            const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ PrefillParams p) {
@@ -95,21 +100,42 @@ __global__ void __launch_bounds__(256, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   // Block -> (query tile, head, batch), heaviest causal tiles first.
-  const int hb = p.Hq * p.B;
   const int lin = blockIdx.x;
-  const int qt = p.n_qblk - 1 - lin / hb;
-  const int rem = lin % hb;
-  const int h = rem % p.Hq, b = rem / p.Hq;
+  int h, b, q0, sp, Tq, Tk, q_base = 0, k_base = 0;
+  if constexpr (PACKED) {
+    h = lin % p.Hq;
+    b = 0;
+    if (warp == 0) {
+      PackedBlocks<C::BM> blocks(p);
+      const PackedBlock at = blocks.find(lin / p.Hq);
+      if (lane == 0) bars->block = at;
+    }
+    __syncthreads();
+    const PackedBlock at = bars->block;
+    q0 = at.qblk * C::BM;
+    sp = at.keys - at.rows;
+    Tq = at.rows;
+    Tk = at.rows > 0 ? at.keys : 0;
+    q_base = at.q_base;
+    k_base = at.k_base;
+  } else {
+    const int hb = p.Hq * p.B;
+    const int qt = p.n_qblk - 1 - lin / hb;
+    const int rem = lin % hb;
+    h = rem % p.Hq, b = rem / p.Hq;
+    q0 = qt * C::BM;
+    sp = p.start_pos_arr ? p.start_pos_arr[b] : p.start_pos;
+    Tq = p.Tq;
+    Tk = p.Tk;
+  }
   const int hk = h / (p.Hq / p.Hkv);
-  const int q0 = qt * C::BM;
-  const int sp = p.start_pos_arr ? p.start_pos_arr[b] : p.start_pos;
   int n;
   if (p.causal) {
-    const int last_row = min(q0 + C::BM - 1, p.Tq - 1);
-    const long long kv_end = min((long long)p.Tk, (long long)sp + last_row + 1);
+    const int last_row = min(q0 + C::BM - 1, Tq - 1);
+    const long long kv_end = min((long long)Tk, (long long)sp + last_row + 1);
     n = kv_end <= 0 ? 0 : (int)((kv_end + C::BN - 1) / C::BN);
   } else {
-    n = (p.Tk + C::BN - 1) / C::BN;
+    n = (Tk + C::BN - 1) / C::BN;
   }
   const int n_items = n == 0 ? 0 : 2 * n;
 
@@ -151,7 +177,7 @@ __global__ void __launch_bounds__(256, 1)
       // -------------------------------------------------------- producer
       mbar_arrive_expect_tx_w(&bars->q_full, C::Q_BYTES);
       for (int c = 0; c < C::KCH; ++c)
-        tma_load_4d_w(sQ + c * C::Q_CHUNK, &tm_q, &bars->q_full, c * 64, q0, h, b);
+        tma_load_4d_w(sQ + c * C::Q_CHUNK, &tm_q, &bars->q_full, c * 64, q_base + q0, h, b);
       int issued = 0;
       for (int i = 0; i < n_items; ++i) {
         const int slot = i % C::STAGES;
@@ -163,8 +189,8 @@ __global__ void __launch_bounds__(256, 1)
         uint8_t* dst = sKV + slot * C::KV_TILE_BYTES;
         mbar_arrive_expect_tx_w(&bars->kv_full[slot], C::KV_TILE_BYTES);
         for (int c = 0; c < C::KCH; ++c)
-          tma_load_4d_w(dst + c * C::KV_CHUNK, is_v ? &tm_v : &tm_k, &bars->kv_full[slot], c * 64, blk * C::BN, hk,
-                      b);
+          tma_load_4d_w(dst + c * C::KV_CHUNK, is_v ? &tm_v : &tm_k, &bars->kv_full[slot], c * 64,
+                        k_base + blk * C::BN, hk, b);
         issued = i + 1;
       }
       if (*abort_flag && lane == 0) {
@@ -224,6 +250,11 @@ __global__ void __launch_bounds__(256, 1)
         if (vslot < 0) break;
         if (!__all_sync(0xffffffffu, mbar_wait(&bars->p_full[j & 1], (uint32_t)(j >> 1) & 1u, abort_flag, p.err)))
           break;
+        // Rows of V past the sequence's end belong to the next one, and a P of
+        // 0 does not hide a NaN there: clear them.
+        if constexpr (PACKED)
+          if ((j + 1) * C::BN > Tk)
+            clear_v_rows<C::D>(smem_u32(sKV) + vslot * C::KV_TILE_BYTES, Tk - j * C::BN, C::BN, C::KV_CHUNK);
         tc_fence_after();
         issue_PV(j & 1, vslot, j > 0);
         tc_commit_w(&bars->pv_done);
@@ -248,9 +279,10 @@ __global__ void __launch_bounds__(256, 1)
     const uint32_t lane_off = (uint32_t)(wq * 32) << 16;
     const uint32_t tO = tmem + lane_off + C::O_COL;
     const int grow = q0 + row;
-    const bool valid = grow < p.Tq;
+    const bool valid = grow < Tq;
+    const int orow = q_base + grow;  // row of o, gate and lse
     const long long row_pos = (long long)sp + grow;
-    const long long kv_last = p.causal ? min(row_pos, (long long)p.Tk - 1) : (long long)p.Tk - 1;
+    const long long kv_last = p.causal ? min(row_pos, (long long)Tk - 1) : (long long)Tk - 1;
     const float sl2 = p.scale_log2;
     float m_run = -INFINITY, l_run = 0.f;
     bool ok = true;
@@ -321,7 +353,7 @@ __global__ void __launch_bounds__(256, 1)
       const uint32_t tP = tmem + lane_off + C::S_COL + buf * C::BN;
       // Warp-uniform choice: the TMEM stores inside are warp-wide.
       if (__all_sync(0xffffffffu, lim == C::BN - 1))
-        l_run += softmax_p_row_tmem<C::BN, true>(s, sl2, m_use, tP);
+        l_run += softmax_p_row_tmem<C::BN, !PACKED>(s, sl2, m_use, tP);  // PACKED: MUFU only (exact to 2^-22)
       else
         l_run += softmax_p_row_tmem<C::BN, false>(s, sl2, m_use, tP);
 #undef S_AT
@@ -352,8 +384,8 @@ __global__ void __launch_bounds__(256, 1)
         uint32_t z[32];
 #pragma unroll
         for (int i = 0; i < 32; ++i) z[i] = 0u;
-        for (int c = 0; c < C::D / 32; ++c) store_out_chunk(p, b, h, grow, c, z, 0.f);
-        if (p.lse) p.lse[((long long)b * p.Hq + h) * p.Tq + grow] = -INFINITY;
+        for (int c = 0; c < C::D / 32; ++c) store_out_chunk(p, b, h, orow, c, z, 0.f);
+        if (p.lse) p.lse[((long long)b * p.Hq + h) * p.Tq + orow] = -INFINITY;
       }
     } else if (ok) {
       const bool w = mbar_wait(&bars->o_full, 0, abort_flag, p.err);
@@ -365,10 +397,10 @@ __global__ void __launch_bounds__(256, 1)
           uint32_t o[32];
           tmem_ld32(tO + 32 * c, o);
           tmem_wait_ld();
-          if (valid) store_out_chunk(p, b, h, grow, c, o, inv_l);
+          if (valid) store_out_chunk(p, b, h, orow, c, o, inv_l);
         }
         if (p.lse && valid)
-          p.lse[((long long)b * p.Hq + h) * p.Tq + grow] =
+          p.lse[((long long)b * p.Hq + h) * p.Tq + orow] =
               l_run > 0.f ? (m_run + __log2f(l_run)) * 0.69314718055994531f : -INFINITY;
       }
     }
@@ -383,16 +415,31 @@ __global__ void __launch_bounds__(256, 1)
   }
 }
 
+namespace {
+
+template <bool PACKED>
+int launch_d256(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const PrefillParams& p,
+                cudaStream_t st) {
+  using C = D256Cfg;
+  if (cudaFuncSetAttribute(fa_prefill_d256_kernel<PACKED>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           C::SMEM_BYTES) != cudaSuccess)
+    return -1;
+  const long long nblk = (long long)p.n_qblk * p.Hq * (PACKED ? 1 : p.B);
+  if (nblk <= 0 || nblk > 0x7fffffffLL) return -2;
+  fa_prefill_d256_kernel<PACKED><<<(unsigned)nblk, C::THREADS, C::SMEM_BYTES, st>>>(tq, tk, tv, p);
+  return cudaGetLastError() == cudaSuccess ? 0 : -1;
+}
+
+}  // namespace
+
 int launch_prefill_d256(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
                         const PrefillParams& p, cudaStream_t st) {
-  using C = D256Cfg;
-  if (cudaFuncSetAttribute(fa_prefill_d256_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES) !=
-      cudaSuccess)
-    return -1;
-  const long long nblk = (long long)p.n_qblk * p.Hq * p.B;
-  if (nblk <= 0 || nblk > 0x7fffffffLL) return -2;
-  fa_prefill_d256_kernel<<<(unsigned)nblk, C::THREADS, C::SMEM_BYTES, st>>>(tq, tk, tv, p);
-  return cudaGetLastError() == cudaSuccess ? 0 : -1;
+  return launch_d256<false>(tq, tk, tv, p, st);
+}
+
+int launch_prefill_packed_d256(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
+                               const PrefillParams& p, cudaStream_t st) {
+  return launch_d256<true>(tq, tk, tv, p, st);
 }
 
 }  // namespace b2a

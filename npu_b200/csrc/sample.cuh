@@ -1,0 +1,28 @@
+// Parameters and launcher of token sampling (sample.cu).
+#pragma once
+
+#include "common.cuh"
+
+namespace b2a {
+
+struct SampleParams {
+  const void* logits;  // [R, V], row stride ld_logits, fp32 or bf16
+  long long ld_logits;
+  int logits_bf16;
+  const float* noise;  // [R, V] of Exp(1), row stride ld_noise; may be null if no row draws (greedy)
+  long long ld_noise;
+  // Per-row settings [R] (device), or nullptr: the value for all rows.
+  const float* temperature;
+  const int* top_k;
+  const float* top_p;
+  const float* min_p;
+  float temperature_all, top_p_all, min_p_all;
+  int top_k_all;
+  long long* out;  // [R] token ids, -1 for a row without a usable logit
+  int R, V;
+};
+
+// Returns 0 or a negative value on launch failure.
+int launch_sample(const SampleParams& p, cudaStream_t st);
+
+}  // namespace b2a

@@ -272,6 +272,24 @@ __device__ __forceinline__ float softmax_half_tmem(uint32_t (&s)[2][32], int lim
   return a;
 }
 
+__device__ __forceinline__ void clear_scores(uint32_t (&s)[2][32], bool keep) {
+#pragma unroll
+  for (int i = 0; i < 64; ++i) s[i >> 5][i & 31] = keep ? s[i >> 5][i & 31] : 0u;
+}
+
+// Zero rows [from, rows) of a V tile in shared memory (D / 64 chunks of
+// `rows` 128-byte rows, chunk_bytes apart) before an MMA reads it. A whole
+// warp calls it; the fence makes its writes visible to the tensor core.
+template <int D>
+__device__ __forceinline__ void clear_v_rows(uint32_t tile, int from, int rows, int chunk_bytes) {
+  const int lane = threadIdx.x & 31;
+  const int units = (rows - from) * 8;
+  for (int c = 0; c < D / 64; ++c)
+    for (int u = lane; u < units; u += 32) st_shared_v4(tile + c * chunk_bytes + from * 128 + u * 16, 0u, 0u, 0u, 0u);
+  fence_proxy_async_smem();
+  __syncwarp();
+}
+
 // sigmoid(g) = 1 / (1 + e^-g) in fp32 (torch.sigmoid, qwen/forward.py:226).
 __device__ __forceinline__ float sigmoidf_(float g) { return __fdividef(1.f, 1.f + __expf(-g)); }
 
