@@ -278,6 +278,7 @@ int b2a_sample(const void* logits, long long ld_logits, int logits_bf16, const f
   p.out = out;
   p.R = R;
   p.V = V;
+  p.err = err;
   return status_of(b2a::launch_sample(p, static_cast<cudaStream_t>(stream)));
 }
 

@@ -20,9 +20,12 @@ struct SampleParams {
   int top_k_all;
   long long* out;  // [R] token ids, -1 for a row without a usable logit
   int R, V;
+  int cluster;  // CTAs per row (a power of two), set by launch_sample
+  int slice;    // tokens per CTA, a multiple of 8
+  int* err;
 };
 
 // Returns 0 or a negative value on launch failure.
-int launch_sample(const SampleParams& p, cudaStream_t st);
+int launch_sample(SampleParams p, cudaStream_t st);
 
 }  // namespace b2a
