@@ -29,98 +29,58 @@ namespace b2a {
 
 namespace {
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8;
 constexpr int kGroup = 8;                      // logits a thread handles at a time
+constexpr int kMaskGroups = 64 / kGroup;
 constexpr int kMaxStageBytes = 200 * 1024;     // slices above this stay in global memory
-
-__device__ __forceinline__ float usable(float x) { return x == x ? __fadd_rn(x, 0.f) : -INFINITY; }
 
 // w(x) = exp(z), z = (x - m) / T rounded as the division rounds: the
 // quotient's estimate q = d rT is corrected by its remainder. 2^t for
 // t = z log2(e) is then corrected for t's rounding and for log2(e)'s (which
-// alone would cost |z| 2^-24): about 2^-22 in all.
+// alone would cost |z| 2^-24): about 2^-22 in all. The passes over all tokens
+// use quick(): |z| 2^-22 off, a third of the instructions, enough for sums
+// and for each thread to pick its candidate; candidates are then compared by
+// the exact form. NaN and -inf weigh 0.
 struct Weight {
   float m, T, rT;
+  __device__ __forceinline__ float quick(float x) const {
+    return ex2(fmaxf((x - m) * (rT * 1.442695040888963f), -150.f));
+  }
   __device__ __forceinline__ float operator()(float x) const {
     constexpr float kHi = 1.442695040888963f, kLo = 1.925963033e-8f;  // log2(e) in two fp32 terms
     const float d = __fsub_rn(x, m);
     const float q = __fmul_rn(d, rT);
-    float z = fmaf(fmaf(-q, T, d), rT, q);
-    z = d > -INFINITY ? fmaxf(z, -104.f) : -104.f;  // exp(-104) is below every fp32 number
+    const float z = fmaxf(fmaf(fmaf(-q, T, d), rT, q), -104.f);  // exp(-104) is below every fp32 number
     const float t = __fmul_rn(z, kHi);
     const float r = fmaf(z, kLo, fmaf(z, kHi, -t));
     const float w = ex2(t);
-    return x == m ? 1.f : fmaf(w, r * 0.6931471805599453f, w);
+    return fmaf(w, r * 0.6931471805599453f, w);
   }
 };
 
-// A race entry: ratio (not negative) in the high word, the index's complement
-// in the low one, so the larger entry is the larger ratio, then the lower index.
-__device__ __forceinline__ unsigned long long entry(float ratio, int i) {
-  return ((unsigned long long)__float_as_uint(fmaxf(ratio, 0.f)) << 32) | (0xffffffffu - (unsigned)i);
-}
-__device__ __forceinline__ int entry_index(unsigned long long e) { return (int)(0xffffffffu - (unsigned)e); }
-
-struct Found {  // 24 bytes, its members 8-byte aligned in pairs
-  unsigned long long best;  // race winner
-  float x;                  // its logit
-  float sum;                // weight
+// What a pass finds, joined over threads, warps and CTAs: the entry with the
+// largest score (ordered bits; 0: none), the lowest token among equals, its
+// logit, and the pass's weight and count.
+constexpr uint32_t kNone = 0xffffffffu;
+struct alignas(8) Found {
+  uint32_t score, token;
+  float x, sum;
   int count;
-  int pad;
 };
+__device__ __forceinline__ Found nothing() { return {0, kNone, 0.f, 0.f, 0}; }
 
-__device__ __forceinline__ Found join(const Found& a, const Found& b) {
-  const bool first = a.best >= b.best;
-  return {first ? a.best : b.best, first ? a.x : b.x, a.sum + b.sum, a.count + b.count, 0};
-}
-
-__device__ __forceinline__ Found warp_join(Found f, int width) {
-  for (int off = width / 2; off > 0; off >>= 1)
-    f = join(f, {__shfl_xor_sync(0xffffffffu, f.best, off), __shfl_xor_sync(0xffffffffu, f.x, off),
-                 __shfl_xor_sync(0xffffffffu, f.sum, off), __shfl_xor_sync(0xffffffffu, f.count, off), 0});
-  return f;
-}
-
-struct Shared {
-  Found warp[kWarps];
-  Found cta[2][kMaxCluster];  // every CTA's value, written by its owner into each CTA of the cluster
-  uint64_t full;
-  int abort_flag;
-};
-
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-
-// Every thread of the cluster gets the joined value; pass counts the calls.
-// A CTA writes pass n's slots after the barrier of pass n - 1, when everyone
-// has read those of pass n - 2, so two sets of slots are enough.
-__device__ __forceinline__ Found cluster_join(Found f, Shared* sh, int rank, int size, int& pass) {
-  f = warp_join(f, 32);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (lane == 0) sh->warp[warp] = f;
-  __syncthreads();
-  f = warp_join(sh->warp[lane % kWarps], kWarps);
-  if (size > 1) {
-    Found* slots = sh->cta[pass & 1];
-    if (threadIdx.x < size) {
-      uint32_t remote;
-      asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_u32(slots + rank)), "r"(threadIdx.x));
-      asm volatile(
-          "st.shared::cluster.u64 [%0], %1;\n\t"
-          "st.shared::cluster.v2.f32 [%0 + 8], {%2, %3};\n\t"
-          "st.shared::cluster.u32 [%0 + 16], %4;" ::"r"(remote),
-          "l"(f.best), "f"(f.x), "f"(f.sum), "r"(f.count)
-          : "memory");
-    }
-    cluster_sync();
-    f = warp_join(slots[lane % size], size);
-  } else {
-    __syncthreads();
-  }
-  ++pass;
+__device__ __forceinline__ Found warp_join(Found f) {
+  const uint32_t score = __reduce_max_sync(0xffffffffu, f.score);
+  const uint32_t token = __reduce_min_sync(0xffffffffu, f.score == score ? f.token : kNone);
+  const unsigned who = __ballot_sync(0xffffffffu, f.score == score && f.token == token);
+  f.x = __shfl_sync(0xffffffffu, f.x, __ffs(who) - 1);
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) f.sum += __shfl_xor_sync(0xffffffffu, f.sum, off);
+  f.count = __reduce_add_sync(0xffffffffu, f.count);
+  f.score = score;
+  f.token = token;
   return f;
 }
 
@@ -144,11 +104,79 @@ __device__ __forceinline__ void load_group(const __nv_bfloat16* p, float (&x)[kG
     x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
   }
 }
+// The larger of a and the group's logits (NaN ignored).
+__device__ __forceinline__ float group_max(float a, const float (&x)[kGroup]) {
+#pragma unroll
+  for (int e = 0; e < kGroup; e += 2) asm("max.f32 %0, %0, %1, %2;" : "+f"(a) : "f"(x[e]), "f"(x[e + 1]));
+  return a;
+}
+
+// The same from 16-byte aligned memory, bf16 in pairs.
+__device__ __forceinline__ float group_max(float a, const float* p) {
+  float x[kGroup];
+  load_group(p, x);
+  return group_max(a, x);
+}
+__device__ __forceinline__ float group_max(float a, const __nv_bfloat16* p) {
+  const uint4 v = *reinterpret_cast<const uint4*>(p);
+  uint32_t y, z;
+  asm("max.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(v.x), "r"(v.y));
+  asm("max.bf16x2 %0, %1, %2;" : "=r"(z) : "r"(v.z), "r"(v.w));
+  asm("max.bf16x2 %0, %0, %1;" : "+r"(y) : "r"(z));
+  asm("max.f32 %0, %0, %1, %2;" : "+f"(a) : "f"(__uint_as_float(y << 16)), "f"(__uint_as_float(y & 0xffff0000u)));
+  return a;
+}
+
+// A thread's candidate in a race.
+struct Candidate {
+  float ratio = 0.f, x = 0.f;
+  int i = -1;
+  __device__ __forceinline__ void offer(float w, float e, float xi, int at) {
+    const float ratio_i = __fdividef(w, e);
+    if (ratio_i > ratio) ratio = ratio_i, x = xi, i = at;
+  }
+};
+
+struct Shared {
+  Found warp[kWarps];
+  Found cta[2][kMaxCluster];  // every CTA's value, written by its owner into each CTA of the cluster
+  uint64_t full;
+  int abort_flag;
+};
+
+// Every thread of the cluster gets the joined value; pass counts the calls.
+// A CTA writes pass n's slots after the barrier of pass n - 1, when everyone
+// has read those of pass n - 2, so two sets of slots are enough.
+__device__ __forceinline__ Found cluster_join(Found f, Shared* sh, int rank, int size, int& pass) {
+  f = warp_join(f);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (lane == 0) sh->warp[warp] = f;
+  __syncthreads();
+  Found* slots = sh->cta[pass & 1];
+  if (warp == 0) {
+    f = warp_join(lane < kWarps ? sh->warp[lane] : nothing());
+    if (lane < size) {
+      uint32_t remote;
+      asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_u32(slots + rank)), "r"(lane));
+      asm volatile(
+          "st.shared::cluster.v2.u32 [%0], {%1, %2};\n\t"
+          "st.shared::cluster.v2.f32 [%0 + 8], {%3, %4};\n\t"
+          "st.shared::cluster.u32 [%0 + 16], %5;" ::"r"(remote),
+          "r"(f.score), "r"(f.token), "f"(f.x), "f"(f.sum), "r"(f.count)
+          : "memory");
+    }
+    __syncwarp();
+  }
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  ++pass;
+  return warp_join(lane < size ? slots[lane] : nothing());
+}
+
 __device__ __forceinline__ float to_float(float x) { return x; }
 __device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
 
 template <typename T, bool STAGED>
-__global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams p) {
+__global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleParams p) {
   constexpr int kPer16 = 16 / sizeof(T);
   extern __shared__ __align__(16) uint8_t stage_raw[];
   __shared__ Shared sh;
@@ -187,7 +215,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
                          smem_u32(stage + shift + head)),
                      "l"(logits + head), "r"(units * 16), "r"(smem_u32(&sh.full))
                      : "memory");
-      if (!greedy) {
+      if (!greedy && !(min_p > 0.f) && !(top_k > 0 && top_k <= kThreads)) {  // read whole below
         const uintptr_t lo = (reinterpret_cast<uintptr_t>(noise) + 15) & ~(uintptr_t)15;
         const uintptr_t hi = reinterpret_cast<uintptr_t>(noise + n) & ~(uintptr_t)15;
         if (hi > lo)
@@ -207,8 +235,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
     __syncthreads();
     if (!mbar_wait_limit(&sh.full, 0, &sh.abort_flag, p.err, kWaitLimitCycles)) mbar_wait_quiet(&sh.full, 0);
   }
-  // Group g holds tokens [g kGroup - shift, +kGroup) of the slice.
-  auto load = [&](int g, float (&x)[kGroup]) {
+  // Group g holds tokens [g kGroup - shift, +kGroup) of the slice, -inf outside it.
+  auto load_raw = [&](int g, float (&x)[kGroup]) {
     const int at = g * kGroup - shift;
     if constexpr (STAGED) {
       load_group(stage + g * kGroup, x);
@@ -218,87 +246,210 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
 #pragma unroll
       for (int e = 0; e < kGroup; ++e) x[e] = at + e >= 0 && at + e < n ? to_float(logits[at + e]) : -INFINITY;
     }
-#pragma unroll
-    for (int e = 0; e < kGroup; ++e) x[e] = usable(x[e]);
   };
 
-  // Maximum, and its lowest index.
   int pass = 0;
-  float mx = -INFINITY;
-  int mi = n;
-  for (int g = threadIdx.x; g < groups; g += kThreads) {
+  float m = -INFINITY;
+  // The larger of a and group g's logits.
+  auto raise = [&](float a, int g) -> float {
+    if constexpr (STAGED) return group_max(a, stage + g * kGroup);
     float x[kGroup];
-    load(g, x);
-#pragma unroll
-    for (int e = 0; e < kGroup; ++e)
-      if (x[e] > mx) mx = x[e], mi = g * kGroup - shift + e;
-  }
+    load_raw(g, x);
+    return group_max(a, x);
+  };
+  for (int g = threadIdx.x; g < groups; g += kThreads) m = raise(m, g);
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-  const unsigned bits = __float_as_uint(mx);
+  m = __fadd_rn(m, 0.f);  // -0 is +0: equal logits have equal bits in the join
+  const unsigned bits = __float_as_uint(m);
   const unsigned ordered = (bits & 0x80000000u) ? ~bits : bits | 0x80000000u;
-  Found f = cluster_join({((unsigned long long)ordered << 32) | (0xffffffffu - (unsigned)(begin + mi)), mx, 0.f, 0, 0},
-                         &sh, rank, size, pass);
-  const float m = f.x;
+  const float own_max = m;
+  m = cluster_join({ordered, kNone, m, 0.f, 0}, &sh, rank, size, pass).x;
+  const float top = m;
+  // The lowest index of the maximum, for a row that needs it.
+  auto first_maximum = [&]() -> int {
+    Found f = nothing();
+    for (int g = threadIdx.x; g < groups && f.score == 0; g += kThreads) {
+      float x[kGroup];
+      load_raw(g, x);
+#pragma unroll
+      for (int e = kGroup - 1; e >= 0; --e)
+        if (x[e] == top) f.score = 1, f.token = begin + g * kGroup - shift + e;
+    }
+    return (int)cluster_join(f, &sh, rank, size, pass).token;
+  };
   if (m == -INFINITY || greedy) {
-    if (rank == 0 && threadIdx.x == 0) p.out[r] = m == -INFINITY ? -1 : entry_index(f.best);
+    const int i = m == -INFINITY ? -1 : first_maximum();
+    if (rank == 0 && threadIdx.x == 0) p.out[r] = i;
     return;
   }
-
-  // The race over all tokens, and the total weight.
+  // A maximum of +inf: the tokens that have it weigh 1, all others 0.
+  const bool infinite = m == INFINITY;
+  if (infinite) m = 0.f;
+  auto load = [&](int g, float (&x)[kGroup]) {
+    load_raw(g, x);
+    if (infinite) {
+#pragma unroll
+      for (int e = 0; e < kGroup; ++e) x[e] = x[e] == INFINITY ? 0.f : -INFINITY;
+    }
+  };
   const Weight weight{m, temperature, __frcp_rn(temperature)};
-  const bool whole16 = (reinterpret_cast<uintptr_t>(noise - shift) & 15) == 0;
-  float best = -1.f, best_x = 0.f, total = 0.f;
-  int best_i = 0;
-  for (int g = threadIdx.x; g < groups; g += kThreads) {
-    const int at = g * kGroup - shift;
-    float x[kGroup], e[kGroup];
-    if (whole16 && at >= 0 && at + kGroup <= n) {
+  // A thread's candidate as the entry it joins with.
+  auto found = [&](const Candidate& c, float sum, int count) -> Found {
+    if (c.i < 0) return {0, kNone, 0.f, sum, count};
+    return {__float_as_uint(fmaxf(__fdividef(weight(c.x), __ldg(noise + c.i)), 0.f)), (uint32_t)(begin + c.i), c.x, sum,
+            count};
+  };
+
+  // Tokens below `cut` are not kept, whatever the race says: they weigh less
+  // than min_p (lowered a little for the logarithm's error), or top_k threads
+  // of this CTA alone have a logit of at least `cut`. The second bound is
+  // bisected on the threads' maxima, down to an eighth of T.
+  float cut = -INFINITY;
+  if (min_p > 0.f && !infinite) cut = m + temperature * (__logf(min_p) - 1e-4f) - 1e-6f * fabsf(m);
+  if (top_k > 0 && top_k <= kThreads && !infinite) {
+    float hi = m, lo = m - 32.f * temperature;
+    if (__syncthreads_count(own_max >= lo) >= top_k) {
+#pragma unroll 1
+      for (int i = 0; i < 8; ++i) {
+        const float mid = 0.5f * (lo + hi);
+        (__syncthreads_count(own_max >= mid) >= top_k ? lo : hi) = mid;
+      }
+      cut = fmaxf(cut, lo);
+    }
+  }
+
+  // A thread's tokens are taken in rounds of 64 (kMaskGroups groups, one bit
+  // each). A slice of one round keeps its mask of tokens that may still be
+  // kept, so passes after the first look only at those; a longer one looks at
+  // all of them again.
+  const int rounds = (groups + kThreads * kMaskGroups - 1) / (kThreads * kMaskGroups);
+  auto group_of = [&](int round, int k) { return (round * kMaskGroups + k) * kThreads + (int)threadIdx.x; };
+  auto logit = [&](int i) -> float {  // token i of the slice
+    float x;
+    if constexpr (STAGED)
+      x = to_float(stage[shift + i]);
+    else
+      x = to_float(logits[i]);
+    return infinite ? (x == INFINITY ? 0.f : -INFINITY) : x;
+  };
+  // Offers the tokens in `mask` of a round to the race, two at a time, and
+  // returns their weight.
+  auto race = [&](Candidate& c, int round, uint64_t mask) -> float {
+    float sum = 0.f;
+    while (mask) {
+      int at[2];
+      float e[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const float4 v = __ldg(reinterpret_cast<const float4*>(noise + at) + h);
-        e[4 * h] = v.x;
-        e[4 * h + 1] = v.y;
-        e[4 * h + 2] = v.z;
-        e[4 * h + 3] = v.w;
+        const int bit = __ffsll((long long)mask) - 1;
+        at[h] = bit < 0 ? -1 : group_of(round, bit / kGroup) * kGroup + bit % kGroup - shift;
+        mask &= mask - 1;
+        e[h] = at[h] >= 0 ? __ldg(noise + at[h]) : 1.f;
       }
-    } else {
 #pragma unroll
-      for (int i = 0; i < kGroup; ++i) e[i] = at + i >= 0 && at + i < n ? __ldg(noise + at + i) : 1.f;
+      for (int h = 0; h < 2; ++h)
+        if (at[h] >= 0) {
+          const float x = logit(at[h]), w = weight.quick(x);
+          sum += w;
+          c.offer(w, e[h], x, at[h]);
+        }
     }
-    load(g, x);
-#pragma unroll
-    for (int i = 0; i < kGroup; ++i) {
-      const float w = weight(x[i]);
-      const float ratio = __fdividef(w, e[i]);
-      total += w;
-      if (ratio > best && x[i] > -INFINITY) best = ratio, best_x = x[i], best_i = at + i;
-    }
-  }
-  f = cluster_join({best >= 0.f ? entry(best, begin + best_i) : 0, best_x, total, 0, 0}, &sh, rank, size, pass);
-  if (top_k > 0 || top_p < 1.f || min_p > 0.f) {
-    const float mass = top_p < 1.f ? top_p * f.sum : INFINITY;
-    while (true) {
-      const float xj = f.x;
-      const int j = entry_index(f.best);
-      Found a{0, 0.f, 0.f, 0, 0};
-      for (int g = threadIdx.x; g < groups; g += kThreads) {
-        const int at = g * kGroup - shift;
+    return sum;
+  };
+
+  // The race over all tokens that may be kept, and the total weight. Without
+  // a cut the noise is read whole; with one only for the tokens above it,
+  // asked for in L2 as they are found.
+  const bool whole16 = (reinterpret_cast<uintptr_t>(noise - shift) & 15) == 0;
+  Candidate c;
+  float total = 0.f;
+  uint64_t mask = ~0ull;
+  if (cut > -INFINITY) {
+    for (int round = 0; round < rounds; ++round) {
+      mask = 0;
+#pragma unroll 2
+      for (int k = 0; k < kMaskGroups; ++k) {
+        const int g = group_of(round, k), at = g * kGroup - shift;
+        if (g >= groups) break;
         float x[kGroup];
         load(g, x);
+        if (top_p < 1.f) {
 #pragma unroll
-        for (int i = 0; i < kGroup; ++i)
-          if (x[i] >= xj && (x[i] > xj || begin + at + i < j)) {
-            const float w = weight(x[i]);
-            a = join(a, {entry(__fdividef(w, __ldg(noise + at + i)), begin + at + i), x[i], w, 1, 0});
-          }
+          for (int i = 0; i < kGroup; ++i) total += weight.quick(x[i]);
+        }
+        if (group_max(-INFINITY, x) >= cut) {
+          unsigned bits = 0;
+#pragma unroll
+          for (int i = 0; i < kGroup; ++i) bits |= (x[i] >= cut ? 1u : 0u) << i;
+          mask |= (uint64_t)bits << (k * kGroup);
+          asm volatile("prefetch.global.L2 [%0];" ::"l"(noise + at + __ffs(bits) - 1));
+        }
       }
-      a = cluster_join(a, &sh, rank, size, pass);
-      const bool kept = (top_k <= 0 || a.count < top_k) && a.sum < mass && weight(xj) >= min_p;
-      if (kept || a.count == 0) break;
-      f = a;
+      race(c, round, mask);
+    }
+  } else {
+    for (int g = threadIdx.x; g < groups; g += kThreads) {
+      const int at = g * kGroup - shift;
+      float x[kGroup], e[kGroup];
+      if (whole16 && at >= 0 && at + kGroup <= n) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float4 v = __ldg(reinterpret_cast<const float4*>(noise + at) + h);
+          e[4 * h] = v.x;
+          e[4 * h + 1] = v.y;
+          e[4 * h + 2] = v.z;
+          e[4 * h + 3] = v.w;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < kGroup; ++i) e[i] = at + i >= 0 && at + i < n ? __ldg(noise + at + i) : 1.f;
+      }
+      load(g, x);
+#pragma unroll
+      for (int i = 0; i < kGroup; ++i) {
+        const float w = weight.quick(x[i]);
+        total += w;
+        c.offer(w, e[i], x[i], at + i);
+      }
     }
   }
-  if (rank == 0 && threadIdx.x == 0) p.out[r] = entry_index(f.best);
+  Found f = cluster_join(found(c, total, 0), &sh, rank, size, pass);
+  const float mass = top_p < 1.f ? top_p * f.sum : INFINITY;
+  while (f.score != 0 && (top_k > 0 || top_p < 1.f || weight(f.x) < min_p)) {
+    const float xj = f.x;
+    const int j = (int)f.token - begin;
+    c = Candidate{};
+    float sum = 0.f;
+    int count = 0;
+    for (int round = 0; round < rounds; ++round) {
+      uint64_t ahead = 0;
+#pragma unroll 1
+      for (int k = 0; k < kMaskGroups; ++k) {
+        const int g = group_of(round, k), at = g * kGroup - shift;
+        if (g >= groups) break;
+        if (rounds == 1 && !(mask >> (k * kGroup) & 0xffu)) continue;
+        if (infinite || raise(-INFINITY, g) >= xj) {
+          float x[kGroup];
+          load(g, x);
+          unsigned bits = 0;
+#pragma unroll
+          for (int i = 0; i < kGroup; ++i)
+            bits |= (x[i] > xj || (x[i] == xj && at + i < j) ? 1u : 0u) << i;
+          ahead |= (uint64_t)bits << (k * kGroup);
+        }
+      }
+      count += __popcll(ahead);
+      sum += race(c, round, ahead);
+      mask = ahead;
+    }
+    const Found a = cluster_join(found(c, sum, count), &sh, rank, size, pass);
+    const bool kept = (top_k <= 0 || a.count < top_k) && a.sum < mass && weight(xj) >= min_p;
+    if (kept || a.count == 0) break;
+    f = a;
+  }
+  // Without a candidate (min_p above 1, say) the first token is kept all the same.
+  const int token = f.score != 0 ? (int)f.token : first_maximum();
+  if (rank == 0 && threadIdx.x == 0) p.out[r] = token;
 }
 
 template <typename T, bool STAGED>
