@@ -3,6 +3,7 @@
 // per-device caches (driver entry point, error-word address, arch check).
 #include <cudaTypedefs.h>
 
+#include <atomic>
 #include <cmath>
 #include <cstdint>
 #include <mutex>
@@ -376,6 +377,18 @@ int* device_error_word() {
 }
 
 int api_prologue(int** err) { return prologue(err); }
+
+int api_sm_count() {
+  static std::atomic<int> count[kMaxDevices];
+  const int dev = current_device();
+  if (dev < 0) return 148;
+  int n = count[dev].load(std::memory_order_relaxed);
+  if (n == 0) {
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) return 148;
+    count[dev].store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
 
 int api_tensor_map(CUtensorMap* m, const void* base, int rank, const unsigned long long* dims,
                    const unsigned long long* byte_strides, const unsigned* box) {

@@ -13,6 +13,9 @@ namespace b2a {
 // the status to return.
 int api_prologue(int** err);
 
+// SMs of the current device (148 where it cannot be asked).
+int api_sm_count();
+
 // Tiled bf16 tensor map with 128-byte swizzle, out-of-range elements read as
 // zero. dims / box have `rank` entries (innermost first), byte_strides
 // rank - 1 (dimension i + 1). Returns B2A_OK or B2A_ERR_TMA.

@@ -116,7 +116,10 @@ int b2a_prefill_varlen(const void* q, const void* k, const void* v, const void* 
 
 size_t b2a_decode_paged_workspace_bytes(int B, int Hq, int Hkv, int D) {
   if (B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || Hq / Hkv > 16 || !head_dim_ok(D)) return 0;
-  return 256;
+  // Two partials per CTA of the split form: O [group, D] and (m, l) [group, 2].
+  const size_t parts = 2 * (size_t)b2a::decode_paged_max_ctas(D, b2a::api_sm_count());
+  return b2a::api_align256(parts * (Hq / Hkv) * D * sizeof(float)) +
+         b2a::api_align256(parts * (Hq / Hkv) * 2 * sizeof(float));
 }
 
 int b2a_decode_paged(const void* q, const void* k_pages, const void* v_pages, const int* block_table,
@@ -174,6 +177,10 @@ int b2a_decode_paged(const void* q, const void* k_pages, const void* v_pages, co
   p.group = Hq / Hkv;
   p.scale_log2 = scale * b2a::kApiLog2e;
   p.err = err;
+  p.n_ctas = b2a::decode_paged_max_ctas(D, b2a::api_sm_count());
+  p.part_o = static_cast<float*>(workspace);
+  p.part_ml = reinterpret_cast<float*>(static_cast<char*>(workspace) +
+                                       b2a::api_align256((size_t)2 * p.n_ctas * p.group * D * sizeof(float)));
   return status_of(b2a::launch_decode_paged(D, tk, tv, p, static_cast<cudaStream_t>(stream)));
 }
 

@@ -14,6 +14,15 @@
 // rounding and what the rounding left), so its relative error is 2^-16
 // instead of 2^-8; the extra MMAs hide behind the loads.
 //
+// Work is split evenly whatever the lengths: the tiles of all (sequence, KV
+// head) pairs, one after another, are cut into one equal stretch per resident
+// CTA, found on the device from the lengths. A CTA walks its stretch with its
+// ring running across pairs; a pair inside one stretch is finished there, a
+// pair cut between CTAs leaves partials (at most two per CTA, so the
+// workspace does not grow with the batch) that a second, dependent launch
+// joins. Caches of a few tiles (kWholeTiles) are not cut: one CTA per pair,
+// one launch.
+//
 // Slots of a page past the sequence's end may hold anything, NaN included:
 // their scores are replaced by -inf and their V rows by zeros in shared
 // memory before they are used.
@@ -92,7 +101,88 @@ __device__ __forceinline__ void store_output(const DecodePagedParams& p, int b, 
     static_cast<__nv_bfloat16*>(p.o)[oi] = __float2bfloat16_rn(v);
 }
 
-template <int D>
+// Keys of sequence b that a call attends: its length, cut to the table.
+__device__ __forceinline__ int keys_of(const DecodePagedParams& p, int b) {
+  const long long cap = (long long)p.table_width * p.page;
+  const int len = p.seqlens[b];
+  return len < 0 ? 0 : (len > cap ? (int)cap : len);
+}
+__device__ __forceinline__ int tiles_of(const DecodePagedParams& p, int b) { return (keys_of(p, b) + 63) / 64; }
+
+// All tiles of the call (all lanes get it). Warp-collective.
+__device__ __forceinline__ long long total_tiles(const DecodePagedParams& p) {
+  long long n = 0;
+  for (int b0 = 0; b0 < p.B; b0 += 32) {
+    const int b = b0 + (threadIdx.x & 31);
+    n += __reduce_add_sync(0xffffffffu, b < p.B ? tiles_of(p, b) : 0);
+  }
+  return n * p.Hkv;
+}
+
+// Tiles per CTA: an equal share, but no less than a few, so that the joining
+// of partials stays small beside the loads.
+constexpr int kMinShare = 4;
+__device__ __forceinline__ long long share_of(long long total, int n_ctas) {
+  const long long share = (total + n_ctas - 1) / n_ctas;
+  return share < kMinShare ? kMinShare : share;
+}
+
+// A stretch of the tiles, pair by pair.
+struct Walk {
+  long long left;  // tiles of the stretch not yet given out
+  int b, g;        // the pair
+  int t0, t1;      // its tiles in the stretch
+  int tiles, len;  // all its tiles, its keys
+  // Positioned at tile `from` of all; `left` tiles to go. Warp-collective.
+  __device__ __forceinline__ Walk(const DecodePagedParams& p, long long from, long long count) {
+    left = count;
+    b = p.B;
+    if (left <= 0) return;
+    const int lane = threadIdx.x & 31;
+    for (int b0 = 0; b0 < p.B; b0 += 32) {
+      const int n = b0 + lane < p.B ? tiles_of(p, b0 + lane) : 0;
+      int upto = n;  // inclusive sum over the lanes
+#pragma unroll
+      for (int off = 1; off < 32; off *= 2) {
+        const int y = __shfl_up_sync(0xffffffffu, upto, off);
+        if (lane >= off) upto += y;
+      }
+      const unsigned past = __ballot_sync(0xffffffffu, (long long)upto * p.Hkv > from);
+      if (past) {
+        const int src = __ffs(past) - 1;
+        const long long before = (long long)(__shfl_sync(0xffffffffu, upto, src) - __shfl_sync(0xffffffffu, n, src)) * p.Hkv;
+        b = b0 + src;
+        len = keys_of(p, b);
+        tiles = (len + 63) / 64;
+        const long long into = from - before;
+        g = (int)(into / tiles);
+        t0 = (int)(into % tiles);
+        break;
+      }
+      from -= (long long)__shfl_sync(0xffffffffu, upto, 31) * p.Hkv;
+    }
+    t1 = (int)min((long long)tiles, t0 + left);
+  }
+  __device__ __forceinline__ Walk(int b_, int g_, int len_)
+      : left((len_ + 63) / 64), b(b_), g(g_), t0(0), t1((len_ + 63) / 64), tiles((len_ + 63) / 64), len(len_) {}
+  __device__ __forceinline__ bool next(const DecodePagedParams& p) {
+    left -= t1 - t0;
+    if (left <= 0) return false;
+    t0 = 0;
+    if (++g == p.Hkv) {
+      g = 0;
+      do {
+        if (++b >= p.B) return false;
+        len = keys_of(p, b);
+        tiles = (len + 63) / 64;
+      } while (tiles == 0);
+    }
+    t1 = (int)min((long long)tiles, left);
+    return true;
+  }
+};
+
+template <int D, bool SPLIT>
 __global__ void __launch_bounds__(PagedCfg<D>::THREADS, PagedCfg<D>::CTAS_PER_SM)
     decode_paged_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                         const __grid_constant__ DecodePagedParams p) {
@@ -104,17 +194,26 @@ __global__ void __launch_bounds__(PagedCfg<D>::THREADS, PagedCfg<D>::CTAS_PER_SM
   volatile int* abort_flag = &bars->abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  const int b = blockIdx.x / p.Hkv, g = blockIdx.x % p.Hkv;
-  const long long cap = (long long)p.table_width * p.page;
-  int len = p.seqlens[b];
-  if (len < 0 || len > cap) {
-    if (threadIdx.x == 0 && g == 0 && p.err) atomicOr(p.err, kErrBadArgs);
-    len = len < 0 ? 0 : (int)cap;
+  if constexpr (SPLIT) grid_dep_launch();  // the joining kernel may take SM slots as they free up
+  if (p.err && blockIdx.x == 0)
+    for (int b = threadIdx.x; b < p.B; b += C::THREADS)
+      if (p.seqlens[b] < 0 || p.seqlens[b] > (long long)p.table_width * p.page) atomicOr(p.err, kErrBadArgs);
+  long long from = 0, count = 1;
+  if constexpr (SPLIT) {
+    const long long total = total_tiles(p), share = share_of(total, p.n_ctas);
+    from = blockIdx.x * share;
+    count = min(share, total - from);
+    if (count <= 0) return;
   }
-  const int n_tiles = (len + C::TK - 1) / C::TK;
-  if (n_tiles == 0) {
+  auto start = [&]() -> Walk {
+    if constexpr (SPLIT) return Walk(p, from, count);
+    const int b = blockIdx.x / p.Hkv;
+    return Walk(b, blockIdx.x % p.Hkv, keys_of(p, b));
+  };
+  Walk w = start();
+  if (!SPLIT && w.tiles == 0) {
     for (int e = threadIdx.x; e < p.group * D; e += C::THREADS)
-      store_output(p, b, g * p.group + e / D, e % D, 0.f);
+      store_output(p, w.b, w.g * p.group + e / D, e % D, 0.f);
     return;
   }
   if (threadIdx.x == 0) {
@@ -136,54 +235,39 @@ __global__ void __launch_bounds__(PagedCfg<D>::THREADS, PagedCfg<D>::CTAS_PER_SM
     const bool is_v = lane >= boxes;
     const bool mine = lane < 2 * boxes;
     const int box_bytes = br * D * 2;
-    auto page_of = [&](int i) -> int {  // page of this lane's box in tile i
-      const int key = i * C::TK + box * br;
-      if (!mine || key >= len) return -1;
-      const int id = p.block_table[b * p.table_ld + key / p.page];
-      if (id >= 0 && id < p.n_pages) return id;
-      if (p.err) atomicOr(p.err, kErrBadArgs);
-      return 0;
-    };
-    int next = page_of(0);
-    int issued = 0;
-    for (int i = 0; i < n_tiles; ++i) {
-      const int slot = i % C::STAGES;
-      const int id = next;
-      if (i + 1 < n_tiles) next = page_of(i + 1);
-      if (!__all_sync(0xffffffffu, mbar_wait(&bars->empty[slot], ((uint32_t)(i / C::STAGES) & 1u) ^ 1u, abort_flag,
-                                             p.err)))
-        break;
-      uint8_t* dst = smem + slot * C::STAGE_BYTES + (is_v ? C::TILE_BYTES : 0) + box * box_bytes;
-      const unsigned copies = __ballot_sync(0xffffffffu, id >= 0);
-      if (lane == 0) mbar_arrive_expect_tx(&bars->full[slot], __popc(copies) * box_bytes);
-      __syncwarp();
-      if (id >= 0)
-        tma_load_5d(dst, is_v ? &tm_v : &tm_k, &bars->full[slot], 0, (i * C::TK + box * br) % p.page, 0, g, id);
-      issued = i + 1;
-    }
+    int n = 0;  // tiles copied so far
+    do {
+      auto page_of = [&](int t) -> int {  // page of this lane's box in tile t
+        const int key = t * C::TK + box * br;
+        if (!mine || key >= w.len) return -1;
+        const int id = p.block_table[w.b * p.table_ld + key / p.page];
+        if (id >= 0 && id < p.n_pages) return id;
+        if (p.err) atomicOr(p.err, kErrBadArgs);
+        return 0;
+      };
+      int next = page_of(w.t0);
+      for (int t = w.t0; t < w.t1; ++t, ++n) {
+        const int slot = n % C::STAGES;
+        const int id = next;
+        if (t + 1 < w.t1) next = page_of(t + 1);
+        if (!__all_sync(0xffffffffu, mbar_wait(&bars->empty[slot], ((uint32_t)(n / C::STAGES) & 1u) ^ 1u, abort_flag,
+                                               p.err)))
+          break;
+        uint8_t* dst = smem + slot * C::STAGE_BYTES + (is_v ? C::TILE_BYTES : 0) + box * box_bytes;
+        const unsigned copies = __ballot_sync(0xffffffffu, id >= 0);
+        if (lane == 0) mbar_arrive_expect_tx(&bars->full[slot], __popc(copies) * box_bytes);
+        __syncwarp();
+        if (id >= 0)
+          tma_load_5d(dst, is_v ? &tm_v : &tm_k, &bars->full[slot], 0, (t * C::TK + box * br) % p.page, 0, w.g, id);
+      }
+    } while (!*abort_flag && w.next(p));
+    const int issued = n;
     if (*abort_flag && lane == 0)
       for (int i = max(0, issued - C::STAGES); i < issued; ++i)
         mbar_wait_quiet(&bars->full[i % C::STAGES], (uint32_t)(i / C::STAGES) & 1u);
   } else {
     // ------------------------------------------------------------ compute warps
     const int gr = lane >> 2, tq = lane & 3;
-    uint32_t qa[D / 16][4];
-    {
-      const bool v0 = gr < p.group, v1 = gr + 8 < p.group;
-      const __nv_bfloat16* q0 = p.q + b * p.q_sb + (long long)(g * p.group + gr) * p.q_sh;
-      const __nv_bfloat16* q1 = q0 + 8 * p.q_sh;
-#pragma unroll
-      for (int k = 0; k < D / 16; ++k) {
-        qa[k][0] = v0 ? *reinterpret_cast<const uint32_t*>(q0 + 16 * k + 2 * tq) : 0u;
-        qa[k][1] = v1 ? *reinterpret_cast<const uint32_t*>(q1 + 16 * k + 2 * tq) : 0u;
-        qa[k][2] = v0 ? *reinterpret_cast<const uint32_t*>(q0 + 16 * k + 2 * tq + 8) : 0u;
-        qa[k][3] = v1 ? *reinterpret_cast<const uint32_t*>(q1 + 16 * k + 2 * tq + 8) : 0u;
-      }
-    }
-    float acc[D / 8][4];
-#pragma unroll
-    for (int n = 0; n < D / 8; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
-    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
     const float sl2 = p.scale_log2;
     const int mi = lane >> 3, mr = lane & 7;  // ldmatrix: matrix index / row in it
     // This warp's 16 keys of a tile lie in one box: its first row there, and
@@ -195,145 +279,273 @@ __global__ void __launch_bounds__(PagedCfg<D>::THREADS, PagedCfg<D>::CTAS_PER_SM
     auto at = [&](uint32_t base, int r, int U) -> uint32_t {
       return base + (U >> 3) * chunk + r * 128 + (((U & 7) ^ (r & 7)) << 4);
     };
-    bool ok = true;
-    for (int i = 0; i < n_tiles; ++i) {
-      const int slot = i % C::STAGES;
-      if (!__all_sync(0xffffffffu,
-                      mbar_wait(&bars->full[slot], (uint32_t)(i / C::STAGES) & 1u, abort_flag, p.err))) {
-        ok = false;
-        break;
+    // A wait that ran out leaves garbage in the result and the error word set;
+    // the warps still meet at every barrier below.
+    bool first = true;
+    int n = 0;  // tiles taken so far
+    do {
+      const int n_last = n + (w.t1 - w.t0) - 1;  // the pair's last one here
+      uint32_t qa[D / 16][4];
+      {
+        const bool v0 = gr < p.group, v1 = gr + 8 < p.group;
+        const __nv_bfloat16* q0 = p.q + w.b * p.q_sb + (long long)(w.g * p.group + gr) * p.q_sh;
+        const __nv_bfloat16* q1 = q0 + 8 * p.q_sh;
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          qa[k][0] = v0 ? *reinterpret_cast<const uint32_t*>(q0 + 16 * k + 2 * tq) : 0u;
+          qa[k][1] = v1 ? *reinterpret_cast<const uint32_t*>(q1 + 16 * k + 2 * tq) : 0u;
+          qa[k][2] = v0 ? *reinterpret_cast<const uint32_t*>(q0 + 16 * k + 2 * tq + 8) : 0u;
+          qa[k][3] = v1 ? *reinterpret_cast<const uint32_t*>(q1 + 16 * k + 2 * tq + 8) : 0u;
+        }
       }
-      const uint32_t kbase = smem_u32(smem + slot * C::STAGE_BYTES) + wbase;
-      const uint32_t vbase = kbase + C::TILE_BYTES;
-      const int have = len - (i * C::TK + 16 * warp);  // keys of this warp's 16 that exist
-      if (have > 0) {
-        float s[2][4];
+      float acc[D / 8][4];
 #pragma unroll
-        for (int ng = 0; ng < 2; ++ng) {
-          s[ng][0] = s[ng][1] = s[ng][2] = s[ng][3] = 0.f;
+      for (int d = 0; d < D / 8; ++d) acc[d][0] = acc[d][1] = acc[d][2] = acc[d][3] = 0.f;
+      float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+      for (int t = w.t0; t < w.t1; ++t, ++n) {
+        const int slot = n % C::STAGES;
+        if (!__all_sync(0xffffffffu,
+                        mbar_wait(&bars->full[slot], (uint32_t)(n / C::STAGES) & 1u, abort_flag, p.err))) {
+          n = n_last + 1;
+          break;
+        }
+        const uint32_t kbase = smem_u32(smem + slot * C::STAGE_BYTES) + wbase;
+        const uint32_t vbase = kbase + C::TILE_BYTES;
+        const int have = w.len - (t * C::TK + 16 * warp);  // keys of this warp's 16 that exist
+        if (have > 0) {
+          float s[2][4];
 #pragma unroll
-          for (int kp = 0; kp < D / 32; ++kp) {
+          for (int ng = 0; ng < 2; ++ng) {
+            s[ng][0] = s[ng][1] = s[ng][2] = s[ng][3] = 0.f;
+#pragma unroll
+            for (int kp = 0; kp < D / 32; ++kp) {
+              uint32_t b0, b1, b2, b3;
+              ldsm4(at(kbase, 8 * ng + mr, 4 * kp + mi), b0, b1, b2, b3);
+              mma16816(s[ng], qa[2 * kp], b0, b1);
+              mma16816(s[ng], qa[2 * kp + 1], b2, b3);
+            }
+          }
+          if (have < 16) {
+#pragma unroll
+            for (int ng = 0; ng < 2; ++ng)
+#pragma unroll
+              for (int e = 0; e < 2; ++e)
+                if (8 * ng + 2 * tq + e >= have) s[ng][e] = s[ng][2 + e] = -INFINITY;
+            // V rows without a key: 0 x anything would not do (NaN).
+            for (int u = lane; u < (16 - have) * (D / 8); u += 32)
+              st_shared_v4(at(vbase, have + u / (D / 8), u % (D / 8)), 0u, 0u, 0u, 0u);
+            fence_proxy_async_smem();  // before the slot's next copy
+            __syncwarp();
+          }
+          float mx0 = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]));
+          float mx1 = fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3]));
+          mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 1));
+          mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 2));
+          mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 1));
+          mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 2));
+          const float mn0 = fmaxf(m0, mx0 * sl2), mn1 = fmaxf(m1, mx1 * sl2);
+          const float u0 = (mn0 == -INFINITY) ? 0.f : mn0, u1 = (mn1 == -INFINITY) ? 0.f : mn1;
+          const float a0 = ex2(m0 - u0), a1 = ex2(m1 - u1);
+          m0 = mn0;
+          m1 = mn1;
+          float pr[2][4];
+#pragma unroll
+          for (int ng = 0; ng < 2; ++ng) {
+            pr[ng][0] = ex2(fmaf(s[ng][0], sl2, -u0));
+            pr[ng][1] = ex2(fmaf(s[ng][1], sl2, -u0));
+            pr[ng][2] = ex2(fmaf(s[ng][2], sl2, -u1));
+            pr[ng][3] = ex2(fmaf(s[ng][3], sl2, -u1));
+          }
+          l0 = l0 * a0 + pr[0][0] + pr[0][1] + pr[1][0] + pr[1][1];
+          l1 = l1 * a1 + pr[0][2] + pr[0][3] + pr[1][2] + pr[1][3];
+#pragma unroll
+          for (int n = 0; n < D / 8; ++n) {
+            acc[n][0] *= a0;
+            acc[n][1] *= a0;
+            acc[n][2] *= a1;
+            acc[n][3] *= a1;
+          }
+          // P = high + low, each bf16.
+          uint32_t ph[4], pl[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float x = pr[e >> 1][2 * (e & 1)], y = pr[e >> 1][2 * (e & 1) + 1];
+            ph[e] = pack_bf16x2(x, y);
+            pl[e] = pack_bf16x2(x - __uint_as_float(ph[e] << 16), y - __uint_as_float(ph[e] & 0xffff0000u));
+          }
+          const int vr = 8 * (mi & 1) + mr;
+#pragma unroll
+          for (int dn = 0; dn < D / 8; dn += 2) {
             uint32_t b0, b1, b2, b3;
-            ldsm4(at(kbase, 8 * ng + mr, 4 * kp + mi), b0, b1, b2, b3);
-            mma16816(s[ng], qa[2 * kp], b0, b1);
-            mma16816(s[ng], qa[2 * kp + 1], b2, b3);
+            ldsm4_t(at(vbase, vr, dn + (mi >> 1)), b0, b1, b2, b3);
+            mma16816(acc[dn], ph, b0, b1);
+            mma16816(acc[dn + 1], ph, b2, b3);
+            mma16816(acc[dn], pl, b0, b1);
+            mma16816(acc[dn + 1], pl, b2, b3);
           }
         }
-        if (have < 16) {
-#pragma unroll
-          for (int ng = 0; ng < 2; ++ng)
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-              if (8 * ng + 2 * tq + e >= have) s[ng][e] = s[ng][2 + e] = -INFINITY;
-          // V rows without a key: 0 x anything would not do (NaN).
-          for (int u = lane; u < (16 - have) * (D / 8); u += 32)
-            st_shared_v4(at(vbase, have + u / (D / 8), u % (D / 8)), 0u, 0u, 0u, 0u);
-          __syncwarp();
-        }
-        float mx0 = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]));
-        float mx1 = fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3]));
-        mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 1));
-        mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 2));
-        mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 1));
-        mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 2));
-        const float mn0 = fmaxf(m0, mx0 * sl2), mn1 = fmaxf(m1, mx1 * sl2);
-        const float u0 = (mn0 == -INFINITY) ? 0.f : mn0, u1 = (mn1 == -INFINITY) ? 0.f : mn1;
-        const float a0 = ex2(m0 - u0), a1 = ex2(m1 - u1);
-        m0 = mn0;
-        m1 = mn1;
-        float pr[2][4];
-#pragma unroll
-        for (int ng = 0; ng < 2; ++ng) {
-          pr[ng][0] = ex2(fmaf(s[ng][0], sl2, -u0));
-          pr[ng][1] = ex2(fmaf(s[ng][1], sl2, -u0));
-          pr[ng][2] = ex2(fmaf(s[ng][2], sl2, -u1));
-          pr[ng][3] = ex2(fmaf(s[ng][3], sl2, -u1));
-        }
-        l0 = l0 * a0 + pr[0][0] + pr[0][1] + pr[1][0] + pr[1][1];
-        l1 = l1 * a1 + pr[0][2] + pr[0][3] + pr[1][2] + pr[1][3];
-#pragma unroll
-        for (int n = 0; n < D / 8; ++n) {
-          acc[n][0] *= a0;
-          acc[n][1] *= a0;
-          acc[n][2] *= a1;
-          acc[n][3] *= a1;
-        }
-        // P = high + low, each bf16.
-        uint32_t ph[4], pl[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float x = pr[e >> 1][2 * (e & 1)], y = pr[e >> 1][2 * (e & 1) + 1];
-          ph[e] = pack_bf16x2(x, y);
-          pl[e] = pack_bf16x2(x - __uint_as_float(ph[e] << 16), y - __uint_as_float(ph[e] & 0xffff0000u));
-        }
-        const int vr = 8 * (mi & 1) + mr;
-#pragma unroll
-        for (int dn = 0; dn < D / 8; dn += 2) {
-          uint32_t b0, b1, b2, b3;
-          ldsm4_t(at(vbase, vr, dn + (mi >> 1)), b0, b1, b2, b3);
-          mma16816(acc[dn], ph, b0, b1);
-          mma16816(acc[dn + 1], ph, b2, b3);
-          mma16816(acc[dn], pl, b0, b1);
-          mma16816(acc[dn + 1], pl, b2, b3);
-        }
+        __syncwarp();
+        if (lane == 0 && n < n_last) mbar_arrive(&bars->empty[slot]);
       }
-      __syncwarp();
-      if (lane == 0 && i + 1 < n_tiles) mbar_arrive(&bars->empty[slot]);
-    }
-    // Merge the four warps' (m, l, O) in the last tile's stage, once all of
-    // them have read it.
-    if (ok) {
+      // Merge the four warps' (m, l, O) in the last tile's stage, once all of
+      // them have read it; the stage is released after that.
       l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
       l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
       l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
       l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
-    }
-    asm volatile("bar.sync 1, 128;" ::: "memory");
-    float* so = reinterpret_cast<float*>(smem + ((n_tiles - 1) % C::STAGES) * C::STAGE_BYTES);  // [4][16][D]
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      const int slot = n_last % C::STAGES;
+      float* so = reinterpret_cast<float*>(smem + slot * C::STAGE_BYTES);  // [4][16][D]
 #pragma unroll
-    for (int n = 0; n < D / 8; ++n) {
-      float* r0 = so + (warp * 16 + gr) * D + 8 * n + 2 * tq;
-      *reinterpret_cast<float2*>(r0) = make_float2(acc[n][0], acc[n][1]);
-      *reinterpret_cast<float2*>(r0 + 8 * D) = make_float2(acc[n][2], acc[n][3]);
-    }
-    if (tq == 0) {
-      bars->m[warp][gr] = m0;
-      bars->m[warp][gr + 8] = m1;
-      bars->l[warp][gr] = l0;
-      bars->l[warp][gr + 8] = l1;
-    }
-    asm volatile("bar.sync 1, 128;" ::: "memory");
-    for (int e = threadIdx.x; e < p.group * D; e += 128) {
-      const int r = e / D, d = e % D;
-      float M = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < 4; ++w) M = fmaxf(M, bars->m[w][r]);
-      const float Mu = (M == -INFINITY) ? 0.f : M;
-      float lsum = 0.f, osum = 0.f;
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const float f = ex2(bars->m[w][r] - Mu);
-        lsum += f * bars->l[w][r];
-        osum += f * so[(w * 16 + r) * D + d];
+      for (int d = 0; d < D / 8; ++d) {
+        float* r0 = so + (warp * 16 + gr) * D + 8 * d + 2 * tq;
+        if (gr < p.group) *reinterpret_cast<float2*>(r0) = make_float2(acc[d][0], acc[d][1]);
+        if (gr + 8 < p.group) *reinterpret_cast<float2*>(r0 + 8 * D) = make_float2(acc[d][2], acc[d][3]);
       }
-      store_output(p, b, g * p.group + r, d, lsum == 0.f ? 0.f : osum / lsum);
-    }
+      if (tq == 0) {
+        bars->m[warp][gr] = m0;
+        bars->m[warp][gr + 8] = m1;
+        bars->l[warp][gr] = l0;
+        bars->l[warp][gr + 8] = l1;
+      }
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      const bool whole = w.t0 == 0 && w.t1 == w.tiles;
+      const long long part = (2LL * blockIdx.x + (first ? 0 : 1)) * p.group;
+      for (int e = threadIdx.x; e < p.group * D; e += 128) {
+        const int r = e / D, d = e % D;
+        float M = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) M = fmaxf(M, bars->m[u][r]);
+        const float Mu = (M == -INFINITY) ? 0.f : M;
+        float lsum = 0.f, osum = 0.f;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          // A warp without keys here has nothing in the sum (its m is -inf).
+          const float f = ex2(bars->m[u][r] - Mu);
+          lsum += f * bars->l[u][r];
+          osum += f * so[(u * 16 + r) * D + d];
+        }
+        if (!SPLIT || whole) {
+          store_output(p, w.b, w.g * p.group + r, d, lsum == 0.f ? 0.f : osum / lsum);
+        } else {
+          p.part_o[(part + r) * D + d] = osum;
+          if (d == 0) {
+            p.part_ml[2 * (part + r)] = M;
+            p.part_ml[2 * (part + r) + 1] = lsum;
+          }
+        }
+      }
+      fence_proxy_async_smem();
+      asm volatile("bar.sync 1, 128;" ::: "memory");  // everyone has read the stage, m and l
+      if (lane == 0) mbar_arrive(&bars->empty[slot]);
+      first = false;
+    } while (w.next(p));
   }
+}
+
+// Joins the partials of (sequence, query head) blockIdx.x, if its keys were
+// cut between CTAs; a sequence without keys gets its zeros here. The parts
+// are the CTAs from the one with the pair's first tile to the one with its
+// last, each with the pair as its first or, in the first of them, as its
+// last. Warps take parts in turn and are joined in a fixed order.
+template <int D>
+__global__ void __launch_bounds__(128) decode_paged_join_kernel(const __grid_constant__ DecodePagedParams p) {
+  constexpr int PER = D / 32;  // columns of a lane
+  __shared__ float s_o[4][D], s_m[4], s_l[4];
+  grid_dep_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int b = blockIdx.x / p.Hq, h = blockIdx.x % p.Hq;
+  const int g = h / p.group, r = h % p.group;
+  long long total = 0, before = 0;  // tiles of all sequences, and of those before b
+  for (int b0 = 0; b0 < p.B; b0 += 32) {
+    const int n = b0 + lane < p.B ? tiles_of(p, b0 + lane) : 0;
+    total += __reduce_add_sync(0xffffffffu, n);
+    before += __reduce_add_sync(0xffffffffu, b0 + lane < b ? n : 0);
+  }
+  const int tiles = tiles_of(p, b);
+  const long long share = share_of(total * p.Hkv, p.n_ctas);
+  const long long lo = before * p.Hkv + (long long)g * tiles;
+  if (tiles == 0) {
+    for (int d = threadIdx.x; d < D; d += 128) store_output(p, b, h, d, 0.f);
+    return;
+  }
+  const long long c0 = lo / share, c1 = (lo + tiles - 1) / share;
+  if (c0 == c1) return;  // finished by its CTA
+  float m = -INFINITY, l = 0.f, o[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) o[i] = 0.f;
+  for (long long c = c0 + warp; c <= c1; c += 4) {
+    const long long part = (2 * c + (c == c0 && c * share < lo ? 1 : 0)) * p.group + r;
+    const float pm = p.part_ml[2 * part], pl = p.part_ml[2 * part + 1];
+    const float mn = fmaxf(m, pm), mu = mn == -INFINITY ? 0.f : mn;
+    const float fo = ex2(m - mu), fp = ex2(pm - mu);
+    m = mn;
+    l = l * fo + pl * fp;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) o[i] = o[i] * fo + p.part_o[part * D + i * 32 + lane] * fp;
+  }
+#pragma unroll
+  for (int i = 0; i < PER; ++i) s_o[warp][i * 32 + lane] = o[i];
+  if (lane == 0) {
+    s_m[warp] = m;
+    s_l[warp] = l;
+  }
+  __syncthreads();
+  float M = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
+  const float Mu = M == -INFINITY ? 0.f : M;
+  for (int d = threadIdx.x; d < D; d += 128) {
+    float lsum = 0.f, osum = 0.f;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const float f = ex2(s_m[u] - Mu);
+      lsum += f * s_l[u];
+      osum += f * s_o[u][d];
+    }
+    store_output(p, b, h, d, lsum == 0.f ? 0.f : osum / lsum);
+  }
+}
+
+constexpr int kWholeTiles = 8;
+
+template <int D, bool SPLIT>
+int launch_main(const CUtensorMap& tk, const CUtensorMap& tv, const DecodePagedParams& p, long long n,
+                cudaStream_t st) {
+  using C = PagedCfg<D>;
+  if (cudaFuncSetAttribute(decode_paged_kernel<D, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           C::SMEM_BYTES) != cudaSuccess)
+    return -1;
+  if (n > 0x7fffffffLL) return -2;
+  decode_paged_kernel<D, SPLIT><<<(unsigned)n, C::THREADS, C::SMEM_BYTES, st>>>(tk, tv, p);
+  return cudaGetLastError() == cudaSuccess ? 0 : -1;
 }
 
 template <int D>
 int launch_t(const CUtensorMap& tk, const CUtensorMap& tv, const DecodePagedParams& p, cudaStream_t st) {
-  using C = PagedCfg<D>;
-  if (cudaFuncSetAttribute(decode_paged_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES) !=
-      cudaSuccess)
-    return -1;
-  const long long n = (long long)p.B * p.Hkv;
-  if (n > 0x7fffffffLL) return -2;
-  decode_paged_kernel<D><<<(unsigned)n, C::THREADS, C::SMEM_BYTES, st>>>(tk, tv, p);
+  if (!decode_paged_splits(p.table_width, p.page)) return launch_main<D, false>(tk, tv, p, (long long)p.B * p.Hkv, st);
+  const long long heads = (long long)p.B * p.Hq;
+  if (heads > 0x7fffffffLL) return -2;
+  const int rc = launch_main<D, true>(tk, tv, p, p.n_ctas, st);
+  if (rc) return rc;
+  // The joining kernel is scheduled while the main one drains and waits for
+  // all of it before it reads anything.
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)heads);
+  cfg.blockDim = dim3(128);
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, decode_paged_join_kernel<D>, p) != cudaSuccess) return -1;
   return cudaGetLastError() == cudaSuccess ? 0 : -1;
 }
 
 }  // namespace
+
+bool decode_paged_splits(int table_width, int page) { return (long long)table_width * page > 64LL * kWholeTiles; }
+
+int decode_paged_max_ctas(int D, int sms) { return sms * (D == 256 ? 1 : 2); }
 
 int launch_decode_paged(int D, const CUtensorMap& tk, const CUtensorMap& tv, const DecodePagedParams& p,
                         cudaStream_t st) {

@@ -22,8 +22,18 @@ struct DecodePagedParams {
   int gate_bf16;
   int B, Hq, Hkv, group;
   float scale_log2;
+  // Split form: partial results of each CTA's first and last (sequence, KV
+  // head), 2 per CTA: O [group, D] before its division and (m, l) [group, 2].
+  float* part_o;
+  float* part_ml;
+  int n_ctas;
   int* err;
 };
+
+// Whether a call runs the split form (partials and a joining kernel), the
+// CTAs it may use for the current device, and its workspace.
+bool decode_paged_splits(int table_width, int page);
+int decode_paged_max_ctas(int D, int sms);
 
 // tk / tv: 5-D maps (64 columns, slot in the page, D / 64, head, page) with
 // box (64, box_rows, D / 64, 1, 1). Returns 0 on success, -3 for an
