@@ -135,8 +135,8 @@ int b2a_decode_paged(const void* q, const void* k_pages, const void* v_pages, co
   if (!(scale > 0.f) || !std::isfinite(scale)) return B2A_ERR_INVALID_ARG;
   if (!head_dim_ok(D)) return B2A_ERR_HEAD_DIM;
   if (Hq % Hkv || Hq / Hkv > 16) return B2A_ERR_GQA;
-  if (!api_aligned(q, 16) || !api_aligned(k_pages, 16) || !api_aligned(v_pages, 16) || !api_aligned(o, out_fp32 ? 4 : 2) ||
-      !api_aligned(block_table, 4) || !api_aligned(seqlens, 4) || !api_aligned(gate, gate_bf16 ? 2 : 4))
+  if (!api_aligned(q, 16) || !api_aligned(k_pages, 16) || !api_aligned(v_pages, 16) ||
+      !api_aligned(o, out_fp32 ? 4 : 2) || !api_aligned(block_table, 4) || !api_aligned(seqlens, 4) || !api_aligned(gate, gate_bf16 ? 2 : 4))
     return B2A_ERR_ALIGNMENT;
   if (!api_strides_ok(qs, 2, 8) || !api_strides_ok(ks, 3, 8) || !api_strides_ok(vs, 3, 8)) return B2A_ERR_ALIGNMENT;
   const size_t need = b2a_decode_paged_workspace_bytes(B, Hq, Hkv, D);
@@ -171,6 +171,10 @@ int b2a_decode_paged(const void* q, const void* k_pages, const void* v_pages, co
     p.g_sh = gs[1];
     p.gate_bf16 = gate_bf16 ? 1 : 0;
   }
+  auto by4 = [](const void* ptr, const long long* st, unsigned size) {
+    return api_aligned(ptr, 4 * size) && st[0] % 4 == 0 && st[1] % 4 == 0;
+  };
+  p.vec4 = by4(o, os, out_fp32 ? 4 : 2) && (!gate || by4(gate, gs, gate_bf16 ? 2 : 4));
   p.B = B;
   p.Hq = Hq;
   p.Hkv = Hkv;

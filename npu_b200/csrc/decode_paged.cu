@@ -85,20 +85,55 @@ __device__ __forceinline__ void tma_load_5d(void* smem_dst, const CUtensorMap* m
       : "memory");
 }
 
-// The output of (sequence b, query head h), column d: attention value v,
-// gated and rounded as the call asks.
-__device__ __forceinline__ void store_output(const DecodePagedParams& p, int b, int h, int d, float v) {
-  if (p.gate) {
-    const long long gi = b * p.g_sb + h * p.g_sh + d;
-    const float g = p.gate_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p.gate)[gi])
-                                : static_cast<const float*>(p.gate)[gi];
-    v *= __fdividef(1.f, 1.f + __expf(-g));
+// The gate of (sequence b, query head h) at columns d .. d + 3.
+__device__ __forceinline__ float4 load_gate(const DecodePagedParams& p, int b, int h, int d) {
+  const long long i = b * p.g_sb + h * p.g_sh + d;
+  if (p.gate_bf16) {
+    const __nv_bfloat16* g = static_cast<const __nv_bfloat16*>(p.gate) + i;
+    if (p.vec4) {
+      const uint2 v = *reinterpret_cast<const uint2*>(g);
+      return make_float4(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16),
+                         __uint_as_float(v.y & 0xffff0000u));
+    }
+    return make_float4(__bfloat162float(g[0]), __bfloat162float(g[1]), __bfloat162float(g[2]), __bfloat162float(g[3]));
   }
-  const long long oi = b * p.o_sb + h * p.o_sh + d;
-  if (p.out_fp32)
-    static_cast<float*>(p.o)[oi] = v;
-  else
-    static_cast<__nv_bfloat16*>(p.o)[oi] = __float2bfloat16_rn(v);
+  const float* g = static_cast<const float*>(p.gate) + i;
+  if (p.vec4) return *reinterpret_cast<const float4*>(g);
+  return make_float4(g[0], g[1], g[2], g[3]);
+}
+
+__device__ __forceinline__ float sigmoid(float g) { return __fdividef(1.f, 1.f + __expf(-g)); }
+
+// The output at columns d .. d + 3: attention values v, gated and rounded as
+// the call asks.
+__device__ __forceinline__ void store_output(const DecodePagedParams& p, int b, int h, int d, float4 v, float4 gate) {
+  if (p.gate)
+    v = make_float4(v.x * sigmoid(gate.x), v.y * sigmoid(gate.y), v.z * sigmoid(gate.z), v.w * sigmoid(gate.w));
+  const long long i = b * p.o_sb + h * p.o_sh + d;
+  if (p.out_fp32) {
+    float* o = static_cast<float*>(p.o) + i;
+    if (p.vec4)
+      *reinterpret_cast<float4*>(o) = v;
+    else
+      o[0] = v.x, o[1] = v.y, o[2] = v.z, o[3] = v.w;
+  } else {
+    __nv_bfloat16* o = static_cast<__nv_bfloat16*>(p.o) + i;
+    if (p.vec4) {
+      *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
+    } else {
+      o[0] = __float2bfloat16_rn(v.x), o[1] = __float2bfloat16_rn(v.y);
+      o[2] = __float2bfloat16_rn(v.z), o[3] = __float2bfloat16_rn(v.w);
+    }
+  }
+}
+
+__device__ __forceinline__ float4 axpy(float a, float4 x, float4 y) {
+  return make_float4(fmaf(a, x.x, y.x), fmaf(a, x.y, y.y), fmaf(a, x.z, y.z), fmaf(a, x.w, y.w));
+}
+__device__ __forceinline__ float4 over(float4 x, float l) {
+  const float f = l == 0.f ? 0.f : 1.f;  // a row without keys gives 0, NaN stays NaN
+  const float d = l == 0.f ? 1.f : l;
+  return make_float4(f * (x.x / d), f * (x.y / d), f * (x.z / d), f * (x.w / d));
 }
 
 // Keys of sequence b that a call attends: its length, cut to the table.
@@ -150,7 +185,7 @@ struct Walk {
       const unsigned past = __ballot_sync(0xffffffffu, (long long)upto * p.Hkv > from);
       if (past) {
         const int src = __ffs(past) - 1;
-        const long long before = (long long)(__shfl_sync(0xffffffffu, upto, src) - __shfl_sync(0xffffffffu, n, src)) * p.Hkv;
+        const long long before = (long long)__shfl_sync(0xffffffffu, upto - n, src) * p.Hkv;
         b = b0 + src;
         len = keys_of(p, b);
         tiles = (len + 63) / 64;
@@ -212,8 +247,9 @@ __global__ void __launch_bounds__(PagedCfg<D>::THREADS, PagedCfg<D>::CTAS_PER_SM
   };
   Walk w = start();
   if (!SPLIT && w.tiles == 0) {
-    for (int e = threadIdx.x; e < p.group * D; e += C::THREADS)
-      store_output(p, w.b, w.g * p.group + e / D, e % D, 0.f);
+    const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int e = 4 * threadIdx.x; e < p.group * D; e += 4 * C::THREADS)
+      store_output(p, w.b, w.g * p.group + e / D, e % D, zero, zero);
     return;
   }
   if (threadIdx.x == 0) {
@@ -408,31 +444,43 @@ __global__ void __launch_bounds__(PagedCfg<D>::THREADS, PagedCfg<D>::CTAS_PER_SM
         bars->l[warp][gr] = l0;
         bars->l[warp][gr + 8] = l1;
       }
-      asm volatile("bar.sync 1, 128;" ::: "memory");
-      const bool whole = w.t0 == 0 && w.t1 == w.tiles;
+      const bool whole = !SPLIT || (w.t0 == 0 && w.t1 == w.tiles);
       const long long part = (2LL * blockIdx.x + (first ? 0 : 1)) * p.group;
-      for (int e = threadIdx.x; e < p.group * D; e += 128) {
+      // Thread x takes columns 4 x .. of the group's rows, 512 apart; the
+      // gates are requested together, ahead of the barrier.
+      constexpr int STEPS = 16 * D / 512;
+      float4 gate[STEPS];
+      if (p.gate && whole) {
+#pragma unroll
+        for (int i = 0; i < STEPS; ++i) {
+          const int e = 4 * threadIdx.x + 512 * i;
+          if (e < p.group * D) gate[i] = load_gate(p, w.b, w.g * p.group + e / D, e % D);
+        }
+      }
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+#pragma unroll
+      for (int i = 0; i < STEPS; ++i) {
+        const int e = 4 * threadIdx.x + 512 * i;
+        if (e >= p.group * D) break;
         const int r = e / D, d = e % D;
         float M = -INFINITY;
 #pragma unroll
         for (int u = 0; u < 4; ++u) M = fmaxf(M, bars->m[u][r]);
         const float Mu = (M == -INFINITY) ? 0.f : M;
-        float lsum = 0.f, osum = 0.f;
+        float lsum = 0.f;
+        float4 osum = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
           // A warp without keys here has nothing in the sum (its m is -inf).
           const float f = ex2(bars->m[u][r] - Mu);
           lsum += f * bars->l[u][r];
-          osum += f * so[(u * 16 + r) * D + d];
+          osum = axpy(f, *reinterpret_cast<const float4*>(so + (u * 16 + r) * D + d), osum);
         }
-        if (!SPLIT || whole) {
-          store_output(p, w.b, w.g * p.group + r, d, lsum == 0.f ? 0.f : osum / lsum);
+        if (whole) {
+          store_output(p, w.b, w.g * p.group + r, d, over(osum, lsum), gate[i]);
         } else {
-          p.part_o[(part + r) * D + d] = osum;
-          if (d == 0) {
-            p.part_ml[2 * (part + r)] = M;
-            p.part_ml[2 * (part + r) + 1] = lsum;
-          }
+          *reinterpret_cast<float4*>(p.part_o + (part + r) * D + d) = osum;
+          if (d == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * (part + r)) = make_float2(M, lsum);
         }
       }
       fence_proxy_async_smem();
@@ -447,13 +495,15 @@ __global__ void __launch_bounds__(PagedCfg<D>::THREADS, PagedCfg<D>::CTAS_PER_SM
 // cut between CTAs; a sequence without keys gets its zeros here. The parts
 // are the CTAs from the one with the pair's first tile to the one with its
 // last, each with the pair as its first or, in the first of them, as its
-// last. Warps take parts in turn and are joined in a fixed order.
+// last. D / 4 threads read one part's row; the parts are dealt to such teams
+// in turn and joined in a fixed order. The lengths are read before the wait
+// for the main kernel (which does not write them).
 template <int D>
 __global__ void __launch_bounds__(128) decode_paged_join_kernel(const __grid_constant__ DecodePagedParams p) {
-  constexpr int PER = D / 32;  // columns of a lane
-  __shared__ float s_o[4][D], s_m[4], s_l[4];
-  grid_dep_wait();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int TEAM = D / 4, TEAMS = 128 / TEAM;
+  __shared__ float4 s_o[TEAMS][TEAM];
+  __shared__ float s_m[TEAMS], s_l[TEAMS];
+  const int lane = threadIdx.x & 31;
   const int b = blockIdx.x / p.Hq, h = blockIdx.x % p.Hq;
   const int g = h / p.group, r = h % p.group;
   long long total = 0, before = 0;  // tiles of all sequences, and of those before b
@@ -465,44 +515,58 @@ __global__ void __launch_bounds__(128) decode_paged_join_kernel(const __grid_con
   const int tiles = tiles_of(p, b);
   const long long share = share_of(total * p.Hkv, p.n_ctas);
   const long long lo = before * p.Hkv + (long long)g * tiles;
+  const int team = threadIdx.x / TEAM, d = 4 * (threadIdx.x % TEAM);
+  const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
   if (tiles == 0) {
-    for (int d = threadIdx.x; d < D; d += 128) store_output(p, b, h, d, 0.f);
+    grid_dep_wait();  // on every path: this grid is not to end before the main one
+    if (team == 0) store_output(p, b, h, d, zero, zero);
     return;
   }
-  const long long c0 = lo / share, c1 = (lo + tiles - 1) / share;
-  if (c0 == c1) return;  // finished by its CTA
-  float m = -INFINITY, l = 0.f, o[PER];
-#pragma unroll
-  for (int i = 0; i < PER; ++i) o[i] = 0.f;
-  for (long long c = c0 + warp; c <= c1; c += 4) {
-    const long long part = (2 * c + (c == c0 && c * share < lo ? 1 : 0)) * p.group + r;
-    const float pm = p.part_ml[2 * part], pl = p.part_ml[2 * part + 1];
-    const float mn = fmaxf(m, pm), mu = mn == -INFINITY ? 0.f : mn;
-    const float fo = ex2(m - mu), fp = ex2(pm - mu);
-    m = mn;
-    l = l * fo + pl * fp;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) o[i] = o[i] * fo + p.part_o[part * D + i * 32 + lane] * fp;
+  const long long c0 = lo / share;
+  const int parts = (int)((lo + tiles - 1) / share - c0) + 1;
+  if (parts == 1) {  // finished by its CTA
+    grid_dep_wait();
+    return;
   }
-#pragma unroll
-  for (int i = 0; i < PER; ++i) s_o[warp][i * 32 + lane] = o[i];
-  if (lane == 0) {
-    s_m[warp] = m;
-    s_l[warp] = l;
+  // Part i's row; the first CTA has the pair as its last unless it starts there.
+  const long long row0 = (2 * c0 + (c0 * share < lo ? 1 : 0)) * p.group + r;
+  auto row_of = [&](int i) { return i == 0 ? row0 : 2 * (c0 + i) * p.group + r; };
+  float4 gate = zero;
+  if (p.gate && team == 0) gate = load_gate(p, b, h, d);
+  grid_dep_wait();
+  float m = -INFINITY;
+#pragma unroll 4
+  for (int i = team; i < parts; i += TEAMS) m = fmaxf(m, p.part_ml[2 * row_of(i)]);
+  const float mu = m == -INFINITY ? 0.f : m;
+  float l = 0.f;
+  float4 o = zero;
+#pragma unroll 4
+  for (int i = team; i < parts; i += TEAMS) {
+    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + 2 * row_of(i));
+    const float f = ex2(ml.x - mu);
+    l = fmaf(f, ml.y, l);
+    o = axpy(f, *reinterpret_cast<const float4*>(p.part_o + row_of(i) * D + d), o);
+  }
+  s_o[team][threadIdx.x % TEAM] = o;
+  if (d == 0) {
+    s_m[team] = m;
+    s_l[team] = l;
   }
   __syncthreads();
-  float M = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
-  const float Mu = M == -INFINITY ? 0.f : M;
-  for (int d = threadIdx.x; d < D; d += 128) {
-    float lsum = 0.f, osum = 0.f;
+  if (team != 0) return;
+  float M = -INFINITY;
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const float f = ex2(s_m[u] - Mu);
-      lsum += f * s_l[u];
-      osum += f * s_o[u][d];
-    }
-    store_output(p, b, h, d, lsum == 0.f ? 0.f : osum / lsum);
+  for (int u = 0; u < TEAMS; ++u) M = fmaxf(M, s_m[u]);
+  const float Mu = M == -INFINITY ? 0.f : M;
+  float lsum = 0.f;
+  float4 osum = zero;
+#pragma unroll
+  for (int u = 0; u < TEAMS; ++u) {
+    const float f = ex2(s_m[u] - Mu);
+    lsum = fmaf(f, s_l[u], lsum);
+    osum = axpy(f, s_o[u][threadIdx.x], osum);
   }
+  store_output(p, b, h, d, over(osum, lsum), gate);
 }
 
 constexpr int kWholeTiles = 8;

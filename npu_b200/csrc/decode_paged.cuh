@@ -20,6 +20,7 @@ struct DecodePagedParams {
   const void* gate;        // optional [B, Hq, D]: o = attention * sigmoid(gate)
   long long g_sb, g_sh;
   int gate_bf16;
+  int vec4;                // o and gate take accesses of four elements
   int B, Hq, Hkv, group;
   float scale_log2;
   // Split form: partial results of each CTA's first and last (sequence, KV
