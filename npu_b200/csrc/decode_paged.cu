@@ -9,8 +9,12 @@
 // group of query heads that shares it (8 to 16 flop per byte). One warp
 // streams 64-key K / V tiles through a shared-memory ring with TMA, one copy
 // per run of keys that lies in one page (box_rows, 16 to 64 keys); four warps
-// take 16 keys of a tile each. The query heads of a group are the 16 rows of
-// mma.sync m16n8k16. P goes into the second product as two bf16 terms (its
+// take 16 keys of a tile each. Both products are computed transposed,
+// S^T = K Q^T and O^T = V^T P^T, with mma.sync m16n8k16: the keys (then the
+// columns of V) are its 16 rows and the query heads of a group its 8 columns,
+// so a group of up to 8 heads wastes no rows and needs half the registers and
+// MMAs of the other orientation (groups of 9 to 16 use two column blocks).
+// P goes into the second product as two bf16 terms (its
 // rounding and what the rounding left), so its relative error is 2^-16
 // instead of 2^-8; the extra MMAs hide behind the loads.
 //
@@ -74,6 +78,13 @@ __device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t& r0, uint32_t& r
                : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
                : "r"(addr)
                : "memory");
+}
+
+// Transpose of an 8x8 matrix of 16-bit elements held as fragments.
+__device__ __forceinline__ uint32_t transposed(uint32_t a) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
 }
 
 __device__ __forceinline__ void tma_load_5d(void* smem_dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1,
@@ -217,7 +228,8 @@ struct Walk {
   }
 };
 
-template <int D, bool SPLIT>
+// NT blocks of 8 query heads cover a group; SPLIT: the even split above.
+template <int D, int NT, bool SPLIT>
 __global__ void __launch_bounds__(PagedCfg<D>::THREADS, PagedCfg<D>::CTAS_PER_SM)
     decode_paged_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                         const __grid_constant__ DecodePagedParams p) {
@@ -321,23 +333,29 @@ __global__ void __launch_bounds__(PagedCfg<D>::THREADS, PagedCfg<D>::CTAS_PER_SM
     int n = 0;  // tiles taken so far
     do {
       const int n_last = n + (w.t1 - w.t0) - 1;  // the pair's last one here
-      uint32_t qa[D / 16][4];
-      {
-        const bool v0 = gr < p.group, v1 = gr + 8 < p.group;
-        const __nv_bfloat16* q0 = p.q + w.b * p.q_sb + (long long)(w.g * p.group + gr) * p.q_sh;
-        const __nv_bfloat16* q1 = q0 + 8 * p.q_sh;
+      // Q^T as the B operand: column (head) gr, k in pairs 2 tq, 2 tq + 8.
+      uint32_t qb[NT][D / 16][2];
+#pragma unroll
+      for (int x = 0; x < NT; ++x) {
+        const int r = 8 * x + gr;
+        const __nv_bfloat16* q = p.q + w.b * p.q_sb + (long long)(w.g * p.group + r) * p.q_sh + 2 * tq;
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
-          qa[k][0] = v0 ? *reinterpret_cast<const uint32_t*>(q0 + 16 * k + 2 * tq) : 0u;
-          qa[k][1] = v1 ? *reinterpret_cast<const uint32_t*>(q1 + 16 * k + 2 * tq) : 0u;
-          qa[k][2] = v0 ? *reinterpret_cast<const uint32_t*>(q0 + 16 * k + 2 * tq + 8) : 0u;
-          qa[k][3] = v1 ? *reinterpret_cast<const uint32_t*>(q1 + 16 * k + 2 * tq + 8) : 0u;
+          qb[x][k][0] = r < p.group ? *reinterpret_cast<const uint32_t*>(q + 16 * k) : 0u;
+          qb[x][k][1] = r < p.group ? *reinterpret_cast<const uint32_t*>(q + 16 * k + 8) : 0u;
         }
       }
-      float acc[D / 8][4];
+      // O^T: rows 16 d + gr (+ 8), columns (heads) 8 x + 2 tq (+ 1); this
+      // thread keeps the running maximum and its part of the sum of those heads.
+      float acc[NT][D / 16][4];
+      float m[NT][2], l[NT][2];
 #pragma unroll
-      for (int d = 0; d < D / 8; ++d) acc[d][0] = acc[d][1] = acc[d][2] = acc[d][3] = 0.f;
-      float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+      for (int x = 0; x < NT; ++x) {
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d) acc[x][d][0] = acc[x][d][1] = acc[x][d][2] = acc[x][d][3] = 0.f;
+        m[x][0] = m[x][1] = -INFINITY;
+        l[x][0] = l[x][1] = 0.f;
+      }
       for (int t = w.t0; t < w.t1; ++t, ++n) {
         const int slot = n % C::STAGES;
         if (!__all_sync(0xffffffffu,
@@ -349,75 +367,74 @@ __global__ void __launch_bounds__(PagedCfg<D>::THREADS, PagedCfg<D>::CTAS_PER_SM
         const uint32_t vbase = kbase + C::TILE_BYTES;
         const int have = w.len - (t * C::TK + 16 * warp);  // keys of this warp's 16 that exist
         if (have > 0) {
-          float s[2][4];
+          float s[NT][4];
 #pragma unroll
-          for (int ng = 0; ng < 2; ++ng) {
-            s[ng][0] = s[ng][1] = s[ng][2] = s[ng][3] = 0.f;
+          for (int x = 0; x < NT; ++x) s[x][0] = s[x][1] = s[x][2] = s[x][3] = 0.f;
 #pragma unroll
-            for (int kp = 0; kp < D / 32; ++kp) {
-              uint32_t b0, b1, b2, b3;
-              ldsm4(at(kbase, 8 * ng + mr, 4 * kp + mi), b0, b1, b2, b3);
-              mma16816(s[ng], qa[2 * kp], b0, b1);
-              mma16816(s[ng], qa[2 * kp + 1], b2, b3);
-            }
+          for (int k = 0; k < D / 16; ++k) {
+            uint32_t a[4];
+            ldsm4(at(kbase, 8 * (mi & 1) + mr, 2 * k + (mi >> 1)), a[0], a[1], a[2], a[3]);
+#pragma unroll
+            for (int x = 0; x < NT; ++x) mma16816(s[x], a, qb[x][k][0], qb[x][k][1]);
           }
           if (have < 16) {
 #pragma unroll
-            for (int ng = 0; ng < 2; ++ng)
-#pragma unroll
-              for (int e = 0; e < 2; ++e)
-                if (8 * ng + 2 * tq + e >= have) s[ng][e] = s[ng][2 + e] = -INFINITY;
+            for (int x = 0; x < NT; ++x) {
+              if (gr >= have) s[x][0] = s[x][1] = -INFINITY;
+              if (gr + 8 >= have) s[x][2] = s[x][3] = -INFINITY;
+            }
             // V rows without a key: 0 x anything would not do (NaN).
             for (int u = lane; u < (16 - have) * (D / 8); u += 32)
               st_shared_v4(at(vbase, have + u / (D / 8), u % (D / 8)), 0u, 0u, 0u, 0u);
             fence_proxy_async_smem();  // before the slot's next copy
             __syncwarp();
           }
-          float mx0 = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]));
-          float mx1 = fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3]));
-          mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 1));
-          mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 2));
-          mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 1));
-          mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 2));
-          const float mn0 = fmaxf(m0, mx0 * sl2), mn1 = fmaxf(m1, mx1 * sl2);
-          const float u0 = (mn0 == -INFINITY) ? 0.f : mn0, u1 = (mn1 == -INFINITY) ? 0.f : mn1;
-          const float a0 = ex2(m0 - u0), a1 = ex2(m1 - u1);
-          m0 = mn0;
-          m1 = mn1;
-          float pr[2][4];
+          // P^T as the B operand, in two bf16 terms: the scores' fragments
+          // hold keys along gr and heads along tq, the operand the reverse.
+          uint32_t ph[NT][2], pl[NT][2];
 #pragma unroll
-          for (int ng = 0; ng < 2; ++ng) {
-            pr[ng][0] = ex2(fmaf(s[ng][0], sl2, -u0));
-            pr[ng][1] = ex2(fmaf(s[ng][1], sl2, -u0));
-            pr[ng][2] = ex2(fmaf(s[ng][2], sl2, -u1));
-            pr[ng][3] = ex2(fmaf(s[ng][3], sl2, -u1));
+          for (int x = 0; x < NT; ++x) {
+            float a[2];
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              float mx = fmaxf(s[x][c], s[x][2 + c]);
+              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+              const float mn = fmaxf(m[x][c], mx * sl2);
+              const float u = mn == -INFINITY ? 0.f : mn;
+              a[c] = ex2(m[x][c] - u);
+              m[x][c] = mn;
+              s[x][c] = ex2(fmaf(s[x][c], sl2, -u));
+              s[x][2 + c] = ex2(fmaf(s[x][2 + c], sl2, -u));
+              l[x][c] = fmaf(l[x][c], a[c], s[x][c] + s[x][2 + c]);
+            }
+            if (__any_sync(0xffffffffu, a[0] != 1.f || a[1] != 1.f)) {
+#pragma unroll
+              for (int d = 0; d < D / 16; ++d) {
+                acc[x][d][0] *= a[0];
+                acc[x][d][1] *= a[1];
+                acc[x][d][2] *= a[0];
+                acc[x][d][3] *= a[1];
+              }
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const uint32_t high = pack_bf16x2(s[x][2 * e], s[x][2 * e + 1]);
+              ph[x][e] = transposed(high);
+              pl[x][e] = transposed(pack_bf16x2(s[x][2 * e] - __uint_as_float(high << 16),
+                                                s[x][2 * e + 1] - __uint_as_float(high & 0xffff0000u)));
+            }
           }
-          l0 = l0 * a0 + pr[0][0] + pr[0][1] + pr[1][0] + pr[1][1];
-          l1 = l1 * a1 + pr[0][2] + pr[0][3] + pr[1][2] + pr[1][3];
 #pragma unroll
-          for (int n = 0; n < D / 8; ++n) {
-            acc[n][0] *= a0;
-            acc[n][1] *= a0;
-            acc[n][2] *= a1;
-            acc[n][3] *= a1;
-          }
-          // P = high + low, each bf16.
-          uint32_t ph[4], pl[4];
+          for (int d = 0; d < D / 16; ++d) {
+            uint32_t a[4];
+            ldsm4_t(at(vbase, 8 * (mi >> 1) + mr, 2 * d + (mi & 1)), a[0], a[1], a[2], a[3]);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float x = pr[e >> 1][2 * (e & 1)], y = pr[e >> 1][2 * (e & 1) + 1];
-            ph[e] = pack_bf16x2(x, y);
-            pl[e] = pack_bf16x2(x - __uint_as_float(ph[e] << 16), y - __uint_as_float(ph[e] & 0xffff0000u));
-          }
-          const int vr = 8 * (mi & 1) + mr;
-#pragma unroll
-          for (int dn = 0; dn < D / 8; dn += 2) {
-            uint32_t b0, b1, b2, b3;
-            ldsm4_t(at(vbase, vr, dn + (mi >> 1)), b0, b1, b2, b3);
-            mma16816(acc[dn], ph, b0, b1);
-            mma16816(acc[dn + 1], ph, b2, b3);
-            mma16816(acc[dn], pl, b0, b1);
-            mma16816(acc[dn + 1], pl, b2, b3);
+            for (int x = 0; x < NT; ++x) {
+              mma16816(acc[x][d], a, ph[x][0], ph[x][1]);
+              mma16816(acc[x][d], a, pl[x][0], pl[x][1]);
+            }
           }
         }
         __syncwarp();
@@ -425,24 +442,34 @@ __global__ void __launch_bounds__(PagedCfg<D>::THREADS, PagedCfg<D>::CTAS_PER_SM
       }
       // Merge the four warps' (m, l, O) in the last tile's stage, once all of
       // them have read it; the stage is released after that.
-      l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
-      l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
-      l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
-      l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
       asm volatile("bar.sync 1, 128;" ::: "memory");
       const int slot = n_last % C::STAGES;
-      float* so = reinterpret_cast<float*>(smem + slot * C::STAGE_BYTES);  // [4][16][D]
+      // [4][16][D], columns swizzled by the head so that neither side's
+      // accesses collide in a bank.
+      float* so = reinterpret_cast<float*>(smem + slot * C::STAGE_BYTES);
+      auto swizzle = [](int r, int d) { return d ^ (((r >> 1) & 3) << 3); };
 #pragma unroll
-      for (int d = 0; d < D / 8; ++d) {
-        float* r0 = so + (warp * 16 + gr) * D + 8 * d + 2 * tq;
-        if (gr < p.group) *reinterpret_cast<float2*>(r0) = make_float2(acc[d][0], acc[d][1]);
-        if (gr + 8 < p.group) *reinterpret_cast<float2*>(r0 + 8 * D) = make_float2(acc[d][2], acc[d][3]);
-      }
-      if (tq == 0) {
-        bars->m[warp][gr] = m0;
-        bars->m[warp][gr + 8] = m1;
-        bars->l[warp][gr] = l0;
-        bars->l[warp][gr + 8] = l1;
+      for (int x = 0; x < NT; ++x) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const int r = 8 * x + 2 * tq + c;
+          float lr = l[x][c];
+          lr += __shfl_xor_sync(0xffffffffu, lr, 4);
+          lr += __shfl_xor_sync(0xffffffffu, lr, 8);
+          lr += __shfl_xor_sync(0xffffffffu, lr, 16);
+          if (gr == 0) {
+            bars->m[warp][r] = m[x][c];
+            bars->l[warp][r] = lr;
+          }
+          if (r < p.group) {
+            float* row = so + (warp * 16 + r) * D;
+#pragma unroll
+            for (int d = 0; d < D / 16; ++d) {
+              row[swizzle(r, 16 * d + gr)] = acc[x][d][c];
+              row[swizzle(r, 16 * d + 8 + gr)] = acc[x][d][2 + c];
+            }
+          }
+        }
       }
       const bool whole = !SPLIT || (w.t0 == 0 && w.t1 == w.tiles);
       const long long part = (2LL * blockIdx.x + (first ? 0 : 1)) * p.group;
@@ -474,7 +501,7 @@ __global__ void __launch_bounds__(PagedCfg<D>::THREADS, PagedCfg<D>::CTAS_PER_SM
           // A warp without keys here has nothing in the sum (its m is -inf).
           const float f = ex2(bars->m[u][r] - Mu);
           lsum += f * bars->l[u][r];
-          osum = axpy(f, *reinterpret_cast<const float4*>(so + (u * 16 + r) * D + d), osum);
+          osum = axpy(f, *reinterpret_cast<const float4*>(so + (u * 16 + r) * D + swizzle(r, d)), osum);
         }
         if (whole) {
           store_output(p, w.b, w.g * p.group + r, d, over(osum, lsum), gate[i]);
@@ -571,24 +598,29 @@ __global__ void __launch_bounds__(128) decode_paged_join_kernel(const __grid_con
 
 constexpr int kWholeTiles = 8;
 
-template <int D, bool SPLIT>
+template <int D, int NT, bool SPLIT>
 int launch_main(const CUtensorMap& tk, const CUtensorMap& tv, const DecodePagedParams& p, long long n,
                 cudaStream_t st) {
   using C = PagedCfg<D>;
-  if (cudaFuncSetAttribute(decode_paged_kernel<D, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+  if (cudaFuncSetAttribute(decode_paged_kernel<D, NT, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                            C::SMEM_BYTES) != cudaSuccess)
     return -1;
   if (n > 0x7fffffffLL) return -2;
-  decode_paged_kernel<D, SPLIT><<<(unsigned)n, C::THREADS, C::SMEM_BYTES, st>>>(tk, tv, p);
+  decode_paged_kernel<D, NT, SPLIT><<<(unsigned)n, C::THREADS, C::SMEM_BYTES, st>>>(tk, tv, p);
   return cudaGetLastError() == cudaSuccess ? 0 : -1;
 }
 
 template <int D>
 int launch_t(const CUtensorMap& tk, const CUtensorMap& tv, const DecodePagedParams& p, cudaStream_t st) {
-  if (!decode_paged_splits(p.table_width, p.page)) return launch_main<D, false>(tk, tv, p, (long long)p.B * p.Hkv, st);
+  const bool narrow = p.group <= 8;
+  if (!decode_paged_splits(p.table_width, p.page)) {
+    const long long pairs = (long long)p.B * p.Hkv;
+    return narrow ? launch_main<D, 1, false>(tk, tv, p, pairs, st) : launch_main<D, 2, false>(tk, tv, p, pairs, st);
+  }
   const long long heads = (long long)p.B * p.Hq;
   if (heads > 0x7fffffffLL) return -2;
-  const int rc = launch_main<D, true>(tk, tv, p, p.n_ctas, st);
+  const int rc =
+      narrow ? launch_main<D, 1, true>(tk, tv, p, p.n_ctas, st) : launch_main<D, 2, true>(tk, tv, p, p.n_ctas, st);
   if (rc) return rc;
   // The joining kernel is scheduled while the main one drains and waits for
   // all of it before it reads anything.
