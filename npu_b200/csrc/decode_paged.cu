@@ -43,7 +43,9 @@ struct PagedCfg {
   static constexpr int STAGE_BYTES = 2 * TILE_BYTES;
   static constexpr int STAGES = D == 64 ? 6 : 3;
   static constexpr int CTAS_PER_SM = D == 256 ? 1 : 2;
-  static constexpr int OFF_BAR = STAGES * STAGE_BYTES;
+  static constexpr int Q_ROW = D * 2 + 16;  // bytes; the 16 keep ldmatrix rows apart
+  static constexpr int OFF_Q = STAGES * STAGE_BYTES;
+  static constexpr int OFF_BAR = OFF_Q + 2 * 16 * Q_ROW;  // two pairs' query heads
   static constexpr int SMEM_BYTES = OFF_BAR + 1024 + 1024;  // barriers and m, l; alignment slack
   static constexpr int THREADS = 160;  // 4 compute warps + 1 producer warp
   static_assert(4 * 16 * D * 4 <= STAGE_BYTES, "the four warps' outputs are merged in one stage");
@@ -53,6 +55,8 @@ struct PagedCfg {
 struct PagedBars {
   uint64_t full[8];
   uint64_t empty[8];
+  uint64_t q_full[2];
+  uint64_t q_empty[2];
   int abort_flag;
   float m[4][16];
   float l[4][16];
@@ -94,6 +98,13 @@ __device__ __forceinline__ void tma_load_5d(void* smem_dst, const CUtensorMap* m
       " [%0], [%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(smem_u32(smem_dst)),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4)
       : "memory");
+}
+
+__device__ __forceinline__ void bulk_load(void* smem_dst, const void* src, int bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   smem_u32(smem_dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
 }
 
 // The gate of (sequence b, query head h) at columns d .. d + 3.
@@ -177,7 +188,8 @@ __device__ __forceinline__ long long share_of(long long total, int n_ctas) {
 struct Walk {
   long long left;  // tiles of the stretch not yet given out
   int b, g;        // the pair
-  int t0, t1;      // its tiles in the stretch
+  int begin, t1;   // its tiles in the stretch
+  int t0;          // the current one (the producer's)
   int tiles, len;  // all its tiles, its keys
   // Positioned at tile `from` of all; `left` tiles to go. Warp-collective.
   __device__ __forceinline__ Walk(const DecodePagedParams& p, long long from, long long count) {
@@ -202,19 +214,20 @@ struct Walk {
         tiles = (len + 63) / 64;
         const long long into = from - before;
         g = (int)(into / tiles);
-        t0 = (int)(into % tiles);
+        begin = (int)(into % tiles);
         break;
       }
       from -= (long long)__shfl_sync(0xffffffffu, upto, 31) * p.Hkv;
     }
-    t1 = (int)min((long long)tiles, t0 + left);
+    t0 = begin;
+    t1 = (int)min((long long)tiles, begin + left);
   }
   __device__ __forceinline__ Walk(int b_, int g_, int len_)
-      : left((len_ + 63) / 64), b(b_), g(g_), t0(0), t1((len_ + 63) / 64), tiles((len_ + 63) / 64), len(len_) {}
+      : left((len_ + 63) / 64), b(b_), g(g_), begin(0), t1((len_ + 63) / 64), t0(0), tiles(t1), len(len_) {}
   __device__ __forceinline__ bool next(const DecodePagedParams& p) {
-    left -= t1 - t0;
+    left -= t1 - begin;
     if (left <= 0) return false;
-    t0 = 0;
+    t0 = begin = 0;
     if (++g == p.Hkv) {
       g = 0;
       do {
@@ -269,9 +282,17 @@ __global__ void __launch_bounds__(PagedCfg<D>::THREADS, PagedCfg<D>::CTAS_PER_SM
       mbar_init(&bars->full[s], 1);
       mbar_init(&bars->empty[s], 4);
     }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&bars->q_full[s], 1);
+      mbar_init(&bars->q_empty[s], 4);
+    }
     bars->abort_flag = 0;
     fence_mbar_init();
   }
+  // Rows of Q past the group stay zero.
+  for (int e = threadIdx.x; e < 2 * C::Q_ROW; e += C::THREADS)
+    st_shared_v4(smem_u32(smem + C::OFF_Q) + 16 * e, 0u, 0u, 0u, 0u);
+  fence_proxy_async_smem();
   __syncthreads();
 
   const int br = p.box_rows;
@@ -283,36 +304,61 @@ __global__ void __launch_bounds__(PagedCfg<D>::THREADS, PagedCfg<D>::CTAS_PER_SM
     const bool is_v = lane >= boxes;
     const bool mine = lane < 2 * boxes;
     const int box_bytes = br * D * 2;
-    int n = 0;  // tiles copied so far
-    do {
-      auto page_of = [&](int t) -> int {  // page of this lane's box in tile t
-        const int key = t * C::TK + box * br;
-        if (!mine || key >= w.len) return -1;
-        const int id = p.block_table[w.b * p.table_ld + key / p.page];
-        if (id >= 0 && id < p.n_pages) return id;
-        if (p.err) atomicOr(p.err, kErrBadArgs);
-        return 0;
-      };
-      int next = page_of(w.t0);
-      for (int t = w.t0; t < w.t1; ++t, ++n) {
-        const int slot = n % C::STAGES;
-        const int id = next;
-        if (t + 1 < w.t1) next = page_of(t + 1);
-        if (!__all_sync(0xffffffffu, mbar_wait(&bars->empty[slot], ((uint32_t)(n / C::STAGES) & 1u) ^ 1u, abort_flag,
+    // Every tile's page is looked up one tile ahead, across pairs too, and
+    // checked when its turn comes (so that nothing waits for the lookup).
+    auto has_keys = [&]() { return mine && w.t0 * C::TK + box * br < w.len; };
+    auto entry_of = [&]() -> int {  // table entry of this lane's box in tile w.t0
+      return has_keys() ? p.block_table[w.b * p.table_ld + (w.t0 * C::TK + box * br) / p.page] : 0;
+    };
+    int n = 0, pairs = 0;  // tiles and pairs copied so far
+    bool more = true, new_pair = true;
+    int entry = entry_of();
+    bool copy = has_keys();
+    while (more) {
+      const int slot = n % C::STAGES;
+      const int g = w.g, row = (w.t0 * C::TK + box * br) % p.page;
+      const __nv_bfloat16* q = p.q + w.b * p.q_sb + (long long)(g * p.group + lane) * p.q_sh;
+      const bool with_q = new_pair;
+      ++w.t0;
+      new_pair = w.t0 == w.t1;
+      if (new_pair) more = w.next(p);
+      const int id = entry;
+      const bool now = copy;
+      if (more) {
+        entry = entry_of();
+        copy = has_keys();
+      }
+      if (with_q) {
+        const int qs = pairs & 1;
+        if (!__all_sync(0xffffffffu, mbar_wait(&bars->q_empty[qs], ((uint32_t)(pairs >> 1) & 1u) ^ 1u, abort_flag,
                                                p.err)))
           break;
-        uint8_t* dst = smem + slot * C::STAGE_BYTES + (is_v ? C::TILE_BYTES : 0) + box * box_bytes;
-        const unsigned copies = __ballot_sync(0xffffffffu, id >= 0);
-        if (lane == 0) mbar_arrive_expect_tx(&bars->full[slot], __popc(copies) * box_bytes);
+        if (lane == 0) mbar_arrive_expect_tx(&bars->q_full[qs], p.group * D * 2);
         __syncwarp();
-        if (id >= 0)
-          tma_load_5d(dst, is_v ? &tm_v : &tm_k, &bars->full[slot], 0, (t * C::TK + box * br) % p.page, 0, w.g, id);
+        if (lane < p.group)
+          bulk_load(smem + C::OFF_Q + (qs * 16 + lane) * C::Q_ROW, q, D * 2, &bars->q_full[qs]);
+        ++pairs;
       }
-    } while (!*abort_flag && w.next(p));
-    const int issued = n;
-    if (*abort_flag && lane == 0)
-      for (int i = max(0, issued - C::STAGES); i < issued; ++i)
+      if (!__all_sync(0xffffffffu, mbar_wait(&bars->empty[slot], ((uint32_t)(n / C::STAGES) & 1u) ^ 1u, abort_flag,
+                                             p.err)))
+        break;
+      uint8_t* dst = smem + slot * C::STAGE_BYTES + (is_v ? C::TILE_BYTES : 0) + box * box_bytes;
+      const unsigned copies = __ballot_sync(0xffffffffu, now);
+      if (lane == 0) mbar_arrive_expect_tx(&bars->full[slot], __popc(copies) * box_bytes);
+      __syncwarp();
+      if (now) {
+        const bool in_pool = id >= 0 && id < p.n_pages;
+        if (!in_pool && p.err) atomicOr(p.err, kErrBadArgs);
+        tma_load_5d(dst, is_v ? &tm_v : &tm_k, &bars->full[slot], 0, row, 0, g, in_pool ? id : 0);
+      }
+      ++n;
+    }
+    if (*abort_flag && lane == 0) {
+      // Let every copy still in flight land before the CTA releases smem.
+      for (int i = max(0, n - C::STAGES); i < n; ++i)
         mbar_wait_quiet(&bars->full[i % C::STAGES], (uint32_t)(i / C::STAGES) & 1u);
+      for (int i = max(0, pairs - 2); i < pairs; ++i) mbar_wait_quiet(&bars->q_full[i & 1], (uint32_t)(i >> 1) & 1u);
+    }
   } else {
     // ------------------------------------------------------------ compute warps
     const int gr = lane >> 2, tq = lane & 3;
@@ -329,22 +375,23 @@ __global__ void __launch_bounds__(PagedCfg<D>::THREADS, PagedCfg<D>::CTAS_PER_SM
     };
     // A wait that ran out leaves garbage in the result and the error word set;
     // the warps still meet at every barrier below.
-    bool first = true;
-    int n = 0;  // tiles taken so far
+    int pair = 0;  // pairs done so far
+    int n = 0;     // tiles taken so far
     do {
-      const int n_last = n + (w.t1 - w.t0) - 1;  // the pair's last one here
+      const int n_last = n + (w.t1 - w.begin) - 1;  // the pair's last one here
       // Q^T as the B operand: column (head) gr, k in pairs 2 tq, 2 tq + 8.
       uint32_t qb[NT][D / 16][2];
+      const bool got = __all_sync(
+          0xffffffffu, mbar_wait(&bars->q_full[pair & 1], (uint32_t)(pair >> 1) & 1u, abort_flag, p.err));
 #pragma unroll
       for (int x = 0; x < NT; ++x) {
-        const int r = 8 * x + gr;
-        const __nv_bfloat16* q = p.q + w.b * p.q_sb + (long long)(w.g * p.group + r) * p.q_sh + 2 * tq;
+        const uint32_t q = smem_u32(smem + C::OFF_Q) + ((pair & 1) * 16 + 8 * x + mr) * C::Q_ROW + mi * 16;
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          qb[x][k][0] = r < p.group ? *reinterpret_cast<const uint32_t*>(q + 16 * k) : 0u;
-          qb[x][k][1] = r < p.group ? *reinterpret_cast<const uint32_t*>(q + 16 * k + 8) : 0u;
-        }
+        for (int k = 0; k < D / 32; ++k)
+          ldsm4(q + 64 * k, qb[x][2 * k][0], qb[x][2 * k][1], qb[x][2 * k + 1][0], qb[x][2 * k + 1][1]);
       }
+      __syncwarp();
+      if (lane == 0 && got) mbar_arrive(&bars->q_empty[pair & 1]);
       // O^T: rows 16 d + gr (+ 8), columns (heads) 8 x + 2 tq (+ 1); this
       // thread keeps the running maximum and its part of the sum of those heads.
       float acc[NT][D / 16][4];
@@ -356,7 +403,7 @@ __global__ void __launch_bounds__(PagedCfg<D>::THREADS, PagedCfg<D>::CTAS_PER_SM
         m[x][0] = m[x][1] = -INFINITY;
         l[x][0] = l[x][1] = 0.f;
       }
-      for (int t = w.t0; t < w.t1; ++t, ++n) {
+      for (int t = w.begin; t < w.t1; ++t, ++n) {
         const int slot = n % C::STAGES;
         if (!__all_sync(0xffffffffu,
                         mbar_wait(&bars->full[slot], (uint32_t)(n / C::STAGES) & 1u, abort_flag, p.err))) {
@@ -471,24 +518,23 @@ __global__ void __launch_bounds__(PagedCfg<D>::THREADS, PagedCfg<D>::CTAS_PER_SM
           }
         }
       }
-      const bool whole = !SPLIT || (w.t0 == 0 && w.t1 == w.tiles);
-      const long long part = (2LL * blockIdx.x + (first ? 0 : 1)) * p.group;
-      // Thread x takes columns 4 x .. of the group's rows, 512 apart; the
-      // gates are requested together, ahead of the barrier.
-      constexpr int STEPS = 16 * D / 512;
-      float4 gate[STEPS];
-      if (p.gate && whole) {
-#pragma unroll
-        for (int i = 0; i < STEPS; ++i) {
-          const int e = 4 * threadIdx.x + 512 * i;
-          if (e < p.group * D) gate[i] = load_gate(p, w.b, w.g * p.group + e / D, e % D);
-        }
-      }
+      const bool whole = !SPLIT || (w.begin == 0 && w.t1 == w.tiles);
+      const long long part = (2LL * blockIdx.x + (pair == 0 ? 0 : 1)) * p.group;
+      // Thread x takes columns 4 x .. of the group's rows, 512 apart, each
+      // step's gate requested a step ahead. A loop, not unrolled: this runs
+      // once per pair, and fetching unrolled code cost more than running it.
+      const int last = p.group * D;
+      float4 gate = make_float4(0.f, 0.f, 0.f, 0.f);
+      const bool gated = p.gate && whole;
+      auto gate_at = [&](int e) {
+        if (gated && e < last) gate = load_gate(p, w.b, w.g * p.group + e / D, e % D);
+      };
+      gate_at(4 * threadIdx.x);
       asm volatile("bar.sync 1, 128;" ::: "memory");
-#pragma unroll
-      for (int i = 0; i < STEPS; ++i) {
-        const int e = 4 * threadIdx.x + 512 * i;
-        if (e >= p.group * D) break;
+#pragma unroll 1
+      for (int e = 4 * threadIdx.x; e < last; e += 512) {
+        const float4 now = gate;
+        gate_at(e + 512);
         const int r = e / D, d = e % D;
         float M = -INFINITY;
 #pragma unroll
@@ -504,7 +550,7 @@ __global__ void __launch_bounds__(PagedCfg<D>::THREADS, PagedCfg<D>::CTAS_PER_SM
           osum = axpy(f, *reinterpret_cast<const float4*>(so + (u * 16 + r) * D + swizzle(r, d)), osum);
         }
         if (whole) {
-          store_output(p, w.b, w.g * p.group + r, d, over(osum, lsum), gate[i]);
+          store_output(p, w.b, w.g * p.group + r, d, over(osum, lsum), now);
         } else {
           *reinterpret_cast<float4*>(p.part_o + (part + r) * D + d) = osum;
           if (d == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * (part + r)) = make_float2(M, lsum);
@@ -513,10 +559,12 @@ __global__ void __launch_bounds__(PagedCfg<D>::THREADS, PagedCfg<D>::CTAS_PER_SM
       fence_proxy_async_smem();
       asm volatile("bar.sync 1, 128;" ::: "memory");  // everyone has read the stage, m and l
       if (lane == 0) mbar_arrive(&bars->empty[slot]);
-      first = false;
+      ++pair;
     } while (w.next(p));
   }
 }
+
+constexpr int kJoinThreads = 256;
 
 // Joins the partials of (sequence, query head) blockIdx.x, if its keys were
 // cut between CTAs; a sequence without keys gets its zeros here. The parts
@@ -526,8 +574,8 @@ __global__ void __launch_bounds__(PagedCfg<D>::THREADS, PagedCfg<D>::CTAS_PER_SM
 // in turn and joined in a fixed order. The lengths are read before the wait
 // for the main kernel (which does not write them).
 template <int D>
-__global__ void __launch_bounds__(128) decode_paged_join_kernel(const __grid_constant__ DecodePagedParams p) {
-  constexpr int TEAM = D / 4, TEAMS = 128 / TEAM;
+__global__ void __launch_bounds__(kJoinThreads) decode_paged_join_kernel(const __grid_constant__ DecodePagedParams p) {
+  constexpr int TEAM = D / 4, TEAMS = kJoinThreads / TEAM;
   __shared__ float4 s_o[TEAMS][TEAM];
   __shared__ float s_m[TEAMS], s_l[TEAMS];
   const int lane = threadIdx.x & 31;
@@ -561,18 +609,33 @@ __global__ void __launch_bounds__(128) decode_paged_join_kernel(const __grid_con
   float4 gate = zero;
   if (p.gate && team == 0) gate = load_gate(p, b, h, d);
   grid_dep_wait();
-  float m = -INFINITY;
-#pragma unroll 4
-  for (int i = team; i < parts; i += TEAMS) m = fmaxf(m, p.part_ml[2 * row_of(i)]);
-  const float mu = m == -INFINITY ? 0.f : m;
-  float l = 0.f;
+  float m = -INFINITY, l = 0.f;
   float4 o = zero;
-#pragma unroll 4
-  for (int i = team; i < parts; i += TEAMS) {
-    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + 2 * row_of(i));
-    const float f = ex2(ml.x - mu);
-    l = fmaf(f, ml.y, l);
-    o = axpy(f, *reinterpret_cast<const float4*>(p.part_o + row_of(i) * D + d), o);
+  for (int i0 = team; i0 < parts; i0 += 4 * TEAMS) {
+    float2 ml[4];
+    float4 po[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int i = i0 + k * TEAMS;
+      ml[k] = make_float2(-INFINITY, 0.f);
+      po[k] = zero;
+      if (i < parts) {
+        ml[k] = *reinterpret_cast<const float2*>(p.part_ml + 2 * row_of(i));
+        po[k] = *reinterpret_cast<const float4*>(p.part_o + row_of(i) * D + d);
+      }
+    }
+    const float mn = fmaxf(fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)), m);
+    const float mu = mn == -INFINITY ? 0.f : mn;
+    const float f0 = ex2(m - mu);
+    m = mn;
+    l *= f0;
+    o = make_float4(o.x * f0, o.y * f0, o.z * f0, o.w * f0);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float f = ex2(ml[k].x - mu);
+      l = fmaf(f, ml[k].y, l);
+      o = axpy(f, po[k], o);
+    }
   }
   s_o[team][threadIdx.x % TEAM] = o;
   if (d == 0) {
@@ -629,7 +692,7 @@ int launch_t(const CUtensorMap& tk, const CUtensorMap& tv, const DecodePagedPara
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)heads);
-  cfg.blockDim = dim3(128);
+  cfg.blockDim = dim3(kJoinThreads);
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
