@@ -116,10 +116,8 @@ int b2a_prefill_varlen(const void* q, const void* k, const void* v, const void* 
 
 size_t b2a_decode_paged_workspace_bytes(int B, int Hq, int Hkv, int D) {
   if (B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || Hq / Hkv > 16 || !head_dim_ok(D)) return 0;
-  // Two partials per CTA of the split form: O [group, D] and (m, l) [group, 2].
-  const size_t parts = 2 * (size_t)b2a::decode_paged_max_ctas(D, b2a::api_sm_count());
-  return b2a::api_align256(parts * (Hq / Hkv) * D * sizeof(float)) +
-         b2a::api_align256(parts * (Hq / Hkv) * 2 * sizeof(float));
+  const size_t rows = b2a::decode_paged_parts(B, Hkv, b2a::decode_paged_max_ctas(D, b2a::api_sm_count())) * (Hq / Hkv);
+  return b2a::api_align256(rows * D * sizeof(float)) + b2a::api_align256(rows * 2 * sizeof(float));
 }
 
 int b2a_decode_paged(const void* q, const void* k_pages, const void* v_pages, const int* block_table,
@@ -136,7 +134,8 @@ int b2a_decode_paged(const void* q, const void* k_pages, const void* v_pages, co
   if (!head_dim_ok(D)) return B2A_ERR_HEAD_DIM;
   if (Hq % Hkv || Hq / Hkv > 16) return B2A_ERR_GQA;
   if (!api_aligned(q, 16) || !api_aligned(k_pages, 16) || !api_aligned(v_pages, 16) ||
-      !api_aligned(o, out_fp32 ? 4 : 2) || !api_aligned(block_table, 4) || !api_aligned(seqlens, 4) || !api_aligned(gate, gate_bf16 ? 2 : 4))
+      !api_aligned(o, out_fp32 ? 4 : 2) || !api_aligned(block_table, 4) || !api_aligned(seqlens, 4) ||
+      !api_aligned(gate, gate_bf16 ? 2 : 4))
     return B2A_ERR_ALIGNMENT;
   if (!api_strides_ok(qs, 2, 8) || !api_strides_ok(ks, 3, 8) || !api_strides_ok(vs, 3, 8)) return B2A_ERR_ALIGNMENT;
   const size_t need = b2a_decode_paged_workspace_bytes(B, Hq, Hkv, D);
@@ -184,7 +183,8 @@ int b2a_decode_paged(const void* q, const void* k_pages, const void* v_pages, co
   p.n_ctas = b2a::decode_paged_max_ctas(D, b2a::api_sm_count());
   p.part_o = static_cast<float*>(workspace);
   p.part_ml = reinterpret_cast<float*>(static_cast<char*>(workspace) +
-                                       b2a::api_align256((size_t)2 * p.n_ctas * p.group * D * sizeof(float)));
+                                       b2a::api_align256(b2a::decode_paged_parts(B, Hkv, p.n_ctas) * p.group * D *
+                                                         sizeof(float)));
   return status_of(b2a::launch_decode_paged(D, tk, tv, p, static_cast<cudaStream_t>(stream)));
 }
 

@@ -21,11 +21,10 @@
 // Work is split evenly whatever the lengths: the tiles of all (sequence, KV
 // head) pairs, one after another, are cut into one equal stretch per resident
 // CTA, found on the device from the lengths. A CTA walks its stretch with its
-// ring running across pairs; a pair inside one stretch is finished there, a
-// pair cut between CTAs leaves partials (at most two per CTA, so the
-// workspace does not grow with the batch) that a second, dependent launch
-// joins. Caches of a few tiles (kWholeTiles) are not cut: one CTA per pair,
-// one launch.
+// ring running across pairs; for each
+// pair a partial (m, l and O before its division) goes to the workspace, and
+// a second, dependent launch joins the partials of a pair. Caches of a few
+// tiles (kWholeTiles) are not cut: one CTA per pair, one launch.
 //
 // Slots of a page past the sequence's end may hold anything, NaN included:
 // their scores are replaced by -inf and their V rows by zeros in shared
@@ -149,6 +148,7 @@ __device__ __forceinline__ void store_output(const DecodePagedParams& p, int b, 
   }
 }
 
+__device__ __forceinline__ float4 zero4() { return make_float4(0.f, 0.f, 0.f, 0.f); }
 __device__ __forceinline__ float4 axpy(float a, float4 x, float4 y) {
   return make_float4(fmaf(a, x.x, y.x), fmaf(a, x.y, y.y), fmaf(a, x.z, y.z), fmaf(a, x.w, y.w));
 }
@@ -166,17 +166,22 @@ __device__ __forceinline__ int keys_of(const DecodePagedParams& p, int b) {
 }
 __device__ __forceinline__ int tiles_of(const DecodePagedParams& p, int b) { return (keys_of(p, b) + 63) / 64; }
 
-// All tiles of the call (all lanes get it). Warp-collective.
-__device__ __forceinline__ long long total_tiles(const DecodePagedParams& p) {
+// The work of a pair in the units that are shared out: its tiles, and one
+// more for starting and finishing it (measured at 1 us beside 0.7 us a tile
+// at head dim 64, 2 beside 1.3 at 256). The extra unit follows the tiles.
+__device__ __forceinline__ int units_of(int tiles) { return tiles > 0 ? tiles + 1 : 0; }
+
+// All units of the call (all lanes get it). Warp-collective.
+__device__ __forceinline__ long long total_units(const DecodePagedParams& p) {
   long long n = 0;
   for (int b0 = 0; b0 < p.B; b0 += 32) {
     const int b = b0 + (threadIdx.x & 31);
-    n += __reduce_add_sync(0xffffffffu, b < p.B ? tiles_of(p, b) : 0);
+    n += __reduce_add_sync(0xffffffffu, b < p.B ? units_of(tiles_of(p, b)) : 0);
   }
   return n * p.Hkv;
 }
 
-// Tiles per CTA: an equal share, but no less than a few, so that the joining
+// Units per CTA: an equal share, but no less than a few, so that the joining
 // of partials stays small beside the loads.
 constexpr int kMinShare = 4;
 __device__ __forceinline__ long long share_of(long long total, int n_ctas) {
@@ -184,21 +189,21 @@ __device__ __forceinline__ long long share_of(long long total, int n_ctas) {
   return share < kMinShare ? kMinShare : share;
 }
 
-// A stretch of the tiles, pair by pair.
+// A stretch of the units, pair by pair: the pairs with a tile in it.
 struct Walk {
-  long long left;  // tiles of the stretch not yet given out
+  long long left;  // units from this pair's first one here to the stretch's end
   int b, g;        // the pair
   int begin, t1;   // its tiles in the stretch
   int t0;          // the current one (the producer's)
   int tiles, len;  // all its tiles, its keys
-  // Positioned at tile `from` of all; `left` tiles to go. Warp-collective.
+  // The pairs of units [from, from + count). Warp-collective. Check valid().
   __device__ __forceinline__ Walk(const DecodePagedParams& p, long long from, long long count) {
     left = count;
     b = p.B;
     if (left <= 0) return;
     const int lane = threadIdx.x & 31;
     for (int b0 = 0; b0 < p.B; b0 += 32) {
-      const int n = b0 + lane < p.B ? tiles_of(p, b0 + lane) : 0;
+      const int n = b0 + lane < p.B ? units_of(tiles_of(p, b0 + lane)) : 0;
       int upto = n;  // inclusive sum over the lanes
 #pragma unroll
       for (int off = 1; off < 32; off *= 2) {
@@ -213,25 +218,30 @@ struct Walk {
         len = keys_of(p, b);
         tiles = (len + 63) / 64;
         const long long into = from - before;
-        g = (int)(into / tiles);
-        begin = (int)(into % tiles);
+        g = (int)(into / units_of(tiles));
+        begin = (int)(into % units_of(tiles));
         break;
       }
       from -= (long long)__shfl_sync(0xffffffffu, upto, 31) * p.Hkv;
     }
     t0 = begin;
     t1 = (int)min((long long)tiles, begin + left);
+    if (begin == tiles) next(p);  // only the pair's extra unit is here
   }
   __device__ __forceinline__ Walk(int b_, int g_, int len_)
       : left((len_ + 63) / 64), b(b_), g(g_), begin(0), t1((len_ + 63) / 64), t0(0), tiles(t1), len(len_) {}
+  __device__ __forceinline__ bool valid() const { return left > 0; }
   __device__ __forceinline__ bool next(const DecodePagedParams& p) {
-    left -= t1 - begin;
+    left -= units_of(tiles) - begin;
     if (left <= 0) return false;
     t0 = begin = 0;
     if (++g == p.Hkv) {
       g = 0;
       do {
-        if (++b >= p.B) return false;
+        if (++b >= p.B) {
+          left = 0;
+          return false;
+        }
         len = keys_of(p, b);
         tiles = (len + 63) / 64;
       } while (tiles == 0);
@@ -240,6 +250,8 @@ struct Walk {
     return true;
   }
 };
+
+__device__ __forceinline__ int swizzle(int r, int d) { return d ^ (((r >> 1) & 3) << 3); }
 
 // NT blocks of 8 query heads cover a group; SPLIT: the even split above.
 template <int D, int NT, bool SPLIT>
@@ -260,7 +272,7 @@ __global__ void __launch_bounds__(PagedCfg<D>::THREADS, PagedCfg<D>::CTAS_PER_SM
       if (p.seqlens[b] < 0 || p.seqlens[b] > (long long)p.table_width * p.page) atomicOr(p.err, kErrBadArgs);
   long long from = 0, count = 1;
   if constexpr (SPLIT) {
-    const long long total = total_tiles(p), share = share_of(total, p.n_ctas);
+    const long long total = total_units(p), share = share_of(total, p.n_ctas);
     from = blockIdx.x * share;
     count = min(share, total - from);
     if (count <= 0) return;
@@ -271,10 +283,10 @@ __global__ void __launch_bounds__(PagedCfg<D>::THREADS, PagedCfg<D>::CTAS_PER_SM
     return Walk(b, blockIdx.x % p.Hkv, keys_of(p, b));
   };
   Walk w = start();
+  if (SPLIT && !w.valid()) return;
   if (!SPLIT && w.tiles == 0) {
-    const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int e = 4 * threadIdx.x; e < p.group * D; e += 4 * C::THREADS)
-      store_output(p, w.b, w.g * p.group + e / D, e % D, zero, zero);
+      store_output(p, w.b, w.g * p.group + e / D, e % D, zero4(), zero4());
     return;
   }
   if (threadIdx.x == 0) {
@@ -491,10 +503,9 @@ __global__ void __launch_bounds__(PagedCfg<D>::THREADS, PagedCfg<D>::CTAS_PER_SM
       // them have read it; the stage is released after that.
       asm volatile("bar.sync 1, 128;" ::: "memory");
       const int slot = n_last % C::STAGES;
-      // [4][16][D], columns swizzled by the head so that neither side's
-      // accesses collide in a bank.
+      // [4][16][D], columns swizzled by the head so that neither side's accesses
+      // collide in a bank.
       float* so = reinterpret_cast<float*>(smem + slot * C::STAGE_BYTES);
-      auto swizzle = [](int r, int d) { return d ^ (((r >> 1) & 3) << 3); };
 #pragma unroll
       for (int x = 0; x < NT; ++x) {
 #pragma unroll
@@ -518,30 +529,21 @@ __global__ void __launch_bounds__(PagedCfg<D>::THREADS, PagedCfg<D>::CTAS_PER_SM
           }
         }
       }
-      const bool whole = !SPLIT || (w.begin == 0 && w.t1 == w.tiles);
-      const long long part = (2LL * blockIdx.x + (pair == 0 ? 0 : 1)) * p.group;
-      // Thread x takes columns 4 x .. of the group's rows, 512 apart, each
-      // step's gate requested a step ahead. A loop, not unrolled: this runs
-      // once per pair, and fetching unrolled code cost more than running it.
-      const int last = p.group * D;
-      float4 gate = make_float4(0.f, 0.f, 0.f, 0.f);
-      const bool gated = p.gate && whole;
-      auto gate_at = [&](int e) {
-        if (gated && e < last) gate = load_gate(p, w.b, w.g * p.group + e / D, e % D);
-      };
-      gate_at(4 * threadIdx.x);
       asm volatile("bar.sync 1, 128;" ::: "memory");
+      // Thread x takes columns 4 x .. of the group's rows, 512 apart. Not
+      // unrolled, and finished by the joining kernel when SPLIT: this runs
+      // once per pair, and fetching more instructions from memory (which the
+      // stream of keys has pushed out of L2) cost more than running them.
+      const long long part = ((long long)w.b * p.Hkv + w.g + blockIdx.x) * p.group;
 #pragma unroll 1
-      for (int e = 4 * threadIdx.x; e < last; e += 512) {
-        const float4 now = gate;
-        gate_at(e + 512);
+      for (int e = 4 * threadIdx.x; e < p.group * D; e += 512) {
         const int r = e / D, d = e % D;
         float M = -INFINITY;
 #pragma unroll
         for (int u = 0; u < 4; ++u) M = fmaxf(M, bars->m[u][r]);
         const float Mu = (M == -INFINITY) ? 0.f : M;
         float lsum = 0.f;
-        float4 osum = make_float4(0.f, 0.f, 0.f, 0.f);
+        float4 osum = zero4();
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
           // A warp without keys here has nothing in the sum (its m is -inf).
@@ -549,11 +551,12 @@ __global__ void __launch_bounds__(PagedCfg<D>::THREADS, PagedCfg<D>::CTAS_PER_SM
           lsum += f * bars->l[u][r];
           osum = axpy(f, *reinterpret_cast<const float4*>(so + (u * 16 + r) * D + swizzle(r, d)), osum);
         }
-        if (whole) {
-          store_output(p, w.b, w.g * p.group + r, d, over(osum, lsum), now);
-        } else {
+        if constexpr (SPLIT) {
           *reinterpret_cast<float4*>(p.part_o + (part + r) * D + d) = osum;
           if (d == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * (part + r)) = make_float2(M, lsum);
+        } else {
+          const int h = w.g * p.group + r;
+          store_output(p, w.b, h, d, over(osum, lsum), p.gate ? load_gate(p, w.b, h, d) : zero4());
         }
       }
       fence_proxy_async_smem();
@@ -566,13 +569,13 @@ __global__ void __launch_bounds__(PagedCfg<D>::THREADS, PagedCfg<D>::CTAS_PER_SM
 
 constexpr int kJoinThreads = 256;
 
-// Joins the partials of (sequence, query head) blockIdx.x, if its keys were
-// cut between CTAs; a sequence without keys gets its zeros here. The parts
-// are the CTAs from the one with the pair's first tile to the one with its
-// last, each with the pair as its first or, in the first of them, as its
-// last. D / 4 threads read one part's row; the parts are dealt to such teams
-// in turn and joined in a fixed order. The lengths are read before the wait
-// for the main kernel (which does not write them).
+// Joins the partials of (sequence, query head) blockIdx.x. The parts are the
+// CTAs from the one with the pair's first tile to the one with its last.
+// D / 4 threads read one part's row; the parts are dealt to such teams in turn
+// and joined in a fixed order. The lengths are read before the wait for the
+// main kernel (which does not write them); so is everything else once, for
+// nothing, which brings the instructions and the gate on chip while the main
+// kernel's last CTAs still run.
 template <int D>
 __global__ void __launch_bounds__(kJoinThreads) decode_paged_join_kernel(const __grid_constant__ DecodePagedParams p) {
   constexpr int TEAM = D / 4, TEAMS = kJoinThreads / TEAM;
@@ -581,82 +584,71 @@ __global__ void __launch_bounds__(kJoinThreads) decode_paged_join_kernel(const _
   const int lane = threadIdx.x & 31;
   const int b = blockIdx.x / p.Hq, h = blockIdx.x % p.Hq;
   const int g = h / p.group, r = h % p.group;
-  long long total = 0, before = 0;  // tiles of all sequences, and of those before b
+  long long total = 0, before = 0;  // units of all sequences, and of those before b
   for (int b0 = 0; b0 < p.B; b0 += 32) {
-    const int n = b0 + lane < p.B ? tiles_of(p, b0 + lane) : 0;
+    const int n = b0 + lane < p.B ? units_of(tiles_of(p, b0 + lane)) : 0;
     total += __reduce_add_sync(0xffffffffu, n);
     before += __reduce_add_sync(0xffffffffu, b0 + lane < b ? n : 0);
   }
   const int tiles = tiles_of(p, b);
   const long long share = share_of(total * p.Hkv, p.n_ctas);
-  const long long lo = before * p.Hkv + (long long)g * tiles;
+  const long long lo = before * p.Hkv + (long long)g * units_of(tiles);
   const int team = threadIdx.x / TEAM, d = 4 * (threadIdx.x % TEAM);
-  const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (tiles == 0) {
-    grid_dep_wait();  // on every path: this grid is not to end before the main one
-    if (team == 0) store_output(p, b, h, d, zero, zero);
-    return;
-  }
-  const long long c0 = lo / share;
-  const int parts = (int)((lo + tiles - 1) / share - c0) + 1;
-  if (parts == 1) {  // finished by its CTA
-    grid_dep_wait();
-    return;
-  }
-  // Part i's row; the first CTA has the pair as its last unless it starts there.
-  const long long row0 = (2 * c0 + (c0 * share < lo ? 1 : 0)) * p.group + r;
-  auto row_of = [&](int i) { return i == 0 ? row0 : 2 * (c0 + i) * p.group + r; };
-  float4 gate = zero;
-  if (p.gate && team == 0) gate = load_gate(p, b, h, d);
-  grid_dep_wait();
-  float m = -INFINITY, l = 0.f;
-  float4 o = zero;
-  for (int i0 = team; i0 < parts; i0 += 4 * TEAMS) {
-    float2 ml[4];
-    float4 po[4];
+  const long long c0 = tiles > 0 ? lo / share : 0;
+  const int parts = tiles > 0 ? (int)((lo + tiles - 1) / share - c0) + 1 : 0;
+  const long long row0 = ((long long)b * p.Hkv + g + c0) * p.group + r;  // part i's row: row0 + i group
+#pragma unroll 1
+  for (int pass = 0; pass < 2; ++pass) {
+    if (pass == 1) grid_dep_wait();
+    float m = -INFINITY, l = 0.f;
+    float4 o = zero4();
+    for (int i0 = team; i0 < parts; i0 += 4 * TEAMS) {
+      float2 ml[4];
+      float4 po[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int i = i0 + k * TEAMS;
-      ml[k] = make_float2(-INFINITY, 0.f);
-      po[k] = zero;
-      if (i < parts) {
-        ml[k] = *reinterpret_cast<const float2*>(p.part_ml + 2 * row_of(i));
-        po[k] = *reinterpret_cast<const float4*>(p.part_o + row_of(i) * D + d);
+      for (int k = 0; k < 4; ++k) {
+        const int i = i0 + k * TEAMS;
+        const long long row = row0 + (long long)i * p.group;
+        ml[k] = i < parts ? __ldcg(reinterpret_cast<const float2*>(p.part_ml + 2 * row)) : make_float2(-INFINITY, 0.f);
+        po[k] = i < parts ? __ldcg(reinterpret_cast<const float4*>(p.part_o + row * D + d)) : zero4();
+      }
+      const float mn = fmaxf(fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)), m);
+      const float mu = mn == -INFINITY ? 0.f : mn;
+      const float f0 = ex2(m - mu);
+      m = mn;
+      l *= f0;
+      o = make_float4(o.x * f0, o.y * f0, o.z * f0, o.w * f0);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float f = ex2(ml[k].x - mu);
+        l = fmaf(f, ml[k].y, l);
+        o = axpy(f, po[k], o);
       }
     }
-    const float mn = fmaxf(fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)), m);
-    const float mu = mn == -INFINITY ? 0.f : mn;
-    const float f0 = ex2(m - mu);
-    m = mn;
-    l *= f0;
-    o = make_float4(o.x * f0, o.y * f0, o.z * f0, o.w * f0);
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float f = ex2(ml[k].x - mu);
-      l = fmaf(f, ml[k].y, l);
-      o = axpy(f, po[k], o);
+    s_o[team][threadIdx.x % TEAM] = o;
+    if (d == 0) {
+      s_m[team] = m;
+      s_l[team] = l;
     }
-  }
-  s_o[team][threadIdx.x % TEAM] = o;
-  if (d == 0) {
-    s_m[team] = m;
-    s_l[team] = l;
-  }
-  __syncthreads();
-  if (team != 0) return;
-  float M = -INFINITY;
+    __syncthreads();
+    if (team == 0) {
+      float M = -INFINITY;
 #pragma unroll
-  for (int u = 0; u < TEAMS; ++u) M = fmaxf(M, s_m[u]);
-  const float Mu = M == -INFINITY ? 0.f : M;
-  float lsum = 0.f;
-  float4 osum = zero;
+      for (int u = 0; u < TEAMS; ++u) M = fmaxf(M, s_m[u]);
+      const float Mu = M == -INFINITY ? 0.f : M;
+      float lsum = 0.f;
+      float4 osum = zero4();
 #pragma unroll
-  for (int u = 0; u < TEAMS; ++u) {
-    const float f = ex2(s_m[u] - Mu);
-    lsum = fmaf(f, s_l[u], lsum);
-    osum = axpy(f, s_o[u][threadIdx.x], osum);
+      for (int u = 0; u < TEAMS; ++u) {
+        const float f = ex2(s_m[u] - Mu);
+        lsum = fmaf(f, s_l[u], lsum);
+        osum = axpy(f, s_o[u][threadIdx.x], osum);
+      }
+      const float4 gate = p.gate ? load_gate(p, b, h, d) : zero4();
+      if (pass == 1) store_output(p, b, h, d, over(osum, lsum), gate);
+    }
+    __syncthreads();
   }
-  store_output(p, b, h, d, over(osum, lsum), gate);
 }
 
 constexpr int kWholeTiles = 8;

@@ -23,8 +23,9 @@ struct DecodePagedParams {
   int vec4;                // o and gate take accesses of four elements
   int B, Hq, Hkv, group;
   float scale_log2;
-  // Split form: partial results of each CTA's first and last (sequence, KV
-  // head), 2 per CTA: O [group, D] before its division and (m, l) [group, 2].
+  // Split form: the partial of pair x = b Hkv + g from CTA c is number x + c
+  // (each step along the stretches raises one of the two): O [group, D]
+  // before its division, and (m, l) [group, 2].
   float* part_o;
   float* part_ml;
   int n_ctas;
@@ -35,6 +36,7 @@ struct DecodePagedParams {
 // CTAs it may use for the current device, and its workspace.
 bool decode_paged_splits(int table_width, int page);
 int decode_paged_max_ctas(int D, int sms);
+inline size_t decode_paged_parts(int B, int Hkv, int n_ctas) { return (size_t)B * Hkv + n_ctas; }
 
 // tk / tv: 5-D maps (64 columns, slot in the page, D / 64, head, page) with
 // box (64, box_rows, D / 64, 1, 1). Returns 0 on success, -3 for an
