@@ -16,7 +16,7 @@
 // elements and their four rotate-half partners (8 contiguous elements past
 // rope_dim), so the rotation needs no exchange between threads; a norm's sum
 // of squares is a shuffle reduction over the row's threads. A warp takes
-// kSteps rows per thread of one token, its loads issued before the token's
+// STEPS rows per thread of one token, its loads issued before the token's
 // sequence, position and page are looked up, so the two latencies overlap;
 // the tables are read once per warp and reused for its heads.
 #include "rope_append_paged.cuh"
@@ -25,33 +25,48 @@ namespace b2a {
 
 namespace {
 
-constexpr int kSteps = 4;  // rows a thread handles
-
-// Four elements as loaded, and as floats.
+// Four elements as loaded, and as two pairs of floats (the arithmetic below is
+// on pairs: one instruction for two).
 template <typename Src>
 struct Four;
 template <>
 struct Four<float> {
   float4 v;
   __device__ __forceinline__ void load(const float* p) { v = *reinterpret_cast<const float4*>(p); }
-  __device__ __forceinline__ void get(float (&x)[4]) const { x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w; }
+  __device__ __forceinline__ void get(float2 (&x)[2]) const {
+    x[0] = make_float2(v.x, v.y);
+    x[1] = make_float2(v.z, v.w);
+  }
 };
 template <>
 struct Four<__nv_bfloat16> {
   uint2 v;
   __device__ __forceinline__ void load(const __nv_bfloat16* p) { v = *reinterpret_cast<const uint2*>(p); }
-  __device__ __forceinline__ void get(float (&x)[4]) const {
-    x[0] = __uint_as_float(v.x << 16), x[1] = __uint_as_float(v.x & 0xffff0000u);
-    x[2] = __uint_as_float(v.y << 16), x[3] = __uint_as_float(v.y & 0xffff0000u);
+  __device__ __forceinline__ void get(float2 (&x)[2]) const {
+    x[0] = make_float2(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u));
+    x[1] = make_float2(__uint_as_float(v.y << 16), __uint_as_float(v.y & 0xffff0000u));
   }
 };
 
-__device__ __forceinline__ void store4(__nv_bfloat16* p, const float (&x)[4]) {
-  *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]));
+// a b rounded by itself: with its rounding spelled out the product is not
+// contracted with the addition that follows.
+__device__ __forceinline__ float2 product(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z;\n\t"
+      "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "mul.rn.f32x2 z, x, y;\n\t"
+      "mov.b64 {%0, %1}, z;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+
+__device__ __forceinline__ void store4(__nv_bfloat16* p, const float2 (&x)[2]) {
+  *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16x2(x[0].x, x[0].y), pack_bf16x2(x[1].x, x[1].y));
 }
 
 template <typename T>
-__device__ __forceinline__ void load4(const void* p, long long at, float (&x)[4]) {
+__device__ __forceinline__ void load4(const void* p, long long at, float2 (&x)[2]) {
   Four<T> f;
   f.load(static_cast<const T*>(p) + at);
   f.get(x);
@@ -74,39 +89,46 @@ __device__ __forceinline__ int find_sequence(const int* cu, int B, long long n) 
   return lo;
 }
 
-template <typename Src, int D>
-__global__ void __launch_bounds__(256) rope_append_paged_kernel(const RopeAppendPagedParams p, int chunks) {
+constexpr int kWarps = 4;  // tokens of a block
+
+// Warp x of block (i, y) takes token i kWarps + x and chunk y of its rows: the
+// first q_chunks chunks are of q, the rest of k and v. A chunk is STEPS times
+// the 32 / (D / 8) rows a warp holds at a time.
+template <typename Src, int D, int STEPS>
+__global__ void __launch_bounds__(32 * kWarps)
+    rope_append_paged_kernel(const __grid_constant__ RopeAppendPagedParams p, int q_chunks) {
   constexpr int LPR = D / 8;       // lanes per row
   constexpr int ROWS = 32 / LPR;   // rows of a warp at a time
   const int lane = threadIdx.x & 31, part = lane % LPR;
-  const int heads = p.Hq + 2 * p.Hkv;
-  const long long warp = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (blockIdx.x == 0 && p.seqlens_out)
-    for (int b = threadIdx.x; b < p.B; b += 256)
+  const long long n = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5);  // token
+  if (blockIdx.x == 0 && blockIdx.y == 0 && p.seqlens_out)
+    for (int b = threadIdx.x; b < p.B; b += 32 * kWarps)
       p.seqlens_out[b] = (p.start_pos_arr ? p.start_pos_arr[b] : p.start_pos) + p.cu_seqlens[b + 1] - p.cu_seqlens[b];
-  const long long n = warp / chunks;  // token
   if (n >= p.N) return;
-  const int j0 = (int)(warp - n * chunks) * (kSteps * ROWS) + lane / LPR;  // step k takes row j0 + k ROWS
+  const bool q_rows = (int)blockIdx.y < q_chunks;  // q, else k and v
+  // Step s takes row j0 + s ROWS of q, or of k and then v.
+  const int j0 = ((int)blockIdx.y - (q_rows ? 0 : q_chunks)) * (STEPS * ROWS) + lane / LPR;
+  const int rows = q_rows ? p.Hq : 2 * p.Hkv;
 
   // This thread's two runs of four elements: o0 and its partner o1.
   const bool turns = 8 * part < p.rope_dim;
   const int o0 = turns ? 4 * part : 8 * part, o1 = turns ? 4 * part + p.rope_dim / 2 : 8 * part + 4;
-  Four<Src> raw[kSteps][2];
+  Four<Src> raw[STEPS][2];
+  {
+    const Src* first = static_cast<const Src*>(q_rows ? p.q : p.k) + n * (q_rows ? p.qs[0] : p.ks[0]);
+    const Src* v = static_cast<const Src*>(p.v) + n * p.vs[0];
+    const long long step = q_rows ? p.qs[1] : p.ks[1];
 #pragma unroll
-  for (int k = 0; k < kSteps; ++k) {
-    const int j = j0 + k * ROWS;
-    const Src* src;
-    if (j < p.Hq)
-      src = static_cast<const Src*>(p.q) + n * p.qs[0] + j * p.qs[1];
-    else if (j < p.Hq + p.Hkv)
-      src = static_cast<const Src*>(p.k) + n * p.ks[0] + (j - p.Hq) * p.ks[1];
-    else
-      src = static_cast<const Src*>(p.v) + n * p.vs[0] + (j - p.Hq - p.Hkv) * p.vs[1];
-    if (j < heads) {
-      raw[k][0].load(src + o0);
-      raw[k][1].load(src + o1);
-    } else {
-      raw[k][0].v = raw[k][1].v = {};
+    for (int s = 0; s < STEPS; ++s) {
+      const int j = j0 + s * ROWS;
+      const Src* src = first + j * step;
+      if (!q_rows && j >= p.Hkv) src = v + (j - p.Hkv) * p.vs[1];
+      if (j < rows) {
+        raw[s][0].load(src + o0);
+        raw[s][1].load(src + o1);
+      } else {
+        raw[s][0].v = raw[s][1].v = {};
+      }
     }
   }
 
@@ -114,75 +136,94 @@ __global__ void __launch_bounds__(256) rope_append_paged_kernel(const RopeAppend
   const int b = find_sequence(p.cu_seqlens, p.B, n);
   const int c0 = p.cu_seqlens[b], c1 = p.cu_seqlens[b + 1];
   if (n < c0 || n >= c1) return;  // a row outside every sequence
-  const long long pos = (long long)(p.start_pos_arr ? p.start_pos_arr[b] : p.start_pos) + (n - c0);
+  const long long at = (long long)(p.start_pos_arr ? p.start_pos_arr[b] : p.start_pos) + (n - c0);
+  const bool counts = at >= 0 && at <= 0x7fffffff;
+  const unsigned pos = counts ? (unsigned)at : 0u;
+  const bool in_table = counts && (p.rope_dim == 0 || pos < (unsigned)p.max_pos);
+  unsigned slot = 0;
   int page_id = -1;
-  long long slot = 0;
-  if (pos >= 0) {
-    const long long e = pos / p.page;
-    slot = pos - e * p.page;
-    if (e < p.table_width) page_id = p.block_table[b * p.table_ld + e];
+  if (!q_rows) {
+    const unsigned entry = pos / (unsigned)p.page;
+    slot = pos - entry * p.page;
+    if (counts && entry < (unsigned)p.table_width) page_id = p.block_table[b * p.table_ld + entry];
   }
-  const bool in_table = pos >= 0 && (p.rope_dim == 0 || pos < p.max_pos);
-  const bool in_pool = pos >= 0 && page_id >= 0 && page_id < p.n_pages;
-  if ((!in_table || !in_pool) && p.err && lane == 0) atomicOr(p.err, kErrBadArgs);
+  const bool in_pool = page_id >= 0 && page_id < p.n_pages;
+  if ((!in_table || !(q_rows || in_pool)) && p.err && lane == 0) atomicOr(p.err, kErrBadArgs);
 
-  float cos0[4], cos1[4], sin0[4], sin1[4];
+  float2 cos0[2], cos1[2], sin0[2], sin1[2];
   if (turns && in_table) {
-    const long long at = pos * p.rope_dim;
+    const long long t = (long long)pos * p.rope_dim;
     if (p.tab_fp32) {
-      load4<float>(p.cos, at + o0, cos0), load4<float>(p.cos, at + o1, cos1);
-      load4<float>(p.sin, at + o0, sin0), load4<float>(p.sin, at + o1, sin1);
+      load4<float>(p.cos, t + o0, cos0), load4<float>(p.cos, t + o1, cos1);
+      load4<float>(p.sin, t + o0, sin0), load4<float>(p.sin, t + o1, sin1);
     } else {
-      load4<__nv_bfloat16>(p.cos, at + o0, cos0), load4<__nv_bfloat16>(p.cos, at + o1, cos1);
-      load4<__nv_bfloat16>(p.sin, at + o0, sin0), load4<__nv_bfloat16>(p.sin, at + o1, sin1);
+      load4<__nv_bfloat16>(p.cos, t + o0, cos0), load4<__nv_bfloat16>(p.cos, t + o1, cos1);
+      load4<__nv_bfloat16>(p.sin, t + o0, sin0), load4<__nv_bfloat16>(p.sin, t + o1, sin1);
     }
   }
+  const void* weights = q_rows ? p.q_norm : p.k_norm;
+  float2 w0[2], w1[2];
+  if (weights) load4<Src>(weights, o0, w0), load4<Src>(weights, o1, w1);
 
-#pragma unroll
-  for (int k = 0; k < kSteps; ++k) {
-    const int j = j0 + k * ROWS;
-    const bool is_q = j < p.Hq, is_k = !is_q && j < p.Hq + p.Hkv;
-    const int h = is_q ? j : (is_k ? j - p.Hq : j - p.Hq - p.Hkv);
-    float x[4], y[4];
-    raw[k][0].get(x);
-    raw[k][1].get(y);
-    if (p.q_norm || p.k_norm) {
-      float ss = 0.f;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) ss = __fmaf_rn(x[e], x[e], __fmaf_rn(y[e], y[e], ss));
+  // RMSNorm (with a weight) and rotation of one row's two runs.
+  auto turn = [&](float2 (&x)[2], float2 (&y)[2], bool is_v) {
+    if (weights) {
+      const float2 s2 =
+          __ffma2_rn(x[0], x[0], __ffma2_rn(x[1], x[1], __ffma2_rn(y[0], y[0], __fmul2_rn(y[1], y[1]))));
+      float ss = s2.x + s2.y;
 #pragma unroll
       for (int off = LPR / 2; off > 0; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
-      const void* wp = is_q ? p.q_norm : (is_k ? p.k_norm : nullptr);
-      if (wp) {
-        const float rms = rsqrtf(__fadd_rn(__fdiv_rn(ss, (float)D), p.norm_eps));
-        float w0[4], w1[4];
-        load4<Src>(wp, o0, w0), load4<Src>(wp, o1, w1);
+      if (!is_v) {
+        const float rms = rsqrtf(__fmaf_rn(ss, 1.f / D, p.norm_eps));
+        const float2 rms2 = make_float2(rms, rms);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          x[e] = __fmul_rn(__fmul_rn(x[e], rms), w0[e]);
-          y[e] = __fmul_rn(__fmul_rn(y[e], rms), w1[e]);
+        for (int e = 0; e < 2; ++e) {
+          x[e] = __fmul2_rn(__fmul2_rn(x[e], rms2), w0[e]);
+          y[e] = __fmul2_rn(__fmul2_rn(y[e], rms2), w1[e]);
         }
       }
     }
-    if ((is_q || is_k) && turns && in_table) {
+    if (turns && in_table && !is_v) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float a = x[e], c = y[e];
-        x[e] = __fadd_rn(__fmul_rn(a, cos0[e]), __fmul_rn(-c, sin0[e]));
-        y[e] = __fadd_rn(__fmul_rn(c, cos1[e]), __fmul_rn(a, sin1[e]));
+      for (int e = 0; e < 2; ++e) {
+        const float2 a = x[e], c = y[e];
+        x[e] = __fadd2_rn(product(a, cos0[e]), product(make_float2(-c.x, -c.y), sin0[e]));
+        y[e] = __fadd2_rn(product(c, cos1[e]), product(a, sin1[e]));
       }
     }
-    if (j >= heads) continue;
-    // A token without a place in the tables or the pool is not written where
-    // it would need it.
-    if (is_q) {
-      __nv_bfloat16* dst = p.q_out + (n * p.Hq + h) * D;
-      if (in_table) store4(dst + o0, x), store4(dst + o1, y);
-    } else if (in_pool && (in_table || !is_k)) {
-      const long long* ps = is_k ? p.kps : p.vps;
-      __nv_bfloat16* dst = (is_k ? p.k_pages : p.v_pages) + page_id * ps[0] + h * ps[1] + slot * ps[2];
+  };
+
+  // A token without a place in the tables or the pool is not written where it
+  // would need it.
+  if (q_rows) {
+    __nv_bfloat16* dst = p.q_out + (n * p.Hq + j0) * D;
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+      float2 x[2], y[2];
+      raw[s][0].get(x);
+      raw[s][1].get(y);
+      turn(x, y, false);
+      if (in_table && j0 + s * ROWS < rows) {
+        store4(dst + s * ROWS * D + o0, x);
+        store4(dst + s * ROWS * D + o1, y);
+      }
+    }
+  } else {
+    __nv_bfloat16* k_dst = p.k_pages + page_id * p.kps[0] + slot * p.kps[2];
+    __nv_bfloat16* v_dst = p.v_pages + page_id * p.vps[0] + slot * p.vps[2];
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+      const int j = j0 + s * ROWS;
+      const bool is_v = j >= p.Hkv;
+      const int h = is_v ? j - p.Hkv : j;
+      float2 x[2], y[2];
+      raw[s][0].get(x);
+      raw[s][1].get(y);
+      turn(x, y, is_v);
+      if (!in_pool || !(in_table || is_v) || j >= rows) continue;
+      __nv_bfloat16* dst = is_v ? v_dst + h * p.vps[1] : k_dst + h * p.kps[1];
       store4(dst + o0, x), store4(dst + o1, y);
-      __nv_bfloat16* packed = is_k ? p.k_out : p.v_out;
+      __nv_bfloat16* packed = is_v ? p.v_out : p.k_out;
       if (packed) {
         packed += (n * p.Hkv + h) * D;
         store4(packed + o0, x), store4(packed + o1, y);
@@ -191,14 +232,24 @@ __global__ void __launch_bounds__(256) rope_append_paged_kernel(const RopeAppend
   }
 }
 
+template <typename Src, int D, int STEPS>
+int launch_steps(const RopeAppendPagedParams& p, cudaStream_t st) {
+  constexpr int ROWS = 32 / (D / 8);
+  const long long blocks = (p.N + kWarps - 1) / kWarps;
+  const int q_chunks = (p.Hq + STEPS * ROWS - 1) / (STEPS * ROWS);
+  const int chunks = q_chunks + (2 * p.Hkv + STEPS * ROWS - 1) / (STEPS * ROWS);
+  if (blocks <= 0 || blocks > 0x7fffffffLL || chunks > 65535) return -2;
+  rope_append_paged_kernel<Src, D, STEPS>
+      <<<dim3((unsigned)blocks, (unsigned)chunks), 32 * kWarps, 0, st>>>(p, q_chunks);
+  return cudaGetLastError() == cudaSuccess ? 0 : -1;
+}
+
+// Four rows per thread spread a token's lookups over more rows; few tokens get
+// one, so that their rows are in more warps at once.
 template <typename Src, int D>
 int launch_t(const RopeAppendPagedParams& p, cudaStream_t st) {
-  constexpr int ROWS = 32 / (D / 8);
-  const int chunks = (p.Hq + 2 * p.Hkv + kSteps * ROWS - 1) / (kSteps * ROWS);
-  const long long blocks = (p.N * chunks + 7) / 8;
-  if (blocks <= 0 || blocks > 0x7fffffffLL) return -2;
-  rope_append_paged_kernel<Src, D><<<(unsigned)blocks, 256, 0, st>>>(p, chunks);
-  return cudaGetLastError() == cudaSuccess ? 0 : -1;
+  const long long row_warps = p.N * ((p.Hq + 2 * p.Hkv) / (32 / (D / 8)) + 1);
+  return row_warps >= 148 * 32 ? launch_steps<Src, D, 4>(p, st) : launch_steps<Src, D, 1>(p, st);
 }
 
 template <typename Src>
