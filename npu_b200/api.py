@@ -18,11 +18,6 @@ import torch
 from . import _lib
 
 
-# The current stream's handle of a device index.
-_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else \
-    lambda index: torch.cuda.current_stream(index).cuda_stream
-
-
 def _stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
@@ -435,41 +430,21 @@ def rope_append(
     return q_out
 
 
-class _SameDevice:
-    __slots__ = ()
-
-    def __enter__(self):
-        return self
-
-    def __exit__(self, *exc):
-        return False
-
-
-_SAME_DEVICE = _SameDevice()
-
-
-def _on(device: torch.device):
-    """torch.cuda.device(device), without its cost when that device is current."""
-    return _SAME_DEVICE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+def _serving():
+    """The compiled binding of the serving operators (loaded with the library, never replaced by a fallback)."""
+    global _serving_module
+    if _serving_module is None:
+        _lib.load()
+        try:
+            from . import _serving as module
+        except ImportError as e:
+            raise _lib.B2AError(_lib.B2A_ERR_CUDA,
+                                f"_serving is not built (run `python -m npu_b200.build`): {e}") from e
+        _serving_module = module
+    return _serving_module
 
 
-def _need_int32(name: str, t: torch.Tensor, numel: int, device: torch.device) -> None:
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.device != device or t.numel() != numel \
-            or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous int32 tensor of {numel} on the inputs' device")
-
-
-def _need_pool(name: str, t: torch.Tensor, device: torch.device) -> None:
-    _need_cuda_bf16(name, t, 4)
-    if t.device != device:
-        raise ValueError(f"{name} must be on the inputs' device")
-
-
-def _need_table(t: torch.Tensor, batch: int, device: torch.device) -> None:
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.device != device or t.dim() != 2 \
-            or t.shape[0] != batch or t.stride(1) != 1:
-        raise ValueError(f"block_table must be an int32 tensor [{batch}, pages] on the inputs' device with a "
-                         "contiguous last dim")
+_serving_module = None
 
 
 def prefill_varlen(
@@ -498,46 +473,8 @@ def prefill_varlen(
     natural-log LSE [Hq, Nq] if return_lse); `gate` ([Nq, Hq, D], fp32 or bf16)
     multiplies the output by sigmoid(gate) as in `prefill`.
     """
-    _need_cuda_bf16("q", q, 3)
-    _need_cuda_bf16("k", k, 3)
-    _need_cuda_bf16("v", v, 3)
-    Nq, Hq, D = q.shape
-    Nk, Hkv, Dk = k.shape
-    device = q.device
-    if Dk != D or v.shape != k.shape or k.device != device or v.device != device:
-        raise ValueError(f"shape or device mismatch q{tuple(q.shape)} k{tuple(k.shape)} v{tuple(v.shape)}")
-    B = cu_seqlens_q.numel() - 1
-    if B < 1:
-        raise ValueError("cu_seqlens_q must hold at least two offsets")
-    _need_int32("cu_seqlens_q", cu_seqlens_q, B + 1, device)
-    if cu_seqlens_k is None:
-        if Nk != Nq:
-            raise ValueError(f"k has {Nk} rows and q {Nq}: cu_seqlens_k is needed")
-        cu_seqlens_k = cu_seqlens_q
-    else:
-        _need_int32("cu_seqlens_k", cu_seqlens_k, B + 1, device)
-    if out_dtype not in (torch.float32, torch.bfloat16):
-        raise ValueError("out_dtype must be float32 or bfloat16")
-    if out is None:
-        out = torch.empty((Nq, Hq, D), dtype=out_dtype, device=device)
-    elif out.dtype != out_dtype or out.shape != q.shape or out.stride(-1) != 1 or out.device != device:
-        raise ValueError("out must match [Nq, Hq, D], out_dtype and q's device, with a contiguous last dim")
-    lse = torch.empty((Hq, Nq), dtype=torch.float32, device=device) if return_lse else None
-    if gate is not None:
-        _check_gate(gate, (Nq, Hq, D), device)
-    ll2 = _lib.ll2
-    with _on(device):
-        rc = _lib.load().b2a_prefill_varlen(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), gate.data_ptr() if gate is not None else None, out.data_ptr(),
-            lse.data_ptr() if return_lse else None, cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(),
-            B, Nq, Nk, Hq, Hkv, D, ll2(*q.stride()[:2]), ll2(*k.stride()[:2]), ll2(*v.stride()[:2]),
-            ll2(*gate.stride()[:2]) if gate is not None else None, ll2(*out.stride()[:2]),
-            1 if gate is not None and gate.dtype == torch.bfloat16 else 0,
-            1.0 / math.sqrt(D) if scale is None else float(scale), 1 if causal else 0,
-            1 if out_dtype == torch.float32 else 0, _raw_stream(device.index),
-        )
-    _lib.check(rc, "b2a_prefill_varlen")
-    return (out, lse) if return_lse else out
+    return _serving().prefill_varlen(q, k, v, cu_seqlens_q, cu_seqlens_k, scale, causal, out_dtype, out, return_lse,
+                                     gate)
 
 
 def decode_paged_workspace_bytes(B: int, Hq: int, Hkv: int, D: int) -> int:
@@ -569,44 +506,7 @@ def decode_paged(
     decode_paged_workspace_bytes) or torch's allocator. `gate` ([B, Hq, D])
     as in `decode`.
     """
-    _need_cuda_bf16("q", q, 3)
-    B, Hq, D = q.shape
-    device = q.device
-    _need_pool("k_pages", k_pages, device)
-    _need_pool("v_pages", v_pages, device)
-    n_pages, Hkv, page, Dk = k_pages.shape
-    if Dk != D or v_pages.shape != k_pages.shape:
-        raise ValueError(f"shape mismatch q{tuple(q.shape)} k_pages{tuple(k_pages.shape)} "
-                         f"v_pages{tuple(v_pages.shape)}")
-    _need_table(block_table, B, device)
-    _need_int32("seqlens", seqlens, B, device)
-    if out is None:
-        if out_dtype not in (torch.float32, torch.bfloat16):
-            raise ValueError("out_dtype must be float32 or bfloat16")
-        out = torch.empty((B, Hq, D), dtype=out_dtype, device=device)
-    elif out.dtype != out_dtype or out.shape != q.shape or out.stride(-1) != 1 or out.device != device:
-        raise ValueError("out must match [B, Hq, D], out_dtype and q's device, with a contiguous last dim")
-    if gate is not None:
-        _check_gate(gate, (B, Hq, D), device)
-    lib = _lib.load()
-    need = int(lib.b2a_decode_paged_workspace_bytes(B, Hq, Hkv, D))
-    if workspace is None:
-        workspace = torch.empty(max(need, 16), dtype=torch.uint8, device=device)
-    elif workspace.device != device or workspace.numel() * workspace.element_size() < need:
-        raise ValueError(f"workspace must be a CUDA tensor of at least {need} bytes on q's device")
-    ll2, ll3 = _lib.ll2, _lib.ll3
-    with _on(device):
-        rc = lib.b2a_decode_paged(
-            q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(), block_table.stride(0),
-            block_table.shape[1], seqlens.data_ptr(), gate.data_ptr() if gate is not None else None, out.data_ptr(),
-            B, Hq, Hkv, n_pages, page, D, ll2(*q.stride()[:2]), ll3(*k_pages.stride()[:3]),
-            ll3(*v_pages.stride()[:3]), ll2(*gate.stride()[:2]) if gate is not None else None,
-            ll2(*out.stride()[:2]), 1 if gate is not None and gate.dtype == torch.bfloat16 else 0,
-            1.0 / math.sqrt(D) if scale is None else float(scale), 1 if out_dtype == torch.float32 else 0,
-            workspace.data_ptr(), need, _raw_stream(device.index),
-        )
-    _lib.check(rc, "b2a_decode_paged")
-    return out
+    return _serving().decode_paged(q, k_pages, v_pages, block_table, seqlens, scale, out_dtype, workspace, out, gate)
 
 
 def rope_append_paged(
@@ -644,74 +544,9 @@ def rope_append_paged(
     return_kv (q, k, v): k rotated and v as packed bf16 [N, Hkv, D] for
     `prefill_varlen` (v itself when it is bf16 already).
     """
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dim() != 3 or t.stride(-1) != 1:
-            raise ValueError(f"{name} must be a CUDA [N, H, D] tensor with a contiguous last dim")
-    N, Hq, D = q.shape
-    Hkv = k.shape[1]
-    device, dtype = q.device, q.dtype
-    if k.shape != (N, Hkv, D) or v.shape != k.shape:
-        raise ValueError(f"shape mismatch q{tuple(q.shape)} k{tuple(k.shape)} v{tuple(v.shape)}")
-    if dtype not in (torch.float32, torch.bfloat16) or k.dtype != dtype or v.dtype != dtype:
-        raise ValueError("q, k, v must share one dtype, float32 or bfloat16")
-    if k.device != device or v.device != device or cos.device != device or sin.device != device:
-        raise ValueError("q, k, v, cos and sin must be on one device")
-    rope_dim = D if rope_dim is None else int(rope_dim)
-    if cos.dtype not in (torch.float32, dtype) or sin.dtype != cos.dtype or not cos.is_contiguous() \
-            or not sin.is_contiguous() or cos.dim() != 2 or cos.shape[1] != rope_dim or sin.shape != cos.shape:
-        raise ValueError("cos/sin must be contiguous [max_pos, rope_dim] tensors, float32 or in q's dtype")
-    _need_pool("k_pages", k_pages, device)
-    _need_pool("v_pages", v_pages, device)
-    n_pages, Hc, page, Dc = k_pages.shape
-    if (Hc, Dc) != (Hkv, D) or v_pages.shape != k_pages.shape:
-        raise ValueError(f"cache shape {tuple(k_pages.shape)} does not fit k{tuple(k.shape)}")
-    B = cu_seqlens.numel() - 1
-    if B < 1:
-        raise ValueError("cu_seqlens must hold at least two offsets")
-    _need_int32("cu_seqlens", cu_seqlens, B + 1, device)
-    _need_table(block_table, B, device)
-    if start_pos_per_batch is not None:
-        _need_int32("start_pos_per_batch", start_pos_per_batch, B, device)
-    if seqlens_out is not None:
-        _need_int32("seqlens_out", seqlens_out, B, device)
-    for name, w in (("q_norm", q_norm), ("k_norm", k_norm)):
-        if w is not None and (w.dtype != dtype or w.device != device or w.shape != (D,) or not w.is_contiguous()):
-            raise ValueError(f"{name} must be a contiguous [D] tensor in q's dtype on q's device")
-    if q_out is None:
-        q_out = torch.empty((N, Hq, D), dtype=torch.bfloat16, device=device)
-    elif q_out.dtype != torch.bfloat16 or q_out.shape != q.shape or not q_out.is_contiguous() \
-            or q_out.device != device:
-        raise ValueError("q_out must be a contiguous bf16 [N, Hq, D] tensor on q's device")
-    bf16 = dtype == torch.bfloat16
-    k_out = torch.empty((N, Hkv, D), dtype=torch.bfloat16, device=device) if return_kv else None
-    v_out = torch.empty((N, Hkv, D), dtype=torch.bfloat16, device=device) if return_kv and not bf16 else None
-    ll2, ll3 = _lib.ll2, _lib.ll3
-    with _on(device):
-        rc = _lib.load().b2a_rope_append_paged(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), ll2(*q.stride()[:2]), ll2(*k.stride()[:2]),
-            ll2(*v.stride()[:2]), 1 if bf16 else 0, q_norm.data_ptr() if q_norm is not None else None,
-            k_norm.data_ptr() if k_norm is not None else None, float(norm_eps), cos.data_ptr(), sin.data_ptr(),
-            1 if cos.dtype == torch.float32 else 0, cos.shape[0], rope_dim, q_out.data_ptr(),
-            k_out.data_ptr() if k_out is not None else None, v_out.data_ptr() if v_out is not None else None,
-            k_pages.data_ptr(), v_pages.data_ptr(), ll3(*k_pages.stride()[:3]), ll3(*v_pages.stride()[:3]),
-            block_table.data_ptr(), block_table.stride(0), block_table.shape[1], n_pages, page,
-            cu_seqlens.data_ptr(), B, N, Hq, Hkv, D, int(start_pos),
-            start_pos_per_batch.data_ptr() if start_pos_per_batch is not None else None,
-            seqlens_out.data_ptr() if seqlens_out is not None else None, _raw_stream(device.index),
-        )
-    _lib.check(rc, "b2a_rope_append_paged")
-    if return_kv:
-        return q_out, k_out, (v if bf16 else v_out)
-    return q_out
-
-
-def _per_row(name: str, value, rows: int, dtype: torch.dtype, device: torch.device):
-    """(device pointer or None, value for every row) of a sampling setting."""
-    if isinstance(value, torch.Tensor):
-        if value.dtype != dtype or value.device != device or value.shape != (rows,) or not value.is_contiguous():
-            raise ValueError(f"{name} must be a number or a contiguous {dtype} tensor [{rows}] on the logits' device")
-        return value.data_ptr(), 0
-    return None, value
+    return _serving().rope_append_paged(q, k, v, cos, sin, k_pages, v_pages, block_table, cu_seqlens, start_pos,
+                                        start_pos_per_batch, seqlens_out, q_out, q_norm, k_norm, norm_eps, rope_dim,
+                                        return_kv)
 
 
 def sample(
@@ -738,35 +573,7 @@ def sample(
     w_i / (sum of the kept w). T <= 0 (or no noise) gives the argmax. NaN logits
     count as -inf; a row without a logit above -inf gives -1.
     """
-    if not isinstance(logits, torch.Tensor) or not logits.is_cuda or logits.dim() != 2 or logits.stride(1) != 1 \
-            or logits.dtype not in (torch.float32, torch.bfloat16):
-        raise ValueError("logits must be a CUDA float32 or bfloat16 tensor [R, V] with a contiguous last dim")
-    R, V = logits.shape
-    device = logits.device
-    if noise is not None:
-        if not isinstance(noise, torch.Tensor) or noise.dtype != torch.float32 or noise.device != device \
-                or noise.shape != logits.shape or noise.stride(1) != 1:
-            raise ValueError(f"noise must be a float32 tensor [{R}, {V}] on the logits' device with a contiguous "
-                             "last dim")
-    elif isinstance(temperature, torch.Tensor) or temperature > 0:
-        raise ValueError("a temperature above 0 needs noise")
-    t_ptr, t_all = _per_row("temperature", temperature, R, torch.float32, device)
-    k_ptr, k_all = _per_row("top_k", top_k, R, torch.int32, device)
-    p_ptr, p_all = _per_row("top_p", top_p, R, torch.float32, device)
-    m_ptr, m_all = _per_row("min_p", min_p, R, torch.float32, device)
-    if out is None:
-        out = torch.empty(R, dtype=torch.int64, device=device)
-    elif out.dtype != torch.int64 or out.shape != (R,) or not out.is_contiguous() or out.device != device:
-        raise ValueError(f"out must be a contiguous int64 tensor [{R}] on the logits' device")
-    with _on(device):
-        rc = _lib.load().b2a_sample(
-            logits.data_ptr(), logits.stride(0) if R > 1 else V, 1 if logits.dtype == torch.bfloat16 else 0,
-            noise.data_ptr() if noise is not None else None, noise.stride(0) if noise is not None and R > 1 else V,
-            R, V, t_ptr, float(t_all), k_ptr, int(k_all), p_ptr, float(p_all), m_ptr, float(m_all),
-            out.data_ptr(), _raw_stream(device.index),
-        )
-    _lib.check(rc, "b2a_sample")
-    return out
+    return _serving().sample(logits, noise, temperature, top_k, top_p, min_p, out)
 
 
 def device_error(clear: bool = True, device: Optional[torch.device] = None) -> int:

@@ -1,4 +1,5 @@
-"""Build recipe for libb2attn.so (sm_100a only), written next to this file.
+"""Build recipe for libb2attn.so (sm_100a only) and the Python module _serving
+that binds its serving operators to torch tensors, written next to this file.
 
     python -m npu_b200.build            # build if sources are newer
     python -m npu_b200.build --force    # rebuild
@@ -22,6 +23,8 @@ CSRC = PKG / "csrc"
 INCLUDE = ROOT / "include"
 LIB = PKG / "libb2attn.so"
 BUILD_DIR = PKG / "_build"
+BINDING = PKG / "_serving.so"
+BINDING_SOURCE = CSRC / "serving_binding.cpp"
 
 SOURCES = ["capi.cu", "capi_serving.cu", "prefill.cu", "prefill_pair.cu", "prefill_d256.cu", "decode.cu", "decode_noalloc.cu",
            "rope_append.cu", "rope_append_paged.cu", "decode_paged.cu", "sample.cu", "diag.cu", "host_pipeline.cu"]
@@ -48,10 +51,40 @@ def _stale() -> bool:
     return any(p.stat().st_mtime > t for p in deps)
 
 
+def _build_binding(force: bool) -> None:
+    """Compile the torch binding against libb2attn.so (found beside it at run time)."""
+    deps = [BINDING_SOURCE, INCLUDE / "b2attn.h", Path(__file__)]
+    if not force and BINDING.exists() and all(p.stat().st_mtime <= BINDING.stat().st_mtime for p in deps):
+        return
+    import sysconfig
+
+    import torch
+
+    root = Path(torch.__file__).resolve().parent
+    nvcc = Path(_nvcc()).resolve()
+    tmp = BINDING.with_suffix(".so.tmp")
+    cmd = [os.environ.get("CXX") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-w",
+           "-I", str(INCLUDE), "-isystem", str(root / "include"),
+           "-isystem", str(root / "include" / "torch" / "csrc" / "api" / "include"),
+           "-isystem", sysconfig.get_paths()["include"], "-isystem", str(nvcc.parent.parent / "include"),
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           str(BINDING_SOURCE), "-o", str(tmp), "-L", str(PKG), "-l:libb2attn.so", "-L", str(root / "lib"),
+           "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"building {BINDING.name} failed:\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, BINDING)
+
+
 def build(force: bool = False, verbose: bool = False) -> Path:
-    """Compile every .cu under csrc/ for sm_100a and link libb2attn.so."""
-    if not force and not _stale():
-        return LIB
+    """Compile every .cu under csrc/ for sm_100a, link libb2attn.so and build the torch binding."""
+    if force or _stale():
+        _build_library(verbose)
+    _build_binding(force)
+    return LIB
+
+
+def _build_library(verbose: bool) -> None:
     nvcc = _nvcc()
     BUILD_DIR.mkdir(exist_ok=True)
     objs = []
@@ -72,7 +105,6 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     if r.returncode != 0:
         raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, LIB)
-    return LIB
 
 
 if __name__ == "__main__":
