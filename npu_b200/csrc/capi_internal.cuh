@@ -7,6 +7,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <atomic>
+
 namespace b2a {
 
 // Current device is sm_100 and its error word is known: B2A_OK and *err, or
@@ -32,6 +34,29 @@ inline bool api_strides_ok(const long long* s, int n, long long mult) {
 }
 
 inline size_t api_align256(size_t x) { return (x + 255) & ~(size_t)255; }
+
+// Runs `prepare` (which sets a kernel's attributes) once per device and
+// kernel: the runtime's attribute calls cost about a microsecond each, and
+// attributes stay with the kernel. A launch that failed forgets it, so that
+// the next call prepares again (a reset device has lost its attributes).
+struct OncePerDevice {
+  std::atomic<unsigned long long> done{0};
+  template <typename F>
+  bool operator()(F&& prepare) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return prepare();
+    const unsigned long long bit = 1ull << dev;
+    if (done.load(std::memory_order_acquire) & bit) return true;
+    if (!prepare()) return false;
+    done.fetch_or(bit, std::memory_order_release);
+    return true;
+  }
+  int launched(cudaError_t e) {
+    if (e == cudaSuccess) return 0;
+    done.store(0, std::memory_order_release);
+    return -1;
+  }
+};
 
 constexpr float kApiLog2e = 1.4426950408889634f;
 

@@ -29,6 +29,7 @@
 // Slots of a page past the sequence's end may hold anything, NaN included:
 // their scores are replaced by -inf and their V rows by zeros in shared
 // memory before they are used.
+#include "capi_internal.cuh"
 #include "decode_paged.cuh"
 
 namespace b2a {
@@ -657,12 +658,14 @@ template <int D, int NT, bool SPLIT>
 int launch_main(const CUtensorMap& tk, const CUtensorMap& tv, const DecodePagedParams& p, long long n,
                 cudaStream_t st) {
   using C = PagedCfg<D>;
-  if (cudaFuncSetAttribute(decode_paged_kernel<D, NT, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           C::SMEM_BYTES) != cudaSuccess)
+  static OncePerDevice once;
+  if (n > 0x7fffffffLL || !once([] {
+        return cudaFuncSetAttribute(decode_paged_kernel<D, NT, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    C::SMEM_BYTES) == cudaSuccess;
+      }))
     return -1;
-  if (n > 0x7fffffffLL) return -2;
   decode_paged_kernel<D, NT, SPLIT><<<(unsigned)n, C::THREADS, C::SMEM_BYTES, st>>>(tk, tv, p);
-  return cudaGetLastError() == cudaSuccess ? 0 : -1;
+  return once.launched(cudaGetLastError());
 }
 
 template <int D>

@@ -3,6 +3,7 @@
 // of this file and is called from capi.cu.
 #include <cstdlib>
 
+#include "capi_internal.cuh"
 #include "packed.cuh"
 #include "prefill.cuh"
 #include "softmax.cuh"
@@ -661,18 +662,20 @@ template <int D, int NQT, bool PAIRS, bool PACKED = false>
 static int launch_prefill_t(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
                             const PrefillParams& p, cudaStream_t st) {
   using C = PrefillCfg<D, NQT>;
-  cudaError_t e = cudaFuncSetAttribute(fa_prefill_kernel<D, NQT, PAIRS, PACKED>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       C::SMEM_BYTES);
-  if (e != cudaSuccess) return -1;
-  // The in-kernel register split needs at least MIN_LAUNCH_REGS per thread.
-  cudaFuncAttributes fa{};
-  if (cudaFuncGetAttributes(&fa, fa_prefill_kernel<D, NQT, PAIRS, PACKED>) != cudaSuccess || fa.numRegs < C::MIN_LAUNCH_REGS)
-    return -1;
+  const auto kernel = fa_prefill_kernel<D, NQT, PAIRS, PACKED>;
+  auto prepare = [&] {
+    // The in-kernel register split needs at least MIN_LAUNCH_REGS per thread.
+    cudaFuncAttributes fa{};
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES) == cudaSuccess &&
+           cudaFuncGetAttributes(&fa, kernel) == cudaSuccess && fa.numRegs >= C::MIN_LAUNCH_REGS;
+  };
+  static OncePerDevice once;
+  if (!once(prepare)) return -1;
   // One CTA per work item (query blocks x query heads, or x head pairs).
   const long long nblk = (long long)p.n_qblk * (PACKED ? 1 : p.B) * (p.head_pairs ? p.Hq / 2 : p.Hq);
   if (nblk <= 0 || nblk > 0x7fffffffLL) return -2;
-  fa_prefill_kernel<D, NQT, PAIRS, PACKED><<<(unsigned)nblk, C::THREADS, C::SMEM_BYTES, st>>>(tq, tk, tv, p);
-  return cudaGetLastError() == cudaSuccess ? 0 : -1;
+  kernel<<<(unsigned)nblk, C::THREADS, C::SMEM_BYTES, st>>>(tq, tk, tv, p);
+  return once.launched(cudaGetLastError());
 }
 
 // One-tile CTAs (two per SM) pay off when a CTA sees few key blocks, so that

@@ -14,6 +14,7 @@
 // MMA order: S(0), S(1), then per block j: PV(j), S(j+2). While the softmax
 // warpgroup turns S(j) into P(j), the tensor core runs PV(j-1) and S(j+1).
 // Warps: 0 TMA, 1 TMEM + MMA issue, 2-3 idle, 4-7 softmax + epilogue.
+#include "capi_internal.cuh"
 #include "packed.cuh"
 #include "prefill.cuh"
 #include "softmax.cuh"
@@ -421,13 +422,16 @@ template <bool PACKED>
 int launch_d256(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const PrefillParams& p,
                 cudaStream_t st) {
   using C = D256Cfg;
-  if (cudaFuncSetAttribute(fa_prefill_d256_kernel<PACKED>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           C::SMEM_BYTES) != cudaSuccess)
+  static OncePerDevice once;
+  if (!once([] {
+        return cudaFuncSetAttribute(fa_prefill_d256_kernel<PACKED>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    C::SMEM_BYTES) == cudaSuccess;
+      }))
     return -1;
   const long long nblk = (long long)p.n_qblk * p.Hq * (PACKED ? 1 : p.B);
   if (nblk <= 0 || nblk > 0x7fffffffLL) return -2;
   fa_prefill_d256_kernel<PACKED><<<(unsigned)nblk, C::THREADS, C::SMEM_BYTES, st>>>(tq, tk, tv, p);
-  return cudaGetLastError() == cudaSuccess ? 0 : -1;
+  return once.launched(cudaGetLastError());
 }
 
 }  // namespace

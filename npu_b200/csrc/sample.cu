@@ -23,6 +23,7 @@
 // the passes' results are joined through the cluster's shared memory in a
 // fixed order. The first race reads the noise once; later ones only for the
 // tokens ahead of the pivot.
+#include "capi_internal.cuh"
 #include "sample.cuh"
 
 namespace b2a {
@@ -454,8 +455,11 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleParams 
 
 template <typename T, bool STAGED>
 int launch_t(const SampleParams& p, size_t smem, cudaStream_t st) {
-  if (smem > 48 * 1024 && cudaFuncSetAttribute(sample_kernel<T, STAGED>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               (int)smem) != cudaSuccess)
+  static OncePerDevice once;
+  if (smem > 48 * 1024 && !once([] {
+        return cudaFuncSetAttribute(sample_kernel<T, STAGED>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    kMaxStageBytes) == cudaSuccess;
+      }))
     return -1;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -468,8 +472,8 @@ int launch_t(const SampleParams& p, size_t smem, cudaStream_t st) {
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, sample_kernel<T, STAGED>, p) != cudaSuccess) return -1;
-  return cudaGetLastError() == cudaSuccess ? 0 : -1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, sample_kernel<T, STAGED>, p);
+  return once.launched(e == cudaSuccess ? cudaGetLastError() : e);
 }
 
 template <typename T>
