@@ -13,6 +13,11 @@ run_batch. Here the same layer math runs as:
   * output projection, RMSNorms and the SwiGLU MLP in torch, as in the
     reference.
 
+Prompts of different lengths run packed instead of padded (prefill_packed,
+decode_packed, generate): b2a_rope_append_paged writes k and v to the pages of
+each sequence, b2a_prefill_varlen and b2a_decode_paged attend, b2a_sample
+chooses the tokens.
+
 Sequence positions stay on the device (KVCache), so a decode step issues no
 host synchronisation. Weights use the reference's HF key names
 (smollm.py:84-93, :256-265). The model may run in fp32 (the reference's NPU
@@ -28,7 +33,7 @@ import torch
 import torch.nn.functional as F
 
 from . import api
-from .kvcache import KVCache
+from .kvcache import KVCache, PagedKVCache, PagedSequences
 from .profiler import profile
 
 
@@ -238,3 +243,105 @@ class SmolLMB200:
         cache.advance()
         x = rms_norm(x, self.final_norm, c.rms_eps)
         return F.linear(x, self.embed)
+
+    # ------------------------------------------------------------ sequences of different lengths
+    def new_paged_cache(self, n_pages: int, page: int = 64) -> PagedKVCache:
+        return PagedKVCache(self.cfg.n_layers, n_pages, self.cfg.n_kv_heads, page, self.cfg.head_dim, self.device)
+
+    def _attention_packed(self, lw: dict, h: torch.Tensor, seqs: PagedSequences, i: int,
+                          cu_seqlens: Optional[torch.Tensor]) -> torch.Tensor:
+        """Attention of layer i before the output projection, [N, Hq * Dh]: of
+        packed prompts with offsets cu_seqlens, or (None) of one token per
+        sequence against its cached keys."""
+        c = self.cfg
+        Hq, Hkv, Dh = c.n_heads, c.n_kv_heads, c.head_dim
+        N = h.shape[0]
+        with profile("qkv"):
+            qkv = F.linear(h, lw["wqkv"])
+        q = qkv[:, :Hq * Dh].view(N, Hq, Dh)
+        k = qkv[:, Hq * Dh:(Hq + Hkv) * Dh].view(N, Hkv, Dh)
+        v = qkv[:, (Hq + Hkv) * Dh:].view(N, Hkv, Dh)
+        k_pages, v_pages = seqs.cache.layer(i)
+        prompts = cu_seqlens is not None
+        with profile("rope"):
+            rot = api.rope_append_paged(q, k, v, self.cos, self.sin, k_pages, v_pages, seqs.block_table,
+                                        cu_seqlens if prompts else seqs.one_each, start_pos_per_batch=seqs.start,
+                                        seqlens_out=seqs.end, return_kv=prompts)
+        with profile("attn"):
+            if prompts:
+                o = api.prefill_varlen(*rot, cu_seqlens, out_dtype=h.dtype)
+            else:
+                o = api.decode_paged(rot, k_pages, v_pages, seqs.block_table, seqs.end, out_dtype=h.dtype)
+        return o.view(N, Hq * Dh)
+
+    def _forward_packed(self, ids: torch.Tensor, seqs: PagedSequences,
+                        cu_seqlens: Optional[torch.Tensor]) -> torch.Tensor:
+        """The final norm's output for packed tokens ids [N]; advances seqs."""
+        c = self.cfg
+        x = self.embed[ids]
+        for i, lw in enumerate(self.layers):
+            with profile("rms1"):
+                h = rms_norm(x, lw["ln1"], c.rms_eps)
+            o = self._attention_packed(lw, h, seqs, i, cu_seqlens)
+            with profile("wo"):
+                x = x + F.linear(o, lw["wo"])
+            with profile("rms2"):
+                h = rms_norm(x, lw["ln2"], c.rms_eps)
+            with profile("gate_up"):
+                gu = F.silu(F.linear(h, lw["w_gate"])) * F.linear(h, lw["w_up"])
+            with profile("w_down"):
+                x = x + F.linear(gu, lw["w_down"])
+        seqs.advance()
+        return rms_norm(x, self.final_norm, c.rms_eps)
+
+    @torch.no_grad()
+    def prefill_packed(self, ids: torch.Tensor, cu_seqlens: torch.Tensor, seqs: PagedSequences) -> torch.Tensor:
+        """Logits [B, vocab] of each prompt's last token, for prompts packed in
+        ids [N] (sequence b: ids[cu_seqlens[b] : cu_seqlens[b + 1]], none empty)
+        into the new, empty sequences `seqs`."""
+        if ids.dim() != 1 or cu_seqlens.numel() != seqs.batch + 1:
+            raise ValueError("ids must be [N] and cu_seqlens [B + 1] with B = seqs.batch")
+        x = self._forward_packed(ids.to(self.device), seqs, cu_seqlens)
+        return F.linear(x[(cu_seqlens[1:] - 1).long()], self.embed)
+
+    @torch.no_grad()
+    def decode_packed(self, ids: torch.Tensor, seqs: PagedSequences) -> torch.Tensor:
+        """Logits [B, vocab] after one more token ids [B] of every sequence."""
+        if ids.dim() != 1 or ids.numel() != seqs.batch:
+            raise ValueError("ids must be [B] with B = seqs.batch")
+        return F.linear(self._forward_packed(ids.to(self.device), seqs, None), self.embed)
+
+    @torch.no_grad()
+    def generate(self, prompts, max_new_tokens: int, *, cache: Optional[PagedKVCache] = None, page: int = 64,
+                 temperature=0.0, top_k=0, top_p=1.0, min_p=0.0,
+                 generator: Optional[torch.Generator] = None) -> torch.Tensor:
+        """max_new_tokens tokens after each prompt (a list of token lists, of
+        any lengths from 1), int64 [B, max_new_tokens] on the device. The
+        settings are those of api.sample; temperature 0 is greedy. Nothing
+        synchronises with the host in between."""
+        lens = [len(p) for p in prompts]
+        if not lens or min(lens) < 1 or max_new_tokens < 1:
+            raise ValueError("every prompt needs a token and max_new_tokens must be positive")
+        if max(lens) + max_new_tokens > self.cfg.max_pos:
+            raise ValueError(f"{max(lens)} + {max_new_tokens} tokens exceed the rotary table length {self.cfg.max_pos}")
+        room = [n + max_new_tokens for n in lens]
+        if cache is None:
+            cache = self.new_paged_cache(sum(-(-r // page) for r in room), page)
+        seqs = cache.reserve(room)
+        try:
+            cu = torch.tensor([0] + lens, dtype=torch.int32).cumsum(0, dtype=torch.int32).to(self.device)
+            ids = torch.tensor([t for p in prompts for t in p], dtype=torch.long, device=self.device)
+            greedy = not isinstance(temperature, torch.Tensor) and temperature <= 0
+            out = torch.empty((max_new_tokens, len(lens)), dtype=torch.long, device=self.device)
+            logits = self.prefill_packed(ids, cu, seqs)
+            for step in range(max_new_tokens):
+                noise = None if greedy else torch.empty(logits.shape, dtype=torch.float32,
+                                                        device=self.device).exponential_(generator=generator)
+                with profile("sample"):
+                    api.sample(logits, noise, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p,
+                               out=out[step])
+                if step + 1 < max_new_tokens:
+                    logits = self.decode_packed(out[step], seqs)
+        finally:
+            seqs.release()
+        return out.T.contiguous()
