@@ -65,7 +65,7 @@ struct Weight {
 // largest score (ordered bits; 0: none), the lowest token among equals, its
 // logit, and the pass's weight and count.
 constexpr uint32_t kNone = 0xffffffffu;
-struct alignas(8) Found {
+struct alignas(16) Found {
   uint32_t score, token;
   float x, sum;
   int count;
@@ -105,6 +105,7 @@ __device__ __forceinline__ void load_group(const __nv_bfloat16* p, float (&x)[kG
     x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
   }
 }
+
 // The larger of a and the group's logits (NaN ignored).
 __device__ __forceinline__ float group_max(float a, const float (&x)[kGroup]) {
 #pragma unroll
@@ -140,38 +141,61 @@ struct Candidate {
 
 struct Shared {
   Found warp[kWarps];
-  Found cta[2][kMaxCluster];  // every CTA's value, written by its owner into each CTA of the cluster
+  Found cta[2][kMaxCluster];  // every CTA's value, sent by its owner to each CTA of the cluster
+  uint64_t arrived[2];        // counts the bytes of the values
   uint64_t full;
   int abort_flag;
 };
 
-// Every thread of the cluster gets the joined value; pass counts the calls.
-// A CTA writes pass n's slots after the barrier of pass n - 1, when everyone
-// has read those of pass n - 2, so two sets of slots are enough.
-__device__ __forceinline__ Found cluster_join(Found f, Shared* sh, int rank, int size, int& pass) {
-  f = warp_join(f);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (lane == 0) sh->warp[warp] = f;
-  __syncthreads();
-  Found* slots = sh->cta[pass & 1];
-  if (warp == 0) {
-    f = warp_join(lane < kWarps ? sh->warp[lane] : nothing());
-    if (lane < size) {
-      uint32_t remote;
-      asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_u32(slots + rank)), "r"(lane));
-      asm volatile(
-          "st.shared::cluster.v2.u32 [%0], {%1, %2};\n\t"
-          "st.shared::cluster.v2.f32 [%0 + 8], {%3, %4};\n\t"
-          "st.shared::cluster.u32 [%0 + 16], %5;" ::"r"(remote),
-          "r"(f.score), "r"(f.token), "f"(f.x), "f"(f.sum), "r"(f.count)
-          : "memory");
-    }
-    __syncwarp();
+// The cluster's CTAs as one: joins of a value from each, in turn.
+struct Cluster {
+  Shared* sh;
+  int rank, size;
+  int* err;
+  int pass = 0;  // joins so far
+
+  // Address of a shared variable of this CTA in CTA `to`, and a store there
+  // that its barrier counts when it lands.
+  static __device__ __forceinline__ uint32_t in_cta(const void* p, int to) {
+    uint32_t remote;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_u32(p)), "r"(to));
+    return remote;
   }
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-  ++pass;
-  return warp_join(lane < size ? slots[lane] : nothing());
-}
+
+  // Every thread of the cluster gets the joined value. Each CTA's first warp
+  // sends its value to every CTA, one hop, and each waits for its own copies:
+  // no barrier of all the CTAs. A CTA sends for pass n + 2 only after it has
+  // everyone's value of pass n + 1, which they sent after reading pass n's:
+  // two sets of slots are enough, and after the last pass nothing is under way.
+  __device__ __forceinline__ Found join(Found f) {
+    f = warp_join(f);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (lane == 0) sh->warp[warp] = f;
+    __syncthreads();
+    Found* slots = sh->cta[pass & 1];
+    uint64_t* bar = &sh->arrived[pass & 1];
+    if (warp == 0) {
+      f = warp_join(lane < kWarps ? sh->warp[lane] : nothing());
+      if (lane == 0) mbar_arrive_expect_tx(bar, size * 20);
+      __syncwarp();
+      if (lane < size) {
+        const uint32_t to = in_cta(slots + rank, lane), remote_bar = in_cta(bar, lane);
+        asm volatile(
+            "st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%6];\n\t"
+            "st.async.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0 + 16], %5, [%6];" ::"r"(to),
+            "r"(f.score), "r"(f.token), "r"(__float_as_uint(f.x)), "r"(__float_as_uint(f.sum)), "r"(f.count),
+            "r"(remote_bar)
+            : "memory");
+      }
+      __syncwarp();
+    }
+    const uint32_t parity = (uint32_t)(pass >> 1) & 1u;
+    if (!mbar_wait_limit(bar, parity, &sh->abort_flag, err, kWaitLimitCycles)) mbar_wait_quiet(bar, parity);
+    __syncwarp();
+    ++pass;
+    return warp_join(lane < size ? slots[lane] : nothing());
+  }
+};
 
 __device__ __forceinline__ float to_float(float x) { return x; }
 __device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
@@ -185,8 +209,16 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleParams 
   uint32_t rank = 0;
   asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
   const int size = p.cluster;
-  // Waited for before the first write into another CTA: it has started.
-  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+  if (threadIdx.x == 0) {
+    mbar_init(&sh.full, 1);
+    mbar_init(&sh.arrived[0], 1);
+    mbar_init(&sh.arrived[1], 1);
+    sh.abort_flag = 0;
+    fence_mbar_init();
+  }
+  // Waited for before the first join: every CTA has started and its barriers
+  // are ready.
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   const int r = blockIdx.x / size;
   const int begin = min((int)rank * p.slice, p.V);
   const int n = min(p.slice, p.V - begin);  // this CTA's tokens [begin, begin + n)
@@ -207,9 +239,6 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleParams 
     const int head = min(n, (kPer16 - shift) % kPer16);
     const int units = (n - head) / kPer16;
     if (threadIdx.x == 0) {
-      mbar_init(&sh.full, 1);
-      sh.abort_flag = 0;
-      fence_mbar_init();
       mbar_arrive_expect_tx(&sh.full, units * 16);
       if (units > 0)
         asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
@@ -249,7 +278,7 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleParams 
     }
   };
 
-  int pass = 0;
+  Cluster cluster{&sh, (int)rank, size, p.err};
   float m = -INFINITY;
   // The larger of a and group g's logits.
   auto raise = [&](float a, int g) -> float {
@@ -264,7 +293,7 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleParams 
   const unsigned bits = __float_as_uint(m);
   const unsigned ordered = (bits & 0x80000000u) ? ~bits : bits | 0x80000000u;
   const float own_max = m;
-  m = cluster_join({ordered, kNone, m, 0.f, 0}, &sh, rank, size, pass).x;
+  m = cluster.join({ordered, kNone, m, 0.f, 0}).x;
   const float top = m;
   // The lowest index of the maximum, for a row that needs it.
   auto first_maximum = [&]() -> int {
@@ -276,7 +305,7 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleParams 
       for (int e = kGroup - 1; e >= 0; --e)
         if (x[e] == top) f.score = 1, f.token = begin + g * kGroup - shift + e;
     }
-    return (int)cluster_join(f, &sh, rank, size, pass).token;
+    return (int)cluster.join(f).token;
   };
   if (m == -INFINITY || greedy) {
     const int i = m == -INFINITY ? -1 : first_maximum();
@@ -325,35 +354,26 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleParams 
   // all of them again.
   const int rounds = (groups + kThreads * kMaskGroups - 1) / (kThreads * kMaskGroups);
   auto group_of = [&](int round, int k) { return (round * kMaskGroups + k) * kThreads + (int)threadIdx.x; };
-  auto logit = [&](int i) -> float {  // token i of the slice
-    float x;
-    if constexpr (STAGED)
-      x = to_float(stage[shift + i]);
-    else
-      x = to_float(logits[i]);
-    return infinite ? (x == INFINITY ? 0.f : -INFINITY) : x;
-  };
-  // Offers the tokens in `mask` of a round to the race, two at a time, and
-  // returns their weight.
+  // Offers the tokens in `mask` of a round to the race and returns their
+  // weight; the noise of a group is requested together.
   auto race = [&](Candidate& c, int round, uint64_t mask) -> float {
     float sum = 0.f;
+#pragma unroll 1
     while (mask) {
-      int at[2];
-      float e[2];
+      const int k = (__ffsll((long long)mask) - 1) / kGroup;
+      const unsigned bits = (unsigned)(mask >> (k * kGroup)) & 0xffu;
+      mask &= ~(0xffull << (k * kGroup));
+      const int g = group_of(round, k), at = g * kGroup - shift;
+      float x[kGroup], e[kGroup];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int bit = __ffsll((long long)mask) - 1;
-        at[h] = bit < 0 ? -1 : group_of(round, bit / kGroup) * kGroup + bit % kGroup - shift;
-        mask &= mask - 1;
-        e[h] = at[h] >= 0 ? __ldg(noise + at[h]) : 1.f;
+      for (int i = 0; i < kGroup; ++i) e[i] = bits >> i & 1 ? __ldg(noise + at + i) : 1.f;
+      load(g, x);
+#pragma unroll
+      for (int i = 0; i < kGroup; ++i) {
+        const float w = bits >> i & 1 ? weight.quick(x[i]) : 0.f;
+        sum += w;
+        c.offer(w, e[i], x[i], at + i);
       }
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-        if (at[h] >= 0) {
-          const float x = logit(at[h]), w = weight.quick(x);
-          sum += w;
-          c.offer(w, e[h], x, at[h]);
-        }
     }
     return sum;
   };
@@ -414,7 +434,7 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleParams 
       }
     }
   }
-  Found f = cluster_join(found(c, total, 0), &sh, rank, size, pass);
+  Found f = cluster.join(found(c, total, 0));
   const float mass = top_p < 1.f ? top_p * f.sum : INFINITY;
   while (f.score != 0 && (top_k > 0 || top_p < 1.f || weight(f.x) < min_p)) {
     const float xj = f.x;
@@ -443,7 +463,7 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleParams 
       sum += race(c, round, ahead);
       mask = ahead;
     }
-    const Found a = cluster_join(found(c, sum, count), &sh, rank, size, pass);
+    const Found a = cluster.join(found(c, sum, count));
     const bool kept = (top_k <= 0 || a.count < top_k) && a.sum < mass && weight(xj) >= min_p;
     if (kept || a.count == 0) break;
     f = a;
