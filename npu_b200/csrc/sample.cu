@@ -354,25 +354,34 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleParams 
   // all of them again.
   const int rounds = (groups + kThreads * kMaskGroups - 1) / (kThreads * kMaskGroups);
   auto group_of = [&](int round, int k) { return (round * kMaskGroups + k) * kThreads + (int)threadIdx.x; };
-  // Offers the tokens in `mask` of a round to the race and returns their
-  // weight; the noise of a group is requested together.
+  auto logit = [&](int i) -> float {  // token i of the slice
+    float x;
+    if constexpr (STAGED)
+      x = to_float(stage[shift + i]);
+    else
+      x = to_float(logits[i]);
+    return infinite ? (x == INFINITY ? 0.f : -INFINITY) : x;
+  };
+  // Offers the tokens in `mask` of a round to the race, four at a time (their
+  // noise is requested together), and returns their weight.
   auto race = [&](Candidate& c, int round, uint64_t mask) -> float {
     float sum = 0.f;
 #pragma unroll 1
     while (mask) {
-      const int k = (__ffsll((long long)mask) - 1) / kGroup;
-      const unsigned bits = (unsigned)(mask >> (k * kGroup)) & 0xffu;
-      mask &= ~(0xffull << (k * kGroup));
-      const int g = group_of(round, k), at = g * kGroup - shift;
-      float x[kGroup], e[kGroup];
+      int at[4];
+      float e[4];
 #pragma unroll
-      for (int i = 0; i < kGroup; ++i) e[i] = bits >> i & 1 ? __ldg(noise + at + i) : 1.f;
-      load(g, x);
+      for (int h = 0; h < 4; ++h) {
+        const int bit = __ffsll((long long)mask) - 1;
+        at[h] = bit < 0 ? -1 : group_of(round, bit / kGroup) * kGroup + bit % kGroup - shift;
+        mask &= mask - 1;
+        e[h] = at[h] >= 0 ? __ldg(noise + at[h]) : 1.f;
+      }
 #pragma unroll
-      for (int i = 0; i < kGroup; ++i) {
-        const float w = bits >> i & 1 ? weight.quick(x[i]) : 0.f;
+      for (int h = 0; h < 4; ++h) {
+        const float x = at[h] >= 0 ? logit(at[h]) : -INFINITY, w = weight.quick(x);
         sum += w;
-        c.offer(w, e[i], x[i], at + i);
+        c.offer(w, e[h], x, at[h]);
       }
     }
     return sum;
