@@ -289,27 +289,32 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleParams 
   };
   for (int g = threadIdx.x; g < groups; g += kThreads) m = raise(m, g);
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-  m = __fadd_rn(m, 0.f);  // -0 is +0: equal logits have equal bits in the join
-  const unsigned bits = __float_as_uint(m);
+  const float own_max = __fadd_rn(m, 0.f);  // -0 is +0: equal logits have equal bits in the join
+  const unsigned bits = __float_as_uint(own_max);
   const unsigned ordered = (bits & 0x80000000u) ? ~bits : bits | 0x80000000u;
-  const float own_max = m;
-  m = cluster.join({ordered, kNone, m, 0.f, 0}).x;
-  const float top = m;
-  // The lowest index of the maximum, for a row that needs it.
+  // The lowest index of the maximum, -1 if that is -inf.
   auto first_maximum = [&]() -> int {
-    Found f = nothing();
-    for (int g = threadIdx.x; g < groups && f.score == 0; g += kThreads) {
+    Found f{ordered, kNone, own_max, 0.f, 0};
+#pragma unroll 1
+    for (int g = threadIdx.x; g < groups && own_max > -INFINITY && f.token == kNone; g += kThreads) {
+      if (raise(-INFINITY, g) < own_max) continue;
       float x[kGroup];
       load_raw(g, x);
 #pragma unroll
       for (int e = kGroup - 1; e >= 0; --e)
-        if (x[e] == top) f.score = 1, f.token = begin + g * kGroup - shift + e;
+        if (x[e] == own_max) f.token = begin + g * kGroup - shift + e;
     }
-    return (int)cluster.join(f).token;
+    f = cluster.join(f);
+    return f.x == -INFINITY ? -1 : (int)f.token;
   };
-  if (m == -INFINITY || greedy) {
-    const int i = m == -INFINITY ? -1 : first_maximum();
+  if (greedy) {
+    const int i = first_maximum();
     if (rank == 0 && threadIdx.x == 0) p.out[r] = i;
+    return;
+  }
+  m = cluster.join({ordered, kNone, own_max, 0.f, 0}).x;
+  if (m == -INFINITY) {
+    if (rank == 0 && threadIdx.x == 0) p.out[r] = -1;
     return;
   }
   // A maximum of +inf: the tokens that have it weigh 1, all others 0.
