@@ -290,6 +290,63 @@ __device__ __forceinline__ void clear_v_rows(uint32_t tile, int from, int rows, 
   __syncwarp();
 }
 
+// softmax_half_tmem for short packed sequences: the same values (kEmuPairs = 0) from
+// a fraction of the code. Rows of short sequences take the masked and the
+// first-block path as often as the plain one, and with each path's 64 columns
+// unrolled separately the kernel did not fit the SM's instruction cache
+// (instruction fetch was the largest stall, 4.6 of 15.8 cycles an issue, at 32
+// prompts of 17 to 2048 tokens). Here one copy serves them all: rows without a
+// running max take the max first, and a half whose max turns out too large is
+// redone by the same loop.
+__device__ __forceinline__ float softmax_half_packed(uint32_t (&s)[2][32], int lim, float sl2, float& m_run,
+                                                     uint32_t tP, float& hsum) {
+  if (!__all_sync(0xffffffffu, lim >= 63)) {
+#pragma unroll
+    for (int i = 0; i < 64; ++i)
+      if (i > lim) s[i >> 5][i & 31] = f2u(-INFINITY);
+  }
+  float a = 1.f;
+  // The half's max moves m_run where there was none, or past the threshold.
+  auto take_max = [&](float m_half) -> bool {
+    if (m_run == -INFINITY) {
+      if (m_half == -INFINITY) return false;
+      a = 0.f;  // everything before was computed from masked keys: zeros
+    } else if (m_half > m_run + kRescaleThreshold) {
+      a = ex2(m_run - m_half);
+    } else {
+      return false;
+    }
+    m_run = m_half;
+    return true;
+  };
+  if (!__all_sync(0xffffffffu, m_run != -INFINITY)) {
+    float mx = -INFINITY, my = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) {
+      mx = fmax3(mx, u2f(s[0][i]), u2f(s[0][i + 1]));
+      my = fmax3(my, u2f(s[1][i]), u2f(s[1][i + 1]));
+    }
+    take_max(fmaxf(mx, my) * sl2);
+  }
+  float2 acc[4];
+  float mx[4];
+#pragma unroll 1
+  while (true) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      acc[k] = make_float2(0.f, 0.f);
+      mx[k] = -INFINITY;
+    }
+    softmax_p_chunks_tmem<2, 0, 2, 0, true>(s, sl2, m_run == -INFINITY ? 0.f : m_run, tP, acc, mx);
+    const bool jump = take_max(fmaxf(fmax3(mx[0], mx[1], mx[2]), mx[3]) * sl2);
+    if (!__any_sync(0xffffffffu, jump)) break;
+    tmem_wait_st();  // this pass's stores land before they are overwritten
+  }
+  const float2 r2 = __fadd2_rn(__fadd2_rn(acc[0], acc[1]), __fadd2_rn(acc[2], acc[3]));
+  hsum = r2.x + r2.y;
+  return a;
+}
+
 // sigmoid(g) = 1 / (1 + e^-g) in fp32 (torch.sigmoid, qwen/forward.py:226).
 __device__ __forceinline__ float sigmoidf_(float g) { return __fdividef(1.f, 1.f + __expf(-g)); }
 
