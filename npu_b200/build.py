@@ -69,7 +69,7 @@ def _build_binding(force: bool) -> None:
            "-isystem", sysconfig.get_paths()["include"], "-isystem", str(nvcc.parent.parent / "include"),
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            str(BINDING_SOURCE), "-o", str(tmp), "-L", str(PKG), "-l:libb2attn.so", "-L", str(root / "lib"),
-           "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
+           "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"building {BINDING.name} failed:\n{r.stdout}\n{r.stderr}")

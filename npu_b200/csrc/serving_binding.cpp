@@ -4,6 +4,8 @@
 // argument lists, several times what a single-token kernel runs; through this
 // module it costs 3 to 5. npu_b200.api documents the functions.
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -69,8 +71,14 @@ int as_int(const char* name, int64_t v) {
   return (int)v;
 }
 
+// A new tensor on like's device, by the allocator of torch's current stream
+// (without the dispatcher, which takes as long as the allocation).
+Tensor empty(at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) {
+  return at::detail::empty_cuda(sizes, type, like.device(), std::nullopt);
+}
+
 Tensor output(const OptTensor& out, at::IntArrayRef sizes, at::ScalarType type, const Tensor& like, const char* what) {
-  if (!out) return at::empty(sizes, like.options().dtype(type));
+  if (!out) return empty(sizes, type, like);
   if (out->scalar_type() != type || out->sizes() != sizes || (out->dim() && out->stride(-1) != 1) ||
       out->device() != like.device())
     refuse(what);
@@ -117,7 +125,7 @@ py::object prefill_varlen(const Tensor& q, const Tensor& k, const Tensor& v, con
   Tensor o = output(out, q.sizes(), out_dtype, q,
                     "out must match [Nq, Hq, D], out_dtype and q's device, with a contiguous last dim");
   OptTensor lse;
-  if (return_lse) lse = at::empty({Hq, Nq}, q.options().dtype(at::kFloat));
+  if (return_lse) lse = empty({Hq, Nq}, at::kFloat, q);
   const Strides gs(gate ? *gate : q, 2);
   check(b2a_prefill_varlen(q.data_ptr(), k.data_ptr(), v.data_ptr(), pointer(gate), o.data_ptr(),
                            static_cast<float*>(pointer(lse)), cu_q.data_ptr<int>(),
@@ -151,13 +159,17 @@ Tensor decode_paged(const Tensor& q, const Tensor& k_pages, const Tensor& v_page
                     "out must match [B, Hq, D], out_dtype and q's device, with a contiguous last dim");
   const size_t need =
       b2a_decode_paged_workspace_bytes(as_int("B", B), as_int("Hq", Hq), as_int("Hkv", Hkv), as_int("D", D));
-  Tensor ws;
+  // Scratch taken here goes back when the call returns; what reuses it on this
+  // stream runs after this call's kernels.
+  c10::DataPtr taken;
+  void* ws;
   if (workspace) {
     if (workspace->device() != device || !workspace->is_contiguous() || workspace->nbytes() < need)
       refuse("workspace must be a contiguous CUDA tensor of at least ", need, " bytes on q's device");
-    ws = *workspace;
+    ws = workspace->data_ptr();
   } else {
-    ws = at::empty({(int64_t)std::max<size_t>(need, 16)}, q.options().dtype(at::kByte));
+    taken = c10::cuda::CUDACachingAllocator::get()->allocate(std::max<size_t>(need, 16));
+    ws = taken.get();
   }
   const Strides gs(gate ? *gate : q, 2);
   check(b2a_decode_paged(q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), table.data_ptr<int>(), table.stride(0),
@@ -165,8 +177,8 @@ Tensor decode_paged(const Tensor& q, const Tensor& k_pages, const Tensor& v_page
                          (int)B, (int)Hq, (int)Hkv, as_int("n_pages", n_pages), as_int("page", page), (int)D,
                          Strides(q, 2), Strides(k_pages, 3), Strides(v_pages, 3), gs, Strides(o, 2),
                          gate && gate->scalar_type() == at::kBFloat16,
-                         (float)scale.value_or(1.0 / std::sqrt((double)D)), out_dtype == at::kFloat, ws.data_ptr(),
-                         ws.nbytes(), stream_of(q)),
+                         (float)scale.value_or(1.0 / std::sqrt((double)D)), out_dtype == at::kFloat, ws, need,
+                         stream_of(q)),
         "b2a_decode_paged");
   return o;
 }
@@ -213,8 +225,8 @@ py::object rope_append_paged(const Tensor& q, const Tensor& k, const Tensor& v, 
   Tensor qo = output(q_out, q.sizes(), at::kBFloat16, q, wants);
   const bool bf16 = type == at::kBFloat16;
   OptTensor ko, vo;
-  if (return_kv) ko = at::empty({N, Hkv, D}, q.options().dtype(at::kBFloat16));
-  if (return_kv && !bf16) vo = at::empty({N, Hkv, D}, q.options().dtype(at::kBFloat16));
+  if (return_kv) ko = empty({N, Hkv, D}, at::kBFloat16, q);
+  if (return_kv && !bf16) vo = empty({N, Hkv, D}, at::kBFloat16, q);
   check(b2a_rope_append_paged(q.data_ptr(), k.data_ptr(), v.data_ptr(), Strides(q, 2), Strides(k, 2), Strides(v, 2),
                               bf16, pointer(q_norm), pointer(k_norm), (float)eps, cos.data_ptr(), sin.data_ptr(),
                               cos.scalar_type() == at::kFloat, as_int("max_pos", cos.size(0)),
