@@ -350,48 +350,52 @@ __device__ __forceinline__ float softmax_half_packed(uint32_t (&s)[2][32], int l
 // sigmoid(g) = 1 / (1 + e^-g) in fp32 (torch.sigmoid, qwen/forward.py:226).
 __device__ __forceinline__ float sigmoidf_(float g) { return __fdividef(1.f, 1.f + __expf(-g)); }
 
-// One 32-column chunk of an output row: O scaled by inv_l and, with a gate,
-// by sigmoid(gate). Only called for rows that exist (the gate is read).
-__device__ __forceinline__ void out_chunk_values(const PrefillParams& p, int b, int h, int grow, int c,
-                                                 const uint32_t (&o)[32], float inv_l, float (&v)[32]) {
+// The gate of one 32-column chunk of an output row, as loaded.
+struct GateChunk {
+  uint4 w[8];  // bf16: the first four
+};
+
+__device__ __forceinline__ void load_gate_chunk(const PrefillParams& p, int b, int h, int grow, int c, GateChunk& g) {
+  const long long gi = (long long)b * p.g_sb + (long long)h * p.g_sh + (long long)grow * p.g_st + 32 * c;
+  if (p.gate_bf16) {
+    const uint4* g4 = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.gate) + gi);
 #pragma unroll
-  for (int i = 0; i < 32; ++i) v[i] = u2f(o[i]) * inv_l;
-  if (p.gate) {
-    const long long gi = (long long)b * p.g_sb + (long long)h * p.g_sh + (long long)grow * p.g_st + 32 * c;
-    if (p.gate_bf16) {
-      const uint4* g4 = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.gate) + gi);
+    for (int i = 0; i < 4; ++i) g.w[i] = g4[i];
+  } else {
+    const uint4* g4 = reinterpret_cast<const uint4*>(static_cast<const float*>(p.gate) + gi);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint4 w = g4[i];
-        const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+    for (int i = 0; i < 8; ++i) g.w[i] = g4[i];
+  }
+}
+
+__device__ __forceinline__ void apply_gate_chunk(const PrefillParams& p, const GateChunk& g, float (&v)[32]) {
+  if (p.gate_bf16) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          v[8 * i + 2 * k] *= sigmoidf_(u2f(ws[k] << 16));
-          v[8 * i + 2 * k + 1] *= sigmoidf_(u2f(ws[k] & 0xffff0000u));
-        }
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t ws[4] = {g.w[i].x, g.w[i].y, g.w[i].z, g.w[i].w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        v[8 * i + 2 * k] *= sigmoidf_(u2f(ws[k] << 16));
+        v[8 * i + 2 * k + 1] *= sigmoidf_(u2f(ws[k] & 0xffff0000u));
       }
-    } else {
-      const float4* g4 = reinterpret_cast<const float4*>(static_cast<const float*>(p.gate) + gi);
+    }
+  } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float4 w = g4[i];
-        v[4 * i] *= sigmoidf_(w.x);
-        v[4 * i + 1] *= sigmoidf_(w.y);
-        v[4 * i + 2] *= sigmoidf_(w.z);
-        v[4 * i + 3] *= sigmoidf_(w.w);
-      }
+    for (int i = 0; i < 8; ++i) {
+      v[4 * i] *= sigmoidf_(u2f(g.w[i].x));
+      v[4 * i + 1] *= sigmoidf_(u2f(g.w[i].y));
+      v[4 * i + 2] *= sigmoidf_(u2f(g.w[i].z));
+      v[4 * i + 3] *= sigmoidf_(u2f(g.w[i].w));
     }
   }
 }
 
-// Scale one 32-column chunk of an output row (out_chunk_values) and store it
-// (fp32 or bf16) with 32-byte stores where O is aligned for them (p.o_v8: a
-// warp's row-per-thread stores then write whole 32-byte sectors, with half
-// the store instructions), else 16-byte stores.
-__device__ __forceinline__ void store_out_chunk(const PrefillParams& p, int b, int h, int grow, int c,
-                                                const uint32_t (&o)[32], float inv_l) {
-  float v[32];
-  out_chunk_values(p, b, h, grow, c, o, inv_l, v);
+// Store one 32-column chunk of an output row (fp32 or bf16) with 32-byte
+// stores where O is aligned for them (p.o_v8: a warp's row-per-thread stores
+// then write whole 32-byte sectors, with half the store instructions), else
+// 16-byte stores.
+__device__ __forceinline__ void store_values(const PrefillParams& p, int b, int h, int grow, int c,
+                                             const float (&v)[32]) {
   const long long base = (long long)b * p.o_sb + (long long)h * p.o_sh + (long long)grow * p.o_st + 32 * c;
   if (p.o_v8) {
     if (p.out_fp32) {
@@ -425,6 +429,22 @@ __device__ __forceinline__ void store_out_chunk(const PrefillParams& p, int b, i
       dst[i] = w;
     }
   }
+}
+
+// Scale one 32-column chunk of an output row by inv_l and, with a gate, by
+// sigmoid(gate), and store it. Only called for rows that exist (the gate is
+// read).
+__device__ __forceinline__ void store_out_chunk(const PrefillParams& p, int b, int h, int grow, int c,
+                                                const uint32_t (&o)[32], float inv_l) {
+  float v[32];
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = u2f(o[i]) * inv_l;
+  if (p.gate) {
+    GateChunk g;
+    load_gate_chunk(p, b, h, grow, c, g);
+    apply_gate_chunk(p, g, v);
+  }
+  store_values(p, b, h, grow, c, v);
 }
 
 }  // namespace b2a
