@@ -380,44 +380,51 @@ __global__ void __launch_bounds__(256, 1)
       tc_fence_before();
       mbar_arrive(&bars->p_full[buf]);
     }
-    if (n == 0) {
-      if (valid) {
-        uint32_t z[32];
-#pragma unroll
-        for (int i = 0; i < 32; ++i) z[i] = 0u;
-        for (int c = 0; c < C::D / 32; ++c) store_out_chunk(p, b, h, orow, c, z, 0.f);
-        if (p.lse) p.lse[((long long)b * p.Hq + h) * p.Tq + orow] = -INFINITY;
-      }
-    } else if (ok) {
-      // Each chunk's gate is requested a chunk ahead, the first before the wait
-      // for O (without that the eight waits for memory are a quarter of a
-      // 24-block item: 8.6 us of 35).
-      const bool gated = p.gate && valid;
-      GateChunk gate;
-      if (gated) load_gate_chunk(p, b, h, orow, 0, gate);
+    // What the epilogue needs of a row: 1 / l. Q's staging tile is free (Q is
+    // in TMEM).
+    if (n > 0 && ok) {
       const bool w = mbar_wait(&bars->o_full, 0, abort_flag, p.err);
-      if (__all_sync(0xffffffffu, w)) {
-        tc_fence_after();
-        const float inv_l = l_run > 0.f ? 1.f / l_run : 0.f;
+      ok = __all_sync(0xffffffffu, w);
+    }
+    reinterpret_cast<float*>(sQ)[row] = l_run > 0.f ? 1.f / l_run : 0.f;
+    if (p.lse && valid && ok)
+      p.lse[((long long)b * p.Hq + h) * p.Tq + orow] =
+          l_run > 0.f ? (m_run + __log2f(l_run)) * 0.69314718055994531f : -INFINITY;
+  }
+
+  // Epilogue, by all eight warps: warp w takes the 32 rows of its TMEM lanes
+  // (w & 3) and half of the columns. Each chunk's gate is requested a chunk
+  // ahead, the first before the barrier (with four warps, each chunk waiting
+  // for its own gate, this was 8.6 us of a 24-block item's 35).
+  {
+    const int row = (warp & 3) * 32 + lane;
+    const int grow = q0 + row, orow = q_base + grow;
+    const bool valid = grow < Tq, gated = p.gate && valid;
+    const int c_end = ((warp >> 2) + 1) * (C::D / 64);
+    int c = (warp >> 2) * (C::D / 64);
+    const uint32_t tO = tmem + ((uint32_t)((warp & 3) * 32) << 16) + C::O_COL;
+    GateChunk gate;
+    if (gated) load_gate_chunk(p, b, h, orow, c, gate);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const float inv_l = reinterpret_cast<const float*>(sQ)[row];
+    if (!*abort_flag) {
 #pragma unroll 1
-        for (int c = 0; c < C::D / 32; ++c) {
-          GateChunk next;
-          if (gated && c + 1 < C::D / 32) load_gate_chunk(p, b, h, orow, c + 1, next);
-          uint32_t o[32];
-          tmem_ld32(tO + 32 * c, o);
-          tmem_wait_ld();
-          if (valid) {
-            float v[32];
+      for (; c < c_end; ++c) {
+        GateChunk next;
+        if (gated && c + 1 < c_end) load_gate_chunk(p, b, h, orow, c + 1, next);
+        uint32_t o[32];
+        tmem_ld32(tO + 32 * c, o);
+        tmem_wait_ld();
+        if (valid) {
+          float v[32];
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = u2f(o[i]) * inv_l;
-            if (gated) apply_gate_chunk(p, gate, v);
-            store_values(p, b, h, orow, c, v);
-          }
-          gate = next;
+          for (int i = 0; i < 32; ++i) v[i] = n > 0 ? u2f(o[i]) * inv_l : 0.f;
+          if (gated) apply_gate_chunk(p, gate, v);
+          store_values(p, b, h, orow, c, v);
         }
-        if (p.lse && valid)
-          p.lse[((long long)b * p.Hq + h) * p.Tq + orow] =
-              l_run > 0.f ? (m_run + __log2f(l_run)) * 0.69314718055994531f : -INFINITY;
+        gate = next;
       }
     }
   }
