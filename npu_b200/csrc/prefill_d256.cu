@@ -100,6 +100,30 @@ __global__ void __launch_bounds__(256, 1)
   volatile int* abort_flag = &bars->abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
+  if (warp == 2 && lane == 0) {
+    mbar_init(&bars->q_full, 1);
+    mbar_init(&bars->q_tmem, 128);
+    for (int s = 0; s < C::STAGES; ++s) {
+      mbar_init(&bars->kv_full[s], 1);
+      mbar_init(&bars->kv_empty[s], 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&bars->s_full[s], 1);
+      mbar_init(&bars->p_full[s], 128);
+    }
+    mbar_init(&bars->pv_done, 1);
+    mbar_init(&bars->o_full, 1);
+    mbar_init(&bars->drain, 1);
+    bars->abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&tm_q);
+    tma_prefetch_desc(&tm_k);
+    tma_prefetch_desc(&tm_v);
+  }
+  if (warp == 1) {
+    tmem_alloc(&bars->tmem_base, C::TMEM_COLS);
+    tmem_relinquish();
+  }
   // Block -> (query tile, head, batch), heaviest causal tiles first.
   const int lin = blockIdx.x;
   int h, b, q0, sp, Tq, Tk, q_base = 0, k_base = 0;
@@ -111,7 +135,9 @@ __global__ void __launch_bounds__(256, 1)
       const PackedBlock at = blocks.find(lin / p.Hq);
       if (lane == 0) bars->block = at;
     }
+    tc_fence_before();
     __syncthreads();
+    tc_fence_after();
     const PackedBlock at = bars->block;
     q0 = at.qblk * C::BM;
     sp = at.keys - at.rows;
@@ -140,35 +166,11 @@ __global__ void __launch_bounds__(256, 1)
   }
   const int n_items = n == 0 ? 0 : 2 * n;
 
-  if (threadIdx.x == 0) {
-    mbar_init(&bars->q_full, 1);
-    mbar_init(&bars->q_tmem, 128);
-    for (int s = 0; s < C::STAGES; ++s) {
-      mbar_init(&bars->kv_full[s], 1);
-      mbar_init(&bars->kv_empty[s], 1);
-    }
-    for (int s = 0; s < 2; ++s) {
-      mbar_init(&bars->s_full[s], 1);
-      mbar_init(&bars->p_full[s], 128);
-    }
-    mbar_init(&bars->pv_done, 1);
-    mbar_init(&bars->o_full, 1);
-    mbar_init(&bars->drain, 1);
-    bars->abort_flag = 0;
-    fence_mbar_init();
+  if constexpr (!PACKED) {
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
   }
-  if (warp == 0 && lane == 0) {
-    tma_prefetch_desc(&tm_q);
-    tma_prefetch_desc(&tm_k);
-    tma_prefetch_desc(&tm_v);
-  }
-  if (warp == 1) {
-    tmem_alloc(&bars->tmem_base, C::TMEM_COLS);
-    tmem_relinquish();
-  }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
   const uint32_t tmem = bars->tmem_base;
 
   if (warp < 4) {
