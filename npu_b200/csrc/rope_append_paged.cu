@@ -19,6 +19,11 @@
 // STEPS rows per thread of one token, its loads issued before the token's
 // sequence, position and page are looked up, so the two latencies overlap;
 // the tables are read once per warp and reused for its heads.
+//
+// Measured on one B200 (device time): 10209 prompt tokens, 16 / 2 heads of 256
+// with norms and 64 turned lanes: 47 us, 4.7 TB/s (0.73 of the measured copy
+// rate; issue slots at 64 % are the next bound); 64 single tokens, 32 / 4 heads
+// of 128: 3.0 us, one launch.
 #include "rope_append_paged.cuh"
 
 namespace b2a {

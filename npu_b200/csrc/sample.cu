@@ -19,10 +19,18 @@
 //
 // A row is spread over a cluster of CTAs. Each copies its slice of the
 // logits to shared memory once (one bulk copy), so every later pass reads
-// shared memory, and asks for its slice of the noise in L2 at the same time;
-// the passes' results are joined through the cluster's shared memory in a
-// fixed order. The first race reads the noise once; later ones only for the
-// tokens ahead of the pivot.
+// shared memory, and asks for its slice of the noise in L2 at the same time if
+// all of it is wanted; the passes' results are joined through the cluster's
+// shared memory in a fixed order. The first race reads the noise whole, or
+// only for tokens above a cut where min_p or top_k gives one; later ones only
+// for the tokens ahead of the pivot.
+//
+// Bound by memory in the plain cases, by the latency of the passes (a join is
+// 1 us) with filters. Measured on one B200 (device time), 256 rows of 131071
+// bf16 logits: greedy 21 us (3.2 TB/s), unfiltered 47 us (4.3 TB/s of logits
+// and noise), min_p 0.05 28 us, top_k 50 65 us, top_p 0.9 87 us, each row its
+// own of such settings 70 us; one row of 49152 fp32 logits: greedy 3.3 us,
+// unfiltered 4.7, top_k 50 with top_p 0.95 8.2.
 #include "capi_internal.cuh"
 #include "sample.cuh"
 
