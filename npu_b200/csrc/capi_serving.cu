@@ -73,8 +73,7 @@ int b2a_prefill_varlen(const void* q, const void* k, const void* v, const void* 
     return B2A_ERR_ALIGNMENT;
   const b2a::PrefillPlan plan = b2a::prefill_plan_packed(D, Hq, Hkv, Nq, B);
   const int rows = plan.rows_per_item;
-  // Query blocks: at most one short one per sequence, and one row each.
-  const long long n_qblk = std::min((long long)Nq, (Nq + (long long)B * (rows - 1)) / rows);
+  const long long n_qblk = b2a::packed_blocks(Nq, B, rows);
   if (n_qblk * Hq > INT_MAX) return B2A_ERR_INVALID_ARG;
 
   int* err = nullptr;
@@ -117,7 +116,8 @@ int b2a_prefill_varlen(const void* q, const void* k, const void* v, const void* 
 size_t b2a_decode_paged_workspace_bytes(int B, int Hq, int Hkv, int D) {
   if (B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || Hq / Hkv > 16 || !head_dim_ok(D)) return 0;
   const size_t rows = b2a::decode_paged_parts(B, Hkv, b2a::decode_paged_max_ctas(D, b2a::api_sm_count())) * (Hq / Hkv);
-  return b2a::api_align256(rows * D * sizeof(float)) + b2a::api_align256(rows * 2 * sizeof(float));
+  return b2a::api_align256(rows * D * sizeof(float)) + b2a::api_align256(rows * 2 * sizeof(float)) +
+         ((size_t)B + 1) * sizeof(long long);
 }
 
 int b2a_decode_paged(const void* q, const void* k_pages, const void* v_pages, const int* block_table,
@@ -181,10 +181,13 @@ int b2a_decode_paged(const void* q, const void* k_pages, const void* v_pages, co
   p.scale_log2 = scale * b2a::kApiLog2e;
   p.err = err;
   p.n_ctas = b2a::decode_paged_max_ctas(D, b2a::api_sm_count());
-  p.part_o = static_cast<float*>(workspace);
-  p.part_ml = reinterpret_cast<float*>(static_cast<char*>(workspace) +
-                                       b2a::api_align256(b2a::decode_paged_parts(B, Hkv, p.n_ctas) * p.group * D *
-                                                         sizeof(float)));
+  const size_t rows = b2a::decode_paged_parts(B, Hkv, p.n_ctas) * p.group;
+  char* scratch = static_cast<char*>(workspace);
+  p.part_o = reinterpret_cast<float*>(scratch);
+  scratch += b2a::api_align256(rows * D * sizeof(float));
+  p.part_ml = reinterpret_cast<float*>(scratch);
+  if ((long long)B * Hq > (long long)b2a::kJoinWave * b2a::api_sm_count())
+    p.units = reinterpret_cast<long long*>(scratch + b2a::api_align256(rows * 2 * sizeof(float)));
   return status_of(b2a::launch_decode_paged(D, tk, tv, p, static_cast<cudaStream_t>(stream)));
 }
 

@@ -182,6 +182,7 @@ __device__ __forceinline__ int units_of(int tiles) { return tiles > 0 ? tiles + 
 // All units of the call (all lanes get it). Warp-collective.
 __device__ __forceinline__ long long total_units(const DecodePagedParams& p) {
   long long n = 0;
+#pragma unroll 4
   for (int b0 = 0; b0 < p.B; b0 += 32) {
     const int b = b0 + (threadIdx.x & 31);
     n += __reduce_add_sync(0xffffffffu, b < p.B ? units_of(tiles_of(p, b)) : 0);
@@ -280,6 +281,21 @@ __global__ void __launch_bounds__(PagedCfg<D>::THREADS, PagedCfg<D>::CTAS_PER_SM
       if (p.seqlens[b] < 0 || p.seqlens[b] > (long long)p.table_width * p.page) atomicOr(p.err, kErrBadArgs);
   long long from = 0, count = 1;
   if constexpr (SPLIT) {
+    if (p.units && blockIdx.x == gridDim.x - 1 && warp == 0) {
+      long long before = 0;
+      for (int b0 = 0; b0 < p.B; b0 += 32) {
+        const int n = b0 + lane < p.B ? units_of(tiles_of(p, b0 + lane)) : 0;
+        int upto = n;
+#pragma unroll
+        for (int off = 1; off < 32; off *= 2) {
+          const int y = __shfl_up_sync(0xffffffffu, upto, off);
+          if (lane >= off) upto += y;
+        }
+        if (b0 + lane < p.B) p.units[b0 + lane] = before + upto - n;
+        before += __shfl_sync(0xffffffffu, upto, 31);
+      }
+      if (lane == 0) p.units[p.B] = before;
+    }
     const long long total = total_units(p), share = share_of(total, p.n_ctas);
     from = blockIdx.x * share;
     count = min(share, total - from);
@@ -583,7 +599,8 @@ constexpr int kJoinThreads = 256;
 // and joined in a fixed order. The lengths are read before the wait for the
 // main kernel (which does not write them); so is everything else once, for
 // nothing, which brings the instructions and the gate on chip while the main
-// kernel's last CTAs still run.
+// kernel's last CTAs still run. Where the joining CTAs come in many waves
+// (p.units) they do neither.
 template <int D>
 __global__ void __launch_bounds__(kJoinThreads) decode_paged_join_kernel(const __grid_constant__ DecodePagedParams p) {
   constexpr int TEAM = D / 4, TEAMS = kJoinThreads / TEAM;
@@ -593,10 +610,16 @@ __global__ void __launch_bounds__(kJoinThreads) decode_paged_join_kernel(const _
   const int b = blockIdx.x / p.Hq, h = blockIdx.x % p.Hq;
   const int g = h / p.group, r = h % p.group;
   long long total = 0, before = 0;  // units of all sequences, and of those before b
-  for (int b0 = 0; b0 < p.B; b0 += 32) {
-    const int n = b0 + lane < p.B ? units_of(tiles_of(p, b0 + lane)) : 0;
-    total += __reduce_add_sync(0xffffffffu, n);
-    before += __reduce_add_sync(0xffffffffu, b0 + lane < b ? n : 0);
+  if (p.units) {
+    grid_dep_wait();
+    total = __ldcg(p.units + p.B);
+    before = __ldcg(p.units + b);
+  } else {
+    for (int b0 = 0; b0 < p.B; b0 += 32) {
+      const int n = b0 + lane < p.B ? units_of(tiles_of(p, b0 + lane)) : 0;
+      total += __reduce_add_sync(0xffffffffu, n);
+      before += __reduce_add_sync(0xffffffffu, b0 + lane < b ? n : 0);
+    }
   }
   const int tiles = tiles_of(p, b);
   const long long share = share_of(total * p.Hkv, p.n_ctas);
@@ -606,7 +629,7 @@ __global__ void __launch_bounds__(kJoinThreads) decode_paged_join_kernel(const _
   const int parts = tiles > 0 ? (int)((lo + tiles - 1) / share - c0) + 1 : 0;
   const long long row0 = ((long long)b * p.Hkv + g + c0) * p.group + r;  // part i's row: row0 + i group
 #pragma unroll 1
-  for (int pass = 0; pass < 2; ++pass) {
+  for (int pass = p.units ? 1 : 0; pass < 2; ++pass) {
     if (pass == 1) grid_dep_wait();
     float m = -INFINITY, l = 0.f;
     float4 o = zero4();

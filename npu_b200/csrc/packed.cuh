@@ -27,6 +27,11 @@ namespace b2a {
 // bisection, and is the (i - S(w + 1))-th of it, found with ballots.
 // Warp-collective. A call takes about log2(longest / kRows) sums of B / 32
 // steps each, on lengths that stay in L1.
+//
+// Above kPackedByPosition sequences, block i is slot i - s(b) of the last
+// sequence with s(b) <= i, s(b) = cu_q[b] / kRows + b: s(b + 1) - s(b) is at
+// least the sequence's number of blocks, and b is found by a search that
+// narrows 32-fold a step.
 template <int kRows>
 struct PackedBlocks {
   const PrefillParams& p;
@@ -47,7 +52,9 @@ struct PackedBlocks {
   }
   __device__ __forceinline__ explicit PackedBlocks(const PrefillParams& params) : p(params) {
     const int lane = threadIdx.x & 31;
+    if (p.B > kPackedByPosition) return;
     int most = 0;
+#pragma unroll 4
     for (int b0 = 0; b0 < p.B; b0 += 32) {
       shape(b0 + lane, own_n, own_off);
       most = max(most, own_n > 0 ? own_n + own_off : 0);
@@ -57,6 +64,7 @@ struct PackedBlocks {
   __device__ __forceinline__ int count_from(int w) const {
     const int lane = threadIdx.x & 31;
     int c = 0;
+#pragma unroll 4
     for (int b0 = 0; b0 < p.B; b0 += 32) {
       int n = own_n, off = own_off;
       if (p.B > 32) shape(b0 + lane, n, off);
@@ -64,10 +72,28 @@ struct PackedBlocks {
     }
     return __reduce_add_sync(0xffffffffu, c);
   }
+  // Block qblk of sequence b, empty if the sequence has no such block.
+  __device__ __forceinline__ PackedBlock block(int b, int qblk) const {
+    int n, off;
+    shape(b, n, off);
+    if (qblk < 0 || qblk >= n) return {0, 0, 0, 0, 0};
+    return {p.cu_q[b], p.cu_q[b + 1] - p.cu_q[b], p.cu_k[b], p.cu_k[b + 1] - p.cu_k[b], qblk};
+  }
   // Block i (every lane gets it). Calls with growing i stay below the last
   // level found.
   __device__ __forceinline__ PackedBlock find(int i) {
     const int lane = threadIdx.x & 31;
+    if (p.B > kPackedByPosition) {
+      int lo = 0, len = p.B;
+      while (len > 1) {
+        const int step = (len + 31) / 32, b = lo + lane * step;
+        const bool before = lane * step < len && (lane == 0 || p.cu_q[b] / kRows + b <= i);
+        const int hit = 31 - __clz(__ballot_sync(0xffffffffu, before));
+        len = min(step, len - hit * step);
+        lo += hit * step;
+      }
+      return block(lo, i - (p.cu_q[lo] / kRows + lo));
+    }
     int lo = 0, hi = top;  // S(hi + 1) <= i always; looking for the largest w with S(w) > i
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
@@ -87,13 +113,7 @@ struct PackedBlocks {
         const bool it = has && __popc(m & ((1u << lane) - 1u)) == skip;
         const int src = __ffs(__ballot_sync(0xffffffffu, it)) - 1;
         const int b = b0 + src;
-        PackedBlock k;
-        k.q_base = p.cu_q[b];
-        k.rows = p.cu_q[b + 1] - k.q_base;
-        k.k_base = p.cu_k[b];
-        k.keys = p.cu_k[b + 1] - k.k_base;
-        k.qblk = lo - __shfl_sync(0xffffffffu, off, src);
-        return k;
+        return block(b, lo - __shfl_sync(0xffffffffu, off, src));
       }
       skip -= __popc(m);
     }

@@ -127,6 +127,19 @@ struct PrefillCfg {
   static_assert(MIN_LAUNCH_REGS * THREADS * CTAS_PER_SM <= 65536, "register budget");
 };
 
+// PACKED: above this many sequences the blocks are numbered by position
+// instead of heaviest first (packed.cuh): with so many none is a large part of
+// the work, and the sums over all of them would be (4096 prompts of 1 to 39
+// tokens: 4.6 ms with them).
+constexpr int kPackedByPosition = 256;
+
+// The query blocks the grid provides for.
+inline long long packed_blocks(long long rows, int B, int block_rows) {
+  if (B > kPackedByPosition) return rows / block_rows + B;
+  const long long most = (rows + (long long)B * (block_rows - 1)) / block_rows;  // one short one each
+  return most < rows ? most : rows;                                              // and a row each
+}
+
 // PACKED: one query block of one sequence. Empty (rows == 0) for the grid's
 // spare blocks.
 struct PackedBlock {

@@ -74,7 +74,8 @@ def test_lengths_pages_and_heads(cuda_dev, Hq, Hkv, D, page, out_dtype):
     check(out, q, ks, vs, 1 / math.sqrt(D))
 
 
-@pytest.mark.parametrize("lens", [[20000], [3, 9000, 1, 700, 0, 12345], [500] * 40, [1] * 200])
+@pytest.mark.parametrize("lens", [[20000], [3, 9000, 1, 700, 0, 12345], [500] * 40, [1] * 200,
+                                  [0, 700, 33] * 45])
 @pytest.mark.parametrize("Hq,Hkv,D", [(9, 3, 64), (32, 4, 128), (16, 2, 256)])
 def test_long_and_many(cuda_dev, lens, Hq, Hkv, D):
     from npu_b200 import decode_paged

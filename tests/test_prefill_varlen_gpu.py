@@ -107,7 +107,7 @@ def test_keys_of_their_own(cuda_dev, causal, Hq, Hkv, D):
     assert (out[253:260] == 0).all()  # the sequence without keys
 
 
-@pytest.mark.parametrize("B", [33, 70, 300])
+@pytest.mark.parametrize("B", [33, 70, 300, 1500])
 @pytest.mark.parametrize("Hq,Hkv,D", [(3, 1, 64), (4, 2, 128), (2, 1, 256)])
 def test_many_sequences(cuda_dev, B, Hq, Hkv, D):
     from npu_b200 import prefill_varlen
@@ -170,6 +170,17 @@ def test_same_bits_as_the_dense_kernel_at_head_dim_128(cuda_dev):
     out = prefill_varlen(q, k, v, offsets([900, 900]).to(cuda_dev))
     dense = prefill(*(x.view(2, 900, -1, 128).transpose(1, 2) for x in (q, k, v)))
     assert torch.equal(out.view(2, 900, 8, 128).transpose(1, 2), dense)
+
+
+@pytest.mark.parametrize("Hq,Hkv,D", HEADS)
+def test_no_keys_at_all_and_no_rows(cuda_dev, Hq, Hkv, D):
+    from npu_b200 import prefill_varlen
+
+    q, k, v = inputs(cuda_dev, [30, 200], [0], Hq, Hkv, D, seed=13)
+    none = torch.zeros(3, dtype=torch.int32, device=cuda_dev)
+    out, lse = prefill_varlen(q, k, v, offsets([30, 200]).to(cuda_dev), none, return_lse=True)
+    assert (out == 0).all() and torch.isinf(lse).all()
+    assert prefill_varlen(q[:0], k, v, none, none).shape == (0, Hq, D)
 
 
 def test_on_another_stream(cuda_dev):

@@ -74,6 +74,12 @@ def test_settings_and_sizes(cuda_dev, T, k, p, m, R, V, dtype):
     compare(*draw(cuda_dev, R, V, dtype, seed=V + R), T, k, p, m)
 
 
+@pytest.mark.parametrize("T,k,p,m", [SETTINGS[0], SETTINGS[1], SETTINGS[4], SETTINGS[9]])
+@pytest.mark.parametrize("V,dtype", [(300_001, torch.bfloat16), (450_000, torch.float32)])
+def test_vocabularies_past_a_slice_of_shared_memory(cuda_dev, T, k, p, m, V, dtype):
+    compare(*draw(cuda_dev, 1, V, dtype, seed=V), T, k, p, m)
+
+
 @pytest.mark.parametrize("R,V,dtype", [(300, 700, torch.float32), (64, 5001, torch.bfloat16)])
 def test_each_row_its_own_settings(cuda_dev, R, V, dtype):
     x, e = draw(cuda_dev, R, V, dtype, seed=R)
