@@ -275,7 +275,11 @@ __global__ void __launch_bounds__(PagedCfg<D>::THREADS, PagedCfg<D>::CTAS_PER_SM
   volatile int* abort_flag = &bars->abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  if constexpr (SPLIT) grid_dep_launch();  // the joining kernel may take SM slots as they free up
+  grid_dep_wait();
+  // The next kernel (the joining one when SPLIT) may take SM slots as they
+  // free up; after the wait, so that what it reads ahead of its own wait (the
+  // lengths) is final.
+  grid_dep_launch();
   if (p.err && blockIdx.x == 0)
     for (int b = threadIdx.x; b < p.B; b += C::THREADS)
       if (p.seqlens[b] < 0 || p.seqlens[b] > (long long)p.table_width * p.page) atomicOr(p.err, kErrBadArgs);
@@ -630,7 +634,10 @@ __global__ void __launch_bounds__(kJoinThreads) decode_paged_join_kernel(const _
   const long long row0 = ((long long)b * p.Hkv + g + c0) * p.group + r;  // part i's row: row0 + i group
 #pragma unroll 1
   for (int pass = p.units ? 1 : 0; pass < 2; ++pass) {
-    if (pass == 1) grid_dep_wait();
+    if (pass == 1) {
+      grid_dep_wait();
+      grid_dep_launch();
+    }
     float m = -INFINITY, l = 0.f;
     float4 o = zero4();
     for (int i0 = team; i0 < parts; i0 += 4 * TEAMS) {
@@ -694,8 +701,8 @@ int launch_main(const CUtensorMap& tk, const CUtensorMap& tv, const DecodePagedP
                                     C::SMEM_BYTES) == cudaSuccess;
       }))
     return -1;
-  decode_paged_kernel<D, NT, SPLIT><<<(unsigned)n, C::THREADS, C::SMEM_BYTES, st>>>(tk, tv, p);
-  return once.launched(cudaGetLastError());
+  return once.launched(launch_dependent(decode_paged_kernel<D, NT, SPLIT>, dim3((unsigned)n), C::THREADS,
+                                        C::SMEM_BYTES, st, 0, tk, tv, p));
 }
 
 template <int D>
@@ -710,19 +717,9 @@ int launch_t(const CUtensorMap& tk, const CUtensorMap& tv, const DecodePagedPara
   const int rc =
       narrow ? launch_main<D, 1, true>(tk, tv, p, p.n_ctas, st) : launch_main<D, 2, true>(tk, tv, p, p.n_ctas, st);
   if (rc) return rc;
-  // The joining kernel is scheduled while the main one drains and waits for
-  // all of it before it reads anything.
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)heads);
-  cfg.blockDim = dim3(kJoinThreads);
-  cfg.stream = st;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, decode_paged_join_kernel<D>, p) != cudaSuccess) return -1;
-  return cudaGetLastError() == cudaSuccess ? 0 : -1;
+  return launch_dependent(decode_paged_join_kernel<D>, dim3((unsigned)heads), kJoinThreads, 0, st, 0, p) == cudaSuccess
+             ? 0
+             : -1;
 }
 
 }  // namespace

@@ -138,6 +138,7 @@ __global__ void __launch_bounds__(PrefillCfg<D, NQT>::THREADS, PrefillCfg<D, NQT
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
+  if constexpr (PACKED && NQT == 1) grid_dep_wait();  // see launch_prefill_t
   auto wait_all = [&](uint64_t* bar, uint32_t parity) -> bool {
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, p.err));
   };
@@ -758,6 +759,11 @@ static int launch_prefill_t(const CUtensorMap& tq, const CUtensorMap& tk, const 
   // One CTA per work item (query blocks x query heads, or x head pairs).
   const long long nblk = (long long)p.n_qblk * (PACKED ? 1 : p.B) * (p.head_pairs ? p.Hq / 2 : p.Hq);
   if (nblk <= 0 || nblk > 0x7fffffffLL) return -2;
+  // Short packed prompts: the launch overlaps the kernel before (6.8 us a call
+  // against 8.2 at 3 prompts of 1 to 40 tokens). The larger items gain nothing.
+  if (PACKED && NQT == 1)
+    return once.launched(
+        launch_dependent(kernel, dim3((unsigned)nblk), C::THREADS, C::SMEM_BYTES, st, 0, tq, tk, tv, p));
   kernel<<<(unsigned)nblk, C::THREADS, C::SMEM_BYTES, st>>>(tq, tk, tv, p);
   return once.launched(cudaGetLastError());
 }

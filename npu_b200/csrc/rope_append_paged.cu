@@ -24,6 +24,7 @@
 // with norms and 64 turned lanes: 47 us, 4.7 TB/s (0.73 of the measured copy
 // rate; issue slots at 64 % are the next bound); 64 single tokens, 32 / 4 heads
 // of 128: 3.0 us, one launch.
+#include "capi_internal.cuh"
 #include "rope_append_paged.cuh"
 
 namespace b2a {
@@ -106,6 +107,8 @@ __global__ void __launch_bounds__(32 * kWarps)
   constexpr int ROWS = 32 / LPR;   // rows of a warp at a time
   const int lane = threadIdx.x & 31, part = lane % LPR;
   const long long n = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5);  // token
+  grid_dep_wait();
+  grid_dep_launch();
   if (blockIdx.x == 0 && blockIdx.y == 0 && p.seqlens_out)
     for (int b = threadIdx.x; b < p.B; b += 32 * kWarps)
       p.seqlens_out[b] = (p.start_pos_arr ? p.start_pos_arr[b] : p.start_pos) + p.cu_seqlens[b + 1] - p.cu_seqlens[b];
@@ -244,9 +247,10 @@ int launch_steps(const RopeAppendPagedParams& p, cudaStream_t st) {
   const int q_chunks = (p.Hq + STEPS * ROWS - 1) / (STEPS * ROWS);
   const int chunks = q_chunks + (2 * p.Hkv + STEPS * ROWS - 1) / (STEPS * ROWS);
   if (blocks <= 0 || blocks > 0x7fffffffLL || chunks > 65535) return -2;
-  rope_append_paged_kernel<Src, D, STEPS>
-      <<<dim3((unsigned)blocks, (unsigned)chunks), 32 * kWarps, 0, st>>>(p, q_chunks);
-  return cudaGetLastError() == cudaSuccess ? 0 : -1;
+  return launch_dependent(rope_append_paged_kernel<Src, D, STEPS>, dim3((unsigned)blocks, (unsigned)chunks),
+                          32 * kWarps, 0, st, 0, p, q_chunks) == cudaSuccess
+             ? 0
+             : -1;
 }
 
 // Four rows per thread spread a token's lookups over more rows; few tokens get

@@ -227,6 +227,8 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleParams 
   // Waited for before the first join: every CTA has started and its barriers
   // are ready.
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  grid_dep_wait();
+  grid_dep_launch();
   const int r = blockIdx.x / size;
   const int begin = min((int)rank * p.slice, p.V);
   const int n = min(p.slice, p.V - begin);  // this CTA's tokens [begin, begin + n)
@@ -503,19 +505,8 @@ int launch_t(const SampleParams& p, size_t smem, cudaStream_t st) {
                                     kMaxStageBytes) == cudaSuccess;
       }))
     return -1;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)p.cluster;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(p.R * p.cluster));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, sample_kernel<T, STAGED>, p);
-  return once.launched(e == cudaSuccess ? cudaGetLastError() : e);
+  return once.launched(launch_dependent(sample_kernel<T, STAGED>, dim3((unsigned)(p.R * p.cluster)), kThreads, smem, st,
+                                        p.cluster, p));
 }
 
 template <typename T>
