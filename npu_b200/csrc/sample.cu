@@ -234,7 +234,10 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleParams 
   const int n = min(p.slice, p.V - begin);  // this CTA's tokens [begin, begin + n)
   const T* logits = static_cast<const T*>(p.logits) + r * p.ld_logits + begin;
   const float* noise = p.noise + r * p.ld_noise + begin;
-  const float temperature = p.temperature ? p.temperature[r] : p.temperature_all;
+  // The highest number does what +inf would, all finite logits weigh 1, and
+  // times 0 is 0.
+  const float given = p.temperature ? p.temperature[r] : p.temperature_all;
+  const float temperature = given == INFINITY ? 3.402823466e38f : given;
   const int top_k = p.top_k ? p.top_k[r] : p.top_k_all;
   const float top_p = p.top_p ? p.top_p[r] : p.top_p_all;
   const float min_p = p.min_p ? p.min_p[r] : p.min_p_all;
@@ -350,7 +353,7 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleParams 
   // of this CTA alone have a logit of at least `cut`. The second bound is
   // bisected on the threads' maxima, down to an eighth of T.
   float cut = -INFINITY;
-  if (min_p > 0.f && !infinite) cut = m + temperature * (__logf(min_p) - 1e-4f) - 1e-6f * fabsf(m);
+  if (min_p > 0.f && !infinite) cut = m + given * (__logf(min_p) - 1e-4f) - 1e-6f * fabsf(m);
   if (top_k > 0 && top_k <= kThreads && !infinite) {
     float hi = m, lo = m - 32.f * temperature;
     if (__syncthreads_count(own_max >= lo) >= top_k) {

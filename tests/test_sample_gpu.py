@@ -158,3 +158,11 @@ def test_noise_against_the_ranking_still_ends(cuda_dev):
     x = torch.linspace(0, -5, 3000, device=cuda_dev)[None].repeat(2, 1)
     e = torch.exp(2 * x) + 1e-6
     compare(x, e, 1.0, 5, 1.0, 0.0)
+
+
+@pytest.mark.parametrize("k,p,m", [(0, 1.0, 0.0), (40, 1.0, 0.0), (0, 0.4, 0.0), (0, 1.0, 0.5)])
+def test_an_infinite_temperature_weighs_all_logits_alike(cuda_dev, k, p, m):
+    x, e = draw(cuda_dev, 6, 9001, seed=8)
+    x[1, ::3] = torch.finfo(torch.float32).min
+    T = torch.tensor([math.inf, math.inf, 1.0, math.inf, 1e30, math.inf], device=cuda_dev)
+    compare(x, e, T, k, p, m)
