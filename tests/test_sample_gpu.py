@@ -38,10 +38,13 @@ def defined(x, e, T, k, p, m):
     return -kept[0][1], best == 0 or max(second, *maybe) < best * (1 - 1e-5)
 
 
-def compare(logits, noise, T, k, p, m):
+def compare(logits, noise, T, k, p, m, rows=None):
     from npu_b200 import sample
 
-    got = sample(logits, noise, temperature=T, top_k=k, top_p=p, min_p=m).tolist()
+    got = sample(logits, noise, temperature=T, top_k=k, top_p=p, min_p=m)
+    if rows is not None:  # of these only
+        logits, noise, got = logits[rows], noise[rows], got[rows]
+    got = got.tolist()
     R = logits.shape[0]
     rows = [t.tolist() if isinstance(t, torch.Tensor) else [t] * R for t in (T, k, p, m)]
     x, e = logits.double().tolist(), noise.double().tolist()
@@ -166,3 +169,19 @@ def test_an_infinite_temperature_weighs_all_logits_alike(cuda_dev, k, p, m):
     x[1, ::3] = torch.finfo(torch.float32).min
     T = torch.tensor([math.inf, math.inf, 1.0, math.inf, 1e30, math.inf], device=cuda_dev)
     compare(x, e, T, k, p, m)
+
+
+@pytest.mark.parametrize("T,k,p,m", SETTINGS)
+@pytest.mark.parametrize("R,V,dtype", [(6, 40_001, torch.float32), (160, 20_000, torch.bfloat16)])
+def test_a_row_whose_parts_differ(cuda_dev, T, k, p, m, R, V, dtype):
+    """Long rows are shared by several blocks: parts without a usable logit, far below the row's maximum, or with
+    its only infinities."""
+    x, e = draw(cuda_dev, R, V, dtype, seed=9)
+    x[0, : V // 2] = -math.inf
+    x[1, V // 8 :] = math.nan
+    x[2, : V - V // 8] -= 60
+    x[3, V // 3] = x[3, V - 2] = math.inf
+    x[4, V // 4 : V // 2] = torch.finfo(dtype).min
+    x[5] = -math.inf
+    near = torch.cat([torch.arange(6), torch.arange(R - 2, R)]).to(cuda_dev) if R > 8 else slice(None)
+    compare(x, e, T, k, p, m, near)
