@@ -529,8 +529,10 @@ __global__ void __launch_bounds__(PrefillCfg<D, NQT>::THREADS, PrefillCfg<D, NQT
       if constexpr (PACKED && NQT == 1) {
         // Short sequences: the steps of the other branch with every piece of
         // code once (softmax_half_packed), the two halves of a block as rounds
-        // of a loop. 8 % faster at 32 prompts of 17 to 2048 tokens (49 us
-        // against 53), 11 % slower in the two-tile items of long ones.
+        // of a loop. Measured at head dim 64, before that had a kernel of its
+        // own (prefill_packed_d64.cu): 8 % faster at 32 prompts of 17 to 2048
+        // tokens (49 us against 53), 11 % slower in the two-tile items of long
+        // ones.
         auto rescale = [&](float f) {
 #pragma unroll 1
           for (int c = 0; c < D / 32; ++c) {
@@ -759,8 +761,9 @@ static int launch_prefill_t(const CUtensorMap& tq, const CUtensorMap& tk, const 
   // One CTA per work item (query blocks x query heads, or x head pairs).
   const long long nblk = (long long)p.n_qblk * (PACKED ? 1 : p.B) * (p.head_pairs ? p.Hq / 2 : p.Hq);
   if (nblk <= 0 || nblk > 0x7fffffffLL) return -2;
-  // Short packed prompts: the launch overlaps the kernel before (6.8 us a call
-  // against 8.2 at 3 prompts of 1 to 40 tokens). The larger items gain nothing.
+  // Short packed prompts: the launch overlaps the kernel before (at head dim 64
+  // 6.8 us a call against 8.2 at 3 prompts of 1 to 40 tokens). The larger items
+  // gain nothing.
   if (PACKED && NQT == 1)
     return once.launched(
         launch_dependent(kernel, dim3((unsigned)nblk), C::THREADS, C::SMEM_BYTES, st, 0, tq, tk, tv, p));
@@ -819,7 +822,7 @@ int launch_prefill_packed(int D, const PrefillPlan& plan, const CUtensorMap& tq,
   const bool one = plan.tiles == 1;
   switch (D) {
     case 64:
-      return one ? launch_prefill_t<64, 1, false, true>(tq, tk, tv, p, st)
+      return one ? launch_prefill_packed_d64(tq, tk, tv, p, st)
                  : (plan.head_pairs ? launch_prefill_t<64, 2, true, true>(tq, tk, tv, p, st)
                                     : launch_prefill_t<64, 2, false, true>(tq, tk, tv, p, st));
     case 128:
