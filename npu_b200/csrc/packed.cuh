@@ -2,10 +2,9 @@
 // sequence an item is, found on the device from the offsets alone (no plan,
 // no workspace, no copy of the lengths to the host).
 //
-// The kernels are prefill_packed_d64.cu, and prefill.cu's and prefill_d256.cu's
-// with PACKED: a
-// sequence's rows and keys are offsets into one tensor map each. Measured on
-// one B200 (device time): prompts of 1122, 1593, 2780 and 8192 tokens, 32 / 4
+// The kernels are prefill_packed_d64.cu, and prefill.cu's (head dim 128) and
+// prefill_d256.cu's with PACKED: a sequence's rows and keys are offsets into
+// one tensor map each. Measured on one B200 (device time): prompts of 1122, 1593, 2780 and 8192 tokens, 32 / 4
 // heads of 128: 590 us, 1.09 PFLOP/s (0.66 of the measured bf16 rate, as the
 // dense kernel); chunks of 65 to 2501 gated tokens behind 500 cached ones,
 // 16 / 2 heads of 256: 205 us, 0.81 PFLOP/s; 32 prompts of 17 to 2048 tokens,

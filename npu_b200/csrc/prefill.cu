@@ -807,11 +807,15 @@ PrefillPlan prefill_plan(int D, int Hq, int Hkv, int Tq, int Tk) {
   return PrefillPlan{256, 2, 0, 0};
 }
 
-// Packed sequences: by the same rules on the average length (the lengths
+// Packed sequences: head dim 64 and 256 have kernels of their own with one-tile
+// items (at 64 faster than two-tile items at every length measured: 8 prompts
+// of 1500, 9 / 3 heads, 55.8 us against 57.2; 4 of 4096, 136.7 against 146.8;
+// 24 of 700, 8 / 2 heads, 45.2 against 50.2; 4 of 4096, 125.6 against 132.0).
+// Head dim 128 goes by the same rules on the average length (the lengths
 // themselves are on the device). Row pairs only for odd groups: an even group
 // shares its key blocks between heads at any length.
 PrefillPlan prefill_plan_packed(int D, int Hq, int Hkv, long long rows, int B) {
-  if (D == 256) return PrefillPlan{128, 1, 0, 0};
+  if (D != 128) return PrefillPlan{128, 1, 0, 0};
   const long long mean = rows / B;
   if ((Hq / Hkv) % 2 == 0) return mean >= kHeadPairMinRows ? PrefillPlan{128, 2, 1, 0} : PrefillPlan{128, 1, 0, 0};
   return mean <= kOneTileMaxRows ? PrefillPlan{128, 1, 0, 0} : PrefillPlan{256, 2, 0, 0};
@@ -821,10 +825,7 @@ int launch_prefill_packed(int D, const PrefillPlan& plan, const CUtensorMap& tq,
                           const CUtensorMap& tv, const PrefillParams& p, cudaStream_t st) {
   const bool one = plan.tiles == 1;
   switch (D) {
-    case 64:
-      return one ? launch_prefill_packed_d64(tq, tk, tv, p, st)
-                 : (plan.head_pairs ? launch_prefill_t<64, 2, true, true>(tq, tk, tv, p, st)
-                                    : launch_prefill_t<64, 2, false, true>(tq, tk, tv, p, st));
+    case 64: return launch_prefill_packed_d64(tq, tk, tv, p, st);
     case 128:
       return one ? launch_prefill_t<128, 1, false, true>(tq, tk, tv, p, st)
                  : (plan.head_pairs ? launch_prefill_t<128, 2, true, true>(tq, tk, tv, p, st)

@@ -189,7 +189,7 @@ PrefillPlan prefill_plan_packed(int D, int Hq, int Hkv, long long rows, int B);
 int launch_prefill_packed(int D, const PrefillPlan& plan, const CUtensorMap& tq, const CUtensorMap& tk,
                           const CUtensorMap& tv, const PrefillParams& p, cudaStream_t st);
 int launch_prefill_packed_d64(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
-                              const PrefillParams& p, cudaStream_t st);  // one-tile items (prefill_packed_d64.cu)
+                              const PrefillParams& p, cudaStream_t st);
 int launch_prefill_packed_d256(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
                                const PrefillParams& p, cudaStream_t st);
 
