@@ -26,8 +26,9 @@ BUILD_DIR = PKG / "_build"
 BINDING = PKG / "_serving.so"
 BINDING_SOURCE = CSRC / "serving_binding.cpp"
 
-SOURCES = ["capi.cu", "capi_serving.cu", "prefill.cu", "prefill_pair.cu", "prefill_d256.cu", "prefill_packed_d64.cu",
-           "decode.cu", "decode_noalloc.cu", "rope_append.cu", "rope_append_paged.cu", "decode_paged.cu", "sample.cu", "diag.cu", "host_pipeline.cu"]
+SOURCES = ["capi.cu", "capi_serving.cu", "prefill.cu", "prefill_pair.cu", "prefill_d256.cu",
+           "prefill_packed_d64.cu", "decode.cu", "decode_noalloc.cu", "rope_append.cu", "rope_append_paged.cu",
+           "decode_paged.cu", "sample.cu", "diag.cu", "host_pipeline.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = [
     "-O3", "-std=c++17", "-lineinfo", "--use_fast_math",

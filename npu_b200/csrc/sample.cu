@@ -28,9 +28,9 @@
 // Bound by memory in the plain cases, by the latency of the passes (a join is
 // 1 us) with filters. Measured on one B200 (device time), 256 rows of 131071
 // bf16 logits: greedy 21 us (3.2 TB/s), unfiltered 47 us (4.3 TB/s of logits
-// and noise), min_p 0.05 28 us, top_k 50 65 us, top_p 0.9 87 us, each row its
-// own of such settings 70 us; one row of 49152 fp32 logits: greedy 3.3 us,
-// unfiltered 4.7, top_k 50 with top_p 0.95 8.2.
+// and noise), min_p 0.05 28 us, top_k 50 60 us, top_p 0.9 88 us, each row its
+// own of such settings 58 to 64 us; one row of 49152 fp32 logits: greedy 2.6 us,
+// unfiltered 4.0, top_k 50 with top_p 0.9 6.2.
 #include "capi_internal.cuh"
 #include "sample.cuh"
 

@@ -2,7 +2,7 @@
 // checks, output and workspace allocation and the call of the C ABI in one
 // step. A call through ctypes costs 13 to 24 us of host time for these
 // argument lists, several times what a single-token kernel runs; through this
-// module it costs 3 to 5. npu_b200.api documents the functions.
+// module it costs 4.6 to 5.5. npu_b200.api documents the functions.
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDACachingAllocator.h>
