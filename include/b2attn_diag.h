@@ -31,6 +31,18 @@ B2A_API int b2a_diag_umma_gemm(const void* a, const void* b, float* c, int b_mn_
  */
 B2A_API int b2a_diag_wait_timeout(long long limit_cycles, void* stream);
 
+/*
+ * b2a_sample of contiguous fp32 logits and noise [R, V] with a wait limit of
+ * `limit_cycles` (1 .. 4e9), in which the last block of those that share a row
+ * stops sending its values at pass `mute_pass` (0: the first). Rows whose
+ * passes get that far give -1 and b2a_get_device_error reports
+ * B2A_ERR_DEVICE_TIMEOUT; the others end as usual. Used by the GPU tests to
+ * check that a wait which runs out ends the call.
+ */
+B2A_API int b2a_diag_sample_timeout(const float* logits, const float* noise, int R, int V, float temperature,
+                                    float top_p, int mute_pass, long long limit_cycles, long long* out,
+                                    void* stream);
+
 #ifdef __cplusplus
 }
 #endif

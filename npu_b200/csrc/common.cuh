@@ -89,10 +89,10 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
 // Bounded wait that ignores the abort flag: used on the abort path to let
 // copies and MMAs already in flight land before shared memory / TMEM is
 // released. Gives up silently after the cycle bound.
-__device__ __forceinline__ void mbar_wait_quiet(uint64_t* bar, uint32_t parity) {
+__device__ __forceinline__ void mbar_wait_quiet(uint64_t* bar, uint32_t parity, long long limit = kWaitLimitCycles) {
   const long long t0 = clock64();
   while (!mbar_try_wait(bar, parity)) {
-    if (clock64() - t0 > kWaitLimitCycles) return;
+    if (clock64() - t0 > limit) return;
   }
 }
 

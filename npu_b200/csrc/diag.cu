@@ -9,6 +9,7 @@
 // threads using the 128-byte swizzle formula.
 #include "b2attn_diag.h"
 #include "common.cuh"
+#include "sample.cuh"
 
 namespace b2a {
 
@@ -134,4 +135,27 @@ extern "C" int b2a_diag_umma_gemm(const void* a, const void* b, float* c, int b_
   b2a::diag_umma_kernel<<<1, 128, smem, static_cast<cudaStream_t>(stream)>>>(
       static_cast<const __nv_bfloat16*>(a), static_cast<const __nv_bfloat16*>(b), c, b_mn_major, nullptr);
   return cudaGetLastError() == cudaSuccess ? 0 : -6;
+}
+
+extern "C" int b2a_diag_sample_timeout(const float* logits, const float* noise, int R, int V, float temperature,
+                                       float top_p, int mute_pass, long long limit_cycles, long long* out,
+                                       void* stream) {
+  if (!logits || !noise || !out || R <= 0 || V <= 0 || mute_pass < 0 || limit_cycles <= 0 ||
+      limit_cycles > b2a::kWaitLimitCycles)
+    return B2A_ERR_INVALID_ARG;
+  int* err = b2a::device_error_word();
+  if (!err) return B2A_ERR_CUDA;
+  b2a::SampleParams p{};
+  p.logits = logits;
+  p.noise = noise;
+  p.ld_logits = p.ld_noise = V;
+  p.temperature_all = temperature;
+  p.top_p_all = top_p;
+  p.out = out;
+  p.R = R;
+  p.V = V;
+  p.err = err;
+  p.wait_limit = limit_cycles;
+  p.mute_pass = mute_pass;
+  return b2a::launch_sample_mute(p, static_cast<cudaStream_t>(stream)) ? B2A_ERR_LAUNCH : B2A_OK;
 }

@@ -73,6 +73,7 @@ struct Weight {
 // largest score (ordered bits; 0: none), the lowest token among equals, its
 // logit, and the pass's weight and count.
 constexpr uint32_t kNone = 0xffffffffu;
+constexpr uint32_t kFailed = 0xffffffffu;  // score of a pass in which a wait ran out: above every logit's
 struct alignas(16) Found {
   uint32_t score, token;
   float x, sum;
@@ -160,7 +161,8 @@ struct Cluster {
   Shared* sh;
   int rank, size;
   int* err;
-  int pass = 0;  // joins so far
+  long long limit;  // of a wait, in cycles
+  int pass = 0;     // joins so far
 
   // Address of a shared variable of this CTA in CTA `to`, and a store there
   // that its barrier counts when it lands.
@@ -175,7 +177,9 @@ struct Cluster {
   // no barrier of all the CTAs. A CTA sends for pass n + 2 only after it has
   // everyone's value of pass n + 1, which they sent after reading pass n's:
   // two sets of slots are enough, and after the last pass nothing is under way.
-  __device__ __forceinline__ Found join(Found f) {
+  // A score of kFailed, the CTA's own or a peer's, is what every thread of the
+  // CTA gets if a wait ran out; the caller then leaves by way of leave().
+  __device__ __forceinline__ Found join(Found f, bool mute = false) {
     f = warp_join(f);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (lane == 0) sh->warp[warp] = f;
@@ -186,7 +190,7 @@ struct Cluster {
       f = warp_join(lane < kWarps ? sh->warp[lane] : nothing());
       if (lane == 0) mbar_arrive_expect_tx(bar, size * 20);
       __syncwarp();
-      if (lane < size) {
+      if (lane < size && !mute) {
         const uint32_t to = in_cta(slots + rank, lane), remote_bar = in_cta(bar, lane);
         asm volatile(
             "st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%6];\n\t"
@@ -197,18 +201,33 @@ struct Cluster {
       }
       __syncwarp();
     }
-    const uint32_t parity = (uint32_t)(pass >> 1) & 1u;
-    if (!mbar_wait_limit(bar, parity, &sh->abort_flag, err, kWaitLimitCycles)) mbar_wait_quiet(bar, parity);
-    __syncwarp();
+    const bool all_here = mbar_wait_limit(bar, (uint32_t)(pass >> 1) & 1u, &sh->abort_flag, err, limit);
     ++pass;
+    if (!__syncthreads_and(all_here)) return {kFailed, kNone, 0.f, 0.f, 0};
     return warp_join(lane < size ? slots[lane] : nothing());
+  }
+
+  // Way out of a CTA that got kFailed: it sends nothing more, and its shared
+  // memory stays until no peer can write to it. Every wait of the peers is
+  // bounded too, so each of them gets here or has exited (which counts as
+  // arriving); what the last pass still had under way is waited for, with a
+  // limit, before.
+  __device__ __forceinline__ void leave() {
+    mbar_wait_quiet(&sh->arrived[(pass - 1) & 1], (uint32_t)((pass - 1) >> 1) & 1u, limit);
+    __syncwarp();
+    asm volatile(
+        "barrier.cluster.arrive.release.aligned;\n\t"
+        "barrier.cluster.wait.acquire.aligned;" ::
+            : "memory");
   }
 };
 
 __device__ __forceinline__ float to_float(float x) { return x; }
 __device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
 
-template <typename T, bool STAGED>
+// MUTE: the cluster's last CTA sends nothing from pass p.mute_pass on, so that
+// the others' waits run out (the failure path's test).
+template <typename T, bool STAGED, bool MUTE>
 __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleParams p) {
   constexpr int kPer16 = 16 / sizeof(T);
   extern __shared__ __align__(16) uint8_t stage_raw[];
@@ -248,6 +267,7 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleParams 
   // ragged ends by threads; the rest of the first and last group is -inf.
   const int shift = (int)((reinterpret_cast<uintptr_t>(logits) & 15) / sizeof(T));
   const int groups = (shift + n + kGroup - 1) / kGroup;
+  bool staged = true;  // false: the slice's copy did not land in time
   if constexpr (STAGED) {
     const int head = min(n, (kPer16 - shift) % kPer16);
     const int units = (n - head) / kPer16;
@@ -276,7 +296,8 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleParams 
         i += ((tail + shift - 1 - i) / kThreads) * kThreads;  // the bulk copy's part
     }
     __syncthreads();
-    if (!mbar_wait_limit(&sh.full, 0, &sh.abort_flag, p.err, kWaitLimitCycles)) mbar_wait_quiet(&sh.full, 0);
+    staged = mbar_wait_limit(&sh.full, 0, &sh.abort_flag, p.err, p.wait_limit);
+    if (!staged) mbar_wait_quiet(&sh.full, 0, p.wait_limit);
   }
   // Group g holds tokens [g kGroup - shift, +kGroup) of the slice, -inf outside it.
   auto load_raw = [&](int g, float (&x)[kGroup]) {
@@ -291,7 +312,10 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleParams 
     }
   };
 
-  Cluster cluster{&sh, (int)rank, size, p.err};
+  Cluster cluster{&sh, (int)rank, size, p.err, p.wait_limit};
+  auto join = [&](const Found& f) -> Found {
+    return cluster.join(f, MUTE && (int)rank == size - 1 && cluster.pass >= p.mute_pass);
+  };
   float m = -INFINITY;
   // The larger of a and group g's logits.
   auto raise = [&](float a, int g) -> float {
@@ -304,9 +328,16 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleParams 
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   const float own_max = __fadd_rn(m, 0.f);  // -0 is +0: equal logits have equal bits in the join
   const unsigned bits = __float_as_uint(own_max);
-  const unsigned ordered = (bits & 0x80000000u) ? ~bits : bits | 0x80000000u;
-  // The lowest index of the maximum, -1 if that is -inf.
-  auto first_maximum = [&]() -> int {
+  // (The first join of every path passes it on, and with it that a copy failed.)
+  const unsigned ordered = !staged ? kFailed : ((bits & 0x80000000u) ? ~bits : bits | 0x80000000u);
+  // The row's answer where a wait ran out.
+  auto give_up = [&] {
+    if (rank == 0 && threadIdx.x == 0) p.out[r] = -1;
+    cluster.leave();
+  };
+  // The lowest index of the maximum, -1 if that is -inf; kFailed as score if a
+  // wait ran out.
+  auto first_maximum = [&]() -> Found {
     Found f{ordered, kNone, own_max, 0.f, 0};
 #pragma unroll 1
     for (int g = threadIdx.x; g < groups && own_max > -INFINITY && f.token == kNone; g += kThreads) {
@@ -317,15 +348,21 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleParams 
       for (int e = kGroup - 1; e >= 0; --e)
         if (x[e] == own_max) f.token = begin + g * kGroup - shift + e;
     }
-    f = cluster.join(f);
-    return f.x == -INFINITY ? -1 : (int)f.token;
+    f = join(f);
+    if (f.x == -INFINITY) f.token = kNone;
+    return f;
   };
   if (greedy) {
-    const int i = first_maximum();
-    if (rank == 0 && threadIdx.x == 0) p.out[r] = i;
+    const Found f = first_maximum();
+    if (f.score == kFailed) return give_up();
+    if (rank == 0 && threadIdx.x == 0) p.out[r] = (int)f.token;
     return;
   }
-  m = cluster.join({ordered, kNone, own_max, 0.f, 0}).x;
+  {
+    const Found f = join({ordered, kNone, own_max, 0.f, 0});
+    if (f.score == kFailed) return give_up();
+    m = f.x;
+  }
   if (m == -INFINITY) {
     if (rank == 0 && threadIdx.x == 0) p.out[r] = -1;
     return;
@@ -461,8 +498,10 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleParams 
       }
     }
   }
-  Found f = cluster.join(found(c, total, 0));
+  Found f = join(found(c, total, 0));
+  if (f.score == kFailed) return give_up();
   const float mass = top_p < 1.f ? top_p * f.sum : INFINITY;
+  int last = 0x7fffffff;  // tokens ahead of the pivot before: fewer every time
   while (f.score != 0 && (top_k > 0 || top_p < 1.f || weight(f.x) < min_p)) {
     const float xj = f.x;
     const int j = (int)f.token - begin;
@@ -490,25 +529,30 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleParams 
       sum += race(c, round, ahead);
       mask = ahead;
     }
-    const Found a = cluster.join(found(c, sum, count));
+    const Found a = join(found(c, sum, count));
+    if (a.score == kFailed) return give_up();
     const bool kept = (top_k <= 0 || a.count < top_k) && a.sum < mass && weight(xj) >= min_p;
-    if (kept || a.count == 0) break;
+    if (kept || a.count == 0 || a.count >= last) break;
+    last = a.count;
     f = a;
   }
   // Without a candidate (min_p above 1, say) the first token is kept all the same.
-  const int token = f.score != 0 ? (int)f.token : first_maximum();
-  if (rank == 0 && threadIdx.x == 0) p.out[r] = token;
+  if (f.score == 0) {
+    f = first_maximum();
+    if (f.score == kFailed) return give_up();
+  }
+  if (rank == 0 && threadIdx.x == 0) p.out[r] = (int)f.token;
 }
 
-template <typename T, bool STAGED>
+template <typename T, bool STAGED, bool MUTE = false>
 int launch_t(const SampleParams& p, size_t smem, cudaStream_t st) {
   static OncePerDevice once;
   if (smem > 48 * 1024 && !once([] {
-        return cudaFuncSetAttribute(sample_kernel<T, STAGED>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+        return cudaFuncSetAttribute(sample_kernel<T, STAGED, MUTE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                     kMaxStageBytes) == cudaSuccess;
       }))
     return -1;
-  return once.launched(launch_dependent(sample_kernel<T, STAGED>, dim3((unsigned)(p.R * p.cluster)), kThreads, smem, st,
+  return once.launched(launch_dependent(sample_kernel<T, STAGED, MUTE>, dim3((unsigned)(p.R * p.cluster)), kThreads, smem, st,
                                         p.cluster, p));
 }
 
@@ -518,18 +562,30 @@ int launch_type(const SampleParams& p, cudaStream_t st) {
   return smem <= kMaxStageBytes ? launch_t<T, true>(p, smem, st) : launch_t<T, false>(p, 0, st);
 }
 
-}  // namespace
-
-int launch_sample(SampleParams p, cudaStream_t st) {
+// CTAs per row and tokens per CTA. False if the grid would be too large.
+bool plan(SampleParams& p) {
   // CTAs per row: enough that a slice is at most 16384 tokens, and with few
   // rows enough to use the SMs while a slice keeps 2048 tokens.
   p.cluster = 1;
   while (p.cluster < kMaxCluster &&
          (p.V > 16384 * p.cluster || ((long long)p.R * p.cluster < 148 && p.V > 2048 * p.cluster)))
     p.cluster *= 2;
-  if ((long long)p.R * p.cluster > 0x7fffffffLL) return -2;
+  if ((long long)p.R * p.cluster > 0x7fffffffLL) return false;
   p.slice = ((p.V + p.cluster - 1) / p.cluster + kGroup - 1) / kGroup * kGroup;
+  return true;
+}
+
+}  // namespace
+
+int launch_sample(SampleParams p, cudaStream_t st) {
+  if (!plan(p)) return -2;
   return p.logits_bf16 ? launch_type<__nv_bfloat16>(p, st) : launch_type<float>(p, st);
+}
+
+int launch_sample_mute(SampleParams p, cudaStream_t st) {
+  if (p.logits_bf16 || !plan(p)) return -2;
+  const size_t smem = ((size_t)p.slice + 2 * kGroup) * sizeof(float);
+  return smem <= kMaxStageBytes ? launch_t<float, true, true>(p, smem, st) : -2;
 }
 
 }  // namespace b2a

@@ -23,9 +23,15 @@ struct SampleParams {
   int cluster;  // CTAs per row (a power of two), set by launch_sample
   int slice;    // tokens per CTA, a multiple of 8
   int* err;
+  long long wait_limit = kWaitLimitCycles;  // of every wait, in cycles
+  int mute_pass;                            // launch_sample_mute only
 };
 
 // Returns 0 or a negative value on launch failure.
 int launch_sample(SampleParams p, cudaStream_t st);
+
+// For the failure path's test: fp32 logits, and the last CTA of each row's
+// cluster stops sending its values at pass mute_pass.
+int launch_sample_mute(SampleParams p, cudaStream_t st);
 
 }  // namespace b2a

@@ -1,0 +1,32 @@
+"""What the serving operators do when a wait runs out or their device-side
+arguments are out of range: they end, report it and leave the context usable."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("mute_pass,temperature,top_p", [(0, 0.0, 1.0), (0, 1.0, 1.0), (1, 1.0, 1.0), (2, 1.0, 0.3)])
+@pytest.mark.parametrize("R,V", [(1, 49152), (5, 40_001), (200, 3000)])
+def test_sampling_ends_when_a_part_of_a_row_stops_answering(cuda_dev, R, V, mute_pass, temperature, top_p):
+    """The last block of every row stops sending at one of the joins: with waits of 1 ms (the kernels' are 2 s) the
+    row's blocks give up together, the rows give -1 and the error word says why."""
+    from npu_b200 import _lib, api
+
+    g = torch.Generator(device=cuda_dev).manual_seed(V)
+    x = 2 * torch.randn(R, V, generator=g, device=cuda_dev)
+    e = torch.empty(R, V, device=cuda_dev).exponential_(generator=g)
+    expected = api.sample(x, e, temperature=temperature, top_p=top_p)
+    assert api.device_error() == 0
+    out = torch.full((R,), -7, dtype=torch.long, device=cuda_dev)
+    rc = _lib.load().b2a_diag_sample_timeout(x.data_ptr(), e.data_ptr(), R, V, temperature, top_p, mute_pass,
+                                             2_000_000, out.data_ptr(),
+                                             torch.cuda.current_stream(cuda_dev).cuda_stream)
+    assert rc == 0
+    assert api.device_error() == _lib.B2A_ERR_DEVICE_TIMEOUT
+    if mute_pass < 2:
+        assert (out == -1).all()
+    else:  # rows whose first race decides never get to the third join
+        assert ((out == -1) | (out == expected)).all() and (out == -1).any()
+    assert torch.equal(api.sample(x, e, temperature=temperature, top_p=top_p), expected)
+    assert api.device_error() == 0
