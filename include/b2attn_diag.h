@@ -43,6 +43,16 @@ B2A_API int b2a_diag_sample_timeout(const float* logits, const float* noise, int
                                     float top_p, int mute_pass, long long limit_cycles, long long* out,
                                     void* stream);
 
+/*
+ * The query blocks of 128 rows that b2a_prefill_varlen makes of packed
+ * sequences: out [n][5] int32 = {first query row, query rows, first key, keys,
+ * block} of the blocks numbered ids[0 .. n - 1] (0 and up, device), asked for
+ * in that order by one warp; no rows where there is no such block. Bad offsets
+ * are reported as there.
+ */
+B2A_API int b2a_diag_packed_blocks(const int* cu_q, const int* cu_k, int B, int Nq, int Nk, int causal,
+                                   const int* ids, int n, int* out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

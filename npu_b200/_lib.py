@@ -143,6 +143,10 @@ SIGNATURES = {
     "b2a_diag_umma_gemm": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int,
                                           ctypes.c_void_p]),
     "b2a_diag_wait_timeout": (ctypes.c_int, [ctypes.c_longlong, ctypes.c_void_p]),
+    "b2a_diag_packed_blocks": (ctypes.c_int, [
+        ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_void_p,
+        ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p,
+    ]),
     "b2a_diag_sample_timeout": (ctypes.c_int, [
         ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_float, ctypes.c_float, ctypes.c_int,
         ctypes.c_longlong, ctypes.c_void_p, ctypes.c_void_p,

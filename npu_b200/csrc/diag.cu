@@ -9,6 +9,7 @@
 // threads using the 128-byte swizzle formula.
 #include "b2attn_diag.h"
 #include "common.cuh"
+#include "packed.cuh"
 #include "sample.cuh"
 
 namespace b2a {
@@ -116,7 +117,35 @@ __global__ void __launch_bounds__(32) diag_wait_timeout_kernel(long long limit, 
   (void)ok;
 }
 
+// One warp finds blocks ids[0], ids[1], ... of packed sequences, in that order.
+__global__ void __launch_bounds__(32)
+    diag_packed_blocks_kernel(const __grid_constant__ PrefillParams p, const int* ids, int n, PackedBlock* out) {
+  PackedBlocks<128> blocks(p);
+  for (int i = 0; i < n; ++i) {
+    const PackedBlock at = blocks.find(ids[i]);
+    if (threadIdx.x == 0) out[i] = at;
+  }
+}
+
 }  // namespace b2a
+
+extern "C" int b2a_diag_packed_blocks(const int* cu_q, const int* cu_k, int B, int Nq, int Nk, int causal,
+                                      const int* ids, int n, int* out, void* stream) {
+  static_assert(sizeof(b2a::PackedBlock) == 5 * sizeof(int), "five numbers a block");
+  if (!cu_q || !cu_k || !ids || !out || B <= 0 || Nq < 0 || Nk < 0 || n <= 0) return B2A_ERR_INVALID_ARG;
+  b2a::PrefillParams p{};
+  p.cu_q = cu_q;
+  p.cu_k = cu_k;
+  p.B = B;
+  p.Tq = Nq;
+  p.Tk = Nk;
+  p.causal = causal ? 1 : 0;
+  p.err = b2a::device_error_word();
+  if (!p.err) return B2A_ERR_CUDA;
+  b2a::diag_packed_blocks_kernel<<<1, 32, 0, static_cast<cudaStream_t>(stream)>>>(
+      p, ids, n, reinterpret_cast<b2a::PackedBlock*>(out));
+  return cudaGetLastError() == cudaSuccess ? B2A_OK : B2A_ERR_LAUNCH;
+}
 
 extern "C" int b2a_diag_wait_timeout(long long limit_cycles, void* stream) {
   if (limit_cycles <= 0 || limit_cycles > 4000000000LL) return -1;
