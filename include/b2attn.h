@@ -318,7 +318,8 @@ B2A_API int b2a_prefill_host(const void* q, const void* k, const void* v, void* 
  * (keys - queries) + r, and a row that sees none gives 0. No replacement in
  * the reference, whose prompts run one at a time (smollm.py:168-253).
  * A pair of offsets that is not a stretch of the tensors leaves its sequence
- * out and reports B2A_ERR_DEVICE_BAD_LEN. Supported D: 64, 128, 256.
+ * out (with more than 256 sequences maybe others too) and reports
+ * B2A_ERR_DEVICE_BAD_LEN. Supported D: 64, 128, 256.
  */
 B2A_API int b2a_prefill_varlen(const void* q, const void* k, const void* v, const void* gate, void* o, float* lse,
                                const int* cu_q, const int* cu_k, int B, int Nq, int Nk, int Hq, int Hkv, int D,

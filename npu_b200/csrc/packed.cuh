@@ -31,7 +31,8 @@ namespace b2a {
 // Above kPackedByPosition sequences, block i is slot i - s(b) of the last
 // sequence with s(b) <= i, s(b) = cu_q[b] / kRows + b: s(b + 1) - s(b) is at
 // least the sequence's number of blocks, and b is found by a search that
-// narrows 32-fold a step.
+// narrows 32-fold a step. Offsets that decrease may hide other sequences from
+// that search, and a bad pair from every block, so block b also checks pair b.
 template <int kRows>
 struct PackedBlocks {
   const PrefillParams& p;
@@ -84,6 +85,10 @@ struct PackedBlocks {
   __device__ __forceinline__ PackedBlock find(int i) {
     const int lane = threadIdx.x & 31;
     if (p.B > kPackedByPosition) {
+      if (i < p.B) {
+        int n, off;
+        shape(i, n, off);
+      }
       int lo = 0, len = p.B;
       while (len > 1) {
         const int step = (len + 31) / 32, b = lo + lane * step;

@@ -63,3 +63,33 @@ def test_blocks_by_position_in_any_order(cuda_dev, order):
     cu = offsets(lens, cuda_dev)
     got = ask(cu, cu, sum(lens), sum(lens), 1, ids.to(torch.int32).to(cuda_dev))
     assert sorted(b for b in got if b[1] > 0) == sorted(numbered(lens, lens, 1))
+
+
+@pytest.mark.parametrize("B", [40, BY_POSITION + 90])
+@pytest.mark.parametrize("which,value", [("q", -5), ("q", 10 ** 9), ("q", 200), ("k", -5), ("k", 10 ** 9), ("k", 200)])
+@pytest.mark.parametrize("at", [20, -1])
+@pytest.mark.parametrize("Hq,Hkv,D", [(2, 1, 64), (2, 1, 128), (1, 1, 256)])
+def test_a_bad_offset_is_reported_wherever_it_is(cuda_dev, B, which, value, at, Hq, Hkv, D):
+    """One offset below 0, past the tensors or below the one before it: the call reports it, and what it writes lies
+    in the output."""
+    from npu_b200 import _lib, device_error, prefill_varlen
+
+    n = 40 * B
+    cu = {x: torch.arange(0, n + 1, 40, dtype=torch.int32, device=cuda_dev) for x in "qk"}
+    cu[which][at] = value
+    g = torch.Generator(device=cuda_dev).manual_seed(B)
+    q = torch.randn(n, Hq, D, generator=g, device=cuda_dev).bfloat16()
+    kv = torch.randn(n, Hkv, D, generator=g, device=cuda_dev).bfloat16()
+    hold = torch.full((n + 256, Hq, D), 5.0, device=cuda_dev)
+    clean = prefill_varlen(q, kv, kv, torch.arange(0, n + 1, 40, dtype=torch.int32, device=cuda_dev))
+    assert device_error() == 0
+    prefill_varlen(q, kv, kv, cu["q"], cu["k"], out=hold[128:-128])
+    assert device_error() == _lib.B2A_ERR_DEVICE_BAD_LEN
+    assert (hold[:128] == 5).all() and (hold[-128:] == 5).all()
+    inner = hold[128:-128]
+    assert torch.isfinite(inner).all()
+    if B <= BY_POSITION and (which, value) != ("q", 200):  # (there the next pair's queries overlap others')
+        kept = torch.ones(n, dtype=torch.bool)  # only the pairs with that offset are left out
+        b = at % (B + 1)
+        kept[40 * (b - 1):40 * (b + 1)] = False
+        assert torch.equal(inner[kept.to(cuda_dev)], clean[kept.to(cuda_dev)])
