@@ -355,7 +355,8 @@ B2A_API int b2a_decode_paged(const void* q, const void* k_pages, const void* v_p
  * q_out [N, Hq, D] and k, v to the sequence's pages (all bf16, q_out
  * contiguous); k_out / v_out, optional, contiguous [N, Hkv, D] bf16, receive
  * the same k and v packed (what b2a_prefill_varlen reads). seqlens_out [B],
- * optional: start + tokens. cos_tab / sin_tab [max_pos, rope_dim] are fp32
+ * optional: start + tokens; must not overlap start_pos_per_batch (refused),
+ * which is read while it is written. cos_tab / sin_tab [max_pos, rope_dim] are fp32
  * (tab_fp32 = 1) or of the source type; computed in fp32, rounded once.
  * Tokens whose position or page is out of range are skipped and report
  * B2A_ERR_DEVICE_BAD_LEN. Supported D: 64, 128, 256.

@@ -537,7 +537,8 @@ def rope_append_paged(
     Token n of sequence b (cu_seqlens[b] <= n < cu_seqlens[b + 1]) is at
     position p_b + n - cu_seqlens[b], p_b = start_pos_per_batch[b] or
     start_pos; its k and v go to the page and slot of that position, which
-    block_table must already name. seqlens_out (int32 [B], optional) receives
+    block_table must already name. seqlens_out (int32 [B], optional, not the
+    tensor start_pos_per_batch, which is read while it is written) receives
     p_b + tokens. cos/sin [max_pos, rope_dim] are fp32 or q's dtype; the
     arithmetic is fp32 and rounds to bf16 once. q_norm, k_norm, norm_eps and
     rope_dim as in `rope_append`. Returns q rotated, [N, Hq, D] bf16; with

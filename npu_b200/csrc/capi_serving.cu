@@ -204,6 +204,10 @@ int b2a_rope_append_paged(const void* q, const void* k, const void* v, const lon
   if (B <= 0 || N <= 0 || Hq <= 0 || Hkv <= 0 || n_pages <= 0 || page <= 0 || table_width <= 0 ||
       table_ld < table_width || (!start_pos_per_batch && start_pos < 0))
     return B2A_ERR_INVALID_ARG;
+  // The positions are read while the lengths are written.
+  if (start_pos_per_batch && seqlens_out && start_pos_per_batch < seqlens_out + B &&
+      seqlens_out < start_pos_per_batch + B)
+    return B2A_ERR_INVALID_ARG;
   if (!head_dim_ok(D)) return B2A_ERR_HEAD_DIM;
   if (rope_dim != 0 && (rope_dim < 16 || rope_dim > D || (rope_dim & (rope_dim - 1)))) return B2A_ERR_INVALID_ARG;
   if (rope_dim && (!cos_tab || !sin_tab || max_pos <= 0)) return B2A_ERR_INVALID_ARG;

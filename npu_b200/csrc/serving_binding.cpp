@@ -215,6 +215,9 @@ py::object rope_append_paged(const Tensor& q, const Tensor& k, const Tensor& v, 
   need_table(table, B, device);
   if (start) need_int32("start_pos_per_batch", *start, B, device);
   if (seqlens_out) need_int32("seqlens_out", *seqlens_out, B, device);
+  if (start && seqlens_out && start->data_ptr<int>() < seqlens_out->data_ptr<int>() + B &&
+      seqlens_out->data_ptr<int>() < start->data_ptr<int>() + B)
+    refuse("seqlens_out must not overlap start_pos_per_batch: the positions are read while it is written");
   for (auto [name, w] : {std::pair<const char*, const OptTensor*>{"q_norm", &q_norm}, {"k_norm", &k_norm}})
     if (*w && ((*w)->scalar_type() != type || (*w)->device() != device || (*w)->dim() != 1 || (*w)->size(0) != D ||
                !(*w)->is_contiguous()))

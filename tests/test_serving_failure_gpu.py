@@ -30,3 +30,25 @@ def test_sampling_ends_when_a_part_of_a_row_stops_answering(cuda_dev, R, V, mute
         assert ((out == -1) | (out == expected)).all() and (out == -1).any()
     assert torch.equal(api.sample(x, e, temperature=temperature, top_p=top_p), expected)
     assert api.device_error() == 0
+
+
+def test_lengths_written_over_the_positions_are_refused(cuda_dev):
+    from npu_b200 import rope_append_paged
+
+    B = 3
+    q = torch.zeros(B, 4, 64, dtype=torch.bfloat16, device=cuda_dev)
+    pool = torch.zeros(4, 2, 16, 64, dtype=torch.bfloat16, device=cuda_dev)
+    tab = torch.zeros(16, 64, dtype=torch.bfloat16, device=cuda_dev)
+    pos = torch.zeros(2, B, dtype=torch.int32, device=cuda_dev)
+    table = torch.arange(B, dtype=torch.int32, device=cuda_dev)[:, None]
+    cu = torch.arange(B + 1, dtype=torch.int32, device=cuda_dev)
+
+    def call(start, end):
+        return rope_append_paged(q, q[:, :2], q[:, :2], tab, tab, pool, pool.clone(), table, cu,
+                                 start_pos_per_batch=start, seqlens_out=end)
+
+    for start, end in [(pos[0], pos[0]), (pos[0], pos.view(-1)[1:4]), (pos.view(-1)[2:5], pos[0])]:
+        with pytest.raises(ValueError, match="overlap"):
+            call(start, end)
+    call(pos[0], pos[1])
+    assert pos.tolist() == [[0] * B, [1] * B]
