@@ -117,7 +117,7 @@ size_t b2a_decode_paged_workspace_bytes(int B, int Hq, int Hkv, int D) {
   if (B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || Hq / Hkv > 16 || !head_dim_ok(D)) return 0;
   const size_t rows = b2a::decode_paged_parts(B, Hkv, b2a::decode_paged_max_ctas(D, b2a::api_sm_count())) * (Hq / Hkv);
   return b2a::api_align256(rows * D * sizeof(float)) + b2a::api_align256(rows * 2 * sizeof(float)) +
-         ((size_t)B + 1) * sizeof(long long);
+         (size_t)B * Hkv * 2 * sizeof(int);
 }
 
 int b2a_decode_paged(const void* q, const void* k_pages, const void* v_pages, const int* block_table,
@@ -186,8 +186,7 @@ int b2a_decode_paged(const void* q, const void* k_pages, const void* v_pages, co
   p.part_o = reinterpret_cast<float*>(scratch);
   scratch += b2a::api_align256(rows * D * sizeof(float));
   p.part_ml = reinterpret_cast<float*>(scratch);
-  if ((long long)B * Hq > (long long)b2a::kJoinWave * b2a::api_sm_count())
-    p.units = reinterpret_cast<long long*>(scratch + b2a::api_align256(rows * 2 * sizeof(float)));
+  p.place = reinterpret_cast<int*>(scratch + b2a::api_align256(rows * 2 * sizeof(float)));
   return status_of(b2a::launch_decode_paged(D, tk, tv, p, static_cast<cudaStream_t>(stream)));
 }
 

@@ -277,29 +277,13 @@ __global__ void __launch_bounds__(PagedCfg<D>::THREADS, PagedCfg<D>::CTAS_PER_SM
 
   grid_dep_wait();
   // The next kernel (the joining one when SPLIT) may take SM slots as they
-  // free up; after the wait, so that what it reads ahead of its own wait (the
-  // lengths) is final.
+  // free up.
   grid_dep_launch();
   if (p.err && blockIdx.x == 0)
     for (int b = threadIdx.x; b < p.B; b += C::THREADS)
       if (p.seqlens[b] < 0 || p.seqlens[b] > (long long)p.table_width * p.page) atomicOr(p.err, kErrBadArgs);
   long long from = 0, count = 1;
   if constexpr (SPLIT) {
-    if (p.units && blockIdx.x == gridDim.x - 1 && warp == 0) {
-      long long before = 0;
-      for (int b0 = 0; b0 < p.B; b0 += 32) {
-        const int n = b0 + lane < p.B ? units_of(tiles_of(p, b0 + lane)) : 0;
-        int upto = n;
-#pragma unroll
-        for (int off = 1; off < 32; off *= 2) {
-          const int y = __shfl_up_sync(0xffffffffu, upto, off);
-          if (lane >= off) upto += y;
-        }
-        if (b0 + lane < p.B) p.units[b0 + lane] = before + upto - n;
-        before += __shfl_sync(0xffffffffu, upto, 31);
-      }
-      if (lane == 0) p.units[p.B] = before;
-    }
     const long long total = total_units(p), share = share_of(total, p.n_ctas);
     from = blockIdx.x * share;
     count = min(share, total - from);
@@ -587,6 +571,11 @@ __global__ void __launch_bounds__(PagedCfg<D>::THREADS, PagedCfg<D>::CTAS_PER_SM
           store_output(p, w.b, h, d, over(osum, lsum), p.gate ? load_gate(p, w.b, h, d) : zero4());
         }
       }
+      if (SPLIT && threadIdx.x == 0) {
+        int* place = p.place + 2 * ((long long)w.b * p.Hkv + w.g);
+        if (w.begin == 0) place[0] = blockIdx.x;
+        if (w.t1 == w.tiles) place[1] = blockIdx.x;
+      }
       fence_proxy_async_smem();
       asm volatile("bar.sync 1, 128;" ::: "memory");  // everyone has read the stage, m and l
       if (lane == 0) mbar_arrive(&bars->empty[slot]);
@@ -598,94 +587,80 @@ __global__ void __launch_bounds__(PagedCfg<D>::THREADS, PagedCfg<D>::CTAS_PER_SM
 constexpr int kJoinThreads = 256;
 
 // Joins the partials of (sequence, query head) blockIdx.x. The parts are the
-// CTAs from the one with the pair's first tile to the one with its last.
-// D / 4 threads read one part's row; the parts are dealt to such teams in turn
-// and joined in a fixed order. The lengths are read before the wait for the
-// main kernel (which does not write them); so is everything else once, for
-// nothing, which brings the instructions and the gate on chip while the main
-// kernel's last CTAs still run. Where the joining CTAs come in many waves
-// (p.units) they do neither.
+// CTAs from the one with the pair's first tile to the one with its last, which
+// the main kernel has noted (p.place): working it out again here from all
+// lengths took 2 us. D / 4 threads read one part's row; the parts are dealt to
+// such teams in turn and joined in a fixed order. Nothing is read before the
+// wait for the main kernel: what it and the kernels before it have written (the
+// lengths, by the append) is only sure to be seen after that. A dry run before
+// the wait, to fetch the instructions, gained nothing (4 to 4096 sequences of
+// 500 to 1500 keys, 32 / 4 heads of 128: 9.5 us to 1.77 ms without, 9.5 us to
+// 1.80 ms with it).
 template <int D>
 __global__ void __launch_bounds__(kJoinThreads) decode_paged_join_kernel(const __grid_constant__ DecodePagedParams p) {
   constexpr int TEAM = D / 4, TEAMS = kJoinThreads / TEAM;
   __shared__ float4 s_o[TEAMS][TEAM];
   __shared__ float s_m[TEAMS], s_l[TEAMS];
-  const int lane = threadIdx.x & 31;
   const int b = blockIdx.x / p.Hq, h = blockIdx.x % p.Hq;
   const int g = h / p.group, r = h % p.group;
-  long long total = 0, before = 0;  // units of all sequences, and of those before b
-  if (p.units) {
-    grid_dep_wait();
-    total = __ldcg(p.units + p.B);
-    before = __ldcg(p.units + b);
-  } else {
-    for (int b0 = 0; b0 < p.B; b0 += 32) {
-      const int n = b0 + lane < p.B ? units_of(tiles_of(p, b0 + lane)) : 0;
-      total += __reduce_add_sync(0xffffffffu, n);
-      before += __reduce_add_sync(0xffffffffu, b0 + lane < b ? n : 0);
+  const int team = threadIdx.x / TEAM, d = 4 * (threadIdx.x % TEAM);
+  const long long pair = (long long)b * p.Hkv + g;
+  grid_dep_wait();
+  grid_dep_launch();
+  const int2 at = __ldcg(reinterpret_cast<const int2*>(p.place) + pair);
+  const float4 gate = p.gate && team == 0 ? load_gate(p, b, h, d) : zero4();
+  int c0 = 0, parts = 0;
+  if (keys_of(p, b) > 0) {
+    // (Within the CTAs there are, even if the lengths changed under the call.)
+    c0 = max(0, min(at.x, p.n_ctas - 1));
+    parts = min(at.y, p.n_ctas - 1) - c0 + 1;
+  }
+  const long long row0 = (pair + c0) * p.group + r;  // part i's row: row0 + i group
+  float m = -INFINITY, l = 0.f;
+  float4 o = zero4();
+  for (int i0 = team; i0 < parts; i0 += 4 * TEAMS) {
+    float2 ml[4];
+    float4 po[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int i = i0 + k * TEAMS;
+      const long long row = row0 + (long long)i * p.group;
+      ml[k] = i < parts ? __ldcg(reinterpret_cast<const float2*>(p.part_ml + 2 * row)) : make_float2(-INFINITY, 0.f);
+      po[k] = i < parts ? __ldcg(reinterpret_cast<const float4*>(p.part_o + row * D + d)) : zero4();
+    }
+    const float mn = fmaxf(fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)), m);
+    const float mu = mn == -INFINITY ? 0.f : mn;
+    const float f0 = ex2(m - mu);
+    m = mn;
+    l *= f0;
+    o = make_float4(o.x * f0, o.y * f0, o.z * f0, o.w * f0);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float f = ex2(ml[k].x - mu);
+      l = fmaf(f, ml[k].y, l);
+      o = axpy(f, po[k], o);
     }
   }
-  const int tiles = tiles_of(p, b);
-  const long long share = share_of(total * p.Hkv, p.n_ctas);
-  const long long lo = before * p.Hkv + (long long)g * units_of(tiles);
-  const int team = threadIdx.x / TEAM, d = 4 * (threadIdx.x % TEAM);
-  const long long c0 = tiles > 0 ? lo / share : 0;
-  const int parts = tiles > 0 ? (int)((lo + tiles - 1) / share - c0) + 1 : 0;
-  const long long row0 = ((long long)b * p.Hkv + g + c0) * p.group + r;  // part i's row: row0 + i group
-#pragma unroll 1
-  for (int pass = p.units ? 1 : 0; pass < 2; ++pass) {
-    if (pass == 1) {
-      grid_dep_wait();
-      grid_dep_launch();
-    }
-    float m = -INFINITY, l = 0.f;
-    float4 o = zero4();
-    for (int i0 = team; i0 < parts; i0 += 4 * TEAMS) {
-      float2 ml[4];
-      float4 po[4];
+  s_o[team][threadIdx.x % TEAM] = o;
+  if (d == 0) {
+    s_m[team] = m;
+    s_l[team] = l;
+  }
+  __syncthreads();
+  if (team == 0) {
+    float M = -INFINITY;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int i = i0 + k * TEAMS;
-        const long long row = row0 + (long long)i * p.group;
-        ml[k] = i < parts ? __ldcg(reinterpret_cast<const float2*>(p.part_ml + 2 * row)) : make_float2(-INFINITY, 0.f);
-        po[k] = i < parts ? __ldcg(reinterpret_cast<const float4*>(p.part_o + row * D + d)) : zero4();
-      }
-      const float mn = fmaxf(fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)), m);
-      const float mu = mn == -INFINITY ? 0.f : mn;
-      const float f0 = ex2(m - mu);
-      m = mn;
-      l *= f0;
-      o = make_float4(o.x * f0, o.y * f0, o.z * f0, o.w * f0);
+    for (int u = 0; u < TEAMS; ++u) M = fmaxf(M, s_m[u]);
+    const float Mu = M == -INFINITY ? 0.f : M;
+    float lsum = 0.f;
+    float4 osum = zero4();
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float f = ex2(ml[k].x - mu);
-        l = fmaf(f, ml[k].y, l);
-        o = axpy(f, po[k], o);
-      }
+    for (int u = 0; u < TEAMS; ++u) {
+      const float f = ex2(s_m[u] - Mu);
+      lsum = fmaf(f, s_l[u], lsum);
+      osum = axpy(f, s_o[u][threadIdx.x], osum);
     }
-    s_o[team][threadIdx.x % TEAM] = o;
-    if (d == 0) {
-      s_m[team] = m;
-      s_l[team] = l;
-    }
-    __syncthreads();
-    if (team == 0) {
-      float M = -INFINITY;
-#pragma unroll
-      for (int u = 0; u < TEAMS; ++u) M = fmaxf(M, s_m[u]);
-      const float Mu = M == -INFINITY ? 0.f : M;
-      float lsum = 0.f;
-      float4 osum = zero4();
-#pragma unroll
-      for (int u = 0; u < TEAMS; ++u) {
-        const float f = ex2(s_m[u] - Mu);
-        lsum = fmaf(f, s_l[u], lsum);
-        osum = axpy(f, s_o[u][threadIdx.x], osum);
-      }
-      const float4 gate = p.gate ? load_gate(p, b, h, d) : zero4();
-      if (pass == 1) store_output(p, b, h, d, over(osum, lsum), gate);
-    }
-    __syncthreads();
+    store_output(p, b, h, d, over(osum, lsum), gate);
   }
 }
 

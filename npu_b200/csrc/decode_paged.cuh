@@ -28,7 +28,7 @@ struct DecodePagedParams {
   // before its division, and (m, l) [group, 2].
   float* part_o;
   float* part_ml;
-  long long* units;  // [B + 1]: units of the sequences before each, or nullptr: see kJoinWave
+  int* place;        // [B Hkv, 2]: the CTAs with a pair's first and last tile
   int n_ctas;
   int* err;
 };
@@ -37,13 +37,6 @@ struct DecodePagedParams {
 // CTAs it may use for the current device, and its workspace.
 bool decode_paged_splits(int table_width, int page);
 int decode_paged_max_ctas(int D, int sms);
-// Joining CTAs (one per sequence and query head) per SM that run at once. With
-// more than that, each takes its place in the work from the main launch
-// (`units`) instead of summing all lengths, and does not warm up. Sequences of
-// 500 to 1500 keys, 32 heads, this way against the other: 16 sequences 15.6 us
-// against 14.8, 128 48 against 52, 1024 304 against 586, 4096 1.17 ms against
-// 5.8.
-constexpr int kJoinWave = 8;
 inline size_t decode_paged_parts(int B, int Hkv, int n_ctas) { return (size_t)B * Hkv + n_ctas; }
 
 // tk / tv: 5-D maps (64 columns, slot in the page, D / 64, head, page) with
