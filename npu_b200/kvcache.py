@@ -117,7 +117,8 @@ class PagedSequences:
     def __init__(self, cache: PagedKVCache, pages: list):
         self.cache, self._pages = cache, pages
         self.batch = len(pages)
-        table = torch.zeros((self.batch, max(len(p) for p in pages)), dtype=torch.int32)
+        # -1 is no page: a token past a sequence's own pages is left out and reported.
+        table = torch.full((self.batch, max(len(p) for p in pages)), -1, dtype=torch.int32)
         for b, p in enumerate(pages):
             table[b, :len(p)] = torch.tensor(p, dtype=torch.int32)
         self.block_table = table.to(cache.device)
@@ -132,6 +133,11 @@ class PagedSequences:
     @property
     def end(self) -> torch.Tensor:
         return self._pos[1]
+
+    @property
+    def released(self) -> bool:
+        """Whether the pages are given back; block_table then names pages of others."""
+        return not self._pages
 
     def advance(self) -> None:
         self._pos[0].copy_(self._pos[1])

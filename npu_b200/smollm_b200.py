@@ -277,6 +277,8 @@ class SmolLMB200:
     def _forward_packed(self, ids: torch.Tensor, seqs: PagedSequences,
                         cu_seqlens: Optional[torch.Tensor]) -> torch.Tensor:
         """The final norm's output for packed tokens ids [N]; advances seqs."""
+        if seqs.released:
+            raise ValueError("the sequences are released: their pages may have other owners")
         c = self.cfg
         x = self.embed[ids]
         for i, lw in enumerate(self.layers):
@@ -306,7 +308,9 @@ class SmolLMB200:
 
     @torch.no_grad()
     def decode_packed(self, ids: torch.Tensor, seqs: PagedSequences) -> torch.Tensor:
-        """Logits [B, vocab] after one more token ids [B] of every sequence."""
+        """Logits [B, vocab] after one more token ids [B] of every sequence. A
+        sequence whose pages are full keeps its keys and its logits mean
+        nothing; api.device_error() reports it."""
         if ids.dim() != 1 or ids.numel() != seqs.batch:
             raise ValueError("ids must be [B] with B = seqs.batch")
         return F.linear(self._forward_packed(ids.to(self.device), seqs, None), self.embed)
