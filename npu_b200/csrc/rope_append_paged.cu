@@ -228,7 +228,7 @@ __global__ void __launch_bounds__(32 * kWarps)
       raw[s][0].get(x);
       raw[s][1].get(y);
       turn(x, y, is_v);
-      if (!in_pool || !(in_table || is_v) || j >= rows) continue;
+      if (!in_pool || !in_table || j >= rows) continue;
       __nv_bfloat16* dst = is_v ? v_dst + h * p.vps[1] : k_dst + h * p.kps[1];
       store4(dst + o0, x), store4(dst + o1, y);
       __nv_bfloat16* packed = is_v ? p.v_out : p.k_out;

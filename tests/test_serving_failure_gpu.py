@@ -52,3 +52,29 @@ def test_lengths_written_over_the_positions_are_refused(cuda_dev):
             call(start, end)
     call(pos[0], pos[1])
     assert pos.tolist() == [[0] * B, [1] * B]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("tokens", [1, 40])
+def test_tokens_past_the_rotary_tables_are_skipped_whole(cuda_dev, dtype, tokens):
+    """Positions that the block table has pages for but the rotary tables no row: q, k and v stay unwritten."""
+    from npu_b200 import _lib, device_error, rope_append_paged
+
+    g = torch.Generator(device=cuda_dev).manual_seed(1)
+    q = torch.randn(tokens, 4, 64, generator=g, device=cuda_dev).to(dtype)
+    kv = torch.randn(2, tokens, 2, 64, generator=g, device=cuda_dev).to(dtype)
+    kp, vp = (torch.full((8, 2, 16, 64), 3.0, dtype=torch.bfloat16, device=cuda_dev) for _ in range(2))
+    table = torch.arange(8, dtype=torch.int32, device=cuda_dev)[None]
+    tab = torch.randn(2, 20, 64, generator=g, device=cuda_dev).to(dtype)
+    q_out = torch.full((tokens, 4, 64), 3.0, dtype=torch.bfloat16, device=cuda_dev)
+    first = 20 - tokens // 2  # the second half of the tokens is past the tables' 20 rows
+    cu = torch.tensor([0, tokens], dtype=torch.int32, device=cuda_dev)
+    assert device_error() == 0
+    rope_append_paged(q, kv[0], kv[1], tab[0], tab[1], kp, vp, table, cu, start_pos=first, q_out=q_out)
+    assert device_error() == _lib.B2A_ERR_DEVICE_BAD_LEN
+    n = tokens // 2
+    for pool in (kp, vp):
+        rows = pool.transpose(1, 2).reshape(128, 2, 64)
+        assert (rows[20:] == 3).all() and (rows[:first] == 3).all()
+        assert (rows[first:20] != 3).any(-1).all()
+    assert (q_out[n:] == 3).all() and (q_out[:n] != 3).any(-1).all()
