@@ -35,32 +35,33 @@ inline bool api_strides_ok(const long long* s, int n, long long mult) {
 
 inline size_t api_align256(size_t x) { return (x + 255) & ~(size_t)255; }
 
-// Runs `prepare` (which sets a kernel's attributes) once per device and
-// kernel: the runtime's attribute calls cost about a microsecond each, and
-// attributes stay with the kernel. A launch that failed forgets it, so that
-// the next call prepares again (a reset device has lost its attributes).
+// Launches a kernel whose attributes `prepare` sets: once per device, since the
+// runtime's attribute calls cost about a microsecond each and attributes stay
+// with the kernel. A device that was reset, or another context of it, has lost
+// them, and the launch fails: it is then prepared and launched once more.
+// `launch` returns the launch's status and leaves no error behind. Returns 0,
+// or -1 on failure.
 struct OncePerDevice {
   std::atomic<unsigned long long> done{0};
-  template <typename F>
-  bool operator()(F&& prepare) {
+  template <typename Prepare, typename Launch>
+  int run(Prepare&& prepare, Launch&& launch) {
     int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return prepare();
-    const unsigned long long bit = 1ull << dev;
-    if (done.load(std::memory_order_acquire) & bit) return true;
-    if (!prepare()) return false;
-    done.fetch_or(bit, std::memory_order_release);
-    return true;
-  }
-  int launched(cudaError_t e) {
-    if (e == cudaSuccess) return 0;
-    done.store(0, std::memory_order_release);
+    const bool known = cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 64;
+    const unsigned long long bit = known ? 1ull << dev : 0;
+    if ((done.load(std::memory_order_acquire) & bit) && launch() == cudaSuccess) return 0;
+    if (prepare() && launch() == cudaSuccess) {
+      done.fetch_or(bit, std::memory_order_release);
+      return 0;
+    }
+    done.fetch_and(~bit, std::memory_order_release);
     return -1;
   }
 };
 
 // Launch as a programmatic dependent: the grid may be scheduled while the
 // kernel before it in the stream drains. Its threads wait (grid_dep_wait)
-// before they touch memory.
+// before they touch memory. Takes a failed launch's error out of the runtime
+// (the next cudaGetLastError would report it as somebody else's).
 template <typename... Params, typename... Args>
 inline cudaError_t launch_dependent(void (*kernel)(Params...), dim3 grid, unsigned threads, size_t smem,
                                     cudaStream_t st, int cluster, const Args&... args) {
@@ -77,8 +78,8 @@ inline cudaError_t launch_dependent(void (*kernel)(Params...), dim3 grid, unsign
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = cluster > 0 ? 2 : 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
-  return e == cudaSuccess ? cudaGetLastError() : e;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...), last = cudaGetLastError();
+  return e == cudaSuccess ? last : e;
 }
 
 constexpr float kApiLog2e = 1.4426950408889634f;

@@ -671,13 +671,16 @@ int launch_main(const CUtensorMap& tk, const CUtensorMap& tv, const DecodePagedP
                 cudaStream_t st) {
   using C = PagedCfg<D>;
   static OncePerDevice once;
-  if (n > 0x7fffffffLL || !once([] {
+  if (n > 0x7fffffffLL) return -1;
+  return once.run(
+      [] {
         return cudaFuncSetAttribute(decode_paged_kernel<D, NT, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                     C::SMEM_BYTES) == cudaSuccess;
-      }))
-    return -1;
-  return once.launched(launch_dependent(decode_paged_kernel<D, NT, SPLIT>, dim3((unsigned)n), C::THREADS,
-                                        C::SMEM_BYTES, st, 0, tk, tv, p));
+      },
+      [&] {
+        return launch_dependent(decode_paged_kernel<D, NT, SPLIT>, dim3((unsigned)n), C::THREADS, C::SMEM_BYTES, st, 0,
+                                tk, tv, p);
+      });
 }
 
 template <int D>

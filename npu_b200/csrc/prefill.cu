@@ -757,18 +757,18 @@ static int launch_prefill_t(const CUtensorMap& tq, const CUtensorMap& tk, const 
            cudaFuncGetAttributes(&fa, kernel) == cudaSuccess && fa.numRegs >= C::MIN_LAUNCH_REGS;
   };
   static OncePerDevice once;
-  if (!once(prepare)) return -1;
   // One CTA per work item (query blocks x query heads, or x head pairs).
   const long long nblk = (long long)p.n_qblk * (PACKED ? 1 : p.B) * (p.head_pairs ? p.Hq / 2 : p.Hq);
   if (nblk <= 0 || nblk > 0x7fffffffLL) return -2;
   // Short packed prompts: the launch overlaps the kernel before (at head dim 64
   // 6.8 us a call against 8.2 at 3 prompts of 1 to 40 tokens). The larger items
   // gain nothing.
-  if (PACKED && NQT == 1)
-    return once.launched(
-        launch_dependent(kernel, dim3((unsigned)nblk), C::THREADS, C::SMEM_BYTES, st, 0, tq, tk, tv, p));
-  kernel<<<(unsigned)nblk, C::THREADS, C::SMEM_BYTES, st>>>(tq, tk, tv, p);
-  return once.launched(cudaGetLastError());
+  return once.run(prepare, [&] {
+    if (PACKED && NQT == 1)
+      return launch_dependent(kernel, dim3((unsigned)nblk), C::THREADS, C::SMEM_BYTES, st, 0, tq, tk, tv, p);
+    kernel<<<(unsigned)nblk, C::THREADS, C::SMEM_BYTES, st>>>(tq, tk, tv, p);
+    return cudaGetLastError();
+  });
 }
 
 // One-tile CTAs (two per SM) pay off when a CTA sees few key blocks, so that

@@ -447,15 +447,17 @@ int launch_d256(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap&
                 cudaStream_t st) {
   using C = D256Cfg;
   static OncePerDevice once;
-  if (!once([] {
-        return cudaFuncSetAttribute(fa_prefill_d256_kernel<PACKED>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                    C::SMEM_BYTES) == cudaSuccess;
-      }))
-    return -1;
   const long long nblk = (long long)p.n_qblk * p.Hq * (PACKED ? 1 : p.B);
   if (nblk <= 0 || nblk > 0x7fffffffLL) return -2;
-  fa_prefill_d256_kernel<PACKED><<<(unsigned)nblk, C::THREADS, C::SMEM_BYTES, st>>>(tq, tk, tv, p);
-  return once.launched(cudaGetLastError());
+  return once.run(
+      [] {
+        return cudaFuncSetAttribute(fa_prefill_d256_kernel<PACKED>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    C::SMEM_BYTES) == cudaSuccess;
+      },
+      [&] {
+        fa_prefill_d256_kernel<PACKED><<<(unsigned)nblk, C::THREADS, C::SMEM_BYTES, st>>>(tq, tk, tv, p);
+        return cudaGetLastError();
+      });
 }
 
 }  // namespace

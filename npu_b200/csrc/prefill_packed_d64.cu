@@ -505,17 +505,19 @@ __global__ void __launch_bounds__(Cfg::THREADS, 2)
 int launch_prefill_packed_d64(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
                               const PrefillParams& p, cudaStream_t st) {
   static OncePerDevice once;
-  if (!once([] {
+  const long long items = (long long)p.n_qblk * p.Hq;
+  if (items <= 0 || items > 0x7fffffffLL) return -2;
+  return once.run(
+      [] {
         cudaFuncAttributes fa{};
         return cudaFuncSetAttribute(prefill_packed_d64_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                     Cfg::SMEM_BYTES) == cudaSuccess &&
                cudaFuncGetAttributes(&fa, prefill_packed_d64_kernel) == cudaSuccess && fa.numRegs >= Cfg::REGS;
-      }))
-    return -1;
-  const long long items = (long long)p.n_qblk * p.Hq;
-  if (items <= 0 || items > 0x7fffffffLL) return -2;
-  return once.launched(launch_dependent(prefill_packed_d64_kernel, dim3((unsigned)items), Cfg::THREADS,
-                                        Cfg::SMEM_BYTES, st, 0, tq, tk, tv, p));
+      },
+      [&] {
+        return launch_dependent(prefill_packed_d64_kernel, dim3((unsigned)items), Cfg::THREADS, Cfg::SMEM_BYTES, st, 0,
+                                tq, tk, tv, p);
+      });
 }
 
 }  // namespace b2a

@@ -547,13 +547,15 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleParams 
 template <typename T, bool STAGED, bool MUTE = false>
 int launch_t(const SampleParams& p, size_t smem, cudaStream_t st) {
   static OncePerDevice once;
-  if (smem > 48 * 1024 && !once([] {
+  return once.run(
+      [] {
         return cudaFuncSetAttribute(sample_kernel<T, STAGED, MUTE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                     kMaxStageBytes) == cudaSuccess;
-      }))
-    return -1;
-  return once.launched(launch_dependent(sample_kernel<T, STAGED, MUTE>, dim3((unsigned)(p.R * p.cluster)), kThreads, smem, st,
-                                        p.cluster, p));
+      },
+      [&] {
+        return launch_dependent(sample_kernel<T, STAGED, MUTE>, dim3((unsigned)(p.R * p.cluster)), kThreads, smem, st,
+                                p.cluster, p);
+      });
 }
 
 template <typename T>
