@@ -30,8 +30,12 @@ SOURCES = ["capi.cu", "capi_serving.cu", "prefill.cu", "prefill_pair.cu", "prefi
            "prefill_packed_d64.cu", "decode.cu", "decode_noalloc.cu", "rope_append.cu", "rope_append_paged.cu",
            "decode_paged.cu", "sample.cu", "diag.cu", "host_pipeline.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
+FAST_MATH = ["--use_fast_math"]
+# The same without its replacement of expf and the like by approximations.
+FLUSH_ONLY = ["--ftz=true", "--prec-div=false", "--prec-sqrt=false"]
+MATH_FLAGS = {"sample.cu": FLUSH_ONLY}
 NVCC_FLAGS = [
-    "-O3", "-std=c++17", "-lineinfo", "--use_fast_math",
+    "-O3", "-std=c++17", "-lineinfo",
     "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
     "-I", str(INCLUDE), "-I", str(CSRC),
 ]
@@ -91,7 +95,7 @@ def _build_library(verbose: bool) -> None:
     objs = []
     for src in SOURCES:
         obj = BUILD_DIR / (Path(src).stem + ".o")
-        cmd = [nvcc, *ARCH, *NVCC_FLAGS, "-c", str(CSRC / src), "-o", str(obj)]
+        cmd = [nvcc, *ARCH, *NVCC_FLAGS, *MATH_FLAGS.get(src, FAST_MATH), "-c", str(CSRC / src), "-o", str(obj)]
         if verbose:
             cmd += ["-Xptxas", "-v"]
         r = subprocess.run(cmd, capture_output=True, text=True)

@@ -45,28 +45,15 @@ constexpr int kGroup = 8;                      // logits a thread handles at a t
 constexpr int kMaskGroups = 64 / kGroup;
 constexpr int kMaxStageBytes = 200 * 1024;     // slices above this stay in global memory
 
-// w(x) = exp(z), z = (x - m) / T rounded as the division rounds: the
-// quotient's estimate q = d rT is corrected by its remainder. 2^t for
-// t = z log2(e) is then corrected for t's rounding and for log2(e)'s (which
-// alone would cost |z| 2^-24): about 2^-22 in all. The passes over all tokens
-// use quick(): |z| 2^-22 off, a third of the instructions, enough for sums
-// and for each thread to pick its candidate; candidates are then compared by
-// the exact form. NaN and -inf weigh 0.
+// w(x) = exp(z), z = (x - m) / T rounded to fp32. The passes over all tokens
+// use quick(), 2^(d log2(e) / T) in one multiplication: |z| 2^-22 off, enough
+// for sums and for each thread to pick its candidate; candidates are then
+// compared by CUDA's division and exponential (this file is compiled with the
+// exact expf). NaN and -inf weigh 0.
 struct Weight {
-  float m, T, rT;
-  __device__ __forceinline__ float quick(float x) const {
-    return ex2(fmaxf((x - m) * (rT * 1.442695040888963f), -150.f));
-  }
-  __device__ __forceinline__ float operator()(float x) const {
-    constexpr float kHi = 1.442695040888963f, kLo = 1.925963033e-8f;  // log2(e) in two fp32 terms
-    const float d = __fsub_rn(x, m);
-    const float q = __fmul_rn(d, rT);
-    const float z = fmaxf(fmaf(fmaf(-q, T, d), rT, q), -104.f);  // exp(-104) is below every fp32 number
-    const float t = __fmul_rn(z, kHi);
-    const float r = fmaf(z, kLo, fmaf(z, kHi, -t));
-    const float w = ex2(t);
-    return fmaf(w, r * 0.6931471805599453f, w);
-  }
+  float m, T, to_log2;  // to_log2: log2(e) / T
+  __device__ __forceinline__ float quick(float x) const { return ex2(fmaxf((x - m) * to_log2, -150.f)); }
+  __device__ __forceinline__ float operator()(float x) const { return expf(__fdiv_rn(__fsub_rn(x, m), T)); }
 };
 
 // What a pass finds, joined over threads, warps and CTAs: the entry with the
@@ -253,10 +240,7 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleParams 
   const int n = min(p.slice, p.V - begin);  // this CTA's tokens [begin, begin + n)
   const T* logits = static_cast<const T*>(p.logits) + r * p.ld_logits + begin;
   const float* noise = p.noise + r * p.ld_noise + begin;
-  // The highest number does what +inf would, all finite logits weigh 1, and
-  // times 0 is 0.
-  const float given = p.temperature ? p.temperature[r] : p.temperature_all;
-  const float temperature = given == INFINITY ? 3.402823466e38f : given;
+  const float temperature = p.temperature ? p.temperature[r] : p.temperature_all;  // +inf: finite logits weigh 1
   const int top_k = p.top_k ? p.top_k[r] : p.top_k_all;
   const float top_p = p.top_p ? p.top_p[r] : p.top_p_all;
   const float min_p = p.min_p ? p.min_p[r] : p.min_p_all;
@@ -377,7 +361,7 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleParams 
       for (int e = 0; e < kGroup; ++e) x[e] = x[e] == INFINITY ? 0.f : -INFINITY;
     }
   };
-  const Weight weight{m, temperature, __frcp_rn(temperature)};
+  const Weight weight{m, temperature, 1.442695040888963f * __frcp_rn(temperature)};
   // A thread's candidate as the entry it joins with.
   auto found = [&](const Candidate& c, float sum, int count) -> Found {
     if (c.i < 0) return {0, kNone, 0.f, sum, count};
@@ -390,7 +374,7 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleParams 
   // of this CTA alone have a logit of at least `cut`. The second bound is
   // bisected on the threads' maxima, down to an eighth of T.
   float cut = -INFINITY;
-  if (min_p > 0.f && !infinite) cut = m + given * (__logf(min_p) - 1e-4f) - 1e-6f * fabsf(m);
+  if (min_p > 0.f && !infinite) cut = m + temperature * (__logf(min_p) - 1e-4f) - 1e-6f * fabsf(m);
   if (top_k > 0 && top_k <= kThreads && !infinite) {
     float hi = m, lo = m - 32.f * temperature;
     if (__syncthreads_count(own_max >= lo) >= top_k) {
