@@ -433,16 +433,38 @@ __device__ __forceinline__ void store_values(const PrefillParams& p, int b, int 
 
 // Scale one 32-column chunk of an output row by inv_l and, with a gate, by
 // sigmoid(gate), and store it. Only called for rows that exist (the gate is
-// read).
+// read, 16 bytes at a time: a whole GateChunk beside the values spilled in the
+// kernels with 128 registers a thread).
 __device__ __forceinline__ void store_out_chunk(const PrefillParams& p, int b, int h, int grow, int c,
                                                 const uint32_t (&o)[32], float inv_l) {
   float v[32];
 #pragma unroll
   for (int i = 0; i < 32; ++i) v[i] = u2f(o[i]) * inv_l;
   if (p.gate) {
-    GateChunk g;
-    load_gate_chunk(p, b, h, grow, c, g);
-    apply_gate_chunk(p, g, v);
+    const long long gi = (long long)b * p.g_sb + (long long)h * p.g_sh + (long long)grow * p.g_st + 32 * c;
+    if (p.gate_bf16) {
+      const uint4* g4 = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.gate) + gi);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint4 w = g4[i];
+        const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          v[8 * i + 2 * k] *= sigmoidf_(u2f(ws[k] << 16));
+          v[8 * i + 2 * k + 1] *= sigmoidf_(u2f(ws[k] & 0xffff0000u));
+        }
+      }
+    } else {
+      const float4* g4 = reinterpret_cast<const float4*>(static_cast<const float*>(p.gate) + gi);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float4 w = g4[i];
+        v[4 * i] *= sigmoidf_(w.x);
+        v[4 * i + 1] *= sigmoidf_(w.y);
+        v[4 * i + 2] *= sigmoidf_(w.z);
+        v[4 * i + 3] *= sigmoidf_(w.w);
+      }
+    }
   }
   store_values(p, b, h, grow, c, v);
 }
