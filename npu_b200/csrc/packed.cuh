@@ -37,8 +37,7 @@ template <int kRows>
 struct PackedBlocks {
   const PrefillParams& p;
   int own_n = 0, own_off = 0;  // this lane's sequence when B <= 32
-  int top = 0;                 // no block from `from` on has a level above this
-  int most = 0, from = 0;      // nor any block above `most`
+  int top = 0;                 // no block has a level above this
 
   __device__ __forceinline__ void shape(int b, int& n, int& off) const {
     n = off = 0;
@@ -55,12 +54,13 @@ struct PackedBlocks {
   __device__ __forceinline__ explicit PackedBlocks(const PrefillParams& params) : p(params) {
     const int lane = threadIdx.x & 31;
     if (p.B > kPackedByPosition) return;
+    int most = 0;
 #pragma unroll 4
     for (int b0 = 0; b0 < p.B; b0 += 32) {
       shape(b0 + lane, own_n, own_off);
       most = max(most, own_n > 0 ? own_n + own_off : 0);
     }
-    top = most = __reduce_max_sync(0xffffffffu, most);
+    top = __reduce_max_sync(0xffffffffu, most);
   }
   __device__ __forceinline__ int count_from(int w) const {
     const int lane = threadIdx.x & 31;
@@ -80,9 +80,8 @@ struct PackedBlocks {
     if (qblk < 0 || qblk >= n) return {0, 0, 0, 0, 0};
     return {p.cu_q[b], p.cu_q[b + 1] - p.cu_q[b], p.cu_k[b], p.cu_k[b + 1] - p.cu_k[b], qblk};
   }
-  // Block i (every lane gets it). Calls with growing i, the usual order, stay
-  // below the last level found; a smaller i starts from the highest again.
-  __device__ __forceinline__ PackedBlock find(int i) {
+  // Block i (every lane gets it).
+  __device__ __forceinline__ PackedBlock find(int i) const {
     const int lane = threadIdx.x & 31;
     if (p.B > kPackedByPosition) {
       if (i < p.B) {
@@ -99,8 +98,6 @@ struct PackedBlocks {
       }
       return block(lo, i - (p.cu_q[lo] / kRows + lo));
     }
-    if (i < from) top = most;
-    from = i;
     int lo = 0, hi = top;  // S(hi + 1) <= i always; looking for the largest w with S(w) > i
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
@@ -109,7 +106,6 @@ struct PackedBlocks {
       else
         hi = mid - 1;
     }
-    top = lo;
     int skip = i - count_from(lo + 1);
     for (int b0 = 0; b0 < p.B; b0 += 32) {
       int n = own_n, off = own_off;
