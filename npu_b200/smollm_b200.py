@@ -326,6 +326,9 @@ class SmolLMB200:
         lens = [len(p) for p in prompts]
         if not lens or min(lens) < 1 or max_new_tokens < 1:
             raise ValueError("every prompt needs a token and max_new_tokens must be positive")
+        flat = [int(t) for p in prompts for t in p]
+        if min(flat) < 0 or max(flat) >= self.embed.shape[0]:
+            raise ValueError(f"prompt tokens must lie in the vocabulary, 0 to {self.embed.shape[0] - 1}")
         if max(lens) + max_new_tokens > self.cfg.max_pos:
             raise ValueError(f"{max(lens)} + {max_new_tokens} tokens exceed the rotary table length {self.cfg.max_pos}")
         room = [n + max_new_tokens for n in lens]
@@ -334,7 +337,7 @@ class SmolLMB200:
         seqs = cache.reserve(room)
         try:
             cu = torch.tensor([0] + lens, dtype=torch.int32).cumsum(0, dtype=torch.int32).to(self.device)
-            ids = torch.tensor([t for p in prompts for t in p], dtype=torch.long, device=self.device)
+            ids = torch.tensor(flat, dtype=torch.long, device=self.device)
             greedy = not isinstance(temperature, torch.Tensor) and temperature <= 0
             out = torch.empty((max_new_tokens, len(lens)), dtype=torch.long, device=self.device)
             logits = self.prefill_packed(ids, cu, seqs)
