@@ -329,9 +329,9 @@ class SmolLMB200:
         flat = [int(t) for p in prompts for t in p]
         if min(flat) < 0 or max(flat) >= self.embed.shape[0]:
             raise ValueError(f"prompt tokens must lie in the vocabulary, 0 to {self.embed.shape[0] - 1}")
-        if max(lens) + max_new_tokens > self.cfg.max_pos:
-            raise ValueError(f"{max(lens)} + {max_new_tokens} tokens exceed the rotary table length {self.cfg.max_pos}")
-        room = [n + max_new_tokens for n in lens]
+        room = [n + max_new_tokens - 1 for n in lens]  # the last token is not fed back
+        if max(room) > self.cfg.max_pos:
+            raise ValueError(f"{max(room)} positions exceed the rotary table length {self.cfg.max_pos}")
         if cache is None:
             cache = self.new_paged_cache(sum(-(-r // page) for r in room), page)
         seqs = cache.reserve(room)
