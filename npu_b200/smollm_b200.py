@@ -308,7 +308,7 @@ class SmolLMB200:
 
     @torch.no_grad()
     def decode_packed(self, ids: torch.Tensor, seqs: PagedSequences) -> torch.Tensor:
-        """Logits [B, vocab] after one more token ids [B] of every sequence. A
+        """Logits [B, vocab] after one more token ids [B], from 0 on, of every sequence. A
         sequence whose pages are full keeps its keys and its logits mean
         nothing; api.device_error() reports it."""
         if ids.dim() != 1 or ids.numel() != seqs.batch:
@@ -321,8 +321,9 @@ class SmolLMB200:
                  generator: Optional[torch.Generator] = None) -> torch.Tensor:
         """max_new_tokens tokens after each prompt (a list of token lists, of
         any lengths from 1), int64 [B, max_new_tokens] on the device. The
-        settings are those of api.sample; temperature 0 is greedy. Nothing
-        synchronises with the host in between."""
+        settings are those of api.sample; temperature 0 is greedy. A prompt
+        whose logits hold no usable one gives -1 there and in the rest of its
+        row. Nothing synchronises with the host in between."""
         lens = [len(p) for p in prompts]
         if not lens or min(lens) < 1 or max_new_tokens < 1:
             raise ValueError("every prompt needs a token and max_new_tokens must be positive")
@@ -347,8 +348,10 @@ class SmolLMB200:
                 with profile("sample"):
                     api.sample(logits, noise, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p,
                                out=out[step])
+                if step > 0:  # once -1, always -1
+                    torch.where(out[step - 1] < 0, out[step - 1], out[step], out=out[step])
                 if step + 1 < max_new_tokens:
-                    logits = self.decode_packed(out[step], seqs)
+                    logits = self.decode_packed(out[step].clamp(min=0), seqs)
         finally:
             seqs.release()
         return out.T.contiguous()
