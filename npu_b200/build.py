@@ -68,13 +68,16 @@ def _build_binding(force: bool) -> None:
     root = Path(torch.__file__).resolve().parent
     nvcc = Path(_nvcc()).resolve()
     tmp = BINDING.with_suffix(".so.tmp")
-    cmd = [os.environ.get("CXX") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-w",
+    # The host compiler that nvcc takes, and torch's libstdc++: a compiler whose own is static would put a second
+    # C++ runtime into the process (CXX named one here), whose locale nobody sets up.
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-w",
            "-I", str(INCLUDE), "-isystem", str(root / "include"),
            "-isystem", str(root / "include" / "torch" / "csrc" / "api" / "include"),
            "-isystem", sysconfig.get_paths()["include"], "-isystem", str(nvcc.parent.parent / "include"),
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            str(BINDING_SOURCE), "-o", str(tmp), "-L", str(PKG), "-l:libb2attn.so", "-L", str(root / "lib"),
-           "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
+           "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", "-l:libstdc++.so.6",
+           "-Wl,-rpath,$ORIGIN"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"building {BINDING.name} failed:\n{r.stdout}\n{r.stderr}")
