@@ -157,6 +157,7 @@ Tensor decode_paged(const Tensor& q, const Tensor& k_pages, const Tensor& v_page
   const c10::cuda::CUDAGuard guard(device);
   Tensor o = output(out, q.sizes(), out_dtype, q,
                     "out must match [B, Hq, D], out_dtype and q's device, with a contiguous last dim");
+  if (B == 0) return o;
   const size_t need =
       b2a_decode_paged_workspace_bytes(as_int("B", B), as_int("Hq", Hq), as_int("Hkv", Hkv), as_int("D", D));
   // Scratch taken here goes back when the call returns; what reuses it on this
@@ -230,6 +231,15 @@ py::object rope_append_paged(const Tensor& q, const Tensor& k, const Tensor& v, 
   OptTensor ko, vo;
   if (return_kv) ko = empty({N, Hkv, D}, at::kBFloat16, q);
   if (return_kv && !bf16) vo = empty({N, Hkv, D}, at::kBFloat16, q);
+  auto result = [&]() -> py::object {
+    if (return_kv) return py::make_tuple(qo, *ko, bf16 ? v : *vo);
+    return py::cast(qo);
+  };
+  if (N == 0) {  // the lengths are the positions
+    if (seqlens_out && start) seqlens_out->copy_(*start);
+    if (seqlens_out && !start) seqlens_out->fill_(start_pos);
+    return result();
+  }
   check(b2a_rope_append_paged(q.data_ptr(), k.data_ptr(), v.data_ptr(), Strides(q, 2), Strides(k, 2), Strides(v, 2),
                               bf16, pointer(q_norm), pointer(k_norm), (float)eps, cos.data_ptr(), sin.data_ptr(),
                               cos.scalar_type() == at::kFloat, as_int("max_pos", cos.size(0)),
@@ -242,8 +252,7 @@ py::object rope_append_paged(const Tensor& q, const Tensor& k, const Tensor& v, 
                               static_cast<int*>(pointer(start)), static_cast<int*>(pointer(seqlens_out)),
                               stream_of(q)),
         "b2a_rope_append_paged");
-  if (return_kv) return py::make_tuple(qo, *ko, bf16 ? v : *vo);
-  return py::cast(qo);
+  return result();
 }
 
 // A sampling setting: a number for every row, or a per-row tensor.
@@ -280,6 +289,7 @@ Tensor sample(const Tensor& logits, const OptTensor& noise, const py::handle& te
   if (!noise && (t.rows || t.all > 0)) refuse("a temperature above 0 needs noise");
   const c10::cuda::CUDAGuard guard(device);
   Tensor o = output(out, {R}, at::kLong, logits, "out must be a contiguous int64 tensor [R] on the logits' device");
+  if (R == 0) return o;
   check(b2a_sample(logits.data_ptr(), logits.stride(0), bf16, static_cast<float*>(pointer(noise)),
                    noise ? noise->stride(0) : 0, as_int("R", R), as_int("V", V), t.rows, (float)t.all, k.rows,
                    (int)std::min(std::max(k.all, -1.0), 2147483647.0), p.rows, (float)p.all, m.rows, (float)m.all,
