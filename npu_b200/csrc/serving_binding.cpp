@@ -79,7 +79,7 @@ Tensor empty(at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) {
 
 Tensor output(const OptTensor& out, at::IntArrayRef sizes, at::ScalarType type, const Tensor& like, const char* what) {
   if (!out) return empty(sizes, type, like);
-  if (out->scalar_type() != type || out->sizes() != sizes || (out->dim() && out->stride(-1) != 1) ||
+  if (out->scalar_type() != type || out->sizes() != sizes || (out->size(-1) > 1 && out->stride(-1) != 1) ||
       out->device() != like.device())
     refuse(what);
   return *out;
@@ -268,7 +268,11 @@ struct Setting {
         refuse(name, " must be a number or a contiguous ", type, " tensor [", R, "] on the logits' device");
       rows = t.data_ptr<T>();
     } else {
-      all = value.cast<double>();
+      try {
+        all = value.cast<double>();
+      } catch (const py::cast_error&) {
+        refuse(name, " must be a number or a tensor [", R, "] on the logits' device");
+      }
     }
   }
 };
@@ -286,6 +290,7 @@ Tensor sample(const Tensor& logits, const OptTensor& noise, const py::handle& te
   const Setting<float> t("temperature", temperature, R, device), p("top_p", top_p, R, device),
       m("min_p", min_p, R, device);
   const Setting<int> k("top_k", top_k, R, device);
+  if (std::isnan(k.all)) refuse("top_k must not be NaN");
   if (!noise && (t.rows || t.all > 0)) refuse("a temperature above 0 needs noise");
   const c10::cuda::CUDAGuard guard(device);
   Tensor o = output(out, {R}, at::kLong, logits, "out must be a contiguous int64 tensor [R] on the logits' device");
