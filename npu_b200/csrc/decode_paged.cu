@@ -27,11 +27,11 @@
 // tiles (kWholeTiles) are not cut: one CTA per pair, one launch.
 //
 // Measured on one B200 (device time): 128 sequences of 1024 to 32768 keys,
-// 32 / 4 heads of 128, pages of 64: 415 us, 6.52 TB/s (1.00 of the measured
+// 32 / 4 heads of 128, pages of 64: 411 us, 6.58 TB/s (1.01 of the measured
 // copy rate); 16 of 100 to 20000, 16 / 2 gated heads of 256, pages of 48: 36 us,
 // 4.9 TB/s, 4 us of it the first tile's latency and 4 the joining launch; 48 of
-// 30 to 4001, 9 / 3 heads of 64, pages of 16: 14 us, of which those two and the
-// launch are 8; one of 77 keys: 4.4 us.
+// 30 to 4001, 9 / 3 heads of 64, pages of 16: 13.2 us, of which those two and
+// the launch are 7; one of 77 keys: 4.2 us.
 //
 // Slots of a page past the sequence's end may hold anything, NaN included:
 // their scores are replaced by -inf and their V rows by zeros in shared

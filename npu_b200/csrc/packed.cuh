@@ -5,12 +5,13 @@
 // The kernels are prefill_packed_d64.cu, and prefill.cu's (head dim 128) and
 // prefill_d256.cu's with PACKED: a sequence's rows and keys are offsets into
 // one tensor map each. Measured on one B200 (device time): prompts of 1122, 1593, 2780 and 8192 tokens, 32 / 4
-// heads of 128: 590 us, 1.09 PFLOP/s (0.66 of the measured bf16 rate, as the
-// dense kernel); chunks of 65 to 2501 gated tokens behind 500 cached ones,
-// 16 / 2 heads of 256: 205 us, 0.81 PFLOP/s; 32 prompts of 17 to 2048 tokens,
-// 9 / 3 heads of 64: 44.5 us, 0.32 PFLOP/s (21 % of each 128 x 128 block is
-// padding or masked and most items have one to five blocks); 3 prompts of 1 to
-// 40: 6.4 us, one launch, of which finding the block is 1.2.
+// heads of 128: 590 us at first to 690 under the power limit, 1.09 to 0.93
+// PFLOP/s (0.66 to 0.57 of the measured bf16 rate, as the dense kernel); chunks
+// of 65 to 2501 gated tokens behind 500 cached ones, 16 / 2 heads of 256: 213 to
+// 229 us, 0.78 to 0.73 PFLOP/s; 32 prompts of 17 to 2048 tokens, 9 / 3 heads of
+// 64: 42.2 us, 0.33 PFLOP/s (21 % of each 128 x 128 block is padding or masked
+// and most items have one to five blocks); 3 prompts of 1 to 40: 5.9 to 6.3 us,
+// one launch, of which finding the block is 1.2.
 #pragma once
 
 #include <type_traits>

@@ -809,8 +809,8 @@ PrefillPlan prefill_plan(int D, int Hq, int Hkv, int Tq, int Tk) {
 
 // Packed sequences: head dim 64 and 256 have kernels of their own with one-tile
 // items (at 64 faster than two-tile items at every length measured: 8 prompts
-// of 1500, 9 / 3 heads, 55.8 us against 57.2; 4 of 4096, 136.7 against 146.8;
-// 24 of 700, 8 / 2 heads, 45.2 against 50.2; 4 of 4096, 125.6 against 132.0).
+// of 1500, 9 / 3 heads, 52.5 us against 57.2; 4 of 4096, 129 against 146.8;
+// 24 of 700, 8 / 2 heads, 41.2 against 50.2; 4 of 4096, 119 against 132).
 // Head dim 128 goes by the same rules on the average length (the lengths
 // themselves are on the device). Row pairs only for odd groups: an even group
 // shares its key blocks between heads at any length.

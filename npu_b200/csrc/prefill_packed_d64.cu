@@ -22,9 +22,9 @@
 // softmax_half_packed). Kept in registers between the two, the scores spill.
 //
 // Measured on one B200 (device time): 32 prompts of 17 to 2048 tokens, 9 / 3
-// heads, 44.5 us against 49.5 with one softmax warpgroup of 64 scores a thread
-// (prefill.cu's one-tile items); 4 prompts of 4096, 136.7 us against 146.8 with
-// its two-tile items; 3 prompts of 1 to 40, 6.4 us against 7.1. A
+// heads, 42.2 us against 49.5 with one softmax warpgroup of 64 scores a thread
+// (prefill.cu's one-tile items); 4 prompts of 4096, 129 us against 146.8 with
+// its two-tile items; 3 prompts of 1 to 40, 5.9 to 6.3 us against 7.1. A
 // block of 128 keys takes 1.9 us a CTA, of which MUFU is busy 1.1 (both CTAs);
 // the rest is the way from P through PV and S to the next scores, 0.55 us.
 //

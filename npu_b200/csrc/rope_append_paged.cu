@@ -21,9 +21,9 @@
 // the tables are read once per warp and reused for its heads.
 //
 // Measured on one B200 (device time): 10209 prompt tokens, 16 / 2 heads of 256
-// with norms and 64 turned lanes: 47 us, 4.7 TB/s (0.73 of the measured copy
-// rate; issue slots at 64 % are the next bound); 64 single tokens, 32 / 4 heads
-// of 128: 3.0 us, one launch.
+// with norms and 64 turned lanes: 45 us, 5.0 TB/s (0.76 of the measured copy
+// rate; issue slots at 64 % are the next bound), from fp32 sources 58 us, 5.9
+// TB/s (0.90); 64 single tokens, 32 / 4 heads of 128: 3.0 us, one launch.
 #include "capi_internal.cuh"
 #include "rope_append_paged.cuh"
 

@@ -25,12 +25,15 @@
 // only for tokens above a cut where min_p or top_k gives one; later ones only
 // for the tokens ahead of the pivot.
 //
-// Bound by memory in the plain cases, by the latency of the passes (a join is
-// 1 us) with filters. Measured on one B200 (device time), 256 rows of 131071
-// bf16 logits: greedy 21 us (3.2 TB/s), unfiltered 47 us (4.3 TB/s of logits
-// and noise), min_p 0.05 28 us, top_k 50 60 us, top_p 0.9 88 us, each row its
-// own of such settings 58 to 64 us; one row of 49152 fp32 logits: greedy 2.6 us,
-// unfiltered 4.0, top_k 50 with top_p 0.9 6.2.
+// Bound by latency: with filters that of the passes (a join is 1 us, a tenth of
+// it for the block to agree that no wait ran out), without them that of the
+// loads (74 rows are resident, and a row's slice is asked for when its cluster
+// starts). Measured on one B200 (device time, 8 draws of the inputs), 256 rows
+// of 131071 bf16 logits: greedy 20 us (3.3 TB/s, half of the measured copy
+// rate), unfiltered 49 us (4.1 TB/s of logits and noise), min_p 0.05 29 us,
+// top_k 50 65 to 69, top_p 0.9 82 to 95, each row its own of such settings 60
+// to 73; one row of 49152 fp32 logits: greedy 2.6 us, unfiltered 4.3, top_k 50
+// with top_p 0.9 6.4 to 8.9.
 #include "capi_internal.cuh"
 #include "sample.cuh"
 
