@@ -58,10 +58,30 @@ struct OncePerDevice {
   }
 };
 
+// Both give this launch's status: an error that somebody left in the runtime
+// before is not taken for it, and a failed launch leaves none (the next
+// cudaGetLastError would report it as somebody else's).
+template <typename... Params, typename... Args>
+inline cudaError_t launch_config(const cudaLaunchConfig_t& cfg, void (*kernel)(Params...), const Args&... args) {
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+  if (e != cudaSuccess) cudaGetLastError();
+  return e;
+}
+
+template <typename... Params, typename... Args>
+inline cudaError_t launch_plain(void (*kernel)(Params...), dim3 grid, unsigned threads, size_t smem, cudaStream_t st,
+                                const Args&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  return launch_config(cfg, kernel, args...);
+}
+
 // Launch as a programmatic dependent: the grid may be scheduled while the
 // kernel before it in the stream drains. Its threads wait (grid_dep_wait)
-// before they touch memory. Takes a failed launch's error out of the runtime
-// (the next cudaGetLastError would report it as somebody else's).
+// before they touch memory.
 template <typename... Params, typename... Args>
 inline cudaError_t launch_dependent(void (*kernel)(Params...), dim3 grid, unsigned threads, size_t smem,
                                     cudaStream_t st, int cluster, const Args&... args) {
@@ -78,8 +98,7 @@ inline cudaError_t launch_dependent(void (*kernel)(Params...), dim3 grid, unsign
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = cluster > 0 ? 2 : 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...), last = cudaGetLastError();
-  return e == cudaSuccess ? last : e;
+  return launch_config(cfg, kernel, args...);
 }
 
 constexpr float kApiLog2e = 1.4426950408889634f;

@@ -766,8 +766,7 @@ static int launch_prefill_t(const CUtensorMap& tq, const CUtensorMap& tk, const 
   return once.run(prepare, [&] {
     if (PACKED && NQT == 1)
       return launch_dependent(kernel, dim3((unsigned)nblk), C::THREADS, C::SMEM_BYTES, st, 0, tq, tk, tv, p);
-    kernel<<<(unsigned)nblk, C::THREADS, C::SMEM_BYTES, st>>>(tq, tk, tv, p);
-    return cudaGetLastError();
+    return launch_plain(kernel, dim3((unsigned)nblk), C::THREADS, C::SMEM_BYTES, st, tq, tk, tv, p);
   });
 }
 

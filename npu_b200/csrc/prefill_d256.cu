@@ -455,8 +455,8 @@ int launch_d256(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap&
                                     C::SMEM_BYTES) == cudaSuccess;
       },
       [&] {
-        fa_prefill_d256_kernel<PACKED><<<(unsigned)nblk, C::THREADS, C::SMEM_BYTES, st>>>(tq, tk, tv, p);
-        return cudaGetLastError();
+        return launch_plain(fa_prefill_d256_kernel<PACKED>, dim3((unsigned)nblk), C::THREADS, C::SMEM_BYTES, st, tq, tk,
+                            tv, p);
       });
 }
 

@@ -20,7 +20,8 @@ extern "C" cudaError_t cudaGetDevice(int* d) { *d = 3; return cudaSuccess; }
 extern "C" cudaError_t cudaGetLastError() { const cudaError_t e = left; left = cudaSuccess; return e; }
 extern "C" cudaError_t cudaLaunchKernelExC(const cudaLaunchConfig_t*, const void*, void**) {
   ++launches;
-  return left = prepared && !broken ? cudaSuccess : cudaErrorInvalidValue;
+  if (prepared && !broken) return cudaSuccess;
+  return left = cudaErrorInvalidValue;
 }
 static void kernel(int) {}
 static b2a::OncePerDevice once;
@@ -41,6 +42,9 @@ int main() {
   CHECK(call() != 0 && left == cudaSuccess);  // reported by the call, not by the next one
   broken = false;
   CHECK(call() == 0 && left == cudaSuccess);
+  left = cudaErrorInvalidDevice;  // somebody else's error: the call works, once, and leaves it to them
+  launches = 0;
+  CHECK(call() == 0 && launches == 1 && left == cudaErrorInvalidDevice);
   return 0;
 }
 """
