@@ -300,11 +300,13 @@ class SmolLMB200:
     def prefill_packed(self, ids: torch.Tensor, cu_seqlens: torch.Tensor, seqs: PagedSequences) -> torch.Tensor:
         """Logits [B, vocab] of each prompt's last token, for prompts packed in
         ids [N] (sequence b: ids[cu_seqlens[b] : cu_seqlens[b + 1]], none empty)
-        into the new, empty sequences `seqs`."""
+        into the new, empty sequences `seqs`. Of offsets that are not a stretch
+        of ids the logits mean nothing; api.device_error() reports them."""
         if ids.dim() != 1 or cu_seqlens.numel() != seqs.batch + 1:
             raise ValueError("ids must be [N] and cu_seqlens [B + 1] with B = seqs.batch")
         x = self._forward_packed(ids.to(self.device), seqs, cu_seqlens)
-        return F.linear(x[(cu_seqlens[1:] - 1).long()], self.embed)
+        last = (cu_seqlens[1:] - 1).long().clamp(0, x.shape[0] - 1)  # an index past the end would fault
+        return F.linear(x[last], self.embed)
 
     @torch.no_grad()
     def decode_packed(self, ids: torch.Tensor, seqs: PagedSequences) -> torch.Tensor:

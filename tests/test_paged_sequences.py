@@ -77,3 +77,25 @@ def test_a_step_past_the_pages_leaves_the_others_alone(cuda_dev):
     assert written.tolist() == [[0, seqs.block_table[0, 1].item(), 0]]
     _, _, _, room_for_both = steps([48, 48])
     assert device_error() == 0 and torch.equal(logits[0], room_for_both[0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cu", [[0, 5, 900], [0, -3, 10], [0, 5, -7]])
+def test_prompt_offsets_past_the_tokens_are_reported(cuda_dev, cu):
+    """Not a fault: the bad prompt is left out, a good one keeps its logits."""
+    from npu_b200 import _lib, device_error
+
+    model = tiny(cuda_dev)
+    ids = torch.arange(10, device=cuda_dev)
+
+    def logits(cu):
+        cache = model.new_paged_cache(8, 16)
+        return model.prefill_packed(ids, torch.tensor(cu, dtype=torch.int32, device=cuda_dev), cache.reserve([16, 16]))
+
+    good = logits([0, 5, 10])
+    assert device_error() == 0
+    got = logits(cu)
+    torch.cuda.synchronize()
+    assert device_error() == _lib.B2A_ERR_DEVICE_BAD_LEN
+    if cu[1] == 5:
+        assert torch.equal(got[0], good[0])
