@@ -359,7 +359,8 @@ B2A_API int b2a_decode_paged(const void* q, const void* k_pages, const void* v_p
  * which is read while it is written. cos_tab / sin_tab [max_pos, rope_dim] are fp32
  * (tab_fp32 = 1) or of the source type; computed in fp32, rounded once.
  * Tokens whose position or page is out of range are skipped (only k and v, if
- * it is only the page) and report B2A_ERR_DEVICE_BAD_LEN. Supported D: 64, 128, 256.
+ * it is only the page) and report B2A_ERR_DEVICE_BAD_LEN; so does a pair of
+ * offsets that is not a stretch of the tokens, whose sequence is left out. Supported D: 64, 128, 256.
  */
 B2A_API int b2a_rope_append_paged(const void* q, const void* k, const void* v, const long long* q_strides,
                                   const long long* k_strides, const long long* v_strides, int src_bf16,

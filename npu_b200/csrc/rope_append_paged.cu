@@ -95,6 +95,11 @@ __device__ __forceinline__ int find_sequence(const int* cu, int B, long long n) 
   return lo;
 }
 
+// Whether offsets c0 and c1 are a stretch of the tokens.
+__device__ __forceinline__ bool is_stretch(const RopeAppendPagedParams& p, int c0, int c1) {
+  return c0 >= 0 && c1 >= c0 && c1 <= p.N;
+}
+
 constexpr int kWarps = 4;  // tokens of a block
 
 // Warp x of block (i, y) takes token i kWarps + x and chunk y of its rows: the
@@ -109,9 +114,14 @@ __global__ void __launch_bounds__(32 * kWarps)
   const long long n = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5);  // token
   grid_dep_wait();
   grid_dep_launch();
-  if (blockIdx.x == 0 && blockIdx.y == 0 && p.seqlens_out)
-    for (int b = threadIdx.x; b < p.B; b += 32 * kWarps)
-      p.seqlens_out[b] = (p.start_pos_arr ? p.start_pos_arr[b] : p.start_pos) + p.cu_seqlens[b + 1] - p.cu_seqlens[b];
+  if (blockIdx.x == 0 && blockIdx.y == 0)
+    for (int b = threadIdx.x; b < p.B; b += 32 * kWarps) {
+      const int c0 = p.cu_seqlens[b], c1 = p.cu_seqlens[b + 1];
+      const bool good = is_stretch(p, c0, c1);
+      if (!good && p.err) atomicOr(p.err, kErrBadArgs);
+      if (p.seqlens_out)
+        p.seqlens_out[b] = (p.start_pos_arr ? p.start_pos_arr[b] : p.start_pos) + (good ? c1 - c0 : 0);
+    }
   if (n >= p.N) return;
   const bool q_rows = (int)blockIdx.y < q_chunks;  // q, else k and v
   // Step s takes row j0 + s ROWS of q, or of k and then v.
@@ -143,7 +153,7 @@ __global__ void __launch_bounds__(32 * kWarps)
   // The token's sequence, position and page: the same for the whole warp.
   const int b = find_sequence(p.cu_seqlens, p.B, n);
   const int c0 = p.cu_seqlens[b], c1 = p.cu_seqlens[b + 1];
-  if (n < c0 || n >= c1) return;  // a row outside every sequence
+  if (n < c0 || n >= c1 || !is_stretch(p, c0, c1)) return;  // a row outside every sequence
   const long long at = (long long)(p.start_pos_arr ? p.start_pos_arr[b] : p.start_pos) + (n - c0);
   const bool counts = at >= 0 && at <= 0x7fffffff;
   const unsigned pos = counts ? (unsigned)at : 0u;

@@ -78,3 +78,33 @@ def test_tokens_past_the_rotary_tables_are_skipped_whole(cuda_dev, dtype, tokens
         assert (rows[20:] == 3).all() and (rows[:first] == 3).all()
         assert (rows[first:20] != 3).any(-1).all()
     assert (q_out[n:] == 3).all() and (q_out[:n] != 3).any(-1).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("cu,good", [([0, 5, 900], 0), ([-3, 5, 10], 1), ([0, 5, -7], 0), ([5, 0, 5], 1),
+                                     ([0, 11, 10], None)])
+@pytest.mark.parametrize("lengths", [True, False])
+def test_append_reports_offsets_that_are_no_stretch(cuda_dev, cu, good, lengths, dtype):
+    """Two sequences over ten tokens, at most one of them good: its tokens are written, the other's are not and its
+    length stays."""
+    from npu_b200 import _lib, device_error, rope_append_paged
+
+    g = torch.Generator(device=cuda_dev).manual_seed(2)
+    q = torch.randn(10, 4, 64, generator=g, device=cuda_dev).to(dtype)
+    kv = torch.randn(2, 10, 2, 64, generator=g, device=cuda_dev).to(dtype)
+    tab = torch.randn(2, 32, 64, generator=g, device=cuda_dev).to(dtype)
+    kp, vp = (torch.full((4, 2, 16, 64), 3.0, dtype=torch.bfloat16, device=cuda_dev) for _ in range(2))
+    table = torch.arange(4, dtype=torch.int32, device=cuda_dev).view(2, 2)
+    end = torch.full((2,), -1, dtype=torch.int32, device=cuda_dev) if lengths else None
+    assert device_error() == 0
+    rope_append_paged(q, kv[0], kv[1], tab[0], tab[1], kp, vp, table, torch.tensor(cu, dtype=torch.int32, device=cuda_dev),
+                      start_pos=4, seqlens_out=end)
+    assert device_error() == _lib.B2A_ERR_DEVICE_BAD_LEN
+    n = [0, 0]
+    if good is not None:
+        n[good] = cu[good + 1] - cu[good]
+    if lengths:
+        assert end.tolist() == [4 + t for t in n]
+    for b in range(2):
+        rows = kp[2 * b:2 * b + 2].transpose(1, 2).reshape(32, 2, 64)
+        assert (rows[4:4 + n[b]] != 3).any(-1).all() and (rows[:4] == 3).all() and (rows[4 + n[b]:] == 3).all()
