@@ -296,7 +296,8 @@ B2A_API int b2a_prefill_host(const void* q, const void* k, const void* v, void* 
 
 /*
  * Serving sequences of different lengths together: attention over packed
- * prompts, a paged KV cache (append, single-token attention) and sampling.
+ * prompts, a paged KV cache (append, single-token attention, reading back), bf16
+ * or 8-bit, penalties on logits and sampling.
  *
  * Packed tensors hold the sequences' tokens one after another: sequence b owns
  * rows [cu[b], cu[b + 1]) of a tensor, cu int32 [B + 1] on the device, not
@@ -371,6 +372,84 @@ B2A_API int b2a_rope_append_paged(const void* q, const void* k, const void* v, c
                                   const int* block_table, long long table_ld, int table_width, int n_pages,
                                   int page, const int* cu_seqlens, int B, int N, int Hq, int Hkv, int D,
                                   int start_pos, const int* start_pos_per_batch, int* seqlens_out, void* stream);
+
+/*
+ * b2a_rope_append_paged into an 8-bit cache: pools of e4m3 values (strides in
+ * elements, multiples of 16) and, for each token and KV head, a scale in
+ * k_scales / v_scales [n_pages, Hkv, page] fp32 (contiguous slots; strides
+ * {page, head} multiples of 4, 16-byte aligned). A row y (k after norm and
+ * rotation, v) is stored as e4m3(y / s), s = max(max|y| / 448, 2^-100), from the
+ * fp32 values; rows with an infinity or a NaN read back as NaN. k_out / v_out
+ * receive the values before that rounding, as bf16.
+ */
+B2A_API int b2a_rope_append_paged_e4m3(const void* q, const void* k, const void* v, const long long* q_strides,
+                                       const long long* k_strides, const long long* v_strides, int src_bf16,
+                                       const void* q_norm, const void* k_norm, float eps, const void* cos_tab,
+                                       const void* sin_tab, int tab_fp32, int max_pos, int rope_dim, void* q_out,
+                                       void* k_out, void* v_out, void* k_pages, void* v_pages,
+                                       const long long* k_page_strides, const long long* v_page_strides,
+                                       float* k_scales, float* v_scales, const long long* k_scale_strides,
+                                       const long long* v_scale_strides, const int* block_table, long long table_ld,
+                                       int table_width, int n_pages, int page, const int* cu_seqlens, int B, int N,
+                                       int Hq, int Hkv, int D, int start_pos, const int* start_pos_per_batch,
+                                       int* seqlens_out, void* stream);
+
+/*
+ * b2a_decode_paged over an 8-bit cache as b2a_rope_append_paged_e4m3 writes it:
+ * key and value are the e4m3 numbers times their row's scale, not rounded to
+ * fewer bits on the way (e4m3's NaN, stored under a NaN scale only, is not looked
+ * for by itself). Slots and scales past a sequence's end may hold anything.
+ */
+B2A_API int b2a_decode_paged_e4m3(const void* q, const void* k_pages, const void* v_pages, const float* k_scales,
+                                  const float* v_scales, const long long* k_scale_strides,
+                                  const long long* v_scale_strides, const int* block_table, long long table_ld,
+                                  int table_width, const int* seqlens, const void* gate, void* o, int B, int Hq,
+                                  int Hkv, int n_pages, int page, int D, const long long* q_strides,
+                                  const long long* k_strides, const long long* v_strides,
+                                  const long long* gate_strides, const long long* o_strides, int gate_bf16,
+                                  float scale, int out_fp32, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * k and v of a stretch of each sequence out of a paged cache, as packed rows
+ * k_out / v_out [N, Hkv, D] bf16 contiguous (what b2a_prefill_varlen reads):
+ * row n of sequence b (cu[b] <= n < cu[b + 1]) is the key at position
+ * start + n - cu[b]. bf16 pools (k_scales and v_scales NULL) or 8-bit ones (as
+ * b2a_rope_append_paged_e4m3; a value is its e4m3 times its scale, rounded to
+ * bf16 once). Rows outside every sequence are not written; a position without
+ * a page gives zeros, a pair of offsets that is not a stretch of the N rows
+ * leaves its sequence out, and both report B2A_ERR_DEVICE_BAD_LEN.
+ * Supported D: 64, 128, 256.
+ */
+B2A_API int b2a_gather_paged(const void* k_pages, const void* v_pages, const long long* k_page_strides,
+                             const long long* v_page_strides, const float* k_scales, const float* v_scales,
+                             const long long* k_scale_strides, const long long* v_scale_strides,
+                             const int* block_table, long long table_ld, int table_width, int n_pages, int page,
+                             const int* cu_seqlens, int B, int N, int Hkv, int D, int start_pos,
+                             const int* start_pos_per_batch, void* k_out, void* v_out, void* stream);
+
+/*
+ * Penalties for repeated tokens, a bias and a mask on logits [R, V] (fp32, or
+ * bf16 with logits_bf16 = 1; row stride ld_logits), before b2a_sample. Row r has
+ * the tokens tokens[r, 0 .. lengths[r] - 1] (int32, or int64 with tokens_64 = 1;
+ * strides tokens_row and tokens_step; lengths NULL: all L), of which the first
+ * prompt_lengths[r] (NULL: none) are its prompt; ids outside 0 .. V - 1 count
+ * for nothing. For token v, c = how often it is among those after the prompt:
+ *   y = x > 0 ? x / repetition : x * repetition   if v is among all of them
+ *   y = y - frequency c - (c > 0 ? presence : 0)
+ *   y = y + bias[r, v]                            (bias optional, fp32)
+ *   y = -inf  unless bit v % 32 of allowed[r, v / 32] is set (optional, int32)
+ * each step rounded in fp32, the result to the logits' type. repetition,
+ * frequency, presence: per-row device arrays [R], or NULL for the *_all value
+ * (repetition_all above 0). ld_bias / ld_allowed 0: one row for all. out
+ * [R, V] (row stride ld_out): the logits themselves, or apart from them. A
+ * length outside 0 .. L is cut and reports B2A_ERR_DEVICE_BAD_LEN. V, L <= 2^30.
+ */
+B2A_API int b2a_penalize(const void* logits, long long ld_logits, int logits_bf16, const void* tokens, int tokens_64,
+                         long long tokens_row, long long tokens_step, int L, const int* lengths,
+                         const int* prompt_lengths, const float* repetition, float repetition_all,
+                         const float* frequency, float frequency_all, const float* presence, float presence_all,
+                         const float* bias, long long ld_bias, const int* allowed, long long ld_allowed, void* out,
+                         long long ld_out, int R, int V, void* stream);
 
 /*
  * The next token of each row of logits [R, V] (fp32, or bf16 with

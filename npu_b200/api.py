@@ -4,7 +4,8 @@ and the fused RoPE + KV-cache append that feeds them.
 These are the B200 entry points behind the reference-compatible wrapper in
 npu_b200.fa (NpuAttention.run_batch), and the operators that serve sequences
 of different lengths together: attention over packed prompts, a paged KV cache
-(append, single-token attention) and token sampling. Tensors are CUDA bf16 with a contiguous
+(append, single-token attention, reading back; bf16 or 8-bit), penalties on
+logits and token sampling. Tensors are CUDA bf16 with a contiguous
 head dimension, except for prefill_host, which takes host bf16 tensors and
 moves them itself; nothing here falls back to a CPU path.
 """
@@ -493,6 +494,8 @@ def decode_paged(
     workspace: Optional[torch.Tensor] = None,
     out: Optional[torch.Tensor] = None,
     gate: Optional[torch.Tensor] = None,
+    k_scales: Optional[torch.Tensor] = None,
+    v_scales: Optional[torch.Tensor] = None,
 ) -> torch.Tensor:
     """`decode` over a paged cache: q [B, Hq, D] against page pools
     [n_pages, Hkv, page, D] (bf16, page a multiple of 16; any stored order with
@@ -504,9 +507,40 @@ def decode_paged(
     keys gives 0. Slots past a sequence's end may hold anything. The lengths
     stay on the device; scratch comes from `workspace` (a uint8 CUDA tensor of
     decode_paged_workspace_bytes) or torch's allocator. `gate` ([B, Hq, D])
-    as in `decode`.
+    as in `decode`. With k_scales and v_scales the pools are 8-bit
+    (float8_e4m3fn), as `rope_append_paged` writes them.
     """
-    return _serving().decode_paged(q, k_pages, v_pages, block_table, seqlens, scale, out_dtype, workspace, out, gate)
+    return _serving().decode_paged(q, k_pages, v_pages, block_table, seqlens, scale, out_dtype, workspace, out, gate,
+                                   k_scales, v_scales)
+
+
+def gather_paged(
+    k_pages: torch.Tensor,
+    v_pages: torch.Tensor,
+    block_table: torch.Tensor,
+    cu_seqlens: torch.Tensor,
+    n_tokens: int,
+    *,
+    start_pos: int = 0,
+    start_pos_per_batch: Optional[torch.Tensor] = None,
+    k_scales: Optional[torch.Tensor] = None,
+    v_scales: Optional[torch.Tensor] = None,
+    k_out: Optional[torch.Tensor] = None,
+    v_out: Optional[torch.Tensor] = None,
+):
+    """Cached keys and values as packed rows (k, v), each [n_tokens, Hkv, D]
+    bf16: what `prefill_varlen` reads, for prompts that continue cached ones.
+
+    Row n of sequence b (cu_seqlens[b] <= n < cu_seqlens[b + 1]; int32 CUDA
+    tensor [B + 1], read on the device) is the key at position p_b + n -
+    cu_seqlens[b], p_b = start_pos_per_batch[b] or start_pos; pools, scales and
+    block_table as `decode_paged`. 8-bit values are multiplied by their scale in
+    fp32 and rounded once. Rows outside every sequence are not written (those of
+    tensors made here hold anything); a position without a page gives zeros and
+    shows in `device_error()`.
+    """
+    return _serving().gather_paged(k_pages, v_pages, block_table, cu_seqlens, n_tokens, start_pos,
+                                   start_pos_per_batch, k_scales, v_scales, k_out, v_out)
 
 
 def rope_append_paged(
@@ -529,6 +563,8 @@ def rope_append_paged(
     norm_eps: float = 1e-6,
     rope_dim: Optional[int] = None,
     return_kv: bool = False,
+    k_scales: Optional[torch.Tensor] = None,
+    v_scales: Optional[torch.Tensor] = None,
 ):
     """`rope_append` for packed tokens and a paged cache: q [N, Hq, D], k and v
     [N, Hkv, D] (fp32 or bf16, last dim contiguous; typically views of one fused
@@ -544,10 +580,51 @@ def rope_append_paged(
     rope_dim as in `rope_append`. Returns q rotated, [N, Hq, D] bf16; with
     return_kv (q, k, v): k rotated and v as packed bf16 [N, Hkv, D] for
     `prefill_varlen` (v itself when it is bf16 already).
+
+    With k_scales and v_scales ([n_pages, Hkv, page] fp32, contiguous slots) the
+    pools are 8-bit (float8_e4m3fn): each token's k and v of a KV head, a row y
+    of D values, is stored as e4m3(y / s) with s = max(max |y| / 448, 2^-100) beside
+    it, from the fp32 values. A row with an infinity or a NaN reads back as NaN.
     """
     return _serving().rope_append_paged(q, k, v, cos, sin, k_pages, v_pages, block_table, cu_seqlens, start_pos,
                                         start_pos_per_batch, seqlens_out, q_out, q_norm, k_norm, norm_eps, rope_dim,
-                                        return_kv)
+                                        return_kv, k_scales, v_scales)
+
+
+def penalize(
+    logits: torch.Tensor,
+    tokens: Optional[torch.Tensor] = None,
+    lengths: Optional[torch.Tensor] = None,
+    *,
+    prompt_lengths: Optional[torch.Tensor] = None,
+    repetition=1.0,
+    frequency=0.0,
+    presence=0.0,
+    bias: Optional[torch.Tensor] = None,
+    allowed: Optional[torch.Tensor] = None,
+    out: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """Penalties for repeated tokens, a bias and a mask on logits [R, V] (fp32 or
+    bf16), before `sample`.
+
+    Row r has the tokens tokens[r, : lengths[r]] (int32 or int64 CUDA tensor
+    [R, L], any strides; lengths: int32 CUDA tensor [R], default all L), of which
+    the first prompt_lengths[r] (default none) are its prompt. Ids outside the
+    vocabulary count for nothing. For token v, found c times after the prompt:
+
+      y = x / repetition if x > 0 else x * repetition    if v is among all of them
+      y = y - frequency * c - (presence if c > 0 else 0)
+      y = y + bias[v]                  bias [V] or [R, V] fp32
+      y = -inf                         unless bit v % 32 of allowed[v // 32] is set
+
+    allowed is an int32 tensor [ceil(V / 32)] or [R, ceil(V / 32)] of 32 tokens a
+    word. repetition (above 0), frequency and presence are numbers or per-row fp32
+    CUDA tensors. Each step is rounded in fp32, the result to the logits' type.
+    `out` may be the logits themselves. A row whose mask leaves nothing is -inf
+    throughout, and `sample` gives -1 for it.
+    """
+    return _serving().penalize(logits, tokens, lengths, prompt_lengths, repetition, frequency, presence, bias, allowed,
+                               out)
 
 
 def sample(

@@ -390,8 +390,8 @@ int api_sm_count() {
   return n;
 }
 
-int api_tensor_map(CUtensorMap* m, const void* base, int rank, const unsigned long long* dims,
-                   const unsigned long long* byte_strides, const unsigned* box) {
+static int tensor_map(CUtensorMap* m, CUtensorMapDataType type, CUtensorMapSwizzle swizzle, const void* base, int rank,
+                      const unsigned long long* dims, const unsigned long long* byte_strides, const unsigned* box) {
   auto fn = encode_fn();
   if (!fn || rank < 1 || rank > 5) return B2A_ERR_TMA;
   cuuint64_t d[5] = {}, s[5] = {};
@@ -401,10 +401,22 @@ int api_tensor_map(CUtensorMap* m, const void* base, int rank, const unsigned lo
     b[i] = box[i];
     if (i + 1 < rank) s[i] = byte_strides[i];
   }
-  const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (cuuint32_t)rank, const_cast<void*>(base), d, s, b, es,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  const CUresult r = fn(m, type, (cuuint32_t)rank, const_cast<void*>(base), d, s, b, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? B2A_OK : B2A_ERR_TMA;
+}
+
+int api_tensor_map(CUtensorMap* m, const void* base, int rank, const unsigned long long* dims,
+                   const unsigned long long* byte_strides, const unsigned* box) {
+  return tensor_map(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, CU_TENSOR_MAP_SWIZZLE_128B, base, rank, dims, byte_strides,
+                    box);
+}
+
+int api_tensor_map_bytes(CUtensorMap* m, const void* base, int rank, const unsigned long long* dims,
+                         const unsigned long long* byte_strides, const unsigned* box) {
+  return tensor_map(m, CU_TENSOR_MAP_DATA_TYPE_UINT8,
+                    box[0] == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, base, rank, dims,
+                    byte_strides, box);
 }
 }  // namespace b2a
 

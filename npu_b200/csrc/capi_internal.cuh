@@ -24,6 +24,10 @@ int api_sm_count();
 int api_tensor_map(CUtensorMap* m, const void* base, int rank, const unsigned long long* dims,
                    const unsigned long long* byte_strides, const unsigned* box);
 
+// The same of bytes, with the swizzle of box[0] bytes (64 or 128).
+int api_tensor_map_bytes(CUtensorMap* m, const void* base, int rank, const unsigned long long* dims,
+                         const unsigned long long* byte_strides, const unsigned* box);
+
 inline bool api_aligned(const void* p, unsigned bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 
 // Strides are not negative and multiples of `mult` elements.

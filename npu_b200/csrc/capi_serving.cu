@@ -8,6 +8,8 @@
 #include "b2attn.h"
 #include "capi_internal.cuh"
 #include "decode_paged.cuh"
+#include "gather_paged.cuh"
+#include "penalize.cuh"
 #include "prefill.cuh"
 #include "rope_append_paged.cuh"
 #include "sample.cuh"
@@ -41,7 +43,190 @@ int pool_map(CUtensorMap* m, const void* base, int D, int n_pages, int heads, in
   return b2a::api_tensor_map(m, base, 5, dims, strides, box);
 }
 
+// The same of an 8-bit pool: 128 columns (head dim 64: 64), slot, column chunks, head, page.
+int pool_map_e4m3(CUtensorMap* m, const void* base, int D, int n_pages, int heads, int page, const long long* s,
+                  int box_rows) {
+  const unsigned columns = D < 128 ? D : 128;
+  const unsigned long long dims[5] = {columns, (unsigned long long)page, (unsigned long long)D / columns,
+                                      (unsigned long long)heads, (unsigned long long)n_pages};
+  const unsigned long long strides[4] = {(unsigned long long)s[2], 128, (unsigned long long)s[1],
+                                         (unsigned long long)s[0]};
+  const unsigned box[5] = {columns, (unsigned)box_rows, (unsigned)D / columns, 1u, 1u};
+  return b2a::api_tensor_map_bytes(m, base, 5, dims, strides, box);
+}
+
+// The scales of 8-bit pools (strides {page, head}): both there, and each page's 16-byte aligned for the copies of 16
+// or more slots that paged decode makes.
+int scales_ok(const void* k_scales, const void* v_scales, const long long* kss, const long long* vss) {
+  if (!k_scales || !v_scales || !kss || !vss) return B2A_ERR_INVALID_ARG;
+  if (!api_aligned(k_scales, 16) || !api_aligned(v_scales, 16) || !api_strides_ok(kss, 2, 4) ||
+      !api_strides_ok(vss, 2, 4))
+    return B2A_ERR_ALIGNMENT;
+  return B2A_OK;
+}
+
 int status_of(int rc) { return rc == -3 ? B2A_ERR_HEAD_DIM : (rc ? B2A_ERR_LAUNCH : B2A_OK); }
+
+int paged_attention(const void* q, const void* k_pages, const void* v_pages, const int* block_table,
+                    const float* k_scales, const float* v_scales, const long long* kss, const long long* vss,
+                    long long table_ld, int table_width, const int* seqlens, const void* gate, void* o, int B,
+                    int Hq, int Hkv, int n_pages, int page, int D, const long long* qs, const long long* ks,
+                    const long long* vs, const long long* gs, const long long* os, int gate_bf16, float scale,
+                    int out_fp32, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!q || !k_pages || !v_pages || !block_table || !seqlens || !o || !qs || !ks || !vs || !os || (gate && !gs))
+    return B2A_ERR_INVALID_ARG;
+  if (B <= 0 || Hq <= 0 || Hkv <= 0 || n_pages <= 0 || page <= 0 || page % 16 || table_width <= 0 ||
+      table_ld < table_width || (long long)table_width * page > INT_MAX - 64)
+    return B2A_ERR_INVALID_ARG;
+  if (!(scale > 0.f) || !std::isfinite(scale)) return B2A_ERR_INVALID_ARG;
+  if (!head_dim_ok(D)) return B2A_ERR_HEAD_DIM;
+  if (Hq % Hkv || Hq / Hkv > 16) return B2A_ERR_GQA;
+  if (!api_aligned(q, 16) || !api_aligned(k_pages, 16) || !api_aligned(v_pages, 16) ||
+      !api_aligned(o, out_fp32 ? 4 : 2) || !api_aligned(block_table, 4) || !api_aligned(seqlens, 4) ||
+      !api_aligned(gate, gate_bf16 ? 2 : 4))
+    return B2A_ERR_ALIGNMENT;
+  const long long pool_mult = k_scales ? 16 : 8;
+  if (!api_strides_ok(qs, 2, 8) || !api_strides_ok(ks, 3, pool_mult) || !api_strides_ok(vs, 3, pool_mult))
+    return B2A_ERR_ALIGNMENT;
+  const size_t need = b2a_decode_paged_workspace_bytes(B, Hq, Hkv, D);
+  if (!workspace || workspace_bytes < need || !api_aligned(workspace, 16)) return B2A_ERR_WORKSPACE;
+
+  int* err = nullptr;
+  int rc = b2a::api_prologue(&err);
+  if (rc) return rc;
+  b2a::DecodePagedParams p{};
+  // Keys per TMA box: a box never crosses a page, a warp's 16 keys never a box.
+  p.box_rows = page % 64 == 0 ? 64 : (page % 32 == 0 ? 32 : 16);
+  CUtensorMap tk, tv;
+  const auto map = k_scales ? pool_map_e4m3 : pool_map;
+  if ((rc = map(&tk, k_pages, D, n_pages, Hkv, page, ks, p.box_rows)) ||
+      (rc = map(&tv, v_pages, D, n_pages, Hkv, page, vs, p.box_rows)))
+    return rc;
+  p.k_scales = k_scales;
+  p.v_scales = v_scales;
+  if (k_scales) {
+    std::copy_n(kss, 2, p.kss);
+    std::copy_n(vss, 2, p.vss);
+  }
+  p.q = static_cast<const __nv_bfloat16*>(q);
+  p.q_sb = qs[0];
+  p.q_sh = qs[1];
+  p.block_table = block_table;
+  p.table_ld = table_ld;
+  p.table_width = table_width;
+  p.n_pages = n_pages;
+  p.page = page;
+  p.seqlens = seqlens;
+  p.o = o;
+  p.o_sb = os[0];
+  p.o_sh = os[1];
+  p.out_fp32 = out_fp32 ? 1 : 0;
+  p.gate = gate;
+  if (gate) {
+    p.g_sb = gs[0];
+    p.g_sh = gs[1];
+    p.gate_bf16 = gate_bf16 ? 1 : 0;
+  }
+  auto by4 = [](const void* ptr, const long long* st, unsigned size) {
+    return api_aligned(ptr, 4 * size) && st[0] % 4 == 0 && st[1] % 4 == 0;
+  };
+  p.vec4 = by4(o, os, out_fp32 ? 4 : 2) && (!gate || by4(gate, gs, gate_bf16 ? 2 : 4));
+  p.B = B;
+  p.Hq = Hq;
+  p.Hkv = Hkv;
+  p.group = Hq / Hkv;
+  p.scale_log2 = scale * b2a::kApiLog2e;
+  p.err = err;
+  p.n_ctas = b2a::decode_paged_max_ctas(D, b2a::api_sm_count());
+  const size_t rows = b2a::decode_paged_parts(B, Hkv, p.n_ctas) * p.group;
+  char* scratch = static_cast<char*>(workspace);
+  p.part_o = reinterpret_cast<float*>(scratch);
+  scratch += b2a::api_align256(rows * D * sizeof(float));
+  p.part_ml = reinterpret_cast<float*>(scratch);
+  p.place = reinterpret_cast<int*>(scratch + b2a::api_align256(rows * 2 * sizeof(float)));
+  return status_of(b2a::launch_decode_paged(D, tk, tv, p, static_cast<cudaStream_t>(stream)));
+}
+
+int append_paged(const void* q, const void* k, const void* v, const long long* qs, const long long* ks,
+                 const long long* vs, int src_bf16, const void* q_norm, const void* k_norm, float eps,
+                 const void* cos_tab, const void* sin_tab, int tab_fp32, int max_pos, int rope_dim,
+                 void* q_out, void* k_out, void* v_out, void* k_pages, void* v_pages, const long long* kps,
+                 const long long* vps, float* k_scales, float* v_scales, const long long* kss,
+                 const long long* vss, const int* block_table, long long table_ld, int table_width,
+                 int n_pages, int page, const int* cu_seqlens, int B, int N, int Hq, int Hkv, int D,
+                 int start_pos, const int* start_pos_per_batch, int* seqlens_out, void* stream) {
+  if (!q || !k || !v || !qs || !ks || !vs || !q_out || !k_pages || !v_pages || !kps || !vps || !block_table ||
+      !cu_seqlens)
+    return B2A_ERR_INVALID_ARG;
+  if (B <= 0 || N <= 0 || Hq <= 0 || Hkv <= 0 || n_pages <= 0 || page <= 0 || table_width <= 0 ||
+      table_ld < table_width || (!start_pos_per_batch && start_pos < 0))
+    return B2A_ERR_INVALID_ARG;
+  // The positions are read while the lengths are written.
+  if (start_pos_per_batch && seqlens_out && start_pos_per_batch < seqlens_out + B &&
+      seqlens_out < start_pos_per_batch + B)
+    return B2A_ERR_INVALID_ARG;
+  if (!head_dim_ok(D)) return B2A_ERR_HEAD_DIM;
+  if (rope_dim != 0 && (rope_dim < 16 || rope_dim > D || (rope_dim & (rope_dim - 1)))) return B2A_ERR_INVALID_ARG;
+  if (rope_dim && (!cos_tab || !sin_tab || max_pos <= 0)) return B2A_ERR_INVALID_ARG;
+  if ((q_norm || k_norm) && !(eps >= 0.f && std::isfinite(eps))) return B2A_ERR_INVALID_ARG;
+  if (!src_bf16 && !tab_fp32) tab_fp32 = 1;
+  for (const void* ptr : {q, k, v, cos_tab, sin_tab, q_norm, k_norm, (const void*)q_out, (const void*)k_out,
+                          (const void*)v_out, (const void*)k_pages, (const void*)v_pages})
+    if (!api_aligned(ptr, 16)) return B2A_ERR_ALIGNMENT;
+  const long long mult = src_bf16 ? 8 : 4, pool_mult = k_scales ? 16 : 8;
+  if (!api_strides_ok(qs, 2, mult) || !api_strides_ok(ks, 2, mult) || !api_strides_ok(vs, 2, mult) ||
+      !api_strides_ok(kps, 3, pool_mult) || !api_strides_ok(vps, 3, pool_mult) || !api_aligned(block_table, 4) ||
+      !api_aligned(cu_seqlens, 4) || !api_aligned(start_pos_per_batch, 4) || !api_aligned(seqlens_out, 4))
+    return B2A_ERR_ALIGNMENT;
+
+  int* err = nullptr;
+  const int rc = b2a::api_prologue(&err);
+  if (rc) return rc;
+  b2a::RopeAppendPagedParams p{};
+  p.q = q;
+  p.k = k;
+  p.v = v;
+  std::copy_n(qs, 2, p.qs);
+  std::copy_n(ks, 2, p.ks);
+  std::copy_n(vs, 2, p.vs);
+  p.cos = cos_tab;
+  p.sin = sin_tab;
+  p.tab_fp32 = tab_fp32;
+  p.max_pos = max_pos;
+  p.rope_dim = rope_dim;
+  p.q_norm = q_norm;
+  p.k_norm = k_norm;
+  p.norm_eps = eps;
+  p.q_out = static_cast<__nv_bfloat16*>(q_out);
+  p.k_out = static_cast<__nv_bfloat16*>(k_out);
+  p.v_out = static_cast<__nv_bfloat16*>(v_out);
+  p.k_pages = k_pages;
+  p.v_pages = v_pages;
+  std::copy_n(kps, 3, p.kps);
+  std::copy_n(vps, 3, p.vps);
+  p.k_scales = k_scales;
+  p.v_scales = v_scales;
+  if (k_scales) {
+    std::copy_n(kss, 2, p.kss);
+    std::copy_n(vss, 2, p.vss);
+  }
+  p.block_table = block_table;
+  p.table_ld = table_ld;
+  p.table_width = table_width;
+  p.n_pages = n_pages;
+  p.page = page;
+  p.cu_seqlens = cu_seqlens;
+  p.start_pos_arr = start_pos_per_batch;
+  p.start_pos = start_pos;
+  p.seqlens_out = seqlens_out;
+  p.B = B;
+  p.Hq = Hq;
+  p.Hkv = Hkv;
+  p.N = N;
+  p.src_bf16 = src_bf16 ? 1 : 0;
+  p.err = err;
+  return status_of(b2a::launch_rope_append_paged(D, p, static_cast<cudaStream_t>(stream)));
+}
 
 }  // namespace
 
@@ -125,69 +310,21 @@ int b2a_decode_paged(const void* q, const void* k_pages, const void* v_pages, co
                      int Hq, int Hkv, int n_pages, int page, int D, const long long* qs, const long long* ks,
                      const long long* vs, const long long* gs, const long long* os, int gate_bf16, float scale,
                      int out_fp32, void* workspace, size_t workspace_bytes, void* stream) {
-  if (!q || !k_pages || !v_pages || !block_table || !seqlens || !o || !qs || !ks || !vs || !os || (gate && !gs))
-    return B2A_ERR_INVALID_ARG;
-  if (B <= 0 || Hq <= 0 || Hkv <= 0 || n_pages <= 0 || page <= 0 || page % 16 || table_width <= 0 ||
-      table_ld < table_width || (long long)table_width * page > INT_MAX - 64)
-    return B2A_ERR_INVALID_ARG;
-  if (!(scale > 0.f) || !std::isfinite(scale)) return B2A_ERR_INVALID_ARG;
-  if (!head_dim_ok(D)) return B2A_ERR_HEAD_DIM;
-  if (Hq % Hkv || Hq / Hkv > 16) return B2A_ERR_GQA;
-  if (!api_aligned(q, 16) || !api_aligned(k_pages, 16) || !api_aligned(v_pages, 16) ||
-      !api_aligned(o, out_fp32 ? 4 : 2) || !api_aligned(block_table, 4) || !api_aligned(seqlens, 4) ||
-      !api_aligned(gate, gate_bf16 ? 2 : 4))
-    return B2A_ERR_ALIGNMENT;
-  if (!api_strides_ok(qs, 2, 8) || !api_strides_ok(ks, 3, 8) || !api_strides_ok(vs, 3, 8)) return B2A_ERR_ALIGNMENT;
-  const size_t need = b2a_decode_paged_workspace_bytes(B, Hq, Hkv, D);
-  if (!workspace || workspace_bytes < need || !api_aligned(workspace, 16)) return B2A_ERR_WORKSPACE;
+  return paged_attention(q, k_pages, v_pages, block_table, nullptr, nullptr, nullptr, nullptr, table_ld, table_width,
+                         seqlens, gate, o, B, Hq, Hkv, n_pages, page, D, qs, ks, vs, gs, os, gate_bf16, scale, out_fp32,
+                         workspace, workspace_bytes, stream);
+}
 
-  int* err = nullptr;
-  int rc = b2a::api_prologue(&err);
-  if (rc) return rc;
-  b2a::DecodePagedParams p{};
-  // Keys per TMA box: a box never crosses a page, a warp's 16 keys never a box.
-  p.box_rows = page % 64 == 0 ? 64 : (page % 32 == 0 ? 32 : 16);
-  CUtensorMap tk, tv;
-  if ((rc = pool_map(&tk, k_pages, D, n_pages, Hkv, page, ks, p.box_rows)) ||
-      (rc = pool_map(&tv, v_pages, D, n_pages, Hkv, page, vs, p.box_rows)))
-    return rc;
-  p.q = static_cast<const __nv_bfloat16*>(q);
-  p.q_sb = qs[0];
-  p.q_sh = qs[1];
-  p.block_table = block_table;
-  p.table_ld = table_ld;
-  p.table_width = table_width;
-  p.n_pages = n_pages;
-  p.page = page;
-  p.seqlens = seqlens;
-  p.o = o;
-  p.o_sb = os[0];
-  p.o_sh = os[1];
-  p.out_fp32 = out_fp32 ? 1 : 0;
-  p.gate = gate;
-  if (gate) {
-    p.g_sb = gs[0];
-    p.g_sh = gs[1];
-    p.gate_bf16 = gate_bf16 ? 1 : 0;
-  }
-  auto by4 = [](const void* ptr, const long long* st, unsigned size) {
-    return api_aligned(ptr, 4 * size) && st[0] % 4 == 0 && st[1] % 4 == 0;
-  };
-  p.vec4 = by4(o, os, out_fp32 ? 4 : 2) && (!gate || by4(gate, gs, gate_bf16 ? 2 : 4));
-  p.B = B;
-  p.Hq = Hq;
-  p.Hkv = Hkv;
-  p.group = Hq / Hkv;
-  p.scale_log2 = scale * b2a::kApiLog2e;
-  p.err = err;
-  p.n_ctas = b2a::decode_paged_max_ctas(D, b2a::api_sm_count());
-  const size_t rows = b2a::decode_paged_parts(B, Hkv, p.n_ctas) * p.group;
-  char* scratch = static_cast<char*>(workspace);
-  p.part_o = reinterpret_cast<float*>(scratch);
-  scratch += b2a::api_align256(rows * D * sizeof(float));
-  p.part_ml = reinterpret_cast<float*>(scratch);
-  p.place = reinterpret_cast<int*>(scratch + b2a::api_align256(rows * 2 * sizeof(float)));
-  return status_of(b2a::launch_decode_paged(D, tk, tv, p, static_cast<cudaStream_t>(stream)));
+int b2a_decode_paged_e4m3(const void* q, const void* k_pages, const void* v_pages, const float* k_scales,
+                          const float* v_scales, const long long* kss, const long long* vss, const int* block_table,
+                          long long table_ld, int table_width, const int* seqlens, const void* gate, void* o, int B,
+                          int Hq, int Hkv, int n_pages, int page, int D, const long long* qs, const long long* ks,
+                          const long long* vs, const long long* gs, const long long* os, int gate_bf16, float scale,
+                          int out_fp32, void* workspace, size_t workspace_bytes, void* stream) {
+  if (const int rc = scales_ok(k_scales, v_scales, kss, vss)) return rc;
+  return paged_attention(q, k_pages, v_pages, block_table, k_scales, v_scales, kss, vss, table_ld, table_width, seqlens,
+                         gate, o, B, Hq, Hkv, n_pages, page, D, qs, ks, vs, gs, os, gate_bf16, scale, out_fp32,
+                         workspace, workspace_bytes, stream);
 }
 
 int b2a_rope_append_paged(const void* q, const void* k, const void* v, const long long* qs, const long long* ks,
@@ -197,55 +334,62 @@ int b2a_rope_append_paged(const void* q, const void* k, const void* v, const lon
                           const long long* vps, const int* block_table, long long table_ld, int table_width,
                           int n_pages, int page, const int* cu_seqlens, int B, int N, int Hq, int Hkv, int D,
                           int start_pos, const int* start_pos_per_batch, int* seqlens_out, void* stream) {
-  if (!q || !k || !v || !qs || !ks || !vs || !q_out || !k_pages || !v_pages || !kps || !vps || !block_table ||
-      !cu_seqlens)
+  return append_paged(q, k, v, qs, ks, vs, src_bf16, q_norm, k_norm, eps, cos_tab, sin_tab, tab_fp32, max_pos, rope_dim,
+                      q_out, k_out, v_out, k_pages, v_pages, kps, vps, nullptr, nullptr, nullptr, nullptr, block_table,
+                      table_ld, table_width, n_pages, page, cu_seqlens, B, N, Hq, Hkv, D, start_pos,
+                      start_pos_per_batch, seqlens_out, stream);
+}
+
+int b2a_rope_append_paged_e4m3(const void* q, const void* k, const void* v, const long long* qs, const long long* ks,
+                               const long long* vs, int src_bf16, const void* q_norm, const void* k_norm, float eps,
+                               const void* cos_tab, const void* sin_tab, int tab_fp32, int max_pos, int rope_dim,
+                               void* q_out, void* k_out, void* v_out, void* k_pages, void* v_pages,
+                               const long long* kps, const long long* vps, float* k_scales, float* v_scales,
+                               const long long* kss, const long long* vss, const int* block_table, long long table_ld,
+                               int table_width, int n_pages, int page, const int* cu_seqlens, int B, int N, int Hq,
+                               int Hkv, int D, int start_pos, const int* start_pos_per_batch, int* seqlens_out,
+                               void* stream) {
+  if (const int rc = scales_ok(k_scales, v_scales, kss, vss)) return rc;
+  return append_paged(q, k, v, qs, ks, vs, src_bf16, q_norm, k_norm, eps, cos_tab, sin_tab, tab_fp32, max_pos, rope_dim,
+                      q_out, k_out, v_out, k_pages, v_pages, kps, vps, k_scales, v_scales, kss, vss, block_table,
+                      table_ld, table_width, n_pages, page, cu_seqlens, B, N, Hq, Hkv, D, start_pos,
+                      start_pos_per_batch, seqlens_out, stream);
+}
+
+int b2a_gather_paged(const void* k_pages, const void* v_pages, const long long* kps, const long long* vps,
+                     const float* k_scales, const float* v_scales, const long long* kss, const long long* vss,
+                     const int* block_table, long long table_ld, int table_width, int n_pages, int page,
+                     const int* cu_seqlens, int B, int N, int Hkv, int D, int start_pos,
+                     const int* start_pos_per_batch, void* k_out, void* v_out, void* stream) {
+  if (!k_pages || !v_pages || !kps || !vps || !block_table || !cu_seqlens || !k_out || !v_out)
     return B2A_ERR_INVALID_ARG;
-  if (B <= 0 || N <= 0 || Hq <= 0 || Hkv <= 0 || n_pages <= 0 || page <= 0 || table_width <= 0 ||
-      table_ld < table_width || (!start_pos_per_batch && start_pos < 0))
-    return B2A_ERR_INVALID_ARG;
-  // The positions are read while the lengths are written.
-  if (start_pos_per_batch && seqlens_out && start_pos_per_batch < seqlens_out + B &&
-      seqlens_out < start_pos_per_batch + B)
+  if (!k_scales != !v_scales) return B2A_ERR_INVALID_ARG;
+  if (B <= 0 || N <= 0 || Hkv <= 0 || n_pages <= 0 || page <= 0 || table_width <= 0 || table_ld < table_width ||
+      (!start_pos_per_batch && start_pos < 0))
     return B2A_ERR_INVALID_ARG;
   if (!head_dim_ok(D)) return B2A_ERR_HEAD_DIM;
-  if (rope_dim != 0 && (rope_dim < 16 || rope_dim > D || (rope_dim & (rope_dim - 1)))) return B2A_ERR_INVALID_ARG;
-  if (rope_dim && (!cos_tab || !sin_tab || max_pos <= 0)) return B2A_ERR_INVALID_ARG;
-  if ((q_norm || k_norm) && !(eps >= 0.f && std::isfinite(eps))) return B2A_ERR_INVALID_ARG;
-  if (!src_bf16 && !tab_fp32) tab_fp32 = 1;
-  for (const void* ptr : {q, k, v, cos_tab, sin_tab, q_norm, k_norm, (const void*)q_out, (const void*)k_out,
-                          (const void*)v_out, (const void*)k_pages, (const void*)v_pages})
+  if (k_scales)
+    if (const int rc = scales_ok(k_scales, v_scales, kss, vss)) return rc;
+  for (const void* ptr : {k_pages, v_pages, (const void*)k_out, (const void*)v_out})
     if (!api_aligned(ptr, 16)) return B2A_ERR_ALIGNMENT;
-  const long long mult = src_bf16 ? 8 : 4;
-  if (!api_strides_ok(qs, 2, mult) || !api_strides_ok(ks, 2, mult) || !api_strides_ok(vs, 2, mult) ||
-      !api_strides_ok(kps, 3, 8) || !api_strides_ok(vps, 3, 8) || !api_aligned(block_table, 4) ||
-      !api_aligned(cu_seqlens, 4) || !api_aligned(start_pos_per_batch, 4) || !api_aligned(seqlens_out, 4))
+  const long long mult = k_scales ? 16 : 8;
+  if (!api_strides_ok(kps, 3, mult) || !api_strides_ok(vps, 3, mult) || !api_aligned(block_table, 4) ||
+      !api_aligned(cu_seqlens, 4) || !api_aligned(start_pos_per_batch, 4))
     return B2A_ERR_ALIGNMENT;
-
   int* err = nullptr;
   const int rc = b2a::api_prologue(&err);
   if (rc) return rc;
-  b2a::RopeAppendPagedParams p{};
-  p.q = q;
-  p.k = k;
-  p.v = v;
-  std::copy_n(qs, 2, p.qs);
-  std::copy_n(ks, 2, p.ks);
-  std::copy_n(vs, 2, p.vs);
-  p.cos = cos_tab;
-  p.sin = sin_tab;
-  p.tab_fp32 = tab_fp32;
-  p.max_pos = max_pos;
-  p.rope_dim = rope_dim;
-  p.q_norm = q_norm;
-  p.k_norm = k_norm;
-  p.norm_eps = eps;
-  p.q_out = static_cast<__nv_bfloat16*>(q_out);
-  p.k_out = static_cast<__nv_bfloat16*>(k_out);
-  p.v_out = static_cast<__nv_bfloat16*>(v_out);
-  p.k_pages = static_cast<__nv_bfloat16*>(k_pages);
-  p.v_pages = static_cast<__nv_bfloat16*>(v_pages);
+  b2a::GatherPagedParams p{};
+  p.k_pages = k_pages;
+  p.v_pages = v_pages;
   std::copy_n(kps, 3, p.kps);
   std::copy_n(vps, 3, p.vps);
+  p.k_scales = k_scales;
+  p.v_scales = v_scales;
+  if (k_scales) {
+    std::copy_n(kss, 2, p.kss);
+    std::copy_n(vss, 2, p.vss);
+  }
   p.block_table = block_table;
   p.table_ld = table_ld;
   p.table_width = table_width;
@@ -254,14 +398,68 @@ int b2a_rope_append_paged(const void* q, const void* k, const void* v, const lon
   p.cu_seqlens = cu_seqlens;
   p.start_pos_arr = start_pos_per_batch;
   p.start_pos = start_pos;
-  p.seqlens_out = seqlens_out;
+  p.k_out = static_cast<__nv_bfloat16*>(k_out);
+  p.v_out = static_cast<__nv_bfloat16*>(v_out);
   p.B = B;
-  p.Hq = Hq;
   p.Hkv = Hkv;
   p.N = N;
-  p.src_bf16 = src_bf16 ? 1 : 0;
   p.err = err;
-  return status_of(b2a::launch_rope_append_paged(D, p, static_cast<cudaStream_t>(stream)));
+  return status_of(b2a::launch_gather_paged(D, p, static_cast<cudaStream_t>(stream)));
+}
+
+int b2a_penalize(const void* logits, long long ld_logits, int logits_bf16, const void* tokens, int tokens_64,
+                 long long tokens_row, long long tokens_step, int L, const int* lengths, const int* prompt_lengths,
+                 const float* repetition, float repetition_all, const float* frequency, float frequency_all,
+                 const float* presence, float presence_all, const float* bias, long long ld_bias, const int* allowed,
+                 long long ld_allowed, void* out, long long ld_out, int R, int V, void* stream) {
+  if (!logits || !out || R <= 0 || V <= 0 || V > (1 << 30) || L < 0 || L > (1 << 30) || (L > 0 && !tokens))
+    return B2A_ERR_INVALID_ARG;
+  if (ld_logits < 0 || ld_out < (R > 1 ? V : 0) || tokens_row < 0 || tokens_step < 0 || ld_bias < 0 || ld_allowed < 0)
+    return B2A_ERR_INVALID_ARG;
+  if ((!repetition && !(repetition_all > 0.f && std::isfinite(repetition_all))) ||
+      (!frequency && !std::isfinite(frequency_all)) || (!presence && !std::isfinite(presence_all)))
+    return B2A_ERR_INVALID_ARG;
+  const unsigned size = logits_bf16 ? 2 : 4;
+  if (!api_aligned(logits, size) || !api_aligned(out, size) || !api_aligned(tokens, tokens_64 ? 8 : 4))
+    return B2A_ERR_ALIGNMENT;
+  for (const void* ptr : {(const void*)lengths, (const void*)prompt_lengths, (const void*)repetition,
+                          (const void*)frequency, (const void*)presence, (const void*)bias, (const void*)allowed})
+    if (!api_aligned(ptr, 4)) return B2A_ERR_ALIGNMENT;
+  // In place, row by row, or apart: chunks of a row run in any order.
+  const uintptr_t x0 = reinterpret_cast<uintptr_t>(logits), y0 = reinterpret_cast<uintptr_t>(out);
+  const uintptr_t x1 = x0 + ((unsigned long long)(R - 1) * ld_logits + V) * size;
+  const uintptr_t y1 = y0 + ((unsigned long long)(R - 1) * ld_out + V) * size;
+  if (x0 < y1 && y0 < x1 && !(x0 == y0 && (ld_logits == ld_out || R == 1))) return B2A_ERR_INVALID_ARG;
+  int* err = nullptr;
+  const int rc = b2a::api_prologue(&err);
+  if (rc) return rc;
+  b2a::PenalizeParams p{};
+  p.logits = logits;
+  p.ld_logits = ld_logits;
+  p.logits_bf16 = logits_bf16 ? 1 : 0;
+  p.out = out;
+  p.ld_out = ld_out;
+  p.tokens = L > 0 ? tokens : nullptr;
+  p.tokens_row = tokens_row;
+  p.tokens_step = tokens_step;
+  p.tokens_64 = tokens_64 ? 1 : 0;
+  p.L = L;
+  p.lengths = lengths;
+  p.prompt_lengths = prompt_lengths;
+  p.repetition = repetition;
+  p.frequency = frequency;
+  p.presence = presence;
+  p.repetition_all = repetition_all;
+  p.frequency_all = frequency_all;
+  p.presence_all = presence_all;
+  p.bias = bias;
+  p.ld_bias = ld_bias;
+  p.allowed = reinterpret_cast<const unsigned*>(allowed);
+  p.ld_allowed = ld_allowed;
+  p.R = R;
+  p.V = V;
+  p.err = err;
+  return status_of(b2a::launch_penalize(p, static_cast<cudaStream_t>(stream)));
 }
 
 int b2a_sample(const void* logits, long long ld_logits, int logits_bf16, const float* noise, long long ld_noise, int R,

@@ -43,25 +43,29 @@ namespace b2a {
 
 namespace {
 
-template <int D>
+template <int D, bool E4M3>
 struct PagedCfg {
   static constexpr int TK = 64;  // keys per tile
-  static constexpr int TILE_BYTES = TK * D * 2;  // K or V tile
+  static constexpr int TILE_BYTES = TK * D * (E4M3 ? 1 : 2);  // K or V tile
   static constexpr int STAGE_BYTES = 2 * TILE_BYTES;
-  static constexpr int STAGES = D == 64 ? 6 : 3;
+  static constexpr int STAGES = (D == 64 ? 6 : 3) * (E4M3 ? 2 : 1);
   static constexpr int CTAS_PER_SM = D == 256 ? 1 : 2;
   static constexpr int Q_ROW = D * 2 + 16;  // bytes; the 16 keep ldmatrix rows apart
   static constexpr int OFF_Q = STAGES * STAGE_BYTES;
-  static constexpr int OFF_BAR = OFF_Q + 2 * 16 * Q_ROW;  // two pairs' query heads
+  static constexpr int OFF_SCALES = OFF_Q + 2 * 16 * Q_ROW;  // two pairs' query heads; [STAGES][K, V][TK] fp32
+  static constexpr int OFF_BAR = OFF_SCALES + (E4M3 ? STAGES * 2 * TK * 4 : 0);
   static constexpr int SMEM_BYTES = OFF_BAR + 1024 + 1024;  // barriers and m, l; alignment slack
   static constexpr int THREADS = 160;  // 4 compute warps + 1 producer warp
-  static_assert(4 * 16 * D * 4 <= STAGE_BYTES, "the four warps' outputs are merged in one stage");
+  // The four warps' outputs are merged in one stage, this many heads at a time.
+  static constexpr int MERGE = E4M3 ? 8 : 16;
+  static_assert(4 * MERGE * D * 4 <= STAGE_BYTES, "the four warps' outputs are merged in one stage");
+  static_assert(STAGES <= 12, "PagedBars");
   static_assert((SMEM_BYTES + 1024) * CTAS_PER_SM <= 233472, "shared memory budget");
 };
 
 struct PagedBars {
-  uint64_t full[8];
-  uint64_t empty[8];
+  uint64_t full[12];
+  uint64_t empty[12];
   uint64_t q_full[2];
   uint64_t q_empty[2];
   int abort_flag;
@@ -260,14 +264,33 @@ struct Walk {
   }
 };
 
+// Two of a word's four e4m3 bytes (the even or the odd ones) as bf16, exactly:
+// moved to bf16's exponent and mantissa bits a value is 2^-120 of itself, the
+// smallest (subnormal) ones too. One shift, two logic operations and the
+// product; the conversion instruction gives f16, which P is too wide for. e4m3's
+// NaN, which the append stores under a NaN scale only, gives 480: a V of finite
+// numbers whatever its bytes are, which a P of 0 hides.
+__device__ __forceinline__ uint32_t from_2_to_minus_120(uint32_t x) {
+  uint32_t r;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(0x7b807b80u));
+  return r;
+}
+__device__ __forceinline__ uint32_t even_e4m3(uint32_t w) {
+  return from_2_to_minus_120(((w << 4) & 0x07f007f0u) | ((w << 8) & 0x80008000u));
+}
+__device__ __forceinline__ uint32_t odd_e4m3(uint32_t w) {
+  return from_2_to_minus_120(((w >> 4) & 0x07f007f0u) | (w & 0x80008000u));
+}
+
 __device__ __forceinline__ int swizzle(int r, int d) { return d ^ (((r >> 1) & 3) << 3); }
 
-// NT blocks of 8 query heads cover a group; SPLIT: the even split above.
-template <int D, int NT, bool SPLIT>
-__global__ void __launch_bounds__(PagedCfg<D>::THREADS, PagedCfg<D>::CTAS_PER_SM)
+// NT blocks of 8 query heads cover a group; SPLIT: the even split above; E4M3:
+// 8-bit pools with a scale per key.
+template <int D, int NT, bool SPLIT, bool E4M3>
+__global__ void __launch_bounds__(PagedCfg<D, E4M3>::THREADS, PagedCfg<D, E4M3>::CTAS_PER_SM)
     decode_paged_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                         const __grid_constant__ DecodePagedParams p) {
-  using C = PagedCfg<D>;
+  using C = PagedCfg<D, E4M3>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const uint32_t pad = (1024u - (smem_u32(smem_raw) & 1023u)) & 1023u;
   uint8_t* smem = smem_raw + pad;
@@ -327,7 +350,7 @@ __global__ void __launch_bounds__(PagedCfg<D>::THREADS, PagedCfg<D>::CTAS_PER_SM
     const int box = lane % boxes;
     const bool is_v = lane >= boxes;
     const bool mine = lane < 2 * boxes;
-    const int box_bytes = br * D * 2;
+    const int box_bytes = br * D * (E4M3 ? 1 : 2);
     // Every tile's page is looked up one tile ahead, across pairs too, and
     // checked when its turn comes (so that nothing waits for the lookup).
     auto has_keys = [&]() { return mine && w.t0 * C::TK + box * br < w.len; };
@@ -368,12 +391,19 @@ __global__ void __launch_bounds__(PagedCfg<D>::THREADS, PagedCfg<D>::CTAS_PER_SM
         break;
       uint8_t* dst = smem + slot * C::STAGE_BYTES + (is_v ? C::TILE_BYTES : 0) + box * box_bytes;
       const unsigned copies = __ballot_sync(0xffffffffu, now);
-      if (lane == 0) mbar_arrive_expect_tx(&bars->full[slot], __popc(copies) * box_bytes);
+      if (lane == 0) mbar_arrive_expect_tx(&bars->full[slot], __popc(copies) * (box_bytes + (E4M3 ? 4 * br : 0)));
       __syncwarp();
       if (now) {
         const bool in_pool = id >= 0 && id < p.n_pages;
         if (!in_pool && p.err) atomicOr(p.err, kErrBadArgs);
         tma_load_5d(dst, is_v ? &tm_v : &tm_k, &bars->full[slot], 0, row, 0, g, in_pool ? id : 0);
+        if constexpr (E4M3) {
+          const long long page = in_pool ? id : 0;
+          const float* scales = is_v ? p.v_scales + page * p.vss[0] + g * p.vss[1] + row
+                                     : p.k_scales + page * p.kss[0] + g * p.kss[1] + row;
+          bulk_load(smem + C::OFF_SCALES + ((slot * 2 + is_v) * C::TK + box * br) * 4, scales, 4 * br,
+                    &bars->full[slot]);
+        }
       }
       ++n;
     }
@@ -390,11 +420,14 @@ __global__ void __launch_bounds__(PagedCfg<D>::THREADS, PagedCfg<D>::CTAS_PER_SM
     const int mi = lane >> 3, mr = lane & 7;  // ldmatrix: matrix index / row in it
     // This warp's 16 keys of a tile lie in one box: its first row there, and
     // the distance of the box's 64-column chunks.
-    const uint32_t wbase = (16 * warp / br) * (br * D * 2) + (16 * warp % br) * 128;
+    constexpr int kLine = E4M3 && D == 64 ? 64 : 128;  // bytes of a row in a chunk
+    const uint32_t wbase = (16 * warp / br) * (br * D * (E4M3 ? 1 : 2)) + (16 * warp % br) * kLine;
     const uint32_t chunk = br * 128;
     // 16-byte unit U of row r (0..15): the swizzle XORs the unit with the
-    // row's place in its group of 8.
+    // row's place in its group of 8 (rows of 64 bytes: of two rows' place in
+    // their group of 4).
     auto at = [&](uint32_t base, int r, int U) -> uint32_t {
+      if constexpr (kLine == 64) return base + r * 64 + ((U ^ ((r >> 1) & 3)) << 4);
       return base + (U >> 3) * chunk + r * 128 + (((U & 7) ^ (r & 7)) << 4);
     };
     // A wait that ran out leaves garbage in the result and the error word set;
@@ -409,14 +442,26 @@ __global__ void __launch_bounds__(PagedCfg<D>::THREADS, PagedCfg<D>::CTAS_PER_SM
           0xffffffffu, mbar_wait(&bars->q_full[pair & 1], (uint32_t)(pair >> 1) & 1u, abort_flag, p.err));
 #pragma unroll
       for (int x = 0; x < NT; ++x) {
-        const uint32_t q = smem_u32(smem + C::OFF_Q) + ((pair & 1) * 16 + 8 * x + mr) * C::Q_ROW + mi * 16;
+        if constexpr (E4M3) {
+          // The order in which a word of K gives its four columns: 0 and 2, then 1 and 3.
+          const uint8_t* q = smem + C::OFF_Q + ((pair & 1) * 16 + 8 * x + gr) * C::Q_ROW + tq * 8;
 #pragma unroll
-        for (int k = 0; k < D / 32; ++k)
-          ldsm4(q + 64 * k, qb[x][2 * k][0], qb[x][2 * k][1], qb[x][2 * k + 1][0], qb[x][2 * k + 1][1]);
+          for (int k = 0; k < D / 16; ++k) {
+            const uint2 w = *reinterpret_cast<const uint2*>(q + 32 * k);
+            qb[x][k][0] = __byte_perm(w.x, w.y, 0x5410);
+            qb[x][k][1] = __byte_perm(w.x, w.y, 0x7632);
+          }
+        } else {
+          const uint32_t q = smem_u32(smem + C::OFF_Q) + ((pair & 1) * 16 + 8 * x + mr) * C::Q_ROW + mi * 16;
+#pragma unroll
+          for (int k = 0; k < D / 32; ++k)
+            ldsm4(q + 64 * k, qb[x][2 * k][0], qb[x][2 * k][1], qb[x][2 * k + 1][0], qb[x][2 * k + 1][1]);
+        }
       }
       __syncwarp();
       if (lane == 0 && got) mbar_arrive(&bars->q_empty[pair & 1]);
-      // O^T: rows 16 d + gr (+ 8), columns (heads) 8 x + 2 tq (+ 1); this
+      // O^T: rows 16 d + gr (+ 8) (E4M3: 16 d + 2 gr (+ 1), the columns of V's
+      // even and odd bytes), columns (heads) 8 x + 2 tq (+ 1); this
       // thread keeps the running maximum and its part of the sum of those heads.
       float acc[NT][D / 16][4];
       float m[NT][2], l[NT][2];
@@ -441,12 +486,37 @@ __global__ void __launch_bounds__(PagedCfg<D>::THREADS, PagedCfg<D>::CTAS_PER_SM
           float s[NT][4];
 #pragma unroll
           for (int x = 0; x < NT; ++x) s[x][0] = s[x][1] = s[x][2] = s[x][3] = 0.f;
+          float sv[2];  // E4M3: the scales of V's rows gr, gr + 8
+          if constexpr (E4M3) {
+            const float* scales = reinterpret_cast<const float*>(smem + C::OFF_SCALES) + slot * 2 * C::TK + 16 * warp;
 #pragma unroll
-          for (int k = 0; k < D / 16; ++k) {
-            uint32_t a[4];
-            ldsm4(at(kbase, 8 * (mi & 1) + mr, 2 * k + (mi >> 1)), a[0], a[1], a[2], a[3]);
+            for (int k = 0; k < D / 32; ++k) {
+              uint32_t w[4];
+              ldsm4(at(kbase, 8 * (mi & 1) + mr, 2 * k + (mi >> 1)), w[0], w[1], w[2], w[3]);
 #pragma unroll
-            for (int x = 0; x < NT; ++x) mma16816(s[x], a, qb[x][k][0], qb[x][k][1]);
+              for (int u = 0; u < 2; ++u) {
+                const uint32_t a[4] = {even_e4m3(w[2 * u]), even_e4m3(w[2 * u + 1]), odd_e4m3(w[2 * u]),
+                                       odd_e4m3(w[2 * u + 1])};
+#pragma unroll
+                for (int x = 0; x < NT; ++x) mma16816(s[x], a, qb[x][2 * k + u][0], qb[x][2 * k + u][1]);
+              }
+            }
+            const float sk[2] = {scales[gr], scales[gr + 8]};
+#pragma unroll
+            for (int x = 0; x < NT; ++x) {
+              s[x][0] *= sk[0], s[x][1] *= sk[0];
+              s[x][2] *= sk[1], s[x][3] *= sk[1];
+            }
+            sv[0] = gr < have ? scales[C::TK + gr] : 0.f;
+            sv[1] = gr + 8 < have ? scales[C::TK + gr + 8] : 0.f;
+          } else {
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k) {
+              uint32_t a[4];
+              ldsm4(at(kbase, 8 * (mi & 1) + mr, 2 * k + (mi >> 1)), a[0], a[1], a[2], a[3]);
+#pragma unroll
+              for (int x = 0; x < NT; ++x) mma16816(s[x], a, qb[x][k][0], qb[x][k][1]);
+            }
           }
           if (have < 16) {
 #pragma unroll
@@ -454,11 +524,13 @@ __global__ void __launch_bounds__(PagedCfg<D>::THREADS, PagedCfg<D>::CTAS_PER_SM
               if (gr >= have) s[x][0] = s[x][1] = -INFINITY;
               if (gr + 8 >= have) s[x][2] = s[x][3] = -INFINITY;
             }
-            // V rows without a key: 0 x anything would not do (NaN).
-            for (int u = lane; u < (16 - have) * (D / 8); u += 32)
-              st_shared_v4(at(vbase, have + u / (D / 8), u % (D / 8)), 0u, 0u, 0u, 0u);
-            fence_proxy_async_smem();  // before the slot's next copy
-            __syncwarp();
+            if constexpr (!E4M3) {
+              // V rows without a key: 0 x anything would not do (NaN).
+              for (int u = lane; u < (16 - have) * (D / 8); u += 32)
+                st_shared_v4(at(vbase, have + u / (D / 8), u % (D / 8)), 0u, 0u, 0u, 0u);
+              fence_proxy_async_smem();  // before the slot's next copy
+              __syncwarp();
+            }
           }
           // P^T as the B operand, in two bf16 terms: the scores' fragments
           // hold keys along gr and heads along tq, the operand the reverse.
@@ -489,6 +561,10 @@ __global__ void __launch_bounds__(PagedCfg<D>::THREADS, PagedCfg<D>::CTAS_PER_SM
                 acc[x][d][3] *= a[1];
               }
             }
+            if constexpr (E4M3) {
+              s[x][0] *= sv[0], s[x][1] *= sv[0];
+              s[x][2] *= sv[1], s[x][3] *= sv[1];
+            }
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
               const uint32_t high = pack_bf16x2(s[x][2 * e], s[x][2 * e + 1]);
@@ -497,14 +573,31 @@ __global__ void __launch_bounds__(PagedCfg<D>::THREADS, PagedCfg<D>::CTAS_PER_SM
                                                 s[x][2 * e + 1] - __uint_as_float(high & 0xffff0000u)));
             }
           }
+          if constexpr (E4M3) {
 #pragma unroll
-          for (int d = 0; d < D / 16; ++d) {
-            uint32_t a[4];
-            ldsm4_t(at(vbase, 8 * (mi >> 1) + mr, 2 * d + (mi & 1)), a[0], a[1], a[2], a[3]);
+            for (int k = 0; k < D / 32; ++k) {
+              uint32_t w[4];
+              ldsm4_t(at(vbase, 8 * (mi >> 1) + mr, 2 * k + (mi & 1)), w[0], w[1], w[2], w[3]);
 #pragma unroll
-            for (int x = 0; x < NT; ++x) {
-              mma16816(acc[x][d], a, ph[x][0], ph[x][1]);
-              mma16816(acc[x][d], a, pl[x][0], pl[x][1]);
+              for (int u = 0; u < 2; ++u) {
+                const uint32_t a[4] = {even_e4m3(w[u]), odd_e4m3(w[u]), even_e4m3(w[u + 2]), odd_e4m3(w[u + 2])};
+#pragma unroll
+                for (int x = 0; x < NT; ++x) {
+                  mma16816(acc[x][2 * k + u], a, ph[x][0], ph[x][1]);
+                  mma16816(acc[x][2 * k + u], a, pl[x][0], pl[x][1]);
+                }
+              }
+            }
+          } else {
+#pragma unroll
+            for (int d = 0; d < D / 16; ++d) {
+              uint32_t a[4];
+              ldsm4_t(at(vbase, 8 * (mi >> 1) + mr, 2 * d + (mi & 1)), a[0], a[1], a[2], a[3]);
+#pragma unroll
+              for (int x = 0; x < NT; ++x) {
+                mma16816(acc[x][d], a, ph[x][0], ph[x][1]);
+                mma16816(acc[x][d], a, pl[x][0], pl[x][1]);
+              }
             }
           }
         }
@@ -515,60 +608,71 @@ __global__ void __launch_bounds__(PagedCfg<D>::THREADS, PagedCfg<D>::CTAS_PER_SM
       // them have read it; the stage is released after that.
       asm volatile("bar.sync 1, 128;" ::: "memory");
       const int slot = n_last % C::STAGES;
-      // [4][16][D], columns swizzled by the head so that neither side's accesses
+      // [4][MERGE][D], columns swizzled by the head so that neither side's accesses
       // collide in a bank.
       float* so = reinterpret_cast<float*>(smem + slot * C::STAGE_BYTES);
+      const long long part = ((long long)w.b * p.Hkv + w.g + blockIdx.x) * p.group;
+      constexpr int kBlocks = C::MERGE / 8 < NT ? C::MERGE / 8 : NT;  // blocks of 8 heads merged at a time
 #pragma unroll
-      for (int x = 0; x < NT; ++x) {
+      for (int x0 = 0; x0 < NT; x0 += kBlocks) {
+        if (x0 > 0) asm volatile("bar.sync 1, 128;" ::: "memory");
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const int r = 8 * x + 2 * tq + c;
-          float lr = l[x][c];
-          lr += __shfl_xor_sync(0xffffffffu, lr, 4);
-          lr += __shfl_xor_sync(0xffffffffu, lr, 8);
-          lr += __shfl_xor_sync(0xffffffffu, lr, 16);
-          if (gr == 0) {
-            bars->m[warp][r] = m[x][c];
-            bars->l[warp][r] = lr;
-          }
-          if (r < p.group) {
-            float* row = so + (warp * 16 + r) * D;
+        for (int x = x0; x < x0 + kBlocks; ++x) {
 #pragma unroll
-            for (int d = 0; d < D / 16; ++d) {
-              row[swizzle(r, 16 * d + gr)] = acc[x][d][c];
-              row[swizzle(r, 16 * d + 8 + gr)] = acc[x][d][2 + c];
+          for (int c = 0; c < 2; ++c) {
+            const int r = 8 * x + 2 * tq + c;
+            float lr = l[x][c];
+            lr += __shfl_xor_sync(0xffffffffu, lr, 4);
+            lr += __shfl_xor_sync(0xffffffffu, lr, 8);
+            lr += __shfl_xor_sync(0xffffffffu, lr, 16);
+            if (gr == 0) {
+              bars->m[warp][r] = m[x][c];
+              bars->l[warp][r] = lr;
+            }
+            if (r < p.group) {
+              float* row = so + (warp * C::MERGE + r - 8 * x0) * D;
+#pragma unroll
+              for (int d = 0; d < D / 16; ++d) {
+                if constexpr (E4M3) {
+                  *reinterpret_cast<float2*>(row + swizzle(r, 16 * d + 2 * gr)) =
+                      make_float2(acc[x][d][c], acc[x][d][2 + c]);
+                } else {
+                  row[swizzle(r, 16 * d + gr)] = acc[x][d][c];
+                  row[swizzle(r, 16 * d + 8 + gr)] = acc[x][d][2 + c];
+                }
+              }
             }
           }
         }
-      }
-      asm volatile("bar.sync 1, 128;" ::: "memory");
-      // Thread x takes columns 4 x .. of the group's rows, 512 apart. Not
-      // unrolled, and finished by the joining kernel when SPLIT: this runs
-      // once per pair, and fetching more instructions from memory (which the
-      // stream of keys has pushed out of L2) cost more than running them.
-      const long long part = ((long long)w.b * p.Hkv + w.g + blockIdx.x) * p.group;
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        // Thread x takes columns 4 x .. of the group's rows, 512 apart. Not
+        // unrolled, and finished by the joining kernel when SPLIT: this runs
+        // once per pair, and fetching more instructions from memory (which the
+        // stream of keys has pushed out of L2) cost more than running them.
+        const int rows_here = min(p.group - 8 * x0, C::MERGE);
 #pragma unroll 1
-      for (int e = 4 * threadIdx.x; e < p.group * D; e += 512) {
-        const int r = e / D, d = e % D;
-        float M = -INFINITY;
+        for (int e = 4 * threadIdx.x; e < rows_here * D; e += 512) {
+          const int rr = e / D, r = 8 * x0 + rr, d = e % D;
+          float M = -INFINITY;
 #pragma unroll
-        for (int u = 0; u < 4; ++u) M = fmaxf(M, bars->m[u][r]);
-        const float Mu = (M == -INFINITY) ? 0.f : M;
-        float lsum = 0.f;
-        float4 osum = zero4();
+          for (int u = 0; u < 4; ++u) M = fmaxf(M, bars->m[u][r]);
+          const float Mu = (M == -INFINITY) ? 0.f : M;
+          float lsum = 0.f;
+          float4 osum = zero4();
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          // A warp without keys here has nothing in the sum (its m is -inf).
-          const float f = ex2(bars->m[u][r] - Mu);
-          lsum += f * bars->l[u][r];
-          osum = axpy(f, *reinterpret_cast<const float4*>(so + (u * 16 + r) * D + swizzle(r, d)), osum);
-        }
-        if constexpr (SPLIT) {
-          *reinterpret_cast<float4*>(p.part_o + (part + r) * D + d) = osum;
-          if (d == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * (part + r)) = make_float2(M, lsum);
-        } else {
-          const int h = w.g * p.group + r;
-          store_output(p, w.b, h, d, over(osum, lsum), p.gate ? load_gate(p, w.b, h, d) : zero4());
+          for (int u = 0; u < 4; ++u) {
+            // A warp without keys here has nothing in the sum (its m is -inf).
+            const float f = ex2(bars->m[u][r] - Mu);
+            lsum += f * bars->l[u][r];
+            osum = axpy(f, *reinterpret_cast<const float4*>(so + (u * C::MERGE + rr) * D + swizzle(r, d)), osum);
+          }
+          if constexpr (SPLIT) {
+            *reinterpret_cast<float4*>(p.part_o + (part + r) * D + d) = osum;
+            if (d == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * (part + r)) = make_float2(M, lsum);
+          } else {
+            const int h = w.g * p.group + r;
+            store_output(p, w.b, h, d, over(osum, lsum), p.gate ? load_gate(p, w.b, h, d) : zero4());
+          }
         }
       }
       if (SPLIT && threadIdx.x == 0) {
@@ -666,34 +770,40 @@ __global__ void __launch_bounds__(kJoinThreads) decode_paged_join_kernel(const _
 
 constexpr int kWholeTiles = 8;
 
-template <int D, int NT, bool SPLIT>
+template <int D, int NT, bool SPLIT, bool E4M3>
 int launch_main(const CUtensorMap& tk, const CUtensorMap& tv, const DecodePagedParams& p, long long n,
                 cudaStream_t st) {
-  using C = PagedCfg<D>;
+  using C = PagedCfg<D, E4M3>;
   static OncePerDevice once;
   if (n > 0x7fffffffLL) return -1;
   return once.run(
       [] {
-        return cudaFuncSetAttribute(decode_paged_kernel<D, NT, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+        return cudaFuncSetAttribute(decode_paged_kernel<D, NT, SPLIT, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                     C::SMEM_BYTES) == cudaSuccess;
       },
       [&] {
-        return launch_dependent(decode_paged_kernel<D, NT, SPLIT>, dim3((unsigned)n), C::THREADS, C::SMEM_BYTES, st, 0,
+        return launch_dependent(decode_paged_kernel<D, NT, SPLIT, E4M3>, dim3((unsigned)n), C::THREADS, C::SMEM_BYTES, st, 0,
                                 tk, tv, p);
       });
 }
 
+template <int D, bool SPLIT>
+int launch_n(const CUtensorMap& tk, const CUtensorMap& tv, const DecodePagedParams& p, long long n, cudaStream_t st) {
+  const bool narrow = p.group <= 8;
+  if (p.k_scales)
+    return narrow ? launch_main<D, 1, SPLIT, true>(tk, tv, p, n, st)
+                  : launch_main<D, 2, SPLIT, true>(tk, tv, p, n, st);
+  return narrow ? launch_main<D, 1, SPLIT, false>(tk, tv, p, n, st)
+                : launch_main<D, 2, SPLIT, false>(tk, tv, p, n, st);
+}
+
 template <int D>
 int launch_t(const CUtensorMap& tk, const CUtensorMap& tv, const DecodePagedParams& p, cudaStream_t st) {
-  const bool narrow = p.group <= 8;
-  if (!decode_paged_splits(p.table_width, p.page)) {
-    const long long pairs = (long long)p.B * p.Hkv;
-    return narrow ? launch_main<D, 1, false>(tk, tv, p, pairs, st) : launch_main<D, 2, false>(tk, tv, p, pairs, st);
-  }
+  if (!decode_paged_splits(p.table_width, p.page))
+    return launch_n<D, false>(tk, tv, p, (long long)p.B * p.Hkv, st);
   const long long heads = (long long)p.B * p.Hq;
   if (heads > 0x7fffffffLL) return -2;
-  const int rc =
-      narrow ? launch_main<D, 1, true>(tk, tv, p, p.n_ctas, st) : launch_main<D, 2, true>(tk, tv, p, p.n_ctas, st);
+  const int rc = launch_n<D, true>(tk, tv, p, p.n_ctas, st);
   if (rc) return rc;
   return launch_dependent(decode_paged_join_kernel<D>, dim3((unsigned)heads), kJoinThreads, 0, st, 0, p) == cudaSuccess
              ? 0

@@ -12,6 +12,9 @@ struct DecodePagedParams {
   const int* block_table;  // [B, table_width], row stride table_ld
   long long table_ld;
   int table_width, n_pages, page;
+  const float* k_scales;  // both or neither: [n_pages, Hkv, page], strides kss (page, head); the pools are then e4m3
+  const float* v_scales;
+  long long kss[2], vss[2];
   int box_rows;            // keys per TMA box: 64, 32 or 16, divides page
   const int* seqlens;      // [B], device
   void* o;                 // [B, Hq, D]
@@ -40,7 +43,8 @@ int decode_paged_max_ctas(int D, int sms);
 inline size_t decode_paged_parts(int B, int Hkv, int n_ctas) { return (size_t)B * Hkv + n_ctas; }
 
 // tk / tv: 5-D maps (64 columns, slot in the page, D / 64, head, page) with
-// box (64, box_rows, D / 64, 1, 1). Returns 0 on success, -3 for an
+// box (64, box_rows, D / 64, 1, 1); of 8-bit pools 128 columns and D / 128 (head
+// dim 64: 64 and 1). Returns 0 on success, -3 for an
 // unsupported head_dim, another negative value on launch failure.
 int launch_decode_paged(int D, const CUtensorMap& tk, const CUtensorMap& tv, const DecodePagedParams& p,
                         cudaStream_t st);

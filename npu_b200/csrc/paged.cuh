@@ -1,0 +1,59 @@
+// What the kernels over packed tokens and a paged cache share: the sequence of a
+// token, and the 8-bit form of a cached row.
+//
+// 8-bit rows (one token's k or v of one KV head): with a = max |y_i|,
+//   s = max(a / 448, 2^-100),  c_i = e4m3(y_i / s),  read back as c_i s.
+// 448 is the largest e4m3 value, so nothing saturates; e4m3 keeps 4 significant
+// bits of c_i >= 2^-6 and steps of 2^-9 below, so a value is off by at most
+// 2^-4 of itself or 2^-10 s. One scale a row and not one a page: rows are
+// written one by one, and a page's scale would change under those already
+// there. The floor 2^-100 keeps 1 / s finite for rows of (nearly) zeros. A row
+// with an infinity or a NaN has the scale NaN and reads back as NaN throughout.
+#pragma once
+
+#include "common.cuh"
+
+namespace b2a {
+
+constexpr float kE4m3Max = 448.f;
+constexpr float kE4m3SmallestScale = 7.888609052210118e-31f;  // 2^-100
+
+// The sequence that owns token n: the largest b with cu[b] <= n (0 when there
+// is none), by a search that narrows 32-fold per step. Warp-collective.
+__device__ __forceinline__ int find_sequence(const int* cu, int B, long long n) {
+  const int lane = threadIdx.x & 31;
+  int lo = 0, len = B;
+  while (len > 1) {
+    const int step = (len + 31) / 32;
+    const int at = lo + lane * step;
+    const bool before = lane * step < len && (lane == 0 || cu[at] <= n);
+    const unsigned m = __ballot_sync(0xffffffffu, before);
+    const int hit = 31 - __clz(m);
+    len = min(step, len - hit * step);
+    lo += hit * step;
+  }
+  return lo;
+}
+
+// Whether offsets c0 and c1 are a stretch of N tokens.
+__device__ __forceinline__ bool is_stretch(int c0, int c1, long long N) { return c0 >= 0 && c1 >= c0 && c1 <= N; }
+
+// Four floats as e4m3, rounded to nearest even, the first in the low byte.
+__device__ __forceinline__ uint32_t pack_e4m3x4(float a, float b, float c, float d) {
+  uint16_t lo, hi;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b), "f"(a));
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
+  return (uint32_t)lo | ((uint32_t)hi << 16);
+}
+
+// |x| as an integer of the same order, in which infinities and NaN are largest.
+__device__ __forceinline__ unsigned magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+
+// The scale of a row whose largest magnitude is m.
+__device__ __forceinline__ float e4m3_scale(unsigned m) {
+  if (m >= 0x7f800000u) return __uint_as_float(0x7fffffffu);  // NaN
+  const float s = __fdiv_rn(__uint_as_float(m), kE4m3Max);
+  return s < kE4m3SmallestScale ? kE4m3SmallestScale : s;
+}
+
+}  // namespace b2a

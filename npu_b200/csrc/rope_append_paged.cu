@@ -24,7 +24,10 @@
 // with norms and 64 turned lanes: 45 us, 5.0 TB/s (0.76 of the measured copy
 // rate; issue slots at 64 % are the next bound), from fp32 sources 58 us, 5.9
 // TB/s (0.90); 64 single tokens, 32 / 4 heads of 128: 3.0 us, one launch.
+#include <type_traits>
+
 #include "capi_internal.cuh"
+#include "paged.cuh"
 #include "rope_append_paged.cuh"
 
 namespace b2a {
@@ -78,34 +81,14 @@ __device__ __forceinline__ void load4(const void* p, long long at, float2 (&x)[2
   f.get(x);
 }
 
-// The sequence that owns token n: the largest b with cu[b] <= n (0 when there
-// is none), by a search that narrows 32-fold per step. Warp-collective.
-__device__ __forceinline__ int find_sequence(const int* cu, int B, long long n) {
-  const int lane = threadIdx.x & 31;
-  int lo = 0, len = B;
-  while (len > 1) {
-    const int step = (len + 31) / 32;
-    const int at = lo + lane * step;
-    const bool before = lane * step < len && (lane == 0 || cu[at] <= n);
-    const unsigned m = __ballot_sync(0xffffffffu, before);
-    const int hit = 31 - __clz(m);
-    len = min(step, len - hit * step);
-    lo += hit * step;
-  }
-  return lo;
-}
-
-// Whether offsets c0 and c1 are a stretch of the tokens.
-__device__ __forceinline__ bool is_stretch(const RopeAppendPagedParams& p, int c0, int c1) {
-  return c0 >= 0 && c1 >= c0 && c1 <= p.N;
-}
-
 constexpr int kWarps = 4;  // tokens of a block
 
 // Warp x of block (i, y) takes token i kWarps + x and chunk y of its rows: the
 // first q_chunks chunks are of q, the rest of k and v. A chunk is STEPS times
-// the 32 / (D / 8) rows a warp holds at a time.
-template <typename Src, int D, int STEPS>
+// the 32 / (D / 8) rows a warp holds at a time. E4M3: the pools are 8-bit
+// (paged.cuh); a row's largest magnitude is a shuffle reduction like a norm's
+// sum, and its first thread stores the scale.
+template <typename Src, int D, int STEPS, bool E4M3>
 __global__ void __launch_bounds__(32 * kWarps)
     rope_append_paged_kernel(const __grid_constant__ RopeAppendPagedParams p, int q_chunks) {
   constexpr int LPR = D / 8;       // lanes per row
@@ -117,7 +100,7 @@ __global__ void __launch_bounds__(32 * kWarps)
   if (blockIdx.x == 0 && blockIdx.y == 0)
     for (int b = threadIdx.x; b < p.B; b += 32 * kWarps) {
       const int c0 = p.cu_seqlens[b], c1 = p.cu_seqlens[b + 1];
-      const bool good = is_stretch(p, c0, c1);
+      const bool good = is_stretch(c0, c1, p.N);
       if (!good && p.err) atomicOr(p.err, kErrBadArgs);
       if (p.seqlens_out)
         p.seqlens_out[b] = (p.start_pos_arr ? p.start_pos_arr[b] : p.start_pos) + (good ? c1 - c0 : 0);
@@ -153,7 +136,7 @@ __global__ void __launch_bounds__(32 * kWarps)
   // The token's sequence, position and page: the same for the whole warp.
   const int b = find_sequence(p.cu_seqlens, p.B, n);
   const int c0 = p.cu_seqlens[b], c1 = p.cu_seqlens[b + 1];
-  if (n < c0 || n >= c1 || !is_stretch(p, c0, c1)) return;  // a row outside every sequence
+  if (n < c0 || n >= c1 || !is_stretch(c0, c1, p.N)) return;  // a row outside every sequence
   const long long at = (long long)(p.start_pos_arr ? p.start_pos_arr[b] : p.start_pos) + (n - c0);
   const bool counts = at >= 0 && at <= 0x7fffffff;
   const unsigned pos = counts ? (unsigned)at : 0u;
@@ -227,8 +210,9 @@ __global__ void __launch_bounds__(32 * kWarps)
       }
     }
   } else {
-    __nv_bfloat16* k_dst = p.k_pages + page_id * p.kps[0] + slot * p.kps[2];
-    __nv_bfloat16* v_dst = p.v_pages + page_id * p.vps[0] + slot * p.vps[2];
+    using Cache = std::conditional_t<E4M3, uint8_t, __nv_bfloat16>;
+    Cache* k_dst = static_cast<Cache*>(p.k_pages) + page_id * p.kps[0] + slot * p.kps[2];
+    Cache* v_dst = static_cast<Cache*>(p.v_pages) + page_id * p.vps[0] + slot * p.vps[2];
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
       const int j = j0 + s * ROWS;
@@ -238,9 +222,28 @@ __global__ void __launch_bounds__(32 * kWarps)
       raw[s][0].get(x);
       raw[s][1].get(y);
       turn(x, y, is_v);
+      float scale = 0.f;
+      if constexpr (E4M3) {
+        unsigned m = 0;
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          m = max(max(max(m, magnitude(x[e].x)), max(magnitude(x[e].y), magnitude(y[e].x))), magnitude(y[e].y));
+#pragma unroll
+        for (int off = LPR / 2; off > 0; off >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, off));
+        scale = e4m3_scale(m);
+      }
       if (!in_pool || !in_table || j >= rows) continue;
-      __nv_bfloat16* dst = is_v ? v_dst + h * p.vps[1] : k_dst + h * p.kps[1];
-      store4(dst + o0, x), store4(dst + o1, y);
+      Cache* dst = is_v ? v_dst + h * p.vps[1] : k_dst + h * p.kps[1];
+      if constexpr (E4M3) {
+        const float f = __fdiv_rn(1.f, scale);
+        *reinterpret_cast<uint32_t*>(dst + o0) = pack_e4m3x4(x[0].x * f, x[0].y * f, x[1].x * f, x[1].y * f);
+        *reinterpret_cast<uint32_t*>(dst + o1) = pack_e4m3x4(y[0].x * f, y[0].y * f, y[1].x * f, y[1].y * f);
+        float* scales = is_v ? p.v_scales + page_id * p.vss[0] + h * p.vss[1]
+                             : p.k_scales + page_id * p.kss[0] + h * p.kss[1];
+        if (part == 0) scales[slot] = scale;
+      } else {
+        store4(dst + o0, x), store4(dst + o1, y);
+      }
       __nv_bfloat16* packed = is_v ? p.v_out : p.k_out;
       if (packed) {
         packed += (n * p.Hkv + h) * D;
@@ -250,14 +253,14 @@ __global__ void __launch_bounds__(32 * kWarps)
   }
 }
 
-template <typename Src, int D, int STEPS>
+template <typename Src, int D, int STEPS, bool E4M3>
 int launch_steps(const RopeAppendPagedParams& p, cudaStream_t st) {
   constexpr int ROWS = 32 / (D / 8);
   const long long blocks = (p.N + kWarps - 1) / kWarps;
   const int q_chunks = (p.Hq + STEPS * ROWS - 1) / (STEPS * ROWS);
   const int chunks = q_chunks + (2 * p.Hkv + STEPS * ROWS - 1) / (STEPS * ROWS);
   if (blocks <= 0 || blocks > 0x7fffffffLL || chunks > 65535) return -2;
-  return launch_dependent(rope_append_paged_kernel<Src, D, STEPS>, dim3((unsigned)blocks, (unsigned)chunks),
+  return launch_dependent(rope_append_paged_kernel<Src, D, STEPS, E4M3>, dim3((unsigned)blocks, (unsigned)chunks),
                           32 * kWarps, 0, st, 0, p, q_chunks) == cudaSuccess
              ? 0
              : -1;
@@ -265,18 +268,18 @@ int launch_steps(const RopeAppendPagedParams& p, cudaStream_t st) {
 
 // Four rows per thread spread a token's lookups over more rows; few tokens get
 // one, so that their rows are in more warps at once.
-template <typename Src, int D>
+template <typename Src, int D, bool E4M3>
 int launch_t(const RopeAppendPagedParams& p, cudaStream_t st) {
   const long long row_warps = p.N * ((p.Hq + 2 * p.Hkv) / (32 / (D / 8)) + 1);
-  return row_warps >= 148 * 32 ? launch_steps<Src, D, 4>(p, st) : launch_steps<Src, D, 1>(p, st);
+  return row_warps >= 148 * 32 ? launch_steps<Src, D, 4, E4M3>(p, st) : launch_steps<Src, D, 1, E4M3>(p, st);
 }
 
-template <typename Src>
+template <typename Src, bool E4M3>
 int launch_src(int D, const RopeAppendPagedParams& p, cudaStream_t st) {
   switch (D) {
-    case 64: return launch_t<Src, 64>(p, st);
-    case 128: return launch_t<Src, 128>(p, st);
-    case 256: return launch_t<Src, 256>(p, st);
+    case 64: return launch_t<Src, 64, E4M3>(p, st);
+    case 128: return launch_t<Src, 128, E4M3>(p, st);
+    case 256: return launch_t<Src, 256, E4M3>(p, st);
     default: return -3;
   }
 }
@@ -284,7 +287,9 @@ int launch_src(int D, const RopeAppendPagedParams& p, cudaStream_t st) {
 }  // namespace
 
 int launch_rope_append_paged(int D, const RopeAppendPagedParams& p, cudaStream_t st) {
-  return p.src_bf16 ? launch_src<__nv_bfloat16>(D, p, st) : launch_src<float>(D, p, st);
+  if (p.k_scales)
+    return p.src_bf16 ? launch_src<__nv_bfloat16, true>(D, p, st) : launch_src<float, true>(D, p, st);
+  return p.src_bf16 ? launch_src<__nv_bfloat16, false>(D, p, st) : launch_src<float, false>(D, p, st);
 }
 
 }  // namespace b2a

@@ -23,9 +23,12 @@ struct RopeAppendPagedParams {
   __nv_bfloat16* q_out;  // [N, Hq, D] contiguous
   __nv_bfloat16* k_out;  // optional [N, Hkv, D] contiguous
   __nv_bfloat16* v_out;  // optional [N, Hkv, D] contiguous
-  __nv_bfloat16* k_pages;  // [n_pages, Hkv, page, D], strides kps (page, head, slot)
-  __nv_bfloat16* v_pages;
+  void* k_pages;  // [n_pages, Hkv, page, D] bf16 (e4m3 with scales), strides kps (page, head, slot)
+  void* v_pages;
   long long kps[3], vps[3];
+  float* k_scales;  // both or neither: [n_pages, Hkv, page], strides kss (page, head); the pools are then e4m3
+  float* v_scales;
+  long long kss[2], vss[2];
   const int* block_table;  // [B, table_width], row stride table_ld
   long long table_ld;
   int table_width, n_pages, page;

@@ -47,6 +47,31 @@ void need_bf16(const char* name, const Tensor& t, int ndim, const c10::Device* d
   if (t.stride(-1) != 1) refuse(name, " needs a contiguous last (head_dim) dimension");
 }
 
+// The page pools [n_pages, Hkv, page, D]: bf16 without scales, e4m3 with them ([n_pages, Hkv, page] fp32).
+void need_pools(const Tensor& k, const Tensor& v, const OptTensor& k_scales, const OptTensor& v_scales,
+                const c10::Device& device) {
+  if (!k_scales && !v_scales) {
+    if (k.scalar_type() == at::kFloat8_e4m3fn || v.scalar_type() == at::kFloat8_e4m3fn)
+      refuse("pools of float8_e4m3fn need k_scales and v_scales");
+    need_bf16("k_pages", k, 4, &device);
+    need_bf16("v_pages", v, 4, &device);
+    return;
+  }
+  if (!k_scales || !v_scales) refuse("k_scales and v_scales come together");
+  for (auto [name, t] : {std::pair<const char*, const Tensor*>{"k_pages", &k}, {"v_pages", &v}}) {
+    need_cuda(name, *t, &device);
+    if (t->scalar_type() != at::kFloat8_e4m3fn)
+      refuse(name, " must be float8_e4m3fn with scales, got ", t->scalar_type());
+    if (t->dim() != 4) refuse(name, " must have 4 dims, got shape ", t->sizes());
+    if (t->stride(-1) != 1) refuse(name, " needs a contiguous last (head_dim) dimension");
+  }
+  for (auto [name, t] : {std::pair<const char*, const Tensor*>{"k_scales", &*k_scales}, {"v_scales", &*v_scales}})
+    if (t->scalar_type() != at::kFloat || t->device() != device || t->sizes() != k.sizes().slice(0, 3) ||
+        t->stride(-1) != 1)
+      refuse(name, " must be a float32 tensor ", k.sizes().slice(0, 3),
+             " on the inputs' device with a contiguous last dim");
+}
+
 void need_int32(const char* name, const Tensor& t, int64_t numel, const c10::Device& device) {
   if (t.scalar_type() != at::kInt || t.device() != device || t.numel() != numel || !t.is_contiguous())
     refuse(name, " must be a contiguous int32 tensor of ", numel, " on the inputs' device");
@@ -141,11 +166,11 @@ py::object prefill_varlen(const Tensor& q, const Tensor& k, const Tensor& v, con
 
 Tensor decode_paged(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table,
                     const Tensor& seqlens, std::optional<double> scale, at::ScalarType out_dtype,
-                    const OptTensor& workspace, const OptTensor& out, const OptTensor& gate) {
+                    const OptTensor& workspace, const OptTensor& out, const OptTensor& gate, const OptTensor& k_scales,
+                    const OptTensor& v_scales) {
   need_bf16("q", q, 3);
   const c10::Device device = q.device();
-  need_bf16("k_pages", k_pages, 4, &device);
-  need_bf16("v_pages", v_pages, 4, &device);
+  need_pools(k_pages, v_pages, k_scales, v_scales, device);
   const int64_t B = q.size(0), Hq = q.size(1), D = q.size(2), n_pages = k_pages.size(0), Hkv = k_pages.size(1),
                 page = k_pages.size(2);
   if (k_pages.size(3) != D || v_pages.sizes() != k_pages.sizes())
@@ -173,14 +198,25 @@ Tensor decode_paged(const Tensor& q, const Tensor& k_pages, const Tensor& v_page
     ws = taken.get();
   }
   const Strides gs(gate ? *gate : q, 2);
-  check(b2a_decode_paged(q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), table.data_ptr<int>(), table.stride(0),
-                         as_int("table width", table.size(1)), seqlens.data_ptr<int>(), pointer(gate), o.data_ptr(),
-                         (int)B, (int)Hq, (int)Hkv, as_int("n_pages", n_pages), as_int("page", page), (int)D,
-                         Strides(q, 2), Strides(k_pages, 3), Strides(v_pages, 3), gs, Strides(o, 2),
-                         gate && gate->scalar_type() == at::kBFloat16,
-                         (float)scale.value_or(1.0 / std::sqrt((double)D)), out_dtype == at::kFloat, ws, need,
-                         stream_of(q)),
-        "b2a_decode_paged");
+  const float used = (float)scale.value_or(1.0 / std::sqrt((double)D));
+  const bool gate_bf16 = gate && gate->scalar_type() == at::kBFloat16;
+  const int pages = as_int("n_pages", n_pages), slots = as_int("page", page),
+            width = as_int("table width", table.size(1));
+  if (k_scales)
+    check(b2a_decode_paged_e4m3(q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), k_scales->data_ptr<float>(),
+                                v_scales->data_ptr<float>(), Strides(*k_scales, 2), Strides(*v_scales, 2),
+                                table.data_ptr<int>(), table.stride(0), width, seqlens.data_ptr<int>(), pointer(gate),
+                                o.data_ptr(), (int)B, (int)Hq, (int)Hkv, pages, slots, (int)D, Strides(q, 2),
+                                Strides(k_pages, 3), Strides(v_pages, 3), gs, Strides(o, 2), gate_bf16, used,
+                                out_dtype == at::kFloat, ws, need, stream_of(q)),
+          "b2a_decode_paged_e4m3");
+  else
+    check(b2a_decode_paged(q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), table.data_ptr<int>(),
+                           table.stride(0), width, seqlens.data_ptr<int>(), pointer(gate), o.data_ptr(), (int)B,
+                           (int)Hq, (int)Hkv, pages, slots, (int)D, Strides(q, 2), Strides(k_pages, 3),
+                           Strides(v_pages, 3), gs, Strides(o, 2), gate_bf16, used, out_dtype == at::kFloat, ws, need,
+                           stream_of(q)),
+          "b2a_decode_paged");
   return o;
 }
 
@@ -188,7 +224,8 @@ py::object rope_append_paged(const Tensor& q, const Tensor& k, const Tensor& v, 
                              const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& cu,
                              int64_t start_pos, const OptTensor& start, const OptTensor& seqlens_out,
                              const OptTensor& q_out, const OptTensor& q_norm, const OptTensor& k_norm, double eps,
-                             std::optional<int64_t> rope_dim, bool return_kv) {
+                             std::optional<int64_t> rope_dim, bool return_kv, const OptTensor& k_scales,
+                             const OptTensor& v_scales) {
   for (auto [name, t] : {std::pair<const char*, const Tensor*>{"q", &q}, {"k", &k}, {"v", &v}})
     if (!t->is_cuda() || t->dim() != 3 || t->stride(-1) != 1)
       refuse(name, " must be a CUDA [N, H, D] tensor with a contiguous last dim");
@@ -206,8 +243,7 @@ py::object rope_append_paged(const Tensor& q, const Tensor& k, const Tensor& v, 
       !cos.is_contiguous() || !sin.is_contiguous() || cos.dim() != 2 || cos.size(1) != rope ||
       sin.sizes() != cos.sizes())
     refuse("cos/sin must be contiguous [max_pos, rope_dim] tensors, float32 or in q's dtype");
-  need_bf16("k_pages", k_pages, 4, &device);
-  need_bf16("v_pages", v_pages, 4, &device);
+  need_pools(k_pages, v_pages, k_scales, v_scales, device);
   if (k_pages.size(1) != Hkv || k_pages.size(3) != D || v_pages.sizes() != k_pages.sizes())
     refuse("cache shape ", k_pages.sizes(), " does not fit k", k.sizes());
   const int64_t B = cu.numel() - 1;
@@ -240,19 +276,63 @@ py::object rope_append_paged(const Tensor& q, const Tensor& k, const Tensor& v, 
     if (seqlens_out && !start) seqlens_out->fill_(start_pos);
     return result();
   }
-  check(b2a_rope_append_paged(q.data_ptr(), k.data_ptr(), v.data_ptr(), Strides(q, 2), Strides(k, 2), Strides(v, 2),
-                              bf16, pointer(q_norm), pointer(k_norm), (float)eps, cos.data_ptr(), sin.data_ptr(),
-                              cos.scalar_type() == at::kFloat, as_int("max_pos", cos.size(0)),
-                              as_int("rope_dim", rope), qo.data_ptr(), pointer(ko), pointer(vo), k_pages.data_ptr(),
-                              v_pages.data_ptr(), Strides(k_pages, 3), Strides(v_pages, 3), table.data_ptr<int>(),
-                              table.stride(0), as_int("table width", table.size(1)),
-                              as_int("n_pages", k_pages.size(0)), as_int("page", k_pages.size(2)),
-                              cu.data_ptr<int>(), as_int("B", B), as_int("N", N), as_int("Hq", Hq),
-                              as_int("Hkv", Hkv), as_int("D", D), as_int("start_pos", start_pos),
-                              static_cast<int*>(pointer(start)), static_cast<int*>(pointer(seqlens_out)),
-                              stream_of(q)),
-        "b2a_rope_append_paged");
+  const int tables_fp32 = cos.scalar_type() == at::kFloat, max_pos = as_int("max_pos", cos.size(0)),
+            width = as_int("table width", table.size(1)), pages = as_int("n_pages", k_pages.size(0)),
+            slots = as_int("page", k_pages.size(2)), first = as_int("start_pos", start_pos);
+  if (k_scales)
+    check(b2a_rope_append_paged_e4m3(
+              q.data_ptr(), k.data_ptr(), v.data_ptr(), Strides(q, 2), Strides(k, 2), Strides(v, 2), bf16,
+              pointer(q_norm), pointer(k_norm), (float)eps, cos.data_ptr(), sin.data_ptr(), tables_fp32, max_pos,
+              as_int("rope_dim", rope), qo.data_ptr(), pointer(ko), pointer(vo), k_pages.data_ptr(), v_pages.data_ptr(),
+              Strides(k_pages, 3), Strides(v_pages, 3), k_scales->data_ptr<float>(), v_scales->data_ptr<float>(),
+              Strides(*k_scales, 2), Strides(*v_scales, 2), table.data_ptr<int>(), table.stride(0), width, pages, slots,
+              cu.data_ptr<int>(), as_int("B", B), as_int("N", N), as_int("Hq", Hq), as_int("Hkv", Hkv), as_int("D", D),
+              first, static_cast<int*>(pointer(start)), static_cast<int*>(pointer(seqlens_out)), stream_of(q)),
+          "b2a_rope_append_paged_e4m3");
+  else
+    check(b2a_rope_append_paged(
+              q.data_ptr(), k.data_ptr(), v.data_ptr(), Strides(q, 2), Strides(k, 2), Strides(v, 2), bf16,
+              pointer(q_norm), pointer(k_norm), (float)eps, cos.data_ptr(), sin.data_ptr(), tables_fp32, max_pos,
+              as_int("rope_dim", rope), qo.data_ptr(), pointer(ko), pointer(vo), k_pages.data_ptr(), v_pages.data_ptr(),
+              Strides(k_pages, 3), Strides(v_pages, 3), table.data_ptr<int>(), table.stride(0), width, pages, slots,
+              cu.data_ptr<int>(), as_int("B", B), as_int("N", N), as_int("Hq", Hq), as_int("Hkv", Hkv), as_int("D", D),
+              first, static_cast<int*>(pointer(start)), static_cast<int*>(pointer(seqlens_out)), stream_of(q)),
+          "b2a_rope_append_paged");
   return result();
+}
+
+py::object gather_paged(const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& cu,
+                        int64_t n_tokens, int64_t start_pos, const OptTensor& start, const OptTensor& k_scales,
+                        const OptTensor& v_scales, const OptTensor& k_out, const OptTensor& v_out) {
+  need_cuda("k_pages", k_pages);
+  const c10::Device device = k_pages.device();
+  need_pools(k_pages, v_pages, k_scales, v_scales, device);
+  if (v_pages.sizes() != k_pages.sizes())
+    refuse("shape mismatch k_pages", k_pages.sizes(), " v_pages", v_pages.sizes());
+  const int64_t Hkv = k_pages.size(1), D = k_pages.size(3), B = cu.numel() - 1;
+  if (n_tokens < 0) refuse("n_tokens must not be negative, got ", n_tokens);
+  if (B < 1) refuse("cu_seqlens must hold at least two offsets");
+  need_int32("cu_seqlens", cu, B + 1, device);
+  need_table(table, B, device);
+  if (start) need_int32("start_pos_per_batch", *start, B, device);
+  const c10::cuda::CUDAGuard guard(device);
+  auto rows = [&](const OptTensor& out, const char* wants) {
+    if (out && !out->is_contiguous()) refuse(wants);
+    return output(out, {n_tokens, Hkv, D}, at::kBFloat16, k_pages, wants);
+  };
+  const Tensor ko = rows(k_out, "k_out must be a contiguous bf16 [n_tokens, Hkv, D] tensor on the pools' device");
+  const Tensor vo = rows(v_out, "v_out must be a contiguous bf16 [n_tokens, Hkv, D] tensor on the pools' device");
+  if (n_tokens > 0)
+    check(b2a_gather_paged(k_pages.data_ptr(), v_pages.data_ptr(), Strides(k_pages, 3), Strides(v_pages, 3),
+                           static_cast<float*>(pointer(k_scales)), static_cast<float*>(pointer(v_scales)),
+                           Strides(k_scales ? *k_scales : k_pages, 2), Strides(v_scales ? *v_scales : v_pages, 2),
+                           table.data_ptr<int>(), table.stride(0), as_int("table width", table.size(1)),
+                           as_int("n_pages", k_pages.size(0)), as_int("page", k_pages.size(2)), cu.data_ptr<int>(),
+                           as_int("B", B), as_int("n_tokens", n_tokens), as_int("Hkv", Hkv), as_int("D", D),
+                           as_int("start_pos", start_pos), static_cast<int*>(pointer(start)), ko.data_ptr(),
+                           vo.data_ptr(), stream_of(k_pages)),
+          "b2a_gather_paged");
+  return py::make_tuple(ko, vo);
 }
 
 // A sampling setting: a number for every row, or a per-row tensor.
@@ -303,11 +383,61 @@ Tensor sample(const Tensor& logits, const OptTensor& noise, const py::handle& te
   return o;
 }
 
+Tensor penalize(const Tensor& logits, const OptTensor& tokens, const OptTensor& lengths,
+                const OptTensor& prompt_lengths, const py::handle& repetition, const py::handle& frequency, const py::handle& presence,
+                const OptTensor& bias, const OptTensor& allowed, const OptTensor& out) {
+  const bool bf16 = logits.scalar_type() == at::kBFloat16;
+  if (!logits.is_cuda() || logits.dim() != 2 || (logits.size(1) > 1 && logits.stride(1) != 1) ||
+      (logits.scalar_type() != at::kFloat && !bf16))
+    refuse("logits must be a CUDA float32 or bfloat16 tensor [R, V] with a contiguous last dim");
+  const int64_t R = logits.size(0), V = logits.size(1), words = (V + 31) / 32;
+  const c10::Device device = logits.device();
+  const bool wide = tokens && tokens->scalar_type() == at::kLong;
+  if (tokens && ((!wide && tokens->scalar_type() != at::kInt) || tokens->device() != device || tokens->dim() != 2 ||
+                 tokens->size(0) != R))
+    refuse("tokens must be an int32 or int64 tensor [", R, ", L] on the logits' device");
+  if (!tokens && (lengths || prompt_lengths)) refuse("lengths and prompt_lengths are of tokens, which are missing");
+  if (lengths) need_int32("lengths", *lengths, R, device);
+  if (prompt_lengths) need_int32("prompt_lengths", *prompt_lengths, R, device);
+  const Setting<float> r("repetition", repetition, R, device), f("frequency", frequency, R, device),
+      a("presence", presence, R, device);
+  if (!r.rows && !(r.all > 0 && std::isfinite((float)r.all))) refuse("repetition must be above 0 and finite");
+  if (!f.rows && !std::isfinite((float)f.all)) refuse("frequency must be finite");
+  if (!a.rows && !std::isfinite((float)a.all)) refuse("presence must be finite");
+  if (bias && (bias->scalar_type() != at::kFloat || bias->device() != device || bias->dim() < 1 || bias->dim() > 2 ||
+               bias->size(-1) != V || (V > 1 && bias->stride(-1) != 1) ||
+               (bias->dim() == 2 && bias->size(0) != R && bias->size(0) != 1)))
+    refuse("bias must be a float32 tensor [", V, "] or [", R, ", ", V,
+           "] on the logits' device with a contiguous last dim");
+  if (allowed && (allowed->scalar_type() != at::kInt || allowed->device() != device || allowed->dim() < 1 ||
+                  allowed->dim() > 2 || allowed->size(-1) != words || (words > 1 && allowed->stride(-1) != 1) ||
+                  (allowed->dim() == 2 && allowed->size(0) != R && allowed->size(0) != 1)))
+    refuse("allowed must be an int32 tensor [", words, "] or [", R, ", ", words,
+           "] on the logits' device with a contiguous last dim");
+  auto row_stride = [](const OptTensor& t) -> int64_t {
+    return t && t->dim() == 2 && t->size(0) > 1 ? t->stride(0) : 0;
+  };
+  const c10::cuda::CUDAGuard guard(device);
+  const Tensor o = output(out, logits.sizes(), logits.scalar_type(), logits,
+                          "out must match the logits' shape, type and device, with a contiguous last dim");
+  if (R == 0 || V == 0) return o;
+  check(b2a_penalize(logits.data_ptr(), logits.stride(0), bf16, pointer(tokens), wide, tokens ? tokens->stride(0) : 0,
+                     tokens ? tokens->stride(1) : 0, tokens ? as_int("L", tokens->size(1)) : 0,
+                     static_cast<int*>(pointer(lengths)), static_cast<int*>(pointer(prompt_lengths)), r.rows,
+                     (float)r.all, f.rows, (float)f.all, a.rows, (float)a.all, static_cast<float*>(pointer(bias)),
+                     row_stride(bias), static_cast<int*>(pointer(allowed)), row_stride(allowed), o.data_ptr(),
+                     o.stride(0), as_int("R", R), as_int("V", V), stream_of(logits)),
+        "b2a_penalize");
+  return o;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_serving, m) {
   m.def("prefill_varlen", &prefill_varlen);
   m.def("decode_paged", &decode_paged);
   m.def("rope_append_paged", &rope_append_paged);
+  m.def("gather_paged", &gather_paged);
+  m.def("penalize", &penalize);
   m.def("sample", &sample);
 }
