@@ -410,6 +410,29 @@ B2A_API int b2a_decode_paged_e4m3(const void* q, const void* k_pages, const void
                                   float scale, int out_fp32, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
+ * b2a_decode_paged for sequences that share the first keys of their cache (a
+ * system prompt, a document): the same result, the shared keys read once and
+ * attended as one matrix product (P rounded to bf16 there, as in b2a_prefill).
+ * Group g is the sequences [cu_groups[g], cu_groups[g + 1]) (device int32
+ * [n_groups + 1]; NULL with n_groups = 1: all of them); their first
+ * prefix_lens[g] keys (device int32 [n_groups]) are the same, whichever
+ * sequence's table names them. Sequences in no group, alone in one, or shorter
+ * than its prefix attend all their keys by themselves, as every sequence does
+ * with the last prefix_lens[g] % 64 of them. A pair of offsets that is not a stretch
+ * of the sequences, groups that overlap or a prefix outside 0 .. table_width * page
+ * report B2A_ERR_DEVICE_BAD_LEN; nothing is shared then for such a group (the prefix
+ * is cut). bf16 pools. Workspace: b2a_decode_paged_shared_workspace_bytes.
+ */
+B2A_API size_t b2a_decode_paged_shared_workspace_bytes(int B, int Hq, int Hkv, int D, int n_groups);
+B2A_API int b2a_decode_paged_shared(const void* q, const void* k_pages, const void* v_pages, const int* block_table,
+                                    long long table_ld, int table_width, const int* seqlens, const int* prefix_lens,
+                                    const int* cu_groups, int n_groups, const void* gate, void* o, int B, int Hq,
+                                    int Hkv, int n_pages, int page, int D, const long long* q_strides,
+                                    const long long* k_strides, const long long* v_strides,
+                                    const long long* gate_strides, const long long* o_strides, int gate_bf16,
+                                    float scale, int out_fp32, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * k and v of a stretch of each sequence out of a paged cache, as packed rows
  * k_out / v_out [N, Hkv, D] bf16 contiguous (what b2a_prefill_varlen reads):
  * row n of sequence b (cu[b] <= n < cu[b + 1]) is the key at position

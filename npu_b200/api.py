@@ -514,6 +514,42 @@ def decode_paged(
                                    k_scales, v_scales)
 
 
+def decode_paged_shared_workspace_bytes(B: int, Hq: int, Hkv: int, D: int, n_groups: int = 1) -> int:
+    return int(_lib.load().b2a_decode_paged_shared_workspace_bytes(B, Hq, Hkv, D, n_groups))
+
+
+def decode_paged_shared(
+    q: torch.Tensor,
+    k_pages: torch.Tensor,
+    v_pages: torch.Tensor,
+    block_table: torch.Tensor,
+    seqlens: torch.Tensor,
+    prefix_lens: torch.Tensor,
+    cu_groups: Optional[torch.Tensor] = None,
+    *,
+    scale: Optional[float] = None,
+    out_dtype: torch.dtype = torch.float32,
+    workspace: Optional[torch.Tensor] = None,
+    out: Optional[torch.Tensor] = None,
+    gate: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """`decode_paged` for sequences that share the first keys of their cache (a
+    system prompt, a document many ask about): the same result, with the shared
+    keys read once for a group and attended as one matrix product.
+
+    Group g is the sequences cu_groups[g] .. cu_groups[g + 1] - 1 (int32 CUDA
+    tensor [groups + 1]; None: all sequences are one group), whose first
+    prefix_lens[g] keys (int32 CUDA tensor [groups]) are the same: block_table
+    names them for every sequence, and any of a group's rows may be read. Whole
+    blocks of 64 keys are shared; a sequence that is alone in its group, in none,
+    or shorter than the prefix attends by itself. Both tensors are read on the
+    device. bf16 pools. P is rounded to bf16 over the shared keys, as in
+    `prefill`. workspace: decode_paged_shared_workspace_bytes.
+    """
+    return _serving().decode_paged_shared(q, k_pages, v_pages, block_table, seqlens, prefix_lens, cu_groups, scale,
+                                          out_dtype, workspace, out, gate)
+
+
 def gather_paged(
     k_pages: torch.Tensor,
     v_pages: torch.Tensor,

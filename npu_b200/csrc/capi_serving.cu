@@ -8,6 +8,7 @@
 #include "b2attn.h"
 #include "capi_internal.cuh"
 #include "decode_paged.cuh"
+#include "decode_shared.cuh"
 #include "gather_paged.cuh"
 #include "penalize.cuh"
 #include "prefill.cuh"
@@ -34,12 +35,12 @@ int packed_map(CUtensorMap* m, const void* base, int D, int rows, int heads, con
 // A page pool [n_pages, heads, page, D] (strides {page, head, slot}): 64
 // columns, slot, D / 64 column chunks, head, page.
 int pool_map(CUtensorMap* m, const void* base, int D, int n_pages, int heads, int page, const long long* s,
-             int box_rows) {
+             int box_rows, int box_chunks) {
   const unsigned long long dims[5] = {64, (unsigned long long)page, (unsigned long long)(D / 64),
                                       (unsigned long long)heads, (unsigned long long)n_pages};
   const unsigned long long strides[4] = {(unsigned long long)s[2] * 2, 128, (unsigned long long)s[1] * 2,
                                          (unsigned long long)s[0] * 2};
-  const unsigned box[5] = {64u, (unsigned)box_rows, (unsigned)(D / 64), 1u, 1u};
+  const unsigned box[5] = {64u, (unsigned)box_rows, (unsigned)box_chunks, 1u, 1u};
   return b2a::api_tensor_map(m, base, 5, dims, strides, box);
 }
 
@@ -67,9 +68,36 @@ int scales_ok(const void* k_scales, const void* v_scales, const long long* kss, 
 
 int status_of(int rc) { return rc == -3 ? B2A_ERR_HEAD_DIM : (rc ? B2A_ERR_LAUNCH : B2A_OK); }
 
+struct SharedPrefix {
+  const int* prefix_lens;
+  const int* cu_groups;
+  int n_groups;
+};
+
+// Where the shared form's scratch is, behind that of the sequences' own keys.
+struct SharedLayout {
+  int max_blocks, n_ctas;
+  size_t groups, seqs, place, part_ml, part_o, bytes;
+};
+SharedLayout shared_layout(int B, int Hq, int Hkv, int D, int n_groups) {
+  SharedLayout at;
+  const int group = Hq / Hkv;
+  // Row blocks: every group of two or more sequences may leave one unfilled.
+  at.max_blocks = B / b2a::decode_shared_block_seqs(D, group) + std::min(n_groups, B / 2);
+  at.n_ctas = b2a::decode_shared_max_ctas(b2a::api_sm_count());
+  const size_t items = (size_t)at.max_blocks * Hkv, rows = (items + at.n_ctas) * b2a::decode_shared_block_rows(D);
+  at.groups = 256;
+  at.seqs = at.groups + b2a::api_align256((size_t)n_groups * sizeof(b2a::SharedGroup));
+  at.place = at.seqs + b2a::api_align256((size_t)B * sizeof(b2a::SharedSeq));
+  at.part_ml = at.place + b2a::api_align256(items * 2 * sizeof(int));
+  at.part_o = at.part_ml + b2a::api_align256(rows * 2 * sizeof(float));
+  at.bytes = at.part_o + rows * D * sizeof(float) + 256;  // and to its own 256-byte boundary
+  return at;
+}
+
 int paged_attention(const void* q, const void* k_pages, const void* v_pages, const int* block_table,
                     const float* k_scales, const float* v_scales, const long long* kss, const long long* vss,
-                    long long table_ld, int table_width, const int* seqlens, const void* gate, void* o, int B,
+                    const SharedPrefix* shared, long long table_ld, int table_width, const int* seqlens, const void* gate, void* o, int B,
                     int Hq, int Hkv, int n_pages, int page, int D, const long long* qs, const long long* ks,
                     const long long* vs, const long long* gs, const long long* os, int gate_bf16, float scale,
                     int out_fp32, void* workspace, size_t workspace_bytes, void* stream) {
@@ -88,7 +116,8 @@ int paged_attention(const void* q, const void* k_pages, const void* v_pages, con
   const long long pool_mult = k_scales ? 16 : 8;
   if (!api_strides_ok(qs, 2, 8) || !api_strides_ok(ks, 3, pool_mult) || !api_strides_ok(vs, 3, pool_mult))
     return B2A_ERR_ALIGNMENT;
-  const size_t need = b2a_decode_paged_workspace_bytes(B, Hq, Hkv, D);
+  const size_t own = b2a_decode_paged_workspace_bytes(B, Hq, Hkv, D);
+  const size_t need = own + (shared ? shared_layout(B, Hq, Hkv, D, shared->n_groups).bytes : 0);
   if (!workspace || workspace_bytes < need || !api_aligned(workspace, 16)) return B2A_ERR_WORKSPACE;
 
   int* err = nullptr;
@@ -98,10 +127,11 @@ int paged_attention(const void* q, const void* k_pages, const void* v_pages, con
   // Keys per TMA box: a box never crosses a page, a warp's 16 keys never a box.
   p.box_rows = page % 64 == 0 ? 64 : (page % 32 == 0 ? 32 : 16);
   CUtensorMap tk, tv;
-  const auto map = k_scales ? pool_map_e4m3 : pool_map;
-  if ((rc = map(&tk, k_pages, D, n_pages, Hkv, page, ks, p.box_rows)) ||
-      (rc = map(&tv, v_pages, D, n_pages, Hkv, page, vs, p.box_rows)))
-    return rc;
+  auto map = [&](CUtensorMap* m, const void* pool, const long long* strides, int box_chunks) {
+    return k_scales ? pool_map_e4m3(m, pool, D, n_pages, Hkv, page, strides, p.box_rows)
+                    : pool_map(m, pool, D, n_pages, Hkv, page, strides, p.box_rows, box_chunks);
+  };
+  if ((rc = map(&tk, k_pages, ks, D / 64)) || (rc = map(&tv, v_pages, vs, D / 64))) return rc;
   p.k_scales = k_scales;
   p.v_scales = v_scales;
   if (k_scales) {
@@ -144,6 +174,58 @@ int paged_attention(const void* q, const void* k_pages, const void* v_pages, con
   scratch += b2a::api_align256(rows * D * sizeof(float));
   p.part_ml = reinterpret_cast<float*>(scratch);
   p.place = reinterpret_cast<int*>(scratch + b2a::api_align256(rows * 2 * sizeof(float)));
+  // Few keys, or one sequence: every sequence reads its own (one launch).
+  if (shared && B > 1 && b2a::decode_paged_splits(table_width, page)) {
+    const SharedLayout at = shared_layout(B, Hq, Hkv, D, shared->n_groups);
+    char* base = reinterpret_cast<char*>(b2a::api_align256(reinterpret_cast<uintptr_t>(workspace) + own));
+    b2a::SharedPlanParams plan{};
+    plan.prefix_lens = shared->prefix_lens;
+    plan.cu_groups = shared->cu_groups;
+    plan.n_groups = shared->n_groups;
+    plan.seqlens = seqlens;
+    plan.B = B;
+    plan.Hkv = Hkv;
+    plan.group = p.group;
+    plan.cap = (long long)table_width * page;
+    plan.max_blocks = at.max_blocks;
+    plan.groups = reinterpret_cast<b2a::SharedGroup*>(base + at.groups);
+    plan.seqs = reinterpret_cast<b2a::SharedSeq*>(base + at.seqs);
+    plan.total = reinterpret_cast<long long*>(base);
+    plan.err = err;
+    b2a::DecodeSharedParams s{};
+    s.block_table = block_table;
+    s.table_ld = table_ld;
+    s.table_width = table_width;
+    s.n_pages = n_pages;
+    s.page = page;
+    s.box_rows = p.box_rows;
+    s.n_groups = shared->n_groups;
+    s.Hkv = Hkv;
+    s.group = p.group;
+    s.scale_log2 = p.scale_log2;
+    s.groups = plan.groups;
+    s.total = plan.total;
+    s.part_o = reinterpret_cast<float*>(base + at.part_o);
+    s.part_ml = reinterpret_cast<float*>(base + at.part_ml);
+    s.place = reinterpret_cast<int*>(base + at.place);
+    s.n_ctas = at.n_ctas;
+    s.err = err;
+    CUtensorMap tq, sk, sv;
+    const unsigned long long dims[3] = {(unsigned long long)D, (unsigned long long)Hq, (unsigned long long)B};
+    const unsigned long long strides[2] = {(unsigned long long)qs[1] * 2, (unsigned long long)qs[0] * 2};
+    const unsigned box[3] = {64u, (unsigned)p.group, 128u / (unsigned)p.group};
+    if ((rc = b2a::api_tensor_map(&tq, q, 3, dims, strides, box)) || (rc = map(&sk, k_pages, ks, 1)) ||
+        (rc = map(&sv, v_pages, vs, 1)))
+      return rc;
+    rc = b2a::launch_decode_shared(D, tq, sk, sv, plan, s, static_cast<cudaStream_t>(stream));
+    if (rc) return status_of(rc);
+    p.seqs = plan.seqs;
+    p.shared_o = s.part_o;
+    p.shared_ml = s.part_ml;
+    p.shared_place = s.place;
+    p.block_rows = b2a::decode_shared_block_rows(D);
+    p.shared_ctas = s.n_ctas;
+  }
   return status_of(b2a::launch_decode_paged(D, tk, tv, p, static_cast<cudaStream_t>(stream)));
 }
 
@@ -310,9 +392,28 @@ int b2a_decode_paged(const void* q, const void* k_pages, const void* v_pages, co
                      int Hq, int Hkv, int n_pages, int page, int D, const long long* qs, const long long* ks,
                      const long long* vs, const long long* gs, const long long* os, int gate_bf16, float scale,
                      int out_fp32, void* workspace, size_t workspace_bytes, void* stream) {
-  return paged_attention(q, k_pages, v_pages, block_table, nullptr, nullptr, nullptr, nullptr, table_ld, table_width,
-                         seqlens, gate, o, B, Hq, Hkv, n_pages, page, D, qs, ks, vs, gs, os, gate_bf16, scale, out_fp32,
-                         workspace, workspace_bytes, stream);
+  return paged_attention(q, k_pages, v_pages, block_table, nullptr, nullptr, nullptr, nullptr, nullptr, table_ld,
+                         table_width, seqlens, gate, o, B, Hq, Hkv, n_pages, page, D, qs, ks, vs, gs, os, gate_bf16,
+                         scale, out_fp32, workspace, workspace_bytes, stream);
+}
+
+size_t b2a_decode_paged_shared_workspace_bytes(int B, int Hq, int Hkv, int D, int n_groups) {
+  const size_t own = b2a_decode_paged_workspace_bytes(B, Hq, Hkv, D);
+  return own == 0 || n_groups <= 0 ? 0 : own + shared_layout(B, Hq, Hkv, D, n_groups).bytes;
+}
+
+int b2a_decode_paged_shared(const void* q, const void* k_pages, const void* v_pages, const int* block_table,
+                            long long table_ld, int table_width, const int* seqlens, const int* prefix_lens,
+                            const int* cu_groups, int n_groups, const void* gate, void* o, int B, int Hq, int Hkv,
+                            int n_pages, int page, int D, const long long* qs, const long long* ks,
+                            const long long* vs, const long long* gs, const long long* os, int gate_bf16, float scale,
+                            int out_fp32, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!prefix_lens || n_groups <= 0 || (!cu_groups && n_groups != 1)) return B2A_ERR_INVALID_ARG;
+  if (!api_aligned(prefix_lens, 4) || !api_aligned(cu_groups, 4)) return B2A_ERR_ALIGNMENT;
+  const SharedPrefix shared{prefix_lens, cu_groups, n_groups};
+  return paged_attention(q, k_pages, v_pages, block_table, nullptr, nullptr, nullptr, nullptr, &shared, table_ld,
+                         table_width, seqlens, gate, o, B, Hq, Hkv, n_pages, page, D, qs, ks, vs, gs, os, gate_bf16,
+                         scale, out_fp32, workspace, workspace_bytes, stream);
 }
 
 int b2a_decode_paged_e4m3(const void* q, const void* k_pages, const void* v_pages, const float* k_scales,
@@ -322,8 +423,8 @@ int b2a_decode_paged_e4m3(const void* q, const void* k_pages, const void* v_page
                           const long long* vs, const long long* gs, const long long* os, int gate_bf16, float scale,
                           int out_fp32, void* workspace, size_t workspace_bytes, void* stream) {
   if (const int rc = scales_ok(k_scales, v_scales, kss, vss)) return rc;
-  return paged_attention(q, k_pages, v_pages, block_table, k_scales, v_scales, kss, vss, table_ld, table_width, seqlens,
-                         gate, o, B, Hq, Hkv, n_pages, page, D, qs, ks, vs, gs, os, gate_bf16, scale, out_fp32,
+  return paged_attention(q, k_pages, v_pages, block_table, k_scales, v_scales, kss, vss, nullptr, table_ld, table_width,
+                         seqlens, gate, o, B, Hq, Hkv, n_pages, page, D, qs, ks, vs, gs, os, gate_bf16, scale, out_fp32,
                          workspace, workspace_bytes, stream);
 }
 

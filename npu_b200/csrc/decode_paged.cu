@@ -176,7 +176,16 @@ __device__ __forceinline__ int keys_of(const DecodePagedParams& p, int b) {
   const int len = p.seqlens[b];
   return len < 0 ? 0 : (len > cap ? (int)cap : len);
 }
-__device__ __forceinline__ int tiles_of(const DecodePagedParams& p, int b) { return (keys_of(p, b) + 63) / 64; }
+// Tiles of sequence b ahead of those that the call itself attends.
+template <bool SHARED>
+__device__ __forceinline__ int tiles_ahead(const DecodePagedParams& p, int b) {
+  if constexpr (SHARED) return load_seq(p.seqs + b).skip / 64;
+  return 0;
+}
+template <bool SHARED>
+__device__ __forceinline__ int tiles_of(const DecodePagedParams& p, int b) {
+  return max((keys_of(p, b) + 63) / 64 - tiles_ahead<SHARED>(p, b), 0);
+}
 
 // The work of a pair in the units that are shared out: its tiles, and one
 // more for starting and finishing it (measured at 1 us beside 0.7 us a tile
@@ -184,12 +193,13 @@ __device__ __forceinline__ int tiles_of(const DecodePagedParams& p, int b) { ret
 __device__ __forceinline__ int units_of(int tiles) { return tiles > 0 ? tiles + 1 : 0; }
 
 // All units of the call (all lanes get it). Warp-collective.
+template <bool SHARED>
 __device__ __forceinline__ long long total_units(const DecodePagedParams& p) {
   long long n = 0;
 #pragma unroll 4
   for (int b0 = 0; b0 < p.B; b0 += 32) {
     const int b = b0 + (threadIdx.x & 31);
-    n += __reduce_add_sync(0xffffffffu, b < p.B ? units_of(tiles_of(p, b)) : 0);
+    n += __reduce_add_sync(0xffffffffu, b < p.B ? units_of(tiles_of<SHARED>(p, b)) : 0);
   }
   return n * p.Hkv;
 }
@@ -203,12 +213,14 @@ __device__ __forceinline__ long long share_of(long long total, int n_ctas) {
 }
 
 // A stretch of the units, pair by pair: the pairs with a tile in it.
+template <bool SHARED>
 struct Walk {
   long long left;  // units from this pair's first one here to the stretch's end
   int b, g;        // the pair
   int begin, t1;   // its tiles in the stretch
   int t0;          // the current one (the producer's)
   int tiles, len;  // all its tiles, its keys
+  int ahead;       // tiles of the sequence before them
   // The pairs of units [from, from + count). Warp-collective. Check valid().
   __device__ __forceinline__ Walk(const DecodePagedParams& p, long long from, long long count) {
     left = count;
@@ -216,7 +228,7 @@ struct Walk {
     if (left <= 0) return;
     const int lane = threadIdx.x & 31;
     for (int b0 = 0; b0 < p.B; b0 += 32) {
-      const int n = b0 + lane < p.B ? units_of(tiles_of(p, b0 + lane)) : 0;
+      const int n = b0 + lane < p.B ? units_of(tiles_of<SHARED>(p, b0 + lane)) : 0;
       int upto = n;  // inclusive sum over the lanes
 #pragma unroll
       for (int off = 1; off < 32; off *= 2) {
@@ -228,8 +240,7 @@ struct Walk {
         const int src = __ffs(past) - 1;
         const long long before = (long long)__shfl_sync(0xffffffffu, upto - n, src) * p.Hkv;
         b = b0 + src;
-        len = keys_of(p, b);
-        tiles = (len + 63) / 64;
+        measure(p);
         const long long into = from - before;
         g = (int)(into / units_of(tiles));
         begin = (int)(into % units_of(tiles));
@@ -242,7 +253,12 @@ struct Walk {
     if (begin == tiles) next(p);  // only the pair's extra unit is here
   }
   __device__ __forceinline__ Walk(int b_, int g_, int len_)
-      : left((len_ + 63) / 64), b(b_), g(g_), begin(0), t1((len_ + 63) / 64), t0(0), tiles(t1), len(len_) {}
+      : left((len_ + 63) / 64), b(b_), g(g_), begin(0), t1((len_ + 63) / 64), t0(0), tiles(t1), len(len_), ahead(0) {}
+  __device__ __forceinline__ void measure(const DecodePagedParams& p) {
+    len = keys_of(p, b);
+    ahead = tiles_ahead<SHARED>(p, b);
+    tiles = max((len + 63) / 64 - ahead, 0);
+  }
   __device__ __forceinline__ bool valid() const { return left > 0; }
   __device__ __forceinline__ bool next(const DecodePagedParams& p) {
     left -= units_of(tiles) - begin;
@@ -255,8 +271,7 @@ struct Walk {
           left = 0;
           return false;
         }
-        len = keys_of(p, b);
-        tiles = (len + 63) / 64;
+        measure(p);
       } while (tiles == 0);
     }
     t1 = (int)min((long long)tiles, left);
@@ -285,8 +300,8 @@ __device__ __forceinline__ uint32_t odd_e4m3(uint32_t w) {
 __device__ __forceinline__ int swizzle(int r, int d) { return d ^ (((r >> 1) & 3) << 3); }
 
 // NT blocks of 8 query heads cover a group; SPLIT: the even split above; E4M3:
-// 8-bit pools with a scale per key.
-template <int D, int NT, bool SPLIT, bool E4M3>
+// 8-bit pools with a scale per key; SHARED: keys from seqs[b].skip on (with SPLIT).
+template <int D, int NT, bool SPLIT, bool E4M3, bool SHARED>
 __global__ void __launch_bounds__(PagedCfg<D, E4M3>::THREADS, PagedCfg<D, E4M3>::CTAS_PER_SM)
     decode_paged_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                         const __grid_constant__ DecodePagedParams p) {
@@ -307,17 +322,17 @@ __global__ void __launch_bounds__(PagedCfg<D, E4M3>::THREADS, PagedCfg<D, E4M3>:
       if (p.seqlens[b] < 0 || p.seqlens[b] > (long long)p.table_width * p.page) atomicOr(p.err, kErrBadArgs);
   long long from = 0, count = 1;
   if constexpr (SPLIT) {
-    const long long total = total_units(p), share = share_of(total, p.n_ctas);
+    const long long total = total_units<SHARED>(p), share = share_of(total, p.n_ctas);
     from = blockIdx.x * share;
     count = min(share, total - from);
     if (count <= 0) return;
   }
-  auto start = [&]() -> Walk {
-    if constexpr (SPLIT) return Walk(p, from, count);
+  auto start = [&]() -> Walk<SHARED> {
+    if constexpr (SPLIT) return Walk<SHARED>(p, from, count);
     const int b = blockIdx.x / p.Hkv;
-    return Walk(b, blockIdx.x % p.Hkv, keys_of(p, b));
+    return Walk<SHARED>(b, blockIdx.x % p.Hkv, keys_of(p, b));
   };
-  Walk w = start();
+  Walk<SHARED> w = start();
   if (SPLIT && !w.valid()) return;
   if (!SPLIT && w.tiles == 0) {
     for (int e = 4 * threadIdx.x; e < p.group * D; e += 4 * C::THREADS)
@@ -353,9 +368,9 @@ __global__ void __launch_bounds__(PagedCfg<D, E4M3>::THREADS, PagedCfg<D, E4M3>:
     const int box_bytes = br * D * (E4M3 ? 1 : 2);
     // Every tile's page is looked up one tile ahead, across pairs too, and
     // checked when its turn comes (so that nothing waits for the lookup).
-    auto has_keys = [&]() { return mine && w.t0 * C::TK + box * br < w.len; };
+    auto has_keys = [&]() { return mine && (w.ahead + w.t0) * C::TK + box * br < w.len; };
     auto entry_of = [&]() -> int {  // table entry of this lane's box in tile w.t0
-      return has_keys() ? p.block_table[w.b * p.table_ld + (w.t0 * C::TK + box * br) / p.page] : 0;
+      return has_keys() ? p.block_table[w.b * p.table_ld + ((w.ahead + w.t0) * C::TK + box * br) / p.page] : 0;
     };
     int n = 0, pairs = 0;  // tiles and pairs copied so far
     bool more = true, new_pair = true;
@@ -363,7 +378,7 @@ __global__ void __launch_bounds__(PagedCfg<D, E4M3>::THREADS, PagedCfg<D, E4M3>:
     bool copy = has_keys();
     while (more) {
       const int slot = n % C::STAGES;
-      const int g = w.g, row = (w.t0 * C::TK + box * br) % p.page;
+      const int g = w.g, row = ((w.ahead + w.t0) * C::TK + box * br) % p.page;
       const __nv_bfloat16* q = p.q + w.b * p.q_sb + (long long)(g * p.group + lane) * p.q_sh;
       const bool with_q = new_pair;
       ++w.t0;
@@ -481,7 +496,7 @@ __global__ void __launch_bounds__(PagedCfg<D, E4M3>::THREADS, PagedCfg<D, E4M3>:
         }
         const uint32_t kbase = smem_u32(smem + slot * C::STAGE_BYTES) + wbase;
         const uint32_t vbase = kbase + C::TILE_BYTES;
-        const int have = w.len - (t * C::TK + 16 * warp);  // keys of this warp's 16 that exist
+        const int have = w.len - ((w.ahead + t) * C::TK + 16 * warp);  // keys of this warp's 16 that exist
         if (have > 0) {
           float s[NT][4];
 #pragma unroll
@@ -700,7 +715,9 @@ constexpr int kJoinThreads = 256;
 // the wait, to fetch the instructions, gained nothing (4 to 4096 sequences of
 // 500 to 1500 keys, 32 / 4 heads of 128: 9.5 us to 1.77 ms without, 9.5 us to
 // 1.80 ms with it).
-template <int D>
+// SHARED: the parts over the shared keys come after those, numbered and placed
+// alike.
+template <int D, bool SHARED>
 __global__ void __launch_bounds__(kJoinThreads) decode_paged_join_kernel(const __grid_constant__ DecodePagedParams p) {
   constexpr int TEAM = D / 4, TEAMS = kJoinThreads / TEAM;
   __shared__ float4 s_o[TEAMS][TEAM];
@@ -714,23 +731,39 @@ __global__ void __launch_bounds__(kJoinThreads) decode_paged_join_kernel(const _
   const int2 at = __ldcg(reinterpret_cast<const int2*>(p.place) + pair);
   const float4 gate = p.gate && team == 0 ? load_gate(p, b, h, d) : zero4();
   int c0 = 0, parts = 0;
-  if (keys_of(p, b) > 0) {
+  if (tiles_of<SHARED>(p, b) > 0) {
     // (Within the CTAs there are, even if the lengths changed under the call.)
     c0 = max(0, min(at.x, p.n_ctas - 1));
     parts = min(at.y, p.n_ctas - 1) - c0 + 1;
   }
   const long long row0 = (pair + c0) * p.group + r;  // part i's row: row0 + i group
+  int more = 0;  // parts over shared keys
+  long long shared0 = 0;
+  if constexpr (SHARED) {
+    const SharedSeq s = load_seq(p.seqs + b);
+    if (s.skip > 0) {
+      const long long item = (long long)s.block * p.Hkv + g;
+      const int2 of = __ldcg(reinterpret_cast<const int2*>(p.shared_place) + item);
+      const int first = max(0, min(of.x, p.shared_ctas - 1));
+      more = min(of.y, p.shared_ctas - 1) - first + 1;
+      shared0 = (item + first) * p.block_rows + s.row + r;
+    }
+  }
   float m = -INFINITY, l = 0.f;
   float4 o = zero4();
-  for (int i0 = team; i0 < parts; i0 += 4 * TEAMS) {
+  for (int i0 = team; i0 < parts + more; i0 += 4 * TEAMS) {
     float2 ml[4];
     float4 po[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const int i = i0 + k * TEAMS;
-      const long long row = row0 + (long long)i * p.group;
-      ml[k] = i < parts ? __ldcg(reinterpret_cast<const float2*>(p.part_ml + 2 * row)) : make_float2(-INFINITY, 0.f);
-      po[k] = i < parts ? __ldcg(reinterpret_cast<const float4*>(p.part_o + row * D + d)) : zero4();
+      const bool own = !SHARED || i < parts;
+      const long long row = own ? row0 + (long long)i * p.group : shared0 + (long long)(i - parts) * p.block_rows;
+      const float* part_ml = own ? p.part_ml : p.shared_ml;
+      const float* part_o = own ? p.part_o : p.shared_o;
+      const bool there = i < parts + more;
+      ml[k] = there ? __ldcg(reinterpret_cast<const float2*>(part_ml + 2 * row)) : make_float2(-INFINITY, 0.f);
+      po[k] = there ? __ldcg(reinterpret_cast<const float4*>(part_o + row * D + d)) : zero4();
     }
     const float mn = fmaxf(fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)), m);
     const float mu = mn == -INFINITY ? 0.f : mn;
@@ -770,7 +803,7 @@ __global__ void __launch_bounds__(kJoinThreads) decode_paged_join_kernel(const _
 
 constexpr int kWholeTiles = 8;
 
-template <int D, int NT, bool SPLIT, bool E4M3>
+template <int D, int NT, bool SPLIT, bool E4M3, bool SHARED = false>
 int launch_main(const CUtensorMap& tk, const CUtensorMap& tv, const DecodePagedParams& p, long long n,
                 cudaStream_t st) {
   using C = PagedCfg<D, E4M3>;
@@ -778,11 +811,11 @@ int launch_main(const CUtensorMap& tk, const CUtensorMap& tv, const DecodePagedP
   if (n > 0x7fffffffLL) return -1;
   return once.run(
       [] {
-        return cudaFuncSetAttribute(decode_paged_kernel<D, NT, SPLIT, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+        return cudaFuncSetAttribute(decode_paged_kernel<D, NT, SPLIT, E4M3, SHARED>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                     C::SMEM_BYTES) == cudaSuccess;
       },
       [&] {
-        return launch_dependent(decode_paged_kernel<D, NT, SPLIT, E4M3>, dim3((unsigned)n), C::THREADS, C::SMEM_BYTES, st, 0,
+        return launch_dependent(decode_paged_kernel<D, NT, SPLIT, E4M3, SHARED>, dim3((unsigned)n), C::THREADS, C::SMEM_BYTES, st, 0,
                                 tk, tv, p);
       });
 }
@@ -803,11 +836,15 @@ int launch_t(const CUtensorMap& tk, const CUtensorMap& tv, const DecodePagedPara
     return launch_n<D, false>(tk, tv, p, (long long)p.B * p.Hkv, st);
   const long long heads = (long long)p.B * p.Hq;
   if (heads > 0x7fffffffLL) return -2;
-  const int rc = launch_n<D, true>(tk, tv, p, p.n_ctas, st);
+  int rc;
+  if (p.seqs)
+    rc = p.group <= 8 ? launch_main<D, 1, true, false, true>(tk, tv, p, p.n_ctas, st)
+                      : launch_main<D, 2, true, false, true>(tk, tv, p, p.n_ctas, st);
+  else
+    rc = launch_n<D, true>(tk, tv, p, p.n_ctas, st);
   if (rc) return rc;
-  return launch_dependent(decode_paged_join_kernel<D>, dim3((unsigned)heads), kJoinThreads, 0, st, 0, p) == cudaSuccess
-             ? 0
-             : -1;
+  const auto join = p.seqs ? decode_paged_join_kernel<D, true> : decode_paged_join_kernel<D, false>;
+  return launch_dependent(join, dim3((unsigned)heads), kJoinThreads, 0, st, 0, p) == cudaSuccess ? 0 : -1;
 }
 
 }  // namespace

@@ -6,6 +6,20 @@
 
 namespace b2a {
 
+// A sequence whose first `skip` keys (a multiple of 64) are attended together
+// with others' (decode_shared.cu): where the partials of its query heads are.
+struct alignas(16) SharedSeq {
+  int skip;   // 0: none
+  int block;  // row block
+  int row;    // its first row there
+  int pad;
+};
+
+__device__ __forceinline__ SharedSeq load_seq(const SharedSeq* p) {  // past L1, see decode_shared.cuh
+  const int4 w = __ldcg(reinterpret_cast<const int4*>(p));
+  return SharedSeq{w.x, w.y, w.z, w.w};
+}
+
 struct DecodePagedParams {
   const __nv_bfloat16* q;  // [B, Hq, D]
   long long q_sb, q_sh;
@@ -33,6 +47,14 @@ struct DecodePagedParams {
   float* part_ml;
   int* place;        // [B Hkv, 2]: the CTAs with a pair's first and last tile
   int n_ctas;
+  // Shared form: with seqs, this call attends the keys from seqs[b].skip on, and
+  // the joining kernel adds the partials of the shared ones, numbered and placed
+  // alike (item block Hkv + g, rows of block_rows, CTAs up to shared_ctas).
+  const SharedSeq* seqs;
+  const float* shared_o;
+  const float* shared_ml;
+  const int* shared_place;
+  int block_rows, shared_ctas;
   int* err;
 };
 

@@ -220,6 +220,55 @@ Tensor decode_paged(const Tensor& q, const Tensor& k_pages, const Tensor& v_page
   return o;
 }
 
+Tensor decode_paged_shared(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table,
+                           const Tensor& seqlens, const Tensor& prefix_lens, const OptTensor& cu_groups,
+                           std::optional<double> scale, at::ScalarType out_dtype, const OptTensor& workspace,
+                           const OptTensor& out, const OptTensor& gate) {
+  need_bf16("q", q, 3);
+  const c10::Device device = q.device();
+  need_bf16("k_pages", k_pages, 4, &device);
+  need_bf16("v_pages", v_pages, 4, &device);
+  const int64_t B = q.size(0), Hq = q.size(1), D = q.size(2), Hkv = k_pages.size(1),
+                groups = cu_groups ? cu_groups->numel() - 1 : 1;
+  if (k_pages.size(3) != D || v_pages.sizes() != k_pages.sizes())
+    refuse("shape mismatch q", q.sizes(), " k_pages", k_pages.sizes(), " v_pages", v_pages.sizes());
+  need_table(table, B, device);
+  need_int32("seqlens", seqlens, B, device);
+  if (groups < 1) refuse("cu_groups must hold at least two offsets");
+  if (cu_groups) need_int32("cu_groups", *cu_groups, groups + 1, device);
+  need_int32("prefix_lens", prefix_lens, groups, device);
+  float_type("out_dtype", out_dtype);
+  if (gate) need_gate(*gate, q);
+  const c10::cuda::CUDAGuard guard(device);
+  Tensor o = output(out, q.sizes(), out_dtype, q,
+                    "out must match [B, Hq, D], out_dtype and q's device, with a contiguous last dim");
+  if (B == 0) return o;
+  const size_t need = b2a_decode_paged_shared_workspace_bytes(as_int("B", B), as_int("Hq", Hq), as_int("Hkv", Hkv),
+                                                              as_int("D", D), as_int("groups", groups));
+  c10::DataPtr taken;  // as in decode_paged
+  void* ws;
+  if (workspace) {
+    if (workspace->device() != device || !workspace->is_contiguous() || workspace->nbytes() < need)
+      refuse("workspace must be a contiguous CUDA tensor of at least ", need, " bytes on q's device");
+    ws = workspace->data_ptr();
+  } else {
+    taken = c10::cuda::CUDACachingAllocator::get()->allocate(std::max<size_t>(need, 16));
+    ws = taken.get();
+  }
+  const Strides gs(gate ? *gate : q, 2);
+  check(b2a_decode_paged_shared(q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), table.data_ptr<int>(),
+                                table.stride(0), as_int("table width", table.size(1)), seqlens.data_ptr<int>(),
+                                prefix_lens.data_ptr<int>(), static_cast<int*>(pointer(cu_groups)), (int)groups,
+                                pointer(gate), o.data_ptr(), (int)B, (int)Hq, (int)Hkv,
+                                as_int("n_pages", k_pages.size(0)), as_int("page", k_pages.size(2)), (int)D,
+                                Strides(q, 2), Strides(k_pages, 3), Strides(v_pages, 3), gs, Strides(o, 2),
+                                gate && gate->scalar_type() == at::kBFloat16,
+                                (float)scale.value_or(1.0 / std::sqrt((double)D)), out_dtype == at::kFloat, ws, need,
+                                stream_of(q)),
+        "b2a_decode_paged_shared");
+  return o;
+}
+
 py::object rope_append_paged(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cos, const Tensor& sin,
                              const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& cu,
                              int64_t start_pos, const OptTensor& start, const OptTensor& seqlens_out,
@@ -436,6 +485,7 @@ Tensor penalize(const Tensor& logits, const OptTensor& tokens, const OptTensor& 
 PYBIND11_MODULE(_serving, m) {
   m.def("prefill_varlen", &prefill_varlen);
   m.def("decode_paged", &decode_paged);
+  m.def("decode_paged_shared", &decode_paged_shared);
   m.def("rope_append_paged", &rope_append_paged);
   m.def("gather_paged", &gather_paged);
   m.def("penalize", &penalize);
