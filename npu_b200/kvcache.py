@@ -15,7 +15,8 @@ the first on the device. The buffers never move, so a step can be captured in
 a CUDA graph and replayed.
 
 PagedKVCache keeps sequences of different lengths in pages of one pool instead
-(npu_b200.api.rope_append_paged, prefill_varlen and decode_paged).
+(npu_b200.api.rope_append_paged, prefill_varlen and decode_paged), in bf16 or 8
+bits; sequences may start with the pages of another (a shared prefix).
 """
 from __future__ import annotations
 
@@ -74,18 +75,26 @@ class PagedKVCache:
     Hkv, page, head_dim] bf16 on `device`. Sequences take pages as they need
     them and give them back (`reserve`, `PagedSequences.release`), so the memory
     held follows the tokens stored instead of batch x longest. The pools are
-    allocated once and never cleared: a page's old contents are not read.
+    allocated once and never cleared: a page's old contents are not read. With
+    dtype torch.float8_e4m3fn they are 8-bit, with a scale for each token and KV
+    head in k_scales, v_scales [n_layers, n_pages, Hkv, page] (rope_append_paged).
     """
 
     def __init__(self, n_layers: int, n_pages: int, n_kv_heads: int, page: int, head_dim: int,
-                 device: torch.device):
+                 device: torch.device, dtype: torch.dtype = torch.bfloat16):
         if min(n_layers, n_pages, n_kv_heads, page, head_dim) <= 0:
             raise ValueError("PagedKVCache dimensions must be positive")
         if page % 16:
             raise ValueError(f"page must be a multiple of 16 tokens, got {page}")
         shape = (n_layers, n_pages, n_kv_heads, page, head_dim)
-        self.k = torch.empty(shape, dtype=torch.bfloat16, device=device)
-        self.v = torch.empty(shape, dtype=torch.bfloat16, device=device)
+        if dtype not in (torch.bfloat16, torch.float8_e4m3fn):
+            raise ValueError(f"the pools are bfloat16 or float8_e4m3fn, got {dtype}")
+        self.k = torch.empty(shape, dtype=dtype, device=device)
+        self.v = torch.empty(shape, dtype=dtype, device=device)
+        self.k_scales = self.v_scales = None
+        if dtype == torch.float8_e4m3fn:
+            self.k_scales = torch.empty(shape[:-1], dtype=torch.float32, device=device)
+            self.v_scales = torch.empty(shape[:-1], dtype=torch.float32, device=device)
         self.page = page
         self.device = self.k.device
         self._free = list(range(n_pages - 1, -1, -1))
@@ -97,32 +106,51 @@ class PagedKVCache:
     def layer(self, i: int):
         return self.k[i], self.v[i]
 
-    def reserve(self, capacities) -> "PagedSequences":
-        """Pages for len(capacities) new, empty sequences of at most that many tokens each."""
+    def scales(self, i: int) -> dict:
+        """Layer i's k_scales and v_scales as the operators' arguments (none of a bf16 cache)."""
+        return {} if self.k_scales is None else dict(k_scales=self.k_scales[i], v_scales=self.v_scales[i])
+
+    def reserve(self, capacities, prefix: "PagedSequences" = None) -> "PagedSequences":
+        """Pages for len(capacities) new, empty sequences of at most that many tokens each. With `prefix`, one
+        sequence of this cache whose capacity is whole pages and full, all of them go on from its tokens: its pages
+        are the first of each (not counted in capacities), and it cannot be released before them."""
+        if prefix is not None and (prefix.cache is not self or prefix.batch != 1 or prefix.released
+                                   or prefix.prefix is not None or prefix.capacities[0] % self.page):
+            raise ValueError("prefix must be one unreleased sequence of this cache with whole pages and no prefix itself")
         capacities = [int(c) for c in capacities]
         if not capacities or min(capacities) < 1:
             raise ValueError("capacities must be one or more positive token counts")
         counts = [-(-c // self.page) for c in capacities]
         if sum(counts) > len(self._free):
             raise ValueError(f"{sum(counts)} pages are needed and {len(self._free)} are free")
-        return PagedSequences(self, [[self._free.pop() for _ in range(n)] for n in counts])
+        return PagedSequences(self, [[self._free.pop() for _ in range(n)] for n in counts], capacities, prefix)
 
 
 class PagedSequences:
     """A batch of sequences in a PagedKVCache: their block table and, like
     KVCache, two vectors of positions on the device, so that steps need no host
     synchronisation. `start`: the next token's position; `end`: the lengths
-    after the step in progress; `advance` finishes a step."""
+    after the step in progress; `advance` finishes a step. Sequences behind a
+    shared prefix start after its prefix_tokens tokens; prefix_lens holds that
+    number on the device."""
 
-    def __init__(self, cache: PagedKVCache, pages: list):
+    def __init__(self, cache: PagedKVCache, pages: list, capacities: list, prefix: "PagedSequences" = None):
         self.cache, self._pages = cache, pages
-        self.batch = len(pages)
+        self.batch, self.capacities = len(pages), capacities
+        self.prefix, self.followers = prefix, 0
+        shared = [] if prefix is None else prefix._pages[0]
+        self.prefix_tokens = len(shared) * cache.page
+        if prefix is not None:
+            prefix.followers += 1
         # -1 is no page: a token past a sequence's own pages is left out and reported.
-        table = torch.full((self.batch, max(len(p) for p in pages)), -1, dtype=torch.int32)
+        table = torch.full((self.batch, len(shared) + max(len(p) for p in pages)), -1, dtype=torch.int32)
         for b, p in enumerate(pages):
-            table[b, :len(p)] = torch.tensor(p, dtype=torch.int32)
+            table[b, :len(shared) + len(p)] = torch.tensor(shared + p, dtype=torch.int32)
         self.block_table = table.to(cache.device)
-        self._pos = torch.zeros((2, self.batch), dtype=torch.int32, device=cache.device)
+        self._pos = torch.full((2, self.batch), self.prefix_tokens, dtype=torch.int32, device=cache.device)
+        self.prefix_lens = None
+        if prefix is not None:
+            self.prefix_lens = torch.tensor([self.prefix_tokens], dtype=torch.int32, device=cache.device)
         # Offsets of a step of one token per sequence.
         self.one_each = torch.arange(self.batch + 1, dtype=torch.int32, device=cache.device)
 
@@ -149,6 +177,10 @@ class PagedSequences:
     def release(self) -> None:
         """Give the pages back. Work already queued on the current stream may
         still read them; later owners are to use the same stream."""
+        if self.followers:
+            raise ValueError(f"{self.followers} batches of sequences still go on from these pages")
+        if self.prefix is not None and not self.released:
+            self.prefix.followers -= 1
         for p in self._pages:
             self.cache._free.extend(reversed(p))
         self._pages = []

@@ -15,8 +15,10 @@ run_batch. Here the same layer math runs as:
 
 Prompts of different lengths run packed instead of padded (prefill_packed,
 decode_packed, generate): b2a_rope_append_paged writes k and v to the pages of
-each sequence, b2a_prefill_varlen and b2a_decode_paged attend, b2a_sample
-chooses the tokens.
+each sequence (bf16 or 8-bit), b2a_prefill_varlen and b2a_decode_paged attend,
+b2a_penalize and b2a_sample choose the tokens. Behind a shared prefix, whose
+pages all sequences name, prompts attend the cached keys that b2a_gather_paged
+reads back, and single tokens go through b2a_decode_paged_shared.
 
 Sequence positions stay on the device (KVCache), so a decode step issues no
 host synchronisation. Weights use the reference's HF key names
@@ -245,8 +247,9 @@ class SmolLMB200:
         return F.linear(x, self.embed)
 
     # ------------------------------------------------------------ sequences of different lengths
-    def new_paged_cache(self, n_pages: int, page: int = 64) -> PagedKVCache:
-        return PagedKVCache(self.cfg.n_layers, n_pages, self.cfg.n_kv_heads, page, self.cfg.head_dim, self.device)
+    def new_paged_cache(self, n_pages: int, page: int = 64, dtype: torch.dtype = torch.bfloat16) -> PagedKVCache:
+        """dtype torch.float8_e4m3fn: an 8-bit cache, about half the memory and traffic."""
+        return PagedKVCache(self.cfg.n_layers, n_pages, self.cfg.n_kv_heads, page, self.cfg.head_dim, self.device, dtype)
 
     def _attention_packed(self, lw: dict, h: torch.Tensor, seqs: PagedSequences, i: int,
                           cu_seqlens: Optional[torch.Tensor]) -> torch.Tensor:
@@ -262,16 +265,26 @@ class SmolLMB200:
         k = qkv[:, Hq * Dh:(Hq + Hkv) * Dh].view(N, Hkv, Dh)
         v = qkv[:, (Hq + Hkv) * Dh:].view(N, Hkv, Dh)
         k_pages, v_pages = seqs.cache.layer(i)
+        scales = seqs.cache.scales(i)
         prompts = cu_seqlens is not None
         with profile("rope"):
             rot = api.rope_append_paged(q, k, v, self.cos, self.sin, k_pages, v_pages, seqs.block_table,
                                         cu_seqlens if prompts else seqs.one_each, start_pos_per_batch=seqs.start,
-                                        seqlens_out=seqs.end, return_kv=prompts)
+                                        seqlens_out=seqs.end, return_kv=prompts, **scales)
         with profile("attn"):
-            if prompts:
+            if prompts and seqs.prefix_tokens:
+                # The prefix's keys and the prompt's own, both as the cache holds them.
+                cu_k = cu_seqlens + seqs.prefix_tokens * seqs.one_each
+                kv = api.gather_paged(k_pages, v_pages, seqs.block_table, cu_k, N + seqs.batch * seqs.prefix_tokens,
+                                      **scales)
+                o = api.prefill_varlen(rot[0], *kv, cu_seqlens, cu_k, out_dtype=h.dtype)
+            elif prompts:
                 o = api.prefill_varlen(*rot, cu_seqlens, out_dtype=h.dtype)
+            elif seqs.prefix_tokens and not scales:
+                o = api.decode_paged_shared(rot, k_pages, v_pages, seqs.block_table, seqs.end, seqs.prefix_lens,
+                                            out_dtype=h.dtype)
             else:
-                o = api.decode_paged(rot, k_pages, v_pages, seqs.block_table, seqs.end, out_dtype=h.dtype)
+                o = api.decode_paged(rot, k_pages, v_pages, seqs.block_table, seqs.end, out_dtype=h.dtype, **scales)
         return o.view(N, Hq * Dh)
 
     def _forward_packed(self, ids: torch.Tensor, seqs: PagedSequences,
@@ -300,7 +313,8 @@ class SmolLMB200:
     def prefill_packed(self, ids: torch.Tensor, cu_seqlens: torch.Tensor, seqs: PagedSequences) -> torch.Tensor:
         """Logits [B, vocab] of each prompt's last token, for prompts packed in
         ids [N] (sequence b: ids[cu_seqlens[b] : cu_seqlens[b + 1]], none empty)
-        into the new, empty sequences `seqs`. Of offsets that are not a stretch
+        into the new, empty sequences `seqs` (behind their shared prefix, if they
+        have one: its tokens are in the cache already). Of offsets that are not a stretch
         of ids the logits mean nothing; api.device_error() reports them."""
         if ids.dim() != 1 or cu_seqlens.numel() != seqs.batch + 1:
             raise ValueError("ids must be [N] and cu_seqlens [B + 1] with B = seqs.batch")
@@ -320,31 +334,52 @@ class SmolLMB200:
     @torch.no_grad()
     def generate(self, prompts, max_new_tokens: int, *, cache: Optional[PagedKVCache] = None, page: int = 64,
                  temperature=0.0, top_k=0, top_p=1.0, min_p=0.0,
-                 generator: Optional[torch.Generator] = None) -> torch.Tensor:
+                 generator: Optional[torch.Generator] = None, prefix=None, repetition_penalty=1.0,
+                 frequency_penalty=0.0, presence_penalty=0.0, logit_bias: Optional[torch.Tensor] = None,
+                 allowed: Optional[torch.Tensor] = None) -> torch.Tensor:
         """max_new_tokens tokens after each prompt (a list of token lists, of
         any lengths from 1), int64 [B, max_new_tokens] on the device. The
         settings are those of api.sample; temperature 0 is greedy. A prompt
         whose logits hold no usable one gives -1 there and in the rest of its
-        row. Nothing synchronises with the host in between."""
+        row. Nothing synchronises with the host in between.
+
+        prefix: tokens ahead of every prompt (a system prompt), run and stored
+        once: their whole pages are shared. The penalties, logit_bias (bias)
+        and allowed are those of api.penalize, over the prefix, the prompt and
+        what was generated."""
         lens = [len(p) for p in prompts]
         if not lens or min(lens) < 1 or max_new_tokens < 1:
             raise ValueError("every prompt needs a token and max_new_tokens must be positive")
         flat = [int(t) for p in prompts for t in p]
-        if min(flat) < 0 or max(flat) >= self.embed.shape[0]:
+        prefix = [] if prefix is None else [int(t) for t in prefix]
+        if min(flat + prefix) < 0 or max(flat + prefix) >= self.embed.shape[0]:
             raise ValueError(f"prompt tokens must lie in the vocabulary, 0 to {self.embed.shape[0] - 1}")
         room = [n + max_new_tokens - 1 for n in lens]  # the last token is not fed back
-        if max(room) > self.cfg.max_pos:
-            raise ValueError(f"{max(room)} positions exceed the rotary table length {self.cfg.max_pos}")
+        if max(room) + len(prefix) > self.cfg.max_pos:
+            raise ValueError(f"{max(room) + len(prefix)} positions exceed the rotary table length {self.cfg.max_pos}")
+        page = page if cache is None else cache.page
+        shared = len(prefix) // page * page
+        prompts = [prefix[shared:] + [int(t) for t in p] for p in prompts]
+        lens, room = [len(p) for p in prompts], [r + len(prefix) - shared for r in room]
         if cache is None:
-            cache = self.new_paged_cache(sum(-(-r // page) for r in room), page)
-        seqs = cache.reserve(room)
+            cache = self.new_paged_cache(shared // page + sum(-(-r // page) for r in room), page)
+        head = cache.reserve([shared]) if shared else None
+        seqs = None
         try:
+            seqs = cache.reserve(room, prefix=head)
             cu = torch.tensor([0] + lens, dtype=torch.int32).cumsum(0, dtype=torch.int32).to(self.device)
-            ids = torch.tensor(flat, dtype=torch.long, device=self.device)
+            ids = torch.tensor([t for p in prompts for t in p], dtype=torch.long, device=self.device)
             greedy = not isinstance(temperature, torch.Tensor) and temperature <= 0
             out = torch.empty((max_new_tokens, len(lens)), dtype=torch.long, device=self.device)
+            adjust = self._penalties([prefix[:shared] + p for p in prompts], max_new_tokens, repetition_penalty,
+                                     frequency_penalty, presence_penalty, logit_bias, allowed)
+            if shared:
+                self.prefill_packed(torch.tensor(prefix[:shared], dtype=torch.long, device=self.device),
+                                    torch.tensor([0, shared], dtype=torch.int32, device=self.device), head)
             logits = self.prefill_packed(ids, cu, seqs)
             for step in range(max_new_tokens):
+                if adjust is not None:
+                    logits = adjust(logits, out[step - 1] if step else None)
                 noise = None if greedy else torch.empty(logits.shape, dtype=torch.float32,
                                                         device=self.device).exponential_(generator=generator)
                 with profile("sample"):
@@ -355,5 +390,35 @@ class SmolLMB200:
                 if step + 1 < max_new_tokens:
                     logits = self.decode_packed(out[step].clamp(min=0), seqs)
         finally:
-            seqs.release()
+            if seqs is not None:
+                seqs.release()
+            if head is not None:
+                head.release()
         return out.T.contiguous()
+
+    def _penalties(self, prompts: list, new_tokens: int, repetition, frequency, presence, bias, allowed):
+        """adjust(logits, the tokens of the step before) -> logits for generate, or None if nothing applies."""
+        def off(value, neutral):
+            return not isinstance(value, torch.Tensor) and value == neutral
+
+        if off(repetition, 1.0) and off(frequency, 0.0) and off(presence, 0.0):
+            if bias is None and allowed is None:
+                return None
+            return lambda logits, last: api.penalize(logits, bias=bias, allowed=allowed, out=logits)
+        lens = [len(p) for p in prompts]
+        history = torch.full((len(lens), max(lens) + new_tokens), -1, dtype=torch.long)
+        for b, p in enumerate(prompts):
+            history[b, :len(p)] = torch.tensor(p, dtype=torch.long)
+        history = history.to(self.device)
+        prompt_lengths = torch.tensor(lens, dtype=torch.int32, device=self.device)
+        lengths = prompt_lengths.clone()
+
+        def adjust(logits, last):
+            if last is not None:
+                history.scatter_(1, lengths[:, None].long(), last[:, None])
+                lengths.add_(1)
+            with profile("penalize"):
+                return api.penalize(logits, history, lengths, prompt_lengths=prompt_lengths, repetition=repetition,
+                                    frequency=frequency, presence=presence, bias=bias, allowed=allowed, out=logits)
+
+        return adjust
