@@ -167,7 +167,7 @@ int paged_attention(const void* q, const void* k_pages, const void* v_pages, con
   p.group = Hq / Hkv;
   p.scale_log2 = scale * b2a::kApiLog2e;
   p.err = err;
-  p.n_ctas = b2a::decode_paged_max_ctas(D, b2a::api_sm_count());
+  p.n_ctas = b2a::decode_paged_max_ctas(D, p.group, k_scales != nullptr, b2a::api_sm_count());
   const size_t rows = b2a::decode_paged_parts(B, Hkv, p.n_ctas) * p.group;
   char* scratch = static_cast<char*>(workspace);
   p.part_o = reinterpret_cast<float*>(scratch);
@@ -382,7 +382,9 @@ int b2a_prefill_varlen(const void* q, const void* k, const void* v, const void* 
 
 size_t b2a_decode_paged_workspace_bytes(int B, int Hq, int Hkv, int D) {
   if (B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || Hq / Hkv > 16 || !head_dim_ok(D)) return 0;
-  const size_t rows = b2a::decode_paged_parts(B, Hkv, b2a::decode_paged_max_ctas(D, b2a::api_sm_count())) * (Hq / Hkv);
+  // Of either cache: 8-bit calls use no fewer CTAs.
+  const int group = Hq / Hkv, ctas = b2a::decode_paged_max_ctas(D, group, true, b2a::api_sm_count());
+  const size_t rows = b2a::decode_paged_parts(B, Hkv, ctas) * group;
   return b2a::api_align256(rows * D * sizeof(float)) + b2a::api_align256(rows * 2 * sizeof(float)) +
          (size_t)B * Hkv * 2 * sizeof(int);
 }

@@ -43,29 +43,31 @@ namespace b2a {
 
 namespace {
 
-template <int D, bool E4M3>
+template <int D, int NT, bool E4M3>
 struct PagedCfg {
-  static constexpr int TK = 64;  // keys per tile
+  // Blocks of 16 keys that a warp takes of a tile. 8-bit tiles come twice as
+  // fast, and with two blocks a warp has two chains of instructions to run and
+  // one maximum to find (128 sequences of 1024 to 32768 keys, 32 / 4 heads of
+  // 128: 294 us with one block, 235 with two).
+  static constexpr int KB = E4M3 ? 2 : 1;
+  static constexpr int TK = 64 * KB;  // keys per tile
   static constexpr int TILE_BYTES = TK * D * (E4M3 ? 1 : 2);  // K or V tile
   static constexpr int STAGE_BYTES = 2 * TILE_BYTES;
-  static constexpr int STAGES = (D == 64 ? 6 : 3) * (E4M3 ? 2 : 1);
-  static constexpr int CTAS_PER_SM = D == 256 ? 1 : 2;
+  static constexpr int CTAS_PER_SM = decode_paged_ctas_per_sm(D, NT, E4M3);
+  static constexpr int STAGES = D == 64 ? (CTAS_PER_SM == 3 ? 4 : 6) : 3;
   static constexpr int Q_ROW = D * 2 + 16;  // bytes; the 16 keep ldmatrix rows apart
   static constexpr int OFF_Q = STAGES * STAGE_BYTES;
   static constexpr int OFF_SCALES = OFF_Q + 2 * 16 * Q_ROW;  // two pairs' query heads; [STAGES][K, V][TK] fp32
   static constexpr int OFF_BAR = OFF_SCALES + (E4M3 ? STAGES * 2 * TK * 4 : 0);
   static constexpr int SMEM_BYTES = OFF_BAR + 1024 + 1024;  // barriers and m, l; alignment slack
   static constexpr int THREADS = 160;  // 4 compute warps + 1 producer warp
-  // The four warps' outputs are merged in one stage, this many heads at a time.
-  static constexpr int MERGE = E4M3 ? 8 : 16;
-  static_assert(4 * MERGE * D * 4 <= STAGE_BYTES, "the four warps' outputs are merged in one stage");
-  static_assert(STAGES <= 12, "PagedBars");
+  static_assert(4 * 16 * D * 4 <= STAGE_BYTES, "the four warps' outputs are merged in one stage");
   static_assert((SMEM_BYTES + 1024) * CTAS_PER_SM <= 233472, "shared memory budget");
 };
 
 struct PagedBars {
-  uint64_t full[12];
-  uint64_t empty[12];
+  uint64_t full[8];
+  uint64_t empty[8];
   uint64_t q_full[2];
   uint64_t q_empty[2];
   int abort_flag;
@@ -76,6 +78,14 @@ struct PagedBars {
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void mma16816_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
       "{%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -176,15 +186,15 @@ __device__ __forceinline__ int keys_of(const DecodePagedParams& p, int b) {
   const int len = p.seqlens[b];
   return len < 0 ? 0 : (len > cap ? (int)cap : len);
 }
-// Tiles of sequence b ahead of those that the call itself attends.
-template <bool SHARED>
+// Tiles of sequence b ahead of those that the call itself attends (TK: keys of a tile).
+template <int TK, bool SHARED>
 __device__ __forceinline__ int tiles_ahead(const DecodePagedParams& p, int b) {
-  if constexpr (SHARED) return load_seq(p.seqs + b).skip / 64;
+  if constexpr (SHARED) return load_seq(p.seqs + b).skip / TK;
   return 0;
 }
-template <bool SHARED>
+template <int TK, bool SHARED>
 __device__ __forceinline__ int tiles_of(const DecodePagedParams& p, int b) {
-  return max((keys_of(p, b) + 63) / 64 - tiles_ahead<SHARED>(p, b), 0);
+  return max((keys_of(p, b) + TK - 1) / TK - tiles_ahead<TK, SHARED>(p, b), 0);
 }
 
 // The work of a pair in the units that are shared out: its tiles, and one
@@ -193,13 +203,13 @@ __device__ __forceinline__ int tiles_of(const DecodePagedParams& p, int b) {
 __device__ __forceinline__ int units_of(int tiles) { return tiles > 0 ? tiles + 1 : 0; }
 
 // All units of the call (all lanes get it). Warp-collective.
-template <bool SHARED>
+template <int TK, bool SHARED>
 __device__ __forceinline__ long long total_units(const DecodePagedParams& p) {
   long long n = 0;
 #pragma unroll 4
   for (int b0 = 0; b0 < p.B; b0 += 32) {
     const int b = b0 + (threadIdx.x & 31);
-    n += __reduce_add_sync(0xffffffffu, b < p.B ? units_of(tiles_of<SHARED>(p, b)) : 0);
+    n += __reduce_add_sync(0xffffffffu, b < p.B ? units_of(tiles_of<TK, SHARED>(p, b)) : 0);
   }
   return n * p.Hkv;
 }
@@ -213,7 +223,7 @@ __device__ __forceinline__ long long share_of(long long total, int n_ctas) {
 }
 
 // A stretch of the units, pair by pair: the pairs with a tile in it.
-template <bool SHARED>
+template <int TK, bool SHARED>
 struct Walk {
   long long left;  // units from this pair's first one here to the stretch's end
   int b, g;        // the pair
@@ -228,7 +238,7 @@ struct Walk {
     if (left <= 0) return;
     const int lane = threadIdx.x & 31;
     for (int b0 = 0; b0 < p.B; b0 += 32) {
-      const int n = b0 + lane < p.B ? units_of(tiles_of<SHARED>(p, b0 + lane)) : 0;
+      const int n = b0 + lane < p.B ? units_of(tiles_of<TK, SHARED>(p, b0 + lane)) : 0;
       int upto = n;  // inclusive sum over the lanes
 #pragma unroll
       for (int off = 1; off < 32; off *= 2) {
@@ -253,11 +263,12 @@ struct Walk {
     if (begin == tiles) next(p);  // only the pair's extra unit is here
   }
   __device__ __forceinline__ Walk(int b_, int g_, int len_)
-      : left((len_ + 63) / 64), b(b_), g(g_), begin(0), t1((len_ + 63) / 64), t0(0), tiles(t1), len(len_), ahead(0) {}
+      : left((len_ + TK - 1) / TK), b(b_), g(g_), begin(0), t1((len_ + TK - 1) / TK), t0(0), tiles(t1), len(len_),
+        ahead(0) {}
   __device__ __forceinline__ void measure(const DecodePagedParams& p) {
     len = keys_of(p, b);
-    ahead = tiles_ahead<SHARED>(p, b);
-    tiles = max((len + 63) / 64 - ahead, 0);
+    ahead = tiles_ahead<TK, SHARED>(p, b);
+    tiles = max((len + TK - 1) / TK - ahead, 0);
   }
   __device__ __forceinline__ bool valid() const { return left > 0; }
   __device__ __forceinline__ bool next(const DecodePagedParams& p) {
@@ -279,33 +290,47 @@ struct Walk {
   }
 };
 
-// Two of a word's four e4m3 bytes (the even or the odd ones) as bf16, exactly:
-// moved to bf16's exponent and mantissa bits a value is 2^-120 of itself, the
-// smallest (subnormal) ones too. One shift, two logic operations and the
-// product; the conversion instruction gives f16, which P is too wide for. e4m3's
-// NaN, which the append stores under a NaN scale only, gives 480: a V of finite
-// numbers whatever its bytes are, which a P of 0 hides.
-__device__ __forceinline__ uint32_t from_2_to_minus_120(uint32_t x) {
+// 8-bit keys and values enter the products as f16, which holds every e4m3
+// number and into which one instruction converts two (moving the bits to bf16
+// and fixing the exponent took 4.5, half of the kernel's instructions). f16's range is
+// too narrow for q and for P times V's scales as they are:
+//   q of a head is scaled by a power of two to a largest magnitude in [1, 2):
+//   what then lies below f16's normal numbers is off by 2^-25 of the largest;
+//   V's scale goes into the exponent, t_j = s_j + log2 sv_j, and the running
+//   maximum M is of t: w_j = 2^(t_j - M + 15) <= 2^15 weighs the e4m3 numbers of V
+//   (in two f16 terms: 2^-22 of w, or 2^-40 of the largest), w_j / sv_j is P
+//   for the sum. With sv_j at least 2^-100 that is at most 2^115.
+__device__ __forceinline__ uint32_t f16_of_e4m3(uint16_t x) {  // two numbers, the low byte's in the low half
   uint32_t r;
-  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(0x7b807b80u));
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(x));
   return r;
 }
-__device__ __forceinline__ uint32_t even_e4m3(uint32_t w) {
-  return from_2_to_minus_120(((w << 4) & 0x07f007f0u) | ((w << 8) & 0x80008000u));
+__device__ __forceinline__ uint32_t low_f16(uint32_t w) { return f16_of_e4m3((uint16_t)w); }
+__device__ __forceinline__ uint32_t high_f16(uint32_t w) { return f16_of_e4m3((uint16_t)(w >> 16)); }
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
 }
-__device__ __forceinline__ uint32_t odd_e4m3(uint32_t w) {
-  return from_2_to_minus_120(((w >> 4) & 0x07f007f0u) | (w & 0x80008000u));
+__device__ __forceinline__ float2 unpack_f16x2(uint32_t x) {
+  float2 r;
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.f32.f16 %0, l;\n\tcvt.f32.f16 %1, h;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "r"(x));
+  return r;
 }
+constexpr float kWeightLog2 = 15.f;               // of the largest weight of V
+constexpr float kSmallestScale = 7.888609052210118e-31f;  // 2^-100
 
 __device__ __forceinline__ int swizzle(int r, int d) { return d ^ (((r >> 1) & 3) << 3); }
 
 // NT blocks of 8 query heads cover a group; SPLIT: the even split above; E4M3:
 // 8-bit pools with a scale per key; SHARED: keys from seqs[b].skip on (with SPLIT).
 template <int D, int NT, bool SPLIT, bool E4M3, bool SHARED>
-__global__ void __launch_bounds__(PagedCfg<D, E4M3>::THREADS, PagedCfg<D, E4M3>::CTAS_PER_SM)
+__global__ void __launch_bounds__(PagedCfg<D, NT, E4M3>::THREADS, PagedCfg<D, NT, E4M3>::CTAS_PER_SM)
     decode_paged_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                         const __grid_constant__ DecodePagedParams p) {
-  using C = PagedCfg<D, E4M3>;
+  using C = PagedCfg<D, NT, E4M3>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const uint32_t pad = (1024u - (smem_u32(smem_raw) & 1023u)) & 1023u;
   uint8_t* smem = smem_raw + pad;
@@ -322,17 +347,18 @@ __global__ void __launch_bounds__(PagedCfg<D, E4M3>::THREADS, PagedCfg<D, E4M3>:
       if (p.seqlens[b] < 0 || p.seqlens[b] > (long long)p.table_width * p.page) atomicOr(p.err, kErrBadArgs);
   long long from = 0, count = 1;
   if constexpr (SPLIT) {
-    const long long total = total_units<SHARED>(p), share = share_of(total, p.n_ctas);
+    const long long total = total_units<C::TK, SHARED>(p), share = share_of(total, p.n_ctas);
     from = blockIdx.x * share;
     count = min(share, total - from);
     if (count <= 0) return;
   }
-  auto start = [&]() -> Walk<SHARED> {
-    if constexpr (SPLIT) return Walk<SHARED>(p, from, count);
+  using W = Walk<C::TK, SHARED>;
+  auto start = [&]() -> W {
+    if constexpr (SPLIT) return W(p, from, count);
     const int b = blockIdx.x / p.Hkv;
-    return Walk<SHARED>(b, blockIdx.x % p.Hkv, keys_of(p, b));
+    return W(b, blockIdx.x % p.Hkv, keys_of(p, b));
   };
-  Walk<SHARED> w = start();
+  W w = start();
   if (SPLIT && !w.valid()) return;
   if (!SPLIT && w.tiles == 0) {
     for (int e = 4 * threadIdx.x; e < p.group * D; e += 4 * C::THREADS)
@@ -433,10 +459,13 @@ __global__ void __launch_bounds__(PagedCfg<D, E4M3>::THREADS, PagedCfg<D, E4M3>:
     const int gr = lane >> 2, tq = lane & 3;
     const float sl2 = p.scale_log2;
     const int mi = lane >> 3, mr = lane & 7;  // ldmatrix: matrix index / row in it
-    // This warp's 16 keys of a tile lie in one box: its first row there, and
-    // the distance of the box's 64-column chunks.
+    // This warp's 16 keys of a tile (E4M3: and 16 of its second half) lie in one
+    // box: its first row there, and the distance of the box's chunks of columns.
     constexpr int kLine = E4M3 && D == 64 ? 64 : 128;  // bytes of a row in a chunk
-    const uint32_t wbase = (16 * warp / br) * (br * D * (E4M3 ? 1 : 2)) + (16 * warp % br) * kLine;
+    auto rows_at = [&](int r) -> uint32_t {
+      return (r / br) * (br * D * (E4M3 ? 1 : 2)) + (r % br) * kLine;
+    };
+    const uint32_t wbase = rows_at(16 * warp);
     const uint32_t chunk = br * 128;
     // 16-byte unit U of row r (0..15): the swizzle XORs the unit with the
     // row's place in its group of 8 (rows of 64 bytes: of two rows' place in
@@ -453,19 +482,36 @@ __global__ void __launch_bounds__(PagedCfg<D, E4M3>::THREADS, PagedCfg<D, E4M3>:
       const int n_last = n + (w.t1 - w.begin) - 1;  // the pair's last one here
       // Q^T as the B operand: column (head) gr, k in pairs 2 tq, 2 tq + 8.
       uint32_t qb[NT][D / 16][2];
+      float qf[NT][2];  // E4M3: what the scores of heads 8 x + 2 tq (+ 1) are multiplied by
       const bool got = __all_sync(
           0xffffffffu, mbar_wait(&bars->q_full[pair & 1], (uint32_t)(pair >> 1) & 1u, abort_flag, p.err));
 #pragma unroll
       for (int x = 0; x < NT; ++x) {
         if constexpr (E4M3) {
-          // The order in which a word of K gives its four columns: 0 and 2, then 1 and 3.
+          // In the order in which a word of K holds its columns: four in a row.
           const uint8_t* q = smem + C::OFF_Q + ((pair & 1) * 16 + 8 * x + gr) * C::Q_ROW + tq * 8;
+          uint32_t top = 0;  // the largest magnitude, as an integer of the same order
 #pragma unroll
           for (int k = 0; k < D / 16; ++k) {
             const uint2 w = *reinterpret_cast<const uint2*>(q + 32 * k);
-            qb[x][k][0] = __byte_perm(w.x, w.y, 0x5410);
-            qb[x][k][1] = __byte_perm(w.x, w.y, 0x7632);
+            qb[x][k][0] = w.x;
+            qb[x][k][1] = w.y;
+            top = max(top, max(max(w.x & 0x7fffu, w.y & 0x7fffu), max((w.x >> 16) & 0x7fffu, (w.y >> 16) & 0x7fffu)));
           }
+          top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+          top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+          // 2^-e and 2^e for 2^e <= the largest < 2^(e + 1); e of a zero row or one of the smallest numbers: -126.
+          const uint32_t e = max(min(top >> 7, 253u), 1u);
+          const float down = __uint_as_float((254u - e) << 23), up = __uint_as_float(e << 23);
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              const uint32_t w = qb[x][k][u];
+              qb[x][k][u] = pack_f16x2(__uint_as_float(w << 16) * down, __uint_as_float(w & 0xffff0000u) * down);
+            }
+          qf[x][0] = sl2 * __shfl_sync(0xffffffffu, up, 8 * tq);
+          qf[x][1] = sl2 * __shfl_sync(0xffffffffu, up, 8 * tq + 4);
         } else {
           const uint32_t q = smem_u32(smem + C::OFF_Q) + ((pair & 1) * 16 + 8 * x + mr) * C::Q_ROW + mi * 16;
 #pragma unroll
@@ -475,8 +521,8 @@ __global__ void __launch_bounds__(PagedCfg<D, E4M3>::THREADS, PagedCfg<D, E4M3>:
       }
       __syncwarp();
       if (lane == 0 && got) mbar_arrive(&bars->q_empty[pair & 1]);
-      // O^T: rows 16 d + gr (+ 8) (E4M3: 16 d + 2 gr (+ 1), the columns of V's
-      // even and odd bytes), columns (heads) 8 x + 2 tq (+ 1); this
+      // O^T: rows 16 d + gr (+ 8) (E4M3: 16 d + 2 gr (+ 1), as V's bytes come),
+      // columns (heads) 8 x + 2 tq (+ 1); this
       // thread keeps the running maximum and its part of the sum of those heads.
       float acc[NT][D / 16][4];
       float m[NT][2], l[NT][2];
@@ -494,37 +540,143 @@ __global__ void __launch_bounds__(PagedCfg<D, E4M3>::THREADS, PagedCfg<D, E4M3>:
           n = n_last + 1;
           break;
         }
-        const uint32_t kbase = smem_u32(smem + slot * C::STAGE_BYTES) + wbase;
-        const uint32_t vbase = kbase + C::TILE_BYTES;
-        const int have = w.len - ((w.ahead + t) * C::TK + 16 * warp);  // keys of this warp's 16 that exist
-        if (have > 0) {
-          float s[NT][4];
+        const uint32_t stage = smem_u32(smem + slot * C::STAGE_BYTES);
+        const int left = w.len - (w.ahead + t) * C::TK;  // keys from the tile's first on
+        if constexpr (E4M3) {
+          if (left > 16 * warp) {
+            uint32_t kbase[C::KB];
+            int have[C::KB];  // keys of each block that exist
 #pragma unroll
-          for (int x = 0; x < NT; ++x) s[x][0] = s[x][1] = s[x][2] = s[x][3] = 0.f;
-          float sv[2];  // E4M3: the scales of V's rows gr, gr + 8
-          if constexpr (E4M3) {
-            const float* scales = reinterpret_cast<const float*>(smem + C::OFF_SCALES) + slot * 2 * C::TK + 16 * warp;
+            for (int i = 0; i < C::KB; ++i) {
+              kbase[i] = stage + rows_at(64 * i + 16 * warp);
+              have[i] = left - 64 * i - 16 * warp;
+            }
+            float s[C::KB][NT][4];
+#pragma unroll
+            for (int i = 0; i < C::KB; ++i)
+#pragma unroll
+              for (int x = 0; x < NT; ++x) s[i][x][0] = s[i][x][1] = s[i][x][2] = s[i][x][3] = 0.f;
 #pragma unroll
             for (int k = 0; k < D / 32; ++k) {
-              uint32_t w[4];
-              ldsm4(at(kbase, 8 * (mi & 1) + mr, 2 * k + (mi >> 1)), w[0], w[1], w[2], w[3]);
 #pragma unroll
-              for (int u = 0; u < 2; ++u) {
-                const uint32_t a[4] = {even_e4m3(w[2 * u]), even_e4m3(w[2 * u + 1]), odd_e4m3(w[2 * u]),
-                                       odd_e4m3(w[2 * u + 1])};
+              for (int i = 0; i < C::KB; ++i) {
+                uint32_t w4[4];
+                ldsm4(at(kbase[i], 8 * (mi & 1) + mr, 2 * k + (mi >> 1)), w4[0], w4[1], w4[2], w4[3]);
 #pragma unroll
-                for (int x = 0; x < NT; ++x) mma16816(s[x], a, qb[x][2 * k + u][0], qb[x][2 * k + u][1]);
+                for (int u = 0; u < 2; ++u) {
+                  const uint32_t a[4] = {low_f16(w4[2 * u]), low_f16(w4[2 * u + 1]), high_f16(w4[2 * u]),
+                                         high_f16(w4[2 * u + 1])};
+#pragma unroll
+                  for (int x = 0; x < NT; ++x) mma16816_f16(s[i][x], a, qb[x][2 * k + u][0], qb[x][2 * k + u][1]);
+                }
               }
             }
-            const float sk[2] = {scales[gr], scales[gr + 8]};
+            const float* scales = reinterpret_cast<const float*>(smem + C::OFF_SCALES) + slot * 2 * C::TK + 16 * warp;
+            float per_sv[C::KB][2];  // 1 / the scales of V's rows gr, gr + 8
+#pragma unroll
+            for (int i = 0; i < C::KB; ++i) {
+#pragma unroll
+              for (int u = 0; u < 2; ++u) {
+                const int r = gr + 8 * u;
+                const float sk = scales[64 * i + r], given = scales[C::TK + 64 * i + r];
+                const float sv = given < kSmallestScale ? kSmallestScale : given, lg = __log2f(sv);  // NaN stays
+                per_sv[i][u] = r < have[i] ? __fdividef(1.f, sv) : 0.f;
+#pragma unroll
+                for (int x = 0; x < NT; ++x) {
+#pragma unroll
+                  for (int c = 0; c < 2; ++c) {
+                    const float tj = fmaf(s[i][x][2 * u + c] * sk, qf[x][c], lg);
+                    s[i][x][2 * u + c] = r < have[i] ? tj : -INFINITY;
+                  }
+                }
+              }
+              if (have[i] < 16) {
+                // V rows without a key: 0 x anything would not do (NaN).
+                const int from = max(have[i], 0);
+                for (int u = lane; u < (16 - from) * (D / 16); u += 32)
+                  st_shared_v4(at(kbase[i] + C::TILE_BYTES, from + u / (D / 16), u % (D / 16)), 0u, 0u, 0u, 0u);
+                fence_proxy_async_smem();  // before the slot's next copy
+                __syncwarp();
+              }
+            }
+            // P^T as the B operand, in two terms: the scores' fragments hold keys along gr and heads along tq, the
+            // operand the reverse.
+            uint32_t ph[C::KB][NT][2], pl[C::KB][NT][2];
 #pragma unroll
             for (int x = 0; x < NT; ++x) {
-              s[x][0] *= sk[0], s[x][1] *= sk[0];
-              s[x][2] *= sk[1], s[x][3] *= sk[1];
+              float a[2];
+#pragma unroll
+              for (int c = 0; c < 2; ++c) {
+                float mx = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < C::KB; ++i) mx = fmaxf(mx, fmaxf(s[i][x][c], s[i][x][2 + c]));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                const float mn = fmaxf(m[x][c], mx);
+                const float u = mn == -INFINITY ? 0.f : mn;
+                a[c] = ex2(m[x][c] - u);
+                m[x][c] = mn;
+                float sum = 0.f;
+#pragma unroll
+                for (int i = 0; i < C::KB; ++i) {
+#pragma unroll
+                  for (int e = 0; e < 2; ++e) {
+                    float& w1 = s[i][x][2 * e + c];
+                    w1 = ex2(w1 - (u - kWeightLog2));
+                    sum = fmaf(w1, per_sv[i][e], sum);
+                  }
+                }
+                l[x][c] = fmaf(l[x][c], a[c], sum);
+              }
+              if (__any_sync(0xffffffffu, a[0] != 1.f || a[1] != 1.f)) {
+#pragma unroll
+                for (int d = 0; d < D / 16; ++d) {
+                  acc[x][d][0] *= a[0];
+                  acc[x][d][1] *= a[1];
+                  acc[x][d][2] *= a[0];
+                  acc[x][d][3] *= a[1];
+                }
+              }
+#pragma unroll
+              for (int i = 0; i < C::KB; ++i) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  const uint32_t high = pack_f16x2(s[i][x][2 * e], s[i][x][2 * e + 1]);
+                  const float2 back = unpack_f16x2(high);
+                  ph[i][x][e] = transposed(high);
+                  pl[i][x][e] = transposed(pack_f16x2(s[i][x][2 * e] - back.x, s[i][x][2 * e + 1] - back.y));
+                }
+              }
             }
-            sv[0] = gr < have ? scales[C::TK + gr] : 0.f;
-            sv[1] = gr + 8 < have ? scales[C::TK + gr + 8] : 0.f;
-          } else {
+#pragma unroll
+            for (int i = 0; i < C::KB; ++i) {
+#pragma unroll
+              for (int k = 0; k < D / 32; ++k) {
+                uint32_t w4[4];
+                ldsm4_t(at(kbase[i] + C::TILE_BYTES, 8 * (mi >> 1) + mr, 2 * k + (mi & 1)), w4[0], w4[1], w4[2], w4[3]);
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                  // A word has two columns of two keys; the operand wants two keys of a column.
+                  const uint32_t w0 = __byte_perm(w4[u], 0, 0x3120), w1 = __byte_perm(w4[u + 2], 0, 0x3120);
+                  const uint32_t a[4] = {low_f16(w0), high_f16(w0), low_f16(w1), high_f16(w1)};
+#pragma unroll
+                  for (int x = 0; x < NT; ++x) {
+                    mma16816_f16(acc[x][2 * k + u], a, ph[i][x][0], ph[i][x][1]);
+                    mma16816_f16(acc[x][2 * k + u], a, pl[i][x][0], pl[i][x][1]);
+                  }
+                }
+              }
+            }
+          }
+        } else {
+          const uint32_t kbase = stage + wbase;
+          const uint32_t vbase = kbase + C::TILE_BYTES;
+          const int have = left - 16 * warp;  // keys of this warp's 16 that exist
+          if (have > 0) {
+            float s[NT][4];
+#pragma unroll
+            for (int x = 0; x < NT; ++x) s[x][0] = s[x][1] = s[x][2] = s[x][3] = 0.f;
 #pragma unroll
             for (int k = 0; k < D / 16; ++k) {
               uint32_t a[4];
@@ -532,78 +684,55 @@ __global__ void __launch_bounds__(PagedCfg<D, E4M3>::THREADS, PagedCfg<D, E4M3>:
 #pragma unroll
               for (int x = 0; x < NT; ++x) mma16816(s[x], a, qb[x][k][0], qb[x][k][1]);
             }
-          }
-          if (have < 16) {
+            if (have < 16) {
 #pragma unroll
-            for (int x = 0; x < NT; ++x) {
-              if (gr >= have) s[x][0] = s[x][1] = -INFINITY;
-              if (gr + 8 >= have) s[x][2] = s[x][3] = -INFINITY;
-            }
-            if constexpr (!E4M3) {
+              for (int x = 0; x < NT; ++x) {
+                if (gr >= have) s[x][0] = s[x][1] = -INFINITY;
+                if (gr + 8 >= have) s[x][2] = s[x][3] = -INFINITY;
+              }
               // V rows without a key: 0 x anything would not do (NaN).
               for (int u = lane; u < (16 - have) * (D / 8); u += 32)
                 st_shared_v4(at(vbase, have + u / (D / 8), u % (D / 8)), 0u, 0u, 0u, 0u);
               fence_proxy_async_smem();  // before the slot's next copy
               __syncwarp();
             }
-          }
-          // P^T as the B operand, in two bf16 terms: the scores' fragments
-          // hold keys along gr and heads along tq, the operand the reverse.
-          uint32_t ph[NT][2], pl[NT][2];
+            // P^T as the B operand, in two bf16 terms: the scores' fragments
+            // hold keys along gr and heads along tq, the operand the reverse.
+            uint32_t ph[NT][2], pl[NT][2];
 #pragma unroll
-          for (int x = 0; x < NT; ++x) {
-            float a[2];
+            for (int x = 0; x < NT; ++x) {
+              float a[2];
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              float mx = fmaxf(s[x][c], s[x][2 + c]);
-              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-              const float mn = fmaxf(m[x][c], mx * sl2);
-              const float u = mn == -INFINITY ? 0.f : mn;
-              a[c] = ex2(m[x][c] - u);
-              m[x][c] = mn;
-              s[x][c] = ex2(fmaf(s[x][c], sl2, -u));
-              s[x][2 + c] = ex2(fmaf(s[x][2 + c], sl2, -u));
-              l[x][c] = fmaf(l[x][c], a[c], s[x][c] + s[x][2 + c]);
-            }
-            if (__any_sync(0xffffffffu, a[0] != 1.f || a[1] != 1.f)) {
-#pragma unroll
-              for (int d = 0; d < D / 16; ++d) {
-                acc[x][d][0] *= a[0];
-                acc[x][d][1] *= a[1];
-                acc[x][d][2] *= a[0];
-                acc[x][d][3] *= a[1];
+              for (int c = 0; c < 2; ++c) {
+                float mx = fmaxf(s[x][c], s[x][2 + c]);
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                const float mn = fmaxf(m[x][c], mx * sl2);
+                const float u = mn == -INFINITY ? 0.f : mn;
+                a[c] = ex2(m[x][c] - u);
+                m[x][c] = mn;
+                s[x][c] = ex2(fmaf(s[x][c], sl2, -u));
+                s[x][2 + c] = ex2(fmaf(s[x][2 + c], sl2, -u));
+                l[x][c] = fmaf(l[x][c], a[c], s[x][c] + s[x][2 + c]);
               }
-            }
-            if constexpr (E4M3) {
-              s[x][0] *= sv[0], s[x][1] *= sv[0];
-              s[x][2] *= sv[1], s[x][3] *= sv[1];
-            }
+              if (__any_sync(0xffffffffu, a[0] != 1.f || a[1] != 1.f)) {
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const uint32_t high = pack_bf16x2(s[x][2 * e], s[x][2 * e + 1]);
-              ph[x][e] = transposed(high);
-              pl[x][e] = transposed(pack_bf16x2(s[x][2 * e] - __uint_as_float(high << 16),
-                                                s[x][2 * e + 1] - __uint_as_float(high & 0xffff0000u)));
-            }
-          }
-          if constexpr (E4M3) {
-#pragma unroll
-            for (int k = 0; k < D / 32; ++k) {
-              uint32_t w[4];
-              ldsm4_t(at(vbase, 8 * (mi >> 1) + mr, 2 * k + (mi & 1)), w[0], w[1], w[2], w[3]);
-#pragma unroll
-              for (int u = 0; u < 2; ++u) {
-                const uint32_t a[4] = {even_e4m3(w[u]), odd_e4m3(w[u]), even_e4m3(w[u + 2]), odd_e4m3(w[u + 2])};
-#pragma unroll
-                for (int x = 0; x < NT; ++x) {
-                  mma16816(acc[x][2 * k + u], a, ph[x][0], ph[x][1]);
-                  mma16816(acc[x][2 * k + u], a, pl[x][0], pl[x][1]);
+                for (int d = 0; d < D / 16; ++d) {
+                  acc[x][d][0] *= a[0];
+                  acc[x][d][1] *= a[1];
+                  acc[x][d][2] *= a[0];
+                  acc[x][d][3] *= a[1];
                 }
               }
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const uint32_t high = pack_bf16x2(s[x][2 * e], s[x][2 * e + 1]);
+                ph[x][e] = transposed(high);
+                pl[x][e] = transposed(pack_bf16x2(s[x][2 * e] - __uint_as_float(high << 16),
+                                                  s[x][2 * e + 1] - __uint_as_float(high & 0xffff0000u)));
+              }
             }
-          } else {
 #pragma unroll
             for (int d = 0; d < D / 16; ++d) {
               uint32_t a[4];
@@ -623,71 +752,65 @@ __global__ void __launch_bounds__(PagedCfg<D, E4M3>::THREADS, PagedCfg<D, E4M3>:
       // them have read it; the stage is released after that.
       asm volatile("bar.sync 1, 128;" ::: "memory");
       const int slot = n_last % C::STAGES;
-      // [4][MERGE][D], columns swizzled by the head so that neither side's accesses
+      // [4][16][D], columns swizzled by the head so that neither side's accesses
       // collide in a bank.
       float* so = reinterpret_cast<float*>(smem + slot * C::STAGE_BYTES);
-      const long long part = ((long long)w.b * p.Hkv + w.g + blockIdx.x) * p.group;
-      constexpr int kBlocks = C::MERGE / 8 < NT ? C::MERGE / 8 : NT;  // blocks of 8 heads merged at a time
 #pragma unroll
-      for (int x0 = 0; x0 < NT; x0 += kBlocks) {
-        if (x0 > 0) asm volatile("bar.sync 1, 128;" ::: "memory");
+      for (int x = 0; x < NT; ++x) {
 #pragma unroll
-        for (int x = x0; x < x0 + kBlocks; ++x) {
+        for (int c = 0; c < 2; ++c) {
+          const int r = 8 * x + 2 * tq + c;
+          float lr = l[x][c];
+          lr += __shfl_xor_sync(0xffffffffu, lr, 4);
+          lr += __shfl_xor_sync(0xffffffffu, lr, 8);
+          lr += __shfl_xor_sync(0xffffffffu, lr, 16);
+          if (gr == 0) {
+            bars->m[warp][r] = m[x][c];
+            bars->l[warp][r] = lr;
+          }
+          if (r < p.group) {
+            float* row = so + (warp * 16 + r) * D;
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const int r = 8 * x + 2 * tq + c;
-            float lr = l[x][c];
-            lr += __shfl_xor_sync(0xffffffffu, lr, 4);
-            lr += __shfl_xor_sync(0xffffffffu, lr, 8);
-            lr += __shfl_xor_sync(0xffffffffu, lr, 16);
-            if (gr == 0) {
-              bars->m[warp][r] = m[x][c];
-              bars->l[warp][r] = lr;
-            }
-            if (r < p.group) {
-              float* row = so + (warp * C::MERGE + r - 8 * x0) * D;
-#pragma unroll
-              for (int d = 0; d < D / 16; ++d) {
-                if constexpr (E4M3) {
-                  *reinterpret_cast<float2*>(row + swizzle(r, 16 * d + 2 * gr)) =
-                      make_float2(acc[x][d][c], acc[x][d][2 + c]);
-                } else {
-                  row[swizzle(r, 16 * d + gr)] = acc[x][d][c];
-                  row[swizzle(r, 16 * d + 8 + gr)] = acc[x][d][2 + c];
-                }
+            for (int d = 0; d < D / 16; ++d) {
+              if constexpr (E4M3) {
+                *reinterpret_cast<float2*>(row + swizzle(r, 16 * d + 2 * gr)) =
+                    make_float2(acc[x][d][c], acc[x][d][2 + c]);
+              } else {
+                row[swizzle(r, 16 * d + gr)] = acc[x][d][c];
+                row[swizzle(r, 16 * d + 8 + gr)] = acc[x][d][2 + c];
               }
             }
           }
         }
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-        // Thread x takes columns 4 x .. of the group's rows, 512 apart. Not
-        // unrolled, and finished by the joining kernel when SPLIT: this runs
-        // once per pair, and fetching more instructions from memory (which the
-        // stream of keys has pushed out of L2) cost more than running them.
-        const int rows_here = min(p.group - 8 * x0, C::MERGE);
+      }
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      // Thread x takes columns 4 x .. of the group's rows, 512 apart. Not
+      // unrolled, and finished by the joining kernel when SPLIT: this runs
+      // once per pair, and fetching more instructions from memory (which the
+      // stream of keys has pushed out of L2) cost more than running them.
+      const long long part = ((long long)w.b * p.Hkv + w.g + blockIdx.x) * p.group;
 #pragma unroll 1
-        for (int e = 4 * threadIdx.x; e < rows_here * D; e += 512) {
-          const int rr = e / D, r = 8 * x0 + rr, d = e % D;
-          float M = -INFINITY;
+      for (int e = 4 * threadIdx.x; e < p.group * D; e += 512) {
+        const int r = e / D, d = e % D;
+        float M = -INFINITY;
 #pragma unroll
-          for (int u = 0; u < 4; ++u) M = fmaxf(M, bars->m[u][r]);
-          const float Mu = (M == -INFINITY) ? 0.f : M;
-          float lsum = 0.f;
-          float4 osum = zero4();
+        for (int u = 0; u < 4; ++u) M = fmaxf(M, bars->m[u][r]);
+        const float Mu = (M == -INFINITY) ? 0.f : M;
+        float lsum = 0.f;
+        float4 osum = zero4();
 #pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            // A warp without keys here has nothing in the sum (its m is -inf).
-            const float f = ex2(bars->m[u][r] - Mu);
-            lsum += f * bars->l[u][r];
-            osum = axpy(f, *reinterpret_cast<const float4*>(so + (u * C::MERGE + rr) * D + swizzle(r, d)), osum);
-          }
-          if constexpr (SPLIT) {
-            *reinterpret_cast<float4*>(p.part_o + (part + r) * D + d) = osum;
-            if (d == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * (part + r)) = make_float2(M, lsum);
-          } else {
-            const int h = w.g * p.group + r;
-            store_output(p, w.b, h, d, over(osum, lsum), p.gate ? load_gate(p, w.b, h, d) : zero4());
-          }
+        for (int u = 0; u < 4; ++u) {
+          // A warp without keys here has nothing in the sum (its m is -inf).
+          const float f = ex2(bars->m[u][r] - Mu);
+          lsum += f * bars->l[u][r];
+          osum = axpy(f, *reinterpret_cast<const float4*>(so + (u * 16 + r) * D + swizzle(r, d)), osum);
+        }
+        if constexpr (SPLIT) {
+          *reinterpret_cast<float4*>(p.part_o + (part + r) * D + d) = osum;
+          if (d == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * (part + r)) = make_float2(M, lsum);
+        } else {
+          const int h = w.g * p.group + r;
+          store_output(p, w.b, h, d, over(osum, lsum), p.gate ? load_gate(p, w.b, h, d) : zero4());
         }
       }
       if (SPLIT && threadIdx.x == 0) {
@@ -731,7 +854,7 @@ __global__ void __launch_bounds__(kJoinThreads) decode_paged_join_kernel(const _
   const int2 at = __ldcg(reinterpret_cast<const int2*>(p.place) + pair);
   const float4 gate = p.gate && team == 0 ? load_gate(p, b, h, d) : zero4();
   int c0 = 0, parts = 0;
-  if (tiles_of<SHARED>(p, b) > 0) {
+  if (tiles_of<64, SHARED>(p, b) > 0) {  // any size of tiles
     // (Within the CTAs there are, even if the lengths changed under the call.)
     c0 = max(0, min(at.x, p.n_ctas - 1));
     parts = min(at.y, p.n_ctas - 1) - c0 + 1;
@@ -806,7 +929,7 @@ constexpr int kWholeTiles = 8;
 template <int D, int NT, bool SPLIT, bool E4M3, bool SHARED = false>
 int launch_main(const CUtensorMap& tk, const CUtensorMap& tv, const DecodePagedParams& p, long long n,
                 cudaStream_t st) {
-  using C = PagedCfg<D, E4M3>;
+  using C = PagedCfg<D, NT, E4M3>;
   static OncePerDevice once;
   if (n > 0x7fffffffLL) return -1;
   return once.run(
@@ -851,7 +974,9 @@ int launch_t(const CUtensorMap& tk, const CUtensorMap& tv, const DecodePagedPara
 
 bool decode_paged_splits(int table_width, int page) { return (long long)table_width * page > 64LL * kWholeTiles; }
 
-int decode_paged_max_ctas(int D, int sms) { return sms * (D == 256 ? 1 : 2); }
+int decode_paged_max_ctas(int D, int group, bool e4m3, int sms) {
+  return sms * decode_paged_ctas_per_sm(D, group <= 8 ? 1 : 2, e4m3);
+}
 
 int launch_decode_paged(int D, const CUtensorMap& tk, const CUtensorMap& tv, const DecodePagedParams& p,
                         cudaStream_t st) {

@@ -58,10 +58,17 @@ struct DecodePagedParams {
   int* err;
 };
 
+// CTAs an SM holds; NT: blocks of 8 query heads of a group. 8-bit keys at head
+// dim 64 are bound by instructions and need few registers: a third CTA hides
+// more of their latency.
+constexpr int decode_paged_ctas_per_sm(int D, int NT, bool e4m3) {
+  return D == 256 ? 1 : (D == 64 && NT == 1 && e4m3 ? 3 : 2);
+}
+
 // Whether a call runs the split form (partials and a joining kernel), the
 // CTAs it may use for the current device, and its workspace.
 bool decode_paged_splits(int table_width, int page);
-int decode_paged_max_ctas(int D, int sms);
+int decode_paged_max_ctas(int D, int group, bool e4m3, int sms);
 inline size_t decode_paged_parts(int B, int Hkv, int n_ctas) { return (size_t)B * Hkv + n_ctas; }
 
 // tk / tv: 5-D maps (64 columns, slot in the page, D / 64, head, page) with

@@ -12,8 +12,11 @@
 // Bound by memory: logits read once and written once. A CTA takes a chunk of
 // one row's vocabulary, requests its logits, counts the row's tokens that fall
 // into the chunk in shared memory (bit 0: in the prompt, from bit 1 on: the
-// count) and applies everything to the registers. The tokens are read once per
-// chunk, from L2 after the first.
+// count) and applies bias and mask to the registers. The few elements that a
+// token names (some 1 %, but a lane in almost every warp) are then done one by
+// one in a loop: with the penalties' code in line for each of a lane's elements the
+// kernel took twice the instructions. The tokens are read once per chunk, from
+// L2 after the first, eight requests at a time.
 #include "capi_internal.cuh"
 #include "penalize.cuh"
 
@@ -28,8 +31,15 @@ struct Elements;  // 16 bytes of logits
 template <>
 struct Elements<float> {
   static constexpr int N = 4;
-  static __device__ __forceinline__ void get(const uint4& w, float (&x)[4]) {
-    x[0] = __uint_as_float(w.x), x[1] = __uint_as_float(w.y), x[2] = __uint_as_float(w.z), x[3] = __uint_as_float(w.w);
+  static __device__ __forceinline__ float get(const uint4& w, int i) {
+    return __uint_as_float(i & 2 ? (i & 1 ? w.w : w.z) : (i & 1 ? w.y : w.x));
+  }
+  static __device__ __forceinline__ void put(uint4& w, int i, float v) {
+    const uint32_t u = __float_as_uint(v);
+    if (i == 0) w.x = u;
+    if (i == 1) w.y = u;
+    if (i == 2) w.z = u;
+    if (i == 3) w.w = u;
   }
   static __device__ __forceinline__ uint4 put(const float (&x)[4]) {
     return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
@@ -40,13 +50,16 @@ struct Elements<float> {
 template <>
 struct Elements<__nv_bfloat16> {
   static constexpr int N = 8;
-  static __device__ __forceinline__ void get(const uint4& w, float (&x)[8]) {
-    const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[2 * i] = __uint_as_float(ws[i] << 16);
-      x[2 * i + 1] = __uint_as_float(ws[i] & 0xffff0000u);
-    }
+  static __device__ __forceinline__ float get(const uint4& w, int i) {
+    const uint32_t u = i & 4 ? (i & 2 ? w.w : w.z) : (i & 2 ? w.y : w.x);
+    return __uint_as_float(i & 1 ? u & 0xffff0000u : u << 16);
+  }
+  static __device__ __forceinline__ void put(uint4& w, int i, float v) {
+    const uint32_t u = pack_bf16x2(v, v), keep = i & 1 ? 0x0000ffffu : 0xffff0000u;
+    if (i >> 1 == 0) w.x = (w.x & keep) | (u & ~keep);
+    if (i >> 1 == 1) w.y = (w.y & keep) | (u & ~keep);
+    if (i >> 1 == 2) w.z = (w.z & keep) | (u & ~keep);
+    if (i >> 1 == 3) w.w = (w.w & keep) | (u & ~keep);
   }
   static __device__ __forceinline__ uint4 put(const float (&x)[8]) {
     return make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]),
@@ -54,6 +67,48 @@ struct Elements<__nv_bfloat16> {
   }
   static __device__ __forceinline__ float load(const __nv_bfloat16* p) { return __bfloat162float(*p); }
   static __device__ __forceinline__ void store(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
+};
+
+// Counters of a chunk, two to a word while a row has few enough tokens.
+constexpr int kNarrowTokens = 32767;
+template <bool WIDE>
+struct Counters {
+  static constexpr int BITS = WIDE ? 32 : 16;
+  static __device__ __forceinline__ void prompt(unsigned* c, int i) {
+    atomicOr(c + (WIDE ? i : i >> 1), 1u << (WIDE ? 0 : 16 * (i & 1)));
+  }
+  static __device__ __forceinline__ void made(unsigned* c, int i) {
+    atomicAdd(c + (WIDE ? i : i >> 1), 2u << (WIDE ? 0 : 16 * (i & 1)));
+  }
+  static __device__ __forceinline__ unsigned get(const unsigned* c, int i) {
+    return WIDE ? c[i] : reinterpret_cast<const uint16_t*>(c)[i];
+  }
+  // Which of the N counters from number i on (a multiple of N) are not 0.
+  template <int N>
+  static __device__ __forceinline__ unsigned used(const unsigned* c, int i) {
+    constexpr int WORDS = N * BITS / 32;
+    uint32_t w[WORDS];
+    if constexpr (WORDS == 2) {
+      *reinterpret_cast<uint2*>(w) = *reinterpret_cast<const uint2*>(c + i * BITS / 32);
+    } else {
+#pragma unroll
+      for (int k = 0; k < WORDS; k += 4)
+        *reinterpret_cast<uint4*>(w + k) = *reinterpret_cast<const uint4*>(c + i * BITS / 32 + k);
+    }
+    unsigned any = 0, m = 0;
+#pragma unroll
+    for (int k = 0; k < WORDS; ++k) any |= w[k];
+    if (any) {
+#pragma unroll
+      for (int k = 0; k < WORDS; ++k) {
+        if constexpr (WIDE)
+          m |= w[k] ? 1u << k : 0u;
+        else
+          m |= (w[k] & 0xffffu ? 1u << (2 * k) : 0u) | (w[k] >> 16 ? 2u << (2 * k) : 0u);
+      }
+    }
+    return m;
+  }
 };
 
 // Bits [v, v + 8) of a row's mask of `words` words (those that exist).
@@ -64,12 +119,31 @@ __device__ __forceinline__ unsigned mask_bits(const unsigned* row, int v, int wo
   return __funnelshift_r(lo, hi, v & 31);
 }
 
+// N floats from p on, which lies `off` floats past a 16-byte boundary (the same for the whole CTA). Reads no further
+// than the 16-byte pieces that hold them.
+template <int N>
+__device__ __forceinline__ void load_floats(const float* p, int off, float (&b)[N]) {
+  const float4* q = reinterpret_cast<const float4*>(p - off);
+  float a[N + 4];
+#pragma unroll
+  for (int k = 0; k < N / 4; ++k) *reinterpret_cast<float4*>(a + 4 * k) = __ldg(q + k);
+  if (off == 0) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) b[i] = a[i];
+    return;
+  }
+  *reinterpret_cast<float4*>(a + N) = __ldg(q + N / 4);
+#pragma unroll
+  for (int i = 0; i < N; ++i) b[i] = off == 1 ? a[i + 1] : (off == 2 ? a[i + 2] : a[i + 3]);
+}
+
 // SLOTS: 16-byte pieces of logits per thread.
-template <typename T, int SLOTS>
+template <typename T, int SLOTS, bool WIDE>
 __global__ void __launch_bounds__(kThreads) penalize_kernel(const __grid_constant__ PenalizeParams p, int chunks) {
   using E = Elements<T>;
+  using Count = Counters<WIDE>;
   constexpr int CHUNK = kThreads * SLOTS * E::N;
-  __shared__ __align__(16) unsigned counts[CHUNK];
+  __shared__ __align__(16) unsigned counts[CHUNK * Count::BITS / 32];
   grid_dep_wait();
   grid_dep_launch();
   const int row = blockIdx.x / chunks;
@@ -97,74 +171,94 @@ __global__ void __launch_bounds__(kThreads) penalize_kernel(const __grid_constan
   }
   const bool counted = n > 0 && (rep != 1.f || freq != 0.f || pres != 0.f);
   if (counted) {
-    for (int i = threadIdx.x; i < CHUNK / 4; i += kThreads)
-      reinterpret_cast<uint4*>(counts)[i] = make_uint4(0u, 0u, 0u, 0u);
     const int prompt = p.prompt_lengths ? p.prompt_lengths[row] : 0;
-    __syncthreads();
-    for (int i = threadIdx.x; i < n; i += kThreads) {
-      const long long at = row * p.tokens_row + i * p.tokens_step;
-      const long long t = p.tokens_64 ? static_cast<const long long*>(p.tokens)[at]
-                                      : (long long)static_cast<const int*>(p.tokens)[at];
-      const long long c = t - v0;
-      if (t < 0 || t >= p.V || c < 0 || c >= CHUNK) continue;
-      if (i < prompt)
-        atomicOr(&counts[c], 1u);
-      else
-        atomicAdd(&counts[c], 2u);
+    for (int i = threadIdx.x; i < CHUNK * Count::BITS / 128; i += kThreads)
+      reinterpret_cast<uint4*>(counts)[i] = make_uint4(0u, 0u, 0u, 0u);
+    const long long first = max(v0, 0), past = min((long long)v0 + CHUNK, (long long)p.V);
+    constexpr int AHEAD = 8;
+    for (int i0 = threadIdx.x; i0 - (int)threadIdx.x < n; i0 += AHEAD * kThreads) {
+      long long t[AHEAD];
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        const int i = i0 + k * kThreads;
+        t[k] = -1;
+        if (i >= n) continue;
+        const long long at = row * p.tokens_row + i * p.tokens_step;
+        t[k] = p.tokens_64 ? __ldg(static_cast<const long long*>(p.tokens) + at)
+                           : (long long)__ldg(static_cast<const int*>(p.tokens) + at);
+      }
+      if (i0 == (int)threadIdx.x) __syncthreads();  // the counters are 0
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        if (t[k] < first || t[k] >= past) continue;
+        const int c = (int)(t[k] - v0);
+        if (i0 + k * kThreads < prompt)
+          Count::prompt(counts, c);
+        else
+          Count::made(counts, c);
+      }
     }
     __syncthreads();
   }
   const float* bias = p.bias ? p.bias + row * p.ld_bias : nullptr;
+  const int bias_off = (int)((reinterpret_cast<uintptr_t>(bias + v0) >> 2) & 3u);
   const unsigned* allowed = p.allowed ? p.allowed + row * p.ld_allowed : nullptr;
   const int words = (int)((p.V + 31LL) / 32);
-  auto apply = [&](float v, unsigned c, float b, bool ok) -> float {
+  // Token v's logit x with count c.
+  auto apply = [&](float x, unsigned c, int v, bool ok) -> float {
     if (c) {
-      v = v > 0.f ? __fdiv_rn(v, rep) : __fmul_rn(v, rep);
-      if (c > 1u) v = __fsub_rn(__fsub_rn(v, __fmul_rn(freq, (float)(c >> 1))), pres);
+      x = x > 0.f ? __fdiv_rn(x, rep) : __fmul_rn(x, rep);
+      if (c > 1u) x = __fsub_rn(__fsub_rn(x, __fmul_rn(freq, (float)(c >> 1))), pres);
     }
-    if (bias) v = __fadd_rn(v, b);
-    return ok ? v : -INFINITY;
+    if (bias) x = __fadd_rn(x, __ldg(bias + v));
+    return ok ? x : -INFINITY;
   };
 #pragma unroll
   for (int s = 0; s < SLOTS; ++s) {
     const int slot = (s * kThreads + threadIdx.x) * E::N;
     const int v = v0 + slot;
-    if (v >= 0 && v + E::N <= p.V) {
-      unsigned c[E::N] = {};
-      if (counted) {
+    // A piece of the bias that is not wholly in it may not be read at once.
+    if (v >= 0 && v + E::N <= p.V && (!bias || (v >= 4 && v + E::N + 4 <= p.V))) {
+      const unsigned bits = allowed ? mask_bits(allowed, v, words) : ~0u;
+      constexpr unsigned kAll = (1u << E::N) - 1u;
+      uint4 out = raw[s];
+      if (bias || (bits & kAll) != kAll) {  // else the bits stay as they are (a NaN's too)
+        float f[E::N];
 #pragma unroll
-        for (int i = 0; i < E::N; i += 4) {
-          const uint4 w = *reinterpret_cast<const uint4*>(counts + slot + i);
-          c[i] = w.x, c[i + 1] = w.y, c[i + 2] = w.z, c[i + 3] = w.w;
+        for (int i = 0; i < E::N; ++i) f[i] = E::get(raw[s], i);
+        if (bias) {
+          float b[E::N];
+          load_floats(bias + v, bias_off, b);
+#pragma unroll
+          for (int i = 0; i < E::N; ++i) f[i] = __fadd_rn(f[i], b[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < E::N; ++i) f[i] = (bits >> i) & 1u ? f[i] : -INFINITY;
+        out = E::put(f);
+      }
+      if (counted) {
+#pragma unroll 1
+        for (unsigned m = Count::template used<E::N>(counts, slot); m; m &= m - 1u) {
+          const int i = __ffs(m) - 1;
+          E::put(out, i, apply(E::get(raw[s], i), Count::get(counts, slot + i), v + i, (bits >> i) & 1u));
         }
       }
-      const unsigned bits = allowed ? mask_bits(allowed, v, words) : ~0u;
-      unsigned any = 0;
-#pragma unroll
-      for (int i = 0; i < E::N; ++i) any |= c[i];
-      constexpr unsigned kAll = (1u << E::N) - 1u;
-      if (any || bias || (bits & kAll) != kAll) {  // else the bits stay as they are (a NaN's too)
-        float f[E::N];
-        E::get(raw[s], f);
-#pragma unroll
-        for (int i = 0; i < E::N; ++i) f[i] = apply(f[i], c[i], bias ? __ldg(bias + v + i) : 0.f, (bits >> i) & 1u);
-        raw[s] = E::put(f);
-      }
       if (together) {
-        *reinterpret_cast<uint4*>(y + v) = raw[s];
+        *reinterpret_cast<uint4*>(y + v) = out;
       } else {
-        const T* values = reinterpret_cast<const T*>(&raw[s]);
+        const T* values = reinterpret_cast<const T*>(&out);
 #pragma unroll
         for (int i = 0; i < E::N; ++i) y[v + i] = values[i];
       }
-    } else {  // the row's first and last piece, element by element
+    } else {  // the row's first and last pieces, element by element
+#pragma unroll 1
       for (int i = 0; i < E::N; ++i) {
         const int w = v + i;
         if (w < 0 || w >= p.V) continue;
         const bool ok = !allowed || ((__ldg(allowed + (w >> 5)) >> (w & 31)) & 1u);
-        const unsigned c = counted ? counts[slot + i] : 0u;
+        const unsigned c = counted ? Count::get(counts, slot + i) : 0u;
         if (c || bias || !ok)
-          E::store(y + w, apply(E::load(x + w), c, bias ? __ldg(bias + w) : 0.f, ok));
+          E::store(y + w, apply(E::load(x + w), c, w, ok));
         else
           y[w] = x[w];
       }
@@ -172,13 +266,13 @@ __global__ void __launch_bounds__(kThreads) penalize_kernel(const __grid_constan
   }
 }
 
-template <typename T, int SLOTS>
+template <typename T, int SLOTS, bool WIDE>
 int launch_slots(const PenalizeParams& p, cudaStream_t st) {
   constexpr int N = Elements<T>::N, CHUNK = kThreads * SLOTS * N;
   // One more than V / CHUNK would need: a row may start up to N - 1 elements into a 16-byte piece.
   const long long chunks = ((long long)p.V + N - 1 + CHUNK - 1) / CHUNK, n = chunks * p.R;
   if (n > 0x7fffffffLL) return -2;
-  return launch_dependent(penalize_kernel<T, SLOTS>, dim3((unsigned)n), kThreads, 0, st, 0, p, (int)chunks) ==
+  return launch_dependent(penalize_kernel<T, SLOTS, WIDE>, dim3((unsigned)n), kThreads, 0, st, 0, p, (int)chunks) ==
                  cudaSuccess
              ? 0
              : -1;
@@ -186,9 +280,10 @@ int launch_slots(const PenalizeParams& p, cudaStream_t st) {
 
 template <typename T>
 int launch_t(const PenalizeParams& p, cudaStream_t st) {
+  if (p.L > kNarrowTokens) return launch_slots<T, 2, true>(p, st);
   // Few rows: small chunks, so that a row is spread over more CTAs.
   const long long pieces = (long long)p.R * ((p.V + Elements<T>::N - 1) / Elements<T>::N);
-  return pieces > 148LL * 8 * kThreads ? launch_slots<T, 4>(p, st) : launch_slots<T, 1>(p, st);
+  return pieces > 148LL * 8 * kThreads ? launch_slots<T, 4, false>(p, st) : launch_slots<T, 1, false>(p, st);
 }
 
 }  // namespace
