@@ -188,6 +188,7 @@ int paged_attention(const void* q, const void* k_pages, const void* v_pages, con
     plan.group = p.group;
     plan.cap = (long long)table_width * page;
     plan.max_blocks = at.max_blocks;
+    plan.least_saved = getenv("LS") ? atoll(getenv("LS")) / (4LL * Hkv * D) : 1;
     plan.groups = reinterpret_cast<b2a::SharedGroup*>(base + at.groups);
     plan.seqs = reinterpret_cast<b2a::SharedSeq*>(base + at.seqs);
     plan.total = reinterpret_cast<long long*>(base);
@@ -503,6 +504,7 @@ int b2a_gather_paged(const void* k_pages, const void* v_pages, const long long* 
   p.start_pos = start_pos;
   p.k_out = static_cast<__nv_bfloat16*>(k_out);
   p.v_out = static_cast<__nv_bfloat16*>(v_out);
+  p.out_v8 = api_aligned(k_out, 32) && api_aligned(v_out, 32);
   p.B = B;
   p.Hkv = Hkv;
   p.N = N;

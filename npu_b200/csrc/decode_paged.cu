@@ -828,18 +828,96 @@ __global__ void __launch_bounds__(PagedCfg<D, NT, E4M3>::THREADS, PagedCfg<D, NT
 
 constexpr int kJoinThreads = 256;
 
-// Joins the partials of (sequence, query head) blockIdx.x. The parts are the
-// CTAs from the one with the pair's first tile to the one with its last, which
-// the main kernel has noted (p.place): working it out again here from all
-// lengths took 2 us. D / 4 threads read one part's row; the parts are dealt to
-// such teams in turn and joined in a fixed order. Nothing is read before the
+// The partials of (sequence b, KV head g): the CTAs from the one with the pair's
+// first tile to the one with its last, which the main kernel has noted (p.place):
+// working it out again here from all lengths took 2 us. SHARED: the parts over
+// the shared keys come after those, numbered and placed alike.
+template <bool SHARED>
+struct Parts {
+  int own, all;       // parts
+  long long row0, shared0;  // row of the head's first own and first shared part
+  __device__ __forceinline__ Parts(const DecodePagedParams& p, int b, int g, int r) : own(0), all(0), row0(0), shared0(0) {
+    const long long pair = (long long)b * p.Hkv + g;
+    const int2 at = __ldcg(reinterpret_cast<const int2*>(p.place) + pair);
+    if (tiles_of<64, SHARED>(p, b) > 0) {  // any size of tiles
+      // (Within the CTAs there are, even if the lengths changed under the call.)
+      const int c0 = max(0, min(at.x, p.n_ctas - 1));
+      own = min(at.y, p.n_ctas - 1) - c0 + 1;
+      row0 = (pair + c0) * p.group + r;
+    }
+    all = own;
+    if constexpr (SHARED) {
+      const SharedSeq s = load_seq(p.seqs + b);
+      if (s.skip > 0) {
+        const long long item = (long long)s.block * p.Hkv + g;
+        const int2 of = __ldcg(reinterpret_cast<const int2*>(p.shared_place) + item);
+        const int first = max(0, min(of.x, p.shared_ctas - 1));
+        all += min(of.y, p.shared_ctas - 1) - first + 1;
+        shared0 = (item + first) * p.block_rows + s.row + r;
+      }
+    }
+  }
+  // Part i's (m, l) and columns d .. d + 3 of O.
+  __device__ __forceinline__ void load(const DecodePagedParams& p, int D, int i, int d, float2& ml, float4& o) const {
+    const bool mine = !SHARED || i < own;
+    const long long row = mine ? row0 + (long long)i * p.group : shared0 + (long long)(i - own) * p.block_rows;
+    const float* part_ml = mine ? p.part_ml : p.shared_ml;
+    const float* part_o = mine ? p.part_o : p.shared_o;
+    ml = i < all ? __ldcg(reinterpret_cast<const float2*>(part_ml + 2 * row)) : make_float2(-INFINITY, 0.f);
+    o = i < all ? __ldcg(reinterpret_cast<const float4*>(part_o + row * D + d)) : zero4();
+  }
+};
+
+// Four more parts into (m, l, o).
+template <bool SHARED>
+__device__ __forceinline__ void join_four(const DecodePagedParams& p, const Parts<SHARED>& parts, int D, int i0, int step,
+                                          int d, float& m, float& l, float4& o) {
+  float2 ml[4];
+  float4 po[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) parts.load(p, D, i0 + k * step, d, ml[k], po[k]);
+  const float mn = fmaxf(fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)), m);
+  const float mu = mn == -INFINITY ? 0.f : mn;
+  const float f0 = ex2(m - mu);
+  m = mn;
+  l *= f0;
+  o = make_float4(o.x * f0, o.y * f0, o.z * f0, o.w * f0);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const float f = ex2(ml[k].x - mu);
+    l = fmaf(f, ml[k].y, l);
+    o = axpy(f, po[k], o);
+  }
+}
+
+// Joins the partials of the query heads of many sequences, which have few parts
+// each: a thread takes four columns of a row and all its parts.
+template <int D, bool SHARED>
+__global__ void __launch_bounds__(kJoinThreads)
+    decode_paged_join_rows_kernel(const __grid_constant__ DecodePagedParams p) {
+  const long long x = (long long)blockIdx.x * kJoinThreads + threadIdx.x;
+  const long long row = x / (D / 4);
+  const int d = 4 * (int)(x % (D / 4));
+  if (row >= (long long)p.B * p.Hq) return;
+  const int b = (int)(row / p.Hq), h = (int)(row % p.Hq), g = h / p.group;
+  grid_dep_wait();
+  grid_dep_launch();
+  const float4 gate = p.gate ? load_gate(p, b, h, d) : zero4();
+  const Parts<SHARED> parts(p, b, g, h % p.group);
+  float m = -INFINITY, l = 0.f;
+  float4 o = zero4();
+  for (int i = 0; i < parts.all; i += 4) join_four(p, parts, D, i, 1, d, m, l, o);
+  store_output(p, b, h, d, over(o, l), gate);
+}
+
+// Joins the partials of (sequence, query head) blockIdx.x. D / 4 threads read one
+// part's row; the parts are dealt to such teams in turn and joined in a fixed
+// order. Nothing is read before the
 // wait for the main kernel: what it and the kernels before it have written (the
 // lengths, by the append) is only sure to be seen after that. A dry run before
 // the wait, to fetch the instructions, gained nothing (4 to 4096 sequences of
 // 500 to 1500 keys, 32 / 4 heads of 128: 9.5 us to 1.77 ms without, 9.5 us to
 // 1.80 ms with it).
-// SHARED: the parts over the shared keys come after those, numbered and placed
-// alike.
 template <int D, bool SHARED>
 __global__ void __launch_bounds__(kJoinThreads) decode_paged_join_kernel(const __grid_constant__ DecodePagedParams p) {
   constexpr int TEAM = D / 4, TEAMS = kJoinThreads / TEAM;
@@ -848,59 +926,13 @@ __global__ void __launch_bounds__(kJoinThreads) decode_paged_join_kernel(const _
   const int b = blockIdx.x / p.Hq, h = blockIdx.x % p.Hq;
   const int g = h / p.group, r = h % p.group;
   const int team = threadIdx.x / TEAM, d = 4 * (threadIdx.x % TEAM);
-  const long long pair = (long long)b * p.Hkv + g;
   grid_dep_wait();
   grid_dep_launch();
-  const int2 at = __ldcg(reinterpret_cast<const int2*>(p.place) + pair);
   const float4 gate = p.gate && team == 0 ? load_gate(p, b, h, d) : zero4();
-  int c0 = 0, parts = 0;
-  if (tiles_of<64, SHARED>(p, b) > 0) {  // any size of tiles
-    // (Within the CTAs there are, even if the lengths changed under the call.)
-    c0 = max(0, min(at.x, p.n_ctas - 1));
-    parts = min(at.y, p.n_ctas - 1) - c0 + 1;
-  }
-  const long long row0 = (pair + c0) * p.group + r;  // part i's row: row0 + i group
-  int more = 0;  // parts over shared keys
-  long long shared0 = 0;
-  if constexpr (SHARED) {
-    const SharedSeq s = load_seq(p.seqs + b);
-    if (s.skip > 0) {
-      const long long item = (long long)s.block * p.Hkv + g;
-      const int2 of = __ldcg(reinterpret_cast<const int2*>(p.shared_place) + item);
-      const int first = max(0, min(of.x, p.shared_ctas - 1));
-      more = min(of.y, p.shared_ctas - 1) - first + 1;
-      shared0 = (item + first) * p.block_rows + s.row + r;
-    }
-  }
+  const Parts<SHARED> parts(p, b, g, r);
   float m = -INFINITY, l = 0.f;
   float4 o = zero4();
-  for (int i0 = team; i0 < parts + more; i0 += 4 * TEAMS) {
-    float2 ml[4];
-    float4 po[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int i = i0 + k * TEAMS;
-      const bool own = !SHARED || i < parts;
-      const long long row = own ? row0 + (long long)i * p.group : shared0 + (long long)(i - parts) * p.block_rows;
-      const float* part_ml = own ? p.part_ml : p.shared_ml;
-      const float* part_o = own ? p.part_o : p.shared_o;
-      const bool there = i < parts + more;
-      ml[k] = there ? __ldcg(reinterpret_cast<const float2*>(part_ml + 2 * row)) : make_float2(-INFINITY, 0.f);
-      po[k] = there ? __ldcg(reinterpret_cast<const float4*>(part_o + row * D + d)) : zero4();
-    }
-    const float mn = fmaxf(fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)), m);
-    const float mu = mn == -INFINITY ? 0.f : mn;
-    const float f0 = ex2(m - mu);
-    m = mn;
-    l *= f0;
-    o = make_float4(o.x * f0, o.y * f0, o.z * f0, o.w * f0);
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float f = ex2(ml[k].x - mu);
-      l = fmaf(f, ml[k].y, l);
-      o = axpy(f, po[k], o);
-    }
-  }
+  for (int i0 = team; i0 < parts.all; i0 += 4 * TEAMS) join_four(p, parts, D, i0, TEAMS, d, m, l, o);
   s_o[team][threadIdx.x % TEAM] = o;
   if (d == 0) {
     s_m[team] = m;
@@ -925,6 +957,7 @@ __global__ void __launch_bounds__(kJoinThreads) decode_paged_join_kernel(const _
 }
 
 constexpr int kWholeTiles = 8;
+constexpr long long kManyRows = 1024;
 
 template <int D, int NT, bool SPLIT, bool E4M3, bool SHARED = false>
 int launch_main(const CUtensorMap& tk, const CUtensorMap& tv, const DecodePagedParams& p, long long n,
@@ -934,12 +967,13 @@ int launch_main(const CUtensorMap& tk, const CUtensorMap& tv, const DecodePagedP
   if (n > 0x7fffffffLL) return -1;
   return once.run(
       [] {
-        return cudaFuncSetAttribute(decode_paged_kernel<D, NT, SPLIT, E4M3, SHARED>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+        return cudaFuncSetAttribute(decode_paged_kernel<D, NT, SPLIT, E4M3, SHARED>,
+                                    cudaFuncAttributeMaxDynamicSharedMemorySize,
                                     C::SMEM_BYTES) == cudaSuccess;
       },
       [&] {
-        return launch_dependent(decode_paged_kernel<D, NT, SPLIT, E4M3, SHARED>, dim3((unsigned)n), C::THREADS, C::SMEM_BYTES, st, 0,
-                                tk, tv, p);
+        return launch_dependent(decode_paged_kernel<D, NT, SPLIT, E4M3, SHARED>, dim3((unsigned)n), C::THREADS,
+                                C::SMEM_BYTES, st, 0, tk, tv, p);
       });
 }
 
@@ -966,6 +1000,13 @@ int launch_t(const CUtensorMap& tk, const CUtensorMap& tv, const DecodePagedPara
   else
     rc = launch_n<D, true>(tk, tv, p, p.n_ctas, st);
   if (rc) return rc;
+  // Many rows have few parts each and need no teams (8-bit and shared forms).
+  if ((p.seqs || p.k_scales) && heads >= kManyRows) {
+    const auto join = p.seqs ? decode_paged_join_rows_kernel<D, true> : decode_paged_join_rows_kernel<D, false>;
+    constexpr int ROWS = kJoinThreads / (D / 4);
+    const dim3 grid((unsigned)((heads + ROWS - 1) / ROWS));
+    return launch_dependent(join, grid, kJoinThreads, 0, st, 0, p) == cudaSuccess ? 0 : -1;
+  }
   const auto join = p.seqs ? decode_paged_join_kernel<D, true> : decode_paged_join_kernel<D, false>;
   return launch_dependent(join, dim3((unsigned)heads), kJoinThreads, 0, st, 0, p) == cudaSuccess ? 0 : -1;
 }

@@ -115,12 +115,20 @@ __device__ __forceinline__ long long block_sum_upto(long long x, long long* per_
 }
 
 // Which sequences share what, the numbers of row blocks and units, and the rows
-// of each sequence. One CTA; groups and sequences are dealt to its threads.
+// of each sequence. One CTA; groups and sequences are dealt to its threads. It is
+// all latency, so the groups are worked out in shared memory where they fit (LOCAL).
+constexpr int kLocalGroups = 1024;
+
+template <bool LOCAL>
 __global__ void __launch_bounds__(kPlanThreads)
     decode_shared_plan_kernel(const __grid_constant__ SharedPlanParams p, int block_seqs, int tile_seqs) {
   __shared__ long long s_sum[kPlanThreads / 32];
+  __shared__ SharedGroup s_groups[LOCAL ? kLocalGroups : 1];
+  __shared__ unsigned long long s_saved;  // keys that need not be read again
+  SharedGroup* groups = LOCAL ? s_groups : p.groups;
   grid_dep_wait();
   grid_dep_launch();
+  if (threadIdx.x == 0) s_saved = 0;
   for (int g = threadIdx.x; g < p.n_groups; g += kPlanThreads) {
     int c0, c1;
     const bool good = group_of(p, g, c0, c1);
@@ -132,11 +140,13 @@ __global__ void __launch_bounds__(kPlanThreads)
     s.ref = INT_MAX;
     s.first = c0;
     s.count = good ? c1 - c0 : 0;
-    p.groups[g] = s;
+    groups[g] = s;
   }
   __syncthreads();
   // The first sequence of a group that has all of the prefix names its pages.
+  unsigned long long saved = 0;
   for (int b = threadIdx.x; b < p.B; b += kPlanThreads) {
+    const int len = p.seqlens[b];
     int lo = 0, hi = p.n_groups - 1;  // the last group that starts at or before b
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
@@ -145,52 +155,57 @@ __global__ void __launch_bounds__(kPlanThreads)
       else
         hi = mid - 1;
     }
-    const SharedGroup* s = p.groups + lo;
+    SharedGroup* s = groups + lo;
     const int eff = s->eff;
-    const bool in = eff > 0 && b >= s->first && b - s->first < s->count && min((long long)p.seqlens[b], p.cap) >= eff;
-    if (in) atomicMin(&p.groups[lo].ref, b);
+    const bool in = eff > 0 && b >= s->first && b - s->first < s->count && min((long long)len, p.cap) >= eff;
+    if (in && atomicMin(&s->ref, b) != INT_MAX) saved += eff;  // all but the first to come
     p.seqs[b] = SharedSeq{in ? eff : 0, lo, 0, 0};
   }
+  if (saved) atomicAdd(&s_saved, saved);
   __syncthreads();
+  const bool worth = (long long)s_saved >= p.least_saved;
   long long blocks_before = 0, units_before = 0;
   for (int g0 = 0; g0 < p.n_groups; g0 += kPlanThreads) {
     const int g = g0 + threadIdx.x;
     int blocks = 0, n = 0;
-    if (g < p.n_groups) {
-      const SharedGroup* s = p.groups + g;
-      if (s->eff > 0 && __ldcg(&s->ref) != INT_MAX) {
-        blocks = (s->count + block_seqs - 1) / block_seqs;
-        n = s->eff / kBlock + 1;  // and one for starting and finishing an item
+    if (g < p.n_groups && worth) {
+      const int ref = LOCAL ? groups[g].ref : __ldcg(&groups[g].ref), eff = groups[g].eff;
+      if (eff > 0 && ref != INT_MAX) {
+        blocks = (groups[g].count + block_seqs - 1) / block_seqs;
+        n = eff / kBlock + 1;  // and one for starting and finishing an item
       }
     }
     const long long upto = block_sum_upto(blocks, s_sum) + blocks_before;
     // More blocks than there is room for: offsets that overlap. Left out (and all after them).
     const bool fits = upto <= p.max_blocks;
-    if (!fits) {
-      if (blocks > 0 && p.err) atomicOr(p.err, kErrBadArgs);
-    }
+    if (!fits && blocks > 0 && p.err) atomicOr(p.err, kErrBadArgs);
     const long long units = fits ? (long long)blocks * p.Hkv * n : 0;
     const long long units_upto = block_sum_upto(units, s_sum) + units_before;
     if (g < p.n_groups) {
-      p.groups[g].block0 = (int)(upto - blocks);
-      p.groups[g].unit0 = units_upto - units;
-      if (!fits || blocks == 0) p.groups[g].count = 0;
+      groups[g].block0 = (int)(upto - blocks);
+      groups[g].unit0 = units_upto - units;
+      if (!fits || blocks == 0) groups[g].count = 0;
+      if constexpr (LOCAL) p.groups[g] = groups[g];
     }
-    __syncthreads();
-    if (threadIdx.x == kPlanThreads - 1) {
-      s_sum[0] = upto;
-      s_sum[1] = units_upto;
+    if (g0 + kPlanThreads < p.n_groups) {
+      __syncthreads();
+      if (threadIdx.x == kPlanThreads - 1) {
+        s_sum[0] = upto;
+        s_sum[1] = units_upto;
+      }
+      __syncthreads();
+      blocks_before = s_sum[0];
+      units_before = s_sum[1];
+      __syncthreads();
+    } else if (threadIdx.x == kPlanThreads - 1) {
+      *p.total = units_upto;
     }
-    __syncthreads();
-    blocks_before = s_sum[0];
-    units_before = s_sum[1];
-    __syncthreads();
   }
-  if (threadIdx.x == 0) *p.total = units_before;
+  __syncthreads();
   for (int b = threadIdx.x; b < p.B; b += kPlanThreads) {
-    SharedSeq s = p.seqs[b];
+    SharedSeq s = p.seqs[b];  // this thread's own
     if (s.skip == 0) continue;
-    const SharedGroup* g = p.groups + s.block;  // still the group's number
+    const SharedGroup* g = groups + s.block;  // still the group's number
     if (g->count == 0) {
       s = SharedSeq{0, 0, 0, 0};
     } else {
@@ -570,8 +585,9 @@ int decode_shared_max_ctas(int sms) { return sms; }
 
 int launch_decode_shared(int D, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
                          const SharedPlanParams& plan, const DecodeSharedParams& p, cudaStream_t st) {
-  if (launch_dependent(decode_shared_plan_kernel, dim3(1), kPlanThreads, 0, st, 0, plan,
-                       decode_shared_block_seqs(D, plan.group), 128 / plan.group) != cudaSuccess)
+  const auto kernel = plan.n_groups <= kLocalGroups ? decode_shared_plan_kernel<true> : decode_shared_plan_kernel<false>;
+  if (launch_dependent(kernel, dim3(1), kPlanThreads, 0, st, 0, plan, decode_shared_block_seqs(D, plan.group),
+                       128 / plan.group) != cudaSuccess)
     return -1;
   switch (D) {
     case 64: return launch_t<64>(tq, tk, tv, p, st);

@@ -33,6 +33,7 @@ struct SharedPlanParams {
   int B, Hkv, group;
   long long cap;       // keys a table can name
   int max_blocks;      // row blocks the workspace has room for
+  long long least_saved;  // keys: sharing that saves reading fewer is not worth its launches
   SharedGroup* groups;  // [n_groups]
   SharedSeq* seqs;      // [B]
   long long* total;     // units of work

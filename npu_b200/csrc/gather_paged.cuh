@@ -21,6 +21,7 @@ struct GatherPagedParams {
   int start_pos;
   __nv_bfloat16* k_out;  // [N, Hkv, D] contiguous
   __nv_bfloat16* v_out;
+  int out_v8;  // both are 32-byte aligned
   int B, Hkv;
   long long N;
   int* err;

@@ -10,13 +10,14 @@
 // each step rounded by itself in fp32, the result to the logits' type once.
 //
 // Bound by memory: logits read once and written once. A CTA takes a chunk of
-// one row's vocabulary, requests its logits, counts the row's tokens that fall
-// into the chunk in shared memory (bit 0: in the prompt, from bit 1 on: the
-// count) and applies bias and mask to the registers. The few elements that a
-// token names (some 1 %, but a lane in almost every warp) are then done one by
-// one in a loop: with the penalties' code in line for each of a lane's elements the
-// kernel took twice the instructions. The tokens are read once per chunk, from
-// L2 after the first, eight requests at a time.
+// one row's vocabulary. Bias and mask are applied to its logits in registers
+// while its tokens are on their way; the tokens that fall into the chunk are
+// counted in shared memory (bit 0: in the prompt, from bit 1 on: the count), and
+// the first to come upon an element puts it on a list. The listed elements, some 1 %,
+// are done one by one from the logits as they were and stored over the others:
+// looking at every element's counter instead took most of the kernel's
+// instructions (256 rows of 131071, 4096 tokens: 75 us). The tokens are read once
+// per chunk, from L2 after the first, eight requests at a time.
 #include "capi_internal.cuh"
 #include "penalize.cuh"
 
@@ -31,119 +32,87 @@ struct Elements;  // 16 bytes of logits
 template <>
 struct Elements<float> {
   static constexpr int N = 4;
-  static __device__ __forceinline__ float get(const uint4& w, int i) {
-    return __uint_as_float(i & 2 ? (i & 1 ? w.w : w.z) : (i & 1 ? w.y : w.x));
-  }
-  static __device__ __forceinline__ void put(uint4& w, int i, float v) {
-    const uint32_t u = __float_as_uint(v);
-    if (i == 0) w.x = u;
-    if (i == 1) w.y = u;
-    if (i == 2) w.z = u;
-    if (i == 3) w.w = u;
+  static __device__ __forceinline__ void get(const uint4& w, float (&x)[4]) {
+    x[0] = __uint_as_float(w.x), x[1] = __uint_as_float(w.y), x[2] = __uint_as_float(w.z), x[3] = __uint_as_float(w.w);
   }
   static __device__ __forceinline__ uint4 put(const float (&x)[4]) {
     return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
   }
+  // -inf wherever the element's bit is not set.
+  static __device__ __forceinline__ void keep(uint4& w, unsigned bits) {
+    if (!(bits & 1u)) w.x = 0xff800000u;
+    if (!(bits & 2u)) w.y = 0xff800000u;
+    if (!(bits & 4u)) w.z = 0xff800000u;
+    if (!(bits & 8u)) w.w = 0xff800000u;
+  }
   static __device__ __forceinline__ float load(const float* p) { return *p; }
-  static __device__ __forceinline__ void store(float* p, float x) { *p = x; }
+  static __device__ __forceinline__ float round(float x) { return x; }
 };
 template <>
 struct Elements<__nv_bfloat16> {
   static constexpr int N = 8;
-  static __device__ __forceinline__ float get(const uint4& w, int i) {
-    const uint32_t u = i & 4 ? (i & 2 ? w.w : w.z) : (i & 2 ? w.y : w.x);
-    return __uint_as_float(i & 1 ? u & 0xffff0000u : u << 16);
-  }
-  static __device__ __forceinline__ void put(uint4& w, int i, float v) {
-    const uint32_t u = pack_bf16x2(v, v), keep = i & 1 ? 0x0000ffffu : 0xffff0000u;
-    if (i >> 1 == 0) w.x = (w.x & keep) | (u & ~keep);
-    if (i >> 1 == 1) w.y = (w.y & keep) | (u & ~keep);
-    if (i >> 1 == 2) w.z = (w.z & keep) | (u & ~keep);
-    if (i >> 1 == 3) w.w = (w.w & keep) | (u & ~keep);
+  static __device__ __forceinline__ void get(const uint4& w, float (&x)[8]) {
+    const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[2 * i] = __uint_as_float(ws[i] << 16);
+      x[2 * i + 1] = __uint_as_float(ws[i] & 0xffff0000u);
+    }
   }
   static __device__ __forceinline__ uint4 put(const float (&x)[8]) {
     return make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]),
                       pack_bf16x2(x[6], x[7]));
   }
+  // Bit k of four is moved to the sign of byte k; prmt with bit 3 of a selector set repeats that byte's sign.
+  template <int BYTES>
+  static __device__ __forceinline__ uint32_t signs(uint32_t x) {
+    uint32_t r;
+    asm("prmt.b32 %0, %1, 0, %2;" : "=r"(r) : "r"(x), "n"(BYTES));
+    return r;
+  }
+  static __device__ __forceinline__ void keep(uint4& w, unsigned bits) {
+    const uint32_t lo = (bits & 15u) * 0x10204080u, hi = ((bits >> 4) & 15u) * 0x10204080u;
+    auto pick = [](uint32_t x, uint32_t m) { return (x & m) | (0xff80ff80u & ~m); };
+    w.x = pick(w.x, signs<0x9988>(lo));
+    w.y = pick(w.y, signs<0xbbaa>(lo));
+    w.z = pick(w.z, signs<0x9988>(hi));
+    w.w = pick(w.w, signs<0xbbaa>(hi));
+  }
   static __device__ __forceinline__ float load(const __nv_bfloat16* p) { return __bfloat162float(*p); }
-  static __device__ __forceinline__ void store(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
+  static __device__ __forceinline__ __nv_bfloat16 round(float x) { return __float2bfloat16_rn(x); }
 };
 
-// Counters of a chunk, two to a word while a row has few enough tokens.
+// Counters of a chunk as wide as its logits, which take their places once the counts are known: 16 bits hold the
+// counts of rows of up to kNarrowTokens tokens.
 constexpr int kNarrowTokens = 32767;
-template <bool WIDE>
-struct Counters {
-  static constexpr int BITS = WIDE ? 32 : 16;
-  static __device__ __forceinline__ void prompt(unsigned* c, int i) {
-    atomicOr(c + (WIDE ? i : i >> 1), 1u << (WIDE ? 0 : 16 * (i & 1)));
-  }
-  static __device__ __forceinline__ void made(unsigned* c, int i) {
-    atomicAdd(c + (WIDE ? i : i >> 1), 2u << (WIDE ? 0 : 16 * (i & 1)));
-  }
-  static __device__ __forceinline__ unsigned get(const unsigned* c, int i) {
-    return WIDE ? c[i] : reinterpret_cast<const uint16_t*>(c)[i];
-  }
-  // Which of the N counters from number i on (a multiple of N) are not 0.
-  template <int N>
-  static __device__ __forceinline__ unsigned used(const unsigned* c, int i) {
-    constexpr int WORDS = N * BITS / 32;
-    uint32_t w[WORDS];
-    if constexpr (WORDS == 2) {
-      *reinterpret_cast<uint2*>(w) = *reinterpret_cast<const uint2*>(c + i * BITS / 32);
-    } else {
-#pragma unroll
-      for (int k = 0; k < WORDS; k += 4)
-        *reinterpret_cast<uint4*>(w + k) = *reinterpret_cast<const uint4*>(c + i * BITS / 32 + k);
-    }
-    unsigned any = 0, m = 0;
-#pragma unroll
-    for (int k = 0; k < WORDS; ++k) any |= w[k];
-    if (any) {
-#pragma unroll
-      for (int k = 0; k < WORDS; ++k) {
-        if constexpr (WIDE)
-          m |= w[k] ? 1u << k : 0u;
-        else
-          m |= (w[k] & 0xffffu ? 1u << (2 * k) : 0u) | (w[k] >> 16 ? 2u << (2 * k) : 0u);
-      }
-    }
-    return m;
-  }
-};
-
-// Bits [v, v + 8) of a row's mask of `words` words (those that exist).
-__device__ __forceinline__ unsigned mask_bits(const unsigned* row, int v, int words) {
-  const int w = v >> 5;
-  const unsigned lo = __ldg(row + w);
-  const unsigned hi = (v & 31) > 24 && w + 1 < words ? __ldg(row + w + 1) : 0u;
-  return __funnelshift_r(lo, hi, v & 31);
+template <typename Word>
+__device__ __forceinline__ unsigned count_token(Word* counts, int i, bool prompt) {  // the count before
+  constexpr bool NARROW = sizeof(Word) == 2;
+  const int at = NARROW ? 16 * (i & 1) : 0;
+  unsigned* word = reinterpret_cast<unsigned*>(counts) + (NARROW ? i >> 1 : i);
+  const unsigned old = prompt ? atomicOr(word, 1u << at) : atomicAdd(word, 2u << at);
+  return NARROW ? (old >> at) & 0xffffu : old;
 }
 
-// N floats from p on, which lies `off` floats past a 16-byte boundary (the same for the whole CTA). Reads no further
-// than the 16-byte pieces that hold them.
-template <int N>
-__device__ __forceinline__ void load_floats(const float* p, int off, float (&b)[N]) {
-  const float4* q = reinterpret_cast<const float4*>(p - off);
-  float a[N + 4];
+// x += the floats OFF places into a.
+template <int N, int OFF>
+__device__ __forceinline__ void add_floats(const float (&a)[N + 4], float (&x)[N]) {
 #pragma unroll
-  for (int k = 0; k < N / 4; ++k) *reinterpret_cast<float4*>(a + 4 * k) = __ldg(q + k);
-  if (off == 0) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) b[i] = a[i];
-    return;
-  }
-  *reinterpret_cast<float4*>(a + N) = __ldg(q + N / 4);
-#pragma unroll
-  for (int i = 0; i < N; ++i) b[i] = off == 1 ? a[i + 1] : (off == 2 ? a[i + 2] : a[i + 3]);
+  for (int i = 0; i < N; ++i) x[i] = __fadd_rn(x[i], a[i + OFF]);
 }
 
-// SLOTS: 16-byte pieces of logits per thread.
-template <typename T, int SLOTS, bool WIDE>
-__global__ void __launch_bounds__(kThreads) penalize_kernel(const __grid_constant__ PenalizeParams p, int chunks) {
+__device__ __forceinline__ float4 zero4() { return make_float4(0.f, 0.f, 0.f, 0.f); }
+
+// SLOTS: 16-byte pieces of logits per thread (256 threads of 4, four CTAs an SM: at 256 rows of 131071 bf16 63 us, with
+// threads or pieces twice as many 65, with six CTAs and 40 registers 82). Word: a counter.
+template <typename T, int SLOTS, typename Word>
+__global__ void __launch_bounds__(kThreads, 4) penalize_kernel(const __grid_constant__ PenalizeParams p, int chunks) {
   using E = Elements<T>;
-  using Count = Counters<WIDE>;
   constexpr int CHUNK = kThreads * SLOTS * E::N;
-  __shared__ __align__(16) unsigned counts[CHUNK * Count::BITS / 32];
+  static_assert(CHUNK <= 65536 && sizeof(Word) >= sizeof(T), "list entries, results in the counters' places");
+  __shared__ __align__(16) Word counts[CHUNK];
+  __shared__ uint16_t list[CHUNK];
+  __shared__ int listed;
   grid_dep_wait();
   grid_dep_launch();
   const int row = blockIdx.x / chunks;
@@ -153,6 +122,7 @@ __global__ void __launch_bounds__(kThreads) penalize_kernel(const __grid_constan
   const int shift = (int)((reinterpret_cast<uintptr_t>(x) & 15u) / sizeof(T));
   const bool together = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(y)) & 15u) == 0;
   const int v0 = (int)(blockIdx.x % chunks) * CHUNK - shift;
+  if (v0 >= p.V) return;  // (the last chunk of a row that starts on a boundary)
   uint4 raw[SLOTS];
 #pragma unroll
   for (int s = 0; s < SLOTS; ++s) {
@@ -170,126 +140,167 @@ __global__ void __launch_bounds__(kThreads) penalize_kernel(const __grid_constan
     if (given != n && p.err && threadIdx.x == 0) atomicOr(p.err, kErrBadArgs);
   }
   const bool counted = n > 0 && (rep != 1.f || freq != 0.f || pres != 0.f);
-  if (counted) {
-    const int prompt = p.prompt_lengths ? p.prompt_lengths[row] : 0;
-    for (int i = threadIdx.x; i < CHUNK * Count::BITS / 128; i += kThreads)
-      reinterpret_cast<uint4*>(counts)[i] = make_uint4(0u, 0u, 0u, 0u);
-    const long long first = max(v0, 0), past = min((long long)v0 + CHUNK, (long long)p.V);
-    constexpr int AHEAD = 8;
-    for (int i0 = threadIdx.x; i0 - (int)threadIdx.x < n; i0 += AHEAD * kThreads) {
-      long long t[AHEAD];
+  const int prompt = counted && p.prompt_lengths ? p.prompt_lengths[row] : 0;
+  // The row's tokens i0, i0 + kThreads, .. less the chunk's first one: as unsigned numbers below `span` if they are in
+  // the chunk.
+  constexpr int AHEAD = 8;
+  const int first = max(v0, 0);
+  const unsigned span = (unsigned)(min((long long)v0 + CHUNK, (long long)p.V) - first);
+  const long long step = p.tokens_step * (p.tokens_64 ? 8 : 4) * kThreads;  // bytes
+  const char* tokens = static_cast<const char*>(p.tokens) +
+                       (row * p.tokens_row + (int)threadIdx.x * p.tokens_step) * (p.tokens_64 ? 8 : 4);
+  unsigned t[AHEAD];
+  auto request = [&](int i0) {
+    const char* at = tokens + i0 / kThreads * step;
+    if (p.tokens_64) {
+      uint2 w[AHEAD];
 #pragma unroll
       for (int k = 0; k < AHEAD; ++k) {
-        const int i = i0 + k * kThreads;
-        t[k] = -1;
-        if (i >= n) continue;
-        const long long at = row * p.tokens_row + i * p.tokens_step;
-        t[k] = p.tokens_64 ? __ldg(static_cast<const long long*>(p.tokens) + at)
-                           : (long long)__ldg(static_cast<const int*>(p.tokens) + at);
+        w[k] = make_uint2(0u, ~0u);
+        if (i0 + k * kThreads + (int)threadIdx.x < n) w[k] = __ldg(reinterpret_cast<const uint2*>(at + k * step));
       }
-      if (i0 == (int)threadIdx.x) __syncthreads();  // the counters are 0
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) t[k] = w[k].y ? ~0u : w[k].x - (unsigned)first;
+    } else {
 #pragma unroll
       for (int k = 0; k < AHEAD; ++k) {
-        if (t[k] < first || t[k] >= past) continue;
-        const int c = (int)(t[k] - v0);
-        if (i0 + k * kThreads < prompt)
-          Count::prompt(counts, c);
-        else
-          Count::made(counts, c);
+        t[k] = ~0u;
+        if (i0 + k * kThreads + (int)threadIdx.x < n)
+          t[k] = __ldg(reinterpret_cast<const unsigned*>(at + k * step)) - (unsigned)first;
+      }
+    }
+  };
+  if (counted) {
+    request(0);
+    for (int i = threadIdx.x; i < (int)(CHUNK * sizeof(Word) / 16); i += kThreads)
+      reinterpret_cast<uint4*>(counts)[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (threadIdx.x == 0) listed = 0;
+  }
+  // Bias and mask: every element.
+  const float* bias = p.bias ? p.bias + row * p.ld_bias : nullptr;
+  const unsigned* allowed = p.allowed ? p.allowed + row * p.ld_allowed : nullptr;
+  const int words = (int)((p.V + 31LL) / 32);
+  // Pieces that do not lie wholly in the row (nor those of the bias that hold them) go element by element.
+  auto whole = [&](int v) { return v >= (bias ? 4 : 0) && v + E::N + (bias ? 4 : 0) <= p.V; };
+  auto is_allowed = [&](int v) { return !allowed || ((__ldg(allowed + (v >> 5)) >> (v & 31)) & 1u); };
+  unsigned mask[SLOTS];
+  const int bias_off = (int)((reinterpret_cast<uintptr_t>(bias + v0) >> 2) & 3u);
+  if (allowed) {  // every piece's words requested before the first is used
+    unsigned lo[SLOTS], hi[SLOTS];
+#pragma unroll
+    for (int s = 0; s < SLOTS; ++s) {
+      const int v = v0 + (s * kThreads + threadIdx.x) * E::N, w = v >> 5;
+      lo[s] = v >= 0 && w < words ? __ldg(allowed + w) : 0u;
+      hi[s] = v >= 0 && (v & 31) > 32 - E::N && w + 1 < words ? __ldg(allowed + w + 1) : 0u;
+    }
+    if (!bias) {
+#pragma unroll
+      for (int s = 0; s < SLOTS; ++s)
+        E::keep(raw[s], __funnelshift_r(lo[s], hi[s], (v0 + (int)threadIdx.x * E::N) & 31));
+    } else {
+#pragma unroll
+      for (int s = 0; s < SLOTS; ++s) mask[s] = __funnelshift_r(lo[s], hi[s], (v0 + (int)threadIdx.x * E::N) & 31);
+    }
+  }
+  if (bias) {
+#pragma unroll
+    for (int s = 0; s < SLOTS; ++s) {
+      const int v = v0 + (s * kThreads + threadIdx.x) * E::N;
+      // The 16-byte pieces that hold these floats.
+      const float4* q = reinterpret_cast<const float4*>(bias + v - bias_off);
+      float a[E::N + 4], f[E::N];
+#pragma unroll
+      for (int k = 0; k <= E::N / 4; ++k) *reinterpret_cast<float4*>(a + 4 * k) = whole(v) ? __ldg(q + k) : zero4();
+      E::get(raw[s], f);
+      if (bias_off < 2)
+        bias_off == 0 ? add_floats<E::N, 0>(a, f) : add_floats<E::N, 1>(a, f);
+      else
+        bias_off == 2 ? add_floats<E::N, 2>(a, f) : add_floats<E::N, 3>(a, f);
+      raw[s] = E::put(f);
+      if (allowed) E::keep(raw[s], mask[s]);
+    }
+  }
+  int named = 0;  // elements of the chunk that tokens name
+  if (counted) {
+    __syncthreads();  // the counters are 0
+    for (int i0 = 0; i0 < n; i0 += AHEAD * kThreads) {
+      if (i0 > 0) request(i0);
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        if (t[k] >= span) continue;
+        const int c = (int)t[k] + first - v0;
+        if (count_token(counts, c, i0 + k * kThreads + (int)threadIdx.x < prompt) == 0)
+          list[atomicAdd(&listed, 1)] = (uint16_t)c;
       }
     }
     __syncthreads();
-  }
-  const float* bias = p.bias ? p.bias + row * p.ld_bias : nullptr;
-  const int bias_off = (int)((reinterpret_cast<uintptr_t>(bias + v0) >> 2) & 3u);
-  const unsigned* allowed = p.allowed ? p.allowed + row * p.ld_allowed : nullptr;
-  const int words = (int)((p.V + 31LL) / 32);
-  // Token v's logit x with count c.
-  auto apply = [&](float x, unsigned c, int v, bool ok) -> float {
-    if (c) {
-      x = x > 0.f ? __fdiv_rn(x, rep) : __fmul_rn(x, rep);
-      if (c > 1u) x = __fsub_rn(__fsub_rn(x, __fmul_rn(freq, (float)(c >> 1))), pres);
+    named = listed;
+    for (int e = threadIdx.x; e < named; e += kThreads) {
+      const int c = list[e], v = v0 + c;
+      const unsigned count = (unsigned)counts[c] >> 1;
+      float f = E::load(x + v);
+      f = f > 0.f ? __fdiv_rn(f, rep) : __fmul_rn(f, rep);
+      if (count > 0) f = __fsub_rn(__fsub_rn(f, __fmul_rn(freq, (float)count)), pres);
+      if (bias) f = __fadd_rn(f, __ldg(bias + v));
+      if (!is_allowed(v)) f = -INFINITY;
+      *reinterpret_cast<T*>(counts + c) = E::round(f);
     }
-    if (bias) x = __fadd_rn(x, __ldg(bias + v));
-    return ok ? x : -INFINITY;
-  };
+    __syncthreads();  // the logits have been read (they may be the output), the results are there
+  }
 #pragma unroll
   for (int s = 0; s < SLOTS; ++s) {
-    const int slot = (s * kThreads + threadIdx.x) * E::N;
-    const int v = v0 + slot;
-    // A piece of the bias that is not wholly in it may not be read at once.
-    if (v >= 0 && v + E::N <= p.V && (!bias || (v >= 4 && v + E::N + 4 <= p.V))) {
-      const unsigned bits = allowed ? mask_bits(allowed, v, words) : ~0u;
-      constexpr unsigned kAll = (1u << E::N) - 1u;
-      uint4 out = raw[s];
-      if (bias || (bits & kAll) != kAll) {  // else the bits stay as they are (a NaN's too)
-        float f[E::N];
-#pragma unroll
-        for (int i = 0; i < E::N; ++i) f[i] = E::get(raw[s], i);
-        if (bias) {
-          float b[E::N];
-          load_floats(bias + v, bias_off, b);
-#pragma unroll
-          for (int i = 0; i < E::N; ++i) f[i] = __fadd_rn(f[i], b[i]);
-        }
-#pragma unroll
-        for (int i = 0; i < E::N; ++i) f[i] = (bits >> i) & 1u ? f[i] : -INFINITY;
-        out = E::put(f);
-      }
-      if (counted) {
-#pragma unroll 1
-        for (unsigned m = Count::template used<E::N>(counts, slot); m; m &= m - 1u) {
-          const int i = __ffs(m) - 1;
-          E::put(out, i, apply(E::get(raw[s], i), Count::get(counts, slot + i), v + i, (bits >> i) & 1u));
-        }
-      }
+    const int v = v0 + (s * kThreads + threadIdx.x) * E::N;
+    if (whole(v)) {
       if (together) {
-        *reinterpret_cast<uint4*>(y + v) = out;
+        *reinterpret_cast<uint4*>(y + v) = raw[s];
       } else {
-        const T* values = reinterpret_cast<const T*>(&out);
+        const T* values = reinterpret_cast<const T*>(&raw[s]);
 #pragma unroll
         for (int i = 0; i < E::N; ++i) y[v + i] = values[i];
       }
-    } else {  // the row's first and last pieces, element by element
+    } else {
 #pragma unroll 1
       for (int i = 0; i < E::N; ++i) {
         const int w = v + i;
         if (w < 0 || w >= p.V) continue;
-        const bool ok = !allowed || ((__ldg(allowed + (w >> 5)) >> (w & 31)) & 1u);
-        const unsigned c = counted ? Count::get(counts, slot + i) : 0u;
-        if (c || bias || !ok)
-          E::store(y + w, apply(E::load(x + w), c, w, ok));
-        else
-          y[w] = x[w];
+        T value = x[w];
+        if (bias) value = E::round(__fadd_rn(E::load(x + w), __ldg(bias + w)));
+        if (!is_allowed(w)) value = E::round(-INFINITY);
+        y[w] = value;
       }
     }
   }
+  if (named > 0) {
+    __syncthreads();  // after the other elements
+    for (int e = threadIdx.x; e < named; e += kThreads) y[v0 + list[e]] = *reinterpret_cast<const T*>(counts + list[e]);
+  }
 }
 
-template <typename T, int SLOTS, bool WIDE>
+template <typename T, int SLOTS, typename Word>
 int launch_slots(const PenalizeParams& p, cudaStream_t st) {
   constexpr int N = Elements<T>::N, CHUNK = kThreads * SLOTS * N;
   // One more than V / CHUNK would need: a row may start up to N - 1 elements into a 16-byte piece.
   const long long chunks = ((long long)p.V + N - 1 + CHUNK - 1) / CHUNK, n = chunks * p.R;
   if (n > 0x7fffffffLL) return -2;
-  return launch_dependent(penalize_kernel<T, SLOTS, WIDE>, dim3((unsigned)n), kThreads, 0, st, 0, p, (int)chunks) ==
+  return launch_dependent(penalize_kernel<T, SLOTS, Word>, dim3((unsigned)n), kThreads, 0, st, 0, p, (int)chunks) ==
                  cudaSuccess
              ? 0
              : -1;
 }
 
-template <typename T>
+// Few rows: small chunks, so that a row is spread over more CTAs.
+template <typename T, typename Word>
 int launch_t(const PenalizeParams& p, cudaStream_t st) {
-  if (p.L > kNarrowTokens) return launch_slots<T, 2, true>(p, st);
-  // Few rows: small chunks, so that a row is spread over more CTAs.
+    constexpr int MOST = sizeof(Word) > sizeof(T) ? 2 : 4;
   const long long pieces = (long long)p.R * ((p.V + Elements<T>::N - 1) / Elements<T>::N);
-  return pieces > 148LL * 8 * kThreads ? launch_slots<T, 4, false>(p, st) : launch_slots<T, 1, false>(p, st);
+  return pieces > 148LL * 8 * kThreads ? launch_slots<T, MOST, Word>(p, st) : launch_slots<T, 1, Word>(p, st);
 }
 
 }  // namespace
 
 int launch_penalize(const PenalizeParams& p, cudaStream_t st) {
-  return p.logits_bf16 ? launch_t<__nv_bfloat16>(p, st) : launch_t<float>(p, st);
+  if (!p.logits_bf16) return launch_t<float, uint32_t>(p, st);
+  return p.L <= kNarrowTokens ? launch_t<__nv_bfloat16, uint16_t>(p, st) : launch_t<__nv_bfloat16, uint32_t>(p, st);
 }
 
 }  // namespace b2a
