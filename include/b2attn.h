@@ -421,13 +421,15 @@ B2A_API int b2a_decode_paged_e4m3(const void* q, const void* k_pages, const void
  * with the last prefix_lens[g] % 64 of them. A pair of offsets that is not a stretch
  * of the sequences, groups that overlap or a prefix outside 0 .. table_width * page
  * report B2A_ERR_DEVICE_BAD_LEN; nothing is shared then for such a group (the prefix
- * is cut). bf16 pools. Workspace: b2a_decode_paged_shared_workspace_bytes.
+ * is cut). Where sharing would save reading fewer than least_saved_bytes bytes of
+ * keys and values (below 0: 36 MB, about where it begins to pay) nothing is
+ * shared. bf16 pools. Workspace: b2a_decode_paged_shared_workspace_bytes.
  */
 B2A_API size_t b2a_decode_paged_shared_workspace_bytes(int B, int Hq, int Hkv, int D, int n_groups);
 B2A_API int b2a_decode_paged_shared(const void* q, const void* k_pages, const void* v_pages, const int* block_table,
                                     long long table_ld, int table_width, const int* seqlens, const int* prefix_lens,
-                                    const int* cu_groups, int n_groups, const void* gate, void* o, int B, int Hq,
-                                    int Hkv, int n_pages, int page, int D, const long long* q_strides,
+                                    const int* cu_groups, int n_groups, long long least_saved_bytes,
+                                    const void* gate, void* o, int B, int Hq, int Hkv, int n_pages, int page, int D, const long long* q_strides,
                                     const long long* k_strides, const long long* v_strides,
                                     const long long* gate_strides, const long long* o_strides, int gate_bf16,
                                     float scale, int out_fp32, void* workspace, size_t workspace_bytes, void* stream);

@@ -72,7 +72,13 @@ struct SharedPrefix {
   const int* prefix_lens;
   const int* cu_groups;
   int n_groups;
+  long long least_saved;  // bytes, below 0: kLeastSaved
 };
+
+// Reading that sharing must save to be worth its plan and its kernel, in bytes. Measured against not sharing (same
+// launches), 32 / 4 heads of 128 and 9 / 3 of 64: 20.2 us against 18.4 at 31 MB, 22.2 / 23.2 at 42, 20.5 / 21.8 at
+// 63, 20.5 / 27.9 at 126, 27.4 / 40.2 at 252.
+constexpr long long kLeastSaved = 36LL << 20;
 
 // Where the shared form's scratch is, behind that of the sequences' own keys.
 struct SharedLayout {
@@ -97,8 +103,8 @@ SharedLayout shared_layout(int B, int Hq, int Hkv, int D, int n_groups) {
 
 int paged_attention(const void* q, const void* k_pages, const void* v_pages, const int* block_table,
                     const float* k_scales, const float* v_scales, const long long* kss, const long long* vss,
-                    const SharedPrefix* shared, long long table_ld, int table_width, const int* seqlens, const void* gate, void* o, int B,
-                    int Hq, int Hkv, int n_pages, int page, int D, const long long* qs, const long long* ks,
+                    const SharedPrefix* shared, long long table_ld, int table_width, const int* seqlens,
+                    const void* gate, void* o, int B, int Hq, int Hkv, int n_pages, int page, int D, const long long* qs, const long long* ks,
                     const long long* vs, const long long* gs, const long long* os, int gate_bf16, float scale,
                     int out_fp32, void* workspace, size_t workspace_bytes, void* stream) {
   if (!q || !k_pages || !v_pages || !block_table || !seqlens || !o || !qs || !ks || !vs || !os || (gate && !gs))
@@ -174,8 +180,12 @@ int paged_attention(const void* q, const void* k_pages, const void* v_pages, con
   scratch += b2a::api_align256(rows * D * sizeof(float));
   p.part_ml = reinterpret_cast<float*>(scratch);
   p.place = reinterpret_cast<int*>(scratch + b2a::api_align256(rows * 2 * sizeof(float)));
-  // Few keys, or one sequence: every sequence reads its own (one launch).
-  if (shared && B > 1 && b2a::decode_paged_splits(table_width, page)) {
+  // Few keys, or one sequence: every sequence reads its own (one launch). So too where sharing could not save enough; how
+  // much it does save is known on the device, where the plan looks again.
+  const long long bytes_a_key = 4LL * Hkv * D;
+  const long long least = !shared ? 0 : (shared->least_saved < 0 ? kLeastSaved : shared->least_saved);
+  if (shared && B > 1 && b2a::decode_paged_splits(table_width, page) &&
+      (B - 1) * ((long long)table_width * page) >= least / bytes_a_key) {
     const SharedLayout at = shared_layout(B, Hq, Hkv, D, shared->n_groups);
     char* base = reinterpret_cast<char*>(b2a::api_align256(reinterpret_cast<uintptr_t>(workspace) + own));
     b2a::SharedPlanParams plan{};
@@ -188,7 +198,7 @@ int paged_attention(const void* q, const void* k_pages, const void* v_pages, con
     plan.group = p.group;
     plan.cap = (long long)table_width * page;
     plan.max_blocks = at.max_blocks;
-    plan.least_saved = getenv("LS") ? atoll(getenv("LS")) / (4LL * Hkv * D) : 1;
+    plan.least_saved = std::max(1LL, least / bytes_a_key);
     plan.groups = reinterpret_cast<b2a::SharedGroup*>(base + at.groups);
     plan.seqs = reinterpret_cast<b2a::SharedSeq*>(base + at.seqs);
     plan.total = reinterpret_cast<long long*>(base);
@@ -407,13 +417,14 @@ size_t b2a_decode_paged_shared_workspace_bytes(int B, int Hq, int Hkv, int D, in
 
 int b2a_decode_paged_shared(const void* q, const void* k_pages, const void* v_pages, const int* block_table,
                             long long table_ld, int table_width, const int* seqlens, const int* prefix_lens,
-                            const int* cu_groups, int n_groups, const void* gate, void* o, int B, int Hq, int Hkv,
+                            const int* cu_groups, int n_groups, long long least_saved_bytes, const void* gate, void* o,
+                            int B, int Hq, int Hkv,
                             int n_pages, int page, int D, const long long* qs, const long long* ks,
                             const long long* vs, const long long* gs, const long long* os, int gate_bf16, float scale,
                             int out_fp32, void* workspace, size_t workspace_bytes, void* stream) {
   if (!prefix_lens || n_groups <= 0 || (!cu_groups && n_groups != 1)) return B2A_ERR_INVALID_ARG;
   if (!api_aligned(prefix_lens, 4) || !api_aligned(cu_groups, 4)) return B2A_ERR_ALIGNMENT;
-  const SharedPrefix shared{prefix_lens, cu_groups, n_groups};
+  const SharedPrefix shared{prefix_lens, cu_groups, n_groups, least_saved_bytes};
   return paged_attention(q, k_pages, v_pages, block_table, nullptr, nullptr, nullptr, nullptr, &shared, table_ld,
                          table_width, seqlens, gate, o, B, Hq, Hkv, n_pages, page, D, qs, ks, vs, gs, os, gate_bf16,
                          scale, out_fp32, workspace, workspace_bytes, stream);

@@ -338,10 +338,17 @@ __global__ void __launch_bounds__(PagedCfg<D, NT, E4M3>::THREADS, PagedCfg<D, NT
   volatile int* abort_flag = &bars->abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  grid_dep_wait();
+  // SHARED: the kernel before is the one over the shared keys, of which nothing
+  // is read here. It let this one start after its own wait for the plan, so the
+  // plan and all before it is done; the two run side by side, and this one ends
+  // after that one (end_shared), so that the joining kernel sees both.
+  if constexpr (!SHARED) grid_dep_wait();
   // The next kernel (the joining one when SPLIT) may take SM slots as they
   // free up.
   grid_dep_launch();
+  auto end_shared = [] {
+    if constexpr (SHARED) grid_dep_wait();
+  };
   if (p.err && blockIdx.x == 0)
     for (int b = threadIdx.x; b < p.B; b += C::THREADS)
       if (p.seqlens[b] < 0 || p.seqlens[b] > (long long)p.table_width * p.page) atomicOr(p.err, kErrBadArgs);
@@ -350,7 +357,10 @@ __global__ void __launch_bounds__(PagedCfg<D, NT, E4M3>::THREADS, PagedCfg<D, NT
     const long long total = total_units<C::TK, SHARED>(p), share = share_of(total, p.n_ctas);
     from = blockIdx.x * share;
     count = min(share, total - from);
-    if (count <= 0) return;
+    if (count <= 0) {
+      end_shared();
+      return;
+    }
   }
   using W = Walk<C::TK, SHARED>;
   auto start = [&]() -> W {
@@ -359,7 +369,10 @@ __global__ void __launch_bounds__(PagedCfg<D, NT, E4M3>::THREADS, PagedCfg<D, NT
     return W(b, blockIdx.x % p.Hkv, keys_of(p, b));
   };
   W w = start();
-  if (SPLIT && !w.valid()) return;
+  if (SPLIT && !w.valid()) {
+    end_shared();
+    return;
+  }
   if (!SPLIT && w.tiles == 0) {
     for (int e = 4 * threadIdx.x; e < p.group * D; e += 4 * C::THREADS)
       store_output(p, w.b, w.g * p.group + e / D, e % D, zero4(), zero4());
@@ -824,6 +837,7 @@ __global__ void __launch_bounds__(PagedCfg<D, NT, E4M3>::THREADS, PagedCfg<D, NT
       ++pair;
     } while (w.next(p));
   }
+  end_shared();
 }
 
 constexpr int kJoinThreads = 256;

@@ -45,8 +45,8 @@ struct SharedCfg {
   static constexpr int KV_CHUNK = kBlock * 128;
   static constexpr int Q_BYTES = KCH * Q_CHUNK;
   static constexpr int TILE_BYTES = KCH * KV_CHUNK;  // 64 keys of K or V
-  static constexpr int KST = D == 64 ? 8 : (D == 128 ? 4 : 2);
-  static constexpr int VST = D == 64 ? 8 : (D == 128 ? 4 : 3);
+  static constexpr int KST = D == 256 ? 2 : 4;
+  static constexpr int VST = D == 256 ? 3 : 4;
   static constexpr int OFF_K = NQT * Q_BYTES;
   static constexpr int OFF_V = OFF_K + KST * TILE_BYTES;
   static constexpr int OFF_BAR = OFF_V + VST * TILE_BYTES;
@@ -90,7 +90,8 @@ __device__ __forceinline__ void tma_load_5d(void* smem_dst, const CUtensorMap* m
 }
 
 // ---------------------------------------------------------------- plan
-constexpr int kPlanThreads = 512;
+constexpr int kPlanThreads = 256;
+constexpr int kPlanWarps = kPlanThreads / 32;
 
 // Offsets of group g, and whether they are a stretch of the sequences.
 __device__ __forceinline__ bool group_of(const SharedPlanParams& p, int g, int& c0, int& c1) {
@@ -99,35 +100,47 @@ __device__ __forceinline__ bool group_of(const SharedPlanParams& p, int g, int& 
   return c0 >= 0 && c1 >= c0 && c1 <= p.B;
 }
 
-// Inclusive sum over the block's threads.
-__device__ __forceinline__ long long block_sum_upto(long long x, long long* per_warp) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+// Inclusive sums of x and y over the warp.
+__device__ __forceinline__ void warp_sums_upto(long long& x, long long& y) {
+  const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int off = 1; off < 32; off *= 2) {
-    const long long y = __shfl_up_sync(0xffffffffu, x, off);
-    if (lane >= off) x += y;
+    const long long u = __shfl_up_sync(0xffffffffu, x, off), v = __shfl_up_sync(0xffffffffu, y, off);
+    if (lane >= off) x += u, y += v;
   }
+}
+
+// Inclusive sums over the block's threads.
+__device__ __forceinline__ void block_sums_upto(long long& x, long long& y, long long (*per_warp)[2]) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  warp_sums_upto(x, y);
   __syncthreads();
-  if (lane == 31) per_warp[warp] = x;
+  if (lane == 31) per_warp[warp][0] = x, per_warp[warp][1] = y;
   __syncthreads();
-  for (int w = 0; w < warp; ++w) x += per_warp[w];
-  return x;
+  long long u = lane < kPlanWarps ? per_warp[lane][0] : 0, v = lane < kPlanWarps ? per_warp[lane][1] : 0;
+  const long long own_u = u, own_v = v;
+  warp_sums_upto(u, v);
+  x += __shfl_sync(0xffffffffu, u - own_u, warp);
+  y += __shfl_sync(0xffffffffu, v - own_v, warp);
 }
 
 // Which sequences share what, the numbers of row blocks and units, and the rows
 // of each sequence. One CTA; groups and sequences are dealt to its threads. It is
-// all latency, so the groups are worked out in shared memory where they fit (LOCAL).
+// all latency, so the groups are worked out in shared memory where they fit
+// (LOCAL), and atomics are few.
 constexpr int kLocalGroups = 1024;
 
 template <bool LOCAL>
 __global__ void __launch_bounds__(kPlanThreads)
     decode_shared_plan_kernel(const __grid_constant__ SharedPlanParams p, int block_seqs, int tile_seqs) {
-  __shared__ long long s_sum[kPlanThreads / 32];
+  __shared__ long long s_sum[kPlanWarps][2];
   __shared__ SharedGroup s_groups[LOCAL ? kLocalGroups : 1];
   __shared__ unsigned long long s_saved;  // keys that need not be read again
   SharedGroup* groups = LOCAL ? s_groups : p.groups;
+  const int lane = threadIdx.x & 31;
   grid_dep_wait();
   grid_dep_launch();
+  const int first_len = (int)threadIdx.x < p.B ? p.seqlens[threadIdx.x] : 0;
   if (threadIdx.x == 0) s_saved = 0;
   for (int g = threadIdx.x; g < p.n_groups; g += kPlanThreads) {
     int c0, c1;
@@ -144,80 +157,89 @@ __global__ void __launch_bounds__(kPlanThreads)
   }
   __syncthreads();
   // The first sequence of a group that has all of the prefix names its pages.
+  SharedSeq first_seq{};  // of this thread's first sequence
   unsigned long long saved = 0;
-  for (int b = threadIdx.x; b < p.B; b += kPlanThreads) {
-    const int len = p.seqlens[b];
+  for (int b0 = 0; b0 < p.B; b0 += kPlanThreads) {
+    const int b = b0 + threadIdx.x;
     int lo = 0, hi = p.n_groups - 1;  // the last group that starts at or before b
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
-      if (p.cu_groups[mid] <= b)
+      if (groups[mid].first <= b)
         lo = mid;
       else
         hi = mid - 1;
     }
-    SharedGroup* s = groups + lo;
-    const int eff = s->eff;
-    const bool in = eff > 0 && b >= s->first && b - s->first < s->count && min((long long)len, p.cap) >= eff;
-    if (in && atomicMin(&s->ref, b) != INT_MAX) saved += eff;  // all but the first to come
-    p.seqs[b] = SharedSeq{in ? eff : 0, lo, 0, 0};
+    const int eff = groups[lo].eff, from = groups[lo].first, count = groups[lo].count;
+    const long long len = b0 == 0 ? first_len : (b < p.B ? p.seqlens[b] : 0);
+    const bool in = b < p.B && eff > 0 && b >= from && b - from < count && min(len, p.cap) >= eff;
+    const int key = in ? lo : -1, before = __shfl_up_sync(0xffffffffu, key, 1);
+    if (in && (lane == 0 || before != key)) atomicMin(&groups[lo].ref, b);  // one of a warp's of a group
+    saved += in ? eff : 0;
+    const SharedSeq s{in ? eff : 0, lo, 0, 0};
+    if (b0 == 0) first_seq = s;
+    if (b0 > 0 && b < p.B) p.seqs[b] = s;
   }
-  if (saved) atomicAdd(&s_saved, saved);
+  __syncthreads();
+  auto ref_of = [&](int g) { return LOCAL ? groups[g].ref : __ldcg(&groups[g].ref); };
+  for (int g = threadIdx.x; g < p.n_groups; g += kPlanThreads)  // one of each group does read them
+    if (groups[g].eff > 0 && ref_of(g) != INT_MAX) saved -= groups[g].eff;
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) saved += __shfl_xor_sync(0xffffffffu, saved, off);
+  if (lane == 0 && saved) atomicAdd(&s_saved, saved);
   __syncthreads();
   const bool worth = (long long)s_saved >= p.least_saved;
   long long blocks_before = 0, units_before = 0;
   for (int g0 = 0; g0 < p.n_groups; g0 += kPlanThreads) {
     const int g = g0 + threadIdx.x;
     int blocks = 0, n = 0;
-    if (g < p.n_groups && worth) {
-      const int ref = LOCAL ? groups[g].ref : __ldcg(&groups[g].ref), eff = groups[g].eff;
-      if (eff > 0 && ref != INT_MAX) {
-        blocks = (groups[g].count + block_seqs - 1) / block_seqs;
-        n = eff / kBlock + 1;  // and one for starting and finishing an item
-      }
+    if (g < p.n_groups && worth && groups[g].eff > 0 && ref_of(g) != INT_MAX) {
+      blocks = (groups[g].count + block_seqs - 1) / block_seqs;
+      n = groups[g].eff / kBlock + 1;  // and one for starting and finishing an item
     }
-    const long long upto = block_sum_upto(blocks, s_sum) + blocks_before;
-    // More blocks than there is room for: offsets that overlap. Left out (and all after them).
+    long long upto = blocks, units_upto = (long long)blocks * p.Hkv * n;
+    const long long units = units_upto;
+    block_sums_upto(upto, units_upto, s_sum);
+    upto += blocks_before;
+    units_upto += units_before;
+    // More blocks than there is room for: offsets that overlap. Left out, and all after them.
     const bool fits = upto <= p.max_blocks;
     if (!fits && blocks > 0 && p.err) atomicOr(p.err, kErrBadArgs);
-    const long long units = fits ? (long long)blocks * p.Hkv * n : 0;
-    const long long units_upto = block_sum_upto(units, s_sum) + units_before;
     if (g < p.n_groups) {
       groups[g].block0 = (int)(upto - blocks);
       groups[g].unit0 = units_upto - units;
       if (!fits || blocks == 0) groups[g].count = 0;
       if constexpr (LOCAL) p.groups[g] = groups[g];
     }
+    // The units end where the first group that does not fit begins.
+    const bool last = g == p.n_groups - 1;
+    if (fits ? last : upto - blocks <= p.max_blocks) *p.total = fits ? units_upto : units_upto - units;
     if (g0 + kPlanThreads < p.n_groups) {
       __syncthreads();
-      if (threadIdx.x == kPlanThreads - 1) {
-        s_sum[0] = upto;
-        s_sum[1] = units_upto;
-      }
+      if (threadIdx.x == kPlanThreads - 1) s_sum[0][0] = upto, s_sum[0][1] = units_upto;
       __syncthreads();
-      blocks_before = s_sum[0];
-      units_before = s_sum[1];
-      __syncthreads();
-    } else if (threadIdx.x == kPlanThreads - 1) {
-      *p.total = units_upto;
+      blocks_before = s_sum[0][0];
+      units_before = s_sum[0][1];
     }
   }
   __syncthreads();
   for (int b = threadIdx.x; b < p.B; b += kPlanThreads) {
-    SharedSeq s = p.seqs[b];  // this thread's own
-    if (s.skip == 0) continue;
-    const SharedGroup* g = groups + s.block;  // still the group's number
-    if (g->count == 0) {
-      s = SharedSeq{0, 0, 0, 0};
-    } else {
+    SharedSeq s = b < kPlanThreads ? first_seq : p.seqs[b];
+    if (s.skip > 0) {
+      const SharedGroup* g = groups + s.block;  // still the group's number
       const int i = b - g->first, at = i % block_seqs;
-      s.block = g->block0 + i / block_seqs;
-      s.row = at / tile_seqs * 128 + at % tile_seqs * p.group;
+      if (g->count == 0)
+        s = SharedSeq{0, 0, 0, 0};
+      else
+        s = SharedSeq{s.skip, g->block0 + i / block_seqs, at / tile_seqs * 128 + at % tile_seqs * p.group, 0};
     }
     p.seqs[b] = s;
   }
 }
 
 // ---------------------------------------------------------------- the shared keys
+// Units per CTA, at least: fewer CTAs leave the others' SMs to the kernel over
+// each sequence's own keys (measured with 1 and 2 as well: up to 5 us slower at
+// 8 to 16 sequences behind 2048 to 8192 keys, 2 us faster behind 1024).
 constexpr int kMinShare = 4;
 
 // A stretch of the units, item by item.
@@ -231,18 +253,30 @@ struct ItemWalk {
   int begin, end;  // key blocks of the item in the stretch
   __device__ __forceinline__ int blocks() const { return (g.count + block_seqs - 1) / block_seqs; }
   __device__ __forceinline__ int units() const { return g.eff / kBlock + 1; }
-  __device__ __forceinline__ ItemWalk(const DecodeSharedParams& params, int seqs, long long from, long long count)
+  // `mine`: the lane's group of up to 32, requested before `from` was known.
+  __device__ __forceinline__ ItemWalk(const DecodeSharedParams& params, int seqs, long long from, long long count,
+                                      SharedGroup mine)
       : p(params), block_seqs(seqs), left(count) {
-    int lo = 0, hi = p.n_groups - 1;  // the last group that starts at or before the unit
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (__ldcg(&p.groups[mid].unit0) <= from)
-        lo = mid;
-      else
-        hi = mid - 1;
+    // The last group that starts at or before the unit: 32 looked at a time, and the last 32 read whole.
+    const int lane = threadIdx.x & 31;
+    int lo = 0, len = p.n_groups;
+    while (len > 32) {
+      const int step = (len + 31) / 32;
+      const bool before =
+          lane * step < len && (lane == 0 || __ldcg(&p.groups[lo + lane * step].unit0) <= from);
+      const int hit = 31 - __clz(__ballot_sync(0xffffffffu, before));
+      len = min(step, len - hit * step);
+      lo += hit * step;
     }
-    gi = lo;
-    g = load_group(p.groups + gi);
+    if (p.n_groups > 32 && lane < len) mine = load_group(p.groups + lo + lane);
+    const int hit = 31 - __clz(__ballot_sync(0xffffffffu, lane < len && (lane == 0 || mine.unit0 <= from)));
+    gi = lo + hit;
+    g.eff = __shfl_sync(0xffffffffu, mine.eff, hit);
+    g.ref = __shfl_sync(0xffffffffu, mine.ref, hit);
+    g.first = __shfl_sync(0xffffffffu, mine.first, hit);
+    g.count = __shfl_sync(0xffffffffu, mine.count, hit);
+    g.block0 = __shfl_sync(0xffffffffu, mine.block0, hit);
+    g.unit0 = __shfl_sync(0xffffffffu, mine.unit0, hit);
     const long long into = from - g.unit0;
     item = (int)(into / units());
     begin = (int)(into % units());
@@ -326,6 +360,7 @@ __global__ void __launch_bounds__(SharedCfg<D>::THREADS, 1)
 
   grid_dep_wait();
   grid_dep_launch();
+  const SharedGroup mine = p.n_groups <= 32 && lane < p.n_groups ? load_group(p.groups + lane) : SharedGroup{};
   const long long total = __ldcg(p.total);
   const long long share = max((total + p.n_ctas - 1) / p.n_ctas, (long long)kMinShare);
   const long long from = blockIdx.x * share, count = min(share, total - from);
@@ -334,7 +369,7 @@ __global__ void __launch_bounds__(SharedCfg<D>::THREADS, 1)
   };
 
   if (count > 0) {
-    ItemWalk w(p, block_seqs, from, count);
+    ItemWalk w(p, block_seqs, from, count, mine);
     if (warp == 0 && w.valid()) {
       // ---------------------------------------------------------- producer
       // Lane x copies 64 columns of one run of box_rows keys of a tile. The

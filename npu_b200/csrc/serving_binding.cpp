@@ -223,11 +223,12 @@ Tensor decode_paged(const Tensor& q, const Tensor& k_pages, const Tensor& v_page
 Tensor decode_paged_shared(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table,
                            const Tensor& seqlens, const Tensor& prefix_lens, const OptTensor& cu_groups,
                            std::optional<double> scale, at::ScalarType out_dtype, const OptTensor& workspace,
-                           const OptTensor& out, const OptTensor& gate) {
+                           const OptTensor& out, const OptTensor& gate, std::optional<int64_t> min_saved) {
   need_bf16("q", q, 3);
   const c10::Device device = q.device();
   need_bf16("k_pages", k_pages, 4, &device);
   need_bf16("v_pages", v_pages, 4, &device);
+  if (min_saved && *min_saved < 0) refuse("min_saved_bytes must not be negative, got ", *min_saved);
   const int64_t B = q.size(0), Hq = q.size(1), D = q.size(2), Hkv = k_pages.size(1),
                 groups = cu_groups ? cu_groups->numel() - 1 : 1;
   if (k_pages.size(3) != D || v_pages.sizes() != k_pages.sizes())
@@ -259,7 +260,7 @@ Tensor decode_paged_shared(const Tensor& q, const Tensor& k_pages, const Tensor&
   check(b2a_decode_paged_shared(q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), table.data_ptr<int>(),
                                 table.stride(0), as_int("table width", table.size(1)), seqlens.data_ptr<int>(),
                                 prefix_lens.data_ptr<int>(), static_cast<int*>(pointer(cu_groups)), (int)groups,
-                                pointer(gate), o.data_ptr(), (int)B, (int)Hq, (int)Hkv,
+                                min_saved.value_or(-1), pointer(gate), o.data_ptr(), (int)B, (int)Hq, (int)Hkv,
                                 as_int("n_pages", k_pages.size(0)), as_int("page", k_pages.size(2)), (int)D,
                                 Strides(q, 2), Strides(k_pages, 3), Strides(v_pages, 3), gs, Strides(o, 2),
                                 gate && gate->scalar_type() == at::kBFloat16,

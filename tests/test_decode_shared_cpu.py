@@ -10,20 +10,20 @@ INVALID, ALIGNMENT = _lib.B2A_ERR_INVALID_ARG, _lib.B2A_ERR_ALIGNMENT
 
 
 def call(**over):
-    a = dict(q=FAKE, k=FAKE, v=FAKE, t=FAKE, ld=80, w=80, sl=FAKE, pre=FAKE, cu=FAKE, n=2, gate=None, o=FAKE, B=4, Hq=8,
-             Hkv=2, pages=20, page=64, D=128, qs=(1024, 128), ks=(16384, 8192, 128), vs=(16384, 8192, 128),
+    a = dict(q=FAKE, k=FAKE, v=FAKE, t=FAKE, ld=80, w=80, sl=FAKE, pre=FAKE, cu=FAKE, n=2, least=-1, gate=None, o=FAKE,
+             B=4, Hq=8, Hkv=2, pages=20, page=64, D=128, qs=(1024, 128), ks=(16384, 8192, 128), vs=(16384, 8192, 128),
              gs=(1024, 128), os=(1024, 128), gb=1, scale=0.1, fp32=1, ws=FAKE, wsb=1 << 30)
     a.update(over)
     return _lib.load().b2a_decode_paged_shared(
-        a["q"], a["k"], a["v"], a["t"], a["ld"], a["w"], a["sl"], a["pre"], a["cu"], a["n"], a["gate"], a["o"], a["B"],
-        a["Hq"], a["Hkv"], a["pages"], a["page"], a["D"], LL2(*a["qs"]), LL3(*a["ks"]), LL3(*a["vs"]), LL2(*a["gs"]),
-        LL2(*a["os"]), a["gb"], a["scale"], a["fp32"], a["ws"], a["wsb"], None)
+        a["q"], a["k"], a["v"], a["t"], a["ld"], a["w"], a["sl"], a["pre"], a["cu"], a["n"], a["least"], a["gate"],
+        a["o"], a["B"], a["Hq"], a["Hkv"], a["pages"], a["page"], a["D"], LL2(*a["qs"]), LL3(*a["ks"]), LL3(*a["vs"]),
+        LL2(*a["gs"]), LL2(*a["os"]), a["gb"], a["scale"], a["fp32"], a["ws"], a["wsb"], None)
 
 
 @pytest.mark.parametrize("over,code", [
     (dict(pre=None), INVALID), (dict(n=0), INVALID), (dict(cu=None), INVALID), (dict(pre=FAKE + 2), ALIGNMENT),
-    (dict(cu=FAKE + 1), ALIGNMENT), (dict(t=None), INVALID), (dict(page=24), INVALID), (dict(D=96), _lib.B2A_ERR_HEAD_DIM),
-    (dict(Hq=34), _lib.B2A_ERR_GQA), (dict(k=FAKE + 8), ALIGNMENT), (dict(ks=(16384, 8192, 130)), ALIGNMENT),
+    (dict(cu=FAKE + 1), ALIGNMENT), (dict(t=None), INVALID), (dict(page=24), INVALID),
+    (dict(D=96), _lib.B2A_ERR_HEAD_DIM), (dict(Hq=34), _lib.B2A_ERR_GQA), (dict(k=FAKE + 8), ALIGNMENT), (dict(ks=(16384, 8192, 130)), ALIGNMENT),
     (dict(ws=None), _lib.B2A_ERR_WORKSPACE), (dict(wsb=1000), _lib.B2A_ERR_WORKSPACE), (dict(scale=0.0), INVALID),
 ])
 def test_refused(over, code):

@@ -1,4 +1,5 @@
 """SmolLMB200.generate with an 8-bit cache, a shared prefix and penalties: the serving operators together."""
+import functools
 import math
 
 import pytest
@@ -56,12 +57,15 @@ def test_prefix_pages():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("least", [0, None])
 @pytest.mark.parametrize("page,length", [(16, 700), (64, 640), (48, 1000), (64, 40)])
-def test_steps_behind_a_prefix_match_the_reference(cuda_dev, weights, page, length):
+def test_steps_behind_a_prefix_match_the_reference(cuda_dev, weights, page, length, least, monkeypatch):
     """The prefix once, five prompts behind it, then three steps fed the reference's greedy tokens: logits and top-1 of
     every sequence, as prompts without a shared prefix are tested."""
     from npu_b200 import api
 
+    # These sizes are below where sharing pays: 0 shares all the same.
+    monkeypatch.setattr(api, "decode_paged_shared", functools.partial(api.decode_paged_shared, min_saved_bytes=least))
     ref, model = SmolLM(weights, Config(n_layers=4)), model_on(cuda_dev, weights)
     (prefix,), ids = some(3, length), some(7, *LENS)
     shared = length // page * page
