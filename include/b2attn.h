@@ -397,8 +397,8 @@ B2A_API int b2a_rope_append_paged_e4m3(const void* q, const void* k, const void*
 /*
  * b2a_decode_paged over an 8-bit cache as b2a_rope_append_paged_e4m3 writes it:
  * key and value are the e4m3 numbers times their row's scale, not rounded to
- * fewer bits on the way (e4m3's NaN, stored under a NaN scale only, is not looked
- * for by itself). Slots and scales past a sequence's end may hold anything.
+ * fewer bits on the way. Scales are positive; one below 2^-100 counts as 2^-100.
+ * Slots and scales past a sequence's end may hold anything.
  */
 B2A_API int b2a_decode_paged_e4m3(const void* q, const void* k_pages, const void* v_pages, const float* k_scales,
                                   const float* v_scales, const long long* k_scale_strides,
@@ -429,10 +429,11 @@ B2A_API size_t b2a_decode_paged_shared_workspace_bytes(int B, int Hq, int Hkv, i
 B2A_API int b2a_decode_paged_shared(const void* q, const void* k_pages, const void* v_pages, const int* block_table,
                                     long long table_ld, int table_width, const int* seqlens, const int* prefix_lens,
                                     const int* cu_groups, int n_groups, long long least_saved_bytes,
-                                    const void* gate, void* o, int B, int Hq, int Hkv, int n_pages, int page, int D, const long long* q_strides,
-                                    const long long* k_strides, const long long* v_strides,
-                                    const long long* gate_strides, const long long* o_strides, int gate_bf16,
-                                    float scale, int out_fp32, void* workspace, size_t workspace_bytes, void* stream);
+                                    const void* gate, void* o, int B, int Hq, int Hkv, int n_pages, int page, int D,
+                                    const long long* q_strides, const long long* k_strides,
+                                    const long long* v_strides, const long long* gate_strides,
+                                    const long long* o_strides, int gate_bf16, float scale, int out_fp32,
+                                    void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * k and v of a stretch of each sequence out of a paged cache, as packed rows

@@ -28,7 +28,8 @@ BINDING_SOURCE = CSRC / "serving_binding.cpp"
 
 SOURCES = ["capi.cu", "capi_serving.cu", "prefill.cu", "prefill_pair.cu", "prefill_d256.cu",
            "prefill_packed_d64.cu", "decode.cu", "decode_noalloc.cu", "rope_append.cu", "rope_append_paged.cu",
-           "gather_paged.cu", "decode_paged.cu", "decode_shared.cu", "penalize.cu", "sample.cu", "diag.cu", "host_pipeline.cu"]
+           "gather_paged.cu", "decode_paged.cu", "decode_shared.cu", "penalize.cu", "sample.cu", "diag.cu",
+           "host_pipeline.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FAST_MATH = ["--use_fast_math"]
 # The same without its replacement of expf and the like by approximations.

@@ -104,9 +104,10 @@ SharedLayout shared_layout(int B, int Hq, int Hkv, int D, int n_groups) {
 int paged_attention(const void* q, const void* k_pages, const void* v_pages, const int* block_table,
                     const float* k_scales, const float* v_scales, const long long* kss, const long long* vss,
                     const SharedPrefix* shared, long long table_ld, int table_width, const int* seqlens,
-                    const void* gate, void* o, int B, int Hq, int Hkv, int n_pages, int page, int D, const long long* qs, const long long* ks,
-                    const long long* vs, const long long* gs, const long long* os, int gate_bf16, float scale,
-                    int out_fp32, void* workspace, size_t workspace_bytes, void* stream) {
+                    const void* gate, void* o, int B, int Hq, int Hkv, int n_pages, int page, int D,
+                    const long long* qs, const long long* ks, const long long* vs, const long long* gs,
+                    const long long* os, int gate_bf16, float scale, int out_fp32, void* workspace,
+                    size_t workspace_bytes, void* stream) {
   if (!q || !k_pages || !v_pages || !block_table || !seqlens || !o || !qs || !ks || !vs || !os || (gate && !gs))
     return B2A_ERR_INVALID_ARG;
   if (B <= 0 || Hq <= 0 || Hkv <= 0 || n_pages <= 0 || page <= 0 || page % 16 || table_width <= 0 ||
@@ -180,8 +181,8 @@ int paged_attention(const void* q, const void* k_pages, const void* v_pages, con
   scratch += b2a::api_align256(rows * D * sizeof(float));
   p.part_ml = reinterpret_cast<float*>(scratch);
   p.place = reinterpret_cast<int*>(scratch + b2a::api_align256(rows * 2 * sizeof(float)));
-  // Few keys, or one sequence: every sequence reads its own (one launch). So too where sharing could not save enough; how
-  // much it does save is known on the device, where the plan looks again.
+  // Few keys, or one sequence: every sequence reads its own (one launch). So too where sharing could not save enough;
+  // how much it does save is known on the device, where the plan looks again.
   const long long bytes_a_key = 4LL * Hkv * D;
   const long long least = !shared ? 0 : (shared->least_saved < 0 ? kLeastSaved : shared->least_saved);
   if (shared && B > 1 && b2a::decode_paged_splits(table_width, page) &&

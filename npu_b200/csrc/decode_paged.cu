@@ -850,7 +850,8 @@ template <bool SHARED>
 struct Parts {
   int own, all;       // parts
   long long row0, shared0;  // row of the head's first own and first shared part
-  __device__ __forceinline__ Parts(const DecodePagedParams& p, int b, int g, int r) : own(0), all(0), row0(0), shared0(0) {
+  __device__ __forceinline__ Parts(const DecodePagedParams& p, int b, int g, int r)
+      : own(0), all(0), row0(0), shared0(0) {
     const long long pair = (long long)b * p.Hkv + g;
     const int2 at = __ldcg(reinterpret_cast<const int2*>(p.place) + pair);
     if (tiles_of<64, SHARED>(p, b) > 0) {  // any size of tiles
@@ -882,22 +883,24 @@ struct Parts {
   }
 };
 
-// Four more parts into (m, l, o).
-template <bool SHARED>
-__device__ __forceinline__ void join_four(const DecodePagedParams& p, const Parts<SHARED>& parts, int D, int i0, int step,
-                                          int d, float& m, float& l, float4& o) {
-  float2 ml[4];
-  float4 po[4];
+// N more parts into (m, l, o).
+template <int N, bool SHARED>
+__device__ __forceinline__ void join_parts(const DecodePagedParams& p, const Parts<SHARED>& parts, int D, int i0,
+                                           int step, int d, float& m, float& l, float4& o) {
+  float2 ml[N];
+  float4 po[N];
 #pragma unroll
-  for (int k = 0; k < 4; ++k) parts.load(p, D, i0 + k * step, d, ml[k], po[k]);
-  const float mn = fmaxf(fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)), m);
+  for (int k = 0; k < N; ++k) parts.load(p, D, i0 + k * step, d, ml[k], po[k]);
+  float mn = m;
+#pragma unroll
+  for (int k = 0; k < N; ++k) mn = fmaxf(mn, ml[k].x);
   const float mu = mn == -INFINITY ? 0.f : mn;
   const float f0 = ex2(m - mu);
   m = mn;
   l *= f0;
   o = make_float4(o.x * f0, o.y * f0, o.z * f0, o.w * f0);
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
+  for (int k = 0; k < N; ++k) {
     const float f = ex2(ml[k].x - mu);
     l = fmaf(f, ml[k].y, l);
     o = axpy(f, po[k], o);
@@ -920,7 +923,7 @@ __global__ void __launch_bounds__(kJoinThreads)
   const Parts<SHARED> parts(p, b, g, h % p.group);
   float m = -INFINITY, l = 0.f;
   float4 o = zero4();
-  for (int i = 0; i < parts.all; i += 4) join_four(p, parts, D, i, 1, d, m, l, o);
+  for (int i = 0; i < parts.all; i += 8) join_parts<8>(p, parts, D, i, 1, d, m, l, o);
   store_output(p, b, h, d, over(o, l), gate);
 }
 
@@ -946,7 +949,7 @@ __global__ void __launch_bounds__(kJoinThreads) decode_paged_join_kernel(const _
   const Parts<SHARED> parts(p, b, g, r);
   float m = -INFINITY, l = 0.f;
   float4 o = zero4();
-  for (int i0 = team; i0 < parts.all; i0 += 4 * TEAMS) join_four(p, parts, D, i0, TEAMS, d, m, l, o);
+  for (int i0 = team; i0 < parts.all; i0 += 4 * TEAMS) join_parts<4>(p, parts, D, i0, TEAMS, d, m, l, o);
   s_o[team][threadIdx.x % TEAM] = o;
   if (d == 0) {
     s_m[team] = m;

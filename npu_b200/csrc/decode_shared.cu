@@ -522,9 +522,9 @@ __global__ void __launch_bounds__(SharedCfg<D>::THREADS, 1)
       const float sl2 = p.scale_log2;
       int c = 0;  // key blocks of this tile so far
       bool ok = true;
-      // PV of block i is done. A parity tells a phase from its neighbours only, so a warp must neither miss one nor fall
-      // two behind: with a barrier for either buffer, PV(i + 2) needs this warp's P(i + 2), which comes after its wait
-      // for PV(i) (in block i + 2 at the latest).
+      // PV of block i is done. A parity tells a phase from its neighbours only, so a warp must neither miss one nor
+      // fall two behind: with a barrier for either buffer, PV(i + 2) needs this warp's P(i + 2), which comes after its
+      // wait for PV(i) (in block i + 2 at the latest).
       auto product_done = [&](int i) { return wait_all(&bars->pv_done[t][i & 1], (uint32_t)(i >> 1) & 1u); };
       do {
         if (w.seqs() <= t * tile_seqs) continue;
@@ -620,7 +620,8 @@ int decode_shared_max_ctas(int sms) { return sms; }
 
 int launch_decode_shared(int D, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
                          const SharedPlanParams& plan, const DecodeSharedParams& p, cudaStream_t st) {
-  const auto kernel = plan.n_groups <= kLocalGroups ? decode_shared_plan_kernel<true> : decode_shared_plan_kernel<false>;
+  const bool local = plan.n_groups <= kLocalGroups;
+  const auto kernel = local ? decode_shared_plan_kernel<true> : decode_shared_plan_kernel<false>;
   if (launch_dependent(kernel, dim3(1), kPlanThreads, 0, st, 0, plan, decode_shared_block_seqs(D, plan.group),
                        128 / plan.group) != cudaSuccess)
     return -1;

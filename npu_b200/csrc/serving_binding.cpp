@@ -434,8 +434,8 @@ Tensor sample(const Tensor& logits, const OptTensor& noise, const py::handle& te
 }
 
 Tensor penalize(const Tensor& logits, const OptTensor& tokens, const OptTensor& lengths,
-                const OptTensor& prompt_lengths, const py::handle& repetition, const py::handle& frequency, const py::handle& presence,
-                const OptTensor& bias, const OptTensor& allowed, const OptTensor& out) {
+                const OptTensor& prompt_lengths, const py::handle& repetition, const py::handle& frequency,
+                const py::handle& presence, const OptTensor& bias, const OptTensor& allowed, const OptTensor& out) {
   const bool bf16 = logits.scalar_type() == at::kBFloat16;
   if (!logits.is_cuda() || logits.dim() != 2 || (logits.size(1) > 1 && logits.stride(1) != 1) ||
       (logits.scalar_type() != at::kFloat && !bf16))

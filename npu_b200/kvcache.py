@@ -116,7 +116,7 @@ class PagedKVCache:
         are the first of each (not counted in capacities), and it cannot be released before them."""
         if prefix is not None and (prefix.cache is not self or prefix.batch != 1 or prefix.released
                                    or prefix.prefix is not None or prefix.capacities[0] % self.page):
-            raise ValueError("prefix must be one unreleased sequence of this cache with whole pages and no prefix itself")
+            raise ValueError("prefix must be one unreleased sequence of this cache with whole pages and no prefix")
         capacities = [int(c) for c in capacities]
         if not capacities or min(capacities) < 1:
             raise ValueError("capacities must be one or more positive token counts")

@@ -249,7 +249,8 @@ class SmolLMB200:
     # ------------------------------------------------------------ sequences of different lengths
     def new_paged_cache(self, n_pages: int, page: int = 64, dtype: torch.dtype = torch.bfloat16) -> PagedKVCache:
         """dtype torch.float8_e4m3fn: an 8-bit cache, about half the memory and traffic."""
-        return PagedKVCache(self.cfg.n_layers, n_pages, self.cfg.n_kv_heads, page, self.cfg.head_dim, self.device, dtype)
+        c = self.cfg
+        return PagedKVCache(c.n_layers, n_pages, c.n_kv_heads, page, c.head_dim, self.device, dtype)
 
     def _attention_packed(self, lw: dict, h: torch.Tensor, seqs: PagedSequences, i: int,
                           cu_seqlens: Optional[torch.Tensor]) -> torch.Tensor:

@@ -23,7 +23,8 @@ def call(**over):
 @pytest.mark.parametrize("over,code", [
     (dict(pre=None), INVALID), (dict(n=0), INVALID), (dict(cu=None), INVALID), (dict(pre=FAKE + 2), ALIGNMENT),
     (dict(cu=FAKE + 1), ALIGNMENT), (dict(t=None), INVALID), (dict(page=24), INVALID),
-    (dict(D=96), _lib.B2A_ERR_HEAD_DIM), (dict(Hq=34), _lib.B2A_ERR_GQA), (dict(k=FAKE + 8), ALIGNMENT), (dict(ks=(16384, 8192, 130)), ALIGNMENT),
+    (dict(D=96), _lib.B2A_ERR_HEAD_DIM), (dict(Hq=34), _lib.B2A_ERR_GQA), (dict(k=FAKE + 8), ALIGNMENT),
+    (dict(ks=(16384, 8192, 130)), ALIGNMENT),
     (dict(ws=None), _lib.B2A_ERR_WORKSPACE), (dict(wsb=1000), _lib.B2A_ERR_WORKSPACE), (dict(scale=0.0), INVALID),
 ])
 def test_refused(over, code):
@@ -50,5 +51,5 @@ def test_valid_calls_without_a_gpu_report_it():
 def test_host_tensors_are_refused():
     pool, lens = torch.zeros(3, 2, 16, 64).bfloat16(), torch.ones(4, dtype=torch.int32)
     with pytest.raises(ValueError):
-        api.decode_paged_shared(torch.zeros(4, 8, 64).bfloat16(), pool, pool, torch.zeros(4, 1, dtype=torch.int32), lens,
-                                lens[:1])
+        api.decode_paged_shared(torch.zeros(4, 8, 64).bfloat16(), pool, pool, torch.zeros(4, 1, dtype=torch.int32),
+                                lens, lens[:1])

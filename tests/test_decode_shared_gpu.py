@@ -123,8 +123,8 @@ def test_sharp_scores(cuda_dev):
 
 
 def test_short_and_lone_sequences(cuda_dev):
-    """Sequences without all of the prefix attend by themselves: the others' keys (NaN, or far larger) do not reach them;
-    nor does a sequence outside every group."""
+    """Sequences without all of the prefix attend by themselves: the others' keys (NaN, or far larger) do not reach
+    them; nor does a sequence outside every group."""
     from npu_b200 import device_error
 
     dev = cuda_dev
@@ -287,7 +287,7 @@ def test_empty(cuda_dev):
 
 
 def test_what_saves_too_little_is_not_shared(cuda_dev):
-    """Below min_saved_bytes every sequence attends by itself (two bf16 terms of P throughout), from it on they share."""
+    """Below min_saved_bytes every sequence attends by itself (P in two bf16 terms), from it on they share."""
     dev = cuda_dev
     ks, vs, kp, vp, table, lens, pre, cu = build(dev, [(640, [50, 60, 70]), (1280, [1, 2, 400, 9])], 4, 128, 64, 6)
     q = torch.randn(7, 32, 128, generator=gen(dev, 1), device=dev).bfloat16()

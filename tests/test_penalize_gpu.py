@@ -165,7 +165,7 @@ def test_histories(cuda_dev, ids):
 
 
 def test_strides(cuda_dev):
-    """Rows of a larger tensor, tokens stored step by step, one bias and one mask for all, an output of other strides."""
+    """Rows of a larger tensor, tokens stored step by step, one bias and one mask for all, other output strides."""
     from npu_b200 import penalize
 
     dev, R, V = cuda_dev, 5, 4099

@@ -97,7 +97,8 @@ def penalize(**over):
     (dict(pa=float("inf")), INVALID), (dict(x=FAKE + 2), ALIGNMENT), (dict(t=FAKE + 4), ALIGNMENT),
     (dict(b=FAKE + 2), ALIGNMENT), (dict(n=FAKE + 1), ALIGNMENT),
     # Overlapping, but not in place: chunks of a row run in any order.
-    (dict(out=FAKE + 4), INVALID), (dict(out=FAKE + 400), INVALID), (dict(lo=101), INVALID), (dict(out=FAKE - 4), INVALID),
+    (dict(out=FAKE + 4), INVALID), (dict(out=FAKE + 400), INVALID), (dict(lo=101), INVALID),
+    (dict(out=FAKE - 4), INVALID),
 ])
 def test_penalize(over, code):
     assert penalize(**over) == code
