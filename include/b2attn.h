@@ -441,7 +441,7 @@ B2A_API int b2a_decode_paged_shared(const void* q, const void* k_pages, const vo
  * row n of sequence b (cu[b] <= n < cu[b + 1]) is the key at position
  * start + n - cu[b]. bf16 pools (k_scales and v_scales NULL) or 8-bit ones (as
  * b2a_rope_append_paged_e4m3; a value is its e4m3 times its scale, rounded to
- * bf16 once). Rows outside every sequence are not written; a position without
+ * bf16 once). k_out and v_out must not overlap. Rows outside every sequence are not written; a position without
  * a page gives zeros, a pair of offsets that is not a stretch of the N rows
  * leaves its sequence out, and both report B2A_ERR_DEVICE_BAD_LEN.
  * Supported D: 64, 128, 256.

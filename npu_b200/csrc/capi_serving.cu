@@ -111,7 +111,7 @@ int paged_attention(const void* q, const void* k_pages, const void* v_pages, con
   if (!q || !k_pages || !v_pages || !block_table || !seqlens || !o || !qs || !ks || !vs || !os || (gate && !gs))
     return B2A_ERR_INVALID_ARG;
   if (B <= 0 || Hq <= 0 || Hkv <= 0 || n_pages <= 0 || page <= 0 || page % 16 || table_width <= 0 ||
-      table_ld < table_width || (long long)table_width * page > INT_MAX - 64)
+      table_ld < table_width || (long long)table_width * page > INT_MAX - 128)
     return B2A_ERR_INVALID_ARG;
   if (!(scale > 0.f) || !std::isfinite(scale)) return B2A_ERR_INVALID_ARG;
   if (!head_dim_ok(D)) return B2A_ERR_HEAD_DIM;
@@ -486,6 +486,9 @@ int b2a_gather_paged(const void* k_pages, const void* v_pages, const long long* 
   if (!head_dim_ok(D)) return B2A_ERR_HEAD_DIM;
   if (k_scales)
     if (const int rc = scales_ok(k_scales, v_scales, kss, vss)) return rc;
+  const unsigned long long bytes = 2ull * N * Hkv * D;  // of either output
+  const uintptr_t ko = reinterpret_cast<uintptr_t>(k_out), vo = reinterpret_cast<uintptr_t>(v_out);
+  if (ko < vo + bytes && vo < ko + bytes) return B2A_ERR_INVALID_ARG;
   for (const void* ptr : {k_pages, v_pages, (const void*)k_out, (const void*)v_out})
     if (!api_aligned(ptr, 16)) return B2A_ERR_ALIGNMENT;
   const long long mult = k_scales ? 16 : 8;

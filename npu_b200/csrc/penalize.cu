@@ -26,6 +26,7 @@ namespace b2a {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kMostRows = 65535;  // of a launch
 
 template <typename T>
 struct Elements;  // 16 bytes of logits
@@ -106,7 +107,7 @@ __device__ __forceinline__ float4 zero4() { return make_float4(0.f, 0.f, 0.f, 0.
 // SLOTS: 16-byte pieces of logits per thread (256 threads of 4, four CTAs an SM: at 256 rows of 131071 bf16 63 us, with
 // threads or pieces twice as many 65, with six CTAs and 40 registers 82). Word: a counter.
 template <typename T, int SLOTS, typename Word>
-__global__ void __launch_bounds__(kThreads, 4) penalize_kernel(const __grid_constant__ PenalizeParams p, int chunks) {
+__global__ void __launch_bounds__(kThreads, 4) penalize_kernel(const __grid_constant__ PenalizeParams p) {
   using E = Elements<T>;
   constexpr int CHUNK = kThreads * SLOTS * E::N;
   static_assert(CHUNK <= 65536 && sizeof(Word) >= sizeof(T), "list entries, results in the counters' places");
@@ -115,13 +116,13 @@ __global__ void __launch_bounds__(kThreads, 4) penalize_kernel(const __grid_cons
   __shared__ int listed;
   grid_dep_wait();
   grid_dep_launch();
-  const int row = blockIdx.x / chunks;
+  const int row = blockIdx.y;
   const T* x = static_cast<const T*>(p.logits) + row * p.ld_logits;
   T* y = static_cast<T*>(p.out) + row * p.ld_out;
   // The chunk starts on a 16-byte boundary of the row, at or before element 0.
   const int shift = (int)((reinterpret_cast<uintptr_t>(x) & 15u) / sizeof(T));
   const bool together = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(y)) & 15u) == 0;
-  const int v0 = (int)(blockIdx.x % chunks) * CHUNK - shift;
+  const int v0 = (int)blockIdx.x * CHUNK - shift;
   if (v0 >= p.V) return;  // (the last chunk of a row that starts on a boundary)
   uint4 raw[SLOTS];
 #pragma unroll
@@ -225,10 +226,18 @@ __global__ void __launch_bounds__(kThreads, 4) penalize_kernel(const __grid_cons
     __syncthreads();  // the counters are 0
     for (int i0 = 0; i0 < n; i0 += AHEAD * kThreads) {
       if (i0 > 0) request(i0);
+      // One in as many tokens as there are chunks is in this one. The few are found first and then counted in turn, so
+      // that a warp runs the counting about twice and not for every k that any of its lanes has one at.
+      unsigned hits = 0;
 #pragma unroll
-      for (int k = 0; k < AHEAD; ++k) {
-        if (t[k] >= span) continue;
-        const int c = (int)t[k] + first - v0;
+      for (int k = 0; k < AHEAD; ++k) hits |= t[k] < span ? 1u << k : 0u;
+#pragma unroll 1
+      for (; hits; hits &= hits - 1u) {
+        const int k = __ffs(hits) - 1;
+        unsigned at = t[0];
+#pragma unroll
+        for (int x = 1; x < AHEAD; ++x) at = k == x ? t[x] : at;
+        const int c = (int)at + first - v0;
         if (count_token(counts, c, i0 + k * kThreads + (int)threadIdx.x < prompt) == 0)
           list[atomicAdd(&listed, 1)] = (uint16_t)c;
       }
@@ -280,10 +289,9 @@ template <typename T, int SLOTS, typename Word>
 int launch_slots(const PenalizeParams& p, cudaStream_t st) {
   constexpr int N = Elements<T>::N, CHUNK = kThreads * SLOTS * N;
   // One more than V / CHUNK would need: a row may start up to N - 1 elements into a 16-byte piece.
-  const long long chunks = ((long long)p.V + N - 1 + CHUNK - 1) / CHUNK, n = chunks * p.R;
-  if (n > 0x7fffffffLL) return -2;
-  return launch_dependent(penalize_kernel<T, SLOTS, Word>, dim3((unsigned)n), kThreads, 0, st, 0, p, (int)chunks) ==
-                 cudaSuccess
+  const long long chunks = ((long long)p.V + N - 1 + CHUNK - 1) / CHUNK;
+  return launch_dependent(penalize_kernel<T, SLOTS, Word>, dim3((unsigned)chunks, (unsigned)p.R), kThreads, 0, st, 0,
+                          p) == cudaSuccess
              ? 0
              : -1;
 }
@@ -298,9 +306,30 @@ int launch_t(const PenalizeParams& p, cudaStream_t st) {
 
 }  // namespace
 
-int launch_penalize(const PenalizeParams& p, cudaStream_t st) {
-  if (!p.logits_bf16) return launch_t<float, uint32_t>(p, st);
-  return p.L <= kNarrowTokens ? launch_t<__nv_bfloat16, uint16_t>(p, st) : launch_t<__nv_bfloat16, uint32_t>(p, st);
+int launch_penalize(const PenalizeParams& all, cudaStream_t st) {
+  // In pieces that a grid's second dimension holds.
+  for (long long r = 0; r < all.R; r += kMostRows) {
+    PenalizeParams p = all;
+    const int size = p.logits_bf16 ? 2 : 4;
+    p.R = (int)(all.R - r < kMostRows ? all.R - r : kMostRows);
+    p.logits = static_cast<const char*>(p.logits) + r * p.ld_logits * size;
+    p.out = static_cast<char*>(p.out) + r * p.ld_out * size;
+    if (p.tokens) p.tokens = static_cast<const char*>(p.tokens) + r * p.tokens_row * (p.tokens_64 ? 8 : 4);
+    if (p.lengths) p.lengths += r;
+    if (p.prompt_lengths) p.prompt_lengths += r;
+    if (p.repetition) p.repetition += r;
+    if (p.frequency) p.frequency += r;
+    if (p.presence) p.presence += r;
+    if (p.bias) p.bias += r * p.ld_bias;
+    if (p.allowed) p.allowed += r * p.ld_allowed;
+    int rc;
+    if (!p.logits_bf16)
+      rc = launch_t<float, uint32_t>(p, st);
+    else
+      rc = p.L <= kNarrowTokens ? launch_t<__nv_bfloat16, uint16_t>(p, st) : launch_t<__nv_bfloat16, uint32_t>(p, st);
+    if (rc) return rc;
+  }
+  return 0;
 }
 
 }  // namespace b2a

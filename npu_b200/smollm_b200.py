@@ -253,10 +253,11 @@ class SmolLMB200:
         return PagedKVCache(c.n_layers, n_pages, c.n_kv_heads, page, c.head_dim, self.device, dtype)
 
     def _attention_packed(self, lw: dict, h: torch.Tensor, seqs: PagedSequences, i: int,
-                          cu_seqlens: Optional[torch.Tensor]) -> torch.Tensor:
+                          cu_seqlens: Optional[torch.Tensor], cu_keys: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Attention of layer i before the output projection, [N, Hq * Dh]: of
-        packed prompts with offsets cu_seqlens, or (None) of one token per
-        sequence against its cached keys."""
+        packed prompts with offsets cu_seqlens (behind a shared prefix, cu_keys
+        those of their keys with it), or (None) of one token per sequence
+        against its cached keys."""
         c = self.cfg
         Hq, Hkv, Dh = c.n_heads, c.n_kv_heads, c.head_dim
         N = h.shape[0]
@@ -275,10 +276,9 @@ class SmolLMB200:
         with profile("attn"):
             if prompts and seqs.prefix_tokens:
                 # The prefix's keys and the prompt's own, both as the cache holds them.
-                cu_k = cu_seqlens + seqs.prefix_tokens * seqs.one_each
-                kv = api.gather_paged(k_pages, v_pages, seqs.block_table, cu_k, N + seqs.batch * seqs.prefix_tokens,
+                kv = api.gather_paged(k_pages, v_pages, seqs.block_table, cu_keys, N + seqs.batch * seqs.prefix_tokens,
                                       **scales)
-                o = api.prefill_varlen(rot[0], *kv, cu_seqlens, cu_k, out_dtype=h.dtype)
+                o = api.prefill_varlen(rot[0], *kv, cu_seqlens, cu_keys, out_dtype=h.dtype)
             elif prompts:
                 o = api.prefill_varlen(*rot, cu_seqlens, out_dtype=h.dtype)
             elif seqs.prefix_tokens and not scales:
@@ -295,10 +295,13 @@ class SmolLMB200:
             raise ValueError("the sequences are released: their pages may have other owners")
         c = self.cfg
         x = self.embed[ids]
+        cu_keys = None
+        if cu_seqlens is not None and seqs.prefix_tokens:
+            cu_keys = cu_seqlens + seqs.prefix_tokens * seqs.one_each
         for i, lw in enumerate(self.layers):
             with profile("rms1"):
                 h = rms_norm(x, lw["ln1"], c.rms_eps)
-            o = self._attention_packed(lw, h, seqs, i, cu_seqlens)
+            o = self._attention_packed(lw, h, seqs, i, cu_seqlens, cu_keys)
             with profile("wo"):
                 x = x + F.linear(o, lw["wo"])
             with profile("rms2"):

@@ -189,6 +189,22 @@ def test_strides(cuda_dev):
         assert torch.equal(wide[:, V:], keep[:, V:])
 
 
+def test_more_rows_than_a_grid_has(cuda_dev):
+    from npu_b200 import penalize
+
+    dev, R, V = cuda_dev, 140000, 37
+    g = gen(dev, 1)
+    x = torch.randn(R, V, generator=g, device=dev)
+    tokens = torch.randint(0, V, (R, 3), generator=g, device=dev)
+    rep = 0.5 + torch.rand(R, generator=g, device=dev)
+    bias = torch.randn(R, V, generator=g, device=dev)
+    got = penalize(x, tokens, ints(dev, [3] * R), repetition=rep, bias=bias, prompt_lengths=ints(dev, [1] * R))
+    seen = torch.zeros_like(x).scatter_(1, tokens, 1.0) > 0
+    y = x.double()
+    y = torch.where(seen, torch.where(y > 0, y / rep[:, None].double(), y * rep[:, None].double()), y) + bias.double()
+    assert ((got.double() - y).abs() <= 3 * 2 ** -24 * (y.abs() + 2 * bias.abs().double() + 1e-30)).all()
+
+
 def test_lengths_out_of_range_are_cut_and_reported(cuda_dev):
     from npu_b200 import device_error, penalize
     from npu_b200._lib import B2A_ERR_DEVICE_BAD_LEN

@@ -61,7 +61,7 @@ def test_append(over, code):
 def gather(**over):
     a = dict(k=FAKE, v=FAKE, ks=(16384, 8192, 128), vs=(16384, 8192, 128), sk=FAKE, sv=FAKE, kss=(128, 64),
              vss=(128, 64), t=FAKE, ld=8, w=8, pages=20, page=64, cu=FAKE, B=2, N=9, Hkv=2, D=128, sp=0, spb=None,
-             ko=FAKE, vo=FAKE)
+             ko=FAKE, vo=FAKE + 4608)
     a.update(over)
     return _lib.load().b2a_gather_paged(
         a["k"], a["v"], LL3(*a["ks"]), LL3(*a["vs"]), a["sk"], a["sv"], ll2(a["kss"]), ll2(a["vss"]), a["t"], a["ld"],
@@ -73,7 +73,9 @@ def gather(**over):
     (dict(k=None), INVALID), (dict(ko=None), INVALID), (dict(cu=None), INVALID), (dict(sk=None), INVALID),
     (dict(kss=None), INVALID), (dict(N=0), INVALID), (dict(B=0), INVALID), (dict(w=9), INVALID),
     (dict(sp=-1), INVALID), (dict(page=0), INVALID), (dict(D=80), _lib.B2A_ERR_HEAD_DIM),
-    (dict(vo=FAKE + 8), ALIGNMENT), (dict(ks=(16384, 8192, 136)), ALIGNMENT), (dict(spb=FAKE + 2), ALIGNMENT),
+    (dict(vo=FAKE + 4616), ALIGNMENT),
+    (dict(vo=FAKE), INVALID), (dict(vo=FAKE + 4592), INVALID),
+    (dict(ko=FAKE + 4608, vo=FAKE + 16), INVALID), (dict(ks=(16384, 8192, 136)), ALIGNMENT), (dict(spb=FAKE + 2), ALIGNMENT),
     (dict(sk=None, sv=None, ks=(16384, 8192, 132)), ALIGNMENT),
 ])
 def test_gather(over, code):
@@ -85,8 +87,8 @@ def penalize(**over):
              p=None, pa=0.2, b=None, lb=0, a=None, la=0, out=FAKE, lo=100, R=2, V=100)
     a.update(over)
     return _lib.load().b2a_penalize(
-        a["x"], a["ld"], a["bf16"], a["t"], a["wide"], a["tr"], a["ts"], a["L"], a["n"], a["m"], a["r"], a["ra"], a["f"],
-        a["fa"], a["p"], a["pa"], a["b"], a["lb"], a["a"], a["la"], a["out"], a["lo"], a["R"], a["V"], None)
+        a["x"], a["ld"], a["bf16"], a["t"], a["wide"], a["tr"], a["ts"], a["L"], a["n"], a["m"], a["r"], a["ra"],
+        a["f"], a["fa"], a["p"], a["pa"], a["b"], a["lb"], a["a"], a["la"], a["out"], a["lo"], a["R"], a["V"], None)
 
 
 @pytest.mark.parametrize("over,code", [
