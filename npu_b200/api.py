@@ -548,9 +548,8 @@ def decode_paged_shared(
     `prefill`. workspace: decode_paged_shared_workspace_bytes.
 
     Where sharing would save reading fewer than min_saved_bytes bytes of keys and
-    values (default 36 MB, about where it begins to pay for its launches), nothing is
-    shared. Calls known to stay below 100 MB are some 5 us faster through
-    `decode_paged`.
+    values nothing is shared. The default goes by what was measured to pay for the
+    launches: 36 MB, and 128 MB if every table were shared to its end.
     """
     return _serving().decode_paged_shared(q, k_pages, v_pages, block_table, seqlens, prefix_lens, cu_groups, scale,
                                           out_dtype, workspace, out, gate, min_saved_bytes)

@@ -75,10 +75,13 @@ struct SharedPrefix {
   long long least_saved;  // bytes, below 0: kLeastSaved
 };
 
-// Reading that sharing must save to be worth its plan and its kernel, in bytes. Measured against not sharing (same
-// launches), 32 / 4 heads of 128 and 9 / 3 of 64: 20.2 us against 18.4 at 31 MB, 22.2 / 23.2 at 42, 20.5 / 21.8 at
-// 63, 20.5 / 27.9 at 126, 27.4 / 40.2 at 252.
-constexpr long long kLeastSaved = 36LL << 20;
+// Reading that sharing must save to be worth its plan and its kernel, in bytes. Known on the device, where it is
+// measured against not sharing with the same launches, 32 / 4 heads of 128 and 9 / 3 of 64: 20.2 us against 18.4 at 31
+// MB, 22.2 / 23.2 at 42, 20.5 / 21.8 at 63, 20.5 / 27.9 at 126, 27.4 / 40.2 at 252. The host knows only what it could
+// save, if all of every table were shared; below kLeastPossible the call is b2a_decode_paged's, against which, by what
+// could be saved: 20.2 / 12.5 at 63 MB, 20.2 / 15.6 at 94, 22.3 / 17.4 and 17.1 / 22.2 at 109, 20.5 / 21.5 at 157,
+// 27.4 / 32.8 at 275, 30 / 101 at 662.
+constexpr long long kLeastSaved = 36LL << 20, kLeastPossible = 128LL << 20;
 
 // Where the shared form's scratch is, behind that of the sequences' own keys.
 struct SharedLayout {
@@ -184,9 +187,11 @@ int paged_attention(const void* q, const void* k_pages, const void* v_pages, con
   // Few keys, or one sequence: every sequence reads its own (one launch). So too where sharing could not save enough;
   // how much it does save is known on the device, where the plan looks again.
   const long long bytes_a_key = 4LL * Hkv * D;
-  const long long least = !shared ? 0 : (shared->least_saved < 0 ? kLeastSaved : shared->least_saved);
+  const bool by_rule = shared && shared->least_saved < 0;
+  const long long least = by_rule ? kLeastSaved : (shared ? shared->least_saved : 0);
+  const long long possible = (B - 1) * ((long long)table_width * page);  // keys
   if (shared && B > 1 && b2a::decode_paged_splits(table_width, page) &&
-      (B - 1) * ((long long)table_width * page) >= least / bytes_a_key) {
+      possible >= (by_rule ? kLeastPossible : least) / bytes_a_key) {
     const SharedLayout at = shared_layout(B, Hq, Hkv, D, shared->n_groups);
     char* base = reinterpret_cast<char*>(b2a::api_align256(reinterpret_cast<uintptr_t>(workspace) + own));
     b2a::SharedPlanParams plan{};

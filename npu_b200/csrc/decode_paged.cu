@@ -202,12 +202,36 @@ __device__ __forceinline__ int tiles_of(const DecodePagedParams& p, int b) {
 // at head dim 64, 2 beside 1.3 at 256). The extra unit follows the tiles.
 __device__ __forceinline__ int units_of(int tiles) { return tiles > 0 ? tiles + 1 : 0; }
 
+// SHARED: the units of the first 128 sequences (lane x: x, 32 + x, ..), which are
+// read past L1: requested together, and kept for the two passes over them.
+template <int TK, bool SHARED>
+struct FirstUnits {
+  __device__ __forceinline__ explicit FirstUnits(const DecodePagedParams&) {}
+};
+template <int TK>
+struct FirstUnits<TK, true> {
+  int n[4];
+  __device__ __forceinline__ explicit FirstUnits(const DecodePagedParams& p) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int b = 32 * k + (threadIdx.x & 31);
+      n[k] = b < p.B ? units_of(tiles_of<TK, true>(p, b)) : 0;
+    }
+  }
+  __device__ __forceinline__ int at(int b0) const { return b0 < 64 ? (b0 < 32 ? n[0] : n[1]) : (b0 < 96 ? n[2] : n[3]); }
+};
+
 // All units of the call (all lanes get it). Warp-collective.
 template <int TK, bool SHARED>
-__device__ __forceinline__ long long total_units(const DecodePagedParams& p) {
+__device__ __forceinline__ long long total_units(const DecodePagedParams& p, const FirstUnits<TK, SHARED>& first) {
   long long n = 0;
+  int b1 = 0;
+  if constexpr (SHARED) {
+    n = __reduce_add_sync(0xffffffffu, first.n[0] + first.n[1] + first.n[2] + first.n[3]);
+    b1 = 128;
+  }
 #pragma unroll 4
-  for (int b0 = 0; b0 < p.B; b0 += 32) {
+  for (int b0 = b1; b0 < p.B; b0 += 32) {
     const int b = b0 + (threadIdx.x & 31);
     n += __reduce_add_sync(0xffffffffu, b < p.B ? units_of(tiles_of<TK, SHARED>(p, b)) : 0);
   }
@@ -232,13 +256,18 @@ struct Walk {
   int tiles, len;  // all its tiles, its keys
   int ahead;       // tiles of the sequence before them
   // The pairs of units [from, from + count). Warp-collective. Check valid().
-  __device__ __forceinline__ Walk(const DecodePagedParams& p, long long from, long long count) {
+  __device__ __forceinline__ Walk(const DecodePagedParams& p, long long from, long long count,
+                                  const FirstUnits<TK, SHARED>& first) {
     left = count;
     b = p.B;
     if (left <= 0) return;
     const int lane = threadIdx.x & 31;
     for (int b0 = 0; b0 < p.B; b0 += 32) {
-      const int n = b0 + lane < p.B ? units_of(tiles_of<TK, SHARED>(p, b0 + lane)) : 0;
+      int n;
+      if constexpr (SHARED)
+        n = b0 < 128 ? first.at(b0) : (b0 + lane < p.B ? units_of(tiles_of<TK, SHARED>(p, b0 + lane)) : 0);
+      else
+        n = b0 + lane < p.B ? units_of(tiles_of<TK, SHARED>(p, b0 + lane)) : 0;
       int upto = n;  // inclusive sum over the lanes
 #pragma unroll
       for (int off = 1; off < 32; off *= 2) {
@@ -353,8 +382,9 @@ __global__ void __launch_bounds__(PagedCfg<D, NT, E4M3>::THREADS, PagedCfg<D, NT
     for (int b = threadIdx.x; b < p.B; b += C::THREADS)
       if (p.seqlens[b] < 0 || p.seqlens[b] > (long long)p.table_width * p.page) atomicOr(p.err, kErrBadArgs);
   long long from = 0, count = 1;
+  const FirstUnits<C::TK, SHARED> first(p);
   if constexpr (SPLIT) {
-    const long long total = total_units<C::TK, SHARED>(p), share = share_of(total, p.n_ctas);
+    const long long total = total_units<C::TK, SHARED>(p, first), share = share_of(total, p.n_ctas);
     from = blockIdx.x * share;
     count = min(share, total - from);
     if (count <= 0) {
@@ -364,7 +394,7 @@ __global__ void __launch_bounds__(PagedCfg<D, NT, E4M3>::THREADS, PagedCfg<D, NT
   }
   using W = Walk<C::TK, SHARED>;
   auto start = [&]() -> W {
-    if constexpr (SPLIT) return W(p, from, count);
+    if constexpr (SPLIT) return W(p, from, count, first);
     const int b = blockIdx.x / p.Hkv;
     return W(b, blockIdx.x % p.Hkv, keys_of(p, b));
   };
