@@ -185,10 +185,20 @@ __device__ __forceinline__ float4 over(float4 x, float l) {
   return make_float4(f * (x.x / d), f * (x.y / d), f * (x.z / d), f * (x.w / d));
 }
 
+// A length or a table's entry. SHARED: past L1, whose lines may be older than the
+// last write, since that form's main kernel does not wait for the kernels before it
+// itself (the one it follows has).
+template <bool SHARED>
+__device__ __forceinline__ int load_int(const int* x) {
+  if constexpr (SHARED) return __ldcg(x);
+  return *x;
+}
+
 // Keys of sequence b that a call attends: its length, cut to the table.
+template <bool SHARED>
 __device__ __forceinline__ int keys_of(const DecodePagedParams& p, int b) {
   const long long cap = (long long)p.table_width * p.page;
-  const int len = p.seqlens[b];
+  const int len = load_int<SHARED>(p.seqlens + b);
   return len < 0 ? 0 : (len > cap ? (int)cap : len);
 }
 // Tiles of sequence b ahead of those that the call itself attends (TK: keys of a tile).
@@ -199,7 +209,7 @@ __device__ __forceinline__ int tiles_ahead(const DecodePagedParams& p, int b) {
 }
 template <int TK, bool SHARED>
 __device__ __forceinline__ int tiles_of(const DecodePagedParams& p, int b) {
-  return max((keys_of(p, b) + TK - 1) / TK - tiles_ahead<TK, SHARED>(p, b), 0);
+  return max((keys_of<SHARED>(p, b) + TK - 1) / TK - tiles_ahead<TK, SHARED>(p, b), 0);
 }
 
 // The work of a pair in the units that are shared out: its tiles, and one
@@ -300,7 +310,7 @@ struct Walk {
       : left((len_ + TK - 1) / TK), b(b_), g(g_), begin(0), t1((len_ + TK - 1) / TK), t0(0), tiles(t1), len(len_),
         ahead(0) {}
   __device__ __forceinline__ void measure(const DecodePagedParams& p) {
-    len = keys_of(p, b);
+    len = keys_of<SHARED>(p, b);
     ahead = tiles_ahead<TK, SHARED>(p, b);
     tiles = max((len + TK - 1) / TK - ahead, 0);
   }
@@ -384,8 +394,10 @@ __global__ void __launch_bounds__(PagedCfg<D, NT, E4M3>::THREADS, PagedCfg<D, NT
     if constexpr (SHARED) grid_dep_wait();
   };
   if (p.err && blockIdx.x == 0)
-    for (int b = threadIdx.x; b < p.B; b += C::THREADS)
-      if (p.seqlens[b] < 0 || p.seqlens[b] > (long long)p.table_width * p.page) atomicOr(p.err, kErrBadArgs);
+    for (int b = threadIdx.x; b < p.B; b += C::THREADS) {
+      const int len = load_int<SHARED>(p.seqlens + b);
+      if (len < 0 || len > (long long)p.table_width * p.page) atomicOr(p.err, kErrBadArgs);
+    }
   long long from = 0, count = 1;
   const FirstUnits<C::TK, SHARED> first(p);
   if constexpr (SPLIT) {
@@ -401,7 +413,7 @@ __global__ void __launch_bounds__(PagedCfg<D, NT, E4M3>::THREADS, PagedCfg<D, NT
   auto start = [&]() -> W {
     if constexpr (SPLIT) return W(p, from, count, first);
     const int b = blockIdx.x / p.Hkv;
-    return W(b, blockIdx.x % p.Hkv, keys_of(p, b));
+    return W(b, blockIdx.x % p.Hkv, keys_of<SHARED>(p, b));
   };
   W w = start();
   if (SPLIT && !w.valid()) {
@@ -444,7 +456,9 @@ __global__ void __launch_bounds__(PagedCfg<D, NT, E4M3>::THREADS, PagedCfg<D, NT
     // checked when its turn comes (so that nothing waits for the lookup).
     auto has_keys = [&]() { return mine && (w.ahead + w.t0) * C::TK + box * br < w.len; };
     auto entry_of = [&]() -> int {  // table entry of this lane's box in tile w.t0
-      return has_keys() ? p.block_table[w.b * p.table_ld + ((w.ahead + w.t0) * C::TK + box * br) / p.page] : 0;
+      return has_keys() ? load_int<SHARED>(p.block_table + w.b * p.table_ld +
+                                           ((w.ahead + w.t0) * C::TK + box * br) / p.page)
+                        : 0;
     };
     int n = 0, pairs = 0;  // tiles and pairs copied so far
     bool more = true, new_pair = true;

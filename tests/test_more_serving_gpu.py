@@ -189,3 +189,66 @@ def test_a_table_that_names_one_page_for_ever(cuda_dev):
     short = decode_paged(q, kp, vp, table, ints(dev, [256]), k_scales=sk, v_scales=sv)
     # The same keys again and again are the same average: sums of 300000 terms in fp32 parts of some thousands.
     assert ((long - short).abs() <= 2 ** -12 * vs[0].abs().amax()).all()
+
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_shared_steps_that_grow(cuda_dev, captured):
+    """Steps that follow one another without a pause, each right behind the append that writes the lengths it reads:
+    what the same steps give when the device has come to rest after every call."""
+    from npu_b200 import rope_append_paged
+
+    dev, Hq, Hkv, D, page, steps = cuda_dev, 9, 3, 64, 16, 60
+    own = [50, 60, 70, 9, 1, 33, 64]
+    total = [640 + t + steps for t in own]
+
+    def start_state():
+        ks, vs, kp, vp, table, lens, pre, cu = build(dev, [(640, [t + steps for t in own])], Hkv, D, page, 6, fill=0.0)
+        g = gen(dev, 2)
+        ang = torch.outer(torch.arange(max(total), device=dev).float(), torch.rand(D // 2, generator=g, device=dev))
+        ang = torch.cat([ang, ang], -1)
+        return dict(kp=kp, vp=vp, table=table, pre=pre, cos=ang.cos(), sin=ang.sin(), start=ints(dev, [640 + t for t in own]),
+                    lens=torch.zeros(len(own), dtype=torch.int32, device=dev),
+                    each=torch.arange(len(own) + 1, dtype=torch.int32, device=dev),
+                    qkv=torch.randn(len(own), Hq + 2 * Hkv, D, generator=g, device=dev))
+
+    def one(st, rest=lambda: None):
+        q = rope_append_paged(st["qkv"][:, :Hq], st["qkv"][:, Hq:Hq + Hkv], st["qkv"][:, Hq + Hkv:], st["cos"], st["sin"],
+                              st["kp"], st["vp"], st["table"], st["each"], start_pos_per_batch=st["start"],
+                              seqlens_out=st["lens"])
+        rest()
+        o = shared(q, st["kp"], st["vp"], st["table"], st["lens"], st["pre"])
+        rest()
+        st["start"].add_(1)
+        st["qkv"].mul_(0.99).add_(o.mean() * 1e-3)
+        rest()
+        return o
+
+    st = start_state()
+    want = [one(st, torch.cuda.synchronize).clone() for _ in range(steps)]
+    st, got = start_state(), []
+    if captured:
+        first = {x: y.clone() for x, y in st.items()}
+        one(st)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            o = one(st)
+        for x, y in first.items():
+            st[x].copy_(y)
+        for _ in range(steps):
+            graph.replay()
+            got.append(o.clone())
+    else:
+        got = [one(st) for _ in range(steps)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
+    assert st["lens"].tolist() == total
+
+
+@pytest.mark.parametrize("dims", [(0,), (1,), (0, 1)])
+def test_shared_prefix_queries_that_are_one(cuda_dev, dims):
+    """Queries expanded over the sequences or the heads, as decode_paged takes them."""
+    dev = cuda_dev
+    ks, vs, kp, vp, table, lens, pre, cu = build(dev, [(900, [50, 60, 70]), (640, [1, 2, 400])], 2, 64, 64, 5)
+    q = torch.randn(*[1 if i in dims else n for i, n in enumerate((6, 8))], 64, generator=gen(dev, 1), device=dev)
+    q = q.bfloat16().expand(6, 8, 64)
+    check(shared(q, kp, vp, table, lens, pre, cu), q, ks, vs, 1 / 8)
