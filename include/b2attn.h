@@ -467,7 +467,8 @@ B2A_API int b2a_gather_paged(const void* k_pages, const void* v_pages, const lon
  * each step rounded in fp32, the result to the logits' type. repetition,
  * frequency, presence: per-row device arrays [R], or NULL for the *_all value
  * (repetition_all above 0). ld_bias / ld_allowed 0: one row for all. out
- * [R, V] (row stride ld_out): the logits themselves, or apart from them. A
+ * [R, V] (row stride ld_out): the logits themselves, or apart from them, and apart
+ * from every other input. A
  * length outside 0 .. L is cut and reports B2A_ERR_DEVICE_BAD_LEN. V, L <= 2^30.
  */
 B2A_API int b2a_penalize(const void* logits, long long ld_logits, int logits_bf16, const void* tokens, int tokens_64,

@@ -661,7 +661,7 @@ def penalize(
     allowed is an int32 tensor [ceil(V / 32)] or [R, ceil(V / 32)] of 32 tokens a
     word. repetition (above 0), frequency and presence are numbers or per-row fp32
     CUDA tensors. Each step is rounded in fp32, the result to the logits' type.
-    `out` may be the logits themselves. A row whose mask leaves nothing is -inf
+    `out` may be the logits themselves and overlaps no other input. A row whose mask leaves nothing is -inf
     throughout, and `sample` gives -1 for it.
     """
     return _serving().penalize(logits, tokens, lengths, prompt_lengths, repetition, frequency, presence, bias, allowed,

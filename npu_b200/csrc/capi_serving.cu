@@ -555,6 +555,18 @@ int b2a_penalize(const void* logits, long long ld_logits, int logits_bf16, const
   const uintptr_t x1 = x0 + ((unsigned long long)(R - 1) * ld_logits + V) * size;
   const uintptr_t y1 = y0 + ((unsigned long long)(R - 1) * ld_out + V) * size;
   if (x0 < y1 && y0 < x1 && !(x0 == y0 && (ld_logits == ld_out || R == 1))) return B2A_ERR_INVALID_ARG;
+  // The rest is read by other chunks than the one that writes, too: apart. (tokens: the caller's
+  // to see to.)
+  auto meets_out = [&](const void* base, unsigned long long bytes) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(base);
+    return base && at < y1 && y0 < at + bytes;
+  };
+  const unsigned long long last = R - 1, words = (V + 31LL) / 32;
+  if (meets_out(bias, (last * ld_bias + V) * 4) || meets_out(allowed, (last * ld_allowed + words) * 4))
+    return B2A_ERR_INVALID_ARG;
+  for (const void* rows : {(const void*)lengths, (const void*)prompt_lengths, (const void*)repetition,
+                           (const void*)frequency, (const void*)presence})
+    if (meets_out(rows, 4ull * R)) return B2A_ERR_INVALID_ARG;
   int* err = nullptr;
   const int rc = b2a::api_prologue(&err);
   if (rc) return rc;

@@ -306,7 +306,7 @@ int launch_slots(const PenalizeParams& p, cudaStream_t st) {
 // Few rows: small chunks, so that a row is spread over more CTAs.
 template <typename T, typename Word>
 int launch_t(const PenalizeParams& p, cudaStream_t st) {
-    constexpr int MOST = sizeof(Word) > sizeof(T) ? 2 : 4;
+  constexpr int MOST = sizeof(Word) > sizeof(T) ? 2 : 4;
   const long long pieces = (long long)p.R * ((p.V + Elements<T>::N - 1) / Elements<T>::N);
   return pieces > 148LL * 8 * kThreads ? launch_slots<T, MOST, Word>(p, st) : launch_slots<T, 1, Word>(p, st);
 }

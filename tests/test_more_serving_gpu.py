@@ -252,3 +252,13 @@ def test_shared_prefix_queries_that_are_one(cuda_dev, dims):
     q = torch.randn(*[1 if i in dims else n for i, n in enumerate((6, 8))], 64, generator=gen(dev, 1), device=dev)
     q = q.bfloat16().expand(6, 8, 64)
     check(shared(q, kp, vp, table, lens, pre, cu), q, ks, vs, 1 / 8)
+
+
+def test_penalize_into_its_bias(cuda_dev):
+    from npu_b200 import penalize
+
+    x = torch.randn(4, 1000, device=cuda_dev)
+    with pytest.raises((ValueError, RuntimeError)):
+        penalize(x, bias=x, out=x)
+    with pytest.raises((ValueError, RuntimeError)):
+        penalize(x.clone(), bias=x[1], out=x)

@@ -127,3 +127,18 @@ def test_host_tensors_are_refused():
         api.gather_paged(pool, pool, table, cu, 4, k_scales=s, v_scales=s)
     with pytest.raises(ValueError):
         api.penalize(torch.zeros(2, 5), torch.zeros(2, 3, dtype=torch.long))
+
+
+@pytest.mark.parametrize("over,apart", [
+    # out is FAKE .. FAKE + 800; a bias of 100 floats, one row or two, masks of 4 words, per-row arrays of two numbers.
+    (dict(b=FAKE), 800), (dict(b=FAKE + 796), 800), (dict(b=FAKE - 396), -400), (dict(b=FAKE - 796, lb=100), -800),
+    (dict(a=FAKE + 400), 800), (dict(a=FAKE - 12), -16), (dict(a=FAKE - 28, la=4), -32),
+    (dict(r=FAKE - 4), -8), (dict(f=FAKE + 792), 800), (dict(p=FAKE), 800), (dict(n=FAKE + 8), 800),
+    (dict(m=FAKE - 4), -8),
+])
+def test_penalize_into_its_other_inputs(over, apart):
+    """Refused one element inside the output, valid right beside it."""
+    assert penalize(**over) == INVALID
+    if not torch.cuda.is_available():
+        name = next(x for x in over if x not in ("lb", "la"))
+        assert penalize(**{**over, name: FAKE + apart}) in CPU
