@@ -269,16 +269,17 @@ class SmolLMB200:
         k_pages, v_pages = seqs.cache.layer(i)
         scales = seqs.cache.scales(i)
         prompts = cu_seqlens is not None
+        behind = prompts and seqs.prefix_tokens > 0
         with profile("rope"):
             rot = api.rope_append_paged(q, k, v, self.cos, self.sin, k_pages, v_pages, seqs.block_table,
                                         cu_seqlens if prompts else seqs.one_each, start_pos_per_batch=seqs.start,
-                                        seqlens_out=seqs.end, return_kv=prompts, **scales)
+                                        seqlens_out=seqs.end, return_kv=prompts and not behind, **scales)
         with profile("attn"):
-            if prompts and seqs.prefix_tokens:
+            if behind:
                 # The prefix's keys and the prompt's own, both as the cache holds them.
                 kv = api.gather_paged(k_pages, v_pages, seqs.block_table, cu_keys, N + seqs.batch * seqs.prefix_tokens,
                                       **scales)
-                o = api.prefill_varlen(rot[0], *kv, cu_seqlens, cu_keys, out_dtype=h.dtype)
+                o = api.prefill_varlen(rot, *kv, cu_seqlens, cu_keys, out_dtype=h.dtype)
             elif prompts:
                 o = api.prefill_varlen(*rot, cu_seqlens, out_dtype=h.dtype)
             elif seqs.prefix_tokens and not scales:
