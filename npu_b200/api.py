@@ -549,7 +549,9 @@ def decode_paged_shared(
 
     Where sharing would save reading fewer than min_saved_bytes bytes of keys and
     values nothing is shared. The default goes by what was measured to pay for the
-    launches: 36 MB, and 128 MB if every table were shared to its end.
+    launches: 36 MB, and 128 MB if every table were shared to its end. That is a
+    guess from sizes alone: many short prefixes or a few sequences can be up to a
+    third slower than `decode_paged`, so a server that knows its shapes sets it.
     """
     return _serving().decode_paged_shared(q, k_pages, v_pages, block_table, seqlens, prefix_lens, cu_groups, scale,
                                           out_dtype, workspace, out, gate, min_saved_bytes)

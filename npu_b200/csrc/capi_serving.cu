@@ -80,7 +80,9 @@ struct SharedPrefix {
 // MB, 22.2 / 23.2 at 42, 20.5 / 21.8 at 63, 20.5 / 27.9 at 126, 27.4 / 40.2 at 252. The host knows only what it could
 // save, if all of every table were shared; below kLeastPossible the call is b2a_decode_paged's, against which, by what
 // could be saved: 20.2 / 12.5 at 63 MB, 20.2 / 15.6 at 94, 22.3 / 17.4 and 17.1 / 22.2 at 109, 20.5 / 21.5 at 157,
-// 27.4 / 32.8 at 275, 30 / 101 at 662.
+// 27.4 / 32.8 at 275, 30 / 101 at 662. Bytes are not all that counts, and some calls share that had better not: 30.2 us
+// against 22.8 for 64 sequences behind 512 keys, 29.4 / 25.6 for 64 in eight groups behind 2048 to 256, 39.4 / 35.6 for
+// 4 behind 32768 (all 32 / 4 heads of 128).
 constexpr long long kLeastSaved = 36LL << 20, kLeastPossible = 128LL << 20;
 
 // Where the shared form's scratch is, behind that of the sequences' own keys.

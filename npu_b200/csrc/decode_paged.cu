@@ -31,9 +31,10 @@
 // copy rate); 16 of 100 to 20000, 16 / 2 gated heads of 256, pages of 48: 36 us,
 // 4.9 TB/s, 4 us of it the first tile's latency and 4 the joining launch; 48 of
 // 30 to 4001, 9 / 3 heads of 64, pages of 16: 13.2 us, of which those two and
-// the launch are 7; one of 77 keys: 4.2 us. From an 8-bit cache: the first 220
-// us, 6.3 TB/s (0.98; bound by HBM again, once two instructions a pair of values
-// did what nine had), with 9 / 3 heads of 64 105 us, 5.1 TB/s (instructions), 16
+// the launch are 7; one of 77 keys: 4.2 us. From an 8-bit cache: the first 218
+// us, 6.4 TB/s (0.99; bound by HBM again, once two instructions a pair of values
+// did what nine had; 243 to 251 after seconds of it, when the power cap holds the
+// clock at 1.6 GHz), with 9 / 3 heads of 64 105 us, 5.1 TB/s (instructions), 16
 // gated ones of head dim 256 28 us, 3.2 TB/s (the same latencies, half the
 // bytes), groups of 16 heads 132 us where their bytes take 79 (instructions: two
 // blocks of columns for each product).

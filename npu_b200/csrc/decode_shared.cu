@@ -26,7 +26,7 @@
 // part, and numbers row blocks and units.
 //
 // Measured on one B200 (device time): 128 sequences of 16 to 2048 keys of their own
-// behind 32768 shared ones, 32 / 4 heads of 128, pages of 64: 111 us, of which the
+// behind 32768 shared ones, 32 / 4 heads of 128, pages of 64: 111 to 124 us; of 111 the
 // shared keys are 78, each further 32768 of them 57 (1.2 PFLOP/s, 0.72 of the
 // measured bf16 burst rate, 0.86 of the sustained one: what the dense prefill
 // reaches). The rest is the plan (4), starting and ending each item, the own keys
