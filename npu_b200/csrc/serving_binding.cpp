@@ -117,10 +117,14 @@ at::ScalarType float_type(const char* name, at::ScalarType type) {
 
 void* pointer(const OptTensor& t) { return t ? t->data_ptr() : nullptr; }
 
+// The strides of the first n dims. A dim of one element may have any stride in
+// torch and none matters; it gets the one it would have beside the next dim, so
+// that the ABI's checks of alignment see nothing odd.
 struct Strides {
   long long s[3];
   explicit Strides(const Tensor& t, int n) {
-    for (int i = 0; i < n; ++i) s[i] = t.stride(i);
+    for (int i = n - 1; i >= 0; --i)
+      s[i] = t.size(i) > 1 ? t.stride(i) : t.size(i + 1) * (i + 1 < n ? s[i + 1] : t.stride(i + 1));
   }
   operator const long long*() const { return s; }
 };
