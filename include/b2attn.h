@@ -397,8 +397,9 @@ B2A_API int b2a_rope_append_paged_e4m3(const void* q, const void* k, const void*
 /*
  * b2a_decode_paged over an 8-bit cache as b2a_rope_append_paged_e4m3 writes it:
  * key and value are the e4m3 numbers times their row's scale, not rounded to
- * fewer bits on the way. Scales are positive; one below 2^-100 counts as 2^-100.
- * Slots and scales past a sequence's end may hold anything.
+ * fewer bits on the way. Scales are positive; of v's, one below 2^-100 counts as
+ * 2^-100 and one above 2^90 as NaN. Slots and scales past a sequence's end may hold
+ * anything.
  */
 B2A_API int b2a_decode_paged_e4m3(const void* q, const void* k_pages, const void* v_pages, const float* k_scales,
                                   const float* v_scales, const long long* k_scale_strides,

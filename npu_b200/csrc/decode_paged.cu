@@ -44,6 +44,7 @@
 // memory before they are used.
 #include "capi_internal.cuh"
 #include "decode_paged.cuh"
+#include "paged.cuh"
 
 namespace b2a {
 
@@ -344,7 +345,12 @@ struct Walk {
 //   V's scale goes into the exponent, t_j = s_j + log2 sv_j, and the running
 //   maximum M is of t: w_j = 2^(t_j - M + 15) <= 2^15 weighs the e4m3 numbers of V
 //   (in two f16 terms: 2^-22 of w, or 2^-40 of the largest), w_j / sv_j is P
-//   for the sum. With sv_j at least 2^-100 that is at most 2^115.
+//   for the sum. With sv_j from 2^-100 (rows of zeros) to 2^90 that is 2^115 to
+//   2^-75 for the largest weight, and the sum has up to 2^31 terms: it is kept
+//   times 2^-24, below 2^122, with 27 bits under the smallest of those before
+//   fp32 ends (O gets the same factor when the warps' parts are merged). A weight
+//   below fp32's range drops out of the sum too: 2^-24 of the largest P where
+//   V's scales in a sequence differ by 2^117, less where by less.
 __device__ __forceinline__ uint32_t f16_of_e4m3(uint16_t x) {  // two numbers, the low byte's in the low half
   uint32_t r;
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(x));
@@ -365,7 +371,7 @@ __device__ __forceinline__ float2 unpack_f16x2(uint32_t x) {
   return r;
 }
 constexpr float kWeightLog2 = 15.f;               // of the largest weight of V
-constexpr float kSmallestScale = 7.888609052210118e-31f;  // 2^-100
+constexpr float kSumUnit = 5.9604644775390625e-08f;  // 2^-24
 
 __device__ __forceinline__ int swizzle(int r, int d) { return d ^ (((r >> 1) & 3) << 3); }
 
@@ -635,15 +641,15 @@ __global__ void __launch_bounds__(PagedCfg<D, NT, E4M3>::THREADS, PagedCfg<D, NT
               }
             }
             const float* scales = reinterpret_cast<const float*>(smem + C::OFF_SCALES) + slot * 2 * C::TK + 16 * warp;
-            float per_sv[C::KB][2];  // 1 / the scales of V's rows gr, gr + 8
+            float per_sv[C::KB][2];  // kSumUnit / the scales of V's rows gr, gr + 8
 #pragma unroll
             for (int i = 0; i < C::KB; ++i) {
 #pragma unroll
               for (int u = 0; u < 2; ++u) {
                 const int r = gr + 8 * u;
                 const float sk = scales[64 * i + r], given = scales[C::TK + 64 * i + r];
-                const float sv = given < kSmallestScale ? kSmallestScale : given, lg = __log2f(sv);  // NaN stays
-                per_sv[i][u] = r < have[i] ? __fdividef(1.f, sv) : 0.f;
+                const float sv = e4m3_scale_in_range(given), lg = __log2f(sv);
+                per_sv[i][u] = r < have[i] ? __fdividef(kSumUnit, sv) : 0.f;
 #pragma unroll
                 for (int x = 0; x < NT; ++x) {
 #pragma unroll
@@ -866,7 +872,7 @@ __global__ void __launch_bounds__(PagedCfg<D, NT, E4M3>::THREADS, PagedCfg<D, NT
           // A warp without keys here has nothing in the sum (its m is -inf).
           const float f = ex2(bars->m[u][r] - Mu);
           lsum += f * bars->l[u][r];
-          osum = axpy(f, *reinterpret_cast<const float4*>(so + (u * 16 + r) * D + swizzle(r, d)), osum);
+          osum = axpy(E4M3 ? f * kSumUnit : f, *reinterpret_cast<const float4*>(so + (u * 16 + r) * D + swizzle(r, d)), osum);
         }
         if constexpr (SPLIT) {
           *reinterpret_cast<float4*>(p.part_o + (part + r) * D + d) = osum;

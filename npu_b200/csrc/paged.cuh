@@ -17,6 +17,7 @@ namespace b2a {
 
 constexpr float kE4m3Max = 448.f;
 constexpr float kE4m3SmallestScale = 7.888609052210118e-31f;  // 2^-100
+constexpr float kE4m3LargestVScale = 1.2379400392853803e+27f;  // 2^90
 
 // The sequence that owns token n: the largest b with cu[b] <= n (0 when there
 // is none), by a search that narrows 32-fold per step. Warp-collective.
@@ -54,6 +55,13 @@ __device__ __forceinline__ float e4m3_scale(unsigned m) {
   if (m >= 0x7f800000u) return __uint_as_float(0x7fffffffu);  // NaN
   const float s = __fdiv_rn(__uint_as_float(m), kE4m3Max);
   return s < kE4m3SmallestScale ? kE4m3SmallestScale : s;
+}
+
+// A scale of V as attention takes it: none below the smallest, and NaN in place of
+// one whose reciprocal its sums have no room for (values above 5e29).
+__device__ __forceinline__ float e4m3_scale_in_range(float s) {
+  s = s > kE4m3LargestVScale ? __uint_as_float(0x7fffffffu) : s;
+  return s < kE4m3SmallestScale ? kE4m3SmallestScale : s;  // NaN stays
 }
 
 }  // namespace b2a
