@@ -367,6 +367,9 @@ __device__ __forceinline__ int clc_cancelled_ctaid_x(const void* resp) {
 // serialization) has completed and its memory is visible; a no-op otherwise.
 // griddepcontrol.launch_dependents: this CTA no longer holds back the launch
 // of the next grid (which still waits in its own griddepcontrol.wait).
+// The wait orders ordinary loads. The non-coherent path (__ldg) is for memory that
+// nothing writes while the grid is there, and grids launched this way are there
+// while the one before them writes: their kernels do not use it.
 __device__ __forceinline__ void grid_dep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void grid_dep_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 

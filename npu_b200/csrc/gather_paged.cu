@@ -111,10 +111,10 @@ __global__ void __launch_bounds__(32 * kWarps)
       const long long* ps = is_v ? p.vps : p.kps;
       const Cache* src = static_cast<const Cache*>(is_v ? p.v_pages : p.k_pages) + page * ps[0] + h * ps[1] +
                          slot * ps[2] + at;
-      raw[s] = __ldg(reinterpret_cast<const uint4*>(src));
+      raw[s] = *reinterpret_cast<const uint4*>(src);
       if constexpr (E4M3) {
         const long long* ss = is_v ? p.vss : p.kss;
-        scale[s] = __ldg((is_v ? p.v_scales : p.k_scales) + page * ss[0] + h * ss[1] + slot);
+        scale[s] = (is_v ? p.v_scales : p.k_scales)[page * ss[0] + h * ss[1] + slot];
       }
     }
 #pragma unroll

@@ -165,7 +165,7 @@ __global__ void __launch_bounds__(kThreads, 4) penalize_kernel(const __grid_cons
 #pragma unroll
       for (int k = 0; k < AHEAD; ++k) {
         w[k] = make_uint2(0u, ~0u);
-        if (i0 + k * kThreads + (int)threadIdx.x < n) w[k] = __ldg(reinterpret_cast<const uint2*>(at + k * step));
+        if (i0 + k * kThreads + (int)threadIdx.x < n) w[k] = *reinterpret_cast<const uint2*>(at + k * step);
       }
 #pragma unroll
       for (int k = 0; k < AHEAD; ++k) t[k] = w[k].y ? ~0u : w[k].x - (unsigned)first;
@@ -174,7 +174,7 @@ __global__ void __launch_bounds__(kThreads, 4) penalize_kernel(const __grid_cons
       for (int k = 0; k < AHEAD; ++k) {
         t[k] = ~0u;
         if (i0 + k * kThreads + (int)threadIdx.x < n)
-          t[k] = __ldg(reinterpret_cast<const unsigned*>(at + k * step)) - (unsigned)first;
+          t[k] = *reinterpret_cast<const unsigned*>(at + k * step) - (unsigned)first;
       }
     }
   };
@@ -190,7 +190,7 @@ __global__ void __launch_bounds__(kThreads, 4) penalize_kernel(const __grid_cons
   const int words = (int)((p.V + 31LL) / 32);
   // Pieces that do not lie wholly in the row (nor those of the bias that hold them) go element by element.
   auto whole = [&](int v) { return v >= (bias ? 4 : 0) && v + E::N + (bias ? 4 : 0) <= p.V; };
-  auto is_allowed = [&](int v) { return !allowed || ((__ldg(allowed + (v >> 5)) >> (v & 31)) & 1u); };
+  auto is_allowed = [&](int v) { return !allowed || ((allowed[v >> 5] >> (v & 31)) & 1u); };
   unsigned mask[SLOTS];
   const int bias_off = (int)((reinterpret_cast<uintptr_t>(bias + v0) >> 2) & 3u);
   if (allowed) {  // every piece's words requested before the first is used
@@ -198,8 +198,8 @@ __global__ void __launch_bounds__(kThreads, 4) penalize_kernel(const __grid_cons
 #pragma unroll
     for (int s = 0; s < SLOTS; ++s) {
       const int v = v0 + (s * kThreads + threadIdx.x) * E::N, w = v >> 5;
-      lo[s] = v >= 0 && w < words ? __ldg(allowed + w) : 0u;
-      hi[s] = v >= 0 && (v & 31) > 32 - E::N && w + 1 < words ? __ldg(allowed + w + 1) : 0u;
+      lo[s] = v >= 0 && w < words ? allowed[w] : 0u;
+      hi[s] = v >= 0 && (v & 31) > 32 - E::N && w + 1 < words ? allowed[w + 1] : 0u;
     }
     if (!bias) {
 #pragma unroll
@@ -218,7 +218,7 @@ __global__ void __launch_bounds__(kThreads, 4) penalize_kernel(const __grid_cons
       const float4* q = reinterpret_cast<const float4*>(bias + v - bias_off);
       float a[E::N + 4], f[E::N];
 #pragma unroll
-      for (int k = 0; k <= E::N / 4; ++k) *reinterpret_cast<float4*>(a + 4 * k) = whole(v) ? __ldg(q + k) : zero4();
+      for (int k = 0; k <= E::N / 4; ++k) *reinterpret_cast<float4*>(a + 4 * k) = whole(v) ? q[k] : zero4();
       E::get(raw[s], f);
       if (bias_off < 2)
         bias_off == 0 ? add_floats<E::N, 0>(a, f) : add_floats<E::N, 1>(a, f);
@@ -257,7 +257,7 @@ __global__ void __launch_bounds__(kThreads, 4) penalize_kernel(const __grid_cons
       float f = E::load(x + v);
       f = f > 0.f ? __fdiv_rn(f, rep) : __fmul_rn(f, rep);
       if (count > 0) f = __fsub_rn(__fsub_rn(f, __fmul_rn(freq, (float)count)), pres);
-      if (bias) f = __fadd_rn(f, __ldg(bias + v));
+      if (bias) f = __fadd_rn(f, bias[v]);
       if (!is_allowed(v)) f = -INFINITY;
       *reinterpret_cast<T*>(counts + c) = E::round(f);
     }
@@ -280,7 +280,7 @@ __global__ void __launch_bounds__(kThreads, 4) penalize_kernel(const __grid_cons
         const int w = v + i;
         if (w < 0 || w >= p.V) continue;
         T value = x[w];
-        if (bias) value = E::round(__fadd_rn(E::load(x + w), __ldg(bias + w)));
+        if (bias) value = E::round(__fadd_rn(E::load(x + w), bias[w]));
         if (!is_allowed(w)) value = E::round(-INFINITY);
         y[w] = value;
       }

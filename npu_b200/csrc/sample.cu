@@ -368,7 +368,7 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleParams 
   // A thread's candidate as the entry it joins with.
   auto found = [&](const Candidate& c, float sum, int count) -> Found {
     if (c.i < 0) return {0, kNone, 0.f, sum, count};
-    return {__float_as_uint(fmaxf(__fdividef(weight(c.x), __ldg(noise + c.i)), 0.f)), (uint32_t)(begin + c.i), c.x, sum,
+    return {__float_as_uint(fmaxf(__fdividef(weight(c.x), noise[c.i]), 0.f)), (uint32_t)(begin + c.i), c.x, sum,
             count};
   };
 
@@ -417,7 +417,7 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleParams 
         const int bit = __ffsll((long long)mask) - 1;
         at[h] = bit < 0 ? -1 : group_of(round, bit / kGroup) * kGroup + bit % kGroup - shift;
         mask &= mask - 1;
-        e[h] = at[h] >= 0 ? __ldg(noise + at[h]) : 1.f;
+        e[h] = at[h] >= 0 ? noise[at[h]] : 1.f;
       }
 #pragma unroll
       for (int h = 0; h < 4; ++h) {
@@ -466,7 +466,7 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleParams 
       if (whole16 && at >= 0 && at + kGroup <= n) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const float4 v = __ldg(reinterpret_cast<const float4*>(noise + at) + h);
+          const float4 v = reinterpret_cast<const float4*>(noise + at)[h];
           e[4 * h] = v.x;
           e[4 * h + 1] = v.y;
           e[4 * h + 2] = v.z;
@@ -474,7 +474,7 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleParams 
         }
       } else {
 #pragma unroll
-        for (int i = 0; i < kGroup; ++i) e[i] = at + i >= 0 && at + i < n ? __ldg(noise + at + i) : 1.f;
+        for (int i = 0; i < kGroup; ++i) e[i] = at + i >= 0 && at + i < n ? noise[at + i] : 1.f;
       }
       load(g, x);
 #pragma unroll
