@@ -53,6 +53,17 @@ B2A_API int b2a_diag_sample_timeout(const float* logits, const float* noise, int
 B2A_API int b2a_diag_packed_blocks(const int* cu_q, const int* cu_k, int B, int Nq, int Nk, int causal,
                                    const int* ids, int n, int* out, void* stream);
 
+/*
+ * How single-token attention over a paged cache numbers its work: out [n][4]
+ * int64 = {units of the call, sequence, KV head, tile} of the units numbered
+ * units[0 .. n - 1] (device), -1 for a unit that holds no tile (the last of each
+ * pair) or does not exist. tile: keys of a tile, 64 or 128. ahead [B][4] int32
+ * (device, 16-byte aligned, or NULL; tiles of 64): the shared form, ahead[b][0]
+ * keys (a multiple of 64) of sequence b attended elsewhere.
+ */
+B2A_API int b2a_diag_paged_units(const int* seqlens, const int* ahead, int B, int Hkv, int table_width, int page,
+                                 int tile, const long long* units, int n, long long* out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -244,7 +244,9 @@ __device__ __forceinline__ long long total_units(const DecodePagedParams& p, con
   long long n = 0;
   int b1 = 0;
   if constexpr (SHARED) {
-    n = __reduce_add_sync(0xffffffffu, first.n[0] + first.n[1] + first.n[2] + first.n[3]);
+    // 32 sequences at a time: of the longest (2^25 units each) all four would pass 32 bits.
+#pragma unroll
+    for (int k = 0; k < 4; ++k) n += __reduce_add_sync(0xffffffffu, first.n[k]);
     b1 = 128;
   }
 #pragma unroll 4
@@ -1032,6 +1034,24 @@ __global__ void __launch_bounds__(kJoinThreads) decode_paged_join_kernel(const _
 constexpr int kWholeTiles = 8;
 constexpr long long kManyRows = 1024;
 
+// All units of a call, and the pair and tile of some of them (b2attn_diag.h). One warp.
+template <int TK, bool SHARED>
+__global__ void decode_paged_units_kernel(const __grid_constant__ DecodePagedParams p, const long long* units, int n,
+                                          long long* out) {
+  const FirstUnits<TK, SHARED> first(p);
+  const long long total = total_units<TK, SHARED>(p, first);
+  for (int i = 0; i < n; ++i) {
+    const Walk<TK, SHARED> w(p, units[i], units[i] < 0 ? 0LL : min(1LL, total - units[i]), first);
+    const bool valid = w.valid();
+    if (threadIdx.x == 0) {
+      out[4 * i] = total;
+      out[4 * i + 1] = valid ? w.b : -1;
+      out[4 * i + 2] = valid ? w.g : -1;
+      out[4 * i + 3] = valid ? w.begin : -1;
+    }
+  }
+}
+
 template <int D, int NT, bool SPLIT, bool E4M3, bool SHARED = false>
 int launch_main(const CUtensorMap& tk, const CUtensorMap& tv, const DecodePagedParams& p, long long n,
                 cudaStream_t st) {
@@ -1090,6 +1110,14 @@ bool decode_paged_splits(int table_width, int page) { return (long long)table_wi
 
 int decode_paged_max_ctas(int D, int group, bool e4m3, int sms) {
   return sms * decode_paged_ctas_per_sm(D, group <= 8 ? 1 : 2, e4m3);
+}
+
+int launch_decode_paged_units(const DecodePagedParams& p, int tile, const long long* units, int n, long long* out,
+                              cudaStream_t st) {
+  const auto kernel = p.seqs ? decode_paged_units_kernel<64, true>
+                             : (tile == 64 ? decode_paged_units_kernel<64, false> : decode_paged_units_kernel<128, false>);
+  kernel<<<1, 32, 0, st>>>(p, units, n, out);
+  return cudaGetLastError() == cudaSuccess ? 0 : -1;
 }
 
 int launch_decode_paged(int D, const CUtensorMap& tk, const CUtensorMap& tv, const DecodePagedParams& p,

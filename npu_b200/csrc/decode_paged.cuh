@@ -78,4 +78,8 @@ inline size_t decode_paged_parts(int B, int Hkv, int n_ctas) { return (size_t)B 
 int launch_decode_paged(int D, const CUtensorMap& tk, const CUtensorMap& tv, const DecodePagedParams& p,
                         cudaStream_t st);
 
+// For the tests (b2a_diag_paged_units); tile: 64 keys, or 128 (8-bit, without p.seqs).
+int launch_decode_paged_units(const DecodePagedParams& p, int tile, const long long* units, int n, long long* out,
+                              cudaStream_t st);
+
 }  // namespace b2a

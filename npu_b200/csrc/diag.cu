@@ -7,8 +7,12 @@
 //                   thread stores its row of A into TMEM with tcgen05.st.
 // A is [M=128][K=128] row-major. Operands are written into shared memory by
 // threads using the 128-byte swizzle formula.
+#include <climits>
+
 #include "b2attn_diag.h"
+#include "capi_internal.cuh"
 #include "common.cuh"
+#include "decode_paged.cuh"
 #include "packed.cuh"
 #include "sample.cuh"
 
@@ -145,6 +149,24 @@ extern "C" int b2a_diag_packed_blocks(const int* cu_q, const int* cu_k, int B, i
   b2a::diag_packed_blocks_kernel<<<1, 32, 0, static_cast<cudaStream_t>(stream)>>>(
       p, ids, n, reinterpret_cast<b2a::PackedBlock*>(out));
   return cudaGetLastError() == cudaSuccess ? B2A_OK : B2A_ERR_LAUNCH;
+}
+
+extern "C" int b2a_diag_paged_units(const int* seqlens, const int* ahead, int B, int Hkv, int table_width, int page,
+                                    int tile, const long long* units, int n, long long* out, void* stream) {
+  static_assert(sizeof(b2a::SharedSeq) == 4 * sizeof(int), "four numbers a sequence");
+  if (!seqlens || !units || !out || B <= 0 || Hkv <= 0 || table_width <= 0 || page <= 0 || n <= 0 ||
+      (tile != 64 && (tile != 128 || ahead)) || (long long)table_width * page > INT_MAX - tile)
+    return B2A_ERR_INVALID_ARG;
+  if (!b2a::api_aligned(ahead, 16)) return B2A_ERR_ALIGNMENT;
+  b2a::DecodePagedParams p{};
+  p.seqlens = seqlens;
+  p.seqs = reinterpret_cast<const b2a::SharedSeq*>(ahead);
+  p.B = B;
+  p.Hkv = Hkv;
+  p.table_width = table_width;
+  p.page = page;
+  return b2a::launch_decode_paged_units(p, tile, units, n, out, static_cast<cudaStream_t>(stream)) ? B2A_ERR_LAUNCH
+                                                                                                    : B2A_OK;
 }
 
 extern "C" int b2a_diag_wait_timeout(long long limit_cycles, void* stream) {
