@@ -210,6 +210,7 @@ int paged_attention(const void* q, const void* k_pages, const void* v_pages, con
     plan.groups = reinterpret_cast<b2a::SharedGroup*>(base + at.groups);
     plan.seqs = reinterpret_cast<b2a::SharedSeq*>(base + at.seqs);
     plan.total = reinterpret_cast<long long*>(base);
+    plan.ready = reinterpret_cast<uint32_t*>(base + 64);
     plan.err = err;
     b2a::DecodeSharedParams s{};
     s.block_table = block_table;
@@ -239,6 +240,7 @@ int paged_attention(const void* q, const void* k_pages, const void* v_pages, con
     rc = b2a::launch_decode_shared(D, tq, sk, sv, plan, s, static_cast<cudaStream_t>(stream));
     if (rc) return status_of(rc);
     p.seqs = plan.seqs;
+    p.ready = plan.ready;
     p.shared_o = s.part_o;
     p.shared_ml = s.part_ml;
     p.shared_place = s.place;

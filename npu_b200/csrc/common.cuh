@@ -373,6 +373,19 @@ __device__ __forceinline__ int clc_cancelled_ctaid_x(const void* resp) {
 __device__ __forceinline__ void grid_dep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void grid_dep_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
+// A word that one kernel of a stream leaves for a later one which does not wait for
+// it itself: whoever reads the released value sees all that came before the release.
+__device__ __forceinline__ void st_release(uint32_t* p, uint32_t x) {
+  asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(p), "r"(x) : "memory");
+}
+__device__ __forceinline__ uint32_t ld_acquire(const uint32_t* p) {
+  uint32_t x;
+  asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(x) : "l"(p) : "memory");
+  return x;
+}
+// Between that and copies by the async proxy (TMA) of what ordinary stores wrote.
+__device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async;" ::: "memory"); }
+
 // 32-byte global store (sm_100 256-bit vector store); p must be 32-byte aligned.
 __device__ __forceinline__ void st_global_v8(void* p, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t a4,
                                              uint32_t a5, uint32_t a6, uint32_t a7) {

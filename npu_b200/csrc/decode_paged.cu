@@ -187,9 +187,7 @@ __device__ __forceinline__ float4 over(float4 x, float l) {
   return make_float4(f * (x.x / d), f * (x.y / d), f * (x.z / d), f * (x.w / d));
 }
 
-// A length or a table's entry. SHARED: past L1, whose lines may be older than the
-// last write, since that form's main kernel does not wait for the kernels before it
-// itself (the one it follows has).
+// A length or a table's entry. SHARED: past L1 (decode_shared.cuh).
 template <bool SHARED>
 __device__ __forceinline__ int load_int(const int* x) {
   if constexpr (SHARED) return __ldcg(x);
@@ -392,10 +390,15 @@ __global__ void __launch_bounds__(PagedCfg<D, NT, E4M3>::THREADS, PagedCfg<D, NT
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   // SHARED: the kernel before is the one over the shared keys, of which nothing
-  // is read here. It let this one start after its own wait for the plan, so the
-  // plan and all before it is done; the two run side by side, and this one ends
-  // after that one (end_shared), so that the joining kernel sees both.
-  if constexpr (!SHARED) grid_dep_wait();
+  // is read here; the two run side by side, and this one ends after that one
+  // (end_shared), so that the joining kernel sees both. The plan and all before it
+  // is acquired (decode_shared.cuh), by each thread for itself.
+  if constexpr (SHARED) {
+    if (ld_acquire(p.ready) != kPlanReady) grid_dep_wait();
+    fence_proxy_async();
+  } else {
+    grid_dep_wait();
+  }
   // The next kernel (the joining one when SPLIT) may take SM slots as they
   // free up.
   grid_dep_launch();
@@ -977,6 +980,7 @@ __global__ void __launch_bounds__(kJoinThreads)
   const int b = (int)(row / p.Hq), h = (int)(row % p.Hq), g = h / p.group;
   grid_dep_wait();
   grid_dep_launch();
+  if (SHARED && x == 0) *p.ready = 0;
   const float4 gate = p.gate ? load_gate(p, b, h, d) : zero4();
   const Parts<SHARED> parts(p, b, g, h % p.group);
   float m = -INFINITY, l = 0.f;
@@ -1003,6 +1007,7 @@ __global__ void __launch_bounds__(kJoinThreads) decode_paged_join_kernel(const _
   const int team = threadIdx.x / TEAM, d = 4 * (threadIdx.x % TEAM);
   grid_dep_wait();
   grid_dep_launch();
+  if (SHARED && blockIdx.x == 0 && threadIdx.x == 0) *p.ready = 0;
   const float4 gate = p.gate && team == 0 ? load_gate(p, b, h, d) : zero4();
   const Parts<SHARED> parts(p, b, g, r);
   float m = -INFINITY, l = 0.f;

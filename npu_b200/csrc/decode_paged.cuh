@@ -6,6 +6,9 @@
 
 namespace b2a {
 
+// What the plan of the shared form leaves when it is done (decode_shared.cuh).
+constexpr uint32_t kPlanReady = 0x706c616eu;
+
 // A sequence whose first `skip` keys (a multiple of 64) are attended together
 // with others' (decode_shared.cu): where the partials of its query heads are.
 struct alignas(16) SharedSeq {
@@ -51,6 +54,7 @@ struct DecodePagedParams {
   // the joining kernel adds the partials of the shared ones, numbered and placed
   // alike (item block Hkv + g, rows of block_rows, CTAs up to shared_ctas).
   const SharedSeq* seqs;
+  uint32_t* ready;
   const float* shared_o;
   const float* shared_ml;
   const int* shared_place;

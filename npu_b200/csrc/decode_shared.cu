@@ -244,6 +244,8 @@ __global__ void __launch_bounds__(kPlanThreads)
     }
     p.seqs[b] = s;
   }
+  __syncthreads();
+  if (threadIdx.x == 0) st_release(p.ready, kPlanReady);  // and with it what the others wrote
 }
 
 // ---------------------------------------------------------------- the shared keys

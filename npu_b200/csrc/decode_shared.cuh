@@ -11,6 +11,14 @@ namespace b2a {
 // What the plan writes is read past L1 (load_group, load_seq): a CTA of the next
 // kernel starts while the planning one runs, perhaps on its SM, whose L1 may
 // hold lines from before the last writes.
+//
+// Four kernels in a row: the plan, the shared keys, the sequences' own keys and the
+// join. The third starts beside the second and waits for it at its end only, so that
+// the two run side by side (waiting at the start: 20 % more for the call, up to 49 %
+// where it is short). What it reads, the plan and what the kernels before the plan
+// wrote, is ordered by `ready`: the plan, which has waited for those kernels, releases
+// kPlanReady there as its last act, the third kernel acquires it, and waits for the
+// second as usual if it finds anything else. The join sets the word back.
 struct alignas(16) SharedGroup {
   int eff, ref;      // eff: a multiple of the key block, 0 for nothing shared
   int first, count;  // its sequences
@@ -37,6 +45,7 @@ struct SharedPlanParams {
   SharedGroup* groups;  // [n_groups]
   SharedSeq* seqs;      // [B]
   long long* total;     // units of work
+  uint32_t* ready;      // see above
   int* err;
 };
 

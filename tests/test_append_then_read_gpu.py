@@ -83,3 +83,45 @@ def test_noise_of_the_kernel_before(cuda_dev, V):
         sample(logits, noise, temperature=1.0, out=out[i])
     want = torch.stack([sample(logits, draws[i].clone(), temperature=1.0) for i in range(steps)])
     assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("Hq,Hkv,D", [(9, 3, 64), (32, 4, 128), (16, 2, 256)])
+@pytest.mark.parametrize("left", [0, 0xff, 0x706c616e])
+def test_shared_step_whatever_the_workspace_holds(cuda_dev, Hq, Hkv, D, left):
+    """Append and attend behind a prefix, step by step without a pause, in a workspace that held anything before (the
+    words the kernels leave for one another among it): the bits of steps that waited for one another."""
+    from npu_b200 import decode_paged_shared, rope_append_paged
+    from npu_b200.api import decode_paged_shared_workspace_bytes
+
+    dev, B, page, prefix, steps = cuda_dev, 12, 64, 1920, 30
+    own = -(-(steps + 1) // page)
+    pages = prefix // page + B * own
+    first = [torch.randn(pages, Hkv, page, D, generator=gen(dev, s), device=dev).bfloat16() for s in (1, 2)]
+    table = torch.arange(prefix // page, dtype=torch.int32, device=dev).expand(B, -1)
+    table = torch.cat([table, prefix // page + torch.arange(B * own, dtype=torch.int32, device=dev).view(B, own)], 1)
+    q, k, v = (torch.randn(steps, B, h, D, generator=gen(dev, 3 + i), device=dev).bfloat16()
+               for i, h in enumerate((Hq, Hkv, Hkv)))
+    cos, sin = torch.ones(4096, D, device=dev).bfloat16(), torch.zeros(4096, D, device=dev).bfloat16()
+    one_each = torch.arange(B + 1, dtype=torch.int32, device=dev)
+    pre = torch.tensor([prefix], dtype=torch.int32, device=dev)
+    need = decode_paged_shared_workspace_bytes(B, Hq, Hkv, D, 1)
+    got = []
+    for pause in (True, False):
+        kp, vp = (x.clone() for x in first)
+        ws = torch.zeros(need // 4 + 1, dtype=torch.int32, device=dev)
+        if not pause:
+            ws.fill_(left)
+        lens = torch.full((2, B), prefix, dtype=torch.int32, device=dev)
+        outs = []
+        torch.cuda.synchronize()
+        for i in range(steps):
+            a, b = lens[i % 2], lens[1 - i % 2]
+            rot = rope_append_paged(q[i], k[i], v[i], cos, sin, kp, vp, table, one_each, start_pos_per_batch=a,
+                                    seqlens_out=b)
+            if pause:
+                torch.cuda.synchronize()
+            outs.append(decode_paged_shared(rot, kp, vp, table, b, pre, min_saved_bytes=0, workspace=ws))
+            if pause:
+                torch.cuda.synchronize()
+        got.append(torch.stack(outs))
+    assert torch.equal(*got)
