@@ -423,8 +423,9 @@ B2A_API int b2a_decode_paged_e4m3(const void* q, const void* k_pages, const void
  * of the sequences, groups that overlap or a prefix outside 0 .. table_width * page
  * report B2A_ERR_DEVICE_BAD_LEN; nothing is shared then for such a group (the prefix
  * is cut). Where sharing would save reading fewer than least_saved_bytes bytes of
- * keys and values nothing is shared (below 0: 36 MB, and 128 MB if every table
- * were shared to its end, about where it begins to pay). bf16 pools. Workspace: b2a_decode_paged_shared_workspace_bytes.
+ * keys and values nothing is shared (below 0: 36 MB, and 160 MB if all sequences
+ * but one of each group shared all that the table can name, about where it begins
+ * to pay). bf16 pools. Workspace: b2a_decode_paged_shared_workspace_bytes.
  */
 B2A_API size_t b2a_decode_paged_shared_workspace_bytes(int B, int Hq, int Hkv, int D, int n_groups);
 B2A_API int b2a_decode_paged_shared(const void* q, const void* k_pages, const void* v_pages, const int* block_table,

@@ -548,10 +548,14 @@ def decode_paged_shared(
     `prefill`. workspace: decode_paged_shared_workspace_bytes.
 
     Where sharing would save reading fewer than min_saved_bytes bytes of keys and
-    values nothing is shared. The default goes by what was measured to pay for the
-    launches: 36 MB, and 128 MB if every table were shared to its end. That is a
-    guess from sizes alone: many short prefixes or a few sequences can be up to a
-    third slower than `decode_paged`, so a server that knows its shapes sets it.
+    values nothing is shared. The default is 36 MB, and 160 MB if all sequences but
+    one of each group shared all that block_table can name (else the call is
+    `decode_paged`'s), about where the launches were measured to pay. The host sees
+    the table's width only: with tables much wider than the sequences a call that
+    has little to share takes 6 to 13 us longer than `decode_paged` (up to 1.75
+    times as long), and with small groups a call can be a third slower. A server that
+    knows its shapes sets min_saved_bytes (0: share whatever there is) or calls
+    `decode_paged`. Whether keys are shared also decides how P is rounded.
     """
     return _serving().decode_paged_shared(q, k_pages, v_pages, block_table, seqlens, prefix_lens, cu_groups, scale,
                                           out_dtype, workspace, out, gate, min_saved_bytes)

@@ -75,15 +75,18 @@ struct SharedPrefix {
   long long least_saved;  // bytes, below 0: kLeastSaved
 };
 
-// Reading that sharing must save to be worth its plan and its kernel, in bytes. Known on the device, where it is
-// measured against not sharing with the same launches, 32 / 4 heads of 128 and 9 / 3 of 64: 20.2 us against 18.4 at 31
-// MB, 22.2 / 23.2 at 42, 20.5 / 21.8 at 63, 20.5 / 27.9 at 126, 27.4 / 40.2 at 252. The host knows only what it could
-// save, if all of every table were shared; below kLeastPossible the call is b2a_decode_paged's, against which, by what
-// could be saved: 20.2 / 12.5 at 63 MB, 20.2 / 15.6 at 94, 22.3 / 17.4 and 17.1 / 22.2 at 109, 20.5 / 21.5 at 157,
-// 27.4 / 32.8 at 275, 30 / 101 at 662. Bytes are not all that counts, and some calls share that had better not: 30.2 us
-// against 22.8 for 64 sequences behind 512 keys, 29.4 / 25.6 for 64 in eight groups behind 2048 to 256, 39.4 / 35.6 for
-// 4 behind 32768 (all 32 / 4 heads of 128).
-constexpr long long kLeastSaved = 36LL << 20, kLeastPossible = 128LL << 20;
+// When a call shares by the default rule, in bytes of keys and values. The device knows what sharing would save to
+// read and weighs it against not sharing with the same launches: kLeastSaved. The host knows only the sizes: the
+// call is b2a_decode_paged's, with fewer launches, below kLeastPossible for all sequences but one of each group sharing
+// all that their tables can name. Both from 168 shapes (4 to 128 sequences, 1, 3 or 8 groups behind 512 to 32000 keys,
+// 32 / 4 and 32 / 8 heads of 128, 9 / 3 of 64, 16 / 2 of 256):
+// - tables as long as their sequences: with 160 MB a call takes 1.4 % longer on average than by the better way, at worst
+//   85.8 us for 65.9 (two sequences in each of 8 groups behind 32000 keys), with 134 MB 2.3 %, with 200 MB 1.8 % (worst
+//   54 for 30), never sharing 7 %, always 15 %;
+// - tables of 32768 keys, so that the device decides: 36 MB is within 1.5 % of the better of its two ways on average, 20
+//   to 45 MB are alike, 100 MB loses 6 %. Against b2a_decode_paged such a call takes 6 us more where nothing is shared
+//   (up to 13, or 1.6 times), and up to 1.75 times where the device shares to little use (8 groups of two).
+constexpr long long kLeastSaved = 36LL << 20, kLeastPossible = 160'000'000LL;
 
 // Where the shared form's scratch is, behind that of the sequences' own keys.
 struct SharedLayout {
@@ -191,7 +194,7 @@ int paged_attention(const void* q, const void* k_pages, const void* v_pages, con
   const long long bytes_a_key = 4LL * Hkv * D;
   const bool by_rule = shared && shared->least_saved < 0;
   const long long least = by_rule ? kLeastSaved : (shared ? shared->least_saved : 0);
-  const long long possible = (B - 1) * ((long long)table_width * page);  // keys
+  const long long possible = (long long)(B - (by_rule ? shared->n_groups : 1)) * table_width * page;  // keys
   if (shared && B > 1 && b2a::decode_paged_splits(table_width, page) &&
       possible >= (by_rule ? kLeastPossible : least) / bytes_a_key) {
     const SharedLayout at = shared_layout(B, Hq, Hkv, D, shared->n_groups);
