@@ -118,8 +118,9 @@ int paged_attention(const void* q, const void* k_pages, const void* v_pages, con
                     size_t workspace_bytes, void* stream) {
   if (!q || !k_pages || !v_pages || !block_table || !seqlens || !o || !qs || !ks || !vs || !os || (gate && !gs))
     return B2A_ERR_INVALID_ARG;
+  const int tile = k_scales ? 128 : 64;  // keys; lengths are rounded up to whole ones
   if (B <= 0 || Hq <= 0 || Hkv <= 0 || n_pages <= 0 || page <= 0 || page % 16 || table_width <= 0 ||
-      table_ld < table_width || (long long)table_width * page > INT_MAX - 128)
+      table_ld < table_width || (long long)table_width * page > INT_MAX - tile)
     return B2A_ERR_INVALID_ARG;
   if (!(scale > 0.f) || !std::isfinite(scale)) return B2A_ERR_INVALID_ARG;
   if (!head_dim_ok(D)) return B2A_ERR_HEAD_DIM;
