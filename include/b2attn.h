@@ -378,8 +378,8 @@ B2A_API int b2a_rope_append_paged(const void* q, const void* k, const void* v, c
  * elements, multiples of 16) and, for each token and KV head, a scale in
  * k_scales / v_scales [n_pages, Hkv, page] fp32 (contiguous slots; strides
  * {page, head} multiples of 4, 16-byte aligned). A row y (k after norm and
- * rotation, v) is stored as e4m3(y / s), s = max(max|y| / 448, 2^-100), from the
- * fp32 values; rows with an infinity or a NaN read back as NaN. k_out / v_out
+ * rotation, v) is stored as e4m3(y r), r = 1 / s and s = max(max|y| / 448, 2^-100)
+ * rounded to fp32, from the fp32 values; rows with an infinity or a NaN read back as NaN. k_out / v_out
  * receive the values before that rounding, as bf16.
  */
 B2A_API int b2a_rope_append_paged_e4m3(const void* q, const void* k, const void* v, const long long* q_strides,
@@ -422,7 +422,8 @@ B2A_API int b2a_decode_paged_e4m3(const void* q, const void* k_pages, const void
  * with the last prefix_lens[g] % 64 of them. A pair of offsets that is not a stretch
  * of the sequences, groups that overlap or a prefix outside 0 .. table_width * page
  * report B2A_ERR_DEVICE_BAD_LEN; nothing is shared then for such a group (the prefix
- * is cut). Where sharing would save reading fewer than least_saved_bytes bytes of
+ * is cut). A call in which the host sees nothing to share (one sequence, a table of no
+ * more than 512 keys, too little to save) does not read either array. Where sharing would save reading fewer than least_saved_bytes bytes of
  * keys and values nothing is shared (below 0: 36 MB, and 160 MB if all sequences
  * but one of each group shared all that the table can name, about where it begins
  * to pay). bf16 pools. Workspace: b2a_decode_paged_shared_workspace_bytes.

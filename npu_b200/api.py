@@ -630,8 +630,8 @@ def rope_append_paged(
 
     With k_scales and v_scales ([n_pages, Hkv, page] fp32, contiguous slots) the
     pools are 8-bit (float8_e4m3fn): each token's k and v of a KV head, a row y
-    of D values, is stored as e4m3(y / s) with s = max(max |y| / 448, 2^-100) beside
-    it, from the fp32 values. A row with an infinity or a NaN reads back as NaN.
+    of D values, is stored as e4m3(y * (1 / s)) with s = max(max |y| / 448, 2^-100)
+    beside it, both quotients rounded to fp32, from the fp32 values. A row with an infinity or a NaN reads back as NaN.
     """
     return _serving().rope_append_paged(q, k, v, cos, sin, k_pages, v_pages, block_table, cu_seqlens, start_pos,
                                         start_pos_per_batch, seqlens_out, q_out, q_norm, k_norm, norm_eps, rope_dim,

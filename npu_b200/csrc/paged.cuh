@@ -2,10 +2,12 @@
 // token, and the 8-bit form of a cached row.
 //
 // 8-bit rows (one token's k or v of one KV head): with a = max |y_i|,
-//   s = max(a / 448, 2^-100),  c_i = e4m3(y_i / s),  read back as c_i s.
-// 448 is the largest e4m3 value, so nothing saturates; e4m3 keeps 4 significant
-// bits of c_i >= 2^-6 and steps of 2^-9 below, so a value is off by at most
-// 2^-4 of itself or 2^-10 s. One scale a row and not one a page: rows are
+//   s = max(a / 448, 2^-100),  c_i = e4m3(y_i r), r = 1 / s,  read back as c_i s,
+// s and r rounded to fp32 (a product for each value and one quotient a row; y_i / s
+// would differ where it lies within 2^-23 of the middle of two codes).
+// 448 is the largest e4m3 value, and what r's rounding adds to it is rounded away, so
+// nothing saturates; e4m3 keeps 4 significant bits of c_i >= 2^-6 and steps of 2^-9
+// below, so a value is off by at most 2^-4 of itself or 2^-10 s (and 2^-23 of that). One scale a row and not one a page: rows are
 // written one by one, and a page's scale would change under those already
 // there. The floor 2^-100 keeps 1 / s finite for rows of (nearly) zeros. A row
 // with an infinity or a NaN has the scale NaN and reads back as NaN throughout.

@@ -349,9 +349,17 @@ class SmolLMB200:
         row. Nothing synchronises with the host in between.
 
         prefix: tokens ahead of every prompt (a system prompt), run and stored
-        once: their whole pages are shared. The penalties, logit_bias (bias)
-        and allowed are those of api.penalize, over the prefix, the prompt and
-        what was generated."""
+        once: their whole pages are shared. Behind them prompts attend keys and
+        values as the cache holds them, their own too (with an 8-bit cache
+        quantised ones, where prompts without a prefix attend theirs before that),
+        and single tokens as api.decode_paged_shared does by default (bf16: P
+        rounded to bf16 over the prefix where it is shared) or api.decode_paged
+        (8-bit: the prefix read once for every sequence).
+
+        The penalties, logit_bias (bias) and allowed are those of api.penalize,
+        over the prefix, the prompt and what was generated; one allowed for all
+        steps (a grammar, whose mask follows the tokens, calls api.penalize between
+        prefill_packed or decode_packed and api.sample)."""
         lens = [len(p) for p in prompts]
         if not lens or min(lens) < 1 or max_new_tokens < 1:
             raise ValueError("every prompt needs a token and max_new_tokens must be positive")
