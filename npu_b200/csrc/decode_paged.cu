@@ -119,15 +119,6 @@ __device__ __forceinline__ uint32_t transposed(uint32_t a) {
   return d;
 }
 
-__device__ __forceinline__ void tma_load_5d(void* smem_dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1,
-                                            int c2, int c3, int c4) {
-  asm volatile(
-      "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(smem_u32(smem_dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4)
-      : "memory");
-}
-
 __device__ __forceinline__ void bulk_load(void* smem_dst, const void* src, int bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
                    smem_u32(smem_dst)),
@@ -351,23 +342,11 @@ struct Walk {
 //   fp32 ends (O gets the same factor when the warps' parts are merged). A weight
 //   below fp32's range drops out of the sum too: 2^-24 of the largest P where
 //   V's scales in a sequence differ by 2^117, less where by less.
-__device__ __forceinline__ uint32_t f16_of_e4m3(uint16_t x) {  // two numbers, the low byte's in the low half
-  uint32_t r;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(x));
-  return r;
-}
 __device__ __forceinline__ uint32_t low_f16(uint32_t w) { return f16_of_e4m3((uint16_t)w); }
 __device__ __forceinline__ uint32_t high_f16(uint32_t w) { return f16_of_e4m3((uint16_t)(w >> 16)); }
 __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-__device__ __forceinline__ float2 unpack_f16x2(uint32_t x) {
-  float2 r;
-  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.f32.f16 %0, l;\n\tcvt.f32.f16 %1, h;\n\t}"
-      : "=f"(r.x), "=f"(r.y)
-      : "r"(x));
   return r;
 }
 constexpr float kWeightLog2 = 15.f;               // of the largest weight of V

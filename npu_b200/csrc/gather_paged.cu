@@ -31,14 +31,8 @@ constexpr int kSteps = 4;       // loads of a lane ahead of its stores
 
 // Two e4m3 values (the low and the high byte of x) times s, as bf16. (To floats by way of f16: exact.)
 __device__ __forceinline__ uint32_t scaled(uint32_t x, float s) {
-  uint32_t h, r;
-  float2 v;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)x));
-  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.f32.f16 %0, l;\n\tcvt.f32.f16 %1, h;\n\t}"
-      : "=f"(v.x), "=f"(v.y)
-      : "r"(h));
-  r = pack_bf16x2(v.x * s, v.y * s);
-  return r;
+  const float2 v = unpack_f16x2(f16_of_e4m3((uint16_t)x));
+  return pack_bf16x2(v.x * s, v.y * s);
 }
 
 // The sequence that owns token n: the largest b with cu[b] <= n (0 when there is none). Each lane for itself.
