@@ -26,12 +26,14 @@
 // part, and numbers row blocks and units.
 //
 // Measured on one B200 (device time): 128 sequences of 16 to 2048 keys of their own
-// behind 32768 shared ones, 32 / 4 heads of 128, pages of 64: 111 to 124 us; of 111 the
-// shared keys are 78, each further 32768 of them 57 (1.2 PFLOP/s, 0.72 of the
-// measured bf16 burst rate, 0.86 of the sustained one: what the dense prefill
-// reaches). The rest is the plan (4), starting and ending each item, the own keys
-// (31, after the shared ones: the two kernels do not fit an SM together at this
-// head dim) and the join (10). Tried without gain: S and P in columns of their own,
+// behind 32768 shared ones, 32 / 4 heads of 128, pages of 64: 111 to 124 us a call. One
+// by one, in a profile in which none overlaps another (125 in all): the plan 4.6, the
+// shared keys 78.6, the own ones 31 (after the shared ones in a call too: the two
+// kernels do not fit an SM together at this head dim), the join 10.3; in a call each
+// starts while the one before it ends. Without the profiler each further 32768 shared
+// keys cost 57 us (1.2 PFLOP/s, 0.72 of the measured bf16 burst rate, 0.86 of the
+// sustained one: what the dense prefill reaches); the other 21 of the 78.6 are not
+// measured apart. Tried without gain: S and P in columns of their own,
 // so that S(j + 1) can go a softmax earlier (128.0 us against 127.5), two softmax
 // warpgroups a tile (137: what they tell each other costs more than it hides).
 // Warps: 0 TMA, 1 .. NQT MMA issue, 4 + 4 t .. softmax and partials of tile t.
