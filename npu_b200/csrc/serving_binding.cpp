@@ -78,10 +78,14 @@ void need_int32(const char* name, const Tensor& t, int64_t numel, const c10::Dev
 }
 
 void need_table(const Tensor& t, int64_t batch, const c10::Device& device) {
-  if (t.scalar_type() != at::kInt || t.device() != device || t.dim() != 2 || t.size(0) != batch || t.stride(1) != 1)
+  if (t.scalar_type() != at::kInt || t.device() != device || t.dim() != 2 || t.size(0) != batch ||
+      (t.size(1) > 1 && t.stride(1) != 1))
     refuse("block_table must be an int32 tensor [", batch,
            ", pages] on the inputs' device with a contiguous last dim");
 }
+
+// Its row stride; a single row may have any in torch.
+int64_t table_stride(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
 
 void need_gate(const Tensor& t, const Tensor& q) {
   if (t.device() != q.device()) refuse("gate must be a CUDA tensor on q's device");
@@ -209,14 +213,14 @@ Tensor decode_paged(const Tensor& q, const Tensor& k_pages, const Tensor& v_page
   if (k_scales)
     check(b2a_decode_paged_e4m3(q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), k_scales->data_ptr<float>(),
                                 v_scales->data_ptr<float>(), Strides(*k_scales, 2), Strides(*v_scales, 2),
-                                table.data_ptr<int>(), table.stride(0), width, seqlens.data_ptr<int>(), pointer(gate),
+                                table.data_ptr<int>(), table_stride(table), width, seqlens.data_ptr<int>(), pointer(gate),
                                 o.data_ptr(), (int)B, (int)Hq, (int)Hkv, pages, slots, (int)D, Strides(q, 2),
                                 Strides(k_pages, 3), Strides(v_pages, 3), gs, Strides(o, 2), gate_bf16, used,
                                 out_dtype == at::kFloat, ws, need, stream_of(q)),
           "b2a_decode_paged_e4m3");
   else
     check(b2a_decode_paged(q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), table.data_ptr<int>(),
-                           table.stride(0), width, seqlens.data_ptr<int>(), pointer(gate), o.data_ptr(), (int)B,
+                           table_stride(table), width, seqlens.data_ptr<int>(), pointer(gate), o.data_ptr(), (int)B,
                            (int)Hq, (int)Hkv, pages, slots, (int)D, Strides(q, 2), Strides(k_pages, 3),
                            Strides(v_pages, 3), gs, Strides(o, 2), gate_bf16, used, out_dtype == at::kFloat, ws, need,
                            stream_of(q)),
@@ -262,7 +266,7 @@ Tensor decode_paged_shared(const Tensor& q, const Tensor& k_pages, const Tensor&
   }
   const Strides gs(gate ? *gate : q, 2);
   check(b2a_decode_paged_shared(q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), table.data_ptr<int>(),
-                                table.stride(0), as_int("table width", table.size(1)), seqlens.data_ptr<int>(),
+                                table_stride(table), as_int("table width", table.size(1)), seqlens.data_ptr<int>(),
                                 prefix_lens.data_ptr<int>(), static_cast<int*>(pointer(cu_groups)), (int)groups,
                                 min_saved.value_or(-1), pointer(gate), o.data_ptr(), (int)B, (int)Hq, (int)Hkv,
                                 as_int("n_pages", k_pages.size(0)), as_int("page", k_pages.size(2)), (int)D,
@@ -339,7 +343,7 @@ py::object rope_append_paged(const Tensor& q, const Tensor& k, const Tensor& v, 
               pointer(q_norm), pointer(k_norm), (float)eps, cos.data_ptr(), sin.data_ptr(), tables_fp32, max_pos,
               as_int("rope_dim", rope), qo.data_ptr(), pointer(ko), pointer(vo), k_pages.data_ptr(), v_pages.data_ptr(),
               Strides(k_pages, 3), Strides(v_pages, 3), k_scales->data_ptr<float>(), v_scales->data_ptr<float>(),
-              Strides(*k_scales, 2), Strides(*v_scales, 2), table.data_ptr<int>(), table.stride(0), width, pages, slots,
+              Strides(*k_scales, 2), Strides(*v_scales, 2), table.data_ptr<int>(), table_stride(table), width, pages, slots,
               cu.data_ptr<int>(), as_int("B", B), as_int("N", N), as_int("Hq", Hq), as_int("Hkv", Hkv), as_int("D", D),
               first, static_cast<int*>(pointer(start)), static_cast<int*>(pointer(seqlens_out)), stream_of(q)),
           "b2a_rope_append_paged_e4m3");
@@ -348,7 +352,7 @@ py::object rope_append_paged(const Tensor& q, const Tensor& k, const Tensor& v, 
               q.data_ptr(), k.data_ptr(), v.data_ptr(), Strides(q, 2), Strides(k, 2), Strides(v, 2), bf16,
               pointer(q_norm), pointer(k_norm), (float)eps, cos.data_ptr(), sin.data_ptr(), tables_fp32, max_pos,
               as_int("rope_dim", rope), qo.data_ptr(), pointer(ko), pointer(vo), k_pages.data_ptr(), v_pages.data_ptr(),
-              Strides(k_pages, 3), Strides(v_pages, 3), table.data_ptr<int>(), table.stride(0), width, pages, slots,
+              Strides(k_pages, 3), Strides(v_pages, 3), table.data_ptr<int>(), table_stride(table), width, pages, slots,
               cu.data_ptr<int>(), as_int("B", B), as_int("N", N), as_int("Hq", Hq), as_int("Hkv", Hkv), as_int("D", D),
               first, static_cast<int*>(pointer(start)), static_cast<int*>(pointer(seqlens_out)), stream_of(q)),
           "b2a_rope_append_paged");
@@ -380,7 +384,7 @@ py::object gather_paged(const Tensor& k_pages, const Tensor& v_pages, const Tens
     check(b2a_gather_paged(k_pages.data_ptr(), v_pages.data_ptr(), Strides(k_pages, 3), Strides(v_pages, 3),
                            static_cast<float*>(pointer(k_scales)), static_cast<float*>(pointer(v_scales)),
                            Strides(k_scales ? *k_scales : k_pages, 2), Strides(v_scales ? *v_scales : v_pages, 2),
-                           table.data_ptr<int>(), table.stride(0), as_int("table width", table.size(1)),
+                           table.data_ptr<int>(), table_stride(table), as_int("table width", table.size(1)),
                            as_int("n_pages", k_pages.size(0)), as_int("page", k_pages.size(2)), cu.data_ptr<int>(),
                            as_int("B", B), as_int("n_tokens", n_tokens), as_int("Hkv", Hkv), as_int("D", D),
                            as_int("start_pos", start_pos), static_cast<int*>(pointer(start)), ko.data_ptr(),
