@@ -123,7 +123,13 @@ class PagedKVCache:
         counts = [-(-c // self.page) for c in capacities]
         if sum(counts) > len(self._free):
             raise ValueError(f"{sum(counts)} pages are needed and {len(self._free)} are free")
-        return PagedSequences(self, [[self._free.pop() for _ in range(n)] for n in counts], capacities, prefix)
+        pages = [[self._free.pop() for _ in range(n)] for n in counts]
+        try:
+            return PagedSequences(self, pages, capacities, prefix)
+        except Exception:  # no memory for the table, say: nobody holds these pages
+            for p in reversed(pages):
+                self._free.extend(reversed(p))
+            raise
 
 
 class PagedSequences:
@@ -140,8 +146,6 @@ class PagedSequences:
         self.prefix, self.followers = prefix, 0
         shared = [] if prefix is None else prefix._pages[0]
         self.prefix_tokens = len(shared) * cache.page
-        if prefix is not None:
-            prefix.followers += 1
         # -1 is no page: a token past a sequence's own pages is left out and reported.
         table = torch.full((self.batch, len(shared) + max(len(p) for p in pages)), -1, dtype=torch.int32)
         for b, p in enumerate(pages):
@@ -153,6 +157,8 @@ class PagedSequences:
             self.prefix_lens = torch.tensor([self.prefix_tokens], dtype=torch.int32, device=cache.device)
         # Offsets of a step of one token per sequence.
         self.one_each = torch.arange(self.batch + 1, dtype=torch.int32, device=cache.device)
+        if prefix is not None:
+            prefix.followers += 1
 
     @property
     def start(self) -> torch.Tensor:
