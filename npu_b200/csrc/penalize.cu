@@ -20,7 +20,7 @@
 // per chunk, from L2 after the first, eight requests at a time.
 //
 // Measured on one B200 (device time): 256 rows of 131071 bf16 logits, up to 4096
-// tokens each, a bias for all and a mask for each: 60 us, 2.3 TB/s (0.37 of the
+// tokens each, a bias for all and a mask for each: 61 us, 2.3 TB/s (0.36 of the
 // measured copy rate; without bias and mask 44, without tokens too 31): instructions,
 // 60 % of the issue slots, and the round trips of a chunk one after another (settings,
 // tokens, counts, listed logits). 128 rows of fp32: 37 us, 3.7 TB/s (0.57). One row of
