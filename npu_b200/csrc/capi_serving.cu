@@ -82,7 +82,7 @@ struct SharedPrefix {
 // 32 / 4 and 32 / 8 heads of 128, 9 / 3 of 64, 16 / 2 of 256):
 // - tables as long as their sequences: with 160 MB a call takes 1.4 % longer on average than by the better way, at worst
 //   85.8 us for 65.9 (two sequences in each of 8 groups behind 32000 keys), with 134 MB 2.3 %, with 200 MB 1.8 % (worst
-//   54 for 30), never sharing 7 %, always 15 %;
+//   31.5 for 17.1), never sharing 7 %, always 15 %;
 // - tables of 32768 keys, so that the device decides: 36 MB is within 1.5 % of the better of its two ways on average, 20
 //   to 45 MB are alike, 100 MB loses 6 %. Against b2a_decode_paged such a call takes 6 us more where nothing is shared
 //   (up to 13, or 1.6 times), and up to 1.75 times where the device shares to little use (8 groups of two).
